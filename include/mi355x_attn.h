@@ -333,6 +333,79 @@ const char* mi355x_linear_noalloc(const void* x, int64_t ldx, const void* w, int
                                   void* stream);
 
 /* ------------------------------------------------------------------------
+ * 8-bit projections: int8 weights with one fp32 scale an output channel, rows
+ * quantised to int8 with one fp32 scale a token. No reference counterpart (its
+ * projections, src/layers/linear.rs:5-7, are 16-bit).
+ * ------------------------------------------------------------------------ */
+
+/* scales[r] = max_k |x[r,k]| / 127, values[r,k] = rint(127 x[r,k] / max_k |x[r,k]|)
+ * (half to even; a row of zeros has scale 0 and zeros). x [rows, width] of dtype 0 bf16,
+ * 1 fp16 or 2 fp32 with row stride ldx and any alignment of its type; values int8
+ * [rows, ldv], ldv a multiple of 16, columns width .. up to the next multiple of 16 written
+ * as zeros; scales fp32. A row with an inf or a NaN gets the scale NaN and zeros, so that its products
+ * are NaN and no other row's are. */
+const char* mi355x_quantize_rows(const void* x, int64_t ldx, void* values, int64_t ldv,
+                                 void* scales, int64_t rows, int64_t width, int dtype,
+                                 void* stream);
+
+/* Workspace bytes of mi355x_linear_int8 (the quantised rows and their scales), -1 for an
+ * invalid shape. Host-only. */
+int64_t mi355x_linear_int8_workspace_bytes(int64_t M, int64_t K);
+
+/* out[m, n] = round(sx[m] w_scales[n] sum_k q[m, k] w[n, k]) with (q, sx) = mi355x_quantize_rows
+ * of x [M, K] (dtype 0 bf16, 1 fp16; out has the same) and w int8 [N, ldw]; the sum is exact
+ * in int32. With silu_mul, w is a gate_up weight (gate rows, then up rows, N even) and
+ * out[m, j] = round(silu(y[m, j]) * y[m, N/2 + j]), y unrounded. K up to 131,072; w rows of
+ * whole 16-byte words (columns past K are multiplied with zeros) and less than 4 GiB in all; x
+ * and out rows of any stride. Calls that overlap need workspaces of their own. */
+const char* mi355x_linear_int8(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                               const float* w_scales, void* out, int64_t ldo, int64_t M,
+                               int64_t N, int64_t K, bool silu_mul, void* workspace,
+                               int64_t workspace_bytes, int64_t dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Layers of experts. No reference counterpart (its layers are dense).
+ * ------------------------------------------------------------------------ */
+
+/* The top_k experts of every token and their weights: p = softmax(logits[t]) in fp32,
+ * ids[t, :] the top_k largest (largest first, equal logits by the lower index), weights[t, s]
+ * = p[ids[t, s]], with `normalize` divided by their sum. logits [tokens, experts] of dtype
+ * 0 bf16, 1 fp16 or 2 fp32 with row stride ld; weights fp32 and ids int32 [tokens, top_k]
+ * contiguous. Up to 1,024 experts, top_k up to 64. A row of only -inf gets the weights 0; a
+ * NaN (which sorts above +inf) or a +inf makes the row's weights NaN. */
+const char* mi355x_route_experts(const void* logits, int64_t ld, void* weights, int32_t* ids,
+                                 int64_t tokens, int64_t experts, int64_t top_k, bool normalize,
+                                 int dtype, void* stream);
+
+/* Workspace bytes of mi355x_expert_mlp (ldx: x's row stride in elements), -1 for an invalid
+ * shape. At most 131,072 slots (or one token) are in flight, more tokens run in several passes.
+ * Host-only. */
+int64_t mi355x_expert_mlp_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts,
+                                          int64_t hidden, int64_t inter, int64_t ldx, bool int8);
+
+/* out[t] = sum_s weights[t, s] down[e] . (silu(g) * u), (g; u) = gate_up[e] . x[t], e = ids[t, s].
+ * x [tokens, hidden] and out of dtype 0 bf16 or 1 fp16, ids int32 and weights fp32
+ * [tokens, top_k] contiguous. gate_up [experts, 2 inter, ld_gate_up] (gate rows, then up rows)
+ * and down [experts, hidden, ld_down], contiguous in experts and rows. A slot whose id is
+ * outside [0, experts) adds nothing (pad rows, experts held elsewhere); an expert may occur
+ * twice in a row.
+ *
+ * Scales NULL: weights of x's type. hidden, inter and ldx are multiples of 8 and rows are 16-byte
+ * aligned. Sums in fp32; silu(g) * u and the weighted slot outputs are rounded to x's type.
+ * Scales given (fp32 [experts, 2 inter] and [experts, hidden]): int8 weights. x is quantised once
+ * a token, silu(g) * u (kept in fp32) once a slot, both as mi355x_quantize_rows does; any sizes and
+ * x strides, weight rows of whole 16-byte words.
+ * Nothing is read back to the host. An expert's weights are less than 4 GiB. Calls that overlap
+ * need workspaces of their own. */
+const char* mi355x_expert_mlp(const void* x, int64_t ldx, const int32_t* ids,
+                              const float* weights, const void* gate_up, int64_t ld_gate_up,
+                              const float* gate_up_scales, const void* down, int64_t ld_down,
+                              const float* down_scales, void* out, int64_t ldo, int64_t tokens,
+                              int64_t top_k, int64_t experts, int64_t hidden, int64_t inter,
+                              void* workspace, int64_t workspace_bytes, int64_t dtype,
+                              void* stream);
+
+/* ------------------------------------------------------------------------
  * Sampling.
  * ------------------------------------------------------------------------ */
 

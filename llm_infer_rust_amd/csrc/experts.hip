@@ -1,0 +1,523 @@
+// Expert layers on gfx950: routing, and the gate_up -> SiLU x mul -> down products of the experts
+// that each token was routed to.
+//
+//   p = softmax(logits[t]);  ids[t, :] = the top_k largest, ties to the lowest index
+//   weights[t, s] = p[ids[t, s]]  (normalised: divided by their sum)
+//   out[t] = sum_s weights[t, s] down[e] . (silu(g) * u),  (g; u) = gate_up[e] . x[t],  e = ids[t, s]
+//
+// The slots (token, s) are grouped by expert on the device, so nothing is read back to the host:
+// the products run over a list of row tiles (expert, first row, end row) and a grid sized for the
+// most tiles that so many slots can need. Replaces, for layers of experts, the MLP of
+// src/models/qwen3/model.rs:478-534; the reference itself has dense layers only.
+#include <algorithm>
+
+#include "quant.h"
+
+namespace mi355x {
+namespace {
+
+// ---------------------------------------------------------------------------- routing
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxTopK = 64;
+
+template <int DT>
+__device__ __forceinline__ float logit(const void* p, int64_t at) {
+  if constexpr (DT == kFloatOut)
+    return static_cast<const float*>(p)[at];
+  else
+    return Elem<DT>::to_float(static_cast<const uint16_t*>(p)[at]);
+}
+
+// Floats in order as unsigned integers (-0 as 0, NaN above +inf); 0 is below every float.
+__device__ __forceinline__ uint32_t order_key(float f) {
+  if (f != f) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(f + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+// One wave a token, expert v * 64 + lane in register v. Selection is on the logits (the softmax
+// keeps their order), so ids are exact; top_k rounds of a wave maximum over (value, lowest index).
+// Latency-bound: a row is E logits.
+template <int DT, int V>
+__global__ __launch_bounds__(256) void route_kernel(const void* __restrict__ logits, int64_t stride,
+                                                    float* __restrict__ weights,
+                                                    int32_t* __restrict__ ids, int64_t tokens,
+                                                    int experts, int top_k, bool normalize) {
+  const int64_t t = blockIdx.x * int64_t(4) + threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave;
+  if (t >= tokens) return;
+  uint32_t key[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int e = v * kWave + lane;
+    key[v] = e < experts ? order_key(logit<DT>(logits, t * stride + e)) : 0u;
+  }
+  uint32_t all[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) all[v] = key[v];
+  float top = 0.f, mine = 0.f;
+  int my_id = 0;
+  for (int s = 0; s < top_k; ++s) {
+    uint64_t best = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const uint64_t c =
+          static_cast<uint64_t>(key[v]) << 32 | (0xffffffffu - static_cast<uint32_t>(v * kWave + lane));
+      best = max(best, c);
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) best = max(best, static_cast<uint64_t>(__shfl_xor(
+                                                      static_cast<unsigned long long>(best), d)));
+    const int id = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
+    const float value = key_value(static_cast<uint32_t>(best >> 32));
+    if (s == 0) top = value;
+    if (lane == s) mine = value, my_id = id;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (v * kWave + lane == id) key[v] = 0;
+  }
+  // A row of only -inf has no expert to weigh: weights 0. NaN and +inf make the row's weights NaN.
+  const bool none = top == -INFINITY;
+  float e = lane < top_k && !none ? expf(mine - top) : 0.f;
+  float sum = 0.f;
+  if (normalize) {
+    sum = wave_sum(e);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (all[v] != 0 && !none) sum += expf(key_value(all[v]) - top);
+    sum = wave_sum(sum);
+  }
+  if (lane < top_k) {
+    weights[t * top_k + lane] = none ? 0.f : e / sum;
+    ids[t * top_k + lane] = my_id;
+  }
+}
+
+template <int DT>
+void launch_route(const void* logits, int64_t stride, float* weights, int32_t* ids, int64_t tokens,
+                  int experts, int top_k, bool normalize, hipStream_t s) {
+  const dim3 grid(static_cast<uint32_t>((tokens + 3) / 4));
+#define MI355X_ROUTE(V)                                                                     \
+  route_kernel<DT, V><<<grid, 256, 0, s>>>(logits, stride, weights, ids, tokens, experts, top_k, \
+                                           normalize)
+  if (experts <= 64)
+    MI355X_ROUTE(1);
+  else if (experts <= 128)
+    MI355X_ROUTE(2);
+  else if (experts <= 256)
+    MI355X_ROUTE(4);
+  else if (experts <= 512)
+    MI355X_ROUTE(8);
+  else
+    MI355X_ROUTE(16);
+#undef MI355X_ROUTE
+}
+
+// ---------------------------------------------------------------------------- grouping
+constexpr int kGroupThreads = 1024;
+constexpr int kGroupChunk = 4096;  // slots a workgroup of the grouping passes takes
+
+__device__ __forceinline__ bool takes_part(int e, int experts) { return e >= 0 && e < experts; }
+
+// counts[chunk][e]: slots of a chunk that go to expert e.
+__global__ __launch_bounds__(kGroupThreads) void count_slots(const int32_t* __restrict__ ids,
+                                                             int slots, int experts,
+                                                             int32_t* __restrict__ counts) {
+  __shared__ int hist[kMaxExperts];
+  for (int e = threadIdx.x; e < experts; e += kGroupThreads) hist[e] = 0;
+  __syncthreads();
+  const int begin = blockIdx.x * kGroupChunk, end = min(slots, begin + kGroupChunk);
+  for (int i = begin + threadIdx.x; i < end; i += kGroupThreads) {
+    const int e = ids[i];
+    if (takes_part(e, experts)) atomicAdd(&hist[e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += kGroupThreads)
+    counts[blockIdx.x * experts + e] = hist[e];
+}
+
+// Exclusive prefix sum of one value a thread over the workgroup.
+__device__ __forceinline__ int block_exclusive(int v, int* wave_totals) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  int s = v;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int o = __shfl_up(s, d);
+    if (lane >= d) s += o;
+  }
+  __syncthreads();
+  if (lane == kWave - 1) wave_totals[wave] = s;
+  __syncthreads();
+  int before = 0;
+  for (int w = 0; w < wave; ++w) before += wave_totals[w];
+  return before + s - v;
+}
+
+// order[row]: the slots in the order of their experts. `counts` may be null with one chunk. The
+// first workgroup writes the list of row tiles of bm rows. The order of the slots within an
+// expert is that of the LDS atomics; a row's products do not depend on the row it stands in.
+__global__ __launch_bounds__(kGroupThreads) void place_slots(const int32_t* __restrict__ ids,
+                                                             int slots, int experts, int bm,
+                                                             const int32_t* __restrict__ counts,
+                                                             int chunks,
+                                                             int32_t* __restrict__ order,
+                                                             int4* __restrict__ tiles,
+                                                             int32_t* __restrict__ tile_count) {
+  __shared__ int cursor[kMaxExperts];
+  __shared__ int wave_totals[kGroupThreads / kWave];
+  const int e = threadIdx.x;
+  const int begin = blockIdx.x * kGroupChunk, end = min(slots, begin + kGroupChunk);
+  int before = 0, total = 0;
+  if (counts) {
+    if (e < experts)
+      for (int c = 0; c < chunks; ++c) {
+        const int n = counts[c * experts + e];
+        total += n;
+        if (c < static_cast<int>(blockIdx.x)) before += n;
+      }
+  } else {
+    cursor[e] = 0;
+    __syncthreads();
+    for (int i = begin + threadIdx.x; i < end; i += kGroupThreads) {
+      const int x = ids[i];
+      if (takes_part(x, experts)) atomicAdd(&cursor[x], 1);
+    }
+    __syncthreads();
+    total = e < experts ? cursor[e] : 0;
+  }
+  const int first = block_exclusive(total, wave_totals);
+  cursor[e] = first + before;
+  if (blockIdx.x == 0) {
+    const int n = (total + bm - 1) / bm;
+    const int at = block_exclusive(n, wave_totals);
+    for (int i = 0; i < n; ++i)
+      tiles[at + i] = make_int4(e, first + i * bm, min(first + (i + 1) * bm, first + total), 0);
+    if (e == kGroupThreads - 1) *tile_count = at + n;
+  }
+  __syncthreads();
+  for (int i = begin + threadIdx.x; i < end; i += kGroupThreads) {
+    const int x = ids[i];
+    if (takes_part(x, experts)) order[atomicAdd(&cursor[x], 1)] = i;
+  }
+}
+
+// ---------------------------------------------------------------------------- the sum over slots
+// out[t] = sum of y[t * top_k + s] over the slots that take part, in fp32, s ascending.
+template <int DT>
+__global__ __launch_bounds__(256) void sum_slots(const uint16_t* __restrict__ y, int64_t ldy,
+                                                 const int32_t* __restrict__ ids,
+                                                 uint16_t* __restrict__ out, int64_t ldo,
+                                                 int64_t tokens, int top_k, int experts, int width,
+                                                 bool vec) {
+  const int chunks = (width + 7) >> 3;
+  const int64_t i = blockIdx.x * int64_t(256) + threadIdx.x;
+  if (i >= tokens * chunks) return;
+  const int64_t t = i / chunks;
+  const int c = static_cast<int>(i - t * chunks) * 8;
+  float sum[8] = {};
+  for (int s = 0; s < top_k; ++s) {
+    const int64_t slot = t * top_k + s;
+    if (!takes_part(ids[slot], experts)) continue;
+    float f[8];
+    unpack8<DT>(ld128(y + slot * ldy + c), f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] += f[e];
+  }
+  uint16_t* o = out + t * ldo + c;
+  if (vec && c + 8 <= width) {
+    st128(o, pack8<DT>(sum));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < width) o[e] = Elem<DT>::from_float(sum[e]);
+  }
+}
+
+// ---------------------------------------------------------------------------- the products
+int64_t pad(int64_t n, int64_t a) { return (n + a - 1) / a * a; }
+
+// Row tile of the grouped products: 0 slots without grouping.
+struct Grouping {
+  int bm;
+};
+
+Grouping choose_grouping(int64_t slots, int64_t experts) {
+  if (slots <= 16) return {0};
+  const int64_t per = slots / experts;
+  if (per <= 8) return {16};
+  if (per <= 64) return {64};
+  return {256};
+}
+
+constexpr int64_t kMaxSlots = 131072;  // slots a pass takes; more tokens run in several passes
+
+struct ExpertWorkspace {
+  int64_t order, tiles, tile_count, counts, xq, xs, act, actq, acts, y, bytes;
+  int64_t tokens;  // a pass
+};
+
+ExpertWorkspace expert_workspace(int64_t tokens, int64_t top_k, int64_t experts, int64_t hidden,
+                                 int64_t inter, bool int8, int64_t x_stride) {
+  ExpertWorkspace w{};
+  // Row offsets into x are 32-bit within a pass.
+  const int64_t most = std::max<int64_t>(
+      1, std::min<int64_t>(kMaxSlots / top_k, ((int64_t(1) << 32) - 1) / x_stride));
+  const int64_t t = std::min(tokens, most);
+  const int64_t slots = t * top_k;
+  w.tokens = t;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at = pad(at + bytes, 256);
+    return o;
+  };
+  w.order = take(slots * 4);
+  w.tiles = take((std::min(experts, slots) + slots / 16 + 1) * 16);
+  w.tile_count = take(4);
+  w.counts = take(pad(slots, kGroupChunk) / kGroupChunk * experts * 4);
+  w.act = take(slots * (int8 ? pad(inter, 4) * 4 : inter * 2));
+  if (int8) {
+    w.xq = take(t * pad(hidden, 16));
+    w.xs = take(t * 4);
+    w.actq = take(slots * pad(inter, 16));
+    w.acts = take(slots * 4);
+  }
+  w.y = take(slots * pad(hidden, 8) * 2);
+  w.bytes = at;
+  return w;
+}
+
+template <int IN, int OT, int MODE, bool SILU>
+void launch_product(const ProductArgs& base, int bm, int64_t slots, int64_t experts,
+                    hipStream_t s) {
+  ProductArgs a = base;
+  // Tiles of bm rows that so many slots need at most: every full one and one more an expert.
+  const int64_t most = bm == 0 ? slots : slots / bm + std::min(experts, slots);
+  auto grid = [&](int bn) {
+    a.tiles_n = (a.columns + bn - 1) / bn;
+    return dim3(static_cast<uint32_t>(pad(most * a.tiles_n, 8)));
+  };
+  if (bm <= 16) {
+    const dim3 g = grid(SILU ? 16 : 32);
+    product_rows<IN, OT, MODE, SILU, 2, 4><<<g, 256, 0, s>>>(a);
+  } else if (bm == 64) {
+    const dim3 g = grid(SILU ? 32 : 64);
+    product_tile<IN, OT, MODE, SILU, 64, 64, 2, 2, 4><<<g, 256, 0, s>>>(a);
+  } else {
+    const dim3 g = grid(SILU ? 128 : 256);
+    product_tile<IN, OT, MODE, SILU, 256, 256, 2, 2, 2><<<g, 256, 0, s>>>(a);
+  }
+}
+
+struct ExpertCall {
+  const uint8_t* x;
+  int64_t x_stride;  // bytes
+  const int32_t* ids;
+  const float* weights;
+  const uint8_t* gate_up;
+  const float* gate_up_scales;
+  const uint8_t* down;
+  const float* down_scales;
+  int64_t ld_gate_up, ld_down;  // bytes a row
+  uint16_t* out;
+  int64_t ldo;
+  int64_t tokens, top_k, experts, hidden, inter;
+};
+
+// One pass over c.tokens tokens. IN: the operands' kind, OT: x's and out's type.
+template <int IN, int OT>
+const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* ws, hipStream_t s) {
+  constexpr bool kQuant = IN == kInt8;
+  const int64_t slots = c.tokens * c.top_k;
+  const Grouping g = choose_grouping(slots, c.experts);
+  auto* order = reinterpret_cast<int32_t*>(ws + w.order);
+  auto* tiles = reinterpret_cast<int4*>(ws + w.tiles);
+  auto* tile_count = reinterpret_cast<int32_t*>(ws + w.tile_count);
+  auto* counts = reinterpret_cast<int32_t*>(ws + w.counts);
+  if (g.bm) {
+    const int chunks = static_cast<int>(pad(slots, kGroupChunk) / kGroupChunk);
+    if (chunks > 1) {
+      count_slots<<<dim3(chunks), kGroupThreads, 0, s>>>(c.ids, static_cast<int>(slots),
+                                                         static_cast<int>(c.experts), counts);
+      if (const char* e = launch_status("count_slots")) return e;
+    }
+    place_slots<<<dim3(chunks), kGroupThreads, 0, s>>>(
+        c.ids, static_cast<int>(slots), static_cast<int>(c.experts), g.bm,
+        chunks > 1 ? counts : nullptr, chunks, order, tiles, tile_count);
+    if (const char* e = launch_status("place_slots")) return e;
+  }
+  ProductArgs a{};
+  a.order = g.bm ? order : nullptr;
+  a.tiles = g.bm ? tiles : nullptr;
+  a.tile_count = tile_count;
+  a.ids = c.ids;
+  a.slot_weights = c.weights;
+  a.rows = static_cast<int32_t>(slots);
+  a.top_k = static_cast<int32_t>(c.top_k);
+  a.experts = static_cast<int32_t>(c.experts);
+  a.vec_out = 1;
+  // gate_up with SiLU x mul into act, one row a slot
+  if (kQuant) {
+    auto* xs = reinterpret_cast<float*>(ws + w.xs);
+    if (const char* e = run_quantize_rows(c.x, c.x_stride, ws + w.xq, pad(c.hidden, 16), xs,
+                                          c.tokens, c.hidden, OT, s))
+      return e;
+    a.x = ws + w.xq;
+    a.x_stride = pad(c.hidden, 16);
+    a.x_scales = xs;
+    a.k_bytes = static_cast<int32_t>(pad(c.hidden, 16));
+  } else {
+    a.x = c.x;
+    a.x_stride = c.x_stride;
+    a.k_bytes = static_cast<int32_t>(c.hidden * 2);
+  }
+  a.w = c.gate_up;
+  a.w_stride = c.ld_gate_up;
+  a.w_expert = 2 * c.inter * c.ld_gate_up;
+  a.w_scales = c.gate_up_scales;
+  a.out = ws + w.act;
+  a.ldo = kQuant ? pad(c.inter, 4) : c.inter;
+  a.columns = static_cast<int32_t>(c.inter);
+  launch_product<IN, kQuant ? kFloatOut : OT, kGateUp, true>(a, g.bm, slots, c.experts, s);
+  if (const char* e = launch_status("product (gate_up)")) return e;
+  // down into y, one weighted row a slot
+  if (kQuant) {
+    // Every row of act is quantised; rows that no slot wrote (ids that take no part) are never read.
+    auto* acts = reinterpret_cast<float*>(ws + w.acts);
+    if (const char* e = run_quantize_rows(ws + w.act, a.ldo * 4, ws + w.actq, pad(c.inter, 16),
+                                          acts, slots, c.inter, kFloatOut, s))
+      return e;
+    a.x = ws + w.actq;
+    a.x_stride = pad(c.inter, 16);
+    a.x_scales = acts;
+    a.k_bytes = static_cast<int32_t>(pad(c.inter, 16));
+  } else {
+    a.x = ws + w.act;
+    a.x_stride = c.inter * 2;
+    a.k_bytes = static_cast<int32_t>(c.inter * 2);
+  }
+  a.w = c.down;
+  a.w_stride = c.ld_down;
+  a.w_expert = c.hidden * c.ld_down;
+  a.w_scales = c.down_scales;
+  a.out = ws + w.y;
+  a.ldo = pad(c.hidden, 8);
+  a.columns = static_cast<int32_t>(c.hidden);
+  launch_product<IN, OT, kDown, false>(a, g.bm, slots, c.experts, s);
+  if (const char* e = launch_status("product (down)")) return e;
+  const int64_t threads = c.tokens * (pad(c.hidden, 8) / 8);
+  sum_slots<OT><<<dim3(static_cast<uint32_t>((threads + 255) / 256)), 256, 0, s>>>(
+      reinterpret_cast<const uint16_t*>(ws + w.y), a.ldo, c.ids, c.out, c.ldo, c.tokens,
+      static_cast<int>(c.top_k), static_cast<int>(c.experts), static_cast<int>(c.hidden),
+      c.ldo % 8 == 0 && aligned(c.out, 16));
+  return launch_status("sum_slots");
+}
+
+bool expert_shape_ok(int64_t tokens, int64_t top_k, int64_t experts, int64_t hidden,
+                     int64_t inter, bool int8) {
+  return tokens >= 0 && tokens < (int64_t(1) << 31) && top_k > 0 && top_k <= kMaxTopK &&
+         experts > 0 && experts <= kMaxExperts && hidden > 0 && inter > 0 &&
+         hidden <= 131072 && inter <= 131072 && (int8 || (hidden % 8 == 0 && inter % 8 == 0));
+}
+
+}  // namespace
+}  // namespace mi355x
+
+using namespace mi355x;
+
+extern "C" const char* mi355x_route_experts(const void* logits, int64_t ld, void* weights,
+                                            int32_t* ids, int64_t tokens, int64_t experts,
+                                            int64_t top_k, bool normalize, int dtype,
+                                            void* stream) {
+  if (tokens < 0 || tokens >= (int64_t(1) << 31) || experts <= 0 || experts > kMaxExperts ||
+      top_k <= 0 || top_k > std::min<int64_t>(experts, kMaxTopK) || ld < experts || dtype < 0 ||
+      dtype > 2)
+    return set_error("mi355x_route_experts: unsupported shape (up to 1024 experts, top_k up to 64)");
+  if (tokens == 0) return nullptr;
+  if (!logits || !weights || !ids) return set_error("mi355x_route_experts: null pointer");
+  if (!aligned(logits, dtype == 2 ? 4 : 2) || !aligned(weights, 4) || !aligned(ids, 4))
+    return set_error("mi355x_route_experts: misaligned operand");
+  auto s = static_cast<hipStream_t>(stream);
+  const int e = static_cast<int>(experts), k = static_cast<int>(top_k);
+  auto* p = static_cast<float*>(weights);
+  if (dtype == 0)
+    launch_route<0>(logits, ld, p, ids, tokens, e, k, normalize, s);
+  else if (dtype == 1)
+    launch_route<1>(logits, ld, p, ids, tokens, e, k, normalize, s);
+  else
+    launch_route<2>(logits, ld, p, ids, tokens, e, k, normalize, s);
+  return launch_status("route_kernel");
+}
+
+extern "C" int64_t mi355x_expert_mlp_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts,
+                                                     int64_t hidden, int64_t inter, int64_t ldx,
+                                                     bool int8) {
+  if (!expert_shape_ok(tokens, top_k, experts, hidden, inter, int8) || ldx < hidden ||
+      ldx >= (int64_t(1) << 31))
+    return -1;
+  return expert_workspace(tokens, top_k, experts, hidden, inter, int8, ldx * 2).bytes;
+}
+
+extern "C" const char* mi355x_expert_mlp(const void* x, int64_t ldx, const int32_t* ids,
+                                         const float* weights, const void* gate_up,
+                                         int64_t ld_gate_up, const float* gate_up_scales,
+                                         const void* down, int64_t ld_down,
+                                         const float* down_scales, void* out, int64_t ldo,
+                                         int64_t tokens, int64_t top_k, int64_t experts,
+                                         int64_t hidden, int64_t inter, void* workspace,
+                                         int64_t workspace_bytes, int64_t dtype, void* stream) {
+  const bool int8 = gate_up_scales != nullptr;
+  if (int8 != (down_scales != nullptr))
+    return set_error("mi355x_expert_mlp: gate_up and down weights must be of one kind");
+  const int64_t size = int8 ? 1 : 2;
+  if (!expert_shape_ok(tokens, top_k, experts, hidden, inter, int8) || ldx < hidden ||
+      ldx >= (int64_t(1) << 31) || ldo < hidden || ld_gate_up < (int8 ? pad(hidden, 16) : hidden) ||
+      ld_down < (int8 ? pad(inter, 16) : inter) || ld_gate_up * size % 16 || ld_down * size % 16 ||
+      (!int8 && ldx % 8) || (dtype != 0 && dtype != 1))
+    return set_error("mi355x_expert_mlp: unsupported shape (up to 1024 experts, top_k up to 64, "
+                     "weight and 16-bit x rows of whole 16-byte words)");
+  if (2 * inter * ld_gate_up * size >= (int64_t(1) << 32) ||
+      hidden * ld_down * size >= (int64_t(1) << 32))
+    return set_error("mi355x_expert_mlp: an expert's weight must be less than 4 GiB");
+  if (tokens == 0) return nullptr;
+  if (!x || !ids || !weights || !gate_up || !down || !out || !workspace)
+    return set_error("mi355x_expert_mlp: null pointer");
+  if (!aligned(x, int8 ? 2 : 16) || !aligned(gate_up, 16) || !aligned(down, 16) ||
+      !aligned(out, 2) || !aligned(workspace, 16) || !aligned(ids, 4) || !aligned(weights, 4))
+    return set_error("mi355x_expert_mlp: misaligned operand");
+  const ExpertWorkspace w =
+      expert_workspace(tokens, top_k, experts, hidden, inter, int8, ldx * 2);
+  if (workspace_bytes < w.bytes) return set_error("mi355x_expert_mlp: workspace too small");
+  auto s = static_cast<hipStream_t>(stream);
+  for (int64_t t = 0; t < tokens; t += w.tokens) {
+    ExpertCall c{};
+    c.x = static_cast<const uint8_t*>(x) + t * ldx * 2;
+    c.x_stride = ldx * 2;
+    c.ids = ids + t * top_k;
+    c.weights = weights + t * top_k;
+    c.gate_up = static_cast<const uint8_t*>(gate_up);
+    c.gate_up_scales = gate_up_scales;
+    c.down = static_cast<const uint8_t*>(down);
+    c.down_scales = down_scales;
+    c.ld_gate_up = ld_gate_up * size;
+    c.ld_down = ld_down * size;
+    c.out = static_cast<uint16_t*>(out) + t * ldo;
+    c.ldo = ldo;
+    c.tokens = std::min(w.tokens, tokens - t);
+    c.top_k = top_k;
+    c.experts = experts;
+    c.hidden = hidden;
+    c.inter = inter;
+    auto* ws = static_cast<uint8_t*>(workspace);
+    const char* e = int8 ? (dtype == 0 ? expert_pass<kInt8, 0>(c, w, ws, s)
+                                       : expert_pass<kInt8, 1>(c, w, ws, s))
+                         : (dtype == 0 ? expert_pass<kBf16, 0>(c, w, ws, s)
+                                       : expert_pass<kFp16, 1>(c, w, ws, s));
+    if (e) return e;
+  }
+  return nullptr;
+}

@@ -1,0 +1,528 @@
+// Tile cores of the products whose weights are 8-bit or chosen per token: out = x . w^T for a
+// dense weight [N, K] (quant.hip) and for the experts' weights [E, N, K] over rows grouped by
+// expert (experts.hip).
+//
+// Both operands are handled as rows of bytes. An MFMA operand is 16 bytes a lane in every type
+// here (8 bf16 / fp16 elements, 16 int8 ones) and a step of the K loop is 128 bytes of a row, so
+// one core serves bf16, fp16 and int8; only the instruction and the accumulator differ:
+//   bf16 / fp16  32x32x16 and 16x16x32, fp32 accumulators
+//   int8         32x32x32 and 16x16x64, int32 accumulators (exact up to K = 131,072)
+//
+// Two kernels:
+//   * product_tile: a BM x BN tile, x and w rows copied to an LDS ring of 128-byte rows
+//     (global_load_lds_dwordx4, 16-byte chunks XOR-swizzled), waves of 32 x 32 MFMA blocks;
+//   * product_rows: up to 16 rows of x, weights from global memory straight into MFMA operands, the
+//     waves of a workgroup sharing K. For few rows, where the weight bytes are all that counts.
+#pragma once
+
+#include <cstdint>
+#include <type_traits>
+
+#include "common.h"
+
+namespace mi355x {
+
+// Element kinds of the operands and of the output.
+constexpr int kBf16 = 0, kFp16 = 1, kInt8 = 2;  // operands
+constexpr int kFloatOut = 2;                    // outputs: 0 bf16, 1 fp16, 2 fp32
+
+// Rows of x and of the output.
+//   kDense    row r of x and of out is r; one weight
+//   kGateUp   row r of the grouped order reads x row order[r] / top_k and writes out row r
+//   kDown     row r of the grouped order reads x row r and writes out row order[r], times that
+//             slot's weight
+constexpr int kDense = 0, kGateUp = 1, kDown = 2;
+
+struct ProductArgs {
+  const uint8_t* x;
+  const uint8_t* w;
+  void* out;
+  const float* x_scales;      // int8: one a row of x
+  const float* w_scales;      // int8: [E][w_rows]
+  const int32_t* order;       // grouped: slot (token * top_k + s) of every grouped row; null: r itself
+  const int32_t* ids;         // with a null tile list: expert of every slot
+  const int4* tiles;          // grouped: {expert, first row, end row, 0} per row tile
+  const int32_t* tile_count;  // grouped: tiles in the list
+  const float* slot_weights;  // kDown: one a slot
+  int64_t x_stride;           // bytes a row
+  int64_t w_stride;           // bytes a row
+  int64_t w_expert;           // bytes an expert
+  int64_t ldo;                // elements a row of out
+  int32_t rows;               // kDense: rows of x. Grouped without a tile list: slots
+  int32_t columns;            // columns of out (SILU: half the weight rows)
+  int32_t k_bytes;            // bytes of K, a multiple of 16
+  int32_t top_k;
+  int32_t experts;
+  int32_t tiles_m, tiles_n;   // kDense: row tiles; column tiles of every row tile
+  int32_t vec_out;            // out rows take aligned stores of four elements
+};
+
+// ---------------------------------------------------------------------------- MFMA by type
+typedef __bf16 prod_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 prod_f16x8 __attribute__((ext_vector_type(8)));
+typedef int prod_i32x4 __attribute__((ext_vector_type(4)));
+typedef float prod_f32x4 __attribute__((ext_vector_type(4)));
+typedef float prod_f32x16 __attribute__((ext_vector_type(16)));
+typedef int prod_i32x16 __attribute__((ext_vector_type(16)));
+
+template <int IN>
+struct Mma {
+  using Acc16 = std::conditional_t<IN == kInt8, prod_i32x16, prod_f32x16>;  // 32 x 32 block
+  using Acc4 = std::conditional_t<IN == kInt8, prod_i32x4, prod_f32x4>;     // 16 x 16 block
+  using Scalar = std::conditional_t<IN == kInt8, int, float>;
+
+  __device__ __forceinline__ static Acc16 block32(const uint4& a, const uint4& b, Acc16 c) {
+    if constexpr (IN == kBf16)
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(prod_bf16x8, a),
+                                                     __builtin_bit_cast(prod_bf16x8, b), c, 0, 0,
+                                                     0);
+    else if constexpr (IN == kFp16)
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(prod_f16x8, a),
+                                                    __builtin_bit_cast(prod_f16x8, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(prod_i32x4, a),
+                                                   __builtin_bit_cast(prod_i32x4, b), c, 0, 0, 0);
+  }
+  __device__ __forceinline__ static Acc4 block16(const uint4& a, const uint4& b, Acc4 c) {
+    if constexpr (IN == kBf16)
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(prod_bf16x8, a),
+                                                     __builtin_bit_cast(prod_bf16x8, b), c, 0, 0,
+                                                     0);
+    else if constexpr (IN == kFp16)
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(prod_f16x8, a),
+                                                    __builtin_bit_cast(prod_f16x8, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(prod_i32x4, a),
+                                                   __builtin_bit_cast(prod_i32x4, b), c, 0, 0, 0);
+  }
+};
+
+// silu(g) * u. exp(-g) overflows to +inf for g below about -88: g / inf = -0, the limit.
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  return (g / (1.f + __expf(-g))) * u;
+}
+
+// Four consecutive output elements of a row, of which the first `n` exist.
+template <int OT>
+__device__ __forceinline__ void store4(void* out, int64_t at, const float (&v)[4], int n, bool vec) {
+  if constexpr (OT == kFloatOut) {
+    float* p = static_cast<float*>(out) + at;
+    if (vec && n >= 4) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      for (int e = 0; e < 4; ++e)
+        if (e < n) p[e] = v[e];
+    }
+  } else {
+    uint16_t* p = static_cast<uint16_t*>(out) + at;
+    if (vec && n >= 4) {
+      *reinterpret_cast<uint2*>(p) =
+          make_uint2(Elem<OT>::pack2(v[0], v[1]), Elem<OT>::pack2(v[2], v[3]));
+    } else {
+      for (int e = 0; e < 4; ++e)
+        if (e < n) p[e] = Elem<OT>::from_float(v[e]);
+    }
+  }
+}
+
+// What a row of a tile is multiplied with and where it goes.
+struct RowOut {
+  int64_t at;    // row of out
+  float scale;   // int8: scale of the x row
+  float weight;  // kDown: weight of the slot
+};
+
+template <int IN, int MODE>
+__device__ __forceinline__ RowOut row_out(const ProductArgs& a, int row) {
+  RowOut r{row, 1.f, 1.f};
+  if constexpr (MODE == kDense) {
+    if constexpr (IN == kInt8) r.scale = a.x_scales[row];
+  } else {
+    const int slot = a.order ? a.order[row] : row;
+    if constexpr (MODE == kGateUp) {
+      if constexpr (IN == kInt8) r.scale = a.x_scales[slot / a.top_k];
+    } else {
+      if constexpr (IN == kInt8) r.scale = a.x_scales[row];
+      r.at = slot;
+      r.weight = a.slot_weights[slot];
+    }
+  }
+  return r;
+}
+
+// The accumulators of four consecutive columns of a row, scaled and stored. `acc` (SILU: the gate
+// columns, with the matching up columns in `up`); the scales are those of the weight rows.
+template <int IN, int OT, int MODE, bool SILU, typename T>
+__device__ __forceinline__ void finish4(const ProductArgs& a, const RowOut& r, int column,
+                                        const float* w_scales, const T (&acc)[4],
+                                        const T (&up)[4]) {
+  const int n = a.columns - column;
+  if (n <= 0) return;
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float g = static_cast<float>(acc[e]);
+    if constexpr (IN == kInt8) g = g * r.scale * w_scales[min(column + e, a.columns - 1)];
+    if constexpr (SILU) {
+      float u = static_cast<float>(up[e]);
+      if constexpr (IN == kInt8)
+        u = u * r.scale * w_scales[a.columns + min(column + e, a.columns - 1)];
+      g = silu_mul(g, u);
+    }
+    v[e] = MODE == kDown ? g * r.weight : g;
+  }
+  store4<OT>(a.out, r.at * a.ldo + column, v, n, a.vec_out);
+}
+
+// A row tile: its expert and rows. Returns false where the workgroup has none.
+struct RowTile {
+  int expert, begin, end;
+};
+
+template <int MODE, int BM>
+__device__ __forceinline__ bool row_tile(const ProductArgs& a, int tm, RowTile* t) {
+  if constexpr (MODE == kDense) {
+    *t = {0, tm * BM, min(a.rows, (tm + 1) * BM)};
+    return true;
+  } else if (a.tiles) {
+    const int4 v = a.tiles[tm];
+    *t = {__builtin_amdgcn_readfirstlane(v.x), __builtin_amdgcn_readfirstlane(v.y),
+          __builtin_amdgcn_readfirstlane(v.z)};
+    return true;
+  } else {  // one slot a tile
+    const int e = __builtin_amdgcn_readfirstlane(a.ids[tm]);
+    *t = {e, tm, tm + 1};
+    return e >= 0 && e < a.experts;
+  }
+}
+
+// Workgroup -> (row tile, column tile). Workgroup i runs on XCD i mod 8; every XCD takes a
+// contiguous eighth of the tiles, so those that share weights or rows of x meet in its L2. Column
+// tiles are innermost. False for the workgroups past the last tile (the grid of a grouped product
+// is sized for the most tiles that its rows can need).
+template <int MODE>
+__device__ __forceinline__ bool tile_of_block(const ProductArgs& a, int* tm, int* tn) {
+  int count;
+  if constexpr (MODE == kDense)
+    count = a.tiles_m;
+  else
+    count = a.tiles ? *a.tile_count : a.rows;
+  const int total = count * a.tiles_n;
+  const int per = (total + 7) >> 3;
+  const int i = static_cast<int>(blockIdx.x >> 3);
+  const int lin = static_cast<int>(blockIdx.x & 7) * per + i;
+  if (i >= per || lin >= total) return false;
+  *tm = lin / a.tiles_n;
+  *tn = lin - *tm * a.tiles_n;
+  return true;
+}
+
+__device__ __forceinline__ uint32_t source_row(const ProductArgs& a, int row, bool gathered) {
+  if (!gathered) return row;
+  return (a.order ? a.order[row] : row) / a.top_k;
+}
+
+// ---------------------------------------------------------------------------- product_tile
+static __device__ __align__(16) const uint32_t kProductZeros[4] = {0, 0, 0, 0};
+
+constexpr int kProdRow = 128;  // bytes of a tile row in a stage
+
+// Swizzled position of 16-byte chunk c in tile row r: any 8 consecutive rows put a chunk in 8
+// positions and over 16 rows the (row parity, position) pairs are distinct, so the 32 lanes of an
+// operand read hit every bank evenly.
+__device__ __forceinline__ int prod_chunk(int c, int r) { return c ^ ((r & 7) ^ ((r >> 3) & 1)); }
+
+// 16 bytes a lane from base + offset into lds_base + 16 * lane (see copy_to_lds).
+__device__ __forceinline__ void copy_offset_to_lds(const uint8_t* base, uint32_t offset,
+                                                   uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_base), "v"(offset),
+               "s"(base)
+               : "m0");
+}
+
+// All of this wave's LDS reads have returned; then the workgroup barrier. The memory clobbers keep
+// the compiler's LDS reads on their side of it.
+__device__ __forceinline__ void barrier_after_reads() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// With SILU, rows 8 q .. 8 q + 7 of each 32-row block of the weight tile are gate rows for even q
+// and the matching up rows for odd q, so a lane holds gate and up of a column side by side.
+// Column of a tile row, relative to the tile's first column:
+__device__ __forceinline__ int silu_column(int r) {
+  const int rr = r & 31;
+  return (r >> 5) * 16 + (rr >> 4) * 8 + (rr & 7);
+}
+
+template <int IN, int OT, int MODE, bool SILU, int BM, int BN, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
+  constexpr int NW = WM * WN;
+  constexpr int kWaveM = BM / WM, kWaveN = BN / WN;
+  constexpr int A_BLK = kWaveN / 32, B_BLK = kWaveM / 32;
+  static_assert(kWaveM % 32 == 0 && kWaveN % 32 == 0, "wave tile must be 32-aligned");
+  constexpr int kGroups = (BM + BN) / 8;
+  static_assert(kGroups % NW == 0 && (BM / 8) % NW == 0, "copies must split evenly over the waves");
+  constexpr int kCopies = kGroups / NW, kCopiesX = BM / 8 / NW;
+  constexpr int kStage = (BM + BN) * kProdRow;
+  static_assert(STAGES >= 2 && STAGES * kStage <= 160 * 1024, "LDS");
+  constexpr int kBnOut = SILU ? BN / 2 : BN;
+  using M = Mma<IN>;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * kStage];
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  if (a.columns < 0) lds[tid] = 0;  // never taken; the copies' LDS writes are invisible
+
+  int tm, tn;
+  if (!tile_of_block<MODE>(a, &tm, &tn)) return;
+  RowTile t;
+  if (!row_tile<MODE, BM>(a, tm, &t)) return;
+  const int n0 = tn * kBnOut;
+  const int n_k = (a.k_bytes + kProdRow - 1) / kProdRow;
+  const bool tail = a.k_bytes % kProdRow != 0;
+
+  // Copy side: copy j of a wave covers tile rows 8 g .. 8 g + 7, g = wave + NW j (x rows first);
+  // lane -> row 8 g + lane / 8, position lane % 8. Rows past the end repeat the last one and are
+  // never stored.
+  const uint32_t lds_base = lds_address(lds);
+  const uint8_t* x_base = a.x;
+  if constexpr (MODE != kGateUp) x_base += t.begin * a.x_stride;
+  const uint8_t* w_base = a.w + t.expert * a.w_expert;
+  if constexpr (!SILU) w_base += static_cast<int64_t>(n0) * a.w_stride;
+  uint32_t off[kCopies];
+#pragma unroll
+  for (int j = 0; j < kCopies; ++j) {
+    const int g = wave + NW * j;
+    int r = 8 * g + (lane >> 3);
+    uint32_t row, stride;
+    if (j < kCopiesX) {
+      const int m = min(t.begin + r, t.end - 1);
+      row = MODE == kGateUp ? source_row(a, m, true) : m - t.begin;
+      stride = static_cast<uint32_t>(a.x_stride);
+    } else {
+      r -= BM;
+      if constexpr (SILU) {
+        const int c = min(n0 + silu_column(r), a.columns - 1);
+        row = ((r >> 3) & 1) ? a.columns + c : c;
+      } else {
+        row = min(r, a.columns - 1 - n0);
+      }
+      stride = static_cast<uint32_t>(a.w_stride);
+    }
+    off[j] = row * stride + prod_chunk(lane & 7, r) * 16;
+  }
+  auto issue = [&](int step, int stage) {
+    const uint32_t dst = lds_base + stage * kStage + wave * 1024;
+    const int64_t k = static_cast<int64_t>(step) * kProdRow;
+    const uint8_t* xb = x_base + k;
+    const uint8_t* wb = w_base + k;
+    if (tail && step == n_k - 1) {
+      // chunks past K come as zeros in both operands
+#pragma unroll
+      for (int j = 0; j < kCopies; ++j) {
+        const int r = 8 * (wave + NW * j) + (lane >> 3);
+        const int c = prod_chunk(lane & 7, j < kCopiesX ? r : r - BM);
+        const uint8_t* src = (j < kCopiesX ? xb : wb) + off[j];
+        if (k + c * 16 >= a.k_bytes) src = reinterpret_cast<const uint8_t*>(kProductZeros);
+        copy_to_lds(src, dst + j * NW * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kCopies; ++j)
+        copy_offset_to_lds(j < kCopiesX ? xb : wb, off[j], dst + j * NW * 1024);
+    }
+  };
+
+  // Operand side: block rows r + 32 i share the swizzle of r; chunk 2 kk + half of a row.
+  const int wm = wave % WM, wn = wave / WM;
+  const int col = lane & 31, half = lane >> 5;
+  const int xr = wm * kWaveM + col, wr = wn * kWaveN + col;
+  uint32_t x_at[4], w_at[4];
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) {
+    x_at[kk] = xr * kProdRow + prod_chunk(2 * kk + half, xr) * 16;
+    w_at[kk] = (BM + wr) * kProdRow + prod_chunk(2 * kk + half, wr) * 16;
+  }
+  typename M::Acc16 acc[A_BLK][B_BLK];
+#pragma unroll
+  for (int i = 0; i < A_BLK; ++i)
+#pragma unroll
+    for (int j = 0; j < B_BLK; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+
+  uint4 af[2][A_BLK], bf[2][B_BLK];
+  auto read = [&](int stage, int kk, int to) {
+    const uint8_t* sb = lds + stage * kStage;
+#pragma unroll
+    for (int i = 0; i < A_BLK; ++i)
+      af[to][i] = *reinterpret_cast<const uint4*>(sb + w_at[kk] + i * 32 * kProdRow);
+#pragma unroll
+    for (int j = 0; j < B_BLK; ++j)
+      bf[to][j] = *reinterpret_cast<const uint4*>(sb + x_at[kk] + j * 32 * kProdRow);
+  };
+
+  // Ring of STAGES steps. The operands of a quarter step are read while the quarter before is
+  // multiplied, also across the barrier between two steps.
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s)
+    if (s < n_k) issue(s, s);
+  wait_tiles_ahead<kCopies, STAGES - 1>(min(STAGES - 1, n_k - 1));
+  barrier_after_reads();
+  read(0, 0, 0);
+  int stage = 0;
+  for (int step = 0; step < n_k; ++step) {
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      if (kk < 3) {
+        read(stage, kk + 1, (kk + 1) & 1);
+      } else if (step + 1 < n_k) {
+        // The next step's copies are in, every wave has read this one: its buffer is free.
+        wait_tiles_ahead<kCopies, STAGES - 2>(min(STAGES - 2, n_k - 2 - step));
+        barrier_after_reads();
+        if (step + STAGES < n_k) issue(step + STAGES, stage);
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
+        read(stage, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < A_BLK; ++i)
+#pragma unroll
+        for (int j = 0; j < B_BLK; ++j)
+          acc[i][j] = M::block32(af[kk & 1][i], bf[kk & 1][j], acc[i][j]);
+    }
+  }
+
+  // A lane holds x row `col` of each B block and weight rows 8 q + 4 half + e of each A block in
+  // accumulator elements 4 q + e.
+  const float* w_scales = nullptr;
+  if constexpr (IN == kInt8)
+    w_scales = a.w_scales + static_cast<int64_t>(t.expert) * (SILU ? 2 : 1) * a.columns;
+#pragma unroll
+  for (int j = 0; j < B_BLK; ++j) {
+    const int row = t.begin + wm * kWaveM + 32 * j + col;
+    if (row >= t.end) continue;
+    const RowOut r = row_out<IN, MODE>(a, row);
+#pragma unroll
+    for (int i = 0; i < A_BLK; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; q += SILU ? 2 : 1) {
+        typename M::Scalar v[4], u[4] = {};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = acc[i][j][4 * q + e];
+          if constexpr (SILU) u[e] = acc[i][j][4 * q + 4 + e];
+        }
+        const int wrow = wn * kWaveN + 32 * i + 8 * q + 4 * half;
+        finish4<IN, OT, MODE, SILU>(a, r, n0 + (SILU ? silu_column(wrow) : wrow), w_scales, v, u);
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------- product_rows
+// Up to 16 rows of x against 16 columns a block (SILU: 16 gate and the matching 16 up rows; else
+// NB blocks of 16 weight rows). The four waves take a quarter of K each and their sums are joined
+// in LDS. A lane's operand rows are lane % 16; of a 128-byte step it holds bytes 32 g .. 32 g + 31,
+// g = lane / 16, as two operands: K is summed in another order than it is stored, the same one in
+// both operands, so whole 128-byte lines are read.
+template <int IN, int OT, int MODE, bool SILU, int NB, int DEPTH>
+__global__ __launch_bounds__(256) void product_rows(ProductArgs a) {
+  static_assert(!SILU || NB == 2, "a gate and an up block");
+  constexpr int kOut = SILU ? 16 : 16 * NB;
+  using M = Mma<IN>;
+  using Acc = typename M::Acc4;
+  __shared__ Acc sums[NB][4][64];
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  int tm, tn;
+  if (!tile_of_block<MODE>(a, &tm, &tn)) return;
+  RowTile t;
+  if (!row_tile<MODE, 16>(a, tm, &t)) return;
+  const int n0 = tn * kOut;
+  const int r = lane & 15, g = lane >> 4;
+
+  const int m = min(t.begin + r, t.end - 1);
+  const uint8_t* x_row =
+      a.x + static_cast<int64_t>(source_row(a, m, MODE == kGateUp)) * a.x_stride + g * 32;
+  const uint8_t* w_row[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int c = min(n0 + (SILU ? 0 : 16 * b) + r, a.columns - 1);
+    w_row[b] = a.w + t.expert * a.w_expert +
+               static_cast<int64_t>(SILU && b ? a.columns + c : c) * a.w_stride + g * 32;
+  }
+  const int n_k = (a.k_bytes + kProdRow - 1) / kProdRow;
+  const int per = (n_k + 3) >> 2;
+  const int first = min(n_k, wave * per), last = min(n_k, first + per);
+
+  uint4 wf[DEPTH][NB][2], xf[DEPTH][2];
+  auto load = [&](int step, int to) {
+    const int64_t k = static_cast<int64_t>(step) * kProdRow;
+    if (k + kProdRow <= a.k_bytes) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) wf[to][b][h] = ld128_nt(w_row[b] + k + 16 * h);
+        xf[to][h] = ld128(x_row + k + 16 * h);
+      }
+    } else {  // the end of K: chunks past it are zeros in both operands
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool in = k + g * 32 + 16 * h < a.k_bytes;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          wf[to][b][h] = in ? ld128(w_row[b] + k + 16 * h) : make_uint4(0, 0, 0, 0);
+        xf[to][h] = in ? ld128(x_row + k + 16 * h) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  };
+  Acc acc[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[b][e] = 0;
+
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d)
+    if (first + d < last) load(first + d, d);
+  for (int step = first; step < last; step += DEPTH) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      if (step + d >= last) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[b] = M::block16(wf[d][b][h], xf[d][h], acc[b]);
+      if (step + d + DEPTH < last) load(step + d + DEPTH, d);
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) sums[b][wave][lane] = acc[b];
+  __syncthreads();
+
+  // Wave b finishes block b (SILU: wave 0 both). A lane holds x row lane % 16 and weight rows
+  // 4 g + e.
+  if (wave >= (SILU ? 1 : NB)) return;
+  const int row = t.begin + r;
+  if (row >= t.end) return;
+  const RowOut ro = row_out<IN, MODE>(a, row);
+  const float* w_scales = nullptr;
+  if constexpr (IN == kInt8)
+    w_scales = a.w_scales + static_cast<int64_t>(t.expert) * (SILU ? 2 : 1) * a.columns;
+  auto total = [&](int b, typename M::Scalar(&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      v[e] = (sums[b][0][lane][e] + sums[b][1][lane][e]) +
+             (sums[b][2][lane][e] + sums[b][3][lane][e]);
+  };
+  typename M::Scalar v[4], u[4] = {};
+  total(SILU ? 0 : wave, v);
+  if constexpr (SILU) total(NB - 1, u);
+  finish4<IN, OT, MODE, SILU>(a, ro, n0 + (SILU ? 0 : 16 * wave) + 4 * g, w_scales, v, u);
+}
+
+}  // namespace mi355x

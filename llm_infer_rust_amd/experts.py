@@ -1,0 +1,114 @@
+"""Layers of experts on the gfx950 kernels.
+
+* ``route_experts(logits, top_k)``: the experts of every token and their weights (softmax, top-k);
+* ``expert_mlp(x, ids, weights, gate_up, down)``: the gate_up, SiLU x mul and down products of the
+  experts that each token was routed to, summed with the router's weights.
+
+In place of the dense MLP of ``src/models/qwen3/model.rs:478-534``; the reference has no layers of
+experts. Nothing is read back to the host, so both can be captured in a HIP graph. Inference only:
+a call whose gradient would be wanted is refused.
+"""
+from __future__ import annotations
+
+import torch
+
+from ._native import NativeError, check, lib, on_device, stream_of
+from .int8 import _ROW_DTYPES, Int8Weight, _check_rows, _refuse_grad, _row_stride
+
+MAX_EXPERTS = 1024
+MAX_TOP_K = 64
+
+
+def route_experts(logits: torch.Tensor, top_k: int,
+                  normalize: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(weights fp32 [T, top_k], ids int32 [T, top_k])`` of router logits ``[T, E]`` (bf16, fp16
+    or fp32): the ``top_k`` largest probabilities of ``softmax(logits)``, largest first, equal ones
+    by the lower index; with ``normalize`` divided by their sum. A row of only -inf gets the
+    weights 0, a row with a NaN or a +inf the weights NaN."""
+    _check_rows(logits, "route_experts")
+    if logits.dtype not in _ROW_DTYPES:
+        raise NativeError(
+            f"route_experts: expected bfloat16, float16 or float32, got {logits.dtype}")
+    t, e = logits.shape
+    top_k = int(top_k)
+    if not 0 < e <= MAX_EXPERTS or not 0 < top_k <= min(e, MAX_TOP_K):
+        raise NativeError(f"route_experts: expected 1 to {MAX_EXPERTS} experts and top_k of 1 to "
+                          f"min(experts, {MAX_TOP_K})")
+    _refuse_grad("route_experts", logits)
+    with on_device(logits.device):
+        weights = torch.empty((t, top_k), dtype=torch.float32, device=logits.device)
+        ids = torch.empty((t, top_k), dtype=torch.int32, device=logits.device)
+        check(lib().mi355x_route_experts(logits.data_ptr(), _row_stride(logits),
+                                         weights.data_ptr(), ids.data_ptr(), t, e, top_k,
+                                         bool(normalize), _ROW_DTYPES[logits.dtype],
+                                         stream_of(logits)), "route_experts")
+    return weights, ids
+
+
+def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
+               gate_up: torch.Tensor | Int8Weight, down: torch.Tensor | Int8Weight,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[t] = sum_s weights[t, s] * down[e] @ (silu(g) * u)``, ``(g, u) = gate_up[e] @ x[t]``,
+    ``e = ids[t, s]``.
+
+    ``x`` ``[T, H]`` bf16 or fp16; ``ids`` int32 and ``weights`` fp32 ``[T, top_k]`` as
+    ``route_experts`` gives them (an id outside ``[0, E)`` adds nothing: pad rows, experts held
+    elsewhere); ``gate_up`` ``[E, 2 I, H]`` (gate rows, then up rows) and ``down`` ``[E, H, I]``,
+    both of x's type (H, I and x's row stride multiples of 8, 16-byte aligned) or both
+    ``Int8Weight`` (any sizes): then x is quantised a token and ``silu(g) * u`` a slot. ``out`` may
+    be given; it must not share memory with ``x``."""
+    _check_rows(x, "expert_mlp")
+    dt = _ROW_DTYPES.get(x.dtype)
+    if dt not in (0, 1):
+        raise NativeError(f"expert_mlp: expected bfloat16 or float16 tensor, got {x.dtype}")
+    t, h = x.shape
+    if (ids.dtype != torch.int32 or weights.dtype != torch.float32 or ids.dim() != 2
+            or ids.size(0) != t or ids.shape != weights.shape or ids.device != x.device
+            or weights.device != x.device or not ids.is_contiguous()
+            or not weights.is_contiguous()):
+        raise NativeError("expert_mlp: expected contiguous int32 ids and fp32 weights [T, top_k]")
+    top_k = ids.size(1)
+    if not 0 < top_k <= MAX_TOP_K:
+        raise NativeError(f"expert_mlp: expected top_k of 1 to {MAX_TOP_K}")
+    int8 = isinstance(gate_up, Int8Weight)
+    if int8 != isinstance(down, Int8Weight):
+        raise NativeError("expert_mlp: gate_up and down must be of one kind")
+    gu, dn = (gate_up.values, down.values) if int8 else (gate_up, down)
+    if (gu.dim() != 3 or dn.dim() != 3 or gu.size(0) != dn.size(0) or gu.size(2) != h
+            or dn.size(1) != h or gu.size(1) != 2 * dn.size(2) or gu.device != x.device
+            or dn.device != x.device or (not int8 and (gu.dtype != x.dtype or dn.dtype != x.dtype
+                                                       or not gu.is_contiguous()
+                                                       or not dn.is_contiguous()))):
+        raise NativeError("expert_mlp: expected gate_up [E, 2 I, H] and down [E, H, I] of x's type "
+                          "on its device")
+    e, inter = gu.size(0), dn.size(2)
+    if 0 in (e, h, inter) or e > MAX_EXPERTS:
+        raise NativeError(f"expert_mlp: expected 1 to {MAX_EXPERTS} experts of no empty dimension")
+    ldx = _row_stride(x)
+    if not int8 and (h % 8 or inter % 8 or ldx % 8 or x.data_ptr() % 16 or gu.data_ptr() % 16
+                     or dn.data_ptr() % 16):
+        raise NativeError("expert_mlp: 16-bit weights need H, I and x's row stride to be multiples "
+                          "of 8 and 16-byte aligned rows")
+    _refuse_grad("expert_mlp", x, weights, gu, dn)
+    if out is None:
+        out = torch.empty((t, h), dtype=x.dtype, device=x.device)
+    elif (out.shape != (t, h) or out.dtype != x.dtype or out.device != x.device
+          or (h > 1 and out.stride(1) != 1) or (t > 1 and out.stride(0) < h)):
+        raise NativeError("expert_mlp: invalid output")
+    elif out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
+        raise NativeError("expert_mlp: out must not share memory with x")
+    with on_device(x.device):
+        need = lib().mi355x_expert_mlp_workspace_bytes(t, top_k, e, h, inter, ldx, int8)
+        if need < 0:
+            raise NativeError("expert_mlp: invalid shape")
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=x.device)
+        check(lib().mi355x_expert_mlp(
+            x.data_ptr(), ldx, ids.data_ptr(), weights.data_ptr(), gu.data_ptr(),
+            gate_up.row_stride if int8 else h, gate_up.scales.data_ptr() if int8 else None,
+            dn.data_ptr(), down.row_stride if int8 else inter,
+            down.scales.data_ptr() if int8 else None, out.data_ptr(), _row_stride(out), t, top_k,
+            e, h, inter, ws.data_ptr(), need, dt, stream_of(x)), "expert_mlp")
+    return out
+
+
+__all__ = ["route_experts", "expert_mlp", "NativeError"]

@@ -1,0 +1,165 @@
+"""Projections in 8-bit integers on the gfx950 kernels.
+
+* ``quantize_rows(x)``: int8 rows with one fp32 scale each (``max |x| / 127``);
+* ``Int8Weight``: an int8 weight with one fp32 scale an output channel, of one matrix ``[N, K]`` or
+  of a stack of experts' matrices ``[E, N, K]``;
+* ``linear_int8(x, weight)``: ``x @ weight.T`` with the 16-bit rows of ``x`` quantised in the call,
+  exact int32 sums and one rounding, optionally with the SiLU x mul of a gate_up projection.
+
+The counterpart of ``src/layers/linear.rs:5-7`` for weights held in 8 bits; the reference itself
+has 16-bit weights only. Inference only: a call whose gradient would be wanted is refused.
+"""
+from __future__ import annotations
+
+import torch
+
+from ._native import NativeError, check, lib, on_device, stream_of
+
+_ROW_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_K = 131072  # 127 * 127 * K stays inside int32
+
+
+def _padded(k: int) -> int:
+    return (k + 15) // 16 * 16
+
+
+def _refuse_grad(what: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise NativeError(f"{what}: no gradient is recorded; call it under torch.no_grad()")
+
+
+def _check_rows(x: torch.Tensor, what: str) -> None:
+    if not x.is_cuda:
+        raise NativeError(f"{what}: expected a GPU tensor")
+    if x.dim() != 2 or (x.size(1) > 1 and x.stride(1) != 1):
+        raise NativeError(f"{what}: expected rows [T, K] of unit column stride")
+    if x.size(0) > 1 and x.stride(0) < x.size(1):
+        raise NativeError(f"{what}: rows must not overlap")
+
+
+def _row_stride(x: torch.Tensor) -> int:
+    """Elements between rows; a single row's stride is never used and may be anything."""
+    return x.stride(0) if x.size(0) > 1 else x.size(1)
+
+
+def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(values int8 [T, K], scales fp32 [T])`` of ``x`` ``[T, K]`` in bf16, fp16 or fp32:
+    ``scales = max |x| / 127`` and ``values = rint(127 x / max |x|)`` a row (half to even). ``values``
+    is a view of rows padded with zeros to 16 columns. A row with an inf or a NaN gets the scale
+    NaN, a row of zeros the scale 0."""
+    _check_rows(x, "quantize_rows")
+    if x.dtype not in _ROW_DTYPES:
+        raise NativeError(f"quantize_rows: expected bfloat16, float16 or float32, got {x.dtype}")
+    if x.size(1) == 0:
+        raise NativeError("quantize_rows: rows must not be empty")
+    _refuse_grad("quantize_rows", x)
+    t, k = x.shape
+    with on_device(x.device):
+        values = torch.empty((t, _padded(k)), dtype=torch.int8, device=x.device)
+        scales = torch.empty(t, dtype=torch.float32, device=x.device)
+        check(lib().mi355x_quantize_rows(x.data_ptr(), _row_stride(x), values.data_ptr(),
+                                         values.size(1), scales.data_ptr(), t, k,
+                                         _ROW_DTYPES[x.dtype], stream_of(x)), "quantize_rows")
+    return values[:, :k], scales
+
+
+class Int8Weight:
+    """int8 ``values`` ``[N, K]`` (or ``[E, N, K]`` for experts) and fp32 ``scales`` ``[N]``
+    (``[E, N]``): the weight ``values * scales[..., None]``. Rows whose length is no multiple of 16
+    are laid out once with a padded stride."""
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor):
+        if (values.dtype != torch.int8 or values.dim() not in (2, 3)
+                or scales.dtype != torch.float32 or scales.shape != values.shape[:-1]
+                or scales.device != values.device):
+            raise NativeError("int8 weight: expected int8 values [N, K] or [E, N, K] and one fp32 "
+                              "scale a row")
+        if not values.is_cuda:
+            raise NativeError("int8 weight: expected GPU tensors")
+        if 0 in values.shape or values.size(-1) > MAX_K:
+            raise NativeError(f"int8 weight: expected 1 to {MAX_K} columns and no empty dimension")
+        k = values.size(-1)
+        if k % 16 or not values.is_contiguous() or values.data_ptr() % 16:
+            padded = torch.zeros((*values.shape[:-1], _padded(k)), dtype=torch.int8,
+                                 device=values.device)
+            padded[..., :k] = values
+            values = padded[..., :k]
+        self.values = values
+        self.scales = scales.contiguous()
+
+    @staticmethod
+    def quantize(weight: torch.Tensor) -> "Int8Weight":
+        """The 8-bit form of a bf16, fp16 or fp32 weight: every row by ``quantize_rows``."""
+        if weight.dim() not in (2, 3):
+            raise NativeError("int8 weight: expected [N, K] or [E, N, K]")
+        values, scales = quantize_rows(weight.detach().reshape(-1, weight.size(-1)))
+        stride = values.stride(0)
+        n = weight.size(-2)
+        shape, strides = tuple(weight.shape), (stride, 1)
+        if weight.dim() == 3:
+            strides = (n * stride, stride, 1)
+        return Int8Weight._of(values.as_strided(shape, strides), scales.view(shape[:-1]))
+
+    @staticmethod
+    def _of(values: torch.Tensor, scales: torch.Tensor) -> "Int8Weight":
+        weight = Int8Weight.__new__(Int8Weight)
+        weight.values, weight.scales = values, scales
+        return weight
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.values.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.values.device
+
+    @property
+    def row_stride(self) -> int:
+        """Bytes between rows, a multiple of 16."""
+        return _padded(self.shape[-1])
+
+    def size(self, dim: int) -> int:
+        return self.values.size(dim)
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        return (self.values.float() * self.scales[..., None]).to(dtype)
+
+
+def linear_int8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = None,
+                silu_mul: bool = False) -> torch.Tensor:
+    """``x @ weight.T`` in 8-bit integers: ``x`` ``[T, K]`` bf16 or fp16 is quantised a row, the int32
+    sums are exact, ``out`` ``[T, N]`` is rounded once. ``silu_mul``: ``weight`` is a gate_up
+    projection (gate rows, then up rows) and the result is ``silu(gate) * up`` ``[T, N / 2]``,
+    rounded once. Rows may have any stride and alignment. A row with an inf or a NaN comes out NaN."""
+    _check_rows(x, "linear_int8")
+    dt = _ROW_DTYPES.get(x.dtype)
+    if dt not in (0, 1):
+        raise NativeError(f"linear_int8: expected bfloat16 or float16 tensor, got {x.dtype}")
+    if not isinstance(weight, Int8Weight) or weight.values.dim() != 2:
+        raise NativeError("linear_int8: expected an Int8Weight [N, K]")
+    n, k = weight.shape
+    if x.size(1) != k or weight.device != x.device:
+        raise NativeError("linear_int8: expected x [T, K] and a weight [N, K] on one device")
+    if silu_mul and n % 2:
+        raise NativeError("linear_int8: a gate_up weight has an even number of rows")
+    _refuse_grad("linear_int8", x)
+    t, width = x.size(0), n // 2 if silu_mul else n
+    with on_device(x.device):
+        if out is None:
+            out = torch.empty((t, width), dtype=x.dtype, device=x.device)
+        elif (out.shape != (t, width) or out.dtype != x.dtype or out.device != x.device
+              or (width > 1 and out.stride(1) != 1) or (t > 1 and out.stride(0) < width)):
+            raise NativeError("linear_int8: invalid output")
+        need = lib().mi355x_linear_int8_workspace_bytes(t, k)
+        if need < 0:
+            raise NativeError("linear_int8: invalid shape")
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=x.device)
+        check(lib().mi355x_linear_int8(x.data_ptr(), _row_stride(x), weight.values.data_ptr(),
+                                       weight.row_stride, weight.scales.data_ptr(),
+                                       out.data_ptr(), _row_stride(out), t, n, k, silu_mul,
+                                       ws.data_ptr(), need, dt, stream_of(x)), "linear_int8")
+    return out
+
+
+__all__ = ["Int8Weight", "linear_int8", "quantize_rows", "NativeError"]
