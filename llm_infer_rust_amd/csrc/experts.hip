@@ -309,7 +309,10 @@ void launch_product(const ProductArgs& base, int bm, int64_t slots, int64_t expe
     product_tile<IN, OT, MODE, SILU, 64, 64, 2, 2, 4><<<g, 256, 0, s>>>(a);
   } else {
     const dim3 g = grid(SILU ? 128 : 256);
-    product_tile<IN, OT, MODE, SILU, 256, 256, 2, 2, 2><<<g, 256, 0, s>>>(a);
+    if (a.k_bytes % kProdRow)
+      product_large<IN, OT, MODE, SILU, 256, true><<<g, kLargeThreads, 0, s>>>(a);
+    else
+      product_large<IN, OT, MODE, SILU, 256, false><<<g, kLargeThreads, 0, s>>>(a);
   }
 }
 
@@ -359,7 +362,7 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   a.rows = static_cast<int32_t>(slots);
   a.top_k = static_cast<int32_t>(c.top_k);
   a.experts = static_cast<int32_t>(c.experts);
-  a.vec_out = 1;
+  a.vec_out = a.vec16_out = 1;
   // gate_up with SiLU x mul into act, one row a slot
   if (kQuant) {
     auto* xs = reinterpret_cast<float*>(ws + w.xs);

@@ -55,6 +55,7 @@ struct ProductArgs {
   int32_t experts;
   int32_t tiles_m, tiles_n;   // kDense: row tiles; column tiles of every row tile
   int32_t vec_out;            // out rows take aligned stores of four elements
+  int32_t vec16_out;          // out rows take aligned 16-byte stores
 };
 
 // ---------------------------------------------------------------------------- MFMA by type
@@ -150,15 +151,12 @@ __device__ __forceinline__ RowOut row_out(const ProductArgs& a, int row) {
   return r;
 }
 
-// The accumulators of four consecutive columns of a row, scaled and stored. `acc` (SILU: the gate
-// columns, with the matching up columns in `up`); the scales are those of the weight rows.
-template <int IN, int OT, int MODE, bool SILU, typename T>
-__device__ __forceinline__ void finish4(const ProductArgs& a, const RowOut& r, int column,
-                                        const float* w_scales, const T (&acc)[4],
-                                        const T (&up)[4]) {
-  const int n = a.columns - column;
-  if (n <= 0) return;
-  float v[4];
+// The accumulators of four consecutive columns of a row, scaled. `acc` (SILU: the gate columns, with
+// the matching up columns in `up`); the scales are those of the weight rows.
+template <int IN, int MODE, bool SILU, typename T>
+__device__ __forceinline__ void finish_values(const ProductArgs& a, const RowOut& r, int column,
+                                              const float* w_scales, const T (&acc)[4],
+                                              const T (&up)[4], float (&v)[4]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     float g = static_cast<float>(acc[e]);
@@ -171,6 +169,17 @@ __device__ __forceinline__ void finish4(const ProductArgs& a, const RowOut& r, i
     }
     v[e] = MODE == kDown ? g * r.weight : g;
   }
+}
+
+// The same, stored.
+template <int IN, int OT, int MODE, bool SILU, typename T>
+__device__ __forceinline__ void finish4(const ProductArgs& a, const RowOut& r, int column,
+                                        const float* w_scales, const T (&acc)[4],
+                                        const T (&up)[4]) {
+  const int n = a.columns - column;
+  if (n <= 0) return;
+  float v[4];
+  finish_values<IN, MODE, SILU>(a, r, column, w_scales, acc, up, v);
   store4<OT>(a.out, r.at * a.ldo + column, v, n, a.vec_out);
 }
 
@@ -418,6 +427,244 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
         const int wrow = wn * kWaveN + 32 * i + 8 * q + 4 * half;
         finish4<IN, OT, MODE, SILU>(a, r, n0 + (SILU ? silu_column(wrow) : wrow), w_scales, v, u);
       }
+  }
+}
+
+// ---------------------------------------------------------------------------- product_large
+// For many rows: a BM x 256 tile on four waves, one a SIMD, each with a (BM / 2) x 128 block of it, and
+// two LDS stages. Bound by the matrix pipe at the clock that the power limit leaves it, so the
+// schedule is written out: an MFMA, then one of the next quarter step's operand reads or one of
+// the next step's copies (all of them in the first quarters, right after the barrier that freed
+// their buffer), fixed by scheduling barriers. The only wait left in a step is the one for its last
+// copies, three quarters after they were issued.
+constexpr int kLargeN = 256;
+constexpr int kLargeThreads = 256;
+
+template <int BM>
+constexpr int large_stage_bytes() {
+  return (BM + kLargeN) * kProdRow;
+}
+
+// The tile's K loop: acc[i][j] of A block i (32 weight rows) and B block j (32 rows of x). TAIL: K ends
+// inside a step. Compiled apart, as the question at every copy costs 8% of the loop.
+template <int IN, int MODE, bool SILU, int BM, bool TAIL>
+__device__ __forceinline__ void large_loop(const ProductArgs& a, const RowTile& t, int n0,
+                                           uint8_t* lds,
+                                           typename Mma<IN>::Acc16 (&acc)[4][BM / 64]) {
+  constexpr int NW = 4, A_BLK = 4, B_BLK = BM / 64;
+  constexpr int kCopies = (BM + kLargeN) / 8 / NW, kCopiesX = BM / 8 / NW;
+  constexpr int kStage = large_stage_bytes<BM>();
+  using M = Mma<IN>;
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  const int n_k = (a.k_bytes + kProdRow - 1) / kProdRow;
+
+  const uint32_t lds_base = lds_address(lds) + wave * 1024;
+  const uint8_t* x_base = a.x;
+  if constexpr (MODE != kGateUp) x_base += t.begin * a.x_stride;
+  const uint8_t* w_base = a.w + t.expert * a.w_expert;
+  if constexpr (!SILU) w_base += static_cast<int64_t>(n0) * a.w_stride;
+  uint32_t off[kCopies];
+#pragma unroll
+  for (int j = 0; j < kCopies; ++j) {
+    int r = 8 * (wave + NW * j) + (lane >> 3);
+    uint32_t row, stride;
+    if (j < kCopiesX) {
+      const int m = min(t.begin + r, t.end - 1);
+      row = MODE == kGateUp ? source_row(a, m, true) : m - t.begin;
+      stride = static_cast<uint32_t>(a.x_stride);
+    } else {
+      r -= BM;
+      if constexpr (SILU) {
+        const int c = min(n0 + silu_column(r), a.columns - 1);
+        row = ((r >> 3) & 1) ? a.columns + c : c;
+      } else {
+        row = min(r, a.columns - 1 - n0);
+      }
+      stride = static_cast<uint32_t>(a.w_stride);
+    }
+    off[j] = row * stride + prod_chunk(lane & 7, r) * 16;
+  }
+  auto copy = [&](int step, int stage, int j) {
+    const int64_t k = static_cast<int64_t>(step) * kProdRow;
+    const uint8_t* base = (j < kCopiesX ? x_base : w_base) + k;
+    const uint32_t dst = lds_base + stage * kStage + j * NW * 1024;
+    if (TAIL && step == n_k - 1) {  // chunks past K come as zeros in both operands
+      int r = 8 * (wave + NW * j) + (lane >> 3);
+      if (j >= kCopiesX) r -= BM;
+      const uint8_t* src = base + off[j];
+      if (k + prod_chunk(lane & 7, r) * 16 >= a.k_bytes)
+        src = reinterpret_cast<const uint8_t*>(kProductZeros);
+      copy_to_lds(src, dst);
+    } else {
+      copy_offset_to_lds(base, off[j], dst);
+    }
+  };
+
+  const int wm = wave & 1, wn = wave >> 1;
+  const int col = lane & 31, half = lane >> 5;
+  const int xr = wm * (BM / 2) + col, wr = wn * 128 + col;
+  uint32_t x_at[4], w_at[4];
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) {
+    x_at[kk] = xr * kProdRow + prod_chunk(2 * kk + half, xr) * 16;
+    w_at[kk] = (BM + wr) * kProdRow + prod_chunk(2 * kk + half, wr) * 16;
+  }
+#pragma unroll
+  for (int i = 0; i < A_BLK; ++i)
+#pragma unroll
+    for (int j = 0; j < B_BLK; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+
+  uint4 af[2][A_BLK], bf[2][B_BLK];
+  constexpr int kReads = A_BLK + B_BLK, kMfma = A_BLK * B_BLK;
+  // in the order in which the MFMAs want them: A block 0, the B blocks, the other A blocks
+  auto read = [&](int stage, int kk, int to, int f) {
+    const uint8_t* sb = lds + stage * kStage;
+    if (f >= 1 && f <= B_BLK) {
+      bf[to][f - 1] = *reinterpret_cast<const uint4*>(sb + x_at[kk] + (f - 1) * 32 * kProdRow);
+    } else {
+      const int i = f == 0 ? 0 : f - B_BLK;
+      af[to][i] = *reinterpret_cast<const uint4*>(sb + w_at[kk] + i * 32 * kProdRow);
+    }
+  };
+  auto barrier = [&] {  // every wave's copies are in and its reads are done
+    wait_vmcnt<0>();
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+
+#pragma unroll
+  for (int j = 0; j < kCopies; ++j) copy(0, 0, j);
+  barrier();
+#pragma unroll
+  for (int f = 0; f < kReads; ++f) read(0, 0, 0, f);
+  for (int step = 0; step < n_k; ++step) {
+    const int stage = step & 1;
+    const bool more = step + 1 < n_k;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      if (kk == 3 && more) barrier();
+#pragma unroll
+      for (int m = 0; m < kMfma; ++m) {
+        const int i = m / B_BLK, j = m % B_BLK;
+        acc[i][j] = M::block32(af[kk & 1][i], bf[kk & 1][j], acc[i][j]);
+        if (m < kReads) {
+          if (kk < 3)
+            read(stage, kk + 1, (kk + 1) & 1, m);
+          else if (more)
+            read(stage ^ 1, 0, 0, m);
+        }
+        if (more && kk * kMfma + m < kCopies) copy(step + 1, stage ^ 1, kk * kMfma + m);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+}
+
+// The epilogue: every wave turns 32 rows of its block at a time through LDS (the stages are free by
+// then), so that rows go out in 16-byte stores of whole 128- or 256-byte pieces instead of 8 bytes
+// a row and store.
+template <int IN, int OT, int MODE, bool SILU, int BM>
+__device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile& t, int n0,
+                                            uint8_t* lds,
+                                            typename Mma<IN>::Acc16 (&acc)[4][BM / 64]) {
+  constexpr int B_BLK = BM / 64;
+  constexpr int kOutSize = OT == kFloatOut ? 4 : 2;
+  constexpr int kCols = SILU ? 64 : 128;                 // columns of a wave
+  constexpr int kPitch = kCols * kOutSize + 16;          // bytes of a row in LDS
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int wm = wave & 1, wn = wave >> 1;
+  const int col = lane & 31, half = lane >> 5;
+  const float* w_scales = nullptr;
+  if constexpr (IN == kInt8)
+    w_scales = a.w_scales + static_cast<int64_t>(t.expert) * (SILU ? 2 : 1) * a.columns;
+  const int first = n0 + wn * kCols;  // first column of the wave
+  uint8_t* turn = lds + wave * 32 * kPitch;
+  __syncthreads();  // every wave is done with the stages
+#pragma unroll
+  for (int j = 0; j < B_BLK; ++j) {
+    const int begin = t.begin + wm * (BM / 2) + 32 * j;
+    if (begin >= t.end) break;
+    const int row = min(begin + col, t.end - 1);
+    const RowOut r = row_out<IN, MODE>(a, row);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; q += SILU ? 2 : 1) {
+        const int at = SILU ? silu_column(32 * i + 8 * q + 4 * half) : 32 * i + 8 * q + 4 * half;
+        typename Mma<IN>::Scalar v[4], u[4] = {};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = acc[i][j][4 * q + e];
+          if constexpr (SILU) u[e] = acc[i][j][4 * q + 4 + e];
+        }
+        float f[4];
+        finish_values<IN, MODE, SILU>(a, r, first + at, w_scales, v, u, f);
+        uint8_t* p = turn + col * kPitch + at * kOutSize;
+        if constexpr (OT == kFloatOut)
+          *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+        else
+          *reinterpret_cast<uint2*>(p) =
+              make_uint2(Elem<OT>::pack2(f[0], f[1]), Elem<OT>::pack2(f[2], f[3]));
+      }
+    // A wave's LDS operations keep their order, so its reads follow its writes of all lanes; the
+    // clobbers keep the compiler from exchanging them.
+    asm volatile("" ::: "memory");
+    constexpr int kChunks = kCols * kOutSize / 16;  // 16-byte pieces of a row
+    constexpr int kPer = 16 / kOutSize;             // elements of a piece
+#pragma unroll
+    for (int s = 0; s < 32 * kChunks / kWave; ++s) {
+      const int p = s * kWave + lane;
+      const int lr = p / kChunks, c = p % kChunks;
+      const uint4 v = *reinterpret_cast<const uint4*>(turn + lr * kPitch + c * 16);
+      const int out_row = begin + lr, column = first + c * kPer;
+      if (out_row >= t.end || column >= a.columns) continue;
+      int64_t at = out_row;
+      if constexpr (MODE == kDown) at = a.order ? a.order[out_row] : out_row;
+      uint8_t* o = static_cast<uint8_t*>(a.out) + (at * a.ldo + column) * kOutSize;
+      if (a.vec16_out && column + kPer <= a.columns) {
+        st128(o, v);
+      } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          if (column + e >= a.columns) continue;
+          if constexpr (OT == kFloatOut)
+            reinterpret_cast<uint32_t*>(o)[e] = w[e];
+          else
+            reinterpret_cast<uint16_t*>(o)[e] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+        }
+      }
+    }
+    asm volatile("" ::: "memory");
+  }
+}
+
+// A tile of up to BM rows. Of the row tiles that a group ends with, those of up to BM / 2 rows run
+// as half tiles: a ragged group of rows then wastes a quarter of a tile on average, not half.
+template <int IN, int OT, int MODE, bool SILU, int BM, bool TAIL>
+__global__ __launch_bounds__(kLargeThreads, 1) void product_large(ProductArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * large_stage_bytes<BM>()];
+  if (a.columns < 0) lds[threadIdx.x] = 0;  // never taken; the copies' LDS writes are invisible
+  int tm, tn;
+  if (!tile_of_block<MODE>(a, &tm, &tn)) return;
+  RowTile t;
+  if (!row_tile<MODE, BM>(a, tm, &t)) return;
+  const int n0 = tn * (SILU ? kLargeN / 2 : kLargeN);
+  if (t.end - t.begin > BM / 2) {
+    typename Mma<IN>::Acc16 acc[4][BM / 64];
+    large_loop<IN, MODE, SILU, BM, TAIL>(a, t, n0, lds, acc);
+    large_store<IN, OT, MODE, SILU, BM>(a, t, n0, lds, acc);
+  } else {
+    typename Mma<IN>::Acc16 acc[4][BM / 128];
+    large_loop<IN, MODE, SILU, BM / 2, TAIL>(a, t, n0, lds, acc);
+    large_store<IN, OT, MODE, SILU, BM / 2>(a, t, n0, lds, acc);
   }
 }
 

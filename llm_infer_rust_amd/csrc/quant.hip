@@ -183,7 +183,10 @@ void launch_int8(const ProductArgs& base, int64_t M, int64_t columns, hipStream_
     product_tile<kInt8, OT, kDense, SILU, 64, 64, 2, 2, 4><<<g, 256, 0, s>>>(a);
   } else {
     const dim3 g = grid(256, SILU ? 128 : 256);
-    product_tile<kInt8, OT, kDense, SILU, 256, 256, 2, 2, 2><<<g, 256, 0, s>>>(a);
+    if (a.k_bytes % kProdRow)
+      product_large<kInt8, OT, kDense, SILU, 256, true><<<g, kLargeThreads, 0, s>>>(a);
+    else
+      product_large<kInt8, OT, kDense, SILU, 256, false><<<g, kLargeThreads, 0, s>>>(a);
   }
 }
 
@@ -269,6 +272,7 @@ extern "C" const char* mi355x_linear_int8(const void* x, int64_t ldx, const void
   a.columns = static_cast<int32_t>(columns);
   a.k_bytes = static_cast<int32_t>(padded16(K));
   a.vec_out = ldo % 4 == 0 && aligned(out, 8);
+  a.vec16_out = ldo % 8 == 0 && aligned(out, 16);
   if (dtype == 0)
     silu_mul ? launch_int8<0, true>(a, M, columns, s) : launch_int8<0, false>(a, M, columns, s);
   else
