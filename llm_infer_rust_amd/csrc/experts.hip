@@ -157,14 +157,16 @@ __device__ __forceinline__ int block_exclusive(int v, int* wave_totals) {
   return before + s - v;
 }
 
-// order[row]: the slots in the order of their experts. `counts` may be null with one chunk. The
+// order[row]: the slots in the order of their experts; row_weights[row]: their weights. `counts` may be null with one chunk. The
 // first workgroup writes the list of row tiles of bm rows. The order of the slots within an
 // expert is that of the LDS atomics; a row's products do not depend on the row it stands in.
 __global__ __launch_bounds__(kGroupThreads) void place_slots(const int32_t* __restrict__ ids,
                                                              int slots, int experts, int bm,
                                                              const int32_t* __restrict__ counts,
                                                              int chunks,
+                                                             const float* __restrict__ weights,
                                                              int32_t* __restrict__ order,
+                                                             float* __restrict__ row_weights,
                                                              int4* __restrict__ tiles,
                                                              int32_t* __restrict__ tile_count) {
   __shared__ int cursor[kMaxExperts];
@@ -201,7 +203,11 @@ __global__ __launch_bounds__(kGroupThreads) void place_slots(const int32_t* __re
   __syncthreads();
   for (int i = begin + threadIdx.x; i < end; i += kGroupThreads) {
     const int x = ids[i];
-    if (takes_part(x, experts)) order[atomicAdd(&cursor[x], 1)] = i;
+    if (takes_part(x, experts)) {
+      const int row = atomicAdd(&cursor[x], 1);
+      order[row] = i;
+      row_weights[row] = weights[i];
+    }
   }
 }
 
@@ -256,7 +262,7 @@ Grouping choose_grouping(int64_t slots, int64_t experts) {
 constexpr int64_t kMaxSlots = 131072;  // slots a pass takes; more tokens run in several passes
 
 struct ExpertWorkspace {
-  int64_t order, tiles, tile_count, counts, xq, xs, act, actq, acts, y, bytes;
+  int64_t order, row_weights, tiles, tile_count, counts, xq, xs, act, actq, acts, y, bytes;
   int64_t tokens;  // a pass
 };
 
@@ -276,6 +282,7 @@ ExpertWorkspace expert_workspace(int64_t tokens, int64_t top_k, int64_t experts,
     return o;
   };
   w.order = take(slots * 4);
+  w.row_weights = take(slots * 4);
   w.tiles = take((std::min(experts, slots) + slots / 16 + 1) * 16);
   w.tile_count = take(4);
   w.counts = take(pad(slots, kGroupChunk) / kGroupChunk * experts * 4);
@@ -310,9 +317,9 @@ void launch_product(const ProductArgs& base, int bm, int64_t slots, int64_t expe
   } else {
     const dim3 g = grid(SILU ? 128 : 256);
     if (a.k_bytes % kProdRow)
-      product_large<IN, OT, MODE, SILU, 256, true><<<g, kLargeThreads, 0, s>>>(a);
+      product_large<IN, OT, MODE, SILU, 256, 8, true><<<g, 512, 0, s>>>(a);
     else
-      product_large<IN, OT, MODE, SILU, 256, false><<<g, kLargeThreads, 0, s>>>(a);
+      product_large<IN, OT, MODE, SILU, 256, 8, false><<<g, 512, 0, s>>>(a);
   }
 }
 
@@ -338,6 +345,7 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   const int64_t slots = c.tokens * c.top_k;
   const Grouping g = choose_grouping(slots, c.experts);
   auto* order = reinterpret_cast<int32_t*>(ws + w.order);
+  auto* row_weights = reinterpret_cast<float*>(ws + w.row_weights);
   auto* tiles = reinterpret_cast<int4*>(ws + w.tiles);
   auto* tile_count = reinterpret_cast<int32_t*>(ws + w.tile_count);
   auto* counts = reinterpret_cast<int32_t*>(ws + w.counts);
@@ -350,7 +358,7 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
     }
     place_slots<<<dim3(chunks), kGroupThreads, 0, s>>>(
         c.ids, static_cast<int>(slots), static_cast<int>(c.experts), g.bm,
-        chunks > 1 ? counts : nullptr, chunks, order, tiles, tile_count);
+        chunks > 1 ? counts : nullptr, chunks, c.weights, order, row_weights, tiles, tile_count);
     if (const char* e = launch_status("place_slots")) return e;
   }
   ProductArgs a{};
@@ -358,7 +366,7 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   a.tiles = g.bm ? tiles : nullptr;
   a.tile_count = tile_count;
   a.ids = c.ids;
-  a.slot_weights = c.weights;
+  a.row_weights = g.bm ? row_weights : c.weights;
   a.rows = static_cast<int32_t>(slots);
   a.top_k = static_cast<int32_t>(c.top_k);
   a.experts = static_cast<int32_t>(c.experts);

@@ -8,13 +8,15 @@
 //   bf16 / fp16  32x32x16 and 16x16x32, fp32 accumulators
 //   int8         32x32x32 and 16x16x64, int32 accumulators (exact up to K = 131,072)
 //
-// Two kernels:
+// Three kernels:
 //   * product_tile: a BM x BN tile, x and w rows copied to an LDS ring of 128-byte rows
-//     (global_load_lds_dwordx4, 16-byte chunks XOR-swizzled), waves of 32 x 32 MFMA blocks;
+//     (global_load_lds_dwordx4, 16-byte chunks XOR-swizzled);
+//   * product_large: the same for many rows, 256 x 256 on a written-out schedule;
 //   * product_rows: up to 16 rows of x, weights from global memory straight into MFMA operands, the
 //     waves of a workgroup sharing K. For few rows, where the weight bytes are all that counts.
 #pragma once
 
+#include <algorithm>
 #include <cstdint>
 #include <type_traits>
 
@@ -43,7 +45,7 @@ struct ProductArgs {
   const int32_t* ids;         // with a null tile list: expert of every slot
   const int4* tiles;          // grouped: {expert, first row, end row, 0} per row tile
   const int32_t* tile_count;  // grouped: tiles in the list
-  const float* slot_weights;  // kDown: one a slot
+  const float* row_weights;   // kDown: weight of every row of the grouped order
   int64_t x_stride;           // bytes a row
   int64_t w_stride;           // bytes a row
   int64_t w_expert;           // bytes an expert
@@ -98,9 +100,10 @@ struct Mma {
   }
 };
 
-// silu(g) * u. exp(-g) overflows to +inf for g below about -88: g / inf = -0, the limit.
+// silu(g) * u, with the hardware reciprocal (1 ulp; an IEEE quotient doubles the epilogue of a large
+// gate_up tile). exp(-g) overflows to +inf for g below about -88: g * 0 = -0, the limit.
 __device__ __forceinline__ float silu_mul(float g, float u) {
-  return (g / (1.f + __expf(-g))) * u;
+  return g * __builtin_amdgcn_rcpf(1.f + __expf(-g)) * u;
 }
 
 // Four consecutive output elements of a row, of which the first `n` exist.
@@ -145,7 +148,7 @@ __device__ __forceinline__ RowOut row_out(const ProductArgs& a, int row) {
     } else {
       if constexpr (IN == kInt8) r.scale = a.x_scales[row];
       r.at = slot;
-      r.weight = a.slot_weights[slot];
+      r.weight = a.row_weights[row];
     }
   }
   return r;
@@ -431,27 +434,35 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
 }
 
 // ---------------------------------------------------------------------------- product_large
-// For many rows: a BM x 256 tile on four waves, one a SIMD, each with a (BM / 2) x 128 block of it, and
-// two LDS stages. Bound by the matrix pipe at the clock that the power limit leaves it, so the
-// schedule is written out: an MFMA, then one of the next quarter step's operand reads or one of
-// the next step's copies (all of them in the first quarters, right after the barrier that freed
-// their buffer), fixed by scheduling barriers. The only wait left in a step is the one for its last
-// copies, three quarters after they were issued.
+// For many rows: a BM x 256 tile on NW = 8 waves, two a SIMD, each with a (BM / 2) x 64 block of it, and as
+// many 128-byte steps in flight as LDS holds. The schedule is written out: an MFMA, then one of the
+// next quarter step's operand reads or one of the copies into the buffer that the last barrier
+// freed, fixed by scheduling barriers.
+// Measured on the experts of an 8,192-token prefill (65,536 rows in 128 groups): the copies
+// alone take 335 us of gate_up's 440 (11 TB/s into LDS, 44% of it from beyond L2), the MFMAs with
+// operands in L1 320; down 247 and 184 of 275. Four waves of 128 x 128 read LDS a third less but leave
+// each SIMD idle at every wait (480 and 316 us); 64-byte steps with 128 KiB in flight instead of 64 are
+// no quicker (480 and 305), so it is not latency.
 constexpr int kLargeN = 256;
-constexpr int kLargeThreads = 256;
 
+template <int BM>
+constexpr int large_stages() {
+  return BM == 256 ? 2 : 3;
+}
 template <int BM>
 constexpr int large_stage_bytes() {
   return (BM + kLargeN) * kProdRow;
 }
+constexpr int kLargeEdges = 3 * large_stage_bytes<128>();  // LDS behind the stages: the edges
+static_assert(kLargeEdges >= 2 * large_stage_bytes<256>(), "the edges follow the stages");
 
 // The tile's K loop: acc[i][j] of A block i (32 weight rows) and B block j (32 rows of x). TAIL: K ends
 // inside a step. Compiled apart, as the question at every copy costs 8% of the loop.
-template <int IN, int MODE, bool SILU, int BM, bool TAIL>
+template <int IN, int MODE, bool SILU, int BM, int NW, bool TAIL>
 __device__ __forceinline__ void large_loop(const ProductArgs& a, const RowTile& t, int n0,
                                            uint8_t* lds,
-                                           typename Mma<IN>::Acc16 (&acc)[4][BM / 64]) {
-  constexpr int NW = 4, A_BLK = 4, B_BLK = BM / 64;
+                                           typename Mma<IN>::Acc16 (&acc)[16 / NW][BM / 64]) {
+  constexpr int A_BLK = 16 / NW, B_BLK = BM / 64, S = large_stages<BM>();
   constexpr int kCopies = (BM + kLargeN) / 8 / NW, kCopiesX = BM / 8 / NW;
   constexpr int kStage = large_stage_bytes<BM>();
   using M = Mma<IN>;
@@ -460,6 +471,7 @@ __device__ __forceinline__ void large_loop(const ProductArgs& a, const RowTile& 
   const int lane = tid & 63;
   const int n_k = (a.k_bytes + kProdRow - 1) / kProdRow;
 
+  // Copy j of a wave covers tile rows 8 g .. 8 g + 7, g = wave + NW j, x rows first.
   const uint32_t lds_base = lds_address(lds) + wave * 1024;
   const uint8_t* x_base = a.x;
   if constexpr (MODE != kGateUp) x_base += t.begin * a.x_stride;
@@ -486,10 +498,10 @@ __device__ __forceinline__ void large_loop(const ProductArgs& a, const RowTile& 
     }
     off[j] = row * stride + prod_chunk(lane & 7, r) * 16;
   }
-  auto copy = [&](int step, int stage, int j) {
+  auto copy = [&](int step, uint32_t buffer, int j) {
     const int64_t k = static_cast<int64_t>(step) * kProdRow;
     const uint8_t* base = (j < kCopiesX ? x_base : w_base) + k;
-    const uint32_t dst = lds_base + stage * kStage + j * NW * 1024;
+    const uint32_t dst = buffer + j * NW * 1024;
     if (TAIL && step == n_k - 1) {  // chunks past K come as zeros in both operands
       int r = 8 * (wave + NW * j) + (lane >> 3);
       if (j >= kCopiesX) r -= BM;
@@ -504,7 +516,7 @@ __device__ __forceinline__ void large_loop(const ProductArgs& a, const RowTile& 
 
   const int wm = wave & 1, wn = wave >> 1;
   const int col = lane & 31, half = lane >> 5;
-  const int xr = wm * (BM / 2) + col, wr = wn * 128 + col;
+  const int xr = wm * (BM / 2) + col, wr = wn * (32 * A_BLK) + col;
   uint32_t x_at[4], w_at[4];
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) {
@@ -520,9 +532,10 @@ __device__ __forceinline__ void large_loop(const ProductArgs& a, const RowTile& 
 
   uint4 af[2][A_BLK], bf[2][B_BLK];
   constexpr int kReads = A_BLK + B_BLK, kMfma = A_BLK * B_BLK;
+  constexpr int kSlots = std::max({kMfma, kReads, kCopies});
   // in the order in which the MFMAs want them: A block 0, the B blocks, the other A blocks
-  auto read = [&](int stage, int kk, int to, int f) {
-    const uint8_t* sb = lds + stage * kStage;
+  auto read = [&](const uint8_t* sb, int kk, int f) {
+    const int to = kk & 1;
     if (f >= 1 && f <= B_BLK) {
       bf[to][f - 1] = *reinterpret_cast<const uint4*>(sb + x_at[kk] + (f - 1) * 32 * kProdRow);
     } else {
@@ -530,8 +543,7 @@ __device__ __forceinline__ void large_loop(const ProductArgs& a, const RowTile& 
       af[to][i] = *reinterpret_cast<const uint4*>(sb + w_at[kk] + i * 32 * kProdRow);
     }
   };
-  auto barrier = [&] {  // every wave's copies are in and its reads are done
-    wait_vmcnt<0>();
+  auto barrier = [&] {  // this wave's reads are done (its copies were waited for); then all waves'
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -539,73 +551,97 @@ __device__ __forceinline__ void large_loop(const ProductArgs& a, const RowTile& 
   };
 
 #pragma unroll
-  for (int j = 0; j < kCopies; ++j) copy(0, 0, j);
+  for (int s = 0; s < S; ++s)
+    if (s < n_k)
+#pragma unroll
+      for (int j = 0; j < kCopies; ++j) copy(s, lds_base + s * kStage, j);
+  wait_tiles_ahead<kCopies, S - 1>(min(S - 1, n_k - 1));
   barrier();
 #pragma unroll
-  for (int f = 0; f < kReads; ++f) read(0, 0, 0, f);
+  for (int f = 0; f < kReads; ++f) read(lds, 0, f);
+  int stage = 0;
   for (int step = 0; step < n_k; ++step) {
-    const int stage = step & 1;
-    const bool more = step + 1 < n_k;
+    const uint8_t* now = lds + stage * kStage;
+    const uint32_t freed = lds_base + stage * kStage;
+    stage = stage == S - 1 ? 0 : stage + 1;
+    const uint8_t* next = lds + stage * kStage;
+    const bool more = step + 1 < n_k, fill = step + S < n_k;
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      if (kk == 3 && more) barrier();
+      if (kk == 3 && more) {  // the next step is in and this one is read: its buffer is free
+        wait_tiles_ahead<kCopies, S - 2>(min(S - 2, n_k - 2 - step));
+        barrier();
+      }
 #pragma unroll
-      for (int m = 0; m < kMfma; ++m) {
+      for (int m = 0; m < kSlots; ++m) {
         const int i = m / B_BLK, j = m % B_BLK;
-        acc[i][j] = M::block32(af[kk & 1][i], bf[kk & 1][j], acc[i][j]);
+        if (m < kMfma) acc[i][j] = M::block32(af[kk & 1][i], bf[kk & 1][j], acc[i][j]);
         if (m < kReads) {
           if (kk < 3)
-            read(stage, kk + 1, (kk + 1) & 1, m);
+            read(now, kk + 1, m);
           else if (more)
-            read(stage ^ 1, 0, 0, m);
+            read(next, 0, m);
         }
-        if (more && kk * kMfma + m < kCopies) copy(step + 1, stage ^ 1, kk * kMfma + m);
+        if (kk == 3 && fill && m < kCopies) copy(step + S, freed, m);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
 }
 
-// The epilogue: every wave turns 32 rows of its block at a time through LDS (the stages are free by
-// then), so that rows go out in 16-byte stores of whole 128- or 256-byte pieces instead of 8 bytes
-// a row and store.
-template <int IN, int OT, int MODE, bool SILU, int BM>
+// What the epilogue needs of the tile's rows and columns, in LDS once the stages are free.
+struct LargeEdges {
+  int32_t out_row[256];
+  float row_scale[256];     // int8: of the x row; kDown: times the slot's weight
+  float column_scale[256];  // int8: of the tile's weight rows (SILU: 128 gate, then 128 up)
+};
+
+// The epilogue: every wave turns 32 rows of its block at a time through LDS, so that rows go out in
+// 16-byte stores of whole 64- to 256-byte pieces instead of 8 bytes a row and store.
+template <int IN, int OT, int MODE, bool SILU, int BM, int NW>
 __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile& t, int n0,
-                                            uint8_t* lds,
-                                            typename Mma<IN>::Acc16 (&acc)[4][BM / 64]) {
-  constexpr int B_BLK = BM / 64;
+                                            uint8_t* lds, const LargeEdges& edges,
+                                            typename Mma<IN>::Acc16 (&acc)[16 / NW][BM / 64]) {
+  constexpr int A_BLK = 16 / NW, B_BLK = BM / 64;
   constexpr int kOutSize = OT == kFloatOut ? 4 : 2;
-  constexpr int kCols = SILU ? 64 : 128;                 // columns of a wave
+  constexpr int kCols = (SILU ? 16 : 32) * A_BLK;        // columns of a wave
   constexpr int kPitch = kCols * kOutSize + 16;          // bytes of a row in LDS
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int wm = wave & 1, wn = wave >> 1;
   const int col = lane & 31, half = lane >> 5;
-  const float* w_scales = nullptr;
-  if constexpr (IN == kInt8)
-    w_scales = a.w_scales + static_cast<int64_t>(t.expert) * (SILU ? 2 : 1) * a.columns;
-  const int first = n0 + wn * kCols;  // first column of the wave
   uint8_t* turn = lds + wave * 32 * kPitch;
-  __syncthreads();  // every wave is done with the stages
 #pragma unroll
   for (int j = 0; j < B_BLK; ++j) {
-    const int begin = t.begin + wm * (BM / 2) + 32 * j;
-    if (begin >= t.end) break;
-    const int row = min(begin + col, t.end - 1);
-    const RowOut r = row_out<IN, MODE>(a, row);
+    const int begin = wm * (BM / 2) + 32 * j;  // row of the tile
+    if (t.begin + begin >= t.end) break;
+    const float row_scale = edges.row_scale[begin + col];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < A_BLK; ++i)
 #pragma unroll
       for (int q = 0; q < 4; q += SILU ? 2 : 1) {
-        const int at = SILU ? silu_column(32 * i + 8 * q + 4 * half) : 32 * i + 8 * q + 4 * half;
-        typename Mma<IN>::Scalar v[4], u[4] = {};
+        const int wrow = 32 * i + 8 * q + 4 * half;
+        const int at = SILU ? silu_column(wrow) : wrow;  // column of the wave
+        float f[4], gs[4] = {1.f, 1.f, 1.f, 1.f}, us[4] = {1.f, 1.f, 1.f, 1.f};
+        if constexpr (IN == kInt8) {
+          *reinterpret_cast<float4*>(gs) =
+              *reinterpret_cast<const float4*>(edges.column_scale + wn * kCols + at);
+          if constexpr (SILU)
+            *reinterpret_cast<float4*>(us) =
+                *reinterpret_cast<const float4*>(edges.column_scale + 128 + wn * kCols + at);
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v[e] = acc[i][j][4 * q + e];
-          if constexpr (SILU) u[e] = acc[i][j][4 * q + 4 + e];
+          float g = static_cast<float>(acc[i][j][4 * q + e]);
+          if constexpr (IN == kInt8 || MODE == kDown) g *= row_scale;
+          if constexpr (IN == kInt8) g *= gs[e];
+          if constexpr (SILU) {
+            float u = static_cast<float>(acc[i][j][(4 * q + 4 + e) & 15]);
+            if constexpr (IN == kInt8) u = u * row_scale * us[e];
+            g = silu_mul(g, u);
+          }
+          f[e] = g;
         }
-        float f[4];
-        finish_values<IN, MODE, SILU>(a, r, first + at, w_scales, v, u, f);
         uint8_t* p = turn + col * kPitch + at * kOutSize;
         if constexpr (OT == kFloatOut)
           *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
@@ -623,11 +659,10 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
       const int p = s * kWave + lane;
       const int lr = p / kChunks, c = p % kChunks;
       const uint4 v = *reinterpret_cast<const uint4*>(turn + lr * kPitch + c * 16);
-      const int out_row = begin + lr, column = first + c * kPer;
-      if (out_row >= t.end || column >= a.columns) continue;
-      int64_t at = out_row;
-      if constexpr (MODE == kDown) at = a.order ? a.order[out_row] : out_row;
-      uint8_t* o = static_cast<uint8_t*>(a.out) + (at * a.ldo + column) * kOutSize;
+      const int64_t out_row = edges.out_row[begin + lr];
+      const int column = n0 + wn * kCols + c * kPer;
+      if (t.begin + begin + lr >= t.end || column >= a.columns) continue;
+      uint8_t* o = static_cast<uint8_t*>(a.out) + (out_row * a.ldo + column) * kOutSize;
       if (a.vec16_out && column + kPer <= a.columns) {
         st128(o, v);
       } else {
@@ -646,26 +681,51 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
   }
 }
 
+template <int IN, int OT, int MODE, bool SILU, int BM, int NW, bool TAIL>
+__device__ __forceinline__ void large_tile(const ProductArgs& a, const RowTile& t, int n0,
+                                           uint8_t* lds) {
+  // Loaded now and needed after the loop: the row and column that this thread stands for.
+  const int r = threadIdx.x & 255;
+  const int row = min(t.begin + r, t.end - 1);
+  int slot = row;
+  float row_scale = 1.f, weight = 1.f, column_scale = 1.f;
+  if constexpr (MODE != kDense) slot = a.order ? a.order[row] : row;
+  if constexpr (MODE == kDown) weight = a.row_weights[row];
+  if constexpr (IN == kInt8 && MODE != kGateUp) row_scale = a.x_scales[row];
+  if constexpr (IN == kInt8) {
+    const float* scales = a.w_scales + static_cast<int64_t>(t.expert) * (SILU ? 2 : 1) * a.columns;
+    const int c = min(n0 + (SILU ? r & 127 : r), a.columns - 1);
+    column_scale = scales[SILU && r >= 128 ? a.columns + c : c];
+  }
+  typename Mma<IN>::Acc16 acc[16 / NW][BM / 64];
+  large_loop<IN, MODE, SILU, BM, NW, TAIL>(a, t, n0, lds, acc);
+  auto& edges = *reinterpret_cast<LargeEdges*>(lds + kLargeEdges);
+  if constexpr (IN == kInt8 && MODE == kGateUp) row_scale = a.x_scales[slot / a.top_k];
+  if (threadIdx.x < 256) {
+    edges.out_row[r] = MODE == kDown ? slot : row;
+    edges.row_scale[r] = row_scale * weight;
+    edges.column_scale[r] = column_scale;
+  }
+  __syncthreads();  // the edges are written and every wave is done with the stages
+  large_store<IN, OT, MODE, SILU, BM, NW>(a, t, n0, lds, edges, acc);
+}
+
 // A tile of up to BM rows. Of the row tiles that a group ends with, those of up to BM / 2 rows run
 // as half tiles: a ragged group of rows then wastes a quarter of a tile on average, not half.
-template <int IN, int OT, int MODE, bool SILU, int BM, bool TAIL>
-__global__ __launch_bounds__(kLargeThreads, 1) void product_large(ProductArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * large_stage_bytes<BM>()];
+template <int IN, int OT, int MODE, bool SILU, int BM, int NW, bool TAIL>
+__global__ __launch_bounds__(64 * NW, 1) void product_large(ProductArgs a) {
+  static_assert(BM == 256, "the edges are those of 256 rows");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kLargeEdges + sizeof(LargeEdges)];
   if (a.columns < 0) lds[threadIdx.x] = 0;  // never taken; the copies' LDS writes are invisible
   int tm, tn;
   if (!tile_of_block<MODE>(a, &tm, &tn)) return;
   RowTile t;
   if (!row_tile<MODE, BM>(a, tm, &t)) return;
   const int n0 = tn * (SILU ? kLargeN / 2 : kLargeN);
-  if (t.end - t.begin > BM / 2) {
-    typename Mma<IN>::Acc16 acc[4][BM / 64];
-    large_loop<IN, MODE, SILU, BM, TAIL>(a, t, n0, lds, acc);
-    large_store<IN, OT, MODE, SILU, BM>(a, t, n0, lds, acc);
-  } else {
-    typename Mma<IN>::Acc16 acc[4][BM / 128];
-    large_loop<IN, MODE, SILU, BM / 2, TAIL>(a, t, n0, lds, acc);
-    large_store<IN, OT, MODE, SILU, BM / 2>(a, t, n0, lds, acc);
-  }
+  if (t.end - t.begin > BM / 2)
+    large_tile<IN, OT, MODE, SILU, BM, NW, TAIL>(a, t, n0, lds);
+  else
+    large_tile<IN, OT, MODE, SILU, BM / 2, NW, TAIL>(a, t, n0, lds);
 }
 
 // ---------------------------------------------------------------------------- product_rows

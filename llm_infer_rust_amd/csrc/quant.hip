@@ -184,9 +184,9 @@ void launch_int8(const ProductArgs& base, int64_t M, int64_t columns, hipStream_
   } else {
     const dim3 g = grid(256, SILU ? 128 : 256);
     if (a.k_bytes % kProdRow)
-      product_large<kInt8, OT, kDense, SILU, 256, true><<<g, kLargeThreads, 0, s>>>(a);
+      product_large<kInt8, OT, kDense, SILU, 256, 8, true><<<g, 512, 0, s>>>(a);
     else
-      product_large<kInt8, OT, kDense, SILU, 256, false><<<g, kLargeThreads, 0, s>>>(a);
+      product_large<kInt8, OT, kDense, SILU, 256, 8, false><<<g, 512, 0, s>>>(a);
   }
 }
 
