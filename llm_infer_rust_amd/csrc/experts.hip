@@ -11,7 +11,7 @@
 // src/models/qwen3/model.rs:478-534; the reference itself has dense layers only.
 #include <algorithm>
 
-#include "quant.h"
+#include "product_vec.h"
 
 namespace mi355x {
 namespace {
@@ -38,6 +38,23 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
+template <int Ctrl>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
+  return max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), Ctrl, 0xf,
+                                                                  0xf, false)));
+}
+
+// Maximum over the wave as a scalar: within rows of 16 lanes by DPP, then over the four rows.
+__device__ __forceinline__ uint32_t wave_max_uniform(uint32_t x) {
+  x = dpp_max<kDppQuadSwap1>(x);
+  x = dpp_max<kDppQuadSwap2>(x);
+  x = dpp_max<kDppRowHalfMirror>(x);
+  x = dpp_max<kDppRowMirror>(x);
+  const uint32_t a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16);
+  const uint32_t c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
+  return max(max(a, b), max(c, d));
+}
+
 // One wave a token, expert v * 64 + lane in register v. Selection is on the logits (the softmax
 // keeps their order), so ids are exact; top_k rounds of a wave maximum over (value, lowest index).
 // Latency-bound: a row is E logits.
@@ -61,18 +78,17 @@ __global__ __launch_bounds__(256) void route_kernel(const void* __restrict__ log
   float top = 0.f, mine = 0.f;
   int my_id = 0;
   for (int s = 0; s < top_k; ++s) {
-    uint64_t best = 0;
+    uint32_t best = key[0];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const uint64_t c =
-          static_cast<uint64_t>(key[v]) << 32 | (0xffffffffu - static_cast<uint32_t>(v * kWave + lane));
-      best = max(best, c);
+    for (int v = 1; v < V; ++v) best = max(best, key[v]);
+    best = wave_max_uniform(best);
+    int id = 0;
+#pragma unroll
+    for (int v = V - 1; v >= 0; --v) {
+      const uint64_t holders = __ballot(key[v] == best);
+      if (holders) id = v * kWave + __builtin_ctzll(holders);
     }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) best = max(best, static_cast<uint64_t>(__shfl_xor(
-                                                      static_cast<unsigned long long>(best), d)));
-    const int id = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
-    const float value = key_value(static_cast<uint32_t>(best >> 32));
+    const float value = key_value(best);
     if (s == 0) top = value;
     if (lane == s) mine = value, my_id = id;
 #pragma unroll
@@ -225,13 +241,24 @@ __global__ __launch_bounds__(256) void sum_slots(const uint16_t* __restrict__ y,
   const int64_t t = i / chunks;
   const int c = static_cast<int>(i - t * chunks) * 8;
   float sum[8] = {};
-  for (int s = 0; s < top_k; ++s) {
-    const int64_t slot = t * top_k + s;
-    if (!takes_part(ids[slot], experts)) continue;
-    float f[8];
-    unpack8<DT>(ld128(y + slot * ldy + c), f);
+  constexpr int kAtOnce = 8;  // slots whose loads are on their way together
+  for (int s0 = 0; s0 < top_k; s0 += kAtOnce) {
+    bool in[kAtOnce];
+    uint4 v[kAtOnce];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] += f[e];
+    for (int i = 0; i < kAtOnce; ++i)
+      in[i] = s0 + i < top_k && takes_part(ids[t * top_k + min(s0 + i, top_k - 1)], experts);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+      if (in[i]) v[i] = ld128(y + (t * top_k + s0 + i) * ldy + c);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (!in[i]) continue;
+      float f[8];
+      unpack8<DT>(v[i], f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += f[e];
+    }
   }
   uint16_t* o = out + t * ldo + c;
   if (vec && c + 8 <= width) {
@@ -251,8 +278,13 @@ struct Grouping {
   int bm;
 };
 
-Grouping choose_grouping(int64_t slots, int64_t experts) {
-  if (slots <= 16) return {0};
+// A few slots run one by one on vector math, without grouping (see product_vec.h): they seldom share
+// an expert, and a token's slots are summed in the down product.
+Grouping choose_grouping(int64_t slots, int64_t top_k, int64_t experts, int64_t hidden,
+                         int64_t inter, bool int8) {
+  const bool fits = top_k <= kVecDownSlots &&
+                    (!int8 || (pad(hidden, 16) <= kVecLds && top_k * pad(inter, 16) <= kVecLds));
+  if (slots <= 16 && fits) return {0};
   const int64_t per = slots / experts;
   if (per <= 8) return {16};
   if (per <= 64) return {64};
@@ -303,12 +335,12 @@ void launch_product(const ProductArgs& base, int bm, int64_t slots, int64_t expe
                     hipStream_t s) {
   ProductArgs a = base;
   // Tiles of bm rows that so many slots need at most: every full one and one more an expert.
-  const int64_t most = bm == 0 ? slots : slots / bm + std::min(experts, slots);
+  const int64_t most = slots / bm + std::min(experts, slots);
   auto grid = [&](int bn) {
     a.tiles_n = (a.columns + bn - 1) / bn;
     return dim3(static_cast<uint32_t>(pad(most * a.tiles_n, 8)));
   };
-  if (bm <= 16) {
+  if (bm == 16) {
     const dim3 g = grid(SILU ? 16 : 32);
     product_rows<IN, OT, MODE, SILU, 2, 4><<<g, 256, 0, s>>>(a);
   } else if (bm == 64) {
@@ -338,35 +370,89 @@ struct ExpertCall {
   int64_t tokens, top_k, experts, hidden, inter;
 };
 
+// The slots one by one.
+template <int IN, int OT>
+const char* expert_slots(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* ws,
+                         hipStream_t s) {
+  constexpr bool kQuant = IN == kInt8;
+  constexpr int kWaves = kQuant ? 16 : 4;
+  const int64_t slots = c.tokens * c.top_k;
+  ProductArgs a{};
+  a.x = c.x;
+  a.x_stride = c.x_stride;
+  a.k_bytes = static_cast<int32_t>(kQuant ? pad(c.hidden, 16) : c.hidden * 2);
+  a.w = c.gate_up;
+  a.w_stride = c.ld_gate_up;
+  a.w_expert = 2 * c.inter * c.ld_gate_up;
+  a.w_scales = c.gate_up_scales;
+  a.ids = c.ids;
+  a.rows = static_cast<int32_t>(slots);
+  a.top_k = static_cast<int32_t>(c.top_k);
+  a.experts = static_cast<int32_t>(c.experts);
+  a.out = ws + w.act;
+  a.ldo = kQuant ? pad(c.inter, 4) : c.inter;
+  a.columns = static_cast<int32_t>(c.inter);
+  a.tiles_n = static_cast<int32_t>((c.inter + kWaves - 1) / kWaves);
+  product_vec<IN, OT, kQuant ? kFloatOut : OT, kGateUp, true, 1, 2, kWaves>
+      <<<dim3(static_cast<uint32_t>(pad(slots * a.tiles_n, 8))), 64 * kWaves, 0, s>>>(
+          a, static_cast<int>(c.hidden), aligned(c.x, 16) && c.x_stride % 16 == 0);
+  if (const char* e = launch_status("product (gate_up)")) return e;
+  DownArgs d{};
+  d.act = ws + w.act;
+  d.act_stride = kQuant ? a.ldo * 4 : a.ldo * 2;
+  d.w = c.down;
+  d.w_stride = c.ld_down;
+  d.w_expert = c.hidden * c.ld_down;
+  d.w_scales = c.down_scales;
+  d.out = c.out;
+  d.ldo = c.ldo;
+  d.ids = c.ids;
+  d.weights = c.weights;
+  d.top_k = a.top_k;
+  d.experts = a.experts;
+  d.columns = static_cast<int32_t>(c.hidden);
+  d.k_bytes = static_cast<int32_t>(kQuant ? pad(c.inter, 16) : c.inter * 2);
+  d.width = static_cast<int32_t>(c.inter);
+  constexpr int kDownWaves = kQuant ? 8 : 4;
+  const dim3 grid(static_cast<uint32_t>((c.hidden + kDownWaves - 1) / kDownWaves),
+                  static_cast<uint32_t>(c.tokens));
+  if (d.k_bytes <= 16 * 48)
+    product_vec_down<IN, OT, 16, 2, kDownWaves><<<grid, 64 * kDownWaves, 0, s>>>(d);
+  else if (d.k_bytes <= 32 * 48)
+    product_vec_down<IN, OT, 32, 4, kDownWaves><<<grid, 64 * kDownWaves, 0, s>>>(d);
+  else
+    product_vec_down<IN, OT, 64, 4, kDownWaves><<<grid, 64 * kDownWaves, 0, s>>>(d);
+  return launch_status("product (down)");
+}
+
 // One pass over c.tokens tokens. IN: the operands' kind, OT: x's and out's type.
 template <int IN, int OT>
 const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* ws, hipStream_t s) {
   constexpr bool kQuant = IN == kInt8;
   const int64_t slots = c.tokens * c.top_k;
-  const Grouping g = choose_grouping(slots, c.experts);
+  const Grouping g =
+      choose_grouping(slots, c.top_k, c.experts, c.hidden, c.inter, kQuant);
+  if (g.bm == 0) return expert_slots<IN, OT>(c, w, ws, s);
   auto* order = reinterpret_cast<int32_t*>(ws + w.order);
   auto* row_weights = reinterpret_cast<float*>(ws + w.row_weights);
   auto* tiles = reinterpret_cast<int4*>(ws + w.tiles);
   auto* tile_count = reinterpret_cast<int32_t*>(ws + w.tile_count);
   auto* counts = reinterpret_cast<int32_t*>(ws + w.counts);
-  if (g.bm) {
-    const int chunks = static_cast<int>(pad(slots, kGroupChunk) / kGroupChunk);
-    if (chunks > 1) {
-      count_slots<<<dim3(chunks), kGroupThreads, 0, s>>>(c.ids, static_cast<int>(slots),
-                                                         static_cast<int>(c.experts), counts);
-      if (const char* e = launch_status("count_slots")) return e;
-    }
-    place_slots<<<dim3(chunks), kGroupThreads, 0, s>>>(
-        c.ids, static_cast<int>(slots), static_cast<int>(c.experts), g.bm,
-        chunks > 1 ? counts : nullptr, chunks, c.weights, order, row_weights, tiles, tile_count);
-    if (const char* e = launch_status("place_slots")) return e;
+  const int chunks = static_cast<int>(pad(slots, kGroupChunk) / kGroupChunk);
+  if (chunks > 1) {
+    count_slots<<<dim3(chunks), kGroupThreads, 0, s>>>(c.ids, static_cast<int>(slots),
+                                                       static_cast<int>(c.experts), counts);
+    if (const char* e = launch_status("count_slots")) return e;
   }
+  place_slots<<<dim3(chunks), kGroupThreads, 0, s>>>(
+      c.ids, static_cast<int>(slots), static_cast<int>(c.experts), g.bm,
+      chunks > 1 ? counts : nullptr, chunks, c.weights, order, row_weights, tiles, tile_count);
+  if (const char* e = launch_status("place_slots")) return e;
   ProductArgs a{};
-  a.order = g.bm ? order : nullptr;
-  a.tiles = g.bm ? tiles : nullptr;
+  a.order = order;
+  a.tiles = tiles;
   a.tile_count = tile_count;
-  a.ids = c.ids;
-  a.row_weights = g.bm ? row_weights : c.weights;
+  a.row_weights = row_weights;
   a.rows = static_cast<int32_t>(slots);
   a.top_k = static_cast<int32_t>(c.top_k);
   a.experts = static_cast<int32_t>(c.experts);

@@ -41,8 +41,8 @@ struct ProductArgs {
   void* out;
   const float* x_scales;      // int8: one a row of x
   const float* w_scales;      // int8: [E][w_rows]
-  const int32_t* order;       // grouped: slot (token * top_k + s) of every grouped row; null: r itself
-  const int32_t* ids;         // with a null tile list: expert of every slot
+  const int32_t* order;       // grouped: slot (token * top_k + s) of every row; null: the row itself
+  const int32_t* ids;         // with a null tile list (one slot a tile): expert of every slot
   const int4* tiles;          // grouped: {expert, first row, end row, 0} per row tile
   const int32_t* tile_count;  // grouped: tiles in the list
   const float* row_weights;   // kDown: weight of every row of the grouped order

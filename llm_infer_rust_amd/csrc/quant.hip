@@ -8,61 +8,14 @@
 // itself has none.
 #include <algorithm>
 
-#include "quant.h"
+#include "product_vec.h"
 
 namespace mi355x {
 namespace {
 
-// 16 elements of a row as floats; `n` of them exist, the others are 0.
-template <int DT>
-__device__ __forceinline__ void load16(const uint8_t* row, int64_t at, int n, bool vec,
-                                       float (&f)[16]) {
-  constexpr int kSize = DT == kFloatOut ? 4 : 2;
-  const uint8_t* p = row + at * kSize;
-  if (vec && n >= 16) {
-    if constexpr (DT == kFloatOut) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 v = *reinterpret_cast<const float4*>(p + 16 * i);
-        f[4 * i] = v.x, f[4 * i + 1] = v.y, f[4 * i + 2] = v.z, f[4 * i + 3] = v.w;
-      }
-    } else {
-      float lo[8], hi[8];
-      unpack8<DT>(ld128(p), lo);
-      unpack8<DT>(ld128(p + 16), hi);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = lo[i], f[8 + i] = hi[i];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (i >= n) {
-        f[i] = 0.f;
-      } else if constexpr (DT == kFloatOut) {
-        f[i] = reinterpret_cast<const float*>(p)[i];
-      } else {
-        f[i] = Elem<DT>::to_float(reinterpret_cast<const uint16_t*>(p)[i]);
-      }
-    }
-  }
-}
-
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(v, d)));
-  return v;
-}
-
 // One row per LANES threads (a wave, or the whole workgroup of 256). The row's first HELD chunks of
 // 16 a thread stay in registers between the two passes, the rest is read again. Bound by memory:
 // every row is read once and written at half its size (8,192 rows of 4,096 bf16: 100 MB).
-//
-// The largest magnitude is taken on the bits, where inf and NaN come out on top: such a row gets
-// the scale NaN, so its products are NaN and no other row's. The quotient 127 x / max is correctly
-// rounded (q0 = p r with the correctly rounded reciprocal r, then one residual step, after
-// P. Markstein, IBM J. Res. Dev. 34, 1990), which makes q the nearest integer of the exact
-// quotient for 16-bit x: 127 x is exact there and no quotient of such numbers lies closer to a half
-// than fp32 resolves. Rows near the ends of the fp32 range are scaled by 2^-32 or 2^64 first.
 template <int DT, int LANES, int HELD>
 __global__ __launch_bounds__(256) void quantize_rows(const uint8_t* __restrict__ x, int64_t stride,
                                                      uint8_t* __restrict__ values, int64_t ldv,
@@ -78,22 +31,18 @@ __global__ __launch_bounds__(256) void quantize_rows(const uint8_t* __restrict__
   const int chunks = (width + 15) >> 4;
   float held[HELD][16];
   uint32_t top = 0;
-  auto bits = [&](const float (&f)[16]) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-  };
 #pragma unroll
   for (int h = 0; h < HELD; ++h) {
     const int c = lane + h * LANES;
     if (c < chunks) {
       load16<DT>(src, c * 16, width - c * 16, vec, held[h]);
-      bits(held[h]);
+      top = max(top, magnitude16(held[h]));
     }
   }
   for (int c = lane + HELD * LANES; c < chunks; c += LANES) {
     float f[16];
     load16<DT>(src, c * 16, width - c * 16, vec, f);
-    bits(f);
+    top = max(top, magnitude16(f));
   }
   top = wave_max(top);
   if constexpr (LANES > kWave) {
@@ -101,29 +50,9 @@ __global__ __launch_bounds__(256) void quantize_rows(const uint8_t* __restrict__
     __syncthreads();
     top = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
   }
-  const float largest = __uint_as_float(top);
-  const bool finite = top < 0x7f800000u;
-  if (lane == 0) scales[row] = finite ? largest / 127.f : __uint_as_float(0x7fc00000u);
-  const float range = largest > 1e30f ? 0x1p-32f : largest < 1e-30f ? 0x1p64f : 1.f;
-  const float a = largest * range, p127 = 127.f * range;
-  const float r = finite && top != 0 ? 1.f / a : 0.f;
-  auto put = [&](int c, const float (&f)[16]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t b[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p = f[4 * i + e] * p127;
-        const float q0 = p * r;
-        const float q = fmaf(fmaf(-q0, a, p), r, q0);
-        // 1.5 * 2^23 leaves the rounded integer in the low bits (half to even)
-        b[e] = __float_as_uint(q + 12582912.f) & 0xffu;
-      }
-      w[i] = finite ? b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24 : 0u;
-    }
-    st128(dst + c * 16, make_uint4(w[0], w[1], w[2], w[3]));
-  };
+  const RowQuant q(top);
+  if (lane == 0) scales[row] = q.scale;
+  auto put = [&](int c, const float (&f)[16]) { st128(dst + c * 16, q.values(f)); };
 #pragma unroll
   for (int h = 0; h < HELD; ++h) {
     const int c = lane + h * LANES;
@@ -159,12 +88,31 @@ struct Int8Workspace {
   int64_t values, scales, bytes;
 };
 
+// One or two rows are quantised inside the product (see product_vec.h) where they fit its LDS.
+bool on_vector_math(int64_t M, int64_t K) { return M <= 2 && M * padded16(K) <= kVecLds; }
+
 Int8Workspace int8_workspace(int64_t M, int64_t K) {
   Int8Workspace w{};
+  if (on_vector_math(M, K)) return w;
   w.values = 0;
   w.scales = padded16(M * padded16(K));
   w.bytes = w.scales + padded16(M * 4);
   return w;
+}
+
+template <int OT, bool SILU>
+void launch_int8_vec(const ProductArgs& base, int64_t M, int64_t columns, int width, bool vec,
+                     hipStream_t s) {
+  ProductArgs a = base;
+  constexpr int kWaves = 16, kRows = 2;
+  const int bn = kWaves * (SILU ? kRows / 2 : kRows);
+  a.tiles_m = 1;
+  a.tiles_n = static_cast<int32_t>((columns + bn - 1) / bn);
+  const dim3 g(static_cast<uint32_t>((a.tiles_n + 7) / 8 * 8));
+  if (M == 1)
+    product_vec<kInt8, OT, OT, kDense, SILU, 1, kRows, kWaves><<<g, 64 * kWaves, 0, s>>>(a, width, vec);
+  else
+    product_vec<kInt8, OT, OT, kDense, SILU, 2, kRows, kWaves><<<g, 64 * kWaves, 0, s>>>(a, width, vec);
 }
 
 template <int OT, bool SILU>
@@ -243,29 +191,21 @@ extern "C" const char* mi355x_linear_int8(const void* x, int64_t ldx, const void
     return set_error("mi355x_linear_int8: unsupported shape (K up to 131072, weight rows of whole "
                      "16-byte words, less than 4 GiB)");
   if (M == 0) return nullptr;
-  if (!x || !w || !w_scales || !out || !workspace)
+  const Int8Workspace ws = int8_workspace(M, K);
+  if (!x || !w || !w_scales || !out || (!workspace && ws.bytes))
     return set_error("mi355x_linear_int8: null pointer");
   if (!aligned(x, 2) || !aligned(w, 16) || !aligned(w_scales, 4) || !aligned(out, 2) ||
       !aligned(workspace, 16))
     return set_error("mi355x_linear_int8: misaligned operand");
-  const Int8Workspace ws = int8_workspace(M, K);
   if (workspace_bytes < ws.bytes) return set_error("mi355x_linear_int8: workspace too small");
   // More row and column tiles than a grid holds (16 x 16 is the smallest tile).
   if ((M + 15) / 16 * ((columns + 15) / 16) >= (int64_t(1) << 30))
     return set_error("mi355x_linear_int8: grid too large");
   auto s = static_cast<hipStream_t>(stream);
-  auto* base = static_cast<uint8_t*>(workspace);
-  auto* scales = reinterpret_cast<float*>(base + ws.scales);
-  if (const char* e = run_quantize_rows(x, ldx * 2, base, padded16(K), scales, M, K,
-                                        static_cast<int>(dtype), s))
-    return e;
   ProductArgs a{};
-  a.x = base;
   a.w = static_cast<const uint8_t*>(w);
   a.out = out;
-  a.x_scales = scales;
   a.w_scales = w_scales;
-  a.x_stride = padded16(K);
   a.w_stride = ldw;
   a.ldo = ldo;
   a.rows = static_cast<int32_t>(M);
@@ -273,6 +213,27 @@ extern "C" const char* mi355x_linear_int8(const void* x, int64_t ldx, const void
   a.k_bytes = static_cast<int32_t>(padded16(K));
   a.vec_out = ldo % 4 == 0 && aligned(out, 8);
   a.vec16_out = ldo % 8 == 0 && aligned(out, 16);
+  if (on_vector_math(M, K)) {
+    a.x = static_cast<const uint8_t*>(x);
+    a.x_stride = ldx * 2;
+    const bool vec = aligned(x, 16) && ldx % 8 == 0;
+    const int width = static_cast<int>(K);
+    if (dtype == 0)
+      silu_mul ? launch_int8_vec<0, true>(a, M, columns, width, vec, s)
+               : launch_int8_vec<0, false>(a, M, columns, width, vec, s);
+    else
+      silu_mul ? launch_int8_vec<1, true>(a, M, columns, width, vec, s)
+               : launch_int8_vec<1, false>(a, M, columns, width, vec, s);
+    return launch_status("product (int8)");
+  }
+  auto* base = static_cast<uint8_t*>(workspace);
+  auto* scales = reinterpret_cast<float*>(base + ws.scales);
+  if (const char* e = run_quantize_rows(x, ldx * 2, base, padded16(K), scales, M, K,
+                                        static_cast<int>(dtype), s))
+    return e;
+  a.x = base;
+  a.x_scales = scales;
+  a.x_stride = padded16(K);
   if (dtype == 0)
     silu_mul ? launch_int8<0, true>(a, M, columns, s) : launch_int8<0, false>(a, M, columns, s);
   else

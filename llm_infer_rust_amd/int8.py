@@ -154,11 +154,12 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = 
         need = lib().mi355x_linear_int8_workspace_bytes(t, k)
         if need < 0:
             raise NativeError("linear_int8: invalid shape")
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=x.device)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         check(lib().mi355x_linear_int8(x.data_ptr(), _row_stride(x), weight.values.data_ptr(),
                                        weight.row_stride, weight.scales.data_ptr(),
                                        out.data_ptr(), _row_stride(out), t, n, k, silu_mul,
-                                       ws.data_ptr(), need, dt, stream_of(x)), "linear_int8")
+                                       None if ws is None else ws.data_ptr(), need, dt,
+                                       stream_of(x)), "linear_int8")
     return out
 
 
