@@ -348,9 +348,10 @@ const char* mi355x_quantize_rows(const void* x, int64_t ldx, void* values, int64
                                  void* scales, int64_t rows, int64_t width, int dtype,
                                  void* stream);
 
-/* Workspace bytes of mi355x_linear_int8 (the quantised rows and their scales), -1 for an
+/* Workspace bytes of mi355x_linear_int8 on a GPU of `cus` compute units (the quantised rows, their
+ * scales and, where K is split, int32 sums; 0 for one or two rows of up to 32 KiB), -1 for an
  * invalid shape. Host-only. */
-int64_t mi355x_linear_int8_workspace_bytes(int64_t M, int64_t K);
+int64_t mi355x_linear_int8_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t cus);
 
 /* out[m, n] = round(sx[m] w_scales[n] sum_k q[m, k] w[n, k]) with (q, sx) = mi355x_quantize_rows
  * of x [M, K] (dtype 0 bf16, 1 fp16; out has the same) and w int8 [N, ldw]; the sum is exact
@@ -361,7 +362,7 @@ int64_t mi355x_linear_int8_workspace_bytes(int64_t M, int64_t K);
 const char* mi355x_linear_int8(const void* x, int64_t ldx, const void* w, int64_t ldw,
                                const float* w_scales, void* out, int64_t ldo, int64_t M,
                                int64_t N, int64_t K, bool silu_mul, void* workspace,
-                               int64_t workspace_bytes, int64_t dtype, void* stream);
+                               int64_t workspace_bytes, int32_t cus, int64_t dtype, void* stream);
 
 /* ------------------------------------------------------------------------
  * Layers of experts. No reference counterpart (its layers are dense).
@@ -402,8 +403,8 @@ const char* mi355x_expert_mlp(const void* x, int64_t ldx, const int32_t* ids,
                               const float* gate_up_scales, const void* down, int64_t ld_down,
                               const float* down_scales, void* out, int64_t ldo, int64_t tokens,
                               int64_t top_k, int64_t experts, int64_t hidden, int64_t inter,
-                              void* workspace, int64_t workspace_bytes, int64_t dtype,
-                              void* stream);
+                              void* workspace, int64_t workspace_bytes, int32_t cus,
+                              int64_t dtype, void* stream);
 
 /* ------------------------------------------------------------------------
  * Sampling.

@@ -106,18 +106,18 @@ SIGNATURES: dict[str, tuple] = {
                                           c_void_p]),
     "mi355x_quantize_rows": (c_char_p, [c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_i64,
                                         c_int, c_void_p]),
-    "mi355x_linear_int8_workspace_bytes": (c_i64, [c_i64, c_i64]),
+    "mi355x_linear_int8_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64, c_i32]),
     "mi355x_linear_int8": (c_char_p, [c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_i64,
-                                      c_i64, c_i64, c_i64, c_bool, c_void_p, c_i64, c_i64,
-                                      c_void_p]),
+                                      c_i64, c_i64, c_i64, c_bool, c_void_p, c_i64, c_i32,
+                                      c_i64, c_void_p]),
     "mi355x_route_experts": (c_char_p, [c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_i64, c_i64,
                                         c_bool, c_int, c_void_p]),
     "mi355x_expert_mlp_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
                                                   c_bool]),
     "mi355x_expert_mlp": (c_char_p, [c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_i64,
                                      c_void_p, c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_i64,
-                                     c_i64, c_i64, c_i64, c_i64, c_void_p, c_i64, c_i64,
-                                     c_void_p]),
+                                     c_i64, c_i64, c_i64, c_i64, c_void_p, c_i64, c_i32,
+                                     c_i64, c_void_p]),
     "mi355x_sample": (c_char_p, [c_void_p, c_i64, c_i64, c_i64, c_int, c_void_p, c_void_p,
                                  c_void_p, c_u64, c_u64, c_void_p, c_void_p]),
     "mi355x_sample_split": (c_char_p, [c_void_p, c_i64, c_i64, c_i64, c_int, c_void_p, c_void_p,

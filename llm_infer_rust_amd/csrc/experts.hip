@@ -135,7 +135,7 @@ void launch_route(const void* logits, int64_t stride, float* weights, int32_t* i
 
 // ---------------------------------------------------------------------------- grouping
 constexpr int kGroupThreads = 1024;
-constexpr int kGroupChunk = 4096;  // slots a workgroup of the grouping passes takes
+constexpr int kGroupChunk = 2048;  // slots a workgroup of the grouping passes takes
 
 __device__ __forceinline__ bool takes_part(int e, int experts) { return e >= 0 && e < experts; }
 
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(kGroupThreads) void count_slots(const int32_t* __re
 }
 
 // Exclusive prefix sum of one value a thread over the workgroup.
-__device__ __forceinline__ int block_exclusive(int v, int* wave_totals) {
+__device__ __forceinline__ int block_exclusive(int v, int4 (&wave_totals)[4]) {
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   int s = v;
 #pragma unroll
@@ -166,55 +166,67 @@ __device__ __forceinline__ int block_exclusive(int v, int* wave_totals) {
     if (lane >= d) s += o;
   }
   __syncthreads();
-  if (lane == kWave - 1) wave_totals[wave] = s;
+  if (lane == kWave - 1) reinterpret_cast<int*>(wave_totals)[wave] = s;
   __syncthreads();
-  int before = 0;
-  for (int w = 0; w < wave; ++w) before += wave_totals[w];
-  return before + s - v;
+  int before = s - v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int4 t = wave_totals[i];
+    before += (4 * i < wave ? t.x : 0) + (4 * i + 1 < wave ? t.y : 0) + (4 * i + 2 < wave ? t.z : 0) +
+              (4 * i + 3 < wave ? t.w : 0);
+  }
+  return before;
 }
 
-// order[row]: the slots in the order of their experts; row_weights[row]: their weights. `counts` may be null with one chunk. The
-// first workgroup writes the list of row tiles of bm rows. The order of the slots within an
+// order[row]: the slots in the order of their experts; row_weights[row]: their weights. `counts` may
+// be null with one chunk. The first workgroup writes the list of row tiles for the gate_up product, the
+// second (or the first, if alone) that for the down product. The order of the slots within an
 // expert is that of the LDS atomics; a row's products do not depend on the row it stands in.
 __global__ __launch_bounds__(kGroupThreads) void place_slots(const int32_t* __restrict__ ids,
-                                                             int slots, int experts, int bm,
+                                                             int slots, int experts,
+                                                             int gate_up_bm, int down_bm,
                                                              const int32_t* __restrict__ counts,
                                                              int chunks,
                                                              const float* __restrict__ weights,
                                                              int32_t* __restrict__ order,
                                                              float* __restrict__ row_weights,
-                                                             int4* __restrict__ tiles,
-                                                             int32_t* __restrict__ tile_count) {
-  __shared__ int cursor[kMaxExperts];
-  __shared__ int wave_totals[kGroupThreads / kWave];
+                                                             int4* __restrict__ gate_up_tiles,
+                                                             int4* __restrict__ down_tiles,
+                                                             int32_t* __restrict__ tile_counts) {
+  static_assert(kMaxExperts == kGroupThreads, "an expert a thread");
+  __shared__ int cursor[kMaxExperts], totals[kMaxExperts];
+  __shared__ int4 wave_totals[4];
   const int e = threadIdx.x;
   const int begin = blockIdx.x * kGroupChunk, end = min(slots, begin + kGroupChunk);
-  int before = 0, total = 0;
+  cursor[e] = totals[e] = 0;  // slots of the chunks before this one, and of all
+  __syncthreads();
   if (counts) {
-    if (e < experts)
-      for (int c = 0; c < chunks; ++c) {
-        const int n = counts[c * experts + e];
-        total += n;
-        if (c < static_cast<int>(blockIdx.x)) before += n;
-      }
+    const int before = static_cast<int>(blockIdx.x) * experts;
+    for (int i = threadIdx.x; i < chunks * experts; i += kGroupThreads) {
+      const int n = counts[i];
+      if (n == 0) continue;
+      atomicAdd(&totals[i % experts], n);
+      if (i < before) atomicAdd(&cursor[i % experts], n);
+    }
   } else {
-    cursor[e] = 0;
-    __syncthreads();
     for (int i = begin + threadIdx.x; i < end; i += kGroupThreads) {
       const int x = ids[i];
-      if (takes_part(x, experts)) atomicAdd(&cursor[x], 1);
+      if (takes_part(x, experts)) atomicAdd(&totals[x], 1);
     }
-    __syncthreads();
-    total = e < experts ? cursor[e] : 0;
   }
+  __syncthreads();
+  const int total = totals[e];
   const int first = block_exclusive(total, wave_totals);
-  cursor[e] = first + before;
-  if (blockIdx.x == 0) {
+  cursor[e] += first;
+  for (int product = 0; product < 2; ++product) {
+    if (static_cast<int>(blockIdx.x) != min(product, chunks - 1)) continue;
+    const int bm = product ? down_bm : gate_up_bm;
+    int4* tiles = product ? down_tiles : gate_up_tiles;
     const int n = (total + bm - 1) / bm;
     const int at = block_exclusive(n, wave_totals);
     for (int i = 0; i < n; ++i)
       tiles[at + i] = make_int4(e, first + i * bm, min(first + (i + 1) * bm, first + total), 0);
-    if (e == kGroupThreads - 1) *tile_count = at + n;
+    if (e == kGroupThreads - 1) tile_counts[product] = at + n;
   }
   __syncthreads();
   for (int i = begin + threadIdx.x; i < end; i += kGroupThreads) {
@@ -273,28 +285,38 @@ __global__ __launch_bounds__(256) void sum_slots(const uint16_t* __restrict__ y,
 // ---------------------------------------------------------------------------- the products
 int64_t pad(int64_t n, int64_t a) { return (n + a - 1) / a * a; }
 
-// Row tile of the grouped products: 0 slots without grouping.
-struct Grouping {
-  int bm;
-};
-
 // A few slots run one by one on vector math, without grouping (see product_vec.h): they seldom share
 // an expert, and a token's slots are summed in the down product.
-Grouping choose_grouping(int64_t slots, int64_t top_k, int64_t experts, int64_t hidden,
-                         int64_t inter, bool int8) {
-  const bool fits = top_k <= kVecDownSlots &&
-                    (!int8 || (pad(hidden, 16) <= kVecLds && top_k * pad(inter, 16) <= kVecLds));
-  if (slots <= 16 && fits) return {0};
-  const int64_t per = slots / experts;
-  if (per <= 8) return {16};
-  if (per <= 64) return {64};
-  return {256};
+bool one_by_one(int64_t slots, int64_t top_k, int64_t hidden, int64_t inter, bool int8) {
+  return slots <= 16 && top_k <= kVecDownSlots &&
+         (!int8 || (pad(hidden, 16) <= kVecLds && top_k * pad(inter, 16) <= kVecLds));
+}
+
+// The tile of a grouped product: the least estimate. How many rows an expert gets is not known on the
+// host; it is taken to be the same for all, with half a tile more each for the ragged ends.
+Tile choose_tile(int64_t slots, int64_t experts, int64_t weight_rows, int64_t k_bytes, int cus) {
+  const float active = static_cast<float>(std::min(slots, experts));
+  const float per = static_cast<float>(slots) / active;
+  const float weights = active * static_cast<float>(weight_rows) * static_cast<float>(k_bytes);
+  Tile best = Tile::k64;
+  float best_us = 1e30f;
+  for (int i = 0; i < 4; ++i) {
+    const TileShape& t = kTileShapes[i];
+    const float tm = active * std::max(1.f, per / static_cast<float>(t.bm) + 0.5f);
+    const float tn = std::ceil(static_cast<float>(weight_rows) / static_cast<float>(t.bn));
+    const float us = tile_estimate(static_cast<Tile>(i), tm, tn, k_bytes, weights, per <= 128.f, cus);
+    if (us < best_us) {
+      best_us = us;
+      best = static_cast<Tile>(i);
+    }
+  }
+  return best;
 }
 
 constexpr int64_t kMaxSlots = 131072;  // slots a pass takes; more tokens run in several passes
 
 struct ExpertWorkspace {
-  int64_t order, row_weights, tiles, tile_count, counts, xq, xs, act, actq, acts, y, bytes;
+  int64_t order, row_weights, gate_up_tiles, down_tiles, tile_counts, counts, xq, xs, act, actq, acts, y, bytes;
   int64_t tokens;  // a pass
 };
 
@@ -315,8 +337,10 @@ ExpertWorkspace expert_workspace(int64_t tokens, int64_t top_k, int64_t experts,
   };
   w.order = take(slots * 4);
   w.row_weights = take(slots * 4);
-  w.tiles = take((std::min(experts, slots) + slots / 16 + 1) * 16);
-  w.tile_count = take(4);
+  const int64_t tiles = std::min(experts, slots) + slots / kTileShapes[0].bm + 1;
+  w.gate_up_tiles = take(tiles * 16);
+  w.down_tiles = take(tiles * 16);
+  w.tile_counts = take(8);
   w.counts = take(pad(slots, kGroupChunk) / kGroupChunk * experts * 4);
   w.act = take(slots * (int8 ? pad(inter, 4) * 4 : inter * 2));
   if (int8) {
@@ -331,27 +355,27 @@ ExpertWorkspace expert_workspace(int64_t tokens, int64_t top_k, int64_t experts,
 }
 
 template <int IN, int OT, int MODE, bool SILU>
-void launch_product(const ProductArgs& base, int bm, int64_t slots, int64_t experts,
+void launch_product(const ProductArgs& base, Tile tile, int64_t slots, int64_t experts,
                     hipStream_t s) {
   ProductArgs a = base;
-  // Tiles of bm rows that so many slots need at most: every full one and one more an expert.
-  const int64_t most = slots / bm + std::min(experts, slots);
-  auto grid = [&](int bn) {
-    a.tiles_n = (a.columns + bn - 1) / bn;
-    return dim3(static_cast<uint32_t>(pad(most * a.tiles_n, 8)));
-  };
-  if (bm == 16) {
-    const dim3 g = grid(SILU ? 16 : 32);
-    product_rows<IN, OT, MODE, SILU, 2, 4><<<g, 256, 0, s>>>(a);
-  } else if (bm == 64) {
-    const dim3 g = grid(SILU ? 32 : 64);
-    product_tile<IN, OT, MODE, SILU, 64, 64, 2, 2, 4><<<g, 256, 0, s>>>(a);
-  } else {
-    const dim3 g = grid(SILU ? 128 : 256);
-    if (a.k_bytes % kProdRow)
-      product_large<IN, OT, MODE, SILU, 256, 8, true><<<g, 512, 0, s>>>(a);
-    else
-      product_large<IN, OT, MODE, SILU, 256, 8, false><<<g, 512, 0, s>>>(a);
+  const TileShape& t = kTileShapes[static_cast<int>(tile)];
+  const int bn = SILU ? t.bn / 2 : t.bn;
+  a.tiles_n = (a.columns + bn - 1) / bn;
+  // Tiles that so many slots need at most: every full one and one more an expert.
+  const int64_t most = slots / t.bm + std::min(experts, slots);
+  const dim3 g(static_cast<uint32_t>(pad(most * a.tiles_n, 8)));
+  switch (tile) {
+    case Tile::k64: product_tile<IN, OT, MODE, SILU, 64, 64, 2, 2, 4><<<g, 256, 0, s>>>(a); break;
+    case Tile::k128: product_tile<IN, OT, MODE, SILU, 128, 128, 4, 2, 4><<<g, 512, 0, s>>>(a); break;
+    case Tile::k256x128:
+      product_tile<IN, OT, MODE, SILU, 256, 128, 4, 2, 3><<<g, 512, 0, s>>>(a);
+      break;
+    case Tile::k256:
+      if (a.k_bytes % kProdRow)
+        product_large<IN, OT, MODE, SILU, 256, 8, true><<<g, 512, 0, s>>>(a);
+      else
+        product_large<IN, OT, MODE, SILU, 256, 8, false><<<g, 512, 0, s>>>(a);
+      break;
   }
 }
 
@@ -368,6 +392,7 @@ struct ExpertCall {
   uint16_t* out;
   int64_t ldo;
   int64_t tokens, top_k, experts, hidden, inter;
+  int32_t cus;
 };
 
 // The slots one by one.
@@ -430,13 +455,17 @@ template <int IN, int OT>
 const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* ws, hipStream_t s) {
   constexpr bool kQuant = IN == kInt8;
   const int64_t slots = c.tokens * c.top_k;
-  const Grouping g =
-      choose_grouping(slots, c.top_k, c.experts, c.hidden, c.inter, kQuant);
-  if (g.bm == 0) return expert_slots<IN, OT>(c, w, ws, s);
+  if (one_by_one(slots, c.top_k, c.hidden, c.inter, kQuant))
+    return expert_slots<IN, OT>(c, w, ws, s);
+  const int64_t gate_up_k = kQuant ? pad(c.hidden, 16) : c.hidden * 2;
+  const int64_t down_k = kQuant ? pad(c.inter, 16) : c.inter * 2;
+  const Tile gate_up_tile = choose_tile(slots, c.experts, 2 * c.inter, gate_up_k, c.cus);
+  const Tile down_tile = choose_tile(slots, c.experts, c.hidden, down_k, c.cus);
   auto* order = reinterpret_cast<int32_t*>(ws + w.order);
   auto* row_weights = reinterpret_cast<float*>(ws + w.row_weights);
-  auto* tiles = reinterpret_cast<int4*>(ws + w.tiles);
-  auto* tile_count = reinterpret_cast<int32_t*>(ws + w.tile_count);
+  auto* gate_up_tiles = reinterpret_cast<int4*>(ws + w.gate_up_tiles);
+  auto* down_tiles = reinterpret_cast<int4*>(ws + w.down_tiles);
+  auto* tile_counts = reinterpret_cast<int32_t*>(ws + w.tile_counts);
   auto* counts = reinterpret_cast<int32_t*>(ws + w.counts);
   const int chunks = static_cast<int>(pad(slots, kGroupChunk) / kGroupChunk);
   if (chunks > 1) {
@@ -445,13 +474,15 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
     if (const char* e = launch_status("count_slots")) return e;
   }
   place_slots<<<dim3(chunks), kGroupThreads, 0, s>>>(
-      c.ids, static_cast<int>(slots), static_cast<int>(c.experts), g.bm,
-      chunks > 1 ? counts : nullptr, chunks, c.weights, order, row_weights, tiles, tile_count);
+      c.ids, static_cast<int>(slots), static_cast<int>(c.experts),
+      kTileShapes[static_cast<int>(gate_up_tile)].bm, kTileShapes[static_cast<int>(down_tile)].bm,
+      chunks > 1 ? counts : nullptr, chunks, c.weights, order, row_weights, gate_up_tiles,
+      down_tiles, tile_counts);
   if (const char* e = launch_status("place_slots")) return e;
   ProductArgs a{};
   a.order = order;
-  a.tiles = tiles;
-  a.tile_count = tile_count;
+  a.tiles = gate_up_tiles;
+  a.tile_count = tile_counts;
   a.row_weights = row_weights;
   a.rows = static_cast<int32_t>(slots);
   a.top_k = static_cast<int32_t>(c.top_k);
@@ -466,11 +497,11 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
     a.x = ws + w.xq;
     a.x_stride = pad(c.hidden, 16);
     a.x_scales = xs;
-    a.k_bytes = static_cast<int32_t>(pad(c.hidden, 16));
+    a.k_bytes = static_cast<int32_t>(gate_up_k);
   } else {
     a.x = c.x;
     a.x_stride = c.x_stride;
-    a.k_bytes = static_cast<int32_t>(c.hidden * 2);
+    a.k_bytes = static_cast<int32_t>(gate_up_k);
   }
   a.w = c.gate_up;
   a.w_stride = c.ld_gate_up;
@@ -479,7 +510,7 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   a.out = ws + w.act;
   a.ldo = kQuant ? pad(c.inter, 4) : c.inter;
   a.columns = static_cast<int32_t>(c.inter);
-  launch_product<IN, kQuant ? kFloatOut : OT, kGateUp, true>(a, g.bm, slots, c.experts, s);
+  launch_product<IN, kQuant ? kFloatOut : OT, kGateUp, true>(a, gate_up_tile, slots, c.experts, s);
   if (const char* e = launch_status("product (gate_up)")) return e;
   // down into y, one weighted row a slot
   if (kQuant) {
@@ -491,12 +522,14 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
     a.x = ws + w.actq;
     a.x_stride = pad(c.inter, 16);
     a.x_scales = acts;
-    a.k_bytes = static_cast<int32_t>(pad(c.inter, 16));
+    a.k_bytes = static_cast<int32_t>(down_k);
   } else {
     a.x = ws + w.act;
     a.x_stride = c.inter * 2;
-    a.k_bytes = static_cast<int32_t>(c.inter * 2);
+    a.k_bytes = static_cast<int32_t>(down_k);
   }
+  a.tiles = down_tiles;
+  a.tile_count = tile_counts + 1;
   a.w = c.down;
   a.w_stride = c.ld_down;
   a.w_expert = c.hidden * c.ld_down;
@@ -504,7 +537,7 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   a.out = ws + w.y;
   a.ldo = pad(c.hidden, 8);
   a.columns = static_cast<int32_t>(c.hidden);
-  launch_product<IN, OT, kDown, false>(a, g.bm, slots, c.experts, s);
+  launch_product<IN, OT, kDown, false>(a, down_tile, slots, c.experts, s);
   if (const char* e = launch_status("product (down)")) return e;
   const int64_t threads = c.tokens * (pad(c.hidden, 8) / 8);
   sum_slots<OT><<<dim3(static_cast<uint32_t>((threads + 255) / 256)), 256, 0, s>>>(
@@ -566,7 +599,8 @@ extern "C" const char* mi355x_expert_mlp(const void* x, int64_t ldx, const int32
                                          const float* down_scales, void* out, int64_t ldo,
                                          int64_t tokens, int64_t top_k, int64_t experts,
                                          int64_t hidden, int64_t inter, void* workspace,
-                                         int64_t workspace_bytes, int64_t dtype, void* stream) {
+                                         int64_t workspace_bytes, int32_t cus, int64_t dtype,
+                                         void* stream) {
   const bool int8 = gate_up_scales != nullptr;
   if (int8 != (down_scales != nullptr))
     return set_error("mi355x_expert_mlp: gate_up and down weights must be of one kind");
@@ -609,6 +643,7 @@ extern "C" const char* mi355x_expert_mlp(const void* x, int64_t ldx, const int32
     c.experts = experts;
     c.hidden = hidden;
     c.inter = inter;
+    c.cus = cus > 0 ? cus : 256;
     auto* ws = static_cast<uint8_t*>(workspace);
     const char* e = int8 ? (dtype == 0 ? expert_pass<kInt8, 0>(c, w, ws, s)
                                        : expert_pass<kInt8, 1>(c, w, ws, s))

@@ -17,6 +17,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <type_traits>
 
@@ -33,7 +34,8 @@ constexpr int kFloatOut = 2;                    // outputs: 0 bf16, 1 fp16, 2 fp
 //   kGateUp   row r of the grouped order reads x row order[r] / top_k and writes out row r
 //   kDown     row r of the grouped order reads x row r and writes out row order[r], times that
 //             slot's weight
-constexpr int kDense = 0, kGateUp = 1, kDown = 2;
+//   kSplit    kDense over a part of K, the int32 sums left as they are (int8 only)
+constexpr int kDense = 0, kGateUp = 1, kDown = 2, kSplit = 3;
 
 struct ProductArgs {
   const uint8_t* x;
@@ -55,7 +57,8 @@ struct ProductArgs {
   int32_t k_bytes;            // bytes of K, a multiple of 16
   int32_t top_k;
   int32_t experts;
-  int32_t tiles_m, tiles_n;   // kDense: row tiles; column tiles of every row tile
+  int32_t tiles_m, tiles_n;   // kDense, kSplit: row tiles; column tiles of every row tile
+  int32_t splits;             // kSplit: parts of K; out is int32 [splits][rows][ldo]
   int32_t vec_out;            // out rows take aligned stores of four elements
   int32_t vec16_out;          // out rows take aligned 16-byte stores
 };
@@ -193,7 +196,7 @@ struct RowTile {
 
 template <int MODE, int BM>
 __device__ __forceinline__ bool row_tile(const ProductArgs& a, int tm, RowTile* t) {
-  if constexpr (MODE == kDense) {
+  if constexpr (MODE == kDense || MODE == kSplit) {
     *t = {0, tm * BM, min(a.rows, (tm + 1) * BM)};
     return true;
   } else if (a.tiles) {
@@ -209,14 +212,16 @@ __device__ __forceinline__ bool row_tile(const ProductArgs& a, int tm, RowTile* 
 }
 
 // Workgroup -> (row tile, column tile). Workgroup i runs on XCD i mod 8; every XCD takes a
-// contiguous eighth of the tiles, so those that share weights or rows of x meet in its L2. Column
-// tiles are innermost. False for the workgroups past the last tile (the grid of a grouped product
-// is sized for the most tiles that its rows can need).
+// contiguous eighth of the tiles, so those that share weights or rows of x meet in its L2. False for the workgroups past the last tile (the grid of a grouped product
+// is sized for the most tiles that its rows can need). kSplit: tm counts the row tiles of every part
+// of K in turn.
 template <int MODE>
 __device__ __forceinline__ bool tile_of_block(const ProductArgs& a, int* tm, int* tn) {
   int count;
   if constexpr (MODE == kDense)
     count = a.tiles_m;
+  else if constexpr (MODE == kSplit)
+    count = a.tiles_m * a.splits;
   else
     count = a.tiles ? *a.tile_count : a.rows;
   const int total = count * a.tiles_n;
@@ -224,8 +229,20 @@ __device__ __forceinline__ bool tile_of_block(const ProductArgs& a, int* tm, int
   const int i = static_cast<int>(blockIdx.x >> 3);
   const int lin = static_cast<int>(blockIdx.x & 7) * per + i;
   if (i >= per || lin >= total) return false;
-  *tm = lin / a.tiles_n;
-  *tn = lin - *tm * a.tiles_n;
+  if constexpr (MODE == kDense) {
+    // Column tiles in groups of eight, every row tile within a group: the 32 tiles that an XCD runs at
+    // once then read 4 x 8 tiles' rows instead of 2 x 16 (int8 8192 x 24576 x 4096 834 -> 788 us; 8192 x
+    // 4096 x 12288 and 6144 x 4096 the same within the noise).
+    constexpr int kGroup = 8;
+    const int group = lin / (kGroup * count);
+    const int wide = min(kGroup, a.tiles_n - group * kGroup);
+    const int in = lin - group * kGroup * count;
+    *tm = in / wide;
+    *tn = group * kGroup + in - *tm * wide;
+  } else {
+    *tm = lin / a.tiles_n;
+    *tn = lin - *tm * a.tiles_n;
+  }
   return true;
 }
 
@@ -260,6 +277,16 @@ __device__ __forceinline__ void barrier_after_reads() {
   asm volatile("" ::: "memory");
 }
 
+// At most `ahead` (up to MAX) steps of PER copies are still under way.
+template <int PER, int MAX>
+__device__ __forceinline__ void wait_steps(int ahead) {
+  static_assert(PER * MAX < 64, "vmcnt range");
+  if constexpr (MAX > 0) {
+    if (ahead < MAX) return wait_steps<PER, MAX - 1>(ahead);
+  }
+  wait_vmcnt<PER * MAX>();
+}
+
 // With SILU, rows 8 q .. 8 q + 7 of each 32-row block of the weight tile are gate rows for even q
 // and the matching up rows for odd q, so a lane holds gate and up of a column side by side.
 // Column of a tile row, relative to the tile's first column:
@@ -290,10 +317,18 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
 
   int tm, tn;
   if (!tile_of_block<MODE>(a, &tm, &tn)) return;
+  const int all_k = (a.k_bytes + kProdRow - 1) / kProdRow;
+  int first_k = 0, n_k = all_k, split = 0;
+  if constexpr (MODE == kSplit) {
+    split = tm / a.tiles_m;
+    tm -= split * a.tiles_m;
+    const int per = (all_k + a.splits - 1) / a.splits;
+    first_k = split * per;
+    n_k = min(per, all_k - first_k);
+  }
   RowTile t;
   if (!row_tile<MODE, BM>(a, tm, &t)) return;
   const int n0 = tn * kBnOut;
-  const int n_k = (a.k_bytes + kProdRow - 1) / kProdRow;
   const bool tail = a.k_bytes % kProdRow != 0;
 
   // Copy side: copy j of a wave covers tile rows 8 g .. 8 g + 7, g = wave + NW j (x rows first);
@@ -328,10 +363,10 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
   }
   auto issue = [&](int step, int stage) {
     const uint32_t dst = lds_base + stage * kStage + wave * 1024;
-    const int64_t k = static_cast<int64_t>(step) * kProdRow;
+    const int64_t k = static_cast<int64_t>(first_k + step) * kProdRow;
     const uint8_t* xb = x_base + k;
     const uint8_t* wb = w_base + k;
-    if (tail && step == n_k - 1) {
+    if (tail && first_k + step == all_k - 1) {
       // chunks past K come as zeros in both operands
 #pragma unroll
       for (int j = 0; j < kCopies; ++j) {
@@ -382,7 +417,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
 #pragma unroll
   for (int s = 0; s < STAGES; ++s)
     if (s < n_k) issue(s, s);
-  wait_tiles_ahead<kCopies, STAGES - 1>(min(STAGES - 1, n_k - 1));
+  wait_steps<kCopies, STAGES - 1>(min(STAGES - 1, n_k - 1));
   barrier_after_reads();
   read(0, 0, 0);
   int stage = 0;
@@ -393,7 +428,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
         read(stage, kk + 1, (kk + 1) & 1);
       } else if (step + 1 < n_k) {
         // The next step's copies are in, every wave has read this one: its buffer is free.
-        wait_tiles_ahead<kCopies, STAGES - 2>(min(STAGES - 2, n_k - 2 - step));
+        wait_steps<kCopies, STAGES - 2>(min(STAGES - 2, n_k - 2 - step));
         barrier_after_reads();
         if (step + STAGES < n_k) issue(step + STAGES, stage);
         stage = stage == STAGES - 1 ? 0 : stage + 1;
@@ -410,12 +445,26 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
   // A lane holds x row `col` of each B block and weight rows 8 q + 4 half + e of each A block in
   // accumulator elements 4 q + e.
   const float* w_scales = nullptr;
-  if constexpr (IN == kInt8)
+  if constexpr (IN == kInt8 && MODE != kSplit)
     w_scales = a.w_scales + static_cast<int64_t>(t.expert) * (SILU ? 2 : 1) * a.columns;
 #pragma unroll
   for (int j = 0; j < B_BLK; ++j) {
     const int row = t.begin + wm * kWaveM + 32 * j + col;
     if (row >= t.end) continue;
+    if constexpr (MODE == kSplit) {
+      int* out = static_cast<int*>(a.out) + (static_cast<int64_t>(split) * a.rows + row) * a.ldo;
+#pragma unroll
+      for (int i = 0; i < A_BLK; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int column = n0 + wn * kWaveN + 32 * i + 8 * q + 4 * half;
+          if (column < a.columns)  // ldo is a multiple of 4
+            *reinterpret_cast<int4*>(out + column) =
+                make_int4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                          acc[i][j][4 * q + 3]);
+        }
+      continue;
+    }
     const RowOut r = row_out<IN, MODE>(a, row);
 #pragma unroll
     for (int i = 0; i < A_BLK; ++i)
@@ -555,7 +604,7 @@ __device__ __forceinline__ void large_loop(const ProductArgs& a, const RowTile& 
     if (s < n_k)
 #pragma unroll
       for (int j = 0; j < kCopies; ++j) copy(s, lds_base + s * kStage, j);
-  wait_tiles_ahead<kCopies, S - 1>(min(S - 1, n_k - 1));
+  wait_steps<kCopies, S - 1>(min(S - 1, n_k - 1));
   barrier();
 #pragma unroll
   for (int f = 0; f < kReads; ++f) read(lds, 0, f);
@@ -569,7 +618,7 @@ __device__ __forceinline__ void large_loop(const ProductArgs& a, const RowTile& 
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       if (kk == 3 && more) {  // the next step is in and this one is read: its buffer is free
-        wait_tiles_ahead<kCopies, S - 2>(min(S - 2, n_k - 2 - step));
+        wait_steps<kCopies, S - 2>(min(S - 2, n_k - 2 - step));
         barrier();
       }
 #pragma unroll
@@ -734,7 +783,7 @@ __global__ __launch_bounds__(64 * NW, 1) void product_large(ProductArgs a) {
 // in LDS. A lane's operand rows are lane % 16; of a 128-byte step it holds bytes 32 g .. 32 g + 31,
 // g = lane / 16, as two operands: K is summed in another order than it is stored, the same one in
 // both operands, so whole 128-byte lines are read.
-template <int IN, int OT, int MODE, bool SILU, int NB, int DEPTH>
+template <int IN, int OT, bool SILU, int NB, int DEPTH>
 __global__ __launch_bounds__(256) void product_rows(ProductArgs a) {
   static_assert(!SILU || NB == 2, "a gate and an up block");
   constexpr int kOut = SILU ? 16 : 16 * NB;
@@ -746,21 +795,20 @@ __global__ __launch_bounds__(256) void product_rows(ProductArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
   int tm, tn;
-  if (!tile_of_block<MODE>(a, &tm, &tn)) return;
+  if (!tile_of_block<kDense>(a, &tm, &tn)) return;
   RowTile t;
-  if (!row_tile<MODE, 16>(a, tm, &t)) return;
+  if (!row_tile<kDense, 16>(a, tm, &t)) return;
   const int n0 = tn * kOut;
   const int r = lane & 15, g = lane >> 4;
 
   const int m = min(t.begin + r, t.end - 1);
   const uint8_t* x_row =
-      a.x + static_cast<int64_t>(source_row(a, m, MODE == kGateUp)) * a.x_stride + g * 32;
+      a.x + static_cast<int64_t>(m) * a.x_stride + g * 32;
   const uint8_t* w_row[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int c = min(n0 + (SILU ? 0 : 16 * b) + r, a.columns - 1);
-    w_row[b] = a.w + t.expert * a.w_expert +
-               static_cast<int64_t>(SILU && b ? a.columns + c : c) * a.w_stride + g * 32;
+    w_row[b] = a.w + static_cast<int64_t>(SILU && b ? a.columns + c : c) * a.w_stride + g * 32;
   }
   const int n_k = (a.k_bytes + kProdRow - 1) / kProdRow;
   const int per = (n_k + 3) >> 2;
@@ -816,10 +864,8 @@ __global__ __launch_bounds__(256) void product_rows(ProductArgs a) {
   if (wave >= (SILU ? 1 : NB)) return;
   const int row = t.begin + r;
   if (row >= t.end) return;
-  const RowOut ro = row_out<IN, MODE>(a, row);
-  const float* w_scales = nullptr;
-  if constexpr (IN == kInt8)
-    w_scales = a.w_scales + static_cast<int64_t>(t.expert) * (SILU ? 2 : 1) * a.columns;
+  const RowOut ro = row_out<IN, kDense>(a, row);
+  const float* w_scales = IN == kInt8 ? a.w_scales : nullptr;
   auto total = [&](int b, typename M::Scalar(&v)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -829,7 +875,41 @@ __global__ __launch_bounds__(256) void product_rows(ProductArgs a) {
   typename M::Scalar v[4], u[4] = {};
   total(SILU ? 0 : wave, v);
   if constexpr (SILU) total(NB - 1, u);
-  finish4<IN, OT, MODE, SILU>(a, ro, n0 + (SILU ? 0 : 16 * wave) + 4 * g, w_scales, v, u);
+  finish4<IN, OT, kDense, SILU>(a, ro, n0 + (SILU ? 0 : 16 * wave) + 4 * g, w_scales, v, u);
+}
+
+// ---------------------------------------------------------------------------- the choice of tiles
+// The tiles that a product can take, smallest first.
+enum class Tile { k64, k128, k256x128, k256 };
+
+struct TileShape {
+  int bm, bn;        // rows of x, weight rows
+  float step, busy;  // us a 128-byte step: with few workgroups, and what a full chip adds
+};
+constexpr TileShape kTileShapes[] = {
+    {64, 64, 0.29f, 0.f}, {128, 128, 0.5f, 0.2f}, {256, 128, 0.8f, 0.3f}, {256, 256, 1.2f, 0.6f}};
+
+// Estimated time in us of `row_tiles` x `column_tiles` tiles over K. A CU's copies into LDS come at
+// about 60 GB/s where they miss L2, whatever the depth of the ring, which makes the step of a tile
+// its bytes; one workgroup a CU, but two of 64 x 64. A 256 x 256 tile of up to 128 rows runs as half a
+// tile. Weights come at 5.8 TB/s at most. Measured, int8: 4096 x 4096 at 64 rows 64 x 64 tiles 13.0 us,
+// 128 x 128 19.5, 256 x 256 25.2; 6144 x 4096 at 512 rows 33.9 / 25.2 / 34.4 (256 x 128) / 47.2, at 1,024
+// rows 62 / 54 / 37.5 / 49, at 2,048 rows 118 / 79 / 76 / 56. bf16 experts 128 x (1536 x 2048) at 64 rows
+// each 202 / 182 / 221 / 187, at 128 rows 296 / 229 / 239 / 208.
+inline float tile_estimate(Tile tile, float row_tiles, float column_tiles, int64_t k_bytes,
+                           float weight_bytes, bool half, int cus) {
+  const TileShape& t = kTileShapes[static_cast<int>(tile)];
+  const float r = row_tiles * column_tiles / static_cast<float>(cus);
+  const float busy = std::min(r, 1.f);
+  float step = t.step + t.busy * busy, rounds = 1.f;
+  if (tile == Tile::k256 && half) step = 0.65f + 0.8f * busy;
+  if (tile == Tile::k64) {
+    if (r > 1.f) rounds = std::max(1.07f * r - 0.07f, std::min(2.f, 1.f + 2.5f * (r - 1.f)));
+  } else if (r > 1.06f) {
+    rounds = r <= 3.f ? std::ceil(r - 0.06f) : r + 0.3f;
+  }
+  const float steps = static_cast<float>((k_bytes + kProdRow - 1) / kProdRow);
+  return 3.3f + std::max(steps * step * rounds, weight_bytes / 5.8e6f);
 }
 
 }  // namespace mi355x

@@ -84,20 +84,84 @@ constexpr int64_t kMaxInt8K = 131072;  // 127 * 127 * K stays inside int32
 
 int64_t padded16(int64_t n) { return (n + 15) / 16 * 16; }
 
-struct Int8Workspace {
-  int64_t values, scales, bytes;
+// How a product is computed.
+struct Int8Plan {
+  enum Kind { kVec, kRows, kTiles } kind;
+  Tile tile;
+  int splits;  // parts of K, summed by a pass of their own where there are several
 };
 
-// One or two rows are quantised inside the product (see product_vec.h) where they fit its LDS.
-bool on_vector_math(int64_t M, int64_t K) { return M <= 2 && M * padded16(K) <= kVecLds; }
+// One or two rows go to vector math, which quantises them itself, where they fit its LDS; up to 16 to
+// the rows kernel or the least estimate of the tiles. K is split where the tiles leave CUs without
+// one: 4096 x 12288 at 64 rows 33 us whole. The rows kernel's step is 0.18 us a round of 32 columns a
+// CU (4096 x 4096 at 16 rows 8.5 us, 4096 x 12288 22, 24576 x 4096 22).
+Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, int cus) {
+  if (M <= 2 && M * padded16(K) <= kVecLds) return {Int8Plan::kVec, Tile::k64, 1};
+  Int8Plan best{Int8Plan::kTiles, Tile::k64, 1};
+  float best_us = 1e30f;
+  const int64_t kb = padded16(K), steps = (kb + kProdRow - 1) / kProdRow;
+  const float weights = static_cast<float>(N) * static_cast<float>(kb);
+  if (M <= 16) {
+    const float rounds = std::max(1.f, 1.1f * static_cast<float>(N) / (32.f * cus));
+    best = {Int8Plan::kRows, Tile::k64, 1};
+    best_us = 3.f + std::max(0.18f * steps * rounds, weights / 5.8e6f);
+  }
+  for (int i = 0; i < 4; ++i) {
+    const TileShape& t = kTileShapes[i];
+    const float tm = static_cast<float>((M + t.bm - 1) / t.bm);
+    const float tn = static_cast<float>((N + t.bn - 1) / t.bn);
+    for (int s = 1; s <= (i < 2 ? 8 : 1); s *= 2) {
+      const int64_t per = (steps + s - 1) / s;
+      if (s > 1 && (per < 4 || per * (s - 1) >= steps || tm * tn * (s / 2) >= cus)) break;
+      float us = tile_estimate(static_cast<Tile>(i), tm * s, tn, per * kProdRow, weights,
+                               M % 256 != 0 && M % 256 <= 128 && M < 256, cus);
+      // the sums go out and come back at about 4.5 TB/s, in one more launch
+      if (s > 1) us += 2.5f + 8e-6f / 4.5f * static_cast<float>(s * M * N);
+      if (us < best_us) {
+        best_us = us;
+        best = {Int8Plan::kTiles, static_cast<Tile>(i), s};
+      }
+    }
+  }
+  return best;
+}
 
-Int8Workspace int8_workspace(int64_t M, int64_t K) {
+struct Int8Workspace {
+  int64_t values, scales, sums, bytes;
+};
+
+Int8Workspace int8_workspace(int64_t M, int64_t N, int64_t K, const Int8Plan& p) {
   Int8Workspace w{};
-  if (on_vector_math(M, K)) return w;
+  if (p.kind == Int8Plan::kVec) return w;
   w.values = 0;
   w.scales = padded16(M * padded16(K));
-  w.bytes = w.scales + padded16(M * 4);
+  w.sums = w.scales + padded16(M * 4);
+  w.bytes = w.sums + (p.splits > 1 ? p.splits * M * (N + 3) / 4 * 4 * 4 + 64 : 0);
   return w;
+}
+
+// out from the int32 sums of the parts of K, four columns a thread.
+template <int OT, bool SILU>
+__global__ __launch_bounds__(256) void finish_splits(ProductArgs a, const int* __restrict__ sums,
+                                                     int64_t lds) {
+  const int quads = (a.columns + 3) / 4;
+  const int64_t i = blockIdx.x * int64_t(256) + threadIdx.x;
+  if (i >= static_cast<int64_t>(a.rows) * quads) return;
+  const int row = static_cast<int>(i / quads);
+  const int c = static_cast<int>(i - static_cast<int64_t>(row) * quads) * 4;
+  const int64_t plane = static_cast<int64_t>(a.rows) * lds;
+  const int* p = sums + row * lds + c;
+  int v[4] = {}, u[4] = {};
+  for (int s = 0; s < a.splits; ++s, p += plane) {
+    const int4 g = *reinterpret_cast<const int4*>(p);
+    v[0] += g.x, v[1] += g.y, v[2] += g.z, v[3] += g.w;
+    if constexpr (SILU) {  // the up columns start anywhere; those past the end repeat the last one
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] += p[a.columns + min(e, a.columns - 1 - c)];
+    }
+  }
+  const RowOut r{row, a.x_scales[row], 1.f};
+  finish4<kInt8, OT, kDense, SILU>(a, r, c, a.w_scales, v, u);
 }
 
 template <int OT, bool SILU>
@@ -115,27 +179,52 @@ void launch_int8_vec(const ProductArgs& base, int64_t M, int64_t columns, int wi
     product_vec<kInt8, OT, OT, kDense, SILU, 2, kRows, kWaves><<<g, 64 * kWaves, 0, s>>>(a, width, vec);
 }
 
-template <int OT, bool SILU>
-void launch_int8(const ProductArgs& base, int64_t M, int64_t columns, hipStream_t s) {
-  ProductArgs a = base;
-  auto grid = [&](int bm, int bn) {
-    a.tiles_m = static_cast<int32_t>((M + bm - 1) / bm);
-    a.tiles_n = static_cast<int32_t>((columns + bn - 1) / bn);
-    return dim3(static_cast<uint32_t>((int64_t(a.tiles_m) * a.tiles_n + 7) / 8 * 8));
-  };
-  if (M <= 16) {
-    const dim3 g = grid(16, SILU ? 16 : 32);
-    product_rows<kInt8, OT, kDense, SILU, 2, 4><<<g, 256, 0, s>>>(a);
-  } else if (M <= 256) {
-    const dim3 g = grid(64, SILU ? 32 : 64);
-    product_tile<kInt8, OT, kDense, SILU, 64, 64, 2, 2, 4><<<g, 256, 0, s>>>(a);
-  } else {
-    const dim3 g = grid(256, SILU ? 128 : 256);
-    if (a.k_bytes % kProdRow)
-      product_large<kInt8, OT, kDense, SILU, 256, 8, true><<<g, 512, 0, s>>>(a);
+template <int OT, int MODE, bool SILU>
+void launch_int8_tiles(ProductArgs& a, Tile tile, hipStream_t s) {
+  const TileShape& t = kTileShapes[static_cast<int>(tile)];
+  const int bn = SILU ? t.bn / 2 : t.bn;
+  a.tiles_m = (a.rows + t.bm - 1) / t.bm;
+  a.tiles_n = (a.columns + bn - 1) / bn;
+  const dim3 g(static_cast<uint32_t>((int64_t(a.tiles_m) * a.tiles_n * a.splits + 7) / 8 * 8));
+  if (tile == Tile::k64) {
+    product_tile<kInt8, OT, MODE, SILU, 64, 64, 2, 2, 4><<<g, 256, 0, s>>>(a);
+  } else if (tile == Tile::k128) {
+    product_tile<kInt8, OT, MODE, SILU, 128, 128, 4, 2, 4><<<g, 512, 0, s>>>(a);
+  } else if constexpr (MODE == kDense) {
+    if (tile == Tile::k256x128)
+      product_tile<kInt8, OT, MODE, SILU, 256, 128, 4, 2, 3><<<g, 512, 0, s>>>(a);
+    else if (a.k_bytes % kProdRow)
+      product_large<kInt8, OT, MODE, SILU, 256, 8, true><<<g, 512, 0, s>>>(a);
     else
-      product_large<kInt8, OT, kDense, SILU, 256, 8, false><<<g, 512, 0, s>>>(a);
+      product_large<kInt8, OT, MODE, SILU, 256, 8, false><<<g, 512, 0, s>>>(a);
   }
+}
+
+template <int OT, bool SILU>
+const char* launch_int8(const ProductArgs& base, const Int8Plan& p, int* sums, hipStream_t s) {
+  ProductArgs a = base;
+  a.splits = p.splits;
+  if (p.kind == Int8Plan::kRows) {
+    const int bn = SILU ? 16 : 32;
+    a.tiles_m = 1;
+    a.tiles_n = (a.columns + bn - 1) / bn;
+    product_rows<kInt8, OT, SILU, 2, 4>
+        <<<dim3(static_cast<uint32_t>((a.tiles_n + 7) / 8 * 8)), 256, 0, s>>>(a);
+  } else if (p.splits == 1) {
+    launch_int8_tiles<OT, kDense, SILU>(a, p.tile, s);
+  } else {
+    ProductArgs parts = a;
+    parts.out = sums;
+    parts.columns = SILU ? 2 * a.columns : a.columns;
+    parts.ldo = (parts.columns + 3) / 4 * 4;
+    launch_int8_tiles<OT, kSplit, false>(parts, p.tile, s);
+    if (const char* e = launch_status("product (int8)")) return e;
+    const int64_t threads = static_cast<int64_t>(a.rows) * ((a.columns + 3) / 4);
+    finish_splits<OT, SILU><<<dim3(static_cast<uint32_t>((threads + 255) / 256)), 256, 0, s>>>(
+        a, sums, parts.ldo);
+    return launch_status("finish_splits");
+  }
+  return launch_status("product (int8)");
 }
 
 }  // namespace
@@ -174,15 +263,19 @@ extern "C" const char* mi355x_quantize_rows(const void* x, int64_t ldx, void* va
                            static_cast<hipStream_t>(stream));
 }
 
-extern "C" int64_t mi355x_linear_int8_workspace_bytes(int64_t M, int64_t K) {
-  if (M < 0 || K <= 0 || K > kMaxInt8K || M > (int64_t(1) << 24)) return -1;
-  return int8_workspace(M, K).bytes;
+extern "C" int64_t mi355x_linear_int8_workspace_bytes(int64_t M, int64_t N, int64_t K,
+                                                      int32_t cus) {
+  if (M < 0 || N <= 0 || K <= 0 || K > kMaxInt8K || M > (int64_t(1) << 24) ||
+      N > (int64_t(1) << 24))
+    return -1;
+  return M == 0 ? 0 : int8_workspace(M, N, K, int8_plan(M, N, K, cus > 0 ? cus : 256)).bytes;
 }
 
 extern "C" const char* mi355x_linear_int8(const void* x, int64_t ldx, const void* w, int64_t ldw,
                                           const float* w_scales, void* out, int64_t ldo, int64_t M,
                                           int64_t N, int64_t K, bool silu_mul, void* workspace,
-                                          int64_t workspace_bytes, int64_t dtype, void* stream) {
+                                          int64_t workspace_bytes, int32_t cus, int64_t dtype,
+                                          void* stream) {
   const int64_t columns = silu_mul ? N / 2 : N;
   if (M < 0 || N <= 0 || K <= 0 || K > kMaxInt8K || N > (int64_t(1) << 24) ||
       M > (int64_t(1) << 24) || (silu_mul && N % 2) || ldx < K || ldo < columns ||
@@ -191,7 +284,8 @@ extern "C" const char* mi355x_linear_int8(const void* x, int64_t ldx, const void
     return set_error("mi355x_linear_int8: unsupported shape (K up to 131072, weight rows of whole "
                      "16-byte words, less than 4 GiB)");
   if (M == 0) return nullptr;
-  const Int8Workspace ws = int8_workspace(M, K);
+  const Int8Plan plan = int8_plan(M, N, K, cus > 0 ? cus : 256);
+  const Int8Workspace ws = int8_workspace(M, N, K, plan);
   if (!x || !w || !w_scales || !out || (!workspace && ws.bytes))
     return set_error("mi355x_linear_int8: null pointer");
   if (!aligned(x, 2) || !aligned(w, 16) || !aligned(w_scales, 4) || !aligned(out, 2) ||
@@ -213,7 +307,7 @@ extern "C" const char* mi355x_linear_int8(const void* x, int64_t ldx, const void
   a.k_bytes = static_cast<int32_t>(padded16(K));
   a.vec_out = ldo % 4 == 0 && aligned(out, 8);
   a.vec16_out = ldo % 8 == 0 && aligned(out, 16);
-  if (on_vector_math(M, K)) {
+  if (plan.kind == Int8Plan::kVec) {
     a.x = static_cast<const uint8_t*>(x);
     a.x_stride = ldx * 2;
     const bool vec = aligned(x, 16) && ldx % 8 == 0;
@@ -234,9 +328,8 @@ extern "C" const char* mi355x_linear_int8(const void* x, int64_t ldx, const void
   a.x = base;
   a.x_scales = scales;
   a.x_stride = padded16(K);
+  int* sums = reinterpret_cast<int*>(base + ws.sums);
   if (dtype == 0)
-    silu_mul ? launch_int8<0, true>(a, M, columns, s) : launch_int8<0, false>(a, M, columns, s);
-  else
-    silu_mul ? launch_int8<1, true>(a, M, columns, s) : launch_int8<1, false>(a, M, columns, s);
-  return launch_status("product (int8)");
+    return silu_mul ? launch_int8<0, true>(a, plan, sums, s) : launch_int8<0, false>(a, plan, sums, s);
+  return silu_mul ? launch_int8<1, true>(a, plan, sums, s) : launch_int8<1, false>(a, plan, sums, s);
 }

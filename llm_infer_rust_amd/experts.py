@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import torch
 
-from ._native import NativeError, check, lib, on_device, stream_of
+from ._native import NativeError, check, device_cus, lib, on_device, stream_of
 from .int8 import _ROW_DTYPES, Int8Weight, _check_rows, _refuse_grad, _row_stride
 
 MAX_EXPERTS = 1024
@@ -107,7 +107,7 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
             gate_up.row_stride if int8 else h, gate_up.scales.data_ptr() if int8 else None,
             dn.data_ptr(), down.row_stride if int8 else inter,
             down.scales.data_ptr() if int8 else None, out.data_ptr(), _row_stride(out), t, top_k,
-            e, h, inter, ws.data_ptr(), need, dt, stream_of(x)), "expert_mlp")
+            e, h, inter, ws.data_ptr(), need, device_cus(x.device), dt, stream_of(x)), "expert_mlp")
     return out
 
 

@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import torch
 
-from ._native import NativeError, check, lib, on_device, stream_of
+from ._native import NativeError, check, device_cus, lib, on_device, stream_of
 
 _ROW_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_K = 131072  # 127 * 127 * K stays inside int32
@@ -151,14 +151,15 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = 
         elif (out.shape != (t, width) or out.dtype != x.dtype or out.device != x.device
               or (width > 1 and out.stride(1) != 1) or (t > 1 and out.stride(0) < width)):
             raise NativeError("linear_int8: invalid output")
-        need = lib().mi355x_linear_int8_workspace_bytes(t, k)
+        cus = device_cus(x.device)
+        need = lib().mi355x_linear_int8_workspace_bytes(t, n, k, cus)
         if need < 0:
             raise NativeError("linear_int8: invalid shape")
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         check(lib().mi355x_linear_int8(x.data_ptr(), _row_stride(x), weight.values.data_ptr(),
                                        weight.row_stride, weight.scales.data_ptr(),
                                        out.data_ptr(), _row_stride(out), t, n, k, silu_mul,
-                                       None if ws is None else ws.data_ptr(), need, dt,
+                                       None if ws is None else ws.data_ptr(), need, cus, dt,
                                        stream_of(x)), "linear_int8")
     return out
 

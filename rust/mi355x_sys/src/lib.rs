@@ -89,10 +89,10 @@ unsafe extern "C" {
     pub fn mi355x_quantize_rows(x: *const c_void, ldx: i64, values: *mut c_void, ldv: i64,
         scales: *mut c_void, rows: i64, width: i64, dtype: c_int,
         stream: *mut c_void) -> *const c_char;
-    pub fn mi355x_linear_int8_workspace_bytes(m: i64, k: i64) -> i64;
+    pub fn mi355x_linear_int8_workspace_bytes(m: i64, n: i64, k: i64, cus: i32) -> i64;
     pub fn mi355x_linear_int8(x: *const c_void, ldx: i64, w: *const c_void, ldw: i64,
         w_scales: *const f32, out: *mut c_void, ldo: i64, m: i64, n: i64, k: i64,
-        silu_mul: bool, workspace: *mut c_void, workspace_bytes: i64, dtype: i64,
+        silu_mul: bool, workspace: *mut c_void, workspace_bytes: i64, cus: i32, dtype: i64,
         stream: *mut c_void) -> *const c_char;
     pub fn mi355x_route_experts(logits: *const c_void, ld: i64, weights: *mut c_void, ids: *mut i32,
         tokens: i64, experts: i64, top_k: i64, normalize: bool, dtype: c_int,
@@ -103,7 +103,7 @@ unsafe extern "C" {
         gate_up: *const c_void, ld_gate_up: i64, gate_up_scales: *const f32,
         down: *const c_void, ld_down: i64, down_scales: *const f32, out: *mut c_void, ldo: i64,
         tokens: i64, top_k: i64, experts: i64, hidden: i64, inter: i64,
-        workspace: *mut c_void, workspace_bytes: i64, dtype: i64,
+        workspace: *mut c_void, workspace_bytes: i64, cus: i32, dtype: i64,
         stream: *mut c_void) -> *const c_char;
     pub fn mi355x_sample(logits: *const c_void, rows: i64, vocab: i64, row_stride: i64,
         dtype: c_int, temperature: *const f32, top_k: *const i32, top_p: *const f32,
