@@ -1,4 +1,4 @@
-"""Dense Qwen3 decoder on the gfx950 kernels (the model the attention path serves).
+"""Qwen3 decoder on the gfx950 kernels (the model the attention path serves).
 
 Follows the reference layer sequence (``src/models/qwen3/model.rs:155-534``):
 
@@ -17,6 +17,10 @@ store pass, o_proj and down fused with the residual RMSNorm that follows them) a
 fused with SiLU x mul, as does the lm_head of up to 64 rows; prefill-sized products and larger
 heads are library GEMMs (torch -> hipBLASLt). Everything around them is this library's HIP code.
 Configuration fields and defaults follow ``src/models/qwen3/config.rs:9-42``.
+
+Two variants that the reference does not have: with ``num_experts`` every layer's MLP is one of
+routed experts (``experts.route_experts``, ``experts.expert_mlp``) in place of the dense one, and
+``Qwen3Model.quantize_int8`` turns the layers' matrices into 8-bit ones.
 """
 from __future__ import annotations
 
@@ -25,8 +29,9 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
-from . import ops
+from . import experts, ops
 from .backend import Attention, AttentionBatch, AttentionSpec
+from .int8 import Int8Weight
 from .kv_cache import BaseAttention, ModelError
 
 
@@ -43,6 +48,12 @@ class Qwen3Config:
     rope_theta: float = 10_000.0
     rms_norm_eps: float = 1e-6
     tie_word_embeddings: bool = False
+    # Experts of every layer's MLP (0: a dense MLP of intermediate_size), how many of them a token
+    # is routed to, their width, and whether the chosen weights are normalised to sum to 1.
+    num_experts: int = 0
+    num_experts_per_tok: int = 0
+    moe_intermediate_size: int = 0
+    norm_topk_prob: bool = True
 
     @staticmethod
     def qwen3_8b() -> "Qwen3Config":
@@ -60,6 +71,10 @@ class Qwen3Config:
             raise ModelError("Qwen3 dimensions must be positive")
         if self.num_attention_heads % self.num_kv_heads:
             raise ModelError("num_attention_heads must be a multiple of num_kv_heads")
+        if self.num_experts and not (
+                0 < self.num_experts <= experts.MAX_EXPERTS and self.moe_intermediate_size > 0
+                and 0 < self.num_experts_per_tok <= min(self.num_experts, experts.MAX_TOP_K)):
+            raise ModelError("invalid expert count, experts per token or expert width")
 
     @property
     def qkv_width(self) -> int:
@@ -75,12 +90,19 @@ class Qwen3Layer:
         self.k_norm = torch.ones(d, dtype=dtype, device=device)
         self.o_proj = torch.empty(h, cfg.num_attention_heads * d, dtype=dtype, device=device)
         self.post_attention_layernorm = torch.ones(h, dtype=dtype, device=device)
-        self.gate_up_proj = torch.empty(2 * cfg.intermediate_size, h, dtype=dtype, device=device)
-        self.down_proj = torch.empty(h, cfg.intermediate_size, dtype=dtype, device=device)
+        # A dense MLP's matrices, or those of all experts ([E, 2 I, h], [E, h, I]) and their router.
+        lead, f = (), cfg.intermediate_size
+        self.router: torch.Tensor | None = None
+        if cfg.num_experts:
+            lead, f = (cfg.num_experts,), cfg.moe_intermediate_size
+            self.router = torch.empty(cfg.num_experts, h, dtype=dtype, device=device)
+        self.gate_up_proj = torch.empty(*lead, 2 * f, h, dtype=dtype, device=device)
+        self.down_proj = torch.empty(*lead, h, f, dtype=dtype, device=device)
         self.base_attention = BaseAttention()
 
     def matrices(self) -> list[torch.Tensor]:
-        return [self.qkv_proj, self.o_proj, self.gate_up_proj, self.down_proj]
+        router = [] if self.router is None else [self.router]
+        return [self.qkv_proj, self.o_proj, *router, self.gate_up_proj, self.down_proj]
 
 
 class Qwen3Model:
@@ -129,14 +151,32 @@ class Qwen3Model:
             out[p + "self_attn.k_norm.weight"] = layer.k_norm
             out[p + "self_attn.o_proj.weight"] = layer.o_proj
             out[p + "post_attention_layernorm.weight"] = layer.post_attention_layernorm
-            out[p + "mlp.gate_up_proj.weight"] = layer.gate_up_proj
-            out[p + "mlp.down_proj.weight"] = layer.down_proj
+            if layer.router is None:
+                out[p + "mlp.gate_up_proj.weight"] = layer.gate_up_proj
+                out[p + "mlp.down_proj.weight"] = layer.down_proj
+            else:
+                out[p + "mlp.gate.weight"] = layer.router
+                out[p + "mlp.experts.gate_up_proj"] = layer.gate_up_proj
+                out[p + "mlp.experts.down_proj"] = layer.down_proj
         return out
+
+    def quantize_int8(self) -> "Qwen3Model":
+        """The layers' QKV, o, gate_up and down matrices (those of experts too) in 8 bits, one scale
+        a row; embeddings, norms, routers and the head stay as they are. Done once, after the
+        weights are loaded, and before a decode graph is captured over them."""
+        for layer in self.layers:
+            for name in ("qkv_proj", "o_proj", "gate_up_proj", "down_proj"):
+                weight = getattr(layer, name)
+                if not isinstance(weight, Int8Weight):
+                    setattr(layer, name, Int8Weight.quantize(weight))
+        return self
 
     def load_weights(self, weights) -> int:
         """Copy tensors by Hugging Face name (``named_parameters`` names); every parameter must
         be supplied with its exact shape (src/models/qwen3/model.rs:231-300). Returns the count."""
         params = self.named_parameters()
+        if any(isinstance(p, Int8Weight) for p in params.values()):
+            raise ModelError("weights are loaded before they are quantised")
         loaded = 0
         for name, value in weights.items():
             if name not in params:
@@ -195,9 +235,15 @@ class Qwen3Model:
             # norm after the last layer): each a projection fused with its residual RMSNorm.
             x, residual = ops.linear_add_rms_norm(attn, layer.o_proj, residual,
                                                   layer.post_attention_layernorm, eps)
+            next_norm = self.layers[i + 1].input_layernorm if i + 1 < n_layers else self.norm
+            if layer.router is not None:
+                weights, ids = experts.route_experts(ops.linear(x, layer.router),
+                                                     cfg.num_experts_per_tok, cfg.norm_topk_prob)
+                x = experts.expert_mlp(x, ids, weights, layer.gate_up_proj, layer.down_proj)
+                x, residual = ops.add_rms_norm(x, residual, next_norm, eps)
+                continue
             # gate_up with SiLU x mul (one launch for decode batches)
             act = ops.linear_silu_mul(x, layer.gate_up_proj)
-            next_norm = self.layers[i + 1].input_layernorm if i + 1 < n_layers else self.norm
             x, residual = ops.linear_add_rms_norm(act, layer.down_proj, residual, next_norm, eps)
         hidden = x
         if logits_indices is not None:

@@ -17,6 +17,9 @@ and ``src/layers/ops.rs:53-127``:
   as one pass (``src/models/qwen3/model.rs:478-514``).
 
 Only CUDA(HIP) bfloat16/float16 tensors are accepted; anything else raises.
+
+The projections take a weight in 8 bits (``int8.Int8Weight``) as well: the product then runs in
+8-bit integers (``int8.linear_int8``) and what follows it as a pass of its own.
 """
 from __future__ import annotations
 
@@ -26,6 +29,7 @@ import torch
 
 from . import _native
 from ._native import NativeError, check, dtype_code, lib, stream_of
+from .int8 import Int8Weight, linear_int8
 
 
 def _require_device(t: torch.Tensor, what: str) -> None:
@@ -226,7 +230,8 @@ def linear_qk_norm_rope_store(x: torch.Tensor, weight: torch.Tensor, q_heads: in
     if q_heads <= 0 or k_heads <= 0 or n % (q_heads + 2 * k_heads):
         raise NativeError("QKV weight rows must be (q_heads + 2 k_heads) * head_dim")
     d = n // (q_heads + 2 * k_heads)  # head_dim
-    fused = (x.is_cuda and x.dim() == 2 and x.stride(1) == 1 and x.stride(0) % 8 == 0
+    fused = (not isinstance(weight, Int8Weight) and x.is_cuda and x.dim() == 2
+             and x.stride(1) == 1 and x.stride(0) % 8 == 0
              and weight.is_contiguous() and d == 128
              and uses_decode_kernel(m, n, k) and attention is not None
              and write_loc is not None and attention.is_bound() and rope_tables is not None)
@@ -356,6 +361,8 @@ def linear_add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.T
     products run as one projection plus one fused reduce/residual/norm pass (bit-identical to
     ``decode_linear`` then ``add_rms_norm``, also for the few rows of a long K that ``linear``
     leaves to hipBLASLt, whose sums run in another order); everything else runs the two steps."""
+    if isinstance(weight, Int8Weight):
+        return add_rms_norm(linear_int8(x, weight), residual, norm_weight, eps)
     m, k = (x.shape if x.dim() == 2 else (0, 0))
     n = weight.size(0)
     if (x.is_cuda and x.dim() == 2 and x.stride(1) == 1 and weight.is_contiguous()
@@ -422,6 +429,8 @@ def decode_linear_silu_mul(x: torch.Tensor, weight: torch.Tensor,
 def linear_silu_mul(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     """The MLP's ``silu_and_mul(linear(x, gate_up))`` (``mlp.rs``, ``ops.rs:53-61``):
     decode-sized products in one fused launch, the rest as the two steps."""
+    if isinstance(weight, Int8Weight):
+        return linear_int8(x, weight, silu_mul=True)
     if (x.is_cuda and x.dim() == 2 and x.stride(1) == 1 and weight.is_contiguous()
             and weight.size(0) % 2 == 0
             and uses_silu_kernel(x.size(0), weight.size(0) // 2, x.size(1))):
@@ -475,6 +484,8 @@ def head_linear(x: torch.Tensor, weight: torch.Tensor,
 def linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     """``x @ weight.T``: decode-sized products on the gfx950 kernel, the rest on
     hipBLASLt (``src/layers/linear.rs:5-7``)."""
+    if isinstance(weight, Int8Weight):
+        return linear_int8(x, weight)
     if (x.is_cuda and x.dim() == 2 and x.stride(1) == 1 and weight.is_contiguous()
             and uses_decode_kernel(x.size(0), weight.size(0), x.size(1))):
         return decode_linear(x, weight)
@@ -483,6 +494,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
 
 __all__ = ["rms_norm", "add_rms_norm", "qk_norm", "silu_and_mul", "linear_silu_mul",
            "HalfSplitRope", "rope", "qk_norm_rope_store", "decode_linear", "linear",
-           "head_linear", "linear_add_rms_norm", "decode_linear_silu_mul",
+           "head_linear", "linear_add_rms_norm", "decode_linear_silu_mul", "Int8Weight",
+           "linear_int8",
            "uses_decode_kernel", "NativeError",
            "_native"]
