@@ -392,10 +392,12 @@ int64_t mi355x_expert_mlp_workspace_bytes(int64_t tokens, int64_t top_k, int64_t
  * twice in a row.
  *
  * Scales NULL: weights of x's type. hidden, inter and ldx are multiples of 8 and rows are 16-byte
- * aligned. Sums in fp32; silu(g) * u and the weighted slot outputs are rounded to x's type.
+ * aligned. Sums in fp32; silu(g) * u is rounded to x's type.
  * Scales given (fp32 [experts, 2 inter] and [experts, hidden]): int8 weights. x is quantised once
  * a token, silu(g) * u (kept in fp32) once a slot, both as mi355x_quantize_rows does; any sizes and
  * x strides, weight rows of whole 16-byte words.
+ * Slot outputs on their way to the sum are held in 16 bits under a scale for every 32 columns (to
+ * 2^-15 of the largest of them, or in fp32 where there are up to 16 slots).
  * Nothing is read back to the host. An expert's weights are less than 4 GiB. Calls that overlap
  * need workspaces of their own. */
 const char* mi355x_expert_mlp(const void* x, int64_t ldx, const int32_t* ids,

@@ -240,45 +240,70 @@ __global__ __launch_bounds__(kGroupThreads) void place_slots(const int32_t* __re
 }
 
 // ---------------------------------------------------------------------------- the sum over slots
-// out[t] = sum of y[t * top_k + s] over the slots that take part, in fp32, s ascending.
+// out[t] = sum of y[t * top_k + s] (SlotCodes) over the slots that take part, in fp32, s ascending. A
+// thread takes 16 columns, half of what a scale covers. Bound by memory: an 8,192-token prefill of 8
+// slots and 2,048 columns reads 277 MB.
 template <int DT>
 __global__ __launch_bounds__(256) void sum_slots(const uint16_t* __restrict__ y, int64_t ldy,
+                                                 const uint16_t* __restrict__ scales,
+                                                 int64_t ld_scales,
                                                  const int32_t* __restrict__ ids,
                                                  uint16_t* __restrict__ out, int64_t ldo,
                                                  int64_t tokens, int top_k, int experts, int width,
                                                  bool vec) {
-  const int chunks = (width + 7) >> 3;
+  const int chunks = (width + 15) >> 4;
   const int64_t i = blockIdx.x * int64_t(256) + threadIdx.x;
   if (i >= tokens * chunks) return;
   const int64_t t = i / chunks;
-  const int c = static_cast<int>(i - t * chunks) * 8;
-  float sum[8] = {};
+  const int c = static_cast<int>(i - t * chunks) * 16;
+  float sum[2][8] = {};
   constexpr int kAtOnce = 8;  // slots whose loads are on their way together
   for (int s0 = 0; s0 < top_k; s0 += kAtOnce) {
     bool in[kAtOnce];
-    uint4 v[kAtOnce];
+    uint4 v[kAtOnce][2];
+    uint16_t scale[kAtOnce];
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i)
       in[i] = s0 + i < top_k && takes_part(ids[t * top_k + min(s0 + i, top_k - 1)], experts);
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i)
-      if (in[i]) v[i] = ld128(y + (t * top_k + s0 + i) * ldy + c);
+      if (in[i]) {
+        const int64_t slot = t * top_k + s0 + i;
+        v[i][0] = ld128_nt(y + slot * ldy + c);
+        v[i][1] = ld128_nt(y + slot * ldy + c + 8);
+        scale[i] = scales[slot * ld_scales + c / 32];
+      }
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
       if (!in[i]) continue;
-      float f[8];
-      unpack8<DT>(v[i], f);
+      const float unit = Elem<kBf16>::to_float(scale[i]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += f[e];
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t w[4] = {v[i][h].x, v[i][h].y, v[i][h].z, v[i][h].w};
+        if (unit < INFINITY) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            sum[h][e] += SlotCode::value(static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1))), unit);
+        } else {
+          float f[8];
+          unpack8<kBf16>(v[i][h], f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[h][e] += f[e];
+        }
+      }
     }
   }
-  uint16_t* o = out + t * ldo + c;
-  if (vec && c + 8 <= width) {
-    st128(o, pack8<DT>(sum));
-  } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (c + e < width) o[e] = Elem<DT>::from_float(sum[e]);
+  for (int h = 0; h < 2; ++h) {
+    const int at = c + 8 * h;
+    uint16_t* o = out + t * ldo + at;
+    if (vec && at + 8 <= width) {
+      st128(o, pack8<DT>(sum[h]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (at + e < width) o[e] = Elem<DT>::from_float(sum[h][e]);
+    }
   }
 }
 
@@ -316,7 +341,7 @@ Tile choose_tile(int64_t slots, int64_t experts, int64_t weight_rows, int64_t k_
 constexpr int64_t kMaxSlots = 131072;  // slots a pass takes; more tokens run in several passes
 
 struct ExpertWorkspace {
-  int64_t order, row_weights, gate_up_tiles, down_tiles, tile_counts, counts, xq, xs, act, actq, acts, y, bytes;
+  int64_t order, row_weights, gate_up_tiles, down_tiles, tile_counts, counts, xq, xs, act, actq, acts, y, y_scales, bytes;
   int64_t tokens;  // a pass
 };
 
@@ -349,7 +374,8 @@ ExpertWorkspace expert_workspace(int64_t tokens, int64_t top_k, int64_t experts,
     w.actq = take(slots * pad(inter, 16));
     w.acts = take(slots * 4);
   }
-  w.y = take(slots * pad(hidden, 8) * 2);
+  w.y = take(slots * pad(hidden, 32) * 2);
+  w.y_scales = take(slots * (pad(hidden, 64) / 32) * 2);
   w.bytes = at;
   return w;
 }
@@ -535,13 +561,15 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   a.w_expert = c.hidden * c.ld_down;
   a.w_scales = c.down_scales;
   a.out = ws + w.y;
-  a.ldo = pad(c.hidden, 8);
+  a.ldo = pad(c.hidden, 32);
+  a.code_scales = reinterpret_cast<uint16_t*>(ws + w.y_scales);
+  a.ld_code_scales = pad(c.hidden, 64) / 32;
   a.columns = static_cast<int32_t>(c.hidden);
   launch_product<IN, OT, kDown, false>(a, down_tile, slots, c.experts, s);
   if (const char* e = launch_status("product (down)")) return e;
-  const int64_t threads = c.tokens * (pad(c.hidden, 8) / 8);
+  const int64_t threads = c.tokens * (pad(c.hidden, 16) / 16);
   sum_slots<OT><<<dim3(static_cast<uint32_t>((threads + 255) / 256)), 256, 0, s>>>(
-      reinterpret_cast<const uint16_t*>(ws + w.y), a.ldo, c.ids, c.out, c.ldo, c.tokens,
+      reinterpret_cast<const uint16_t*>(ws + w.y), a.ldo, a.code_scales, a.ld_code_scales, c.ids, c.out, c.ldo, c.tokens,
       static_cast<int>(c.top_k), static_cast<int>(c.experts), static_cast<int>(c.hidden),
       c.ldo % 8 == 0 && aligned(c.out, 16));
   return launch_status("sum_slots");

@@ -33,7 +33,7 @@ constexpr int kFloatOut = 2;                    // outputs: 0 bf16, 1 fp16, 2 fp
 //   kDense    row r of x and of out is r; one weight
 //   kGateUp   row r of the grouped order reads x row order[r] / top_k and writes out row r
 //   kDown     row r of the grouped order reads x row r and writes out row order[r], times that
-//             slot's weight
+//             slot's weight, as SlotCodes
 //   kSplit    kDense over a part of K, the int32 sums left as they are (int8 only)
 constexpr int kDense = 0, kGateUp = 1, kDown = 2, kSplit = 3;
 
@@ -48,6 +48,8 @@ struct ProductArgs {
   const int4* tiles;          // grouped: {expert, first row, end row, 0} per row tile
   const int32_t* tile_count;  // grouped: tiles in the list
   const float* row_weights;   // kDown: weight of every row of the grouped order
+  uint16_t* code_scales;      // kDown: scale of every 32 columns of an out row (see SlotCode)
+  int64_t ld_code_scales;
   int64_t x_stride;           // bytes a row
   int64_t w_stride;           // bytes a row
   int64_t w_expert;           // bytes an expert
@@ -132,6 +134,54 @@ __device__ __forceinline__ void store4(void* out, int64_t at, const float (&v)[4
   }
 }
 
+// Slot outputs on their way to the sum over a token's slots: a signed 16-bit mantissa a value under a
+// power of two for every 32 columns. Half a unit is 2^-15 of the largest of the 32 or less, where bf16 would round every value by 2^-9 and cost the layer's output a third of its error
+// (relative to 64 bits 2.9e-3 in bf16, so 2.4e-3), at the traffic of 16 bits: fp32 slots would be
+// 0.5 GB more of it in an 8,192-token prefill, some 100 us of 780. Where a value is inf or NaN the scale
+// is inf and the 32 values are plain bf16.
+struct SlotCode {
+  float factor, highest;
+  uint16_t scale;  // bf16
+
+  __device__ __forceinline__ SlotCode() {}
+  // of the largest magnitude, as its bits
+  __device__ __forceinline__ explicit SlotCode(uint32_t top) {
+    const uint32_t e = max(top >> 23, 15u);               // 2^(e - 126) is above the largest
+    factor = __uint_as_float((268u - e) << 23);           // 2^(141 - e): to below 2^15
+    highest = 32767.f * __uint_as_float((e - 14) << 23);  // the last half unit has no code
+    scale = top >= 0x7f800000u ? 0x7f80 : (e - 14) << 7;  // 2^(e - 141)
+  }
+  __device__ __forceinline__ bool plain() const { return scale == 0x7f80; }
+  // Two values; 1.5 * 2^23 rounds them to integers in the low bits.
+  __device__ __forceinline__ uint32_t pack(float a, float b) const {
+    const uint32_t lo = __float_as_uint(fmaf(fminf(a, highest), factor, 12582912.f));
+    const uint32_t hi = __float_as_uint(fmaf(fminf(b, highest), factor, 12582912.f));
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100);
+  }
+  // The codes of a lane's 16 values, two a word.
+  __device__ __forceinline__ void pack16(const float (&v)[16], uint32_t (&w)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = pack(v[2 * i], v[2 * i + 1]);
+    if (__any(plain())) {  // seldom
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (plain()) w[i] = Elem<kBf16>::pack2(v[2 * i], v[2 * i + 1]);
+    }
+  }
+  __device__ __forceinline__ static float value(uint16_t code, float scale) {
+    return static_cast<float>(static_cast<int16_t>(code)) * scale;
+  }
+};
+
+// The largest magnitude of a lane's 16 values and those of lane ^ 32: the 32 columns of a row.
+__device__ __forceinline__ uint32_t block_magnitude(const float (&v)[16]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 16; i += 2)
+    top = max(max(top, __float_as_uint(v[i]) & 0x7fffffffu), __float_as_uint(v[i + 1]) & 0x7fffffffu);
+  return max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+}
+
 // What a row of a tile is multiplied with and where it goes.
 struct RowOut {
   int64_t at;    // row of out
@@ -173,7 +223,7 @@ __device__ __forceinline__ void finish_values(const ProductArgs& a, const RowOut
         u = u * r.scale * w_scales[a.columns + min(column + e, a.columns - 1)];
       g = silu_mul(g, u);
     }
-    v[e] = MODE == kDown ? g * r.weight : g;
+    v[e] = g;
   }
 }
 
@@ -466,6 +516,30 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
       continue;
     }
     const RowOut r = row_out<IN, MODE>(a, row);
+    if constexpr (MODE == kDown) {
+#pragma unroll
+      for (int i = 0; i < A_BLK; ++i) {
+        const int column = n0 + wn * kWaveN + 32 * i;
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          v[e] = static_cast<float>(acc[i][j][e]) * (r.scale * r.weight);
+          if constexpr (IN == kInt8)
+            v[e] *= w_scales[min(column + 8 * (e >> 2) + 4 * half + (e & 3), a.columns - 1)];
+        }
+        const SlotCode code(block_magnitude(v));
+        if (column >= a.columns) continue;
+        if (half == 0) a.code_scales[r.at * a.ld_code_scales + column / 32] = code.scale;
+        uint32_t w[8];
+        code.pack16(v, w);
+        // ldo is a multiple of 32: codes past the end have their place
+        uint16_t* p = static_cast<uint16_t*>(a.out) + r.at * a.ldo + column + 4 * half;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint2*>(p + 8 * q) = make_uint2(w[2 * q], w[2 * q + 1]);
+      }
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < A_BLK; ++i)
 #pragma unroll
@@ -665,13 +739,15 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
     const int begin = wm * (BM / 2) + 32 * j;  // row of the tile
     if (t.begin + begin >= t.end) break;
     const float row_scale = edges.row_scale[begin + col];
+    uint32_t scales = 0;  // kDown: of the codes of both A blocks
 #pragma unroll
-    for (int i = 0; i < A_BLK; ++i)
+    for (int i = 0; i < A_BLK; ++i) {
+      float f[16];  // of 32 columns (SILU: the 8 of 16)
 #pragma unroll
       for (int q = 0; q < 4; q += SILU ? 2 : 1) {
         const int wrow = 32 * i + 8 * q + 4 * half;
         const int at = SILU ? silu_column(wrow) : wrow;  // column of the wave
-        float f[4], gs[4] = {1.f, 1.f, 1.f, 1.f}, us[4] = {1.f, 1.f, 1.f, 1.f};
+        float gs[4] = {1.f, 1.f, 1.f, 1.f}, us[4] = {1.f, 1.f, 1.f, 1.f};
         if constexpr (IN == kInt8) {
           *reinterpret_cast<float4*>(gs) =
               *reinterpret_cast<const float4*>(edges.column_scale + wn * kCols + at);
@@ -689,15 +765,36 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
             if constexpr (IN == kInt8) u = u * row_scale * us[e];
             g = silu_mul(g, u);
           }
-          f[e] = g;
+          f[4 * q + e] = g;
         }
-        uint8_t* p = turn + col * kPitch + at * kOutSize;
-        if constexpr (OT == kFloatOut)
-          *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+      }
+      uint32_t codes[8];
+      if constexpr (MODE == kDown) {
+        const SlotCode code(block_magnitude(f));
+        code.pack16(f, codes);
+        scales |= static_cast<uint32_t>(code.scale) << (16 * i);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; q += SILU ? 2 : 1) {
+        const int wrow = 32 * i + 8 * q + 4 * half;
+        uint8_t* p = turn + col * kPitch + (SILU ? silu_column(wrow) : wrow) * kOutSize;
+        const float* v = f + 4 * q;
+        if constexpr (MODE == kDown)
+          *reinterpret_cast<uint2*>(p) = make_uint2(codes[2 * q], codes[2 * q + 1]);
+        else if constexpr (OT == kFloatOut)
+          *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
         else
           *reinterpret_cast<uint2*>(p) =
-              make_uint2(Elem<OT>::pack2(f[0], f[1]), Elem<OT>::pack2(f[2], f[3]));
+              make_uint2(Elem<OT>::pack2(v[0], v[1]), Elem<OT>::pack2(v[2], v[3]));
       }
+    }
+    if constexpr (MODE == kDown) {
+      static_assert(A_BLK == 2, "two scales a word");
+      const int column = n0 + wn * kCols;  // rows of scales are padded to whole words
+      if (half == 0 && t.begin + begin + col < t.end && column < a.columns)
+        *reinterpret_cast<uint32_t*>(a.code_scales + edges.out_row[begin + col] * a.ld_code_scales +
+                                     column / 32) = scales;
+    }
     // A wave's LDS operations keep their order, so its reads follow its writes of all lanes; the
     // clobbers keep the compiler from exchanging them.
     asm volatile("" ::: "memory");
