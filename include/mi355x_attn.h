@@ -355,7 +355,7 @@ int64_t mi355x_linear_int8_workspace_bytes(int64_t M, int64_t N, int64_t K, int3
 
 /* out[m, n] = round(sx[m] w_scales[n] sum_k q[m, k] w[n, k]) with (q, sx) = mi355x_quantize_rows
  * of x [M, K] (dtype 0 bf16, 1 fp16; out has the same) and w int8 [N, ldw]; the sum is exact
- * in int32. With silu_mul, w is a gate_up weight (gate rows, then up rows, N even) and
+ * in int32. out must not overlap x. With silu_mul, w is a gate_up weight (gate rows, then up rows, N even) and
  * out[m, j] = round(silu(y[m, j]) * y[m, N/2 + j]), y unrounded. K up to 131,072; w rows of
  * whole 16-byte words (columns past K are multiplied with zeros) and less than 4 GiB in all; x
  * and out rows of any stride. Calls that overlap need workspaces of their own. */
@@ -378,11 +378,12 @@ const char* mi355x_route_experts(const void* logits, int64_t ld, void* weights, 
                                  int64_t tokens, int64_t experts, int64_t top_k, bool normalize,
                                  int dtype, void* stream);
 
-/* Workspace bytes of mi355x_expert_mlp (ldx: x's row stride in elements), -1 for an invalid
- * shape. At most 131,072 slots (or one token) are in flight, more tokens run in several passes.
+/* Workspace bytes of mi355x_expert_mlp on a GPU of `cus` compute units (ldx: x's row stride in
+ * elements), -1 for an invalid shape. At most 131,072 slots (or one token) are in flight, more tokens run in several passes.
  * Host-only. */
 int64_t mi355x_expert_mlp_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts,
-                                          int64_t hidden, int64_t inter, int64_t ldx, bool int8);
+                                          int64_t hidden, int64_t inter, int64_t ldx, bool int8,
+                                          int32_t cus);
 
 /* out[t] = sum_s weights[t, s] down[e] . (silu(g) * u), (g; u) = gate_up[e] . x[t], e = ids[t, s].
  * x [tokens, hidden] and out of dtype 0 bf16 or 1 fp16, ids int32 and weights fp32

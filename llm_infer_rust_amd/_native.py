@@ -113,7 +113,7 @@ SIGNATURES: dict[str, tuple] = {
     "mi355x_route_experts": (c_char_p, [c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_i64, c_i64,
                                         c_bool, c_int, c_void_p]),
     "mi355x_expert_mlp_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
-                                                  c_bool]),
+                                                  c_bool, c_i32]),
     "mi355x_expert_mlp": (c_char_p, [c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_i64,
                                      c_void_p, c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_i64,
                                      c_i64, c_i64, c_i64, c_i64, c_void_p, c_i64, c_i32,

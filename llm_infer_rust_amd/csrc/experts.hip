@@ -240,8 +240,8 @@ __global__ __launch_bounds__(kGroupThreads) void place_slots(const int32_t* __re
 }
 
 // ---------------------------------------------------------------------------- the sum over slots
-// out[t] = sum of y[t * top_k + s] (SlotCodes) over the slots that take part, in fp32, s ascending. A
-// thread takes 16 columns, half of what a scale covers. Bound by memory: an 8,192-token prefill of 8
+// out[t] = sum of y[t * top_k + s] (SlotCodes) over the slots that take part and the parts of K, in fp32
+// and in this order. A thread takes 16 columns, half of what a scale covers. Bound by memory: an 8,192-token prefill of 8
 // slots and 2,048 columns reads 277 MB.
 template <int DT>
 __global__ __launch_bounds__(256) void sum_slots(const uint16_t* __restrict__ y, int64_t ldy,
@@ -249,8 +249,8 @@ __global__ __launch_bounds__(256) void sum_slots(const uint16_t* __restrict__ y,
                                                  int64_t ld_scales,
                                                  const int32_t* __restrict__ ids,
                                                  uint16_t* __restrict__ out, int64_t ldo,
-                                                 int64_t tokens, int top_k, int experts, int width,
-                                                 bool vec) {
+                                                 int64_t tokens, int top_k, int splits, int experts,
+                                                 int width, bool vec) {
   const int chunks = (width + 15) >> 4;
   const int64_t i = blockIdx.x * int64_t(256) + threadIdx.x;
   if (i >= tokens * chunks) return;
@@ -258,17 +258,24 @@ __global__ __launch_bounds__(256) void sum_slots(const uint16_t* __restrict__ y,
   const int c = static_cast<int>(i - t * chunks) * 16;
   float sum[2][8] = {};
   constexpr int kAtOnce = 8;  // slots whose loads are on their way together
-  for (int s0 = 0; s0 < top_k; s0 += kAtOnce) {
+  const int64_t plane = tokens * top_k;  // slots of a part
+  for (int s0 = 0; s0 < top_k * splits; s0 += kAtOnce) {
     bool in[kAtOnce];
+    int64_t slots[kAtOnce];
     uint4 v[kAtOnce][2];
     uint16_t scale[kAtOnce];
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i)
-      in[i] = s0 + i < top_k && takes_part(ids[t * top_k + min(s0 + i, top_k - 1)], experts);
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int n = min(s0 + i, top_k * splits - 1);
+      const int part = splits == 1 ? 0 : n / top_k;
+      const int64_t slot = t * top_k + (n - part * top_k);
+      slots[i] = part * plane + slot;
+      in[i] = s0 + i < top_k * splits && takes_part(ids[slot], experts);
+    }
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i)
       if (in[i]) {
-        const int64_t slot = t * top_k + s0 + i;
+        const int64_t slot = slots[i];
         v[i][0] = ld128_nt(y + slot * ldy + c);
         v[i][1] = ld128_nt(y + slot * ldy + c + 8);
         scale[i] = scales[slot * ld_scales + c / 32];
@@ -317,22 +324,41 @@ bool one_by_one(int64_t slots, int64_t top_k, int64_t hidden, int64_t inter, boo
          (!int8 || (pad(hidden, 16) <= kVecLds && top_k * pad(inter, 16) <= kVecLds));
 }
 
-// The tile of a grouped product: the least estimate. How many rows an expert gets is not known on the
-// host; it is taken to be the same for all, with half a tile more each for the ragged ends.
-Tile choose_tile(int64_t slots, int64_t experts, int64_t weight_rows, int64_t k_bytes, int cus) {
+// How a grouped product is computed: the tiles and, for the down product, the parts of K.
+struct GroupedPlan {
+  Tile tile;
+  int splits;
+};
+
+// The least estimate. How many rows an expert gets is not known on the host; it is taken to be the
+// same for all, with half a tile more each for the ragged ends. A product whose slot outputs are
+// summed afterwards may be cut along K as well, where its tiles leave CUs without one: the parts are
+// summed with the slots (down of 8 experts 1024 x 2816 at 77 tokens 17.0 us whole, 11.6 in two parts).
+GroupedPlan choose_grouped(int64_t slots, int64_t experts, int64_t weight_rows, int64_t k_bytes,
+                           bool summed, int cus) {
   const float active = static_cast<float>(std::min(slots, experts));
   const float per = static_cast<float>(slots) / active;
   const float weights = active * static_cast<float>(weight_rows) * static_cast<float>(k_bytes);
-  Tile best = Tile::k64;
+  const int64_t steps = (k_bytes + kProdRow - 1) / kProdRow;
+  GroupedPlan best{Tile::k64, 1};
   float best_us = 1e30f;
   for (int i = 0; i < 4; ++i) {
     const TileShape& t = kTileShapes[i];
     const float tm = active * std::max(1.f, per / static_cast<float>(t.bm) + 0.5f);
     const float tn = std::ceil(static_cast<float>(weight_rows) / static_cast<float>(t.bn));
-    const float us = tile_estimate(static_cast<Tile>(i), tm, tn, k_bytes, weights, per <= 128.f, cus);
-    if (us < best_us) {
-      best_us = us;
-      best = static_cast<Tile>(i);
+    for (int s = 1; s <= (summed && i < 2 ? 4 : 1); s *= 2) {
+      const int64_t part = (steps + s - 1) / s;
+      if (s > 1 && (part < 8 || part * (s - 1) >= steps || tm * tn * static_cast<float>(s / 2) >=
+                                                                static_cast<float>(cus)))
+        break;
+      float us = tile_estimate(static_cast<Tile>(i), tm * s, tn, part * kProdRow, weights,
+                               per <= 128.f, cus);
+      // two bytes a value more, out and back
+      us += static_cast<float>(s - 1) * (0.3f + static_cast<float>(slots * weight_rows) * 4 / 4.5e6f);
+      if (us < best_us) {
+        best_us = us;
+        best = {static_cast<Tile>(i), s};
+      }
     }
   }
   return best;
@@ -343,10 +369,11 @@ constexpr int64_t kMaxSlots = 131072;  // slots a pass takes; more tokens run in
 struct ExpertWorkspace {
   int64_t order, row_weights, gate_up_tiles, down_tiles, tile_counts, counts, xq, xs, act, actq, acts, y, y_scales, bytes;
   int64_t tokens;  // a pass
+  GroupedPlan gate_up, down;
 };
 
 ExpertWorkspace expert_workspace(int64_t tokens, int64_t top_k, int64_t experts, int64_t hidden,
-                                 int64_t inter, bool int8, int64_t x_stride) {
+                                 int64_t inter, bool int8, int64_t x_stride, int cus) {
   ExpertWorkspace w{};
   // Row offsets into x are 32-bit within a pass.
   const int64_t most = std::max<int64_t>(
@@ -354,6 +381,8 @@ ExpertWorkspace expert_workspace(int64_t tokens, int64_t top_k, int64_t experts,
   const int64_t t = std::min(tokens, most);
   const int64_t slots = t * top_k;
   w.tokens = t;
+  w.gate_up = choose_grouped(slots, experts, 2 * inter, int8 ? pad(hidden, 16) : hidden * 2, false, cus);
+  w.down = choose_grouped(slots, experts, hidden, int8 ? pad(inter, 16) : inter * 2, true, cus);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -374,8 +403,8 @@ ExpertWorkspace expert_workspace(int64_t tokens, int64_t top_k, int64_t experts,
     w.actq = take(slots * pad(inter, 16));
     w.acts = take(slots * 4);
   }
-  w.y = take(slots * pad(hidden, 32) * 2);
-  w.y_scales = take(slots * (pad(hidden, 64) / 32) * 2);
+  w.y = take(slots * w.down.splits * pad(hidden, 32) * 2);
+  w.y_scales = take(slots * w.down.splits * (pad(hidden, 64) / 32) * 2);
   w.bytes = at;
   return w;
 }
@@ -389,7 +418,7 @@ void launch_product(const ProductArgs& base, Tile tile, int64_t slots, int64_t e
   a.tiles_n = (a.columns + bn - 1) / bn;
   // Tiles that so many slots need at most: every full one and one more an expert.
   const int64_t most = slots / t.bm + std::min(experts, slots);
-  const dim3 g(static_cast<uint32_t>(pad(most * a.tiles_n, 8)));
+  const dim3 g(static_cast<uint32_t>(pad(most * a.tiles_n * a.splits, 8)));
   switch (tile) {
     case Tile::k64: product_tile<IN, OT, MODE, SILU, 64, 64, 2, 2, 4><<<g, 256, 0, s>>>(a); break;
     case Tile::k128: product_tile<IN, OT, MODE, SILU, 128, 128, 4, 2, 4><<<g, 512, 0, s>>>(a); break;
@@ -418,7 +447,6 @@ struct ExpertCall {
   uint16_t* out;
   int64_t ldo;
   int64_t tokens, top_k, experts, hidden, inter;
-  int32_t cus;
 };
 
 // The slots one by one.
@@ -485,8 +513,6 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
     return expert_slots<IN, OT>(c, w, ws, s);
   const int64_t gate_up_k = kQuant ? pad(c.hidden, 16) : c.hidden * 2;
   const int64_t down_k = kQuant ? pad(c.inter, 16) : c.inter * 2;
-  const Tile gate_up_tile = choose_tile(slots, c.experts, 2 * c.inter, gate_up_k, c.cus);
-  const Tile down_tile = choose_tile(slots, c.experts, c.hidden, down_k, c.cus);
   auto* order = reinterpret_cast<int32_t*>(ws + w.order);
   auto* row_weights = reinterpret_cast<float*>(ws + w.row_weights);
   auto* gate_up_tiles = reinterpret_cast<int4*>(ws + w.gate_up_tiles);
@@ -501,7 +527,8 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   }
   place_slots<<<dim3(chunks), kGroupThreads, 0, s>>>(
       c.ids, static_cast<int>(slots), static_cast<int>(c.experts),
-      kTileShapes[static_cast<int>(gate_up_tile)].bm, kTileShapes[static_cast<int>(down_tile)].bm,
+      kTileShapes[static_cast<int>(w.gate_up.tile)].bm,
+      kTileShapes[static_cast<int>(w.down.tile)].bm,
       chunks > 1 ? counts : nullptr, chunks, c.weights, order, row_weights, gate_up_tiles,
       down_tiles, tile_counts);
   if (const char* e = launch_status("place_slots")) return e;
@@ -513,6 +540,7 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   a.rows = static_cast<int32_t>(slots);
   a.top_k = static_cast<int32_t>(c.top_k);
   a.experts = static_cast<int32_t>(c.experts);
+  a.splits = 1;
   a.vec_out = a.vec16_out = 1;
   // gate_up with SiLU x mul into act, one row a slot
   if (kQuant) {
@@ -536,7 +564,7 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   a.out = ws + w.act;
   a.ldo = kQuant ? pad(c.inter, 4) : c.inter;
   a.columns = static_cast<int32_t>(c.inter);
-  launch_product<IN, kQuant ? kFloatOut : OT, kGateUp, true>(a, gate_up_tile, slots, c.experts, s);
+  launch_product<IN, kQuant ? kFloatOut : OT, kGateUp, true>(a, w.gate_up.tile, slots, c.experts, s);
   if (const char* e = launch_status("product (gate_up)")) return e;
   // down into y, one weighted row a slot
   if (kQuant) {
@@ -561,17 +589,18 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   a.w_expert = c.hidden * c.ld_down;
   a.w_scales = c.down_scales;
   a.out = ws + w.y;
+  a.splits = w.down.splits;
   a.ldo = pad(c.hidden, 32);
   a.code_scales = reinterpret_cast<uint16_t*>(ws + w.y_scales);
   a.ld_code_scales = pad(c.hidden, 64) / 32;
   a.columns = static_cast<int32_t>(c.hidden);
-  launch_product<IN, OT, kDown, false>(a, down_tile, slots, c.experts, s);
+  launch_product<IN, OT, kDown, false>(a, w.down.tile, slots, c.experts, s);
   if (const char* e = launch_status("product (down)")) return e;
   const int64_t threads = c.tokens * (pad(c.hidden, 16) / 16);
   sum_slots<OT><<<dim3(static_cast<uint32_t>((threads + 255) / 256)), 256, 0, s>>>(
       reinterpret_cast<const uint16_t*>(ws + w.y), a.ldo, a.code_scales, a.ld_code_scales, c.ids, c.out, c.ldo, c.tokens,
-      static_cast<int>(c.top_k), static_cast<int>(c.experts), static_cast<int>(c.hidden),
-      c.ldo % 8 == 0 && aligned(c.out, 16));
+      static_cast<int>(c.top_k), w.down.splits, static_cast<int>(c.experts),
+      static_cast<int>(c.hidden), c.ldo % 8 == 0 && aligned(c.out, 16));
   return launch_status("sum_slots");
 }
 
@@ -613,11 +642,13 @@ extern "C" const char* mi355x_route_experts(const void* logits, int64_t ld, void
 
 extern "C" int64_t mi355x_expert_mlp_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts,
                                                      int64_t hidden, int64_t inter, int64_t ldx,
-                                                     bool int8) {
+                                                     bool int8, int32_t cus) {
   if (!expert_shape_ok(tokens, top_k, experts, hidden, inter, int8) || ldx < hidden ||
       ldx >= (int64_t(1) << 31))
     return -1;
-  return expert_workspace(tokens, top_k, experts, hidden, inter, int8, ldx * 2).bytes;
+  return expert_workspace(tokens, top_k, experts, hidden, inter, int8, ldx * 2,
+                          cus > 0 ? cus : 256)
+      .bytes;
 }
 
 extern "C" const char* mi355x_expert_mlp(const void* x, int64_t ldx, const int32_t* ids,
@@ -649,7 +680,7 @@ extern "C" const char* mi355x_expert_mlp(const void* x, int64_t ldx, const int32
       !aligned(out, 2) || !aligned(workspace, 16) || !aligned(ids, 4) || !aligned(weights, 4))
     return set_error("mi355x_expert_mlp: misaligned operand");
   const ExpertWorkspace w =
-      expert_workspace(tokens, top_k, experts, hidden, inter, int8, ldx * 2);
+      expert_workspace(tokens, top_k, experts, hidden, inter, int8, ldx * 2, cus > 0 ? cus : 256);
   if (workspace_bytes < w.bytes) return set_error("mi355x_expert_mlp: workspace too small");
   auto s = static_cast<hipStream_t>(stream);
   for (int64_t t = 0; t < tokens; t += w.tokens) {
@@ -671,7 +702,6 @@ extern "C" const char* mi355x_expert_mlp(const void* x, int64_t ldx, const int32
     c.experts = experts;
     c.hidden = hidden;
     c.inter = inter;
-    c.cus = cus > 0 ? cus : 256;
     auto* ws = static_cast<uint8_t*>(workspace);
     const char* e = int8 ? (dtype == 0 ? expert_pass<kInt8, 0>(c, w, ws, s)
                                        : expert_pass<kInt8, 1>(c, w, ws, s))

@@ -60,7 +60,8 @@ struct ProductArgs {
   int32_t top_k;
   int32_t experts;
   int32_t tiles_m, tiles_n;   // kDense, kSplit: row tiles; column tiles of every row tile
-  int32_t splits;             // kSplit: parts of K; out is int32 [splits][rows][ldo]
+  int32_t splits;             // parts of K. kSplit: out is int32 [splits][rows][ldo]. kDown
+                              // (product_tile): out has a plane of `rows` slots a part, summed later
   int32_t vec_out;            // out rows take aligned stores of four elements
   int32_t vec16_out;          // out rows take aligned 16-byte stores
 };
@@ -263,17 +264,17 @@ __device__ __forceinline__ bool row_tile(const ProductArgs& a, int tm, RowTile* 
 
 // Workgroup -> (row tile, column tile). Workgroup i runs on XCD i mod 8; every XCD takes a
 // contiguous eighth of the tiles, so those that share weights or rows of x meet in its L2. False for the workgroups past the last tile (the grid of a grouped product
-// is sized for the most tiles that its rows can need). kSplit: tm counts the row tiles of every part
-// of K in turn.
+// is sized for the most tiles that its rows can need). Where K is split, tm counts the
+// row tiles of every part in turn.
 template <int MODE>
-__device__ __forceinline__ bool tile_of_block(const ProductArgs& a, int* tm, int* tn) {
+__device__ __forceinline__ bool tile_of_block(const ProductArgs& a, int splits, int* tm, int* tn) {
   int count;
   if constexpr (MODE == kDense)
     count = a.tiles_m;
   else if constexpr (MODE == kSplit)
-    count = a.tiles_m * a.splits;
+    count = a.tiles_m * splits;
   else
-    count = a.tiles ? *a.tile_count : a.rows;
+    count = (a.tiles ? *a.tile_count : a.rows) * splits;
   const int total = count * a.tiles_n;
   const int per = (total + 7) >> 3;
   const int i = static_cast<int>(blockIdx.x >> 3);
@@ -366,12 +367,14 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
   if (a.columns < 0) lds[tid] = 0;  // never taken; the copies' LDS writes are invisible
 
   int tm, tn;
-  if (!tile_of_block<MODE>(a, &tm, &tn)) return;
+  constexpr bool kParts = MODE == kSplit || MODE == kDown;
+  if (!tile_of_block<MODE>(a, kParts ? a.splits : 1, &tm, &tn)) return;
   const int all_k = (a.k_bytes + kProdRow - 1) / kProdRow;
   int first_k = 0, n_k = all_k, split = 0;
-  if constexpr (MODE == kSplit) {
-    split = tm / a.tiles_m;
-    tm -= split * a.tiles_m;
+  if constexpr (kParts) {
+    const int row_tiles = MODE == kSplit ? a.tiles_m : *a.tile_count;
+    split = tm / row_tiles;
+    tm -= split * row_tiles;
     const int per = (all_k + a.splits - 1) / a.splits;
     first_k = split * per;
     n_k = min(per, all_k - first_k);
@@ -515,8 +518,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
         }
       continue;
     }
-    const RowOut r = row_out<IN, MODE>(a, row);
+    RowOut r = row_out<IN, MODE>(a, row);
     if constexpr (MODE == kDown) {
+      r.at += static_cast<int64_t>(split) * a.rows;
 #pragma unroll
       for (int i = 0; i < A_BLK; ++i) {
         const int column = n0 + wn * kWaveN + 32 * i;
@@ -864,7 +868,7 @@ __global__ __launch_bounds__(64 * NW, 1) void product_large(ProductArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kLargeEdges + sizeof(LargeEdges)];
   if (a.columns < 0) lds[threadIdx.x] = 0;  // never taken; the copies' LDS writes are invisible
   int tm, tn;
-  if (!tile_of_block<MODE>(a, &tm, &tn)) return;
+  if (!tile_of_block<MODE>(a, 1, &tm, &tn)) return;
   RowTile t;
   if (!row_tile<MODE, BM>(a, tm, &t)) return;
   const int n0 = tn * (SILU ? kLargeN / 2 : kLargeN);
@@ -892,7 +896,7 @@ __global__ __launch_bounds__(256) void product_rows(ProductArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
   int tm, tn;
-  if (!tile_of_block<kDense>(a, &tm, &tn)) return;
+  if (!tile_of_block<kDense>(a, 1, &tm, &tn)) return;
   RowTile t;
   if (!row_tile<kDense, 16>(a, tm, &t)) return;
   const int n0 = tn * kOut;

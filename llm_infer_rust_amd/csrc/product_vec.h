@@ -97,7 +97,7 @@ __global__ __launch_bounds__(64 * WAVES) void product_vec(ProductArgs a, int wid
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   int tm, tn;
-  if (!tile_of_block<MODE>(a, &tm, &tn)) return;
+  if (!tile_of_block<MODE>(a, 1, &tm, &tn)) return;
   RowTile t;
   if (!row_tile<MODE, MR>(a, tm, &t)) return;
   const int n0 = (tn * WAVES + wave) * kOut;

@@ -98,7 +98,8 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     elif out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
         raise NativeError("expert_mlp: out must not share memory with x")
     with on_device(x.device):
-        need = lib().mi355x_expert_mlp_workspace_bytes(t, top_k, e, h, inter, ldx, int8)
+        cus = device_cus(x.device)
+        need = lib().mi355x_expert_mlp_workspace_bytes(t, top_k, e, h, inter, ldx, int8, cus)
         if need < 0:
             raise NativeError("expert_mlp: invalid shape")
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=x.device)
@@ -107,7 +108,7 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
             gate_up.row_stride if int8 else h, gate_up.scales.data_ptr() if int8 else None,
             dn.data_ptr(), down.row_stride if int8 else inter,
             down.scales.data_ptr() if int8 else None, out.data_ptr(), _row_stride(out), t, top_k,
-            e, h, inter, ws.data_ptr(), need, device_cus(x.device), dt, stream_of(x)), "expert_mlp")
+            e, h, inter, ws.data_ptr(), need, cus, dt, stream_of(x)), "expert_mlp")
     return out
 
 

@@ -131,7 +131,8 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = 
     """``x @ weight.T`` in 8-bit integers: ``x`` ``[T, K]`` bf16 or fp16 is quantised a row, the int32
     sums are exact, ``out`` ``[T, N]`` is rounded once. ``silu_mul``: ``weight`` is a gate_up
     projection (gate rows, then up rows) and the result is ``silu(gate) * up`` ``[T, N / 2]``,
-    rounded once. Rows may have any stride and alignment. A row with an inf or a NaN comes out NaN."""
+    rounded once. Rows may have any stride and alignment; ``out`` may be
+    given and must not share memory with ``x``. A row with an inf or a NaN comes out NaN."""
     _check_rows(x, "linear_int8")
     dt = _ROW_DTYPES.get(x.dtype)
     if dt not in (0, 1):
@@ -151,6 +152,8 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = 
         elif (out.shape != (t, width) or out.dtype != x.dtype or out.device != x.device
               or (width > 1 and out.stride(1) != 1) or (t > 1 and out.stride(0) < width)):
             raise NativeError("linear_int8: invalid output")
+        elif out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
+            raise NativeError("linear_int8: out must not share memory with x")
         cus = device_cus(x.device)
         need = lib().mi355x_linear_int8_workspace_bytes(t, n, k, cus)
         if need < 0:

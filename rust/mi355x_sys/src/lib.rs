@@ -98,7 +98,7 @@ unsafe extern "C" {
         tokens: i64, experts: i64, top_k: i64, normalize: bool, dtype: c_int,
         stream: *mut c_void) -> *const c_char;
     pub fn mi355x_expert_mlp_workspace_bytes(tokens: i64, top_k: i64, experts: i64, hidden: i64,
-        inter: i64, ldx: i64, int8: bool) -> i64;
+        inter: i64, ldx: i64, int8: bool, cus: i32) -> i64;
     pub fn mi355x_expert_mlp(x: *const c_void, ldx: i64, ids: *const i32, weights: *const f32,
         gate_up: *const c_void, ld_gate_up: i64, gate_up_scales: *const f32,
         down: *const c_void, ld_down: i64, down_scales: *const f32, out: *mut c_void, ldo: i64,

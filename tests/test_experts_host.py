@@ -80,13 +80,13 @@ def test_entries_refuse_bad_arguments_before_launching():
         assert "shape" in err(route(**bad)), bad
 
     size = f.mi355x_expert_mlp_workspace_bytes
-    assert size(0, 2, 8, 64, 32, 64, False) >= 0
-    assert size(4, 2, 8, 60, 32, 64, False) == -1 and size(4, 2, 8, 60, 32, 64, True) > 0
-    assert size(4, 65, 8, 64, 32, 64, False) == -1 and size(4, 2, 1025, 64, 32, 64, False) == -1
-    assert size(4, 2, 8, 64, 32, 63, False) == -1
+    assert size(0, 2, 8, 64, 32, 64, False, 256) >= 0
+    assert size(4, 2, 8, 60, 32, 64, False, 256) == -1 and size(4, 2, 8, 60, 32, 64, True, 256) > 0
+    assert size(4, 65, 8, 64, 32, 64, False, 256) == -1 and size(4, 2, 1025, 64, 32, 64, False, 256) == -1
+    assert size(4, 2, 8, 64, 32, 63, False, 256) == -1
     # the slots of one pass bound the workspace, however many tokens there are
-    assert size(1 << 22, 8, 8, 64, 32, 64, False) < 131072 * (32 + 64 + 64) * 4
-    need = size(40, 2, 8, 64, 32, 64, False)
+    assert size(1 << 22, 8, 8, 64, 32, 64, False, 256) < 131072 * (32 + 64 + 64) * 4
+    need = size(40, 2, 8, 64, 32, 64, False, 256)
 
     def mlp(x=A, ldx=64, ids=B, gu=C, ldg=64, gs=None, dn=D, ldd=32, ds=None, t=40, k=2, e=8,
             h=64, i=32, wsp=A, n=need, dt=0, ldo=64):

@@ -160,6 +160,7 @@ SHAPES = [
     (1, 8, 2, 64, 64), (1, 4, 4, 8, 8), (2, 16, 8, 136, 72), (3, 5, 1, 1000, 24),
     (16, 8, 2, 256, 128), (17, 128, 8, 128, 64), (40, 3, 2, 512, 200), (77, 8, 2, 264, 520),
     (200, 4, 2, 192, 320), (300, 7, 3, 328, 264), (1200, 5, 2, 136, 136),
+    (40, 6, 2, 104, 2056), (90, 2, 2, 72, 4104),  # down cut along K, in two parts and in four
 ]
 
 

@@ -182,6 +182,7 @@ def test_empty_batch_and_refusals(gpu):
                 lambda: int8.linear_int8(x, odd, silu_mul=True),
                 lambda: int8.linear_int8(x.t().contiguous().t(), weight),
                 lambda: int8.linear_int8(x, weight, out=torch.empty(4, 9, dtype=x.dtype, device=gpu)),
+                lambda: int8.linear_int8(x, weight, out=x[:, :8]),
                 lambda: int8.linear_int8(x, weight.values), lambda: int8.linear_int8(x[0], weight),
                 lambda: int8.linear_int8(x.clone().requires_grad_(), weight),
                 lambda: int8.quantize_rows(x.double()), lambda: int8.quantize_rows(x[:, :0]),
