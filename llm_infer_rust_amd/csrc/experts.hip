@@ -420,7 +420,7 @@ void launch_product(const ProductArgs& base, Tile tile, int64_t slots, int64_t e
   const int64_t most = slots / t.bm + std::min(experts, slots);
   const dim3 g(static_cast<uint32_t>(pad(most * a.tiles_n * a.splits, 8)));
   switch (tile) {
-    case Tile::k64: product_tile<IN, OT, MODE, SILU, 64, 64, 2, 2, 4><<<g, 256, 0, s>>>(a); break;
+    case Tile::k64: product_tile<IN, OT, MODE, SILU, 64, 64, 2, 2, 3><<<g, 256, 0, s>>>(a); break;
     case Tile::k128: product_tile<IN, OT, MODE, SILU, 128, 128, 4, 2, 4><<<g, 512, 0, s>>>(a); break;
     case Tile::k256x128:
       product_tile<IN, OT, MODE, SILU, 256, 128, 4, 2, 3><<<g, 512, 0, s>>>(a);

@@ -992,7 +992,8 @@ constexpr TileShape kTileShapes[] = {
 
 // Estimated time in us of `row_tiles` x `column_tiles` tiles over K. A CU's copies into LDS come at
 // about 60 GB/s where they miss L2, whatever the depth of the ring, which makes the step of a tile
-// its bytes; one workgroup a CU, but two of 64 x 64. A 256 x 256 tile of up to 128 rows runs as half a
+// its bytes; one workgroup a CU, but three of 64 x 64 (with three stages in LDS; with four, two of them:
+// the 8-bit experts of 40 tokens 57 + 33 us instead of 53 + 29). A 256 x 256 tile of up to 128 rows runs as half a
 // tile. Weights come at 5.8 TB/s at most. Measured, int8: 4096 x 4096 at 64 rows 64 x 64 tiles 13.0 us,
 // 128 x 128 19.5, 256 x 256 25.2; 6144 x 4096 at 512 rows 33.9 / 25.2 / 34.4 (256 x 128) / 47.2, at 1,024
 // rows 62 / 54 / 37.5 / 49, at 2,048 rows 118 / 79 / 76 / 56. bf16 experts 128 x (1536 x 2048) at 64 rows

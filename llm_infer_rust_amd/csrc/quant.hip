@@ -187,7 +187,7 @@ void launch_int8_tiles(ProductArgs& a, Tile tile, hipStream_t s) {
   a.tiles_n = (a.columns + bn - 1) / bn;
   const dim3 g(static_cast<uint32_t>((int64_t(a.tiles_m) * a.tiles_n * a.splits + 7) / 8 * 8));
   if (tile == Tile::k64) {
-    product_tile<kInt8, OT, MODE, SILU, 64, 64, 2, 2, 4><<<g, 256, 0, s>>>(a);
+    product_tile<kInt8, OT, MODE, SILU, 64, 64, 2, 2, 3><<<g, 256, 0, s>>>(a);
   } else if (tile == Tile::k128) {
     product_tile<kInt8, OT, MODE, SILU, 128, 128, 4, 2, 4><<<g, 512, 0, s>>>(a);
   } else if constexpr (MODE == kDense) {
