@@ -182,36 +182,38 @@ __device__ __forceinline__ int block_exclusive(int v, int4 (&wave_totals)[4]) {
 // be null with one chunk. The first workgroup writes the list of row tiles for the gate_up product, the
 // second (or the first, if alone) that for the down product. The order of the slots within an
 // expert is that of the LDS atomics; a row's products do not depend on the row it stands in.
-__global__ __launch_bounds__(kGroupThreads) void place_slots(const int32_t* __restrict__ ids,
-                                                             int slots, int experts,
-                                                             int gate_up_bm, int down_bm,
-                                                             const int32_t* __restrict__ counts,
-                                                             int chunks,
-                                                             const float* __restrict__ weights,
-                                                             int32_t* __restrict__ order,
-                                                             float* __restrict__ row_weights,
-                                                             int4* __restrict__ gate_up_tiles,
-                                                             int4* __restrict__ down_tiles,
-                                                             int32_t* __restrict__ tile_counts) {
+struct SlotsToPlace {
+  const int32_t* ids;
+  const float* weights;
+  const int32_t* counts;
+  int32_t* order;
+  float* row_weights;
+  int4* gate_up_tiles;
+  int4* down_tiles;
+  int32_t* tile_counts;
+  int32_t slots, experts, gate_up_bm, down_bm, chunks;
+};
+
+__device__ __forceinline__ void place_chunk(const SlotsToPlace& p) {
   static_assert(kMaxExperts == kGroupThreads, "an expert a thread");
   __shared__ int cursor[kMaxExperts], totals[kMaxExperts];
   __shared__ int4 wave_totals[4];
   const int e = threadIdx.x;
-  const int begin = blockIdx.x * kGroupChunk, end = min(slots, begin + kGroupChunk);
+  const int begin = blockIdx.x * kGroupChunk, end = min(p.slots, begin + kGroupChunk);
   cursor[e] = totals[e] = 0;  // slots of the chunks before this one, and of all
   __syncthreads();
-  if (counts) {
-    const int before = static_cast<int>(blockIdx.x) * experts;
-    for (int i = threadIdx.x; i < chunks * experts; i += kGroupThreads) {
-      const int n = counts[i];
+  if (p.counts) {
+    const int before = static_cast<int>(blockIdx.x) * p.experts;
+    for (int i = threadIdx.x; i < p.chunks * p.experts; i += kGroupThreads) {
+      const int n = p.counts[i];
       if (n == 0) continue;
-      atomicAdd(&totals[i % experts], n);
-      if (i < before) atomicAdd(&cursor[i % experts], n);
+      atomicAdd(&totals[i % p.experts], n);
+      if (i < before) atomicAdd(&cursor[i % p.experts], n);
     }
   } else {
     for (int i = begin + threadIdx.x; i < end; i += kGroupThreads) {
-      const int x = ids[i];
-      if (takes_part(x, experts)) atomicAdd(&totals[x], 1);
+      const int x = p.ids[i];
+      if (takes_part(x, p.experts)) atomicAdd(&totals[x], 1);
     }
   }
   __syncthreads();
@@ -219,65 +221,87 @@ __global__ __launch_bounds__(kGroupThreads) void place_slots(const int32_t* __re
   const int first = block_exclusive(total, wave_totals);
   cursor[e] += first;
   for (int product = 0; product < 2; ++product) {
-    if (static_cast<int>(blockIdx.x) != min(product, chunks - 1)) continue;
-    const int bm = product ? down_bm : gate_up_bm;
-    int4* tiles = product ? down_tiles : gate_up_tiles;
+    if (static_cast<int>(blockIdx.x) != min(product, p.chunks - 1)) continue;
+    const int bm = product ? p.down_bm : p.gate_up_bm;
+    int4* tiles = product ? p.down_tiles : p.gate_up_tiles;
     const int n = (total + bm - 1) / bm;
     const int at = block_exclusive(n, wave_totals);
     for (int i = 0; i < n; ++i)
       tiles[at + i] = make_int4(e, first + i * bm, min(first + (i + 1) * bm, first + total), 0);
-    if (e == kGroupThreads - 1) tile_counts[product] = at + n;
+    if (e == kGroupThreads - 1) p.tile_counts[product] = at + n;
   }
   __syncthreads();
   for (int i = begin + threadIdx.x; i < end; i += kGroupThreads) {
-    const int x = ids[i];
-    if (takes_part(x, experts)) {
+    const int x = p.ids[i];
+    if (takes_part(x, p.experts)) {
       const int row = atomicAdd(&cursor[x], 1);
-      order[row] = i;
-      row_weights[row] = weights[i];
+      p.order[row] = i;
+      p.row_weights[row] = p.weights[i];
     }
   }
 }
 
+__global__ __launch_bounds__(kGroupThreads) void place_slots(SlotsToPlace p) { place_chunk(p); }
+
+// The same with the rows of x quantised by the workgroups behind the chunks', four rows each: one
+// launch less before the products (8-bit experts of 40 tokens 110 -> 108 us).
+template <int DT>
+__global__ __launch_bounds__(kGroupThreads) void place_and_quantize(SlotsToPlace p,
+                                                                    RowsToQuantize q) {
+  __shared__ uint32_t wave_top[kGroupThreads / kWave];
+  if (static_cast<int>(blockIdx.x) < p.chunks)
+    place_chunk(p);
+  else
+    quantize_row<DT, 256, 1>(
+        q, (int64_t(blockIdx.x) - p.chunks) * (kGroupThreads / 256) + threadIdx.x / 256, wave_top);
+}
+
 // ---------------------------------------------------------------------------- the sum over slots
 // out[t] = sum of y[t * top_k + s] (SlotCodes) over the slots that take part and the parts of K, in fp32
-// and in this order. A thread takes 16 columns, half of what a scale covers. Bound by memory: an 8,192-token prefill of 8
-// slots and 2,048 columns reads 277 MB.
-template <int DT>
-__global__ __launch_bounds__(256) void sum_slots(const uint16_t* __restrict__ y, int64_t ldy,
+// and in this order. A thread takes 8 H columns, a quarter or half of what a scale covers. Bound by
+// memory where there are many tokens (8,192 of 8 slots and 2,048 columns: 277 MB in 60 us with H 2, 69
+// with H 1), else by latency: H 1 and workgroups of a wave spread over the chip (40 tokens 7.1 us with
+// H 2 and 256 threads).
+template <int DT, int H, int THREADS, bool PARTS>
+__global__ __launch_bounds__(THREADS) void sum_slots(const uint16_t* __restrict__ y, int64_t ldy,
                                                  const uint16_t* __restrict__ scales,
                                                  int64_t ld_scales,
                                                  const int32_t* __restrict__ ids,
                                                  uint16_t* __restrict__ out, int64_t ldo,
                                                  int64_t tokens, int top_k, int splits, int experts,
                                                  int width, bool vec) {
-  const int chunks = (width + 15) >> 4;
-  const int64_t i = blockIdx.x * int64_t(256) + threadIdx.x;
-  if (i >= tokens * chunks) return;
-  const int64_t t = i / chunks;
-  const int c = static_cast<int>(i - t * chunks) * 16;
-  float sum[2][8] = {};
+  const int chunks = (width + 8 * H - 1) / (8 * H);
+  // at most 2^17 tokens of 2^14 chunks a pass
+  const uint32_t i = blockIdx.x * uint32_t(THREADS) + threadIdx.x;
+  const uint32_t t = i / static_cast<uint32_t>(chunks);
+  if (t >= tokens) return;
+  const int c = static_cast<int>(i - t * chunks) * (8 * H);
+  float sum[H][8] = {};
   constexpr int kAtOnce = 8;  // slots whose loads are on their way together
-  const int64_t plane = tokens * top_k;  // slots of a part
+  const int first = static_cast<int>(t) * top_k, plane = static_cast<int>(tokens) * top_k;
   for (int s0 = 0; s0 < top_k * splits; s0 += kAtOnce) {
     bool in[kAtOnce];
-    int64_t slots[kAtOnce];
-    uint4 v[kAtOnce][2];
+    int32_t slots[kAtOnce];
+    uint4 v[kAtOnce][H];
     uint16_t scale[kAtOnce];
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
       const int n = min(s0 + i, top_k * splits - 1);
-      const int part = splits == 1 ? 0 : n / top_k;
-      const int64_t slot = t * top_k + (n - part * top_k);
-      slots[i] = part * plane + slot;
+      int slot = first + n;
+      slots[i] = slot;
+      if constexpr (PARTS) {  // plane n / top_k of the slots
+        const int part = n / top_k;
+        slot -= part * top_k;
+        slots[i] = part * plane + slot;
+      }
       in[i] = s0 + i < top_k * splits && takes_part(ids[slot], experts);
     }
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i)
       if (in[i]) {
         const int64_t slot = slots[i];
-        v[i][0] = ld128_nt(y + slot * ldy + c);
-        v[i][1] = ld128_nt(y + slot * ldy + c + 8);
+#pragma unroll
+        for (int h = 0; h < H; ++h) v[i][h] = ld128(y + slot * ldy + c + 8 * h);
         scale[i] = scales[slot * ld_scales + c / 32];
       }
 #pragma unroll
@@ -285,7 +309,7 @@ __global__ __launch_bounds__(256) void sum_slots(const uint16_t* __restrict__ y,
       if (!in[i]) continue;
       const float unit = Elem<kBf16>::to_float(scale[i]);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < H; ++h) {
         const uint32_t w[4] = {v[i][h].x, v[i][h].y, v[i][h].z, v[i][h].w};
         if (unit < INFINITY) {
 #pragma unroll
@@ -301,9 +325,9 @@ __global__ __launch_bounds__(256) void sum_slots(const uint16_t* __restrict__ y,
     }
   }
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < H; ++h) {
     const int at = c + 8 * h;
-    uint16_t* o = out + t * ldo + at;
+    uint16_t* o = out + static_cast<int64_t>(t) * ldo + at;
     if (vec && at + 8 <= width) {
       st128(o, pack8<DT>(sum[h]));
     } else {
@@ -525,12 +549,30 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
                                                        static_cast<int>(c.experts), counts);
     if (const char* e = launch_status("count_slots")) return e;
   }
-  place_slots<<<dim3(chunks), kGroupThreads, 0, s>>>(
-      c.ids, static_cast<int>(slots), static_cast<int>(c.experts),
-      kTileShapes[static_cast<int>(w.gate_up.tile)].bm,
-      kTileShapes[static_cast<int>(w.down.tile)].bm,
-      chunks > 1 ? counts : nullptr, chunks, c.weights, order, row_weights, gate_up_tiles,
-      down_tiles, tile_counts);
+  const SlotsToPlace place{c.ids,
+                           c.weights,
+                           chunks > 1 ? counts : nullptr,
+                           order,
+                           row_weights,
+                           gate_up_tiles,
+                           down_tiles,
+                           tile_counts,
+                           static_cast<int32_t>(slots),
+                           static_cast<int32_t>(c.experts),
+                           kTileShapes[static_cast<int>(w.gate_up.tile)].bm,
+                           kTileShapes[static_cast<int>(w.down.tile)].bm,
+                           chunks};
+  auto* xs = reinterpret_cast<float*>(ws + w.xs);
+  if constexpr (kQuant) {
+    const RowsToQuantize rows = rows_to_quantize(c.x, c.x_stride, ws + w.xq, pad(c.hidden, 16), xs,
+                                                 c.tokens, c.hidden);
+    constexpr int kRows = kGroupThreads / 256;
+    place_and_quantize<OT>
+        <<<dim3(static_cast<uint32_t>(chunks + (c.tokens + kRows - 1) / kRows)), kGroupThreads, 0,
+           s>>>(place, rows);
+  } else {
+    place_slots<<<dim3(chunks), kGroupThreads, 0, s>>>(place);
+  }
   if (const char* e = launch_status("place_slots")) return e;
   ProductArgs a{};
   a.order = order;
@@ -544,10 +586,6 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   a.vec_out = a.vec16_out = 1;
   // gate_up with SiLU x mul into act, one row a slot
   if (kQuant) {
-    auto* xs = reinterpret_cast<float*>(ws + w.xs);
-    if (const char* e = run_quantize_rows(c.x, c.x_stride, ws + w.xq, pad(c.hidden, 16), xs,
-                                          c.tokens, c.hidden, OT, s))
-      return e;
     a.x = ws + w.xq;
     a.x_stride = pad(c.hidden, 16);
     a.x_scales = xs;
@@ -596,11 +634,22 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   a.columns = static_cast<int32_t>(c.hidden);
   launch_product<IN, OT, kDown, false>(a, w.down.tile, slots, c.experts, s);
   if (const char* e = launch_status("product (down)")) return e;
-  const int64_t threads = c.tokens * (pad(c.hidden, 16) / 16);
-  sum_slots<OT><<<dim3(static_cast<uint32_t>((threads + 255) / 256)), 256, 0, s>>>(
-      reinterpret_cast<const uint16_t*>(ws + w.y), a.ldo, a.code_scales, a.ld_code_scales, c.ids, c.out, c.ldo, c.tokens,
-      static_cast<int>(c.top_k), w.down.splits, static_cast<int>(c.experts),
-      static_cast<int>(c.hidden), c.ldo % 8 == 0 && aligned(c.out, 16));
+  const auto* y = reinterpret_cast<const uint16_t*>(ws + w.y);
+  const bool vec = c.ldo % 8 == 0 && aligned(c.out, 16);
+  auto sum = [&](auto kernel, int columns, int threads) {
+    const int64_t n = c.tokens * ((c.hidden + columns - 1) / columns);
+    kernel<<<dim3(static_cast<uint32_t>((n + threads - 1) / threads)), threads, 0, s>>>(
+        y, a.ldo, a.code_scales, a.ld_code_scales, c.ids, c.out, c.ldo, c.tokens,
+        static_cast<int>(c.top_k), w.down.splits, static_cast<int>(c.experts),
+        static_cast<int>(c.hidden), vec);
+  };
+  const bool many = c.tokens * c.hidden >= (int64_t(1) << 22);
+  if (w.down.splits > 1)
+    sum(sum_slots<OT, 1, kWave, true>, 8, kWave);
+  else if (many)
+    sum(sum_slots<OT, 2, 256, false>, 16, 256);
+  else
+    sum(sum_slots<OT, 1, kWave, false>, 8, kWave);
   return launch_status("sum_slots");
 }
 

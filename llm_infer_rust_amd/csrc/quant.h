@@ -91,6 +91,69 @@ struct RowQuant {
   }
 };
 
+struct RowsToQuantize {
+  const uint8_t* x;
+  uint8_t* values;
+  float* scales;
+  int64_t stride, ldv, rows;  // stride in bytes
+  int32_t width;
+  bool vec;                   // rows take 16-byte loads
+};
+
+inline RowsToQuantize rows_to_quantize(const void* x, int64_t stride, void* values, int64_t ldv,
+                                       float* scales, int64_t rows, int64_t width) {
+  return {static_cast<const uint8_t*>(x), static_cast<uint8_t*>(values), scales, stride, ldv, rows,
+          static_cast<int32_t>(width), aligned(x, 16) && stride % 16 == 0};
+}
+
+// One row per LANES threads (a wave, or four). The row's first HELD chunks of
+// 16 a thread stay in registers between the two passes, the rest is read again. Bound by memory:
+// every row is read once and written at half its size (8,192 rows of 4,096 bf16: 100 MB). `wave_top` is an LDS word a wave of the workgroup.
+template <int DT, int LANES, int HELD>
+__device__ __forceinline__ void quantize_row(const RowsToQuantize& q, int64_t row,
+                                             uint32_t* wave_top) {
+  static_assert(LANES == kWave || LANES == 4 * kWave, "a wave or four");
+  const int lane = threadIdx.x % LANES;
+  const bool there = row < q.rows;
+  const uint8_t* src = q.x + (there ? row : 0) * q.stride;
+  uint8_t* dst = q.values + row * q.ldv;
+  const int chunks = there ? (q.width + 15) >> 4 : 0;
+  float held[HELD][16];
+  uint32_t top = 0;
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) {
+    const int c = lane + h * LANES;
+    if (c < chunks) {
+      load16<DT>(src, c * 16, q.width - c * 16, q.vec, held[h]);
+      top = max(top, magnitude16(held[h]));
+    }
+  }
+  for (int c = lane + HELD * LANES; c < chunks; c += LANES) {
+    float f[16];
+    load16<DT>(src, c * 16, q.width - c * 16, q.vec, f);
+    top = max(top, magnitude16(f));
+  }
+  top = wave_max(top);
+  if constexpr (LANES > kWave) {
+    wave_top += threadIdx.x / LANES * 4;
+    if (threadIdx.x % kWave == 0) wave_top[threadIdx.x % LANES / kWave] = top;
+    __syncthreads();
+    top = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
+  }
+  const RowQuant form(top);
+  if (there && lane == 0) q.scales[row] = form.scale;
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) {
+    const int c = lane + h * LANES;
+    if (c < chunks) st128(dst + c * 16, form.values(held[h]));
+  }
+  for (int c = lane + HELD * LANES; c < chunks; c += LANES) {
+    float f[16];
+    load16<DT>(src, c * 16, q.width - c * 16, q.vec, f);
+    st128(dst + c * 16, form.values(f));
+  }
+}
+
 // values[r, :] and scales[r] of `rows` rows of `width` elements (dtype 0 bf16, 1 fp16, 2 fp32), row
 // stride in bytes. Columns up to the next multiple of 16 are written as zeros.
 const char* run_quantize_rows(const void* x, int64_t stride, void* values, int64_t ldv,

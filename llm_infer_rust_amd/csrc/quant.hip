@@ -13,71 +13,23 @@
 namespace mi355x {
 namespace {
 
-// One row per LANES threads (a wave, or the whole workgroup of 256). The row's first HELD chunks of
-// 16 a thread stay in registers between the two passes, the rest is read again. Bound by memory:
-// every row is read once and written at half its size (8,192 rows of 4,096 bf16: 100 MB).
 template <int DT, int LANES, int HELD>
-__global__ __launch_bounds__(256) void quantize_rows(const uint8_t* __restrict__ x, int64_t stride,
-                                                     uint8_t* __restrict__ values, int64_t ldv,
-                                                     float* __restrict__ scales, int64_t rows,
-                                                     int width, bool vec) {
-  constexpr int kRows = 256 / LANES;
+__global__ __launch_bounds__(256) void quantize_rows(RowsToQuantize q) {
   __shared__ uint32_t wave_top[4];
-  const int64_t row = blockIdx.x * int64_t(kRows) + threadIdx.x / LANES;
-  const int lane = threadIdx.x % LANES;
-  if (LANES == kWave && row >= rows) return;
-  const uint8_t* src = x + row * stride;
-  uint8_t* dst = values + row * ldv;
-  const int chunks = (width + 15) >> 4;
-  float held[HELD][16];
-  uint32_t top = 0;
-#pragma unroll
-  for (int h = 0; h < HELD; ++h) {
-    const int c = lane + h * LANES;
-    if (c < chunks) {
-      load16<DT>(src, c * 16, width - c * 16, vec, held[h]);
-      top = max(top, magnitude16(held[h]));
-    }
-  }
-  for (int c = lane + HELD * LANES; c < chunks; c += LANES) {
-    float f[16];
-    load16<DT>(src, c * 16, width - c * 16, vec, f);
-    top = max(top, magnitude16(f));
-  }
-  top = wave_max(top);
-  if constexpr (LANES > kWave) {
-    if (threadIdx.x % kWave == 0) wave_top[threadIdx.x / kWave] = top;
-    __syncthreads();
-    top = max(max(wave_top[0], wave_top[1]), max(wave_top[2], wave_top[3]));
-  }
-  const RowQuant q(top);
-  if (lane == 0) scales[row] = q.scale;
-  auto put = [&](int c, const float (&f)[16]) { st128(dst + c * 16, q.values(f)); };
-#pragma unroll
-  for (int h = 0; h < HELD; ++h) {
-    const int c = lane + h * LANES;
-    if (c < chunks) put(c, held[h]);
-  }
-  for (int c = lane + HELD * LANES; c < chunks; c += LANES) {
-    float f[16];
-    load16<DT>(src, c * 16, width - c * 16, vec, f);
-    put(c, f);
-  }
+  const int64_t row = blockIdx.x * int64_t(256 / LANES) + threadIdx.x / LANES;
+  quantize_row<DT, LANES, HELD>(q, row, wave_top);
 }
 
 template <int DT>
-void launch_quantize(const uint8_t* x, int64_t stride, uint8_t* values, int64_t ldv, float* scales,
-                     int64_t rows, int width, bool vec, hipStream_t s) {
+void launch_quantize(const RowsToQuantize& q, hipStream_t s) {
+  const auto rows = static_cast<uint32_t>(q.rows);
   // A wave a row where that keeps the row in registers, a workgroup a row for longer ones.
-  if (width <= 1024)
-    quantize_rows<DT, kWave, 1><<<dim3(static_cast<uint32_t>((rows + 3) / 4)), 256, 0, s>>>(
-        x, stride, values, ldv, scales, rows, width, vec);
-  else if (width <= 4096)
-    quantize_rows<DT, 256, 1><<<dim3(static_cast<uint32_t>(rows)), 256, 0, s>>>(
-        x, stride, values, ldv, scales, rows, width, vec);
+  if (q.width <= 1024)
+    quantize_rows<DT, kWave, 1><<<dim3((rows + 3) / 4), 256, 0, s>>>(q);
+  else if (q.width <= 4096)
+    quantize_rows<DT, 256, 1><<<dim3(rows), 256, 0, s>>>(q);
   else
-    quantize_rows<DT, 256, 3><<<dim3(static_cast<uint32_t>(rows)), 256, 0, s>>>(
-        x, stride, values, ldv, scales, rows, width, vec);
+    quantize_rows<DT, 256, 3><<<dim3(rows), 256, 0, s>>>(q);
 }
 
 constexpr int64_t kMaxInt8K = 131072;  // 127 * 127 * K stays inside int32
@@ -232,15 +184,13 @@ const char* launch_int8(const ProductArgs& base, const Int8Plan& p, int* sums, h
 const char* run_quantize_rows(const void* x, int64_t stride, void* values, int64_t ldv,
                               float* scales, int64_t rows, int64_t width, int dtype,
                               hipStream_t s) {
-  const bool vec = aligned(x, 16) && stride % 16 == 0;
-  const auto* xb = static_cast<const uint8_t*>(x);
-  auto* vb = static_cast<uint8_t*>(values);
+  const RowsToQuantize q = rows_to_quantize(x, stride, values, ldv, scales, rows, width);
   if (dtype == 0)
-    launch_quantize<0>(xb, stride, vb, ldv, scales, rows, static_cast<int>(width), vec, s);
+    launch_quantize<0>(q, s);
   else if (dtype == 1)
-    launch_quantize<1>(xb, stride, vb, ldv, scales, rows, static_cast<int>(width), vec, s);
+    launch_quantize<1>(q, s);
   else
-    launch_quantize<2>(xb, stride, vb, ldv, scales, rows, static_cast<int>(width), vec, s);
+    launch_quantize<2>(q, s);
   return launch_status("quantize_rows");
 }
 

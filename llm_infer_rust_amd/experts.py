@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from ._native import NativeError, check, device_cus, lib, on_device, stream_of
-from .int8 import _ROW_DTYPES, Int8Weight, _check_rows, _refuse_grad, _row_stride
+from .int8 import _ROW_DTYPES, Int8Weight, _output, _refuse_grad, _rows
 
 MAX_EXPERTS = 1024
 MAX_TOP_K = 64
@@ -25,22 +25,21 @@ def route_experts(logits: torch.Tensor, top_k: int,
     or fp32): the ``top_k`` largest probabilities of ``softmax(logits)``, largest first, equal ones
     by the lower index; with ``normalize`` divided by their sum. A row of only -inf gets the
     weights 0, a row with a NaN or a +inf the weights NaN."""
-    _check_rows(logits, "route_experts")
-    if logits.dtype not in _ROW_DTYPES:
+    t, e, ld = _rows(logits, "route_experts")
+    dt = _ROW_DTYPES.get(logits.dtype)
+    if dt is None:
         raise NativeError(
             f"route_experts: expected bfloat16, float16 or float32, got {logits.dtype}")
-    t, e = logits.shape
     top_k = int(top_k)
     if not 0 < e <= MAX_EXPERTS or not 0 < top_k <= min(e, MAX_TOP_K):
         raise NativeError(f"route_experts: expected 1 to {MAX_EXPERTS} experts and top_k of 1 to "
                           f"min(experts, {MAX_TOP_K})")
     _refuse_grad("route_experts", logits)
+    weights = logits.new_empty((t, top_k), dtype=torch.float32)
+    ids = logits.new_empty((t, top_k), dtype=torch.int32)
     with on_device(logits.device):
-        weights = torch.empty((t, top_k), dtype=torch.float32, device=logits.device)
-        ids = torch.empty((t, top_k), dtype=torch.int32, device=logits.device)
-        check(lib().mi355x_route_experts(logits.data_ptr(), _row_stride(logits),
-                                         weights.data_ptr(), ids.data_ptr(), t, e, top_k,
-                                         bool(normalize), _ROW_DTYPES[logits.dtype],
+        check(lib().mi355x_route_experts(logits.data_ptr(), ld, weights.data_ptr(),
+                                         ids.data_ptr(), t, e, top_k, bool(normalize), dt,
                                          stream_of(logits)), "route_experts")
     return weights, ids
 
@@ -57,14 +56,15 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     both of x's type (H, I and x's row stride multiples of 8, 16-byte aligned) or both
     ``Int8Weight`` (any sizes): then x is quantised a token and ``silu(g) * u`` a slot. ``out`` may
     be given; it must not share memory with ``x``."""
-    _check_rows(x, "expert_mlp")
-    dt = _ROW_DTYPES.get(x.dtype)
-    if dt not in (0, 1):
-        raise NativeError(f"expert_mlp: expected bfloat16 or float16 tensor, got {x.dtype}")
-    t, h = x.shape
+    t, h, ldx = _rows(x, "expert_mlp")
+    dtype, device = x.dtype, x.device
+    dt = _ROW_DTYPES.get(dtype)
+    if dt is None or dt == 2:
+        raise NativeError(f"expert_mlp: expected bfloat16 or float16 tensor, got {dtype}")
+    index = device.index
     if (ids.dtype != torch.int32 or weights.dtype != torch.float32 or ids.dim() != 2
-            or ids.size(0) != t or ids.shape != weights.shape or ids.device != x.device
-            or weights.device != x.device or not ids.is_contiguous()
+            or ids.size(0) != t or ids.shape != weights.shape or ids.get_device() != index
+            or weights.get_device() != index or not ids.is_contiguous()
             or not weights.is_contiguous()):
         raise NativeError("expert_mlp: expected contiguous int32 ids and fp32 weights [T, top_k]")
     top_k = ids.size(1)
@@ -74,41 +74,37 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     if int8 != isinstance(down, Int8Weight):
         raise NativeError("expert_mlp: gate_up and down must be of one kind")
     gu, dn = (gate_up.values, down.values) if int8 else (gate_up, down)
-    if (gu.dim() != 3 or dn.dim() != 3 or gu.size(0) != dn.size(0) or gu.size(2) != h
-            or dn.size(1) != h or gu.size(1) != 2 * dn.size(2) or gu.device != x.device
-            or dn.device != x.device or (not int8 and (gu.dtype != x.dtype or dn.dtype != x.dtype
-                                                       or not gu.is_contiguous()
-                                                       or not dn.is_contiguous()))):
+    if (gu.dim() != 3 or dn.dim() != 3 or gu.get_device() != index or dn.get_device() != index
+            or (not int8 and (gu.dtype != dtype or dn.dtype != dtype
+                              or not gu.is_contiguous() or not dn.is_contiguous()))):
         raise NativeError("expert_mlp: expected gate_up [E, 2 I, H] and down [E, H, I] of x's type "
                           "on its device")
-    e, inter = gu.size(0), dn.size(2)
-    if 0 in (e, h, inter) or e > MAX_EXPERTS:
+    e, _, inter = dn.shape
+    if gu.shape != (e, 2 * inter, h) or dn.size(1) != h:
+        raise NativeError(f"expert_mlp: expected gate_up [E, 2 I, {h}] and down [E, {h}, I], got "
+                          f"{tuple(gu.shape)} and {tuple(dn.shape)}")
+    if not e or not h or not inter or e > MAX_EXPERTS:
         raise NativeError(f"expert_mlp: expected 1 to {MAX_EXPERTS} experts of no empty dimension")
-    ldx = _row_stride(x)
-    if not int8 and (h % 8 or inter % 8 or ldx % 8 or x.data_ptr() % 16 or gu.data_ptr() % 16
-                     or dn.data_ptr() % 16):
+    xp, gp, dp = x.data_ptr(), gu.data_ptr(), dn.data_ptr()
+    if not int8 and ((h | inter | ldx) % 8 or (xp | gp | dp) % 16):
         raise NativeError("expert_mlp: 16-bit weights need H, I and x's row stride to be multiples "
                           "of 8 and 16-byte aligned rows")
     _refuse_grad("expert_mlp", x, weights, gu, dn)
-    if out is None:
-        out = torch.empty((t, h), dtype=x.dtype, device=x.device)
-    elif (out.shape != (t, h) or out.dtype != x.dtype or out.device != x.device
-          or (h > 1 and out.stride(1) != 1) or (t > 1 and out.stride(0) < h)):
-        raise NativeError("expert_mlp: invalid output")
-    elif out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
-        raise NativeError("expert_mlp: out must not share memory with x")
-    with on_device(x.device):
-        cus = device_cus(x.device)
-        need = lib().mi355x_expert_mlp_workspace_bytes(t, top_k, e, h, inter, ldx, int8, cus)
-        if need < 0:
-            raise NativeError("expert_mlp: invalid shape")
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=x.device)
-        check(lib().mi355x_expert_mlp(
-            x.data_ptr(), ldx, ids.data_ptr(), weights.data_ptr(), gu.data_ptr(),
-            gate_up.row_stride if int8 else h, gate_up.scales.data_ptr() if int8 else None,
-            dn.data_ptr(), down.row_stride if int8 else inter,
-            down.scales.data_ptr() if int8 else None, out.data_ptr(), _row_stride(out), t, top_k,
-            e, h, inter, ws.data_ptr(), need, cus, dt, stream_of(x)), "expert_mlp")
+    out, ldo = _output(out, x, h, "expert_mlp")
+    cus = device_cus(device)
+    native = lib()
+    need = native.mi355x_expert_mlp_workspace_bytes(t, top_k, e, h, inter, ldx, int8, cus)
+    if need < 0:
+        raise NativeError("expert_mlp: invalid shape")
+    ws = x.new_empty(need or 16, dtype=torch.uint8)
+    ldg, ldd, gs, ds = h, inter, None, None
+    if int8:
+        ldg, ldd = gate_up.row_stride, down.row_stride
+        gs, ds = gate_up.scales.data_ptr(), down.scales.data_ptr()
+    with on_device(device):
+        check(native.mi355x_expert_mlp(
+            xp, ldx, ids.data_ptr(), weights.data_ptr(), gp, ldg, gs, dp, ldd, ds, out.data_ptr(),
+            ldo, t, top_k, e, h, inter, ws.data_ptr(), need, cus, dt, stream_of(x)), "expert_mlp")
     return out
 
 

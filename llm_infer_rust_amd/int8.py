@@ -24,22 +24,39 @@ def _padded(k: int) -> int:
 
 
 def _refuse_grad(what: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise NativeError(f"{what}: no gradient is recorded; call it under torch.no_grad()")
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise NativeError(f"{what}: no gradient is recorded; call it under torch.no_grad()")
 
 
-def _check_rows(x: torch.Tensor, what: str) -> None:
+def _rows(x: torch.Tensor, what: str) -> tuple[int, int, int]:
+    """Rows, columns and row stride of a 2-D GPU tensor of unit column stride whose rows do not
+    overlap. A single row's stride is never used and may be anything: its length stands for it."""
     if not x.is_cuda:
         raise NativeError(f"{what}: expected a GPU tensor")
-    if x.dim() != 2 or (x.size(1) > 1 and x.stride(1) != 1):
+    if x.dim() != 2:
+        raise NativeError(f"{what}: expected rows [T, K]")
+    (t, k), (stride, unit) = x.shape, x.stride()
+    if k > 1 and unit != 1:
         raise NativeError(f"{what}: expected rows [T, K] of unit column stride")
-    if x.size(0) > 1 and x.stride(0) < x.size(1):
+    if t <= 1:
+        return t, k, k
+    if stride < k:
         raise NativeError(f"{what}: rows must not overlap")
+    return t, k, stride
 
 
-def _row_stride(x: torch.Tensor) -> int:
-    """Elements between rows; a single row's stride is never used and may be anything."""
-    return x.stride(0) if x.size(0) > 1 else x.size(1)
+def _output(out: torch.Tensor | None, x: torch.Tensor, width: int,
+            what: str) -> tuple[torch.Tensor, int]:
+    """The output rows ``[T, width]`` of x's type, given or new, and their stride."""
+    t = x.size(0)
+    if out is None:
+        return x.new_empty((t, width)), width
+    if out.shape != (t, width) or out.dtype != x.dtype or out.device != x.device:
+        raise NativeError(f"{what}: invalid output")
+    if out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
+        raise NativeError(f"{what}: out must not share memory with x")
+    return out, _rows(out, what)[2]
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -47,17 +64,16 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     ``scales = max |x| / 127`` and ``values = rint(127 x / max |x|)`` a row (half to even). ``values``
     is a view of rows padded with zeros to 16 columns. A row with an inf or a NaN gets the scale
     NaN, a row of zeros the scale 0."""
-    _check_rows(x, "quantize_rows")
+    t, k, ldx = _rows(x, "quantize_rows")
     if x.dtype not in _ROW_DTYPES:
         raise NativeError(f"quantize_rows: expected bfloat16, float16 or float32, got {x.dtype}")
-    if x.size(1) == 0:
+    if k == 0:
         raise NativeError("quantize_rows: rows must not be empty")
     _refuse_grad("quantize_rows", x)
-    t, k = x.shape
     with on_device(x.device):
         values = torch.empty((t, _padded(k)), dtype=torch.int8, device=x.device)
         scales = torch.empty(t, dtype=torch.float32, device=x.device)
-        check(lib().mi355x_quantize_rows(x.data_ptr(), _row_stride(x), values.data_ptr(),
+        check(lib().mi355x_quantize_rows(x.data_ptr(), ldx, values.data_ptr(),
                                          values.size(1), scales.data_ptr(), t, k,
                                          _ROW_DTYPES[x.dtype], stream_of(x)), "quantize_rows")
     return values[:, :k], scales
@@ -133,37 +149,32 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = 
     projection (gate rows, then up rows) and the result is ``silu(gate) * up`` ``[T, N / 2]``,
     rounded once. Rows may have any stride and alignment; ``out`` may be
     given and must not share memory with ``x``. A row with an inf or a NaN comes out NaN."""
-    _check_rows(x, "linear_int8")
+    t, k, ldx = _rows(x, "linear_int8")
     dt = _ROW_DTYPES.get(x.dtype)
-    if dt not in (0, 1):
+    if dt is None or dt == 2:
         raise NativeError(f"linear_int8: expected bfloat16 or float16 tensor, got {x.dtype}")
     if not isinstance(weight, Int8Weight) or weight.values.dim() != 2:
         raise NativeError("linear_int8: expected an Int8Weight [N, K]")
-    n, k = weight.shape
-    if x.size(1) != k or weight.device != x.device:
+    values, scales = weight.values, weight.scales
+    n = values.size(0)
+    device = x.device
+    if k != values.size(1) or values.get_device() != device.index:
         raise NativeError("linear_int8: expected x [T, K] and a weight [N, K] on one device")
     if silu_mul and n % 2:
         raise NativeError("linear_int8: a gate_up weight has an even number of rows")
     _refuse_grad("linear_int8", x)
-    t, width = x.size(0), n // 2 if silu_mul else n
-    with on_device(x.device):
-        if out is None:
-            out = torch.empty((t, width), dtype=x.dtype, device=x.device)
-        elif (out.shape != (t, width) or out.dtype != x.dtype or out.device != x.device
-              or (width > 1 and out.stride(1) != 1) or (t > 1 and out.stride(0) < width)):
-            raise NativeError("linear_int8: invalid output")
-        elif out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
-            raise NativeError("linear_int8: out must not share memory with x")
-        cus = device_cus(x.device)
-        need = lib().mi355x_linear_int8_workspace_bytes(t, n, k, cus)
-        if need < 0:
-            raise NativeError("linear_int8: invalid shape")
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        check(lib().mi355x_linear_int8(x.data_ptr(), _row_stride(x), weight.values.data_ptr(),
-                                       weight.row_stride, weight.scales.data_ptr(),
-                                       out.data_ptr(), _row_stride(out), t, n, k, silu_mul,
-                                       None if ws is None else ws.data_ptr(), need, cus, dt,
-                                       stream_of(x)), "linear_int8")
+    out, ldo = _output(out, x, n // 2 if silu_mul else n, "linear_int8")
+    cus = device_cus(device)
+    native = lib()
+    need = native.mi355x_linear_int8_workspace_bytes(t, n, k, cus)
+    if need < 0:
+        raise NativeError("linear_int8: invalid shape")
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    with on_device(device):
+        check(native.mi355x_linear_int8(
+            x.data_ptr(), ldx, values.data_ptr(), _padded(k), scales.data_ptr(), out.data_ptr(),
+            ldo, t, n, k, silu_mul, None if ws is None else ws.data_ptr(), need, cus, dt,
+            stream_of(x)), "linear_int8")
     return out
 
 
