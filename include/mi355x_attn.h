@@ -357,8 +357,8 @@ int64_t mi355x_linear_int8_workspace_bytes(int64_t M, int64_t N, int64_t K, int3
  * of x [M, K] (dtype 0 bf16, 1 fp16; out has the same) and w int8 [N, ldw]; the sum is exact
  * in int32. out must not overlap x. With silu_mul, w is a gate_up weight (gate rows, then up rows, N even) and
  * out[m, j] = round(silu(y[m, j]) * y[m, N/2 + j]), y unrounded. K up to 131,072; w rows of
- * whole 16-byte words (columns past K are multiplied with zeros) and less than 4 GiB in all; x
- * and out rows of any stride. Calls that overlap need workspaces of their own. */
+ * whole 16-byte words, ideally 128-byte ones (what a row holds past K is multiplied with zeros), and
+ * less than 4 GiB in all; x and out rows of any stride. Calls that overlap need workspaces of their own. */
 const char* mi355x_linear_int8(const void* x, int64_t ldx, const void* w, int64_t ldw,
                                const float* w_scales, void* out, int64_t ldo, int64_t M,
                                int64_t N, int64_t K, bool silu_mul, void* workspace,
@@ -396,7 +396,7 @@ int64_t mi355x_expert_mlp_workspace_bytes(int64_t tokens, int64_t top_k, int64_t
  * aligned. Sums in fp32; silu(g) * u is rounded to x's type.
  * Scales given (fp32 [experts, 2 inter] and [experts, hidden]): int8 weights. x is quantised once
  * a token, silu(g) * u (kept in fp32) once a slot, both as mi355x_quantize_rows does; any sizes and
- * x strides, weight rows of whole 16-byte words.
+ * x strides, weight rows as for mi355x_linear_int8.
  * Slot outputs on their way to the sum are held in 16 bits under a scale for every 32 columns (to
  * 2^-15 of the largest of them, or in fp32 where there are up to 16 slots).
  * Nothing is read back to the host. An expert's weights are less than 4 GiB. Calls that overlap

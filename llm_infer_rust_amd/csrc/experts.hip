@@ -422,9 +422,9 @@ ExpertWorkspace expert_workspace(int64_t tokens, int64_t top_k, int64_t experts,
   w.counts = take(pad(slots, kGroupChunk) / kGroupChunk * experts * 4);
   w.act = take(slots * (int8 ? pad(inter, 4) * 4 : inter * 2));
   if (int8) {
-    w.xq = take(t * pad(hidden, 16));
+    w.xq = take(t * pad(hidden, 128));
     w.xs = take(t * 4);
-    w.actq = take(slots * pad(inter, 16));
+    w.actq = take(slots * pad(inter, 128));
     w.acts = take(slots * 4);
   }
   w.y = take(slots * w.down.splits * pad(hidden, 32) * 2);
@@ -535,8 +535,8 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   const int64_t slots = c.tokens * c.top_k;
   if (one_by_one(slots, c.top_k, c.hidden, c.inter, kQuant))
     return expert_slots<IN, OT>(c, w, ws, s);
-  const int64_t gate_up_k = kQuant ? pad(c.hidden, 16) : c.hidden * 2;
-  const int64_t down_k = kQuant ? pad(c.inter, 16) : c.inter * 2;
+  const int64_t gate_up_k = kQuant ? int8_k(c.hidden, c.ld_gate_up) : c.hidden * 2;
+  const int64_t down_k = kQuant ? int8_k(c.inter, c.ld_down) : c.inter * 2;
   auto* order = reinterpret_cast<int32_t*>(ws + w.order);
   auto* row_weights = reinterpret_cast<float*>(ws + w.row_weights);
   auto* gate_up_tiles = reinterpret_cast<int4*>(ws + w.gate_up_tiles);
@@ -564,8 +564,8 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
                            chunks};
   auto* xs = reinterpret_cast<float*>(ws + w.xs);
   if constexpr (kQuant) {
-    const RowsToQuantize rows = rows_to_quantize(c.x, c.x_stride, ws + w.xq, pad(c.hidden, 16), xs,
-                                                 c.tokens, c.hidden);
+    const RowsToQuantize rows = rows_to_quantize(c.x, c.x_stride, ws + w.xq, gate_up_k, xs,
+                                                 c.tokens, c.hidden, gate_up_k);
     constexpr int kRows = kGroupThreads / 256;
     place_and_quantize<OT>
         <<<dim3(static_cast<uint32_t>(chunks + (c.tokens + kRows - 1) / kRows)), kGroupThreads, 0,
@@ -587,7 +587,7 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   // gate_up with SiLU x mul into act, one row a slot
   if (kQuant) {
     a.x = ws + w.xq;
-    a.x_stride = pad(c.hidden, 16);
+    a.x_stride = gate_up_k;
     a.x_scales = xs;
     a.k_bytes = static_cast<int32_t>(gate_up_k);
   } else {
@@ -608,11 +608,11 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   if (kQuant) {
     // Every row of act is quantised; rows that no slot wrote (ids that take no part) are never read.
     auto* acts = reinterpret_cast<float*>(ws + w.acts);
-    if (const char* e = run_quantize_rows(ws + w.act, a.ldo * 4, ws + w.actq, pad(c.inter, 16),
-                                          acts, slots, c.inter, kFloatOut, s))
+    if (const char* e = run_quantize_rows(ws + w.act, a.ldo * 4, ws + w.actq, down_k, acts, slots,
+                                          c.inter, down_k, kFloatOut, s))
       return e;
     a.x = ws + w.actq;
-    a.x_stride = pad(c.inter, 16);
+    a.x_stride = down_k;
     a.x_scales = acts;
     a.k_bytes = static_cast<int32_t>(down_k);
   } else {

@@ -96,14 +96,23 @@ struct RowsToQuantize {
   uint8_t* values;
   float* scales;
   int64_t stride, ldv, rows;  // stride in bytes
-  int32_t width;
+  int32_t width, chunks;      // chunks of 16 columns to write, zeros past the width
   bool vec;                   // rows take 16-byte loads
 };
 
 inline RowsToQuantize rows_to_quantize(const void* x, int64_t stride, void* values, int64_t ldv,
-                                       float* scales, int64_t rows, int64_t width) {
+                                       float* scales, int64_t rows, int64_t width,
+                                       int64_t padded) {
   return {static_cast<const uint8_t*>(x), static_cast<uint8_t*>(values), scales, stride, ldv, rows,
-          static_cast<int32_t>(width), aligned(x, 16) && stride % 16 == 0};
+          static_cast<int32_t>(width), static_cast<int32_t>(padded / 16),
+          aligned(x, 16) && stride % 16 == 0};
+}
+
+// K of an int8 product in bytes: the weight rows' elements and, where their stride `ld` holds them, the
+// rest of the last 128-byte step, else of the last 16 bytes. The quantised rows are zeros there.
+inline int64_t int8_k(int64_t k, int64_t ld) {
+  const int64_t steps = (k + 127) / 128 * 128;
+  return ld >= steps ? steps : (k + 15) / 16 * 16;
 }
 
 // One row per LANES threads (a wave, or four). The row's first HELD chunks of
@@ -117,7 +126,7 @@ __device__ __forceinline__ void quantize_row(const RowsToQuantize& q, int64_t ro
   const bool there = row < q.rows;
   const uint8_t* src = q.x + (there ? row : 0) * q.stride;
   uint8_t* dst = q.values + row * q.ldv;
-  const int chunks = there ? (q.width + 15) >> 4 : 0;
+  const int chunks = there ? q.chunks : 0;
   float held[HELD][16];
   uint32_t top = 0;
 #pragma unroll
@@ -155,9 +164,9 @@ __device__ __forceinline__ void quantize_row(const RowsToQuantize& q, int64_t ro
 }
 
 // values[r, :] and scales[r] of `rows` rows of `width` elements (dtype 0 bf16, 1 fp16, 2 fp32), row
-// stride in bytes. Columns up to the next multiple of 16 are written as zeros.
+// stride in bytes. Columns up to `padded`, a multiple of 16, are written as zeros.
 const char* run_quantize_rows(const void* x, int64_t stride, void* values, int64_t ldv,
-                              float* scales, int64_t rows, int64_t width, int dtype,
+                              float* scales, int64_t rows, int64_t width, int64_t padded, int dtype,
                               hipStream_t s);
 
 }  // namespace mi355x

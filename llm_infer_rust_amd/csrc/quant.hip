@@ -86,7 +86,7 @@ Int8Workspace int8_workspace(int64_t M, int64_t N, int64_t K, const Int8Plan& p)
   Int8Workspace w{};
   if (p.kind == Int8Plan::kVec) return w;
   w.values = 0;
-  w.scales = padded16(M * padded16(K));
+  w.scales = M * ((K + 127) / 128 * 128);
   w.sums = w.scales + padded16(M * 4);
   w.bytes = w.sums + (p.splits > 1 ? p.splits * M * (N + 3) / 4 * 4 * 4 + 64 : 0);
   return w;
@@ -182,9 +182,9 @@ const char* launch_int8(const ProductArgs& base, const Int8Plan& p, int* sums, h
 }  // namespace
 
 const char* run_quantize_rows(const void* x, int64_t stride, void* values, int64_t ldv,
-                              float* scales, int64_t rows, int64_t width, int dtype,
+                              float* scales, int64_t rows, int64_t width, int64_t padded, int dtype,
                               hipStream_t s) {
-  const RowsToQuantize q = rows_to_quantize(x, stride, values, ldv, scales, rows, width);
+  const RowsToQuantize q = rows_to_quantize(x, stride, values, ldv, scales, rows, width, padded);
   if (dtype == 0)
     launch_quantize<0>(q, s);
   else if (dtype == 1)
@@ -209,7 +209,7 @@ extern "C" const char* mi355x_quantize_rows(const void* x, int64_t ldx, void* va
   if (!aligned(values, 16) || !aligned(scales, 4) || !aligned(x, dtype == 2 ? 4 : 2))
     return set_error("mi355x_quantize_rows: misaligned operand");
   return run_quantize_rows(x, ldx * (dtype == 2 ? 4 : 2), values, ldv,
-                           static_cast<float*>(scales), rows, width, dtype,
+                           static_cast<float*>(scales), rows, width, padded16(width), dtype,
                            static_cast<hipStream_t>(stream));
 }
 
@@ -272,12 +272,14 @@ extern "C" const char* mi355x_linear_int8(const void* x, int64_t ldx, const void
   }
   auto* base = static_cast<uint8_t*>(workspace);
   auto* scales = reinterpret_cast<float*>(base + ws.scales);
-  if (const char* e = run_quantize_rows(x, ldx * 2, base, padded16(K), scales, M, K,
+  const int64_t k = int8_k(K, ldw);
+  if (const char* e = run_quantize_rows(x, ldx * 2, base, k, scales, M, K, k,
                                         static_cast<int>(dtype), s))
     return e;
+  a.k_bytes = static_cast<int32_t>(k);
   a.x = base;
   a.x_scales = scales;
-  a.x_stride = padded16(K);
+  a.x_stride = k;
   int* sums = reinterpret_cast<int*>(base + ws.sums);
   if (dtype == 0)
     return silu_mul ? launch_int8<0, true>(a, plan, sums, s) : launch_int8<0, false>(a, plan, sums, s);

@@ -17,10 +17,11 @@ from ._native import NativeError, check, device_cus, lib, on_device, stream_of
 
 _ROW_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_K = 131072  # 127 * 127 * K stays inside int32
+_STEP = 128     # bytes of K a product takes at once
 
 
-def _padded(k: int) -> int:
-    return (k + 15) // 16 * 16
+def _padded(k: int, to: int) -> int:
+    return (k + to - 1) // to * to
 
 
 def _refuse_grad(what: str, *tensors: torch.Tensor) -> None:
@@ -54,7 +55,7 @@ def _output(out: torch.Tensor | None, x: torch.Tensor, width: int,
         return x.new_empty((t, width)), width
     if out.shape != (t, width) or out.dtype != x.dtype or out.device != x.device:
         raise NativeError(f"{what}: invalid output")
-    if out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
+    if t and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
         raise NativeError(f"{what}: out must not share memory with x")
     return out, _rows(out, what)[2]
 
@@ -71,7 +72,7 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise NativeError("quantize_rows: rows must not be empty")
     _refuse_grad("quantize_rows", x)
     with on_device(x.device):
-        values = torch.empty((t, _padded(k)), dtype=torch.int8, device=x.device)
+        values = torch.empty((t, _padded(k, 16)), dtype=torch.int8, device=x.device)
         scales = torch.empty(t, dtype=torch.float32, device=x.device)
         check(lib().mi355x_quantize_rows(x.data_ptr(), ldx, values.data_ptr(),
                                          values.size(1), scales.data_ptr(), t, k,
@@ -81,8 +82,8 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 class Int8Weight:
     """int8 ``values`` ``[N, K]`` (or ``[E, N, K]`` for experts) and fp32 ``scales`` ``[N]``
-    (``[E, N]``): the weight ``values * scales[..., None]``. Rows whose length is no multiple of 16
-    are laid out once with a padded stride."""
+    (``[E, N]``): the weight ``values * scales[..., None]``. Rows whose length is no multiple of 128
+    are laid out once with a stride that is, so that every row is whole steps of a product."""
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
         if (values.dtype != torch.int8 or values.dim() not in (2, 3)
@@ -95,8 +96,8 @@ class Int8Weight:
         if 0 in values.shape or values.size(-1) > MAX_K:
             raise NativeError(f"int8 weight: expected 1 to {MAX_K} columns and no empty dimension")
         k = values.size(-1)
-        if k % 16 or not values.is_contiguous() or values.data_ptr() % 16:
-            padded = torch.zeros((*values.shape[:-1], _padded(k)), dtype=torch.int8,
+        if k % _STEP or not values.is_contiguous() or values.data_ptr() % 16:
+            padded = torch.zeros((*values.shape[:-1], _padded(k, _STEP)), dtype=torch.int8,
                                  device=values.device)
             padded[..., :k] = values
             values = padded[..., :k]
@@ -109,18 +110,8 @@ class Int8Weight:
         if weight.dim() not in (2, 3):
             raise NativeError("int8 weight: expected [N, K] or [E, N, K]")
         values, scales = quantize_rows(weight.detach().reshape(-1, weight.size(-1)))
-        stride = values.stride(0)
-        n = weight.size(-2)
-        shape, strides = tuple(weight.shape), (stride, 1)
-        if weight.dim() == 3:
-            strides = (n * stride, stride, 1)
-        return Int8Weight._of(values.as_strided(shape, strides), scales.view(shape[:-1]))
-
-    @staticmethod
-    def _of(values: torch.Tensor, scales: torch.Tensor) -> "Int8Weight":
-        weight = Int8Weight.__new__(Int8Weight)
-        weight.values, weight.scales = values, scales
-        return weight
+        return Int8Weight(values.view(weight.shape) if values.is_contiguous()
+                          else values.reshape(weight.shape), scales.view(weight.shape[:-1]))
 
     @property
     def shape(self) -> torch.Size:
@@ -132,8 +123,8 @@ class Int8Weight:
 
     @property
     def row_stride(self) -> int:
-        """Bytes between rows, a multiple of 16."""
-        return _padded(self.shape[-1])
+        """Bytes between rows, a multiple of 128."""
+        return _padded(self.values.size(-1), _STEP)
 
     def size(self, dim: int) -> int:
         return self.values.size(dim)
@@ -172,9 +163,9 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = 
     ws = x.new_empty(need, dtype=torch.uint8) if need else None
     with on_device(device):
         check(native.mi355x_linear_int8(
-            x.data_ptr(), ldx, values.data_ptr(), _padded(k), scales.data_ptr(), out.data_ptr(),
-            ldo, t, n, k, silu_mul, None if ws is None else ws.data_ptr(), need, cus, dt,
-            stream_of(x)), "linear_int8")
+            x.data_ptr(), ldx, values.data_ptr(), _padded(k, _STEP), scales.data_ptr(),
+            out.data_ptr(), ldo, t, n, k, silu_mul, None if ws is None else ws.data_ptr(), need,
+            cus, dt, stream_of(x)), "linear_int8")
     return out
 
 

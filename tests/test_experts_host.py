@@ -52,7 +52,7 @@ def test_entries_refuse_bad_arguments_before_launching():
 
     ws = f.mi355x_linear_int8_workspace_bytes
     assert ws(1, 64, 4096, 256) == 0 and ws(0, 64, 64, 256) == 0
-    assert ws(40, 64, 100, 256) >= 40 * 112 + 160
+    assert ws(40, 64, 100, 256) >= 40 * 128 + 160
     assert ws(40, 64, int8.MAX_K + 1, 256) == -1 and ws(-1, 64, 64, 256) == -1
     # K split in parts where the tiles would leave most compute units idle
     assert ws(64, 4096, 12288, 256) >= 64 * 12288 + 2 * 64 * 4096 * 4

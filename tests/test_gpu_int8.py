@@ -167,8 +167,28 @@ def test_weights(gpu):
     assert torch.equal(weight.values.cpu().double().view(30, 37), q)
     assert weight.shape == (3, 10, 37) and weight.scales.shape == (3, 10)
     again = int8.Int8Weight(weight.values.contiguous(), weight.scales)
-    assert torch.equal(again.values, weight.values) and again.row_stride == 48
+    assert torch.equal(again.values, weight.values) and again.row_stride == 128
     assert torch.allclose(weight.dequantize().cpu().double().view(30, 37), q * s, rtol=1e-6)
+
+
+def test_weight_rows_of_whole_16_byte_words(gpu):
+    """The C entry takes rows that end inside a 128-byte step too: K = 150 in rows of 160 bytes, the
+    padding of any value."""
+    from llm_infer_rust_amd._native import check as ok, lib
+    g = gen(9)
+    for t in (2, 9, 70, 600):
+        x = torch.randn(t, 150, generator=g).to(torch.bfloat16).to(gpu)
+        padded = torch.randint(-128, 128, (200, 160), generator=g, dtype=torch.int8).to(gpu)
+        scales = torch.rand(200, generator=g).to(gpu)
+        want = int8.linear_int8(x, int8.Int8Weight(padded[:, :150], scales))
+        out = torch.empty_like(want)
+        need = lib().mi355x_linear_int8_workspace_bytes(t, 200, 150, 256)
+        ws = torch.empty(need + 16, dtype=torch.uint8, device=gpu)
+        ok(lib().mi355x_linear_int8(x.data_ptr(), 150, padded.data_ptr(), 160, scales.data_ptr(),
+                                    out.data_ptr(), 200, t, 200, 150, False, ws.data_ptr(), need,
+                                    256, 0, torch.cuda.current_stream().cuda_stream), "linear")
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
 
 
 def test_empty_batch_and_refusals(gpu):
