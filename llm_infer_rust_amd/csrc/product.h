@@ -980,15 +980,18 @@ __global__ __launch_bounds__(256) void product_rows(ProductArgs a) {
 }
 
 // ---------------------------------------------------------------------------- the choice of tiles
-// The tiles that a product can take, smallest first.
-enum class Tile { k64, k128, k256x128, k256 };
+// The tiles that a product can take, smallest first. k128 has four stages and a CU for itself, k128Two
+// has two stages and shares the CU with another.
+enum class Tile { k64, k128, k128Two, k256x128, k256 };
+constexpr int kTiles = 5;
 
 struct TileShape {
   int bm, bn;        // rows of x, weight rows
   float step, busy;  // us a 128-byte step: with few workgroups, and what a full chip adds
 };
 constexpr TileShape kTileShapes[] = {
-    {64, 64, 0.29f, 0.f}, {128, 128, 0.5f, 0.2f}, {256, 128, 0.8f, 0.3f}, {256, 256, 1.2f, 0.6f}};
+    {64, 64, 0.29f, 0.f},   {128, 128, 0.5f, 0.2f},  {128, 128, 0.58f, 0.f},
+    {256, 128, 0.8f, 0.3f}, {256, 256, 1.2f, 0.6f}};
 
 // Estimated time in us of `row_tiles` x `column_tiles` tiles over K. A CU's copies into LDS come at
 // about 60 GB/s where they miss L2, whatever the depth of the ring, which makes the step of a tile
@@ -1007,6 +1010,8 @@ inline float tile_estimate(Tile tile, float row_tiles, float column_tiles, int64
   if (tile == Tile::k256 && half) step = 0.65f + 0.8f * busy;
   if (tile == Tile::k64) {
     if (r > 1.f) rounds = std::max(1.07f * r - 0.07f, std::min(2.f, 1.f + 2.5f * (r - 1.f)));
+  } else if (tile == Tile::k128Two) {
+    rounds = std::max(2.f, r + 0.3f);
   } else if (r > 1.06f) {
     rounds = r <= 3.f ? std::ceil(r - 0.06f) : r + 0.3f;
   }

@@ -58,7 +58,7 @@ Int8Plan int8_plan(int64_t M, int64_t N, int64_t K, int cus) {
     best = {Int8Plan::kRows, Tile::k64, 1};
     best_us = 3.f + std::max(0.18f * steps * rounds, weights / 5.8e6f);
   }
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kTiles; ++i) {
     const TileShape& t = kTileShapes[i];
     const float tm = static_cast<float>((M + t.bm - 1) / t.bm);
     const float tn = static_cast<float>((N + t.bn - 1) / t.bn);
@@ -143,7 +143,9 @@ void launch_int8_tiles(ProductArgs& a, Tile tile, hipStream_t s) {
   } else if (tile == Tile::k128) {
     product_tile<kInt8, OT, MODE, SILU, 128, 128, 4, 2, 4><<<g, 512, 0, s>>>(a);
   } else if constexpr (MODE == kDense) {
-    if (tile == Tile::k256x128)
+    if (tile == Tile::k128Two)
+      product_tile<kInt8, OT, MODE, SILU, 128, 128, 4, 2, 2><<<g, 512, 0, s>>>(a);
+    else if (tile == Tile::k256x128)
       product_tile<kInt8, OT, MODE, SILU, 256, 128, 4, 2, 3><<<g, 512, 0, s>>>(a);
     else if (a.k_bytes % kProdRow)
       product_large<kInt8, OT, MODE, SILU, 256, 8, true><<<g, 512, 0, s>>>(a);
