@@ -172,6 +172,24 @@ def test_expert_mlp(gpu, dtype, t, e, k, h, i):
     check16(got, *p, gpu)
 
 
+# The larger tiles, chosen by size: 128 x 128 for both products, 256 x 256 (groups of rows that end in a
+# half tile and in a whole one) for either, with K in whole 128-byte steps and not; the most slots a
+# token, one expert, and more experts than slots.
+LARGE = [(1200, 2, 2, 72, 1032), (1200, 2, 2, 2056, 72), (600, 16, 2, 72, 1032), (600, 16, 2, 2056, 72),
+         (2500, 6, 2, 1032, 520), (3000, 3, 2, 512, 1024), (1, 64, 64, 64, 64), (5, 64, 64, 72, 40),
+         (33, 1, 1, 128, 64), (700, 1, 1, 128, 64), (50, 1024, 3, 64, 32)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,e,k,h,i", LARGE)
+def test_expert_mlp_of_many_rows(gpu, dtype, t, e, k, h, i):
+    p = problem(t, e, k, h, i, dtype, t * 7 + e)
+    out = torch.full((t + 1, h + 8), 7.0, dtype=dtype, device=gpu)
+    got = experts.expert_mlp(*(a.to(gpu) for a in p), out=out[:t, :h])
+    check16(got, *p, gpu)
+    assert bool((out[t] == 7).all()) and bool((out[:, h:] == 7).all())
+
+
 @pytest.mark.parametrize("t,e,k", [(6, 12, 4), (300, 16, 4), (3000, 8, 4)])
 def test_ids_outside_add_nothing(gpu, t, e, k):
     x, ids, w, gu, dn = problem(t, e, k, 128, 64, torch.bfloat16, t)
@@ -265,6 +283,108 @@ def test_expert_mlp_int8(gpu, dtype, t, e, k, h, i):
     check8(got, x, ids, w, gu8, dn8, gpu)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,e,k,h,i", LARGE + [(1200, 2, 2, 2055, 67), (600, 16, 2, 71, 1033),
+                                                (600, 16, 2, 2055, 131)])
+def test_expert_mlp_int8_of_many_rows(gpu, dtype, t, e, k, h, i):
+    x, ids, w, gu, dn = problem(t, e, k, h, i, dtype, t * 5 + e)
+    gu8, dn8 = (int8.Int8Weight.quantize(m.to(gpu)) for m in (gu, dn))
+    out = torch.full((t + 1, h + 8), 7.0, dtype=dtype, device=gpu)
+    got = experts.expert_mlp(x.to(gpu), ids.to(gpu), w.to(gpu), gu8, dn8, out=out[:t, :h])
+    check8(got, x, ids, w, gu8, dn8, gpu)
+    assert bool((out[t] == 7).all()) and bool((out[:, h:] == 7).all())
+
+
+@pytest.mark.parametrize("t", [1, 40, 600])
+def test_weights_of_more_than_four_gib(gpu, t):
+    """Experts 0 and 19 of 20 whose matrices start up to 5 GB behind the first."""
+    h, i = 8192, 8192
+    gu = torch.zeros(20, 2 * i, h, dtype=torch.bfloat16, device=gpu)
+    dn = torch.zeros(20, h, i, dtype=torch.bfloat16, device=gpu)
+    g = torch.Generator(device=gpu).manual_seed(t)
+    for e in (0, 19):
+        gu[e].normal_(0, h ** -0.5, generator=g)
+        dn[e].normal_(0, i ** -0.5, generator=g)
+    x = torch.randn(t, h, generator=g, device=gpu).to(torch.bfloat16)
+    ids = torch.randint(0, 2, (t, 2), generator=g, device=gpu, dtype=torch.int32)
+    w = torch.rand(t, 2, generator=g, device=gpu)
+    got = experts.expert_mlp(x, ids * 19, w, gu, dn)
+    check16(got, x, ids, w, gu[::19], dn[::19], gpu)
+
+
+@pytest.mark.parametrize("h,i", [(64, 17408), (17408, 64)])
+@pytest.mark.parametrize("i8", [False, True])
+def test_slots_of_more_than_four_gib(gpu, h, i, i8):
+    """65,536 tokens of two slots: 131,072 rows of 34 KB between the products, or behind them. The
+    tokens that are checked have their slots at both ends of the grouped order."""
+    t = 65536
+    g = torch.Generator(device=gpu).manual_seed(h)
+    x = torch.randn(t, h, generator=g, device=gpu).to(torch.bfloat16)
+    gu = (torch.randn(2, 2 * i, h, generator=g, device=gpu) * h ** -0.5).to(torch.bfloat16)
+    dn = (torch.randn(2, h, i, generator=g, device=gpu) * i ** -0.5).to(torch.bfloat16)
+    ids = torch.tensor([0, 1], dtype=torch.int32, device=gpu).repeat(t, 1)
+    w = torch.rand(t, 2, generator=g, device=gpu)
+    if i8:
+        gu, dn = int8.Int8Weight.quantize(gu), int8.Int8Weight.quantize(dn)
+    got = experts.expert_mlp(x, ids, w, gu, dn)
+    some = torch.tensor([0, 1, 777, t // 2, t - 300, t - 2, t - 1], device=gpu)
+    (check8 if i8 else check16)(got[some], x[some], ids[some], w[some], gu, dn, gpu)
+
+
+@pytest.mark.parametrize("k", [2, 20])
+def test_rows_gigabytes_apart(gpu, k):
+    x, ids, w, gu, dn = (a.to(gpu) for a in problem(3, 32, k, 128, 64, torch.bfloat16, k))
+    wide = torch.empty((2 << 30) + 4096, dtype=torch.bfloat16, device=gpu)
+    rows = wide.as_strided((3, 128), ((1 << 30) + 8, 1))
+    rows.copy_(x)
+    check16(experts.expert_mlp(rows, ids, w, gu, dn), x, ids, w, gu, dn, gpu)
+    gu8, dn8 = int8.Int8Weight.quantize(gu), int8.Int8Weight.quantize(dn)
+    check8(experts.expert_mlp(rows, ids, w, gu8, dn8), x, ids, w, gu8, dn8, gpu)
+    weights, chosen = experts.route_experts(rows, 5)
+    want, want_ids = experts.route_experts(x, 5)
+    assert torch.equal(weights, want) and torch.equal(chosen, want_ids)
+
+
+@pytest.mark.parametrize("t", [3, 60, 1200])
+def test_infinite_weights(gpu, t):
+    """An infinity in `down` reaches its column and no other; the 32 columns that share its scale are
+    then held in bf16, half a step of 2^-9 for each slot of the expert."""
+    x, ids, w, gu, dn = problem(t, 2, 2, 2056, 72, torch.bfloat16, t)
+    dn[1, 40, 3] = float("inf")
+    got = experts.expert_mlp(*(a.to(gpu) for a in (x, ids, w, gu, dn)))
+    assert not bool(got[:, 40].isfinite().any())
+    rest = [c for c in range(2056) if c != 40]
+    assert bool(got[:, rest].isfinite().all())
+    dn[1, 40, 3] = 0.0
+    out, terms, first = reference(x, ids, w, gu, dn, gpu)
+    half = 2.0 ** -8
+    bound = terms * (half * 1.01 + 80 * 2.0 ** -24) + out.abs() * half * 1.01 + first * 1.01
+    bound[:, 32:64] += terms[:, 32:64] * 2.0 ** -8
+    err = (got.double() - out).abs()[:, rest]
+    assert bool((err <= bound[:, rest]).all()), float((err / bound[:, rest]).max())
+
+
+def test_two_streams_at_once(gpu):
+    jobs = []
+    for t, h, i, i8 in ((2, 128, 64, False), (40, 104, 2056, False), (90, 128, 64, True),
+                        (600, 2056, 72, False), (1200, 72, 1032, True)):
+        x, ids, w, gu, dn = (a.to(gpu) for a in problem(t, 4, 2, h, i, torch.bfloat16, t))
+        if i8:
+            gu, dn = int8.Int8Weight.quantize(gu), int8.Int8Weight.quantize(dn)
+        args = (x, ids, w, gu, dn)
+        jobs.append((args, experts.expert_mlp(*args)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[] for _ in jobs]
+    for _ in range(10):
+        for (args, _), stream, mine in zip(jobs, streams, got):
+            with torch.cuda.stream(stream):
+                mine.append(experts.expert_mlp(*args))
+    torch.cuda.synchronize()
+    for (_, want), mine in zip(jobs, got):
+        assert all(torch.equal(want, out) for out in mine)
+
+
 def test_more_slots_than_a_pass_takes(gpu):
     t, k = 9000, 16  # 144,000 slots: two passes
     x, ids, w, gu, dn = problem(t, 32, k, 64, 64, torch.bfloat16, 1)
@@ -285,6 +405,8 @@ def test_empty_batch_and_refusals(gpu):
                  (x, ids[:, :0], w[:, :0], gu, dn), (x.clone().requires_grad_(), ids, w, gu, dn)):
         with pytest.raises(NativeError):
             experts.expert_mlp(*args)
+    none = torch.empty(0, 64, dtype=x.dtype, device=gpu)
+    assert experts.expert_mlp(x[:0], ids[:0], w[:0], gu, dn, out=none).shape == (0, 64)
     with pytest.raises(NativeError):
         experts.expert_mlp(x, ids, w, gu, dn, out=x)
     with pytest.raises(NativeError):

@@ -116,6 +116,27 @@ def test_linear_int8(gpu, dtype, t, n, k, silu):
     check(int8.linear_int8(x.to(gpu), weight, silu_mul=silu), x, weight, silu)
 
 
+# Every tile and split that is chosen by size: 64 x 64 in two and four parts of K, 128 x 128 whole, in
+# parts and two a compute unit, 256 x 128, 256 x 256 (with a row tile of half the rows and with one of
+# more), ragged in every dimension.
+LARGE = [(1040, 258, 4110), (64, 4100, 4110), (1030, 2050, 65), (130, 8198, 4110), (1290, 6146, 65),
+         (4100, 1028, 65), (1550, 6146, 65), (1630, 6146, 129), (2500, 4098, 640)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,n,k", LARGE)
+@pytest.mark.parametrize("silu", [False, True])
+def test_linear_int8_of_many_rows(gpu, dtype, t, n, k, silu):
+    g = torch.Generator(device=gpu).manual_seed(t + n + k)
+    x = torch.randn(t, k, generator=g, device=gpu).to(dtype)
+    weight = int8.Int8Weight.quantize(torch.randn(n, k, generator=g, device=gpu) * k ** -0.5)
+    out = torch.full((t + 1, n), 7.0, dtype=dtype, device=gpu)
+    width = n // 2 if silu else n
+    got = int8.linear_int8(x, weight, out=out[:t, :width], silu_mul=silu)
+    check(got, x, weight, silu)
+    assert bool((out[t] == 7).all()) and bool((out[:, width:] == 7).all())
+
+
 @pytest.mark.parametrize("t", [1, 40, 300])
 def test_extreme_values_do_not_overflow(gpu, t):
     """K at the longest that is taken, every product 127 * 127: the int32 sum is 2,114,076,672."""
@@ -176,16 +197,16 @@ def test_weight_rows_of_whole_16_byte_words(gpu):
     padding of any value."""
     from llm_infer_rust_amd._native import check as ok, lib
     g = gen(9)
-    for t in (2, 9, 70, 600):
+    for t, n in ((2, 200), (9, 200), (70, 200), (600, 200), (1290, 6146), (1550, 6146)):
         x = torch.randn(t, 150, generator=g).to(torch.bfloat16).to(gpu)
-        padded = torch.randint(-128, 128, (200, 160), generator=g, dtype=torch.int8).to(gpu)
-        scales = torch.rand(200, generator=g).to(gpu)
+        padded = torch.randint(-128, 128, (n, 160), generator=g, dtype=torch.int8).to(gpu)
+        scales = torch.rand(n, generator=g).to(gpu)
         want = int8.linear_int8(x, int8.Int8Weight(padded[:, :150], scales))
         out = torch.empty_like(want)
-        need = lib().mi355x_linear_int8_workspace_bytes(t, 200, 150, 256)
+        need = lib().mi355x_linear_int8_workspace_bytes(t, n, 150, 256)
         ws = torch.empty(need + 16, dtype=torch.uint8, device=gpu)
         ok(lib().mi355x_linear_int8(x.data_ptr(), 150, padded.data_ptr(), 160, scales.data_ptr(),
-                                    out.data_ptr(), 200, t, 200, 150, False, ws.data_ptr(), need,
+                                    out.data_ptr(), n, t, n, 150, False, ws.data_ptr(), need,
                                     256, 0, torch.cuda.current_stream().cuda_stream), "linear")
         torch.cuda.synchronize()
         assert torch.equal(out, want)
@@ -214,6 +235,46 @@ def test_empty_batch_and_refusals(gpu):
             bad()
 
 
+def test_rows_gigabytes_apart(gpu):
+    wide = torch.empty((2 << 30) + 4096, dtype=torch.bfloat16, device=gpu)
+    rows = wide.as_strided((3, 250), ((1 << 30) + 5, 1))
+    rows.copy_(torch.randn(3, 250, generator=gen(3)))
+    weight = int8.Int8Weight.quantize(torch.randn(66, 250, generator=gen(4)).to(gpu))
+    assert torch.equal(int8.linear_int8(rows, weight), int8.linear_int8(rows.contiguous(), weight))
+    values, scales = int8.quantize_rows(rows)
+    want, want_scales = int8.quantize_rows(rows.contiguous())
+    assert torch.equal(values, want) and torch.equal(scales, want_scales)
+
+
+def test_given_output_of_no_rows_and_one(gpu):
+    weight = int8.Int8Weight.quantize(torch.randn(8, 32, generator=gen(1)).to(gpu))
+    x = torch.randn(1, 32, generator=gen(2)).to(torch.float16).to(gpu)
+    out = torch.empty(0, 8, dtype=x.dtype, device=gpu)
+    assert int8.linear_int8(x[:0], weight, out=out).shape == (0, 8)
+    out = torch.full((1, 11), 7.0, dtype=x.dtype, device=gpu)
+    assert torch.equal(int8.linear_int8(x, weight, out=out[:, 2:10]), int8.linear_int8(x, weight))
+    assert out[0, :2].tolist() == [7.0] * 2 and float(out[0, 10]) == 7.0
+
+
+def test_two_streams_at_once(gpu):
+    """Calls with and without a split K, each stream's results as if it ran alone."""
+    jobs = []
+    for t, n, k in ((64, 4100, 4110), (1, 512, 1000), (40, 258, 300), (1550, 6146, 65)):
+        x = torch.randn(t, k, generator=gen(t)).to(torch.bfloat16).to(gpu)
+        weight = int8.Int8Weight.quantize(torch.randn(n, k, generator=gen(n)).to(gpu))
+        jobs.append((x, weight, int8.linear_int8(x, weight)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[] for _ in jobs]
+    for _ in range(10):
+        for (x, weight, _), stream, mine in zip(jobs, streams, got):
+            with torch.cuda.stream(stream):
+                mine.append(int8.linear_int8(x, weight))
+    torch.cuda.synchronize()
+    for (_, _, want), mine in zip(jobs, got):
+        assert all(torch.equal(want, out) for out in mine)
+
+
 def test_captured_replays(gpu):
     calls = []
     for t in (1, 48, 300):
@@ -230,3 +291,22 @@ def test_captured_replays(gpu):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, int8.linear_int8(x, weight))
+
+
+def test_captured_replays_of_a_split_product(gpu):
+    calls = []
+    for seed in (1, 2):  # two graphs with workspaces of their own
+        weight = int8.Int8Weight.quantize(torch.randn(4100, 4110, generator=gen(seed)).to(gpu))
+        x = torch.randn(64, 4110, generator=gen(seed + 2)).to(torch.bfloat16).to(gpu)
+        int8.linear_int8(x, weight, silu_mul=True)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = int8.linear_int8(x, weight, silu_mul=True)
+        calls.append((x, weight, graph, out))
+    for r in range(3):
+        for x, _, graph, _ in calls:
+            x.copy_(torch.randn(x.shape, generator=gen(r)).to(x.dtype))
+            graph.replay()
+        torch.cuda.synchronize()
+        for x, weight, _, out in calls:
+            assert torch.equal(out, int8.linear_int8(x, weight, silu_mul=True))
