@@ -136,52 +136,51 @@ __device__ __forceinline__ void store4(void* out, int64_t at, const float (&v)[4
 }
 
 // Slot outputs on their way to the sum over a token's slots: a signed 16-bit mantissa a value under a
-// power of two for every 32 columns. Half a unit is 2^-15 of the largest of the 32 or less, where bf16 would round every value by 2^-9 and cost the layer's output a third of its error
-// (relative to 64 bits 2.9e-3 in bf16, so 2.4e-3), at the traffic of 16 bits: fp32 slots would be
-// 0.5 GB more of it in an 8,192-token prefill, some 100 us of 780. Where a value is inf or NaN the scale
-// is inf and the 32 values are plain bf16.
+// power of two for every 32 columns. Half a unit is 2^-15 of the largest of the 32 or less, where bf16
+// would round every value by 2^-9 and cost the layer's output a third of its accuracy (relative to 64 bits
+// 2.9e-3 in bf16, so 2.4e-3), at the traffic of 16 bits: fp32 slots would be 0.5 GB more of it in an
+// 8,192-token prefill, some 100 us of 780. Where a value is inf or NaN the scale is inf and the 32 values
+// are plain bf16.
 struct SlotCode {
-  float factor, highest;
-  uint16_t scale;  // bf16
-
-  __device__ __forceinline__ SlotCode() {}
-  // of the largest magnitude, as its bits
-  __device__ __forceinline__ explicit SlotCode(uint32_t top) {
-    const uint32_t e = max(top >> 23, 15u);               // 2^(e - 126) is above the largest
-    factor = __uint_as_float((268u - e) << 23);           // 2^(141 - e): to below 2^15
-    highest = 32767.f * __uint_as_float((e - 14) << 23);  // the last half unit has no code
-    scale = top >= 0x7f800000u ? 0x7f80 : (e - 14) << 7;  // 2^(e - 141)
-  }
-  __device__ __forceinline__ bool plain() const { return scale == 0x7f80; }
-  // Two values; 1.5 * 2^23 rounds them to integers in the low bits.
-  __device__ __forceinline__ uint32_t pack(float a, float b) const {
-    const uint32_t lo = __float_as_uint(fmaf(fminf(a, highest), factor, 12582912.f));
-    const uint32_t hi = __float_as_uint(fmaf(fminf(b, highest), factor, 12582912.f));
-    return __builtin_amdgcn_perm(hi, lo, 0x05040100);
-  }
-  // The codes of a lane's 16 values, two a word.
-  __device__ __forceinline__ void pack16(const float (&v)[16], uint32_t (&w)[8]) const {
+  // The codes of a lane's 16 values v * scale, two a word; lane ^ 32 holds the other 16 of the 32
+  // columns. Returns the power of two as bf16.
+  __device__ __forceinline__ static uint16_t pack(const float (&v)[16], float scale,
+                                                  uint32_t (&w)[8]) {
+    float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = pack(v[2 * i], v[2 * i + 1]);
-    if (__any(plain())) {  // seldom
+    for (int i = 0; i < 16; i += 2) most = fmaxf(fmaxf(most, fabsf(v[i])), fabsf(v[i + 1]));
+    const uint32_t top = joined(__float_as_uint(most * fabsf(scale)), true);
+    // The largest comes to below 2^15 with a margin for the rounding to an integer.
+    const uint32_t e = max((top + 0x180) >> 23, 15u);
+    const float factor = scale * __uint_as_float((268u - e) << 23);  // 2^(141 - e)
+    // 1.5 * 2^23 rounds to integers in the low bits. What is not finite leaves its exponent here.
+    uint32_t seen = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t lo = __float_as_uint(fmaf(v[2 * i], factor, 12582912.f));
+      const uint32_t hi = __float_as_uint(fmaf(v[2 * i + 1], factor, 12582912.f));
+      seen |= lo | hi;
+      w[i] = __builtin_amdgcn_perm(hi, lo, 0x05040100);
+    }
+    const bool plain = (joined(seen, false) & 0x34000000u) != 0 || top >= 0x7f800000u;
+    if (__any(plain)) {  // seldom
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (plain()) w[i] = Elem<kBf16>::pack2(v[2 * i], v[2 * i + 1]);
+        if (plain) w[i] = Elem<kBf16>::pack2(v[2 * i] * scale, v[2 * i + 1] * scale);
     }
+    return plain ? 0x7f80 : (e - 14) << 7;  // 2^(e - 141)
   }
   __device__ __forceinline__ static float value(uint16_t code, float scale) {
     return static_cast<float>(static_cast<int16_t>(code)) * scale;
   }
-};
 
-// The largest magnitude of a lane's 16 values and those of lane ^ 32: the 32 columns of a row.
-__device__ __forceinline__ uint32_t block_magnitude(const float (&v)[16]) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 16; i += 2)
-    top = max(max(top, __float_as_uint(v[i]) & 0x7fffffffu), __float_as_uint(v[i + 1]) & 0x7fffffffu);
-  return max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
-}
+ private:
+  // With the word of lane ^ 32: the larger, or the bits of both.
+  __device__ __forceinline__ static uint32_t joined(uint32_t x, bool larger) {
+    const auto both = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return larger ? max(both[0], both[1]) : both[0] | both[1];
+  }
+};
 
 // What a row of a tile is multiplied with and where it goes.
 struct RowOut {
@@ -527,15 +526,14 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
         float v[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          v[e] = static_cast<float>(acc[i][j][e]) * (r.scale * r.weight);
+          v[e] = static_cast<float>(acc[i][j][e]);
           if constexpr (IN == kInt8)
             v[e] *= w_scales[min(column + 8 * (e >> 2) + 4 * half + (e & 3), a.columns - 1)];
         }
-        const SlotCode code(block_magnitude(v));
-        if (column >= a.columns) continue;
-        if (half == 0) a.code_scales[r.at * a.ld_code_scales + column / 32] = code.scale;
         uint32_t w[8];
-        code.pack16(v, w);
+        const uint16_t scale = SlotCode::pack(v, r.scale * r.weight, w);
+        if (column >= a.columns) continue;
+        if (half == 0) a.code_scales[r.at * a.ld_code_scales + column / 32] = scale;
         // ldo is a multiple of 32: codes past the end have their place
         uint16_t* p = static_cast<uint16_t*>(a.out) + r.at * a.ldo + column + 4 * half;
 #pragma unroll
@@ -762,7 +760,7 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float g = static_cast<float>(acc[i][j][4 * q + e]);
-          if constexpr (IN == kInt8 || MODE == kDown) g *= row_scale;
+          if constexpr (IN == kInt8 && MODE != kDown) g *= row_scale;
           if constexpr (IN == kInt8) g *= gs[e];
           if constexpr (SILU) {
             float u = static_cast<float>(acc[i][j][(4 * q + 4 + e) & 15]);
@@ -774,9 +772,7 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
       }
       uint32_t codes[8];
       if constexpr (MODE == kDown) {
-        const SlotCode code(block_magnitude(f));
-        code.pack16(f, codes);
-        scales |= static_cast<uint32_t>(code.scale) << (16 * i);
+        scales |= static_cast<uint32_t>(SlotCode::pack(f, row_scale, codes)) << (16 * i);
       }
 #pragma unroll
       for (int q = 0; q < 4; q += SILU ? 2 : 1) {

@@ -35,9 +35,10 @@ def route_experts(logits: torch.Tensor, top_k: int,
         raise NativeError(f"route_experts: expected 1 to {MAX_EXPERTS} experts and top_k of 1 to "
                           f"min(experts, {MAX_TOP_K})")
     _refuse_grad("route_experts", logits)
-    weights = logits.new_empty((t, top_k), dtype=torch.float32)
-    ids = logits.new_empty((t, top_k), dtype=torch.int32)
-    with on_device(logits.device):
+    device = logits.device
+    weights = torch.empty(t, top_k, dtype=torch.float32, device=device)
+    ids = torch.empty(t, top_k, dtype=torch.int32, device=device)
+    with on_device(device):
         check(lib().mi355x_route_experts(logits.data_ptr(), ld, weights.data_ptr(),
                                          ids.data_ptr(), t, e, top_k, bool(normalize), dt,
                                          stream_of(logits)), "route_experts")
@@ -96,7 +97,7 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     need = native.mi355x_expert_mlp_workspace_bytes(t, top_k, e, h, inter, ldx, int8, cus)
     if need < 0:
         raise NativeError("expert_mlp: invalid shape")
-    ws = x.new_empty(need or 16, dtype=torch.uint8)
+    ws = torch.empty(need or 16, dtype=torch.uint8, device=device)
     ldg, ldd, gs, ds = h, inter, None, None
     if int8:
         ldg, ldd = gate_up.row_stride, down.row_stride

@@ -52,7 +52,7 @@ def _output(out: torch.Tensor | None, x: torch.Tensor, width: int,
     """The output rows ``[T, width]`` of x's type, given or new, and their stride."""
     t = x.size(0)
     if out is None:
-        return x.new_empty((t, width)), width
+        return torch.empty(t, width, dtype=x.dtype, device=x.device), width
     if out.shape != (t, width) or out.dtype != x.dtype or out.device != x.device:
         raise NativeError(f"{what}: invalid output")
     if t and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
@@ -160,7 +160,7 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = 
     need = native.mi355x_linear_int8_workspace_bytes(t, n, k, cus)
     if need < 0:
         raise NativeError("linear_int8: invalid shape")
-    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     with on_device(device):
         check(native.mi355x_linear_int8(
             x.data_ptr(), ldx, values.data_ptr(), _padded(k, _STEP), scales.data_ptr(),
