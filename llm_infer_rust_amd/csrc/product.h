@@ -716,6 +716,7 @@ __device__ __forceinline__ void large_loop(const ProductArgs& a, const RowTile& 
 
 // What the epilogue needs of the tile's rows and columns, in LDS once the stages are free.
 struct LargeEdges {
+  int64_t out[256];         // byte offset of the row
   int32_t out_row[256];
   float row_scale[256];     // int8: of the x row; kDown: times the slot's weight
   float column_scale[256];  // int8: of the tile's weight rows (SILU: 128 gate, then 128 up)
@@ -736,6 +737,28 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
   const int wm = wave & 1, wn = wave >> 1;
   const int col = lane & 31, half = lane >> 5;
   uint8_t* turn = lds + wave * 32 * kPitch;
+  // int8: scales of the weight rows of a lane's quads
+  float gs[A_BLK][4][4], us[A_BLK][4][4];
+  if constexpr (IN == kInt8) {
+#pragma unroll
+    for (int i = 0; i < A_BLK; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; q += SILU ? 2 : 1) {
+        const int wrow = 32 * i + 8 * q + 4 * half;
+        const float* at = edges.column_scale + wn * kCols + (SILU ? silu_column(wrow) : wrow);
+        *reinterpret_cast<float4*>(gs[i][q]) = *reinterpret_cast<const float4*>(at);
+        if constexpr (SILU)
+          *reinterpret_cast<float4*>(us[i][q]) = *reinterpret_cast<const float4*>(at + 128);
+      }
+  }
+  // A lane stores 16-byte piece lane % kChunks of rows kRows apart.
+  constexpr int kChunks = kCols * kOutSize / 16;  // pieces of a row
+  constexpr int kPer = 16 / kOutSize;             // elements of a piece
+  constexpr int kRows = kWave / kChunks;
+  const int piece = lane % kChunks, piece_row = lane / kChunks;
+  const int column = n0 + wn * kCols + piece * kPer;
+  const bool whole = a.vec16_out && column + kPer <= a.columns;
+  uint8_t* out = static_cast<uint8_t*>(a.out) + static_cast<int64_t>(column) * kOutSize;
 #pragma unroll
   for (int j = 0; j < B_BLK; ++j) {
     const int begin = wm * (BM / 2) + 32 * j;  // row of the tile
@@ -747,33 +770,22 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
       float f[16];  // of 32 columns (SILU: the 8 of 16)
 #pragma unroll
       for (int q = 0; q < 4; q += SILU ? 2 : 1) {
-        const int wrow = 32 * i + 8 * q + 4 * half;
-        const int at = SILU ? silu_column(wrow) : wrow;  // column of the wave
-        float gs[4] = {1.f, 1.f, 1.f, 1.f}, us[4] = {1.f, 1.f, 1.f, 1.f};
-        if constexpr (IN == kInt8) {
-          *reinterpret_cast<float4*>(gs) =
-              *reinterpret_cast<const float4*>(edges.column_scale + wn * kCols + at);
-          if constexpr (SILU)
-            *reinterpret_cast<float4*>(us) =
-                *reinterpret_cast<const float4*>(edges.column_scale + 128 + wn * kCols + at);
-        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float g = static_cast<float>(acc[i][j][4 * q + e]);
           if constexpr (IN == kInt8 && MODE != kDown) g *= row_scale;
-          if constexpr (IN == kInt8) g *= gs[e];
+          if constexpr (IN == kInt8) g *= gs[i][q][e];
           if constexpr (SILU) {
             float u = static_cast<float>(acc[i][j][(4 * q + 4 + e) & 15]);
-            if constexpr (IN == kInt8) u = u * row_scale * us[e];
+            if constexpr (IN == kInt8) u = u * row_scale * us[i][q][e];
             g = silu_mul(g, u);
           }
           f[4 * q + e] = g;
         }
       }
       uint32_t codes[8];
-      if constexpr (MODE == kDown) {
+      if constexpr (MODE == kDown)
         scales |= static_cast<uint32_t>(SlotCode::pack(f, row_scale, codes)) << (16 * i);
-      }
 #pragma unroll
       for (int q = 0; q < 4; q += SILU ? 2 : 1) {
         const int wrow = 32 * i + 8 * q + 4 * half;
@@ -790,26 +802,21 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
     }
     if constexpr (MODE == kDown) {
       static_assert(A_BLK == 2, "two scales a word");
-      const int column = n0 + wn * kCols;  // rows of scales are padded to whole words
-      if (half == 0 && t.begin + begin + col < t.end && column < a.columns)
+      const int block = n0 + wn * kCols;  // rows of scales are padded to whole words
+      if (half == 0 && t.begin + begin + col < t.end && block < a.columns)
         *reinterpret_cast<uint32_t*>(a.code_scales + edges.out_row[begin + col] * a.ld_code_scales +
-                                     column / 32) = scales;
+                                     block / 32) = scales;
     }
     // A wave's LDS operations keep their order, so its reads follow its writes of all lanes; the
     // clobbers keep the compiler from exchanging them.
     asm volatile("" ::: "memory");
-    constexpr int kChunks = kCols * kOutSize / 16;  // 16-byte pieces of a row
-    constexpr int kPer = 16 / kOutSize;             // elements of a piece
 #pragma unroll
-    for (int s = 0; s < 32 * kChunks / kWave; ++s) {
-      const int p = s * kWave + lane;
-      const int lr = p / kChunks, c = p % kChunks;
-      const uint4 v = *reinterpret_cast<const uint4*>(turn + lr * kPitch + c * 16);
-      const int64_t out_row = edges.out_row[begin + lr];
-      const int column = n0 + wn * kCols + c * kPer;
+    for (int s = 0; s < 32 / kRows; ++s) {
+      const int lr = s * kRows + piece_row;
+      const uint4 v = *reinterpret_cast<const uint4*>(turn + lr * kPitch + piece * 16);
       if (t.begin + begin + lr >= t.end || column >= a.columns) continue;
-      uint8_t* o = static_cast<uint8_t*>(a.out) + (out_row * a.ldo + column) * kOutSize;
-      if (a.vec16_out && column + kPer <= a.columns) {
+      uint8_t* o = out + edges.out[begin + lr];
+      if (whole) {
         st128(o, v);
       } else {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -848,7 +855,9 @@ __device__ __forceinline__ void large_tile(const ProductArgs& a, const RowTile& 
   auto& edges = *reinterpret_cast<LargeEdges*>(lds + kLargeEdges);
   if constexpr (IN == kInt8 && MODE == kGateUp) row_scale = a.x_scales[slot / a.top_k];
   if (threadIdx.x < 256) {
-    edges.out_row[r] = MODE == kDown ? slot : row;
+    const int out_row = MODE == kDown ? slot : row;
+    edges.out_row[r] = out_row;
+    edges.out[r] = out_row * a.ldo * (OT == kFloatOut ? 4 : 2);
     edges.row_scale[r] = row_scale * weight;
     edges.column_scale[r] = column_scale;
   }
