@@ -341,11 +341,25 @@ __global__ __launch_bounds__(THREADS) void sum_slots(const uint16_t* __restrict_
 // ---------------------------------------------------------------------------- the products
 int64_t pad(int64_t n, int64_t a) { return (n + a - 1) / a * a; }
 
-// A few slots run one by one on vector math, without grouping (see product_vec.h): they seldom share
-// an expert, and a token's slots are summed in the down product.
-bool one_by_one(int64_t slots, int64_t top_k, int64_t hidden, int64_t inter, bool int8) {
-  return slots <= 16 && top_k <= kVecDownSlots &&
-         (!int8 || (pad(hidden, 16) <= kVecLds && top_k * pad(inter, 16) <= kVecLds));
+// A few slots run one by one on vector math, without grouping (see product_vec.h), a token's slots summed
+// in the down product. That reads an expert's weights once a slot in two launches; the grouped products
+// read them once in four and more. Estimated in us: a slot costs 0.2 and its weights (b MB) at 7.1 TB/s, in
+// 8 bits, where each workgroup quantises the rows it takes, at 4; grouping costs 12 and the weights of the
+// experts that so many tokens reach on average, at 7.1. Measured one by one / grouped: 128 experts of 9.4
+// MB, 8 a token, bf16, 1 to 8 tokens 18 / 31, 28 / 39, 39 / 49, 49 / 60, 70 / 84 (6), 91 / 91 us; 8 of 17
+// MB, 2 a token 30 / 29 at 4 tokens, 52 / 32 at 8; in 8 bits 34 / 26 and 59 / 28. Over 96 such batches the
+// rule costs 1.3% more than the better of the two every time (a limit of 16 slots 13%).
+bool one_by_one(int64_t tokens, int64_t top_k, int64_t experts, int64_t hidden, int64_t inter,
+                bool int8) {
+  const int64_t slots = tokens * top_k;
+  if (slots > 64 || top_k > kVecDownSlots ||
+      (int8 && (pad(hidden, 16) > kVecLds || top_k * pad(inter, 16) > kVecLds)))
+    return false;
+  const float b = static_cast<float>(3 * hidden * inter) * (int8 ? 1e-6f : 2e-6f);
+  const float e = static_cast<float>(experts);
+  const float share = std::min(1.f, static_cast<float>(top_k) / e);
+  const float reached = e * (1.f - std::pow(1.f - share, static_cast<float>(tokens)));
+  return static_cast<float>(slots) * (0.2f + (int8 ? 0.25f : 0.14f) * b) < 12.f + reached * 0.14f * b;
 }
 
 // How a grouped product is computed: the tiles and, for the down product, the parts of K.
@@ -534,7 +548,7 @@ template <int IN, int OT>
 const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* ws, hipStream_t s) {
   constexpr bool kQuant = IN == kInt8;
   const int64_t slots = c.tokens * c.top_k;
-  if (one_by_one(slots, c.top_k, c.hidden, c.inter, kQuant))
+  if (one_by_one(c.tokens, c.top_k, c.experts, c.hidden, c.inter, kQuant))
     return expert_slots<IN, OT>(c, w, ws, s);
   const int64_t gate_up_k = kQuant ? int8_k(c.hidden, c.ld_gate_up) : c.hidden * 2;
   const int64_t down_k = kQuant ? int8_k(c.inter, c.ld_down) : c.inter * 2;
