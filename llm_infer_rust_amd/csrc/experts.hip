@@ -269,7 +269,7 @@ __global__ __launch_bounds__(THREADS) void sum_slots(const uint16_t* __restrict_
                                                  const int32_t* __restrict__ ids,
                                                  uint16_t* __restrict__ out, int64_t ldo,
                                                  int64_t tokens, int top_k, int splits, int experts,
-                                                 int width, bool vec) {
+                                                 int width) {
   const int chunks = (width + 8 * H - 1) / (8 * H);
   // at most 2^17 tokens of 2^14 chunks a pass
   const uint32_t i = blockIdx.x * uint32_t(THREADS) + threadIdx.x;
@@ -328,8 +328,8 @@ __global__ __launch_bounds__(THREADS) void sum_slots(const uint16_t* __restrict_
   for (int h = 0; h < H; ++h) {
     const int at = c + 8 * h;
     uint16_t* o = out + static_cast<int64_t>(t) * ldo + at;
-    if (vec && at + 8 <= width) {
-      st128(o, pack8<DT>(sum[h]));
+    if (at + 8 <= width) {
+      st128_any(o, pack8<DT>(sum[h]));
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -513,7 +513,7 @@ const char* expert_slots(const ExpertCall& c, const ExpertWorkspace& w, uint8_t*
   a.tiles_n = static_cast<int32_t>((c.inter + kWaves - 1) / kWaves);
   product_vec<IN, OT, kQuant ? kFloatOut : OT, kGateUp, true, 1, 2, kWaves>
       <<<dim3(static_cast<uint32_t>(pad(slots * a.tiles_n, 8))), 64 * kWaves, 0, s>>>(
-          a, static_cast<int>(c.hidden), aligned(c.x, 16) && c.x_stride % 16 == 0);
+          a, static_cast<int>(c.hidden));
   if (const char* e = launch_status("product (gate_up)")) return e;
   DownArgs d{};
   d.act = ws + w.act;
@@ -598,7 +598,6 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   a.top_k = static_cast<int32_t>(c.top_k);
   a.experts = static_cast<int32_t>(c.experts);
   a.splits = 1;
-  a.vec_out = a.vec16_out = 1;
   // gate_up with SiLU x mul into act, one row a slot
   if (kQuant) {
     a.x = ws + w.xq;
@@ -650,13 +649,12 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   launch_product<IN, OT, kDown, false>(a, w.down.tile, slots, c.experts, s);
   if (const char* e = launch_status("product (down)")) return e;
   const auto* y = reinterpret_cast<const uint16_t*>(ws + w.y);
-  const bool vec = c.ldo % 8 == 0 && aligned(c.out, 16);
   auto sum = [&](auto kernel, int columns, int threads) {
     const int64_t n = c.tokens * ((c.hidden + columns - 1) / columns);
     kernel<<<dim3(static_cast<uint32_t>((n + threads - 1) / threads)), threads, 0, s>>>(
         y, a.ldo, a.code_scales, a.ld_code_scales, c.ids, c.out, c.ldo, c.tokens,
         static_cast<int>(c.top_k), w.down.splits, static_cast<int>(c.experts),
-        static_cast<int>(c.hidden), vec);
+        static_cast<int>(c.hidden));
   };
   const bool many = c.tokens * c.hidden >= (int64_t(1) << 22);
   if (w.down.splits > 1)

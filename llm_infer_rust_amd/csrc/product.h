@@ -62,8 +62,6 @@ struct ProductArgs {
   int32_t tiles_m, tiles_n;   // kDense, kSplit: row tiles; column tiles of every row tile
   int32_t splits;             // parts of K. kSplit: out is int32 [splits][rows][ldo]. kDown
                               // (product_tile): out has a plane of `rows` slots a part, summed later
-  int32_t vec_out;            // out rows take aligned stores of four elements
-  int32_t vec16_out;          // out rows take aligned 16-byte stores
 };
 
 // ---------------------------------------------------------------------------- MFMA by type
@@ -114,20 +112,20 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
 
 // Four consecutive output elements of a row, of which the first `n` exist.
 template <int OT>
-__device__ __forceinline__ void store4(void* out, int64_t at, const float (&v)[4], int n, bool vec) {
+__device__ __forceinline__ void store4(void* out, int64_t at, const float (&v)[4], int n) {
   if constexpr (OT == kFloatOut) {
     float* p = static_cast<float*>(out) + at;
-    if (vec && n >= 4) {
-      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    if (n >= 4) {
+      st128_any(p, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                              __float_as_uint(v[3])));
     } else {
       for (int e = 0; e < 4; ++e)
         if (e < n) p[e] = v[e];
     }
   } else {
     uint16_t* p = static_cast<uint16_t*>(out) + at;
-    if (vec && n >= 4) {
-      *reinterpret_cast<uint2*>(p) =
-          make_uint2(Elem<OT>::pack2(v[0], v[1]), Elem<OT>::pack2(v[2], v[3]));
+    if (n >= 4) {
+      st64_any(p, make_uint2(Elem<OT>::pack2(v[0], v[1]), Elem<OT>::pack2(v[2], v[3])));
     } else {
       for (int e = 0; e < 4; ++e)
         if (e < n) p[e] = Elem<OT>::from_float(v[e]);
@@ -236,7 +234,7 @@ __device__ __forceinline__ void finish4(const ProductArgs& a, const RowOut& r, i
   if (n <= 0) return;
   float v[4];
   finish_values<IN, MODE, SILU>(a, r, column, w_scales, acc, up, v);
-  store4<OT>(a.out, r.at * a.ldo + column, v, n, a.vec_out);
+  store4<OT>(a.out, r.at * a.ldo + column, v, n);
 }
 
 // A row tile: its expert and rows. Returns false where the workgroup has none.
@@ -757,7 +755,7 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
   constexpr int kRows = kWave / kChunks;
   const int piece = lane % kChunks, piece_row = lane / kChunks;
   const int column = n0 + wn * kCols + piece * kPer;
-  const bool whole = a.vec16_out && column + kPer <= a.columns;
+  const bool whole = column + kPer <= a.columns;
   uint8_t* out = static_cast<uint8_t*>(a.out) + static_cast<int64_t>(column) * kOutSize;
 #pragma unroll
   for (int j = 0; j < B_BLK; ++j) {
@@ -817,7 +815,7 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
       if (t.begin + begin + lr >= t.end || column >= a.columns) continue;
       uint8_t* o = out + edges.out[begin + lr];
       if (whole) {
-        st128(o, v);
+        st128_any(o, v);
       } else {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll

@@ -39,13 +39,13 @@ __device__ __forceinline__ T group_sum(T v) {
 // The 8-bit form of a row of `width` elements of type XT in LDS (whole 16-byte words, zeros behind the
 // end) and its scale, by a workgroup of THREADS. `tops` is an LDS word a wave.
 template <int XT, int THREADS>
-__device__ __forceinline__ float quantize_to_lds(const uint8_t* row, int width, bool vec,
+__device__ __forceinline__ float quantize_to_lds(const uint8_t* row, int width,
                                                  uint8_t* to, uint32_t* tops) {
   const int chunks = (width + 15) >> 4;
   uint32_t top = 0;
   float f[16];
   for (int c = threadIdx.x; c < chunks; c += THREADS) {
-    load16<XT>(row, c * 16, width - c * 16, vec, f);
+    load16<XT>(row, c * 16, width - c * 16, f);
     top = max(top, magnitude16(f));
   }
   top = wave_max(top);
@@ -56,7 +56,7 @@ __device__ __forceinline__ float quantize_to_lds(const uint8_t* row, int width, 
   for (int w = 0; w < THREADS / kWave; ++w) top = max(top, tops[w]);
   const RowQuant q(top);
   for (int c = threadIdx.x; c < chunks; c += THREADS) {
-    if (chunks > THREADS) load16<XT>(row, c * 16, width - c * 16, vec, f);
+    if (chunks > THREADS) load16<XT>(row, c * 16, width - c * 16, f);
     st128(to + c * 16, q.values(f));
   }
   return q.scale;
@@ -64,19 +64,19 @@ __device__ __forceinline__ float quantize_to_lds(const uint8_t* row, int width, 
 
 // The same by one wave. No barrier: the row is for the workgroup after its next one.
 template <int XT>
-__device__ __forceinline__ float quantize_by_wave(const uint8_t* row, int width, bool vec,
+__device__ __forceinline__ float quantize_by_wave(const uint8_t* row, int width,
                                                   uint8_t* to) {
   const int lane = threadIdx.x % kWave;
   const int chunks = (width + 15) >> 4;
   uint32_t top = 0;
   float f[16];
   for (int c = lane; c < chunks; c += kWave) {
-    load16<XT>(row, c * 16, width - c * 16, vec, f);
+    load16<XT>(row, c * 16, width - c * 16, f);
     top = max(top, magnitude16(f));
   }
   const RowQuant q(wave_max(top));
   for (int c = lane; c < chunks; c += kWave) {
-    if (chunks > kWave) load16<XT>(row, c * 16, width - c * 16, vec, f);
+    if (chunks > kWave) load16<XT>(row, c * 16, width - c * 16, f);
     st128(to + c * 16, q.values(f));
   }
   return q.scale;
@@ -88,7 +88,7 @@ constexpr int kVecLds = 32 * 1024;  // bytes of quantised rows that a workgroup 
 // R / 2 gate rows and the matching up rows). For int8 the rows of x, of type XT, are quantised in
 // the workgroup while its first weights are on their way.
 template <int IN, int XT, int OT, int MODE, bool SILU, int MR, int R, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void product_vec(ProductArgs a, int width, bool vec_x) {
+__global__ __launch_bounds__(64 * WAVES) void product_vec(ProductArgs a, int width) {
   constexpr int kOut = SILU ? R / 2 : R;  // columns of a wave
   constexpr int U = 4;                    // pieces of a row on their way at once
   constexpr bool kQuant = IN == kInt8;
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(64 * WAVES) void product_vec(ProductArgs a, int wid
   if constexpr (kQuant) {
 #pragma unroll
     for (int m = 0; m < MR; ++m)
-      scale[m] = quantize_to_lds<XT, 64 * WAVES>(x_row[m], width, vec_x, rows + m * a.k_bytes, tops);
+      scale[m] = quantize_to_lds<XT, 64 * WAVES>(x_row[m], width, rows + m * a.k_bytes, tops);
     __syncthreads();
   }
   for (int k = kBatch; k < a.k_bytes; k += kBatch) {
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(64 * WAVES) void product_vec_down(DownArgs a) {
       const int e = a.ids[first + s];
       if (e < 0 || e >= a.experts) continue;
       const float scale = quantize_by_wave<kFloatOut>(a.act + (first + s) * a.act_stride, a.width,
-                                                      true, rows + s * a.k_bytes);
+                                                      rows + s * a.k_bytes);
       if (lane == 0) scales[s] = scale;
     }
     __syncthreads();

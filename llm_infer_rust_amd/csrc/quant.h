@@ -7,21 +7,21 @@ namespace mi355x {
 
 // 16 elements of a row as floats; `n` of them exist, the others are 0.
 template <int DT>
-__device__ __forceinline__ void load16(const uint8_t* row, int64_t at, int n, bool vec,
-                                       float (&f)[16]) {
+__device__ __forceinline__ void load16(const uint8_t* row, int64_t at, int n, float (&f)[16]) {
   constexpr int kSize = DT == kFloatOut ? 4 : 2;
   const uint8_t* p = row + at * kSize;
-  if (vec && n >= 16) {
+  if (n >= 16) {
     if constexpr (DT == kFloatOut) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float4 v = *reinterpret_cast<const float4*>(p + 16 * i);
-        f[4 * i] = v.x, f[4 * i + 1] = v.y, f[4 * i + 2] = v.z, f[4 * i + 3] = v.w;
+        const uint4 v = ld128_any(p + 16 * i);
+        f[4 * i] = __uint_as_float(v.x), f[4 * i + 1] = __uint_as_float(v.y);
+        f[4 * i + 2] = __uint_as_float(v.z), f[4 * i + 3] = __uint_as_float(v.w);
       }
     } else {
       float lo[8], hi[8];
-      unpack8<DT>(ld128(p), lo);
-      unpack8<DT>(ld128(p + 16), hi);
+      unpack8<DT>(ld128_any(p), lo);
+      unpack8<DT>(ld128_any(p + 16), hi);
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = lo[i], f[8 + i] = hi[i];
     }
@@ -97,15 +97,13 @@ struct RowsToQuantize {
   float* scales;
   int64_t stride, ldv, rows;  // stride in bytes
   int32_t width, chunks;      // chunks of 16 columns to write, zeros past the width
-  bool vec;                   // rows take 16-byte loads
 };
 
 inline RowsToQuantize rows_to_quantize(const void* x, int64_t stride, void* values, int64_t ldv,
                                        float* scales, int64_t rows, int64_t width,
                                        int64_t padded) {
   return {static_cast<const uint8_t*>(x), static_cast<uint8_t*>(values), scales, stride, ldv, rows,
-          static_cast<int32_t>(width), static_cast<int32_t>(padded / 16),
-          aligned(x, 16) && stride % 16 == 0};
+          static_cast<int32_t>(width), static_cast<int32_t>(padded / 16)};
 }
 
 // K of an int8 product in bytes: the weight rows' elements and, where their stride `ld` holds them, the
@@ -133,13 +131,13 @@ __device__ __forceinline__ void quantize_row(const RowsToQuantize& q, int64_t ro
   for (int h = 0; h < HELD; ++h) {
     const int c = lane + h * LANES;
     if (c < chunks) {
-      load16<DT>(src, c * 16, q.width - c * 16, q.vec, held[h]);
+      load16<DT>(src, c * 16, q.width - c * 16, held[h]);
       top = max(top, magnitude16(held[h]));
     }
   }
   for (int c = lane + HELD * LANES; c < chunks; c += LANES) {
     float f[16];
-    load16<DT>(src, c * 16, q.width - c * 16, q.vec, f);
+    load16<DT>(src, c * 16, q.width - c * 16, f);
     top = max(top, magnitude16(f));
   }
   top = wave_max(top);
@@ -158,7 +156,7 @@ __device__ __forceinline__ void quantize_row(const RowsToQuantize& q, int64_t ro
   }
   for (int c = lane + HELD * LANES; c < chunks; c += LANES) {
     float f[16];
-    load16<DT>(src, c * 16, q.width - c * 16, q.vec, f);
+    load16<DT>(src, c * 16, q.width - c * 16, f);
     st128(dst + c * 16, form.values(f));
   }
 }

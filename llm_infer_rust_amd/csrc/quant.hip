@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256) void finish_splits(ProductArgs a, const int* _
 }
 
 template <int OT, bool SILU>
-void launch_int8_vec(const ProductArgs& base, int64_t M, int64_t columns, int width, bool vec,
+void launch_int8_vec(const ProductArgs& base, int64_t M, int64_t columns, int width,
                      hipStream_t s) {
   ProductArgs a = base;
   constexpr int kWaves = 16, kRows = 2;
@@ -126,9 +126,9 @@ void launch_int8_vec(const ProductArgs& base, int64_t M, int64_t columns, int wi
   a.tiles_n = static_cast<int32_t>((columns + bn - 1) / bn);
   const dim3 g(static_cast<uint32_t>((a.tiles_n + 7) / 8 * 8));
   if (M == 1)
-    product_vec<kInt8, OT, OT, kDense, SILU, 1, kRows, kWaves><<<g, 64 * kWaves, 0, s>>>(a, width, vec);
+    product_vec<kInt8, OT, OT, kDense, SILU, 1, kRows, kWaves><<<g, 64 * kWaves, 0, s>>>(a, width);
   else
-    product_vec<kInt8, OT, OT, kDense, SILU, 2, kRows, kWaves><<<g, 64 * kWaves, 0, s>>>(a, width, vec);
+    product_vec<kInt8, OT, OT, kDense, SILU, 2, kRows, kWaves><<<g, 64 * kWaves, 0, s>>>(a, width);
 }
 
 template <int OT, int MODE, bool SILU>
@@ -257,19 +257,16 @@ extern "C" const char* mi355x_linear_int8(const void* x, int64_t ldx, const void
   a.rows = static_cast<int32_t>(M);
   a.columns = static_cast<int32_t>(columns);
   a.k_bytes = static_cast<int32_t>(padded16(K));
-  a.vec_out = ldo % 4 == 0 && aligned(out, 8);
-  a.vec16_out = ldo % 8 == 0 && aligned(out, 16);
   if (plan.kind == Int8Plan::kVec) {
     a.x = static_cast<const uint8_t*>(x);
     a.x_stride = ldx * 2;
-    const bool vec = aligned(x, 16) && ldx % 8 == 0;
     const int width = static_cast<int>(K);
     if (dtype == 0)
-      silu_mul ? launch_int8_vec<0, true>(a, M, columns, width, vec, s)
-               : launch_int8_vec<0, false>(a, M, columns, width, vec, s);
+      silu_mul ? launch_int8_vec<0, true>(a, M, columns, width, s)
+               : launch_int8_vec<0, false>(a, M, columns, width, s);
     else
-      silu_mul ? launch_int8_vec<1, true>(a, M, columns, width, vec, s)
-               : launch_int8_vec<1, false>(a, M, columns, width, vec, s);
+      silu_mul ? launch_int8_vec<1, true>(a, M, columns, width, s)
+               : launch_int8_vec<1, false>(a, M, columns, width, s);
     return launch_status("product (int8)");
   }
   auto* base = static_cast<uint8_t*>(workspace);
