@@ -370,12 +370,31 @@ struct GroupedPlan {
   int splits;
 };
 
+// Estimated time in us of `count` tiles over `steps` 128-byte steps of K, as tile_estimate does for dense
+// rows but with what gathered rows and ragged groups cost: a step of 128 rows two a CU 0.66 instead of
+// 0.58, and a second round of 256-row tiles from 0.95 of a round on, as the groups are never even.
+float grouped_estimate(Tile tile, float count, float steps, float weight_bytes, bool half, int cus) {
+  const float r = count / static_cast<float>(cus), busy = std::min(r, 1.f);
+  float step, rounds = 1.f;
+  if (tile == Tile::k64) {
+    step = 0.27f;
+    if (r > 1.f) rounds = std::max(1.07f * r - 0.07f, std::min(2.f, 1.f + 2.5f * (r - 1.f)));
+  } else if (tile == Tile::k128Two) {
+    step = 0.66f;
+    rounds = std::max(2.f, r + 0.3f);
+  } else {
+    step = half ? 0.65f + 0.7f * busy : 1.2f + 0.6f * busy;
+    if (r > 0.95f) rounds = r <= 3.f ? std::ceil(r + 0.05f) : r + 0.3f;
+  }
+  return 3.3f + std::max(steps * step * rounds, weight_bytes / 5.8e6f);
+}
+
 // The least estimate. How many rows an expert gets is not known on the host; it is taken to be the
-// same for all, with 0.6 of a tile more each for the ragged ends. Tiles of 64, of 128 two a CU and of 256
-// rows: over 41 products of 8 to 128 experts and 8 to 512 rows each, int8 and bf16, the choice costs
-// 2.9% more than the best of nine shapes every time (6.7% with 128 rows one a CU and 256 x 128). A product whose slot outputs are
-// summed afterwards may be cut along K as well, where its tiles leave CUs without one: the parts are
-// summed with the slots (down of 8 experts 1024 x 2816 at 77 tokens 17.0 us whole, 11.6 in two parts).
+// same for all, with 0.4 of a tile more each for the ragged ends. Tiles of 64, of 128 two a CU and of 256
+// rows: over 114 products of 4 to 132 experts and 8 to 1,637 rows each, int8 and bf16, the choice costs
+// 2.4% more than the best of the three every time. A product whose slot outputs are summed afterwards
+// may be cut along K as well, where its tiles leave CUs without one: the parts are summed with the slots
+// (down of 8 experts 1024 x 2816 at 77 tokens 17.0 us whole, 11.6 in two parts).
 GroupedPlan choose_grouped(int64_t slots, int64_t experts, int64_t weight_rows, int64_t k_bytes,
                            bool summed, int cus) {
   const float active = static_cast<float>(std::min(slots, experts));
@@ -386,15 +405,15 @@ GroupedPlan choose_grouped(int64_t slots, int64_t experts, int64_t weight_rows, 
   float best_us = 1e30f;
   for (const Tile tile : {Tile::k64, Tile::k128Two, Tile::k256}) {
     const TileShape& t = kTileShapes[static_cast<int>(tile)];
-    const float tm = active * std::max(1.f, per / static_cast<float>(t.bm) + 0.6f);
-    const float tn = std::ceil(static_cast<float>(weight_rows) / static_cast<float>(t.bn));
+    const float count = active * std::max(1.f, per / static_cast<float>(t.bm) + 0.4f) *
+                        std::ceil(static_cast<float>(weight_rows) / static_cast<float>(t.bn));
     for (int s = 1; s <= (summed && tile == Tile::k64 ? 4 : 1); s *= 2) {
       const int64_t part = (steps + s - 1) / s;
-      if (s > 1 && (part < 8 || part * (s - 1) >= steps || tm * tn * static_cast<float>(s / 2) >=
-                                                                static_cast<float>(cus)))
+      if (s > 1 && (part < 8 || part * (s - 1) >= steps ||
+                    count * static_cast<float>(s / 2) >= static_cast<float>(cus)))
         break;
-      float us = tile_estimate(tile, tm * s, tn, part * kProdRow, weights,
-                               per <= 128.f, cus);
+      float us = grouped_estimate(tile, count * static_cast<float>(s), static_cast<float>(part),
+                                  weights, per <= 128.f, cus);
       // two bytes a value more, out and back
       us += static_cast<float>(s - 1) * (0.3f + static_cast<float>(slots * weight_rows) * 4 / 4.5e6f);
       if (us < best_us) {

@@ -177,7 +177,9 @@ def test_expert_mlp(gpu, dtype, t, e, k, h, i):
 # token, one expert, and more experts than slots.
 LARGE = [(1200, 2, 2, 72, 1032), (1200, 2, 2, 2056, 72), (600, 16, 2, 72, 1032), (600, 16, 2, 2056, 72),
          (2500, 6, 2, 1032, 520), (3000, 3, 2, 512, 1024), (1, 64, 64, 64, 64), (5, 64, 64, 72, 40),
-         (33, 1, 1, 128, 64), (700, 1, 1, 128, 64), (50, 1024, 3, 64, 32)]
+         (33, 1, 1, 128, 64), (700, 1, 1, 128, 64), (50, 1024, 3, 64, 32),
+         (2100, 5, 2, 2056, 72), (2100, 5, 2, 72, 1032), (4100, 5, 2, 1032, 520),
+         (3000, 3, 2, 2056, 128), (1000, 8, 1, 72, 1544)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -285,7 +287,8 @@ def test_expert_mlp_int8(gpu, dtype, t, e, k, h, i):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("t,e,k,h,i", LARGE + [(1200, 2, 2, 2055, 67), (600, 16, 2, 71, 1033),
-                                                (600, 16, 2, 2055, 131)])
+                                                (600, 16, 2, 2055, 131), (2100, 5, 2, 2055, 67),
+                                                (2100, 5, 2, 71, 1033)])
 def test_expert_mlp_int8_of_many_rows(gpu, dtype, t, e, k, h, i):
     x, ids, w, gu, dn = problem(t, e, k, h, i, dtype, t * 5 + e)
     gu8, dn8 = (int8.Int8Weight.quantize(m.to(gpu)) for m in (gu, dn))
@@ -345,7 +348,7 @@ def test_rows_gigabytes_apart(gpu, k):
     assert torch.equal(weights, want) and torch.equal(chosen, want_ids)
 
 
-@pytest.mark.parametrize("t", [3, 60, 1200])
+@pytest.mark.parametrize("t", [3, 60, 1200, 3100])
 def test_infinite_weights(gpu, t):
     """An infinity in `down` reaches its column and no other; the 32 columns that share its scale are
     then held in bf16, half a step of 2^-9 for each slot of the expert."""
