@@ -393,7 +393,8 @@ int64_t mi355x_expert_mlp_workspace_bytes(int64_t tokens, int64_t top_k, int64_t
  * twice in a row.
  *
  * Scales NULL: weights of x's type. hidden, inter and ldx are multiples of 8 and rows are 16-byte
- * aligned. Sums in fp32; silu(g) * u is rounded to x's type.
+ * aligned. Sums in fp32; silu(g) * u is rounded to x's type (kept in fp32 where a few slots run one
+ * by one).
  * Scales given (fp32 [experts, 2 inter] and [experts, hidden]): int8 weights. x is quantised once
  * a token, silu(g) * u (kept in fp32) once a slot, both as mi355x_quantize_rows does; any sizes and
  * x strides, weight rows as for mi355x_linear_int8.

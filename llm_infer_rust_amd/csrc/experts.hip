@@ -351,10 +351,11 @@ int64_t pad(int64_t n, int64_t a) { return (n + a - 1) / a * a; }
 // MB, 8 a token, bf16, 1 to 8 tokens 18 / 31, 28 / 39, 39 / 49, 49 / 60, 70 / 84 (6), 91 / 91 us; 8 of 17
 // MB, 2 a token 30 / 29 at 4 tokens, 52 / 32 at 8; in 8 bits 34 / 26 and 59 / 28. Over 96 such batches the
 // rule costs 1.3% more than the better of the two every time (a limit of 16 slots 13%).
+constexpr int64_t kMaxOneByOne = 64;
 bool one_by_one(int64_t tokens, int64_t top_k, int64_t experts, int64_t hidden, int64_t inter,
                 bool int8) {
   const int64_t slots = tokens * top_k;
-  if (slots > 64 || top_k > kVecDownSlots ||
+  if (slots > kMaxOneByOne || top_k > kVecDownSlots ||
       (int8 && (pad(hidden, 16) > kVecLds || top_k * pad(inter, 16) > kVecLds)))
     return false;
   const float b = static_cast<float>(3 * hidden * inter) * (int8 ? 1e-6f : 2e-6f);
@@ -457,7 +458,9 @@ ExpertWorkspace expert_workspace(int64_t tokens, int64_t top_k, int64_t experts,
   w.down_tiles = take(tiles * 16);
   w.tile_counts = take(8);
   w.counts = take(pad(slots, kGroupChunk) / kGroupChunk * experts * 4);
-  w.act = take(slots * (int8 ? pad(inter, 4) * 4 : inter * 2));
+  // fp32 for int8 and where slots run one by one
+  w.act = take(std::max(slots * (int8 ? pad(inter, 4) * 4 : inter * 2),
+                        std::min(slots, kMaxOneByOne) * inter * 4));
   if (int8) {
     w.xq = take(t * pad(hidden, 128));
     w.xs = take(t * 4);
@@ -532,13 +535,13 @@ const char* expert_slots(const ExpertCall& c, const ExpertWorkspace& w, uint8_t*
   a.ldo = kQuant ? pad(c.inter, 4) : c.inter;
   a.columns = static_cast<int32_t>(c.inter);
   a.tiles_n = static_cast<int32_t>((c.inter + kWaves - 1) / kWaves);
-  product_vec<IN, OT, kQuant ? kFloatOut : OT, kGateUp, true, 1, 2, kWaves>
+  product_vec<IN, OT, kFloatOut, kGateUp, true, 1, 2, kWaves>
       <<<dim3(static_cast<uint32_t>(pad(slots * a.tiles_n, 8))), 64 * kWaves, 0, s>>>(
           a, static_cast<int>(c.hidden));
   if (const char* e = launch_status("product (gate_up)")) return e;
   DownArgs d{};
   d.act = ws + w.act;
-  d.act_stride = kQuant ? a.ldo * 4 : a.ldo * 2;
+  d.act_stride = a.ldo * 4;
   d.w = c.down;
   d.w_stride = c.ld_down;
   d.w_expert = c.hidden * c.ld_down;

@@ -198,7 +198,7 @@ __global__ __launch_bounds__(64 * WAVES) void product_vec(ProductArgs a, int wid
 // three pieces), 64 / G slots at a time. A wave takes a column, a workgroup WAVES of them. For int8 the
 // token's rows of act (fp32) are quantised in the workgroup.
 struct DownArgs {
-  const uint8_t* act;   // a row a slot: the operands' type, or fp32 for int8
+  const uint8_t* act;   // fp32, a row a slot
   const uint8_t* w;
   uint16_t* out;
   const float* w_scales;
@@ -215,6 +215,7 @@ template <int IN, int OT, int G, int N, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void product_vec_down(DownArgs a) {
   constexpr bool kQuant = IN == kInt8;
   constexpr int kAtOnce = kWave / G, U = 3;
+  constexpr int kXWords = kQuant ? 1 : 2;  // 16-byte words of act to one of the weight
   __shared__ __attribute__((aligned(16))) uint8_t rows[kQuant ? kVecLds : 16];
   __shared__ float scales[kVecDownSlots];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(64 * WAVES) void product_vec_down(DownArgs a) {
     }
     typename Mma<IN>::Scalar acc[N] = {};
     for (int k = l * 16; k < a.k_bytes; k += U * G * 16) {
-      uint4 w[N][U], x[N][U];
+      uint4 w[N][U], x[N][U][kXWords];
 #pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -258,17 +259,26 @@ __global__ __launch_bounds__(64 * WAVES) void product_vec_down(DownArgs a) {
           const bool there = in[i] && at < a.k_bytes;
           w[i][u] = there ? ld128_nt(a.w + e[i] * a.w_expert + c * a.w_stride + at)
                           : make_uint4(0, 0, 0, 0);
-          if constexpr (kQuant)
-            x[i][u] = there ? *reinterpret_cast<const uint4*>(rows + slot[i] * a.k_bytes + at)
-                            : make_uint4(0, 0, 0, 0);
-          else
-            x[i][u] = there ? ld128(a.act + (first + slot[i]) * a.act_stride + at)
-                            : make_uint4(0, 0, 0, 0);
+          const uint8_t* from = kQuant ? rows + slot[i] * a.k_bytes + at
+                                       : a.act + (first + slot[i]) * a.act_stride + 2 * at;
+#pragma unroll
+          for (int h = 0; h < kXWords; ++h)
+            x[i][u][h] = there ? ld128(from + 16 * h) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int u = 0; u < U; ++u) dot_piece<IN>(w[i][u], x[i][u], acc[i]);
+        for (int u = 0; u < U; ++u) {
+          if constexpr (kQuant) {
+            dot_piece<IN>(w[i][u], x[i][u][0], acc[i]);
+          } else {
+            float f[8];
+            unpack8<IN>(w[i][u], f);
+            const float* v = reinterpret_cast<const float*>(x[i][u]);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) acc[i] = fmaf(f[q], v[q], acc[i]);
+          }
+        }
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
