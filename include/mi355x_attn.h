@@ -339,11 +339,11 @@ const char* mi355x_linear_noalloc(const void* x, int64_t ldx, const void* w, int
  * ------------------------------------------------------------------------ */
 
 /* scales[r] = max_k |x[r,k]| / 127, values[r,k] = rint(127 x[r,k] / max_k |x[r,k]|)
- * (half to even; a row of zeros has scale 0 and zeros). x [rows, width] of dtype 0 bf16,
- * 1 fp16 or 2 fp32 with row stride ldx and any alignment of its type; values int8
- * [rows, ldv], ldv a multiple of 16, columns width .. up to the next multiple of 16 written
- * as zeros; scales fp32. A row with an inf or a NaN gets the scale NaN and zeros, so that its products
- * are NaN and no other row's are. */
+ * (half to even; a row of zeros has scale 0 and zeros). x [rows, width] of dtype 0 bf16, 1 fp16 or
+ * 2 fp32 with row stride ldx and any alignment of its type; values int8 [rows, ldv], ldv a multiple
+ * of 16, columns width .. up to the next multiple of 16 written as zeros; scales fp32. A row with
+ * an inf or a NaN gets the scale NaN and zeros, so that its products are NaN and no other row's
+ * are. */
 const char* mi355x_quantize_rows(const void* x, int64_t ldx, void* values, int64_t ldv,
                                  void* scales, int64_t rows, int64_t width, int dtype,
                                  void* stream);
@@ -354,11 +354,12 @@ const char* mi355x_quantize_rows(const void* x, int64_t ldx, void* values, int64
 int64_t mi355x_linear_int8_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t cus);
 
 /* out[m, n] = round(sx[m] w_scales[n] sum_k q[m, k] w[n, k]) with (q, sx) = mi355x_quantize_rows
- * of x [M, K] (dtype 0 bf16, 1 fp16; out has the same) and w int8 [N, ldw]; the sum is exact
- * in int32. out must not overlap x. With silu_mul, w is a gate_up weight (gate rows, then up rows, N even) and
- * out[m, j] = round(silu(y[m, j]) * y[m, N/2 + j]), y unrounded. K up to 131,072; w rows of
- * whole 16-byte words, ideally 128-byte ones (what a row holds past K is multiplied with zeros), and
- * less than 4 GiB in all; x and out rows of any stride. Calls that overlap need workspaces of their own. */
+ * of x [M, K] (dtype 0 bf16, 1 fp16; out has the same) and w int8 [N, ldw]; the sum is exact in
+ * int32. out must not overlap x. With silu_mul, w is a gate_up weight (gate rows, then up rows, N
+ * even) and out[m, j] = round(silu(y[m, j]) * y[m, N/2 + j]), y unrounded. K up to 131,072; w rows
+ * of whole 16-byte words, ideally 128-byte ones (what a row holds past K is multiplied with zeros),
+ * and less than 4 GiB in all; x and out rows of any stride. Calls that overlap need workspaces of
+ * their own. */
 const char* mi355x_linear_int8(const void* x, int64_t ldx, const void* w, int64_t ldw,
                                const float* w_scales, void* out, int64_t ldo, int64_t M,
                                int64_t N, int64_t K, bool silu_mul, void* workspace,
@@ -379,8 +380,8 @@ const char* mi355x_route_experts(const void* logits, int64_t ld, void* weights, 
                                  int dtype, void* stream);
 
 /* Workspace bytes of mi355x_expert_mlp on a GPU of `cus` compute units (ldx: x's row stride in
- * elements), -1 for an invalid shape. At most 131,072 slots (or one token) are in flight, more tokens run in several passes.
- * Host-only. */
+ * elements), -1 for an invalid shape. At most 131,072 slots (or one token) are in flight, more
+ * tokens run in several passes. Host-only. */
 int64_t mi355x_expert_mlp_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts,
                                           int64_t hidden, int64_t inter, int64_t ldx, bool int8,
                                           int32_t cus);

@@ -229,8 +229,8 @@ __device__ __forceinline__ uint4 ld128(const void* p) {
 __device__ __forceinline__ void st128(void* p, const uint4& v) {
   *reinterpret_cast<uint4*>(p) = v;
 }
-// The same at the address of any 16-bit element: the compiler keeps one instruction, as the hardware takes
-// unaligned ones.
+// The same at the address of any 16-bit element: one instruction all the same, as the hardware takes
+// unaligned addresses.
 typedef uint32_t Words2Any __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t Words4Any __attribute__((ext_vector_type(4), aligned(2)));
 __device__ __forceinline__ uint4 ld128_any(const void* p) {

@@ -178,10 +178,11 @@ __device__ __forceinline__ int block_exclusive(int v, int4 (&wave_totals)[4]) {
   return before;
 }
 
-// order[row]: the slots in the order of their experts; row_weights[row]: their weights. `counts` may
-// be null with one chunk. The first workgroup writes the list of row tiles for the gate_up product, the
-// second (or the first, if alone) that for the down product. The order of the slots within an
-// expert is that of the LDS atomics; a row's products do not depend on the row it stands in.
+// order[row]: the slots in the order of their experts; row_weights[row]: their weights. `counts`
+// may be null with one chunk. The first workgroup writes the list of row tiles for the gate_up
+// product, the second (or the first, if alone) that for the down product. The order of the slots
+// within an expert is that of the LDS atomics; a row's products do not depend on the row it stands
+// in.
 struct SlotsToPlace {
   const int32_t* ids;
   const float* weights;
@@ -243,9 +244,9 @@ __device__ __forceinline__ void place_chunk(const SlotsToPlace& p) {
 
 __global__ __launch_bounds__(kGroupThreads) void place_slots(SlotsToPlace p) { place_chunk(p); }
 
-// The same with the rows of x quantised by the workgroups behind the chunks': one launch less before the
-// products (8-bit experts of 40 tokens 110 -> 108 us). A wave a row of up to 2,048 columns (6,208 rows of
-// 1,497 in 12.8 us, 19.8 with four waves each).
+// The same with the rows of x quantised by the workgroups behind the chunks': one launch less
+// before the products (8-bit experts of 40 tokens 110 -> 108 us). A wave a row of up to 2,048
+// columns (6,208 rows of 1,497 in 12.8 us, 19.8 with four waves each).
 template <int DT, int LANES, int HELD>
 __global__ __launch_bounds__(kGroupThreads) void place_and_quantize(SlotsToPlace p,
                                                                     RowsToQuantize q) {
@@ -259,11 +260,11 @@ __global__ __launch_bounds__(kGroupThreads) void place_and_quantize(SlotsToPlace
 }
 
 // ---------------------------------------------------------------------------- the sum over slots
-// out[t] = sum of y[t * top_k + s] (SlotCodes) over the slots that take part and the parts of K, in fp32
-// and in this order. A thread takes 8 H columns, a quarter or half of what a scale covers. Bound by
-// memory where there are many tokens (8,192 of 8 slots and 2,048 columns: 277 MB in 60 us with H 2, 69
-// with H 1), else by latency: H 1 and workgroups of a wave spread over the chip (40 tokens 7.1 us with
-// H 2 and 256 threads).
+// out[t] = sum of y[t * top_k + s] (SlotCodes) over the slots that take part and the parts of K, in
+// fp32 and in this order. A thread takes 8 H columns, a quarter or half of what a scale covers.
+// Bound by memory where there are many tokens (8,192 of 8 slots and 2,048 columns: 277 MB in 60 us
+// with H 2, 69 with H 1), else by latency: H 1 and workgroups of a wave spread over the chip (40
+// tokens 7.1 us with H 2 and 256 threads).
 template <int DT, int H, int THREADS, bool PARTS>
 __global__ __launch_bounds__(THREADS) void sum_slots(const uint16_t* __restrict__ y, int64_t ldy,
                                                  const uint16_t* __restrict__ scales,
@@ -343,14 +344,15 @@ __global__ __launch_bounds__(THREADS) void sum_slots(const uint16_t* __restrict_
 // ---------------------------------------------------------------------------- the products
 int64_t pad(int64_t n, int64_t a) { return (n + a - 1) / a * a; }
 
-// A few slots run one by one on vector math, without grouping (see product_vec.h), a token's slots summed
-// in the down product. That reads an expert's weights once a slot in two launches; the grouped products
-// read them once in four and more. Estimated in us: a slot costs 0.2 and its weights (b MB) at 7.1 TB/s, in
-// 8 bits, where each workgroup quantises the rows it takes, at 4; grouping costs 12 and the weights of the
-// experts that so many tokens reach on average, at 7.1. Measured one by one / grouped: 128 experts of 9.4
-// MB, 8 a token, bf16, 1 to 8 tokens 18 / 31, 28 / 39, 39 / 49, 49 / 60, 70 / 84 (6), 91 / 91 us; 8 of 17
-// MB, 2 a token 30 / 29 at 4 tokens, 52 / 32 at 8; in 8 bits 34 / 26 and 59 / 28. Over 96 such batches the
-// rule costs 1.3% more than the better of the two every time (a limit of 16 slots 13%).
+// A few slots run one by one on vector math, without grouping (see product_vec.h), a token's slots
+// summed in the down product. That reads an expert's weights once a slot in two launches; the
+// grouped products read them once in four and more. Estimated in us: a slot costs 0.2 and its
+// weights (b MB) at 7.1 TB/s, in 8 bits, where each workgroup quantises the rows it takes, at 4;
+// grouping costs 12 and the weights of the experts that so many tokens reach on average, at 7.1.
+// Measured one by one / grouped: 128 experts of 9.4 MB, 8 a token, bf16, 1 to 8 tokens 18 / 31, 28
+// / 39, 39 / 49, 49 / 60, 70 / 84 (6), 91 / 91 us; 8 of 17 MB, 2 a token 30 / 29 at 4 tokens, 52 /
+// 32 at 8; in 8 bits 34 / 26 and 59 / 28. Over 96 such batches the rule costs 1.3% more than the
+// better of the two every time (a limit of 16 slots 13%).
 constexpr int64_t kMaxOneByOne = 64;
 bool one_by_one(int64_t tokens, int64_t top_k, int64_t experts, int64_t hidden, int64_t inter,
                 bool int8) {
@@ -371,9 +373,10 @@ struct GroupedPlan {
   int splits;
 };
 
-// Estimated time in us of `count` tiles over `steps` 128-byte steps of K, as tile_estimate does for dense
-// rows but with what gathered rows and ragged groups cost: a step of 128 rows two a CU 0.66 instead of
-// 0.58, and a second round of 256-row tiles from 0.95 of a round on, as the groups are never even.
+// Estimated time in us of `count` tiles over `steps` 128-byte steps of K, as tile_estimate does for
+// dense rows but with what gathered rows and ragged groups cost: a step of 128 rows two a CU 0.66
+// instead of 0.58, and a second round of 256-row tiles from 0.95 of a round on, as the groups are
+// never even.
 float grouped_estimate(Tile tile, float count, float steps, float weight_bytes, bool half, int cus) {
   const float r = count / static_cast<float>(cus), busy = std::min(r, 1.f);
   float step, rounds = 1.f;
@@ -391,11 +394,12 @@ float grouped_estimate(Tile tile, float count, float steps, float weight_bytes, 
 }
 
 // The least estimate. How many rows an expert gets is not known on the host; it is taken to be the
-// same for all, with 0.4 of a tile more each for the ragged ends. Tiles of 64, of 128 two a CU and of 256
-// rows: over 114 products of 4 to 132 experts and 8 to 1,637 rows each, int8 and bf16, the choice costs
-// 2.4% more than the best of the three every time. A product whose slot outputs are summed afterwards
-// may be cut along K as well, where its tiles leave CUs without one: the parts are summed with the slots
-// (down of 8 experts 1024 x 2816 at 77 tokens 17.0 us whole, 11.6 in two parts).
+// same for all, with 0.4 of a tile more each for the ragged ends. Tiles of 64, of 128 two a CU and
+// of 256 rows: over 114 products of 4 to 132 experts and 8 to 1,637 rows each, int8 and bf16, the
+// choice costs 2.4% more than the best of the three every time. A product whose slot outputs are
+// summed afterwards may be cut along K as well, where its tiles leave CUs without one: the parts
+// are summed with the slots (down of 8 experts 1024 x 2816 at 77 tokens 17.0 us whole, 11.6 in two
+// parts).
 GroupedPlan choose_grouped(int64_t slots, int64_t experts, int64_t weight_rows, int64_t k_bytes,
                            bool summed, int cus) {
   const float active = static_cast<float>(std::min(slots, experts));
@@ -429,7 +433,8 @@ GroupedPlan choose_grouped(int64_t slots, int64_t experts, int64_t weight_rows, 
 constexpr int64_t kMaxSlots = 131072;  // slots a pass takes; more tokens run in several passes
 
 struct ExpertWorkspace {
-  int64_t order, row_weights, gate_up_tiles, down_tiles, tile_counts, counts, xq, xs, act, actq, acts, y, y_scales, bytes;
+  int64_t order, row_weights, gate_up_tiles, down_tiles, tile_counts, counts, xq, xs, act, actq, acts,
+      y, y_scales, bytes;
   int64_t tokens;  // a pass
   GroupedPlan gate_up, down;
 };
@@ -443,7 +448,8 @@ ExpertWorkspace expert_workspace(int64_t tokens, int64_t top_k, int64_t experts,
   const int64_t t = std::min(tokens, most);
   const int64_t slots = t * top_k;
   w.tokens = t;
-  w.gate_up = choose_grouped(slots, experts, 2 * inter, int8 ? pad(hidden, 16) : hidden * 2, false, cus);
+  w.gate_up =
+      choose_grouped(slots, experts, 2 * inter, int8 ? pad(hidden, 16) : hidden * 2, false, cus);
   w.down = choose_grouped(slots, experts, hidden, int8 ? pad(inter, 16) : inter * 2, true, cus);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {

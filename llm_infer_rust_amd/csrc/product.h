@@ -133,12 +133,12 @@ __device__ __forceinline__ void store4(void* out, int64_t at, const float (&v)[4
   }
 }
 
-// Slot outputs on their way to the sum over a token's slots: a signed 16-bit mantissa a value under a
-// power of two for every 32 columns. Half a unit is 2^-15 of the largest of the 32 or less, where bf16
-// would round every value by 2^-9 and cost the layer's output a third of its accuracy (relative to 64 bits
-// 2.9e-3 in bf16, so 2.4e-3), at the traffic of 16 bits: fp32 slots would be 0.5 GB more of it in an
-// 8,192-token prefill, some 100 us of 780. Where a value is inf or NaN the scale is inf and the 32 values
-// are plain bf16.
+// Slot outputs on their way to the sum over a token's slots: a signed 16-bit mantissa a value under
+// a power of two for every 32 columns. Half a unit is 2^-15 of the largest of the 32 or less, where
+// bf16 would round every value by 2^-9 and cost the layer's output a third of its accuracy
+// (relative to 64 bits 2.9e-3 in bf16, so 2.4e-3), at the traffic of 16 bits: fp32 slots would be
+// 0.5 GB more of it in an 8,192-token prefill, some 100 us of 780. Where a value is inf or NaN the
+// scale is inf and the 32 values are plain bf16.
 struct SlotCode {
   // The codes of a lane's 16 values v * scale, two a word; lane ^ 32 holds the other 16 of the 32
   // columns. Returns the power of two as bf16.
@@ -260,9 +260,9 @@ __device__ __forceinline__ bool row_tile(const ProductArgs& a, int tm, RowTile* 
 }
 
 // Workgroup -> (row tile, column tile). Workgroup i runs on XCD i mod 8; every XCD takes a
-// contiguous eighth of the tiles, so those that share weights or rows of x meet in its L2. False for the workgroups past the last tile (the grid of a grouped product
-// is sized for the most tiles that its rows can need). Where K is split, tm counts the
-// row tiles of every part in turn.
+// contiguous eighth of the tiles, so those that share weights or rows of x meet in its L2. False
+// for the workgroups past the last tile (the grid of a grouped product is sized for the most tiles
+// that its rows can need). Where K is split, tm counts the row tiles of every part in turn.
 template <int MODE>
 __device__ __forceinline__ bool tile_of_block(const ProductArgs& a, int splits, int* tm, int* tn) {
   int count;
@@ -278,9 +278,9 @@ __device__ __forceinline__ bool tile_of_block(const ProductArgs& a, int splits, 
   const int lin = static_cast<int>(blockIdx.x & 7) * per + i;
   if (i >= per || lin >= total) return false;
   if constexpr (MODE == kDense) {
-    // Column tiles in groups of eight, every row tile within a group: the 32 tiles that an XCD runs at
-    // once then read 4 x 8 tiles' rows instead of 2 x 16 (int8 8192 x 24576 x 4096 834 -> 788 us; 8192 x
-    // 4096 x 12288 and 6144 x 4096 the same within the noise).
+    // Column tiles in groups of eight, every row tile within a group: the 32 tiles that an XCD runs
+    // at once then read 4 x 8 tiles' rows instead of 2 x 16 (int8 8192 x 24576 x 4096 834 -> 788
+    // us; 8192 x 4096 x 12288 and 6144 x 4096 the same within the noise).
     constexpr int kGroup = 8;
     const int group = lin / (kGroup * count);
     const int wide = min(kGroup, a.tiles_n - group * kGroup);
@@ -556,16 +556,15 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
   }
 }
 
-// ---------------------------------------------------------------------------- product_large
-// For many rows: a BM x 256 tile on NW = 8 waves, two a SIMD, each with a (BM / 2) x 64 block of it, and as
-// many 128-byte steps in flight as LDS holds. The schedule is written out: an MFMA, then one of the
-// next quarter step's operand reads or one of the copies into the buffer that the last barrier
-// freed, fixed by scheduling barriers.
-// Measured on the experts of an 8,192-token prefill (65,536 rows in 128 groups): the copies
-// alone take 335 us of gate_up's 440 (11 TB/s into LDS, 44% of it from beyond L2), the MFMAs with
-// operands in L1 320; down 247 and 184 of 275. Four waves of 128 x 128 read LDS a third less but leave
-// each SIMD idle at every wait (480 and 316 us); 64-byte steps with 128 KiB in flight instead of 64 are
-// no quicker (480 and 305), so it is not latency.
+// ---------------------------------------------------------------------------- product_large For
+// many rows: a BM x 256 tile on NW = 8 waves, two a SIMD, each with a (BM / 2) x 64 block of it,
+// and as many 128-byte steps in flight as LDS holds. The schedule is written out: an MFMA, then one
+// of the next quarter step's operand reads or one of the copies into the buffer that the last
+// barrier freed, fixed by scheduling barriers. Measured on the experts of an 8,192-token prefill
+// (65,536 rows in 128 groups): the copies alone take 335 us of gate_up's 440 (11 TB/s into LDS, 44%
+// of it from beyond L2), the MFMAs with operands in L1 320; down 247 and 184 of 275. Four waves of
+// 128 x 128 read LDS a third less but leave each SIMD idle at every wait (480 and 316 us); 64-byte
+// steps with 128 KiB in flight instead of 64 are no quicker (480 and 305), so it is not latency.
 constexpr int kLargeN = 256;
 
 template <int BM>
@@ -579,8 +578,8 @@ constexpr int large_stage_bytes() {
 constexpr int kLargeEdges = 3 * large_stage_bytes<128>();  // LDS behind the stages: the edges
 static_assert(kLargeEdges >= 2 * large_stage_bytes<256>(), "the edges follow the stages");
 
-// The tile's K loop: acc[i][j] of A block i (32 weight rows) and B block j (32 rows of x). TAIL: K ends
-// inside a step. Compiled apart, as the question at every copy costs 8% of the loop.
+// The tile's K loop: acc[i][j] of A block i (32 weight rows) and B block j (32 rows of x). TAIL: K
+// ends inside a step. Compiled apart, as the question at every copy costs 8% of the loop.
 template <int IN, int MODE, bool SILU, int BM, int NW, bool TAIL>
 __device__ __forceinline__ void large_loop(const ProductArgs& a, const RowTile& t, int n0,
                                            uint8_t* lds,
@@ -983,8 +982,8 @@ __global__ __launch_bounds__(256) void product_rows(ProductArgs a) {
 }
 
 // ---------------------------------------------------------------------------- the choice of tiles
-// The tiles that a product can take, smallest first. k128 has four stages and a CU for itself, k128Two
-// has two stages and shares the CU with another.
+// The tiles that a product can take, smallest first. k128 has four stages and a CU for itself,
+// k128Two has two stages and shares the CU with another.
 enum class Tile { k64, k128, k128Two, k256x128, k256 };
 constexpr int kTiles = 5;
 
@@ -998,12 +997,13 @@ constexpr TileShape kTileShapes[] = {
 
 // Estimated time in us of `row_tiles` x `column_tiles` tiles over K. A CU's copies into LDS come at
 // about 60 GB/s where they miss L2, whatever the depth of the ring, which makes the step of a tile
-// its bytes; one workgroup a CU, but three of 64 x 64 (with three stages in LDS; with four, two of them:
-// the 8-bit experts of 40 tokens 57 + 33 us instead of 53 + 29). A 256 x 256 tile of up to 128 rows runs as half a
-// tile. Weights come at 5.8 TB/s at most. Measured, int8: 4096 x 4096 at 64 rows 64 x 64 tiles 13.0 us,
-// 128 x 128 19.5, 256 x 256 25.2; 6144 x 4096 at 512 rows 33.9 / 25.2 / 34.4 (256 x 128) / 47.2, at 1,024
-// rows 62 / 54 / 37.5 / 49, at 2,048 rows 118 / 79 / 76 / 56. bf16 experts 128 x (1536 x 2048) at 64 rows
-// each 202 / 182 / 221 / 187, at 128 rows 296 / 229 / 239 / 208.
+// its bytes; one workgroup a CU, but three of 64 x 64 (with three stages in LDS; with four, two of
+// them: the 8-bit experts of 40 tokens 57 + 33 us instead of 53 + 29). A 256 x 256 tile of up to
+// 128 rows runs as half a tile. Weights come at 5.8 TB/s at most. Measured, int8: 4096 x 4096 at 64
+// rows 64 x 64 tiles 13.0 us, 128 x 128 19.5, 256 x 256 25.2; 6144 x 4096 at 512 rows 33.9 / 25.2 /
+// 34.4 (256 x 128) / 47.2, at 1,024 rows 62 / 54 / 37.5 / 49, at 2,048 rows 118 / 79 / 76 / 56.
+// bf16 experts 128 x (1536 x 2048) at 64 rows each 202 / 182 / 221 / 187, at 128 rows 296 / 229 /
+// 239 / 208.
 inline float tile_estimate(Tile tile, float row_tiles, float column_tiles, int64_t k_bytes,
                            float weight_bytes, bool half, int cus) {
   const TileShape& t = kTileShapes[static_cast<int>(tile)];

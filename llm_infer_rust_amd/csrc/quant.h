@@ -106,16 +106,18 @@ inline RowsToQuantize rows_to_quantize(const void* x, int64_t stride, void* valu
           static_cast<int32_t>(width), static_cast<int32_t>(padded / 16)};
 }
 
-// K of an int8 product in bytes: the weight rows' elements and, where their stride `ld` holds them, the
-// rest of the last 128-byte step, else of the last 16 bytes. The quantised rows are zeros there.
+// K of an int8 product in bytes: the weight rows' elements and, where their stride `ld` holds them,
+// the rest of the last 128-byte step, else of the last 16 bytes. The quantised rows are zeros
+// there.
 inline int64_t int8_k(int64_t k, int64_t ld) {
   const int64_t steps = (k + 127) / 128 * 128;
   return ld >= steps ? steps : (k + 15) / 16 * 16;
 }
 
-// One row per LANES threads (a wave, or four). The row's first HELD chunks of
-// 16 a thread stay in registers between the two passes, the rest is read again. Bound by memory:
-// every row is read once and written at half its size (8,192 rows of 4,096 bf16: 100 MB). `wave_top` is an LDS word a wave of the workgroup.
+// One row per LANES threads (a wave, or four). The row's first HELD chunks of 16 a thread stay in
+// registers between the two passes, the rest is read again. Bound by memory: every row is read once
+// and written at half its size (8,192 rows of 4,096 bf16: 100 MB). `wave_top` is an LDS word a wave
+// of the workgroup.
 template <int DT, int LANES, int HELD>
 __device__ __forceinline__ void quantize_row(const RowsToQuantize& q, int64_t row,
                                              uint32_t* wave_top) {
