@@ -134,6 +134,8 @@ class Qwen3Model:
         mats = [self.embed_tokens] + [m for layer in self.layers for m in layer.matrices()]
         if not self.cfg.tie_word_embeddings:
             mats.append(self.lm_head)
+        if any(isinstance(m, Int8Weight) for m in mats):
+            raise ModelError("weights are drawn before they are quantised")
         for m in mats:
             m.normal_(0.0, std, generator=g)
         return self

@@ -303,6 +303,8 @@ def decode_linear(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | Non
     tiling (tuning and tests); -1 lets the library choose. Replaces the decode-time
     ``x.matmul(w.T)`` of ``src/layers/linear.rs:5-7``."""
     _require_device(x, "decode_linear")
+    if isinstance(weight, Int8Weight):
+        raise NativeError("decode_linear: a weight in 8 bits goes to linear_int8")
     dt = dtype_code(x)
     if (x.dim() != 2 or weight.dim() != 2 or x.stride(1) != 1 or not weight.is_contiguous()
             or weight.dtype != x.dtype or weight.device != x.device
@@ -407,6 +409,8 @@ def decode_linear_silu_mul(x: torch.Tensor, weight: torch.Tensor,
     and one split followed by ``silu_and_mul`` (another tile width, or another number of row
     tiles, sums K in another order)."""
     _require_device(x, "decode_linear_silu_mul")
+    if isinstance(weight, Int8Weight):
+        raise NativeError("decode_linear_silu_mul: a weight in 8 bits goes to linear_int8")
     dt = dtype_code(x)
     if (x.dim() != 2 or weight.dim() != 2 or x.stride(1) != 1 or not weight.is_contiguous()
             or weight.dtype != x.dtype or weight.device != x.device
@@ -460,6 +464,8 @@ def head_linear(x: torch.Tensor, weight: torch.Tensor,
                 out: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T`` for the lm_head (``weight [vocab, K]``), into ``out`` when given. A
     product whose gradient or tangent is wanted stays with torch, which records it."""
+    if isinstance(weight, Int8Weight):
+        return linear_int8(x, weight, out=out)
     wants_grad = torch.is_grad_enabled() and (
         x.requires_grad or weight.requires_grad or (out is not None and out.requires_grad))
     if (not wants_grad and _ordinary(x, weight) and x.is_cuda and x.dim() == 2

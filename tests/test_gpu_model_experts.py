@@ -167,6 +167,11 @@ def test_ops_take_8_bit_weights(gpu):
     want = ops.add_rms_norm(y.clone(), residual.clone(), gamma, 1e-6)
     got = ops.linear_add_rms_norm(x, w, residual, gamma, 1e-6)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+    out = torch.empty_like(y)
+    assert torch.equal(ops.head_linear(x, w), y) and torch.equal(ops.head_linear(x, w, out=out), y)
+    for entry in (ops.decode_linear, ops.decode_linear_silu_mul):  # the 16-bit kernels themselves
+        with pytest.raises(ops.NativeError):
+            entry(x, w)
 
 
 def test_quantized_weights_are_not_loaded_over(gpu):
@@ -177,6 +182,8 @@ def test_quantized_weights_are_not_loaded_over(gpu):
     assert model.quantize_int8().layers[0].qkv_proj is first  # once
     with pytest.raises(ModelError):
         model.load_weights(params)
+    with pytest.raises(ModelError):
+        model.init_random(3)
 
 
 def test_expert_model_loads_its_weights(gpu):
