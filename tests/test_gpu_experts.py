@@ -370,7 +370,8 @@ def test_infinite_weights(gpu, t):
 def test_two_streams_at_once(gpu):
     jobs = []
     for t, h, i, i8 in ((2, 128, 64, False), (40, 104, 2056, False), (90, 128, 64, True),
-                        (600, 2056, 72, False), (1200, 72, 1032, True)):
+                        (600, 2056, 72, False), (1200, 72, 1032, True),
+                        (4100, 1032, 520, False), (3001, 2056, 72, True)):
         x, ids, w, gu, dn = (a.to(gpu) for a in problem(t, 4, 2, h, i, torch.bfloat16, t))
         if i8:
             gu, dn = int8.Int8Weight.quantize(gu), int8.Int8Weight.quantize(dn)
