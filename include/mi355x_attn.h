@@ -399,8 +399,7 @@ int64_t mi355x_expert_mlp_workspace_bytes(int64_t tokens, int64_t top_k, int64_t
  * Scales given (fp32 [experts, 2 inter] and [experts, hidden]): int8 weights. x is quantised once
  * a token, silu(g) * u (kept in fp32) once a slot, both as mi355x_quantize_rows does; any sizes and
  * x strides, weight rows as for mi355x_linear_int8.
- * Slot outputs on their way to the sum are held in 16 bits under a scale for every 32 columns (to
- * 2^-15 of the largest of them, or in fp32 where a few slots run one by one).
+ * Slot outputs are fp32 up to the sum over a token's slots, which is rounded once.
  * Nothing is read back to the host. An expert's weights are less than 4 GiB. Calls that overlap
  * need workspaces of their own. */
 const char* mi355x_expert_mlp(const void* x, int64_t ldx, const int32_t* ids,

@@ -260,33 +260,28 @@ __global__ __launch_bounds__(kGroupThreads) void place_and_quantize(SlotsToPlace
 }
 
 // ---------------------------------------------------------------------------- the sum over slots
-// out[t] = sum of y[t * top_k + s] (SlotCodes) over the slots that take part and the parts of K, in
-// fp32 and in this order. A thread takes 8 H columns, a quarter or half of what a scale covers.
-// Bound by memory where there are many tokens (8,192 of 8 slots and 2,048 columns: 277 MB in 60 us
-// with H 2, 69 with H 1), else by latency: H 1 and workgroups of a wave spread over the chip (40
-// tokens 7.1 us with H 2 and 256 threads).
+// out[t] = sum of y[t * top_k + s] (fp32) over the slots that take part and the parts of K, in
+// fp32 and in this order. A thread takes 4 H columns. Bound by memory where there are many tokens,
+// else by latency: H 1 and workgroups of a wave spread over the chip.
 template <int DT, int H, int THREADS, bool PARTS>
-__global__ __launch_bounds__(THREADS) void sum_slots(const uint16_t* __restrict__ y, int64_t ldy,
-                                                 const uint16_t* __restrict__ scales,
-                                                 int64_t ld_scales,
+__global__ __launch_bounds__(THREADS) void sum_slots(const float* __restrict__ y, int64_t ldy,
                                                  const int32_t* __restrict__ ids,
                                                  uint16_t* __restrict__ out, int64_t ldo,
                                                  int64_t tokens, int top_k, int splits, int experts,
                                                  int width) {
-  const int chunks = (width + 8 * H - 1) / (8 * H);
-  // at most 2^17 tokens of 2^14 chunks a pass
+  const int chunks = (width + 4 * H - 1) / (4 * H);
+  // at most 2^17 tokens of 2^14 chunks a pass (H 1: fewer than kManyValues values)
   const uint32_t i = blockIdx.x * uint32_t(THREADS) + threadIdx.x;
   const uint32_t t = i / static_cast<uint32_t>(chunks);
   if (t >= tokens) return;
-  const int c = static_cast<int>(i - t * chunks) * (8 * H);
-  float sum[H][8] = {};
+  const int c = static_cast<int>(i - t * chunks) * (4 * H);
+  float sum[4 * H] = {};
   constexpr int kAtOnce = 8;  // slots whose loads are on their way together
   const int first = static_cast<int>(t) * top_k, plane = static_cast<int>(tokens) * top_k;
   for (int s0 = 0; s0 < top_k * splits; s0 += kAtOnce) {
     bool in[kAtOnce];
     int32_t slots[kAtOnce];
     uint4 v[kAtOnce][H];
-    uint16_t scale[kAtOnce];
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
       const int n = min(s0 + i, top_k * splits - 1);
@@ -302,42 +297,33 @@ __global__ __launch_bounds__(THREADS) void sum_slots(const uint16_t* __restrict_
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i)
       if (in[i]) {
-        const int64_t slot = slots[i];
+        // rows of y are padded to 8 columns
 #pragma unroll
-        for (int h = 0; h < H; ++h) v[i][h] = ld128(y + slot * ldy + c + 8 * h);
-        scale[i] = scales[slot * ld_scales + c / 32];
+        for (int h = 0; h < H; ++h)
+          v[i][h] = ld128(y + static_cast<int64_t>(slots[i]) * ldy + c + 4 * h);
       }
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
       if (!in[i]) continue;
-      const float unit = Elem<kBf16>::to_float(scale[i]);
 #pragma unroll
       for (int h = 0; h < H; ++h) {
-        const uint32_t w[4] = {v[i][h].x, v[i][h].y, v[i][h].z, v[i][h].w};
-        if (unit < INFINITY) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            sum[h][e] += SlotCode::value(static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1))), unit);
-        } else {
-          float f[8];
-          unpack8<kBf16>(v[i][h], f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) sum[h][e] += f[e];
-        }
+        sum[4 * h] += __uint_as_float(v[i][h].x);
+        sum[4 * h + 1] += __uint_as_float(v[i][h].y);
+        sum[4 * h + 2] += __uint_as_float(v[i][h].z);
+        sum[4 * h + 3] += __uint_as_float(v[i][h].w);
       }
     }
   }
+  uint16_t* o = out + static_cast<int64_t>(t) * ldo + c;
+  if (c + 4 * H <= width) {
+    if constexpr (H == 2)
+      st128_any(o, pack8<DT>(sum));
+    else
+      st64_any(o, make_uint2(Elem<DT>::pack2(sum[0], sum[1]), Elem<DT>::pack2(sum[2], sum[3])));
+  } else {
 #pragma unroll
-  for (int h = 0; h < H; ++h) {
-    const int at = c + 8 * h;
-    uint16_t* o = out + static_cast<int64_t>(t) * ldo + at;
-    if (at + 8 <= width) {
-      st128_any(o, pack8<DT>(sum[h]));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (at + e < width) o[e] = Elem<DT>::from_float(sum[h][e]);
-    }
+    for (int e = 0; e < 4 * H; ++e)
+      if (c + e < width) o[e] = Elem<DT>::from_float(sum[e]);
   }
 }
 
@@ -400,6 +386,7 @@ float grouped_estimate(Tile tile, float count, float steps, float weight_bytes, 
 // summed afterwards may be cut along K as well, where its tiles leave CUs without one: the parts
 // are summed with the slots (down of 8 experts 1024 x 2816 at 77 tokens 17.0 us whole, 11.6 in two
 // parts).
+constexpr int64_t kManyValues = int64_t(1) << 22;  // slot outputs that fill the chip by themselves
 GroupedPlan choose_grouped(int64_t slots, int64_t experts, int64_t weight_rows, int64_t k_bytes,
                            bool summed, int cus) {
   const float active = static_cast<float>(std::min(slots, experts));
@@ -415,12 +402,13 @@ GroupedPlan choose_grouped(int64_t slots, int64_t experts, int64_t weight_rows, 
     for (int s = 1; s <= (summed && tile == Tile::k64 ? 4 : 1); s *= 2) {
       const int64_t part = (steps + s - 1) / s;
       if (s > 1 && (part < 8 || part * (s - 1) >= steps ||
-                    count * static_cast<float>(s / 2) >= static_cast<float>(cus)))
+                    count * static_cast<float>(s / 2) >= static_cast<float>(cus) ||
+                    slots * weight_rows >= kManyValues))
         break;
       float us = grouped_estimate(tile, count * static_cast<float>(s), static_cast<float>(part),
                                   weights, per <= 128.f, cus);
-      // two bytes a value more, out and back
-      us += static_cast<float>(s - 1) * (0.3f + static_cast<float>(slots * weight_rows) * 4 / 4.5e6f);
+      // four bytes a value more, out and back
+      us += static_cast<float>(s - 1) * (0.3f + static_cast<float>(slots * weight_rows) * 8 / 4.5e6f);
       if (us < best_us) {
         best_us = us;
         best = {tile, s};
@@ -434,7 +422,7 @@ constexpr int64_t kMaxSlots = 131072;  // slots a pass takes; more tokens run in
 
 struct ExpertWorkspace {
   int64_t order, row_weights, gate_up_tiles, down_tiles, tile_counts, counts, xq, xs, act, actq, acts,
-      y, y_scales, bytes;
+      y, bytes;
   int64_t tokens;  // a pass
   GroupedPlan gate_up, down;
 };
@@ -473,8 +461,7 @@ ExpertWorkspace expert_workspace(int64_t tokens, int64_t top_k, int64_t experts,
     w.actq = take(slots * pad(inter, 128));
     w.acts = take(slots * 4);
   }
-  w.y = take(slots * w.down.splits * pad(hidden, 32) * 2);
-  w.y_scales = take(slots * w.down.splits * (pad(hidden, 64) / 32) * 2);
+  w.y = take(slots * w.down.splits * pad(hidden, 8) * 4);
   w.bytes = at;
   return w;
 }
@@ -676,27 +663,24 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   a.w_scales = c.down_scales;
   a.out = ws + w.y;
   a.splits = w.down.splits;
-  a.ldo = pad(c.hidden, 32);
-  a.code_scales = reinterpret_cast<uint16_t*>(ws + w.y_scales);
-  a.ld_code_scales = pad(c.hidden, 64) / 32;
+  a.ldo = pad(c.hidden, 8);
   a.columns = static_cast<int32_t>(c.hidden);
-  launch_product<IN, OT, kDown, false>(a, w.down.tile, slots, c.experts, s);
+  launch_product<IN, kFloatOut, kDown, false>(a, w.down.tile, slots, c.experts, s);
   if (const char* e = launch_status("product (down)")) return e;
-  const auto* y = reinterpret_cast<const uint16_t*>(ws + w.y);
+  const auto* y = reinterpret_cast<const float*>(ws + w.y);
   auto sum = [&](auto kernel, int columns, int threads) {
     const int64_t n = c.tokens * ((c.hidden + columns - 1) / columns);
     kernel<<<dim3(static_cast<uint32_t>((n + threads - 1) / threads)), threads, 0, s>>>(
-        y, a.ldo, a.code_scales, a.ld_code_scales, c.ids, c.out, c.ldo, c.tokens,
+        y, a.ldo, c.ids, c.out, c.ldo, c.tokens,
         static_cast<int>(c.top_k), w.down.splits, static_cast<int>(c.experts),
         static_cast<int>(c.hidden));
   };
-  const bool many = c.tokens * c.hidden >= (int64_t(1) << 22);
   if (w.down.splits > 1)
-    sum(sum_slots<OT, 1, kWave, true>, 8, kWave);
-  else if (many)
-    sum(sum_slots<OT, 2, 256, false>, 16, 256);
+    sum(sum_slots<OT, 1, kWave, true>, 4, kWave);
+  else if (c.tokens * c.hidden >= kManyValues)
+    sum(sum_slots<OT, 2, 256, false>, 8, 256);
   else
-    sum(sum_slots<OT, 1, kWave, false>, 8, kWave);
+    sum(sum_slots<OT, 1, kWave, false>, 4, kWave);
   return launch_status("sum_slots");
 }
 

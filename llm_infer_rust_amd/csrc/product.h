@@ -33,7 +33,7 @@ constexpr int kFloatOut = 2;                    // outputs: 0 bf16, 1 fp16, 2 fp
 //   kDense    row r of x and of out is r; one weight
 //   kGateUp   row r of the grouped order reads x row order[r] / top_k and writes out row r
 //   kDown     row r of the grouped order reads x row r and writes out row order[r], times that
-//             slot's weight, as SlotCodes
+//             slot's weight, in fp32
 //   kSplit    kDense over a part of K, the int32 sums left as they are (int8 only)
 constexpr int kDense = 0, kGateUp = 1, kDown = 2, kSplit = 3;
 
@@ -48,8 +48,6 @@ struct ProductArgs {
   const int4* tiles;          // grouped: {expert, first row, end row, 0} per row tile
   const int32_t* tile_count;  // grouped: tiles in the list
   const float* row_weights;   // kDown: weight of every row of the grouped order
-  uint16_t* code_scales;      // kDown: scale of every 32 columns of an out row (see SlotCode)
-  int64_t ld_code_scales;
   int64_t x_stride;           // bytes a row
   int64_t w_stride;           // bytes a row
   int64_t w_expert;           // bytes an expert
@@ -133,53 +131,6 @@ __device__ __forceinline__ void store4(void* out, int64_t at, const float (&v)[4
   }
 }
 
-// Slot outputs on their way to the sum over a token's slots: a signed 16-bit mantissa a value under
-// a power of two for every 32 columns. Half a unit is 2^-15 of the largest of the 32 or less, where
-// bf16 would round every value by 2^-9 and cost the layer's output a third of its accuracy
-// (relative to 64 bits 2.9e-3 in bf16, so 2.4e-3), at the traffic of 16 bits: fp32 slots would be
-// 0.5 GB more of it in an 8,192-token prefill, some 100 us of 780. Where a value is inf or NaN the
-// scale is inf and the 32 values are plain bf16.
-struct SlotCode {
-  // The codes of a lane's 16 values v * scale, two a word; lane ^ 32 holds the other 16 of the 32
-  // columns. Returns the power of two as bf16.
-  __device__ __forceinline__ static uint16_t pack(const float (&v)[16], float scale,
-                                                  uint32_t (&w)[8]) {
-    float most = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; i += 2) most = fmaxf(fmaxf(most, fabsf(v[i])), fabsf(v[i + 1]));
-    const uint32_t top = joined(__float_as_uint(most * fabsf(scale)), true);
-    // The largest comes to below 2^15 with a margin for the rounding to an integer.
-    const uint32_t e = max((top + 0x180) >> 23, 15u);
-    const float factor = scale * __uint_as_float((268u - e) << 23);  // 2^(141 - e)
-    // 1.5 * 2^23 rounds to integers in the low bits. What is not finite leaves its exponent here.
-    uint32_t seen = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t lo = __float_as_uint(fmaf(v[2 * i], factor, 12582912.f));
-      const uint32_t hi = __float_as_uint(fmaf(v[2 * i + 1], factor, 12582912.f));
-      seen |= lo | hi;
-      w[i] = __builtin_amdgcn_perm(hi, lo, 0x05040100);
-    }
-    const bool plain = (joined(seen, false) & 0x34000000u) != 0 || top >= 0x7f800000u;
-    if (__any(plain)) {  // seldom
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (plain) w[i] = Elem<kBf16>::pack2(v[2 * i] * scale, v[2 * i + 1] * scale);
-    }
-    return plain ? 0x7f80 : (e - 14) << 7;  // 2^(e - 141)
-  }
-  __device__ __forceinline__ static float value(uint16_t code, float scale) {
-    return static_cast<float>(static_cast<int16_t>(code)) * scale;
-  }
-
- private:
-  // With the word of lane ^ 32: the larger, or the bits of both.
-  __device__ __forceinline__ static uint32_t joined(uint32_t x, bool larger) {
-    const auto both = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    return larger ? max(both[0], both[1]) : both[0] | both[1];
-  }
-};
-
 // What a row of a tile is multiplied with and where it goes.
 struct RowOut {
   int64_t at;    // row of out
@@ -214,7 +165,12 @@ __device__ __forceinline__ void finish_values(const ProductArgs& a, const RowOut
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     float g = static_cast<float>(acc[e]);
-    if constexpr (IN == kInt8) g = g * r.scale * w_scales[min(column + e, a.columns - 1)];
+    if constexpr (MODE == kDown) {
+      if constexpr (IN == kInt8) g *= w_scales[min(column + e, a.columns - 1)];
+      g *= r.scale * r.weight;
+    } else if constexpr (IN == kInt8) {
+      g = g * r.scale * w_scales[min(column + e, a.columns - 1)];
+    }
     if constexpr (SILU) {
       float u = static_cast<float>(up[e]);
       if constexpr (IN == kInt8)
@@ -516,30 +472,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
       continue;
     }
     RowOut r = row_out<IN, MODE>(a, row);
-    if constexpr (MODE == kDown) {
-      r.at += static_cast<int64_t>(split) * a.rows;
-#pragma unroll
-      for (int i = 0; i < A_BLK; ++i) {
-        const int column = n0 + wn * kWaveN + 32 * i;
-        float v[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          v[e] = static_cast<float>(acc[i][j][e]);
-          if constexpr (IN == kInt8)
-            v[e] *= w_scales[min(column + 8 * (e >> 2) + 4 * half + (e & 3), a.columns - 1)];
-        }
-        uint32_t w[8];
-        const uint16_t scale = SlotCode::pack(v, r.scale * r.weight, w);
-        if (column >= a.columns) continue;
-        if (half == 0) a.code_scales[r.at * a.ld_code_scales + column / 32] = scale;
-        // ldo is a multiple of 32: codes past the end have their place
-        uint16_t* p = static_cast<uint16_t*>(a.out) + r.at * a.ldo + column + 4 * half;
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<uint2*>(p + 8 * q) = make_uint2(w[2 * q], w[2 * q + 1]);
-      }
-      continue;
-    }
+    if constexpr (MODE == kDown) r.at += static_cast<int64_t>(split) * a.rows;
 #pragma unroll
     for (int i = 0; i < A_BLK; ++i)
 #pragma unroll
@@ -715,7 +648,6 @@ __device__ __forceinline__ void large_loop(const ProductArgs& a, const RowTile& 
 // What the epilogue needs of the tile's rows and columns, in LDS once the stages are free.
 struct LargeEdges {
   int64_t out[256];         // byte offset of the row
-  int32_t out_row[256];
   float row_scale[256];     // int8: of the x row; kDown: times the slot's weight
   float column_scale[256];  // int8: of the tile's weight rows (SILU: 128 gate, then 128 up)
 };
@@ -762,7 +694,6 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
     const int begin = wm * (BM / 2) + 32 * j;  // row of the tile
     if (t.begin + begin >= t.end) break;
     const float row_scale = edges.row_scale[begin + col];
-    uint32_t scales = 0;  // kDown: of the codes of both A blocks
 #pragma unroll
     for (int i = 0; i < A_BLK; ++i) {
       float f[16];  // of 32 columns (SILU: the 8 of 16)
@@ -773,6 +704,7 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
           float g = static_cast<float>(acc[i][j][4 * q + e]);
           if constexpr (IN == kInt8 && MODE != kDown) g *= row_scale;
           if constexpr (IN == kInt8) g *= gs[i][q][e];
+          if constexpr (MODE == kDown) g *= row_scale;
           if constexpr (SILU) {
             float u = static_cast<float>(acc[i][j][(4 * q + 4 + e) & 15]);
             if constexpr (IN == kInt8) u = u * row_scale * us[i][q][e];
@@ -781,29 +713,17 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
           f[4 * q + e] = g;
         }
       }
-      uint32_t codes[8];
-      if constexpr (MODE == kDown)
-        scales |= static_cast<uint32_t>(SlotCode::pack(f, row_scale, codes)) << (16 * i);
 #pragma unroll
       for (int q = 0; q < 4; q += SILU ? 2 : 1) {
         const int wrow = 32 * i + 8 * q + 4 * half;
         uint8_t* p = turn + col * kPitch + (SILU ? silu_column(wrow) : wrow) * kOutSize;
         const float* v = f + 4 * q;
-        if constexpr (MODE == kDown)
-          *reinterpret_cast<uint2*>(p) = make_uint2(codes[2 * q], codes[2 * q + 1]);
-        else if constexpr (OT == kFloatOut)
+        if constexpr (OT == kFloatOut)
           *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
         else
           *reinterpret_cast<uint2*>(p) =
               make_uint2(Elem<OT>::pack2(v[0], v[1]), Elem<OT>::pack2(v[2], v[3]));
       }
-    }
-    if constexpr (MODE == kDown) {
-      static_assert(A_BLK == 2, "two scales a word");
-      const int block = n0 + wn * kCols;  // rows of scales are padded to whole words
-      if (half == 0 && t.begin + begin + col < t.end && block < a.columns)
-        *reinterpret_cast<uint32_t*>(a.code_scales + edges.out_row[begin + col] * a.ld_code_scales +
-                                     block / 32) = scales;
     }
     // A wave's LDS operations keep their order, so its reads follow its writes of all lanes; the
     // clobbers keep the compiler from exchanging them.
@@ -853,9 +773,7 @@ __device__ __forceinline__ void large_tile(const ProductArgs& a, const RowTile& 
   auto& edges = *reinterpret_cast<LargeEdges*>(lds + kLargeEdges);
   if constexpr (IN == kInt8 && MODE == kGateUp) row_scale = a.x_scales[slot / a.top_k];
   if (threadIdx.x < 256) {
-    const int out_row = MODE == kDown ? slot : row;
-    edges.out_row[r] = out_row;
-    edges.out[r] = out_row * a.ldo * (OT == kFloatOut ? 4 : 2);
+    edges.out[r] = (MODE == kDown ? slot : row) * a.ldo * (OT == kFloatOut ? 4 : 2);
     edges.row_scale[r] = row_scale * weight;
     edges.column_scale[r] = column_scale;
   }
