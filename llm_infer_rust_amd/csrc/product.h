@@ -156,7 +156,9 @@ __device__ __forceinline__ RowOut row_out(const ProductArgs& a, int row) {
   return r;
 }
 
-// The accumulators of four consecutive columns of a row, scaled. `acc` (SILU: the gate columns, with
+// The accumulators of four consecutive columns of a row, scaled: first with the weight row's scale,
+// which is of ordinary size in any weight, so that the largest and smallest rows of x stay inside
+// the range of fp32 wherever the result does. `acc` (SILU: the gate columns, with
 // the matching up columns in `up`); the scales are those of the weight rows.
 template <int IN, int MODE, bool SILU, typename T>
 __device__ __forceinline__ void finish_values(const ProductArgs& a, const RowOut& r, int column,
@@ -165,16 +167,15 @@ __device__ __forceinline__ void finish_values(const ProductArgs& a, const RowOut
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     float g = static_cast<float>(acc[e]);
-    if constexpr (MODE == kDown) {
-      if constexpr (IN == kInt8) g *= w_scales[min(column + e, a.columns - 1)];
+    if constexpr (IN == kInt8) g *= w_scales[min(column + e, a.columns - 1)];
+    if constexpr (MODE == kDown)
       g *= r.scale * r.weight;
-    } else if constexpr (IN == kInt8) {
-      g = g * r.scale * w_scales[min(column + e, a.columns - 1)];
-    }
+    else if constexpr (IN == kInt8)
+      g *= r.scale;
     if constexpr (SILU) {
       float u = static_cast<float>(up[e]);
       if constexpr (IN == kInt8)
-        u = u * r.scale * w_scales[a.columns + min(column + e, a.columns - 1)];
+        u = u * w_scales[a.columns + min(column + e, a.columns - 1)] * r.scale;
       g = silu_mul(g, u);
     }
     v[e] = g;
@@ -702,12 +703,11 @@ __device__ __forceinline__ void large_store(const ProductArgs& a, const RowTile&
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float g = static_cast<float>(acc[i][j][4 * q + e]);
-          if constexpr (IN == kInt8 && MODE != kDown) g *= row_scale;
           if constexpr (IN == kInt8) g *= gs[i][q][e];
-          if constexpr (MODE == kDown) g *= row_scale;
+          if constexpr (IN == kInt8 || MODE == kDown) g *= row_scale;
           if constexpr (SILU) {
             float u = static_cast<float>(acc[i][j][(4 * q + 4 + e) & 15]);
-            if constexpr (IN == kInt8) u = u * row_scale * us[i][q][e];
+            if constexpr (IN == kInt8) u = u * us[i][q][e] * row_scale;
             g = silu_mul(g, u);
           }
           f[4 * q + e] = g;

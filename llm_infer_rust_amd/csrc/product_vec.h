@@ -178,10 +178,10 @@ __global__ __launch_bounds__(64 * WAVES) void product_vec(ProductArgs a, int wid
       const int c = n0 + (SILU ? r / 2 : r);
       if (c >= a.columns) continue;
       float v = static_cast<float>(acc[m][r]);
-      if constexpr (kQuant) v = v * scale[m] * w_scales[c];
+      if constexpr (kQuant) v = v * w_scales[c] * scale[m];
       if constexpr (SILU) {
         float u = static_cast<float>(acc[m][r + 1]);
-        if constexpr (kQuant) u = u * scale[m] * w_scales[a.columns + c];
+        if constexpr (kQuant) u = u * w_scales[a.columns + c] * scale[m];
         v = silu_mul(v, u);
       }
       if constexpr (OT == kFloatOut)
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(64 * WAVES) void product_vec_down(DownArgs a) {
       if (!in[i]) continue;
       float v = static_cast<float>(total);
       if constexpr (kQuant)
-        v = v * scales[slot[i]] * a.w_scales[static_cast<int64_t>(e[i]) * a.columns + c];
+        v = v * a.w_scales[static_cast<int64_t>(e[i]) * a.columns + c] * scales[slot[i]];
       sum += v * weight[i];
     }
   }
