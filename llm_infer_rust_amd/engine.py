@@ -463,7 +463,8 @@ class Engine:
         collecting = gc.isenabled()
         gc.disable()
         try:
-            self._capture_buckets()
+            with self.model.captured_for(self):
+                self._capture_buckets()
         finally:
             if collecting:
                 gc.enable()

@@ -24,6 +24,9 @@ routed experts (``experts.route_experts``, ``experts.expert_mlp``) in place of t
 """
 from __future__ import annotations
 
+import contextlib
+import gc
+import weakref
 from dataclasses import dataclass
 
 import torch
@@ -125,6 +128,10 @@ class Qwen3Model:
                                       device)
         self.attention = Attention.new(attention_backend, AttentionSpec(
             cfg.num_attention_heads, cfg.num_kv_heads, cfg.head_dim, dtype, device))
+        # Who holds captured graphs that read the weights where they are now (see quantize_int8).
+        self._graph_holders: weakref.WeakSet = weakref.WeakSet()
+        self._captured_by_caller = False
+        self._capturing = False
 
     # ------------------------------------------------------------------ weights
     def init_random(self, seed: int, std: float = 0.02) -> "Qwen3Model":
@@ -165,7 +172,13 @@ class Qwen3Model:
     def quantize_int8(self) -> "Qwen3Model":
         """The layers' QKV, o, gate_up and down matrices (those of experts too) in 8 bits, one scale
         a row; embeddings, norms, routers and the head stay as they are. Done once, after the
-        weights are loaded, and before a decode graph is captured over them."""
+        weights are loaded, and before a graph is captured over them: refused while an engine with
+        captured graphs exists, and for good after any other capture of ``forward``, as a replay
+        would read the memory of the 16-bit matrices that are let go here."""
+        if len(self._graph_holders):
+            gc.collect()  # engines that nothing refers to any more
+        if self._captured_by_caller or len(self._graph_holders):
+            raise ModelError("weights are quantised before a graph is captured over them")
         for layer in self.layers:
             for name in ("qkv_proj", "o_proj", "gate_up_proj", "down_proj"):
                 weight = getattr(layer, name)
@@ -194,6 +207,16 @@ class Qwen3Model:
             raise ModelError(f"missing weights: {missing[:4]}")
         return loaded
 
+    @contextlib.contextmanager
+    def captured_for(self, holder):
+        """Around captures of ``forward`` whose graphs live no longer than ``holder``."""
+        self._graph_holders.add(holder)
+        self._capturing = True
+        try:
+            yield
+        finally:
+            self._capturing = False
+
     def bind_kv_cache(self, pool, reserved_slot: int = 0) -> None:
         """Bind every layer to its views of a ``KVCachePool`` (page 0 reserved)."""
         if pool.layout.num_layers != self.cfg.num_layers:
@@ -218,6 +241,8 @@ class Qwen3Model:
         cfg = self.cfg
         if input_ids.dim() != 1 or positions.shape != input_ids.shape:
             raise ModelError("input_ids and positions must have identical lengths")
+        if not self._capturing and torch.cuda.is_current_stream_capturing():
+            self._captured_by_caller = True
         t = input_ids.size(0)
         hq, hkv, d = cfg.num_attention_heads, cfg.num_kv_heads, cfg.head_dim
         eps = cfg.rms_norm_eps
