@@ -90,7 +90,8 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     if not int8 and ((h | inter | ldx) % 8 or (xp | gp | dp) % 16):
         raise NativeError("expert_mlp: 16-bit weights need H, I and x's row stride to be multiples "
                           "of 8 and 16-byte aligned rows")
-    _refuse_grad("expert_mlp", x, weights, gu, dn)
+    gs, ds = (gate_up.scales, down.scales) if int8 else (None, None)
+    _refuse_grad("expert_mlp", x, weights, gu, dn, gs, ds, out)
     out, ldo = _output(out, x, h, "expert_mlp")
     cus = device_cus(device)
     native = lib()
@@ -98,10 +99,10 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     if need < 0:
         raise NativeError("expert_mlp: invalid shape")
     ws = torch.empty(need or 16, dtype=torch.uint8, device=device)
-    ldg, ldd, gs, ds = h, inter, None, None
+    ldg, ldd = h, inter
     if int8:
         ldg, ldd = gate_up.row_stride, down.row_stride
-        gs, ds = gate_up.scales.data_ptr(), down.scales.data_ptr()
+        gs, ds = gs.data_ptr(), ds.data_ptr()
     with on_device(device):
         check(native.mi355x_expert_mlp(
             xp, ldx, ids.data_ptr(), weights.data_ptr(), gp, ldg, gs, dp, ldd, ds, out.data_ptr(),

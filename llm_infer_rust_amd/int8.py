@@ -24,9 +24,11 @@ def _padded(k: int, to: int) -> int:
     return (k + to - 1) // to * to
 
 
-def _refuse_grad(what: str, *tensors: torch.Tensor) -> None:
+def _refuse_grad(what: str, *tensors: torch.Tensor | None) -> None:
+    if not torch.is_grad_enabled():
+        return
     for t in tensors:
-        if t.requires_grad and torch.is_grad_enabled():
+        if t is not None and t.requires_grad:
             raise NativeError(f"{what}: no gradient is recorded; call it under torch.no_grad()")
 
 
@@ -153,7 +155,7 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = 
         raise NativeError("linear_int8: expected x [T, K] and a weight [N, K] on one device")
     if silu_mul and n % 2:
         raise NativeError("linear_int8: a gate_up weight has an even number of rows")
-    _refuse_grad("linear_int8", x)
+    _refuse_grad("linear_int8", x, scales, out)
     out, ldo = _output(out, x, n // 2 if silu_mul else n, "linear_int8")
     cus = device_cus(device)
     native = lib()
