@@ -6,7 +6,7 @@
 
 In place of the dense MLP of ``src/models/qwen3/model.rs:478-534``; the reference has no layers of
 experts. Nothing is read back to the host, so both can be captured in a HIP graph. Inference only:
-a call whose gradient would be wanted is refused.
+a call whose derivative would be wanted is refused.
 """
 from __future__ import annotations
 
@@ -75,6 +75,8 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     if int8 != isinstance(down, Int8Weight):
         raise NativeError("expert_mlp: gate_up and down must be of one kind")
     gu, dn = (gate_up.values, down.values) if int8 else (gate_up, down)
+    _refuse_grad("expert_mlp", x, weights, *((gate_up.scales, down.scales) if int8 else (gu, dn)),
+                 out)
     if (gu.dim() != 3 or dn.dim() != 3 or gu.get_device() != index or dn.get_device() != index
             or (not int8 and (gu.dtype != dtype or dn.dtype != dtype
                               or not gu.is_contiguous() or not dn.is_contiguous()))):
@@ -90,8 +92,6 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     if not int8 and ((h | inter | ldx) % 8 or (xp | gp | dp) % 16):
         raise NativeError("expert_mlp: 16-bit weights need H, I and x's row stride to be multiples "
                           "of 8 and 16-byte aligned rows")
-    gs, ds = (gate_up.scales, down.scales) if int8 else (None, None)
-    _refuse_grad("expert_mlp", x, weights, gu, dn, gs, ds, out)
     out, ldo = _output(out, x, h, "expert_mlp")
     cus = device_cus(device)
     native = lib()
@@ -99,10 +99,10 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     if need < 0:
         raise NativeError("expert_mlp: invalid shape")
     ws = torch.empty(need or 16, dtype=torch.uint8, device=device)
-    ldg, ldd = h, inter
+    ldg, ldd, gs, ds = h, inter, None, None
     if int8:
         ldg, ldd = gate_up.row_stride, down.row_stride
-        gs, ds = gs.data_ptr(), ds.data_ptr()
+        gs, ds = gate_up.scales.data_ptr(), down.scales.data_ptr()
     with on_device(device):
         check(native.mi355x_expert_mlp(
             xp, ldx, ids.data_ptr(), weights.data_ptr(), gp, ldg, gs, dp, ldd, ds, out.data_ptr(),

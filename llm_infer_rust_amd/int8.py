@@ -7,11 +7,12 @@
   exact int32 sums and one rounding, optionally with the SiLU x mul of a gate_up projection.
 
 The counterpart of ``src/layers/linear.rs:5-7`` for weights held in 8 bits; the reference itself
-has 16-bit weights only. Inference only: a call whose gradient would be wanted is refused.
+has 16-bit weights only. Inference only: a call whose derivative would be wanted is refused.
 """
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from ._native import NativeError, check, device_cus, lib, on_device, stream_of
 
@@ -25,6 +26,18 @@ def _padded(k: int, to: int) -> int:
 
 
 def _refuse_grad(what: str, *tensors: torch.Tensor | None) -> None:
+    """Refuse a call that torch would have to record: operands that want a gradient or carry a
+    tangent, operands of a function transform (vmap, grad, jvp), tracing."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NativeError(f"{what}: no tangent is carried")
+    if torch._C._functorch.maybe_current_level() is not None:
+        for t in tensors:
+            if t is not None and torch._C._functorch.is_functorch_wrapped_tensor(t):
+                raise NativeError(f"{what}: not for torch.func's transforms")
+    if torch._C._get_tracing_state() is not None:
+        raise NativeError(f"{what}: a trace would not hold the call")
     if not torch.is_grad_enabled():
         return
     for t in tensors:

@@ -49,3 +49,40 @@ def test_gradients(gpu):
             pytest.fail(name)
         with torch.no_grad():
             call()
+
+
+def test_tangents(gpu):
+    import torch.autograd.forward_ad as fwad
+    with fwad.dual_level():
+        for name, call in calls(gpu, lambda t: fwad.make_dual(t, torch.ones_like(t))):
+            with pytest.raises(NativeError):
+                call()
+                pytest.fail(name)
+        for _, call in calls(gpu, lambda t: t):  # no operand carries one
+            call()
+
+
+def test_transforms(gpu):
+    x, logits, gu, dn = operands(gpu)
+    w, ids = experts.route_experts(logits, 2)
+    one = int8.Int8Weight.quantize(gu[0])
+    for f, arg in ((lambda t: int8.linear_int8(t, one), x), (lambda t: int8.quantize_rows(t)[1], x),
+                   (lambda t: experts.route_experts(t, 2)[0], logits),
+                   (lambda t: experts.expert_mlp(t, ids, w, gu, dn), x)):
+        for transformed in (lambda a: torch.vmap(f)(torch.stack([a, a])),
+                            lambda a: torch.func.jvp(f, (a,), (torch.ones_like(a),)),
+                            lambda a: torch.func.vjp(f, a)):
+            with pytest.raises(NativeError):
+                transformed(arg)
+        # operands that the transform does not touch
+        got = torch.vmap(lambda s: s * f(arg).float())(torch.ones(2, device=gpu))
+        assert torch.equal(got[1], f(arg).float())
+
+
+def test_tracing(gpu):
+    x, logits, gu, _ = operands(gpu)
+    one = int8.Int8Weight.quantize(gu[0])
+    for f, arg in ((lambda t: int8.linear_int8(t, one), x),
+                   (lambda t: experts.route_experts(t, 2)[0], logits)):
+        with pytest.raises(NativeError):
+            torch.jit.trace(f, (arg,), check_trace=False)
