@@ -181,6 +181,7 @@ class _Ahead:
 
 class Engine:
     def __init__(self, model: Qwen3Model, config: EngineConfig | None = None):
+        model.check_runnable()
         self.model = model
         self.cfg = config or EngineConfig()
         cfg, mcfg = self.cfg, model.cfg

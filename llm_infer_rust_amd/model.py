@@ -52,7 +52,8 @@ class Qwen3Config:
     rms_norm_eps: float = 1e-6
     tie_word_embeddings: bool = False
     # Experts of every layer's MLP (0: a dense MLP of intermediate_size), how many of them a token
-    # is routed to, their width, and whether the chosen weights are normalised to sum to 1.
+    # is routed to, their width, and whether the chosen weights are normalised to sum to 1. Experts
+    # in 16 bits need hidden_size and their width to be multiples of 8, those in 8 bits do not.
     num_experts: int = 0
     num_experts_per_tok: int = 0
     moe_intermediate_size: int = 0
@@ -217,6 +218,17 @@ class Qwen3Model:
         finally:
             self._capturing = False
 
+    def check_runnable(self) -> None:
+        """Raise for weights that no forward takes: 16-bit experts of a width that is no multiple of
+        8 (``quantize_int8`` makes them runnable)."""
+        cfg = self.cfg
+        if not cfg.num_experts or (cfg.hidden_size | cfg.moe_intermediate_size) % 8 == 0:
+            return
+        if any(not isinstance(m, Int8Weight) for layer in self.layers
+               for m in (layer.gate_up_proj, layer.down_proj)):
+            raise ModelError("16-bit experts need hidden_size and moe_intermediate_size to be "
+                             "multiples of 8")
+
     def bind_kv_cache(self, pool, reserved_slot: int = 0) -> None:
         """Bind every layer to its views of a ``KVCachePool`` (page 0 reserved)."""
         if pool.layout.num_layers != self.cfg.num_layers:
@@ -241,6 +253,7 @@ class Qwen3Model:
         cfg = self.cfg
         if input_ids.dim() != 1 or positions.shape != input_ids.shape:
             raise ModelError("input_ids and positions must have identical lengths")
+        self.check_runnable()
         if not self._capturing and torch.cuda.is_current_stream_capturing():
             self._captured_by_caller = True
         t = input_ids.size(0)
