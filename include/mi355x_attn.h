@@ -353,6 +353,12 @@ const char* mi355x_quantize_rows(const void* x, int64_t ldx, void* values, int64
  * invalid shape. Host-only. */
 int64_t mi355x_linear_int8_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t cus);
 
+/* How mi355x_linear_int8 computes such a product: plan[0] 0 vector math (a row or two), 1 up to 16
+ * rows against the weight stream, 2 tiles; plan[1] the tile, 0 64 x 64, 1 128 x 128 one a compute
+ * unit, 2 128 x 128 two a compute unit, 3 256 x 128, 4 256 x 256; plan[2] the parts of K. False
+ * for an empty or invalid shape. Host-only. */
+bool mi355x_linear_int8_plan(int64_t M, int64_t N, int64_t K, int32_t cus, int32_t* plan);
+
 /* out[m, n] = round(sx[m] w_scales[n] sum_k q[m, k] w[n, k]) with (q, sx) = mi355x_quantize_rows
  * of x [M, K] (dtype 0 bf16, 1 fp16; out has the same) and w int8 [N, ldw]; the sum is exact in
  * int32. out must not overlap x. With silu_mul, w is a gate_up weight (gate rows, then up rows, N
@@ -385,6 +391,13 @@ const char* mi355x_route_experts(const void* logits, int64_t ld, void* weights, 
 int64_t mi355x_expert_mlp_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts,
                                           int64_t hidden, int64_t inter, int64_t ldx, bool int8,
                                           int32_t cus);
+
+/* How mi355x_expert_mlp computes (the first pass of) such a call: plan[0] 1 where the slots run one
+ * by one, else 0 and plan[1] the gate_up tile, plan[2] the down tile (as for
+ * mi355x_linear_int8_plan: 0, 2 or 4), plan[3] the parts of the down product's K. False for an
+ * empty or invalid shape. Host-only. */
+bool mi355x_expert_mlp_plan(int64_t tokens, int64_t top_k, int64_t experts, int64_t hidden,
+                            int64_t inter, int64_t ldx, bool int8, int32_t cus, int32_t* plan);
 
 /* out[t] = sum_s weights[t, s] down[e] . (silu(g) * u), (g; u) = gate_up[e] . x[t], e = ids[t, s].
  * x [tokens, hidden] and out of dtype 0 bf16 or 1 fp16, ids int32 and weights fp32

@@ -107,6 +107,7 @@ SIGNATURES: dict[str, tuple] = {
     "mi355x_quantize_rows": (c_char_p, [c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_i64,
                                         c_int, c_void_p]),
     "mi355x_linear_int8_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64, c_i32]),
+    "mi355x_linear_int8_plan": (c_bool, [c_i64, c_i64, c_i64, c_i32, c_void_p]),
     "mi355x_linear_int8": (c_char_p, [c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_i64,
                                       c_i64, c_i64, c_i64, c_bool, c_void_p, c_i64, c_i32,
                                       c_i64, c_void_p]),
@@ -114,6 +115,8 @@ SIGNATURES: dict[str, tuple] = {
                                         c_bool, c_int, c_void_p]),
     "mi355x_expert_mlp_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
                                                   c_bool, c_i32]),
+    "mi355x_expert_mlp_plan": (c_bool, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_bool, c_i32,
+                                        c_void_p]),
     "mi355x_expert_mlp": (c_char_p, [c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_i64,
                                      c_void_p, c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_i64,
                                      c_i64, c_i64, c_i64, c_i64, c_void_p, c_i64, c_i32,

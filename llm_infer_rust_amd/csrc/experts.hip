@@ -731,6 +731,21 @@ extern "C" int64_t mi355x_expert_mlp_workspace_bytes(int64_t tokens, int64_t top
       .bytes;
 }
 
+extern "C" bool mi355x_expert_mlp_plan(int64_t tokens, int64_t top_k, int64_t experts,
+                                       int64_t hidden, int64_t inter, int64_t ldx, bool int8,
+                                       int32_t cus, int32_t* plan) {
+  if (!plan || tokens == 0 ||
+      mi355x_expert_mlp_workspace_bytes(tokens, top_k, experts, hidden, inter, ldx, int8, cus) < 0)
+    return false;
+  const ExpertWorkspace w =
+      expert_workspace(tokens, top_k, experts, hidden, inter, int8, ldx * 2, cus > 0 ? cus : 256);
+  plan[0] = one_by_one(w.tokens, top_k, experts, hidden, inter, int8);
+  plan[1] = static_cast<int32_t>(w.gate_up.tile);
+  plan[2] = static_cast<int32_t>(w.down.tile);
+  plan[3] = w.down.splits;
+  return true;
+}
+
 extern "C" const char* mi355x_expert_mlp(const void* x, int64_t ldx, const int32_t* ids,
                                          const float* weights, const void* gate_up,
                                          int64_t ld_gate_up, const float* gate_up_scales,

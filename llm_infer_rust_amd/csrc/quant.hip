@@ -223,6 +223,16 @@ extern "C" int64_t mi355x_linear_int8_workspace_bytes(int64_t M, int64_t N, int6
   return M == 0 ? 0 : int8_workspace(M, N, K, int8_plan(M, N, K, cus > 0 ? cus : 256)).bytes;
 }
 
+extern "C" bool mi355x_linear_int8_plan(int64_t M, int64_t N, int64_t K, int32_t cus,
+                                        int32_t* plan) {
+  if (!plan || M == 0 || mi355x_linear_int8_workspace_bytes(M, N, K, cus) < 0) return false;
+  const Int8Plan p = int8_plan(M, N, K, cus > 0 ? cus : 256);
+  plan[0] = static_cast<int32_t>(p.kind);
+  plan[1] = static_cast<int32_t>(p.tile);
+  plan[2] = p.splits;
+  return true;
+}
+
 extern "C" const char* mi355x_linear_int8(const void* x, int64_t ldx, const void* w, int64_t ldw,
                                           const float* w_scales, void* out, int64_t ldo, int64_t M,
                                           int64_t N, int64_t K, bool silu_mul, void* workspace,

@@ -90,6 +90,7 @@ unsafe extern "C" {
         scales: *mut c_void, rows: i64, width: i64, dtype: c_int,
         stream: *mut c_void) -> *const c_char;
     pub fn mi355x_linear_int8_workspace_bytes(m: i64, n: i64, k: i64, cus: i32) -> i64;
+    pub fn mi355x_linear_int8_plan(m: i64, n: i64, k: i64, cus: i32, plan: *mut i32) -> bool;
     pub fn mi355x_linear_int8(x: *const c_void, ldx: i64, w: *const c_void, ldw: i64,
         w_scales: *const f32, out: *mut c_void, ldo: i64, m: i64, n: i64, k: i64,
         silu_mul: bool, workspace: *mut c_void, workspace_bytes: i64, cus: i32, dtype: i64,
@@ -99,6 +100,8 @@ unsafe extern "C" {
         stream: *mut c_void) -> *const c_char;
     pub fn mi355x_expert_mlp_workspace_bytes(tokens: i64, top_k: i64, experts: i64, hidden: i64,
         inter: i64, ldx: i64, int8: bool, cus: i32) -> i64;
+    pub fn mi355x_expert_mlp_plan(tokens: i64, top_k: i64, experts: i64, hidden: i64, inter: i64,
+        ldx: i64, int8: bool, cus: i32, plan: *mut i32) -> bool;
     pub fn mi355x_expert_mlp(x: *const c_void, ldx: i64, ids: *const i32, weights: *const f32,
         gate_up: *const c_void, ld_gate_up: i64, gate_up_scales: *const f32,
         down: *const c_void, ld_down: i64, down_scales: *const f32, out: *mut c_void, ldo: i64,
