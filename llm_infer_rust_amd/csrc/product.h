@@ -5,15 +5,15 @@
 // Both operands are handled as rows of bytes. An MFMA operand is 16 bytes a lane in every type
 // here (8 bf16 / fp16 elements, 16 int8 ones) and a step of the K loop is 128 bytes of a row, so
 // one core serves bf16, fp16 and int8; only the instruction and the accumulator differ:
-//   bf16 / fp16  32x32x16 and 16x16x32, fp32 accumulators
+//   bf16 / fp16  32x32x16, fp32 accumulators
 //   int8         32x32x32 and 16x16x64, int32 accumulators (exact up to K = 131,072)
 //
 // Three kernels:
 //   * product_tile: a BM x BN tile, x and w rows copied to an LDS ring of 128-byte rows
 //     (global_load_lds_dwordx4, 16-byte chunks XOR-swizzled);
 //   * product_large: the same for many rows, 256 x 256 on a written-out schedule;
-//   * product_rows: up to 16 rows of x, weights from global memory straight into MFMA operands, the
-//     waves of a workgroup sharing K. For few rows, where the weight bytes are all that counts.
+//   * product_rows (int8): up to 16 rows of x, weights from global memory straight into MFMA operands,
+//     the waves of a workgroup sharing K. For few rows, where the weight bytes are all that counts.
 #pragma once
 
 #include <algorithm>
@@ -43,7 +43,7 @@ struct ProductArgs {
   void* out;
   const float* x_scales;      // int8: one a row of x
   const float* w_scales;      // int8: [E][w_rows]
-  const int32_t* order;       // grouped: slot (token * top_k + s) of every row; null: the row itself
+  const int32_t* order;       // grouped: slot (token * top_k + s) of every row; null (product_vec): the row
   const int32_t* ids;         // with a null tile list (one slot a tile): expert of every slot
   const int4* tiles;          // grouped: {expert, first row, end row, 0} per row tile
   const int32_t* tile_count;  // grouped: tiles in the list
@@ -66,14 +66,12 @@ struct ProductArgs {
 typedef __bf16 prod_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 prod_f16x8 __attribute__((ext_vector_type(8)));
 typedef int prod_i32x4 __attribute__((ext_vector_type(4)));
-typedef float prod_f32x4 __attribute__((ext_vector_type(4)));
 typedef float prod_f32x16 __attribute__((ext_vector_type(16)));
 typedef int prod_i32x16 __attribute__((ext_vector_type(16)));
 
 template <int IN>
 struct Mma {
   using Acc16 = std::conditional_t<IN == kInt8, prod_i32x16, prod_f32x16>;  // 32 x 32 block
-  using Acc4 = std::conditional_t<IN == kInt8, prod_i32x4, prod_f32x4>;     // 16 x 16 block
   using Scalar = std::conditional_t<IN == kInt8, int, float>;
 
   __device__ __forceinline__ static Acc16 block32(const uint4& a, const uint4& b, Acc16 c) {
@@ -88,19 +86,13 @@ struct Mma {
       return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(prod_i32x4, a),
                                                    __builtin_bit_cast(prod_i32x4, b), c, 0, 0, 0);
   }
-  __device__ __forceinline__ static Acc4 block16(const uint4& a, const uint4& b, Acc4 c) {
-    if constexpr (IN == kBf16)
-      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(prod_bf16x8, a),
-                                                     __builtin_bit_cast(prod_bf16x8, b), c, 0, 0,
-                                                     0);
-    else if constexpr (IN == kFp16)
-      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(prod_f16x8, a),
-                                                    __builtin_bit_cast(prod_f16x8, b), c, 0, 0, 0);
-    else
-      return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(prod_i32x4, a),
-                                                   __builtin_bit_cast(prod_i32x4, b), c, 0, 0, 0);
-  }
 };
+
+// A 16 x 16 block in 8 bits.
+__device__ __forceinline__ prod_i32x4 block16_int8(const uint4& a, const uint4& b, prod_i32x4 c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(prod_i32x4, a),
+                                               __builtin_bit_cast(prod_i32x4, b), c, 0, 0, 0);
+}
 
 // silu(g) * u, with the hardware reciprocal (1 ulp; an IEEE quotient doubles the epilogue of a large
 // gate_up tile). exp(-g) overflows to +inf for g below about -88: g * 0 = -0, the limit.
@@ -144,7 +136,7 @@ __device__ __forceinline__ RowOut row_out(const ProductArgs& a, int row) {
   if constexpr (MODE == kDense) {
     if constexpr (IN == kInt8) r.scale = a.x_scales[row];
   } else {
-    const int slot = a.order ? a.order[row] : row;
+    const int slot = a.order[row];
     if constexpr (MODE == kGateUp) {
       if constexpr (IN == kInt8) r.scale = a.x_scales[slot / a.top_k];
     } else {
@@ -760,7 +752,7 @@ __device__ __forceinline__ void large_tile(const ProductArgs& a, const RowTile& 
   const int row = min(t.begin + r, t.end - 1);
   int slot = row;
   float row_scale = 1.f, weight = 1.f, column_scale = 1.f;
-  if constexpr (MODE != kDense) slot = a.order ? a.order[row] : row;
+  if constexpr (MODE != kDense) slot = a.order[row];
   if constexpr (MODE == kDown) weight = a.row_weights[row];
   if constexpr (IN == kInt8 && MODE != kGateUp) row_scale = a.x_scales[row];
   if constexpr (IN == kInt8) {
@@ -805,13 +797,11 @@ __global__ __launch_bounds__(64 * NW, 1) void product_large(ProductArgs a) {
 // in LDS. A lane's operand rows are lane % 16; of a 128-byte step it holds bytes 32 g .. 32 g + 31,
 // g = lane / 16, as two operands: K is summed in another order than it is stored, the same one in
 // both operands, so whole 128-byte lines are read.
-template <int IN, int OT, bool SILU, int NB, int DEPTH>
+template <int OT, bool SILU, int NB, int DEPTH>
 __global__ __launch_bounds__(256) void product_rows(ProductArgs a) {
   static_assert(!SILU || NB == 2, "a gate and an up block");
   constexpr int kOut = SILU ? 16 : 16 * NB;
-  using M = Mma<IN>;
-  using Acc = typename M::Acc4;
-  __shared__ Acc sums[NB][4][64];
+  __shared__ prod_i32x4 sums[NB][4][64];
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -857,7 +847,7 @@ __global__ __launch_bounds__(256) void product_rows(ProductArgs a) {
       }
     }
   };
-  Acc acc[NB];
+  prod_i32x4 acc[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -873,7 +863,7 @@ __global__ __launch_bounds__(256) void product_rows(ProductArgs a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int b = 0; b < NB; ++b) acc[b] = M::block16(wf[d][b][h], xf[d][h], acc[b]);
+        for (int b = 0; b < NB; ++b) acc[b] = block16_int8(wf[d][b][h], xf[d][h], acc[b]);
       if (step + d + DEPTH < last) load(step + d + DEPTH, d);
     }
   }
@@ -886,18 +876,17 @@ __global__ __launch_bounds__(256) void product_rows(ProductArgs a) {
   if (wave >= (SILU ? 1 : NB)) return;
   const int row = t.begin + r;
   if (row >= t.end) return;
-  const RowOut ro = row_out<IN, kDense>(a, row);
-  const float* w_scales = IN == kInt8 ? a.w_scales : nullptr;
-  auto total = [&](int b, typename M::Scalar(&v)[4]) {
+  const RowOut ro = row_out<kInt8, kDense>(a, row);
+  auto total = [&](int b, int(&v)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       v[e] = (sums[b][0][lane][e] + sums[b][1][lane][e]) +
              (sums[b][2][lane][e] + sums[b][3][lane][e]);
   };
-  typename M::Scalar v[4], u[4] = {};
+  int v[4], u[4] = {};
   total(SILU ? 0 : wave, v);
   if constexpr (SILU) total(NB - 1, u);
-  finish4<IN, OT, kDense, SILU>(a, ro, n0 + (SILU ? 0 : 16 * wave) + 4 * g, w_scales, v, u);
+  finish4<kInt8, OT, kDense, SILU>(a, ro, n0 + (SILU ? 0 : 16 * wave) + 4 * g, a.w_scales, v, u);
 }
 
 // ---------------------------------------------------------------------------- the choice of tiles

@@ -162,7 +162,7 @@ const char* launch_int8(const ProductArgs& base, const Int8Plan& p, int* sums, h
     const int bn = SILU ? 16 : 32;
     a.tiles_m = 1;
     a.tiles_n = (a.columns + bn - 1) / bn;
-    product_rows<kInt8, OT, SILU, 2, 4>
+    product_rows<OT, SILU, 2, 4>
         <<<dim3(static_cast<uint32_t>((a.tiles_n + 7) / 8 * 8)), 256, 0, s>>>(a);
   } else if (p.splits == 1) {
     launch_int8_tiles<OT, kDense, SILU>(a, p.tile, s);
