@@ -466,6 +466,15 @@ ExpertWorkspace expert_workspace(int64_t tokens, int64_t top_k, int64_t experts,
   return w;
 }
 
+// Workgroups of a grouped product over `columns` columns in tiles of `bn` of them: the row tiles that
+// so many slots need at most (every full one and one more an expert) by the column tiles.
+int64_t grouped_grid(Tile tile, int64_t bn, int64_t slots, int64_t experts, int64_t columns,
+                     int64_t splits) {
+  const int64_t most =
+      slots / kTileShapes[static_cast<int>(tile)].bm + std::min(experts, slots);
+  return pad(most * ((columns + bn - 1) / bn) * splits, 8);
+}
+
 template <int IN, int OT, int MODE, bool SILU>
 void launch_product(const ProductArgs& base, Tile tile, int64_t slots, int64_t experts,
                     hipStream_t s) {
@@ -473,9 +482,8 @@ void launch_product(const ProductArgs& base, Tile tile, int64_t slots, int64_t e
   const TileShape& t = kTileShapes[static_cast<int>(tile)];
   const int bn = SILU ? t.bn / 2 : t.bn;
   a.tiles_n = (a.columns + bn - 1) / bn;
-  // Tiles that so many slots need at most: every full one and one more an expert.
-  const int64_t most = slots / t.bm + std::min(experts, slots);
-  const dim3 g(static_cast<uint32_t>(pad(most * a.tiles_n * a.splits, 8)));
+  const dim3 g(
+      static_cast<uint32_t>(grouped_grid(tile, bn, slots, experts, a.columns, a.splits)));
   switch (tile) {
     case Tile::k64: product_tile<IN, OT, MODE, SILU, 64, 64, 2, 2, 3><<<g, 256, 0, s>>>(a); break;
     case Tile::k128Two:
@@ -711,13 +719,20 @@ extern "C" const char* mi355x_route_experts(const void* logits, int64_t ld, void
   auto s = static_cast<hipStream_t>(stream);
   const int e = static_cast<int>(experts), k = static_cast<int>(top_k);
   auto* p = static_cast<float*>(weights);
-  if (dtype == 0)
-    launch_route<0>(logits, ld, p, ids, tokens, e, k, normalize, s);
-  else if (dtype == 1)
-    launch_route<1>(logits, ld, p, ids, tokens, e, k, normalize, s);
-  else
-    launch_route<2>(logits, ld, p, ids, tokens, e, k, normalize, s);
-  return launch_status("route_kernel");
+  for (int64_t t = 0; t < tokens; t += kMaxLaunchRows) {
+    const int64_t n = std::min(kMaxLaunchRows, tokens - t);
+    const auto* rows = static_cast<const uint8_t*>(logits) + t * ld * (dtype == 2 ? 4 : 2);
+    float* w = p + t * top_k;
+    int32_t* chosen = ids + t * top_k;
+    if (dtype == 0)
+      launch_route<0>(rows, ld, w, chosen, n, e, k, normalize, s);
+    else if (dtype == 1)
+      launch_route<1>(rows, ld, w, chosen, n, e, k, normalize, s);
+    else
+      launch_route<2>(rows, ld, w, chosen, n, e, k, normalize, s);
+    if (const char* err = launch_status("route_kernel")) return err;
+  }
+  return nullptr;
 }
 
 extern "C" int64_t mi355x_expert_mlp_workspace_bytes(int64_t tokens, int64_t top_k, int64_t experts,
@@ -777,6 +792,14 @@ extern "C" const char* mi355x_expert_mlp(const void* x, int64_t ldx, const int32
   const ExpertWorkspace w =
       expert_workspace(tokens, top_k, experts, hidden, inter, int8, ldx * 2, cus > 0 ? cus : 256);
   if (workspace_bytes < w.bytes) return set_error("mi355x_expert_mlp: workspace too small");
+  const auto threads = [&](Tile tile, bool silu, int64_t columns, int64_t splits) {
+    const int bn = kTileShapes[static_cast<int>(tile)].bn / (silu ? 2 : 1);
+    return grouped_grid(tile, bn, w.tokens * top_k, experts, columns, splits) *
+           (tile == Tile::k64 ? 256 : 512);
+  };
+  if (threads(w.gate_up.tile, true, inter, 1) > kMaxGridThreads ||
+      threads(w.down.tile, false, hidden, w.down.splits) > kMaxGridThreads)
+    return set_error("mi355x_expert_mlp: grid too large");
   auto s = static_cast<hipStream_t>(stream);
   for (int64_t t = 0; t < tokens; t += w.tokens) {
     ExpertCall c{};

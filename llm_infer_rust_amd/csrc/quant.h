@@ -99,6 +99,11 @@ struct RowsToQuantize {
   int32_t width, chunks;      // chunks of 16 columns to write, zeros past the width
 };
 
+// A grid has fewer than 2^32 threads: of a larger one a part is launched, without an error.
+constexpr int64_t kMaxGridThreads = (int64_t(1) << 32) - 1;
+// Rows that one launch takes where up to 256 threads stand for each.
+constexpr int64_t kMaxLaunchRows = int64_t(1) << 23;
+
 inline RowsToQuantize rows_to_quantize(const void* x, int64_t stride, void* values, int64_t ldv,
                                        float* scales, int64_t rows, int64_t width,
                                        int64_t padded) {

@@ -186,14 +186,19 @@ const char* launch_int8(const ProductArgs& base, const Int8Plan& p, int* sums, h
 const char* run_quantize_rows(const void* x, int64_t stride, void* values, int64_t ldv,
                               float* scales, int64_t rows, int64_t width, int64_t padded, int dtype,
                               hipStream_t s) {
-  const RowsToQuantize q = rows_to_quantize(x, stride, values, ldv, scales, rows, width, padded);
-  if (dtype == 0)
-    launch_quantize<0>(q, s);
-  else if (dtype == 1)
-    launch_quantize<1>(q, s);
-  else
-    launch_quantize<2>(q, s);
-  return launch_status("quantize_rows");
+  for (int64_t r = 0; r < rows; r += kMaxLaunchRows) {
+    const RowsToQuantize q = rows_to_quantize(
+        static_cast<const uint8_t*>(x) + r * stride, stride, static_cast<uint8_t*>(values) + r * ldv,
+        ldv, scales + r, std::min(kMaxLaunchRows, rows - r), width, padded);
+    if (dtype == 0)
+      launch_quantize<0>(q, s);
+    else if (dtype == 1)
+      launch_quantize<1>(q, s);
+    else
+      launch_quantize<2>(q, s);
+    if (const char* e = launch_status("quantize_rows")) return e;
+  }
+  return nullptr;
 }
 
 }  // namespace mi355x
@@ -254,8 +259,12 @@ extern "C" const char* mi355x_linear_int8(const void* x, int64_t ldx, const void
       !aligned(workspace, 16))
     return set_error("mi355x_linear_int8: misaligned operand");
   if (workspace_bytes < ws.bytes) return set_error("mi355x_linear_int8: workspace too small");
-  // More row and column tiles than a grid holds (16 x 16 is the smallest tile).
-  if ((M + 15) / 16 * ((columns + 15) / 16) >= (int64_t(1) << 30))
+  const TileShape& tile = kTileShapes[static_cast<int>(plan.tile)];
+  const int64_t bn = silu_mul && plan.splits == 1 ? tile.bn / 2 : tile.bn;
+  const int64_t across = plan.splits == 1 ? columns : N;
+  if (plan.kind == Int8Plan::kTiles &&
+      ((M + tile.bm - 1) / tile.bm * ((across + bn - 1) / bn) * plan.splits + 8) * 512 >
+          kMaxGridThreads)
     return set_error("mi355x_linear_int8: grid too large");
   auto s = static_cast<hipStream_t>(stream);
   ProductArgs a{};
