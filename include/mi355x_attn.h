@@ -407,13 +407,13 @@ bool mi355x_expert_mlp_plan(int64_t tokens, int64_t top_k, int64_t experts, int6
  * twice in a row.
  *
  * Scales NULL: weights of x's type. hidden, inter and ldx are multiples of 8 and rows are 16-byte
- * aligned. Sums in fp32; silu(g) * u is rounded to x's type (kept in fp32 where a few slots run one
- * by one).
+ * aligned. Sums in fp32; silu(g) * u is rounded to x's type (above 65,504 in fp16 it is inf), but
+ * kept in fp32 where a few slots run one by one (mi355x_expert_mlp_plan).
  * Scales given (fp32 [experts, 2 inter] and [experts, hidden]): int8 weights. x is quantised once
  * a token, silu(g) * u (kept in fp32) once a slot, both as mi355x_quantize_rows does; any sizes and
  * x strides, weight rows as for mi355x_linear_int8.
  * Slot outputs are fp32 up to the sum over a token's slots, which is rounded once.
- * Nothing is read back to the host. An expert's weights are less than 4 GiB. Calls that overlap
+ * out must not overlap any operand. Nothing is read back to the host. An expert's weights are less than 4 GiB. Calls that overlap
  * need workspaces of their own. */
 const char* mi355x_expert_mlp(const void* x, int64_t ldx, const int32_t* ids,
                               const float* weights, const void* gate_up, int64_t ld_gate_up,

@@ -261,8 +261,9 @@ __global__ __launch_bounds__(kGroupThreads) void place_and_quantize(SlotsToPlace
 
 // ---------------------------------------------------------------------------- the sum over slots
 // out[t] = sum of y[t * top_k + s] (fp32) over the slots that take part and the parts of K, in
-// fp32 and in this order. A thread takes 4 H columns. Bound by memory where there are many tokens,
-// else by latency: H 1 and workgroups of a wave spread over the chip.
+// fp32 and in this order. A thread takes 4 H columns. Bound by memory where there are many tokens
+// (8,192 of 8 slots and 2,048 columns: 570 MB in 111 us, 5.1 TB/s), else by latency: H 1 and
+// workgroups of a wave spread over the chip (40 tokens 4.0 to 4.8 us).
 template <int DT, int H, int THREADS, bool PARTS>
 __global__ __launch_bounds__(THREADS) void sum_slots(const float* __restrict__ y, int64_t ldy,
                                                  const int32_t* __restrict__ ids,
@@ -627,7 +628,12 @@ const char* expert_pass(const ExpertCall& c, const ExpertWorkspace& w, uint8_t* 
   a.top_k = static_cast<int32_t>(c.top_k);
   a.experts = static_cast<int32_t>(c.experts);
   a.splits = 1;
-  // gate_up with SiLU x mul into act, one row a slot
+  // gate_up with SiLU x mul into act, one row a slot. In 16 bits act is rounded to x's type, as it is
+  // the operand of the next product's matrix instructions: one more independent rounding beside the
+  // output's (rms error against 64 bits 0.0023 for 0.0017 in bf16, 0.00029 for 0.00021 in fp16). Two
+  // operands for its high and low half would double that product's instructions, which already take
+  // a third of an 8,192-token layer. Past fp16's range act is inf, as in the dense MLP. In 8 bits it
+  // stays fp32 for the row pass behind it.
   if (kQuant) {
     a.x = ws + w.xq;
     a.x_stride = gate_up_k;

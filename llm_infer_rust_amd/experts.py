@@ -55,7 +55,9 @@ def expert_mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     ``route_experts`` gives them (an id outside ``[0, E)`` adds nothing: pad rows, experts held
     elsewhere); ``gate_up`` ``[E, 2 I, H]`` (gate rows, then up rows) and ``down`` ``[E, H, I]``,
     both of x's type (H, I and x's row stride multiples of 8, 16-byte aligned) or both
-    ``Int8Weight`` (any sizes): then x is quantised a token and ``silu(g) * u`` a slot. ``out`` may
+    ``Int8Weight`` (any sizes): then x is quantised a token and ``silu(g) * u`` a slot. Sums are fp32.
+    With 16-bit weights ``silu(g) * u`` is rounded to x's type between the products, as in a dense
+    MLP (in fp16 inf above 65,504); a few slots, which run one by one, keep it in fp32. ``out`` may
     be given; it must not share memory with ``x``."""
     t, h, ldx = _rows(x, "expert_mlp")
     dtype, device = x.dtype, x.device

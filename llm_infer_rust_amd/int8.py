@@ -153,7 +153,7 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = 
     """``x @ weight.T`` in 8-bit integers: ``x`` ``[T, K]`` bf16 or fp16 is quantised a row, the int32
     sums are exact, ``out`` ``[T, N]`` is rounded once. ``silu_mul``: ``weight`` is a gate_up
     projection (gate rows, then up rows) and the result is ``silu(gate) * up`` ``[T, N / 2]``,
-    rounded once. Rows may have any stride and alignment; ``out`` may be
+    rounded once. Rows that do not overlap may have any stride and alignment; ``out`` may be
     given and must not share memory with ``x``. A row with an inf or a NaN comes out NaN."""
     t, k, ldx = _rows(x, "linear_int8")
     dt = _ROW_DTYPES.get(x.dtype)

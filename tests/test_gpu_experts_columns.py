@@ -96,3 +96,22 @@ def test_small_columns_beside_large_ones_int8(gpu, t, e, k, h, i):
     out, bound = bounds8(x, ids, w, gu, dn)
     err = (experts.expert_mlp(x, ids, w, gu, dn).double() - out).abs()
     assert bool((err <= bound).all()), float((err / bound).max())
+
+
+def test_fp16_activations_past_the_range(gpu):
+    """Grouped, silu(g) u above 65,504 is inf in fp16 and its token's result not finite, and no other
+    token's; alone the token keeps it in fp32."""
+    x, ids, w, gu, _ = problem(40, 4, 2, 128, 64, torch.float16, gpu)
+    dn = torch.full((4, 128, 64), 2.0 ** -6, dtype=torch.float16, device=gpu)
+    clean = experts.expert_mlp(x, ids, w, gu, dn)
+    x[7] *= 400.0
+    act = glu(x[7].double() @ gu[int(ids[7, 0])].double().T)
+    assert float(act.abs().max()) > 70000.0
+    got = experts.expert_mlp(x, ids, w, gu, dn)
+    rest = [t for t in range(40) if t != 7]
+    assert not bool(got[7].isfinite().any()) and torch.equal(got[rest], clean[rest])
+    one = (x[7:8], ids[7:8].contiguous(), w[7:8].contiguous(), gu, dn)
+    out, bound = bounds16(*one)
+    assert float(out.abs().max()) < 65504.0
+    err = (experts.expert_mlp(*one).double() - out).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
