@@ -11,6 +11,8 @@ has 16-bit weights only. Inference only: a call whose derivative would be wanted
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd import forward_ad
 
@@ -19,6 +21,12 @@ from ._native import NativeError, check, device_cus, lib, on_device, stream_of
 _ROW_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_K = 131072  # 127 * 127 * K stays inside int32
 _STEP = 128     # bytes of K a product takes at once
+
+# Looked up once: every call asks (0.1 us of 8).
+_transform_level = torch._C._functorch.maybe_current_level
+_of_transform = torch._C._functorch.is_functorch_wrapped_tensor
+_is_tracing = torch._C._is_tracing
+_is_grad_enabled = torch.is_grad_enabled
 
 
 def _padded(k: int, to: int) -> int:
@@ -32,13 +40,13 @@ def _refuse_grad(what: str, *tensors: torch.Tensor | None) -> None:
         for t in tensors:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 raise NativeError(f"{what}: no tangent is carried")
-    if torch._C._functorch.maybe_current_level() is not None:
+    if _transform_level() is not None:
         for t in tensors:
-            if t is not None and torch._C._functorch.is_functorch_wrapped_tensor(t):
+            if t is not None and _of_transform(t):
                 raise NativeError(f"{what}: not for torch.func's transforms")
-    if torch._C._get_tracing_state() is not None:
+    if _is_tracing():
         raise NativeError(f"{what}: a trace would not hold the call")
-    if not torch.is_grad_enabled():
+    if not _is_grad_enabled():
         return
     for t in tensors:
         if t is not None and t.requires_grad:
@@ -148,6 +156,13 @@ class Int8Weight:
         return (self.values.float() * self.scales[..., None]).to(dtype)
 
 
+@functools.lru_cache(maxsize=4096)
+def _linear_workspace(t: int, n: int, k: int, cus: int) -> int:
+    """Workspace bytes of a product, -1 for an invalid shape: a function of the sizes alone, kept as
+    the question costs 0.6 us of a one-row call's 8."""
+    return lib().mi355x_linear_int8_workspace_bytes(t, n, k, cus)
+
+
 def linear_int8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = None,
                 silu_mul: bool = False) -> torch.Tensor:
     """``x @ weight.T`` in 8-bit integers: ``x`` ``[T, K]`` bf16 or fp16 is quantised a row, the int32
@@ -171,13 +186,12 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = 
     _refuse_grad("linear_int8", x, scales, out)
     out, ldo = _output(out, x, n // 2 if silu_mul else n, "linear_int8")
     cus = device_cus(device)
-    native = lib()
-    need = native.mi355x_linear_int8_workspace_bytes(t, n, k, cus)
+    need = _linear_workspace(t, n, k, cus)
     if need < 0:
         raise NativeError("linear_int8: invalid shape")
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     with on_device(device):
-        check(native.mi355x_linear_int8(
+        check(lib().mi355x_linear_int8(
             x.data_ptr(), ldx, values.data_ptr(), _padded(k, _STEP), scales.data_ptr(),
             out.data_ptr(), ldo, t, n, k, silu_mul, None if ws is None else ws.data_ptr(), need,
             cus, dt, stream_of(x)), "linear_int8")
