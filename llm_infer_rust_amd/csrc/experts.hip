@@ -385,7 +385,7 @@ float grouped_estimate(Tile tile, float count, float steps, float weight_bytes, 
 // of 256 rows: over 114 products of 4 to 132 experts and 8 to 1,637 rows each, int8 and bf16, the
 // choice costs 2.4% more than the best of the three every time. A product whose slot outputs are
 // summed afterwards may be cut along K as well, where its tiles leave CUs without one: the parts
-// are summed with the slots (down of 8 experts 1024 x 2816 at 77 tokens 17.0 us whole, 11.6 in two
+// are summed with the slots (down of 8 experts 1024 x 2816 at 77 tokens 17.0 us whole, 11.9 in two
 // parts).
 constexpr int64_t kManyValues = int64_t(1) << 22;  // slot outputs that fill the chip by themselves
 GroupedPlan choose_grouped(int64_t slots, int64_t experts, int64_t weight_rows, int64_t k_bytes,

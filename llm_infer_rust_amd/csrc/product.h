@@ -487,11 +487,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile(ProductArgs a) {
 // and as many 128-byte steps in flight as LDS holds. The schedule is written out: an MFMA, then one
 // of the next quarter step's operand reads or one of the copies into the buffer that the last
 // barrier freed, fixed by scheduling barriers.
-// Measured on the experts of an 8,192-token prefill
-// (65,536 rows in 128 groups): the copies alone take 335 us of gate_up's 440 (11 TB/s into LDS, 44%
-// of it from beyond L2), the MFMAs with operands in L1 320; down 247 and 184 of 275. Four waves of
-// 128 x 128 read LDS a third less but leave each SIMD idle at every wait (480 and 316 us); 64-byte
-// steps with 128 KiB in flight instead of 64 are no quicker (480 and 305), so it is not latency.
+// Measured on the experts of an 8,192-token prefill (65,536 rows in 128 groups): the copies alone take
+// 335 us of gate_up's 440 (11 TB/s into LDS, 44% of it from beyond L2), the MFMAs with operands in L1
+// 320; down 247 and 184 of 333, its fp32 outputs being half a gigabyte. Four waves of 128 x 128 read LDS
+// a third less but leave each SIMD idle at every wait (480 us for gate_up); 64-byte steps with 128 KiB
+// in flight instead of 64 are no quicker (480), so it is not latency.
 constexpr int kLargeN = 256;
 
 template <int BM>

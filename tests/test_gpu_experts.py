@@ -3,12 +3,12 @@
 Bounds. Routing: ids are exact (selection is on the logits themselves); the weights are two fp32
 exponentials and a quotient, 2^-20 relative. 16-bit experts: the products sum in fp32 (K 2^-24 of the
 sum of magnitudes), silu(g) u is rounded to x's type (half a step, eps / 2 of every term of the
-second product), and the sum over the slots (eps / 2). The weighted slot outputs are held as 16-bit
-mantissas under a power of two for every 32 columns: the largest of the 32 is at least 2^14 units, so
-half a unit is 2^-15 of it (a unit, 2^-14, for a value within half a unit of the top, which has
-no code of its own). 8-bit experts: integer sums are exact; silu(g) u differs by fp32 rounding from
-the 64-bit value and may fall on the other side of a rounding border, a step of its scale for one
-element a row.
+second product), and the sum over the slots (eps / 2). The weighted slot outputs are fp32; the bounds
+leave room for 16-bit mantissas under a power of two for every 32 columns (``block_errors``: half a
+unit, 2^-15 of the largest of the 32, or a unit for a value within half a unit of the top). Bounds of
+every column's own are in test_gpu_experts_columns.py. 8-bit experts: integer sums are exact;
+silu(g) u differs by fp32 rounding from the 64-bit value and may fall on the other side of a rounding
+border, a step of its scale for one element a row.
 """
 import pytest
 import torch
@@ -160,7 +160,7 @@ SHAPES = [
     (1, 8, 2, 64, 64), (1, 4, 4, 8, 8), (2, 16, 8, 136, 72), (3, 5, 1, 1000, 24),
     (16, 8, 2, 256, 128), (17, 128, 8, 128, 64), (40, 3, 2, 512, 200), (77, 8, 2, 264, 520),
     (200, 4, 2, 192, 320), (300, 7, 3, 328, 264), (1200, 5, 2, 136, 136),
-    (40, 6, 2, 104, 2056), (90, 2, 2, 72, 4104),  # down cut along K, in two parts and in four
+    (40, 6, 2, 104, 2056), (90, 2, 2, 72, 4104),  # down cut along K, in four parts (8 bits: two and four)
 ]
 
 
@@ -172,9 +172,9 @@ def test_expert_mlp(gpu, dtype, t, e, k, h, i):
     check16(got, *p, gpu)
 
 
-# The larger tiles, chosen by size: 128 x 128 for both products, 256 x 256 (groups of rows that end in a
-# half tile and in a whole one) for either, with K in whole 128-byte steps and not; the most slots a
-# token, one expert, and more experts than slots.
+# The larger tiles, chosen by size (test_gpu_product_forms.py says which): 128 x 128 for both products,
+# 256 x 256 (groups of rows that end in a half tile and in a whole one) for either, with K in whole
+# 128-byte steps and not; the most slots a token, one expert, and more experts than slots.
 LARGE = [(1200, 2, 2, 72, 1032), (1200, 2, 2, 2056, 72), (600, 16, 2, 72, 1032), (600, 16, 2, 2056, 72),
          (2500, 6, 2, 1032, 520), (3000, 3, 2, 512, 1024), (1, 64, 64, 64, 64), (5, 64, 64, 72, 40),
          (33, 1, 1, 128, 64), (700, 1, 1, 128, 64), (50, 1024, 3, 64, 32),
