@@ -51,6 +51,17 @@ const char* mi355x_store_kv(const void* k, const void* v, void* kc, void* vc, co
                             int64_t kt, int64_t kh, int64_t vt, int64_t vh, int64_t reserved,
                             bool index64, int32_t* error_count, void* stream);
 
+/* Copies of cache pages in every plane (a layer's K or V) of a pool [planes, plane_pages,
+ * page_tokens, token_bytes]: the first tokens[i] tokens (page_tokens where tokens is NULL) of page
+ * src[i] go to page dst[i]. src, dst and tokens are host arrays of `pairs` entries, read before the
+ * call returns. A page may be the source of several copies; the destinations are distinct and none
+ * of them is a source, so the order of the copies does not matter. token_bytes is a multiple of 2.
+ * No reference counterpart (its pool, src/engine/kvcache/pool.rs:81-179, never copies a page). */
+const char* mi355x_copy_pages(void* pool, int64_t planes, int64_t plane_pages,
+                              int64_t page_tokens, int64_t token_bytes, const int32_t* src,
+                              const int32_t* dst, const int32_t* tokens, int64_t pairs,
+                              void* stream);
+
 /* ------------------------------------------------------------------------
  * Norms (fp32 accumulation, output rounded to the activation dtype).
  * ------------------------------------------------------------------------ */
@@ -463,6 +474,27 @@ const char* mi355x_sample_split(const void* logits, int64_t rows, int64_t vocab,
  * 151,936 logits 1.8 MB at 5 rows, 33 MB at 256, 132 MB at 1,024; 1.15 GB at most (1,024 rows
  * of 2 million). Host-only. */
 int64_t mi355x_sample_workspace_bytes(int64_t rows, int64_t vocab, bool top_p_rows);
+
+/* Log probabilities of given tokens, entropy and the most likely alternatives of logits rows
+ * (dtype 0 bf16, 1 fp16, 2 fp32; row stride in elements, any alignment of the type):
+ * logprobs[r] = log softmax(x[r])[tokens[r]] (NaN for a token outside [0, vocab)), entropy[r] =
+ * -sum p log p in nats, top_ids[r, :] the `top` (0 to 64, at most vocab) largest logits, largest
+ * first, equal ones by the lower index, top_logprobs[r, :] theirs. logprobs, entropy and
+ * top_logprobs fp32, tokens and top_ids int64, contiguous. A row with a NaN (which sorts above
+ * +inf) or a +inf, and one of only -inf, gets NaN for every probability and its entropy. Sums are
+ * fp32. Few rows are spread over several workgroups each: their parts go to `workspace` (16-byte
+ * aligned, mi355x_token_logprobs_workspace_bytes for the same sizes and compute units; calls that
+ * overlap need workspaces of their own). No reference counterpart. */
+const char* mi355x_token_logprobs(const void* logits, int64_t rows, int64_t vocab,
+                                  int64_t row_stride, int dtype, const int64_t* tokens,
+                                  int64_t top, void* logprobs, void* entropy, int64_t* top_ids,
+                                  void* top_logprobs, void* workspace, int64_t workspace_bytes,
+                                  int32_t cus, void* stream);
+
+/* Workspace bytes of mi355x_token_logprobs on a GPU of `cus` compute units (0: none), -1 for an
+ * invalid shape. Host-only. */
+int64_t mi355x_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top,
+                                              int32_t cus);
 
 #pragma GCC visibility pop
 

@@ -39,6 +39,8 @@ SIGNATURES: dict[str, tuple] = {
     "mi355x_store_kv": (c_char_p, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                    c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
                                    c_bool, c_void_p, c_void_p]),
+    "mi355x_copy_pages": (c_char_p, [c_void_p, c_i64, c_i64, c_i64, c_i64, c_void_p, c_void_p,
+                                     c_void_p, c_i64, c_void_p]),
     "mi355x_rms_norm": (c_char_p, [c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_i64, c_i64,
                                    c_i64, c_double, c_int, c_void_p]),
     "mi355x_add_rms_norm": (c_char_p, [c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_i64,
@@ -127,6 +129,10 @@ SIGNATURES: dict[str, tuple] = {
                                        c_void_p, c_u64, c_u64, c_void_p, c_bool, c_void_p,
                                        c_i64, c_void_p]),
     "mi355x_sample_workspace_bytes": (c_i64, [c_i64, c_i64, c_bool]),
+    "mi355x_token_logprobs": (c_char_p, [c_void_p, c_i64, c_i64, c_i64, c_int, c_void_p, c_i64,
+                                         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_i64,
+                                         c_i32, c_void_p]),
+    "mi355x_token_logprobs_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64, c_i32]),
 }
 
 _lock = threading.Lock()

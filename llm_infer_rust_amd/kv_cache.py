@@ -8,6 +8,9 @@ Mirrors:
   ``(pages, page_size, kv_heads, head_dim)`` K/V views, the reserved write
   slot, and ``write_kv`` with its shape checks and error messages.
 
+``KVCachePool.copy_pages`` copies pages over all layers in one launch (sequences that are forked,
+pages that move); the reference's pool never copies a page.
+
 Device writes go through ``mi355x_store_kv``. Out-of-range slots are never
 written; they are counted in a per-binding device word and reported by
 ``check_write_errors()`` (the reference aborts with a device assert instead,
@@ -16,10 +19,12 @@ written; they are counted in a per-binding device word and reported by
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import Sequence
 
+import numpy as np
 import torch
 
-from ._native import NativeError, check, lib, stream_of
+from ._native import NativeError, check, lib, on_device, stream_of
 
 
 class ModelError(RuntimeError):
@@ -42,6 +47,16 @@ class KVCacheLayout:
                 self.head_dim)
 
 
+def _host_ids(values: Sequence[int]) -> np.ndarray:
+    """A host sequence of ids as a contiguous int32 array; ids that int32 does not hold raise."""
+    wide = np.asarray(values)
+    if wide.ndim != 1 or wide.dtype.kind not in "iu":
+        raise ModelError("page ids and token counts must be sequences of integers")
+    if wide.size and (int(wide.min()) < -2 ** 31 or int(wide.max()) >= 2 ** 31):
+        raise ModelError("page id exceeds i32")
+    return np.ascontiguousarray(wide, np.int32)
+
+
 class KVCachePool:
     """One contiguous K/V buffer for every layer; page 0 is reserved and zeroed."""
 
@@ -52,6 +67,36 @@ class KVCachePool:
 
     def layer(self, index: int) -> tuple[torch.Tensor, torch.Tensor]:
         return self.buffer[0, index], self.buffer[1, index]
+
+    def copy_pages(self, src: Sequence[int], dst: Sequence[int],
+                   tokens: Sequence[int] | None = None) -> None:
+        """Copy pages ``src[i]`` to pages ``dst[i]`` in every layer's K and V: whole pages, or with
+        ``tokens`` only the first ``tokens[i]`` tokens of each (what is behind them stays as it is).
+
+        For a sequence that is forked inside a page, or pages that move. All three are host
+        sequences, and nothing of them is kept or uploaded. A page may be copied to several, but the
+        destinations are distinct, none of them is a source, and none is the reserved page 0; the
+        copies' order does not matter then."""
+        buf, layout = self.buffer, self.layout
+        if not buf.is_cuda or not buf.is_contiguous():
+            raise NativeError("copy_pages requires a contiguous pool on a GPU")
+        if buf.requires_grad:
+            raise NativeError("copy_pages: no gradient is recorded")
+        n = len(src)
+        if len(dst) != n or (tokens is not None and len(tokens) != n):
+            raise ModelError("copy_pages needs as many sources, destinations and token counts")
+        if n == 0:
+            return
+        a, b = _host_ids(src), _host_ids(dst)
+        if int(b.min()) <= 0:
+            raise ModelError("copy_pages: the reserved page 0 and negative pages are not written")
+        c = None if tokens is None else _host_ids(tokens)
+        with on_device(buf.device):
+            check(lib().mi355x_copy_pages(
+                buf.data_ptr(), 2 * layout.num_layers, layout.num_pages + 1, layout.page_size,
+                layout.num_kv_heads * layout.head_dim * buf.element_size(), a.ctypes.data,
+                b.ctypes.data, None if c is None else c.ctypes.data, n, stream_of(buf)),
+                "copy_pages")
 
 
 class BaseAttention:

@@ -16,16 +16,22 @@ whole heterogeneous batch: the parameters travel as per-row device arrays.
 The call is one launch, or two to six where rows are spread over several
 workgroups. The random stream is (seed, offset): ``manual_seed`` resets both
 and every sampling call advances the offset by one.
+
+``token_logprobs(logits, tokens, top)`` gives the log probabilities of given
+tokens, the entropy of their distributions and the most likely alternatives;
+the reference's sampler returns ids only.
 """
 from __future__ import annotations
 
 import math
 from collections import Counter
 from dataclasses import dataclass, replace
+from typing import NamedTuple
 
 import torch
 
-from ._native import NativeError, check, lib, stream_of
+from ._native import NativeError, check, device_cus, lib, on_device, stream_of
+from .int8 import _refuse_grad, _rows
 
 
 class SamplingError(RuntimeError):
@@ -232,4 +238,58 @@ class Sampler:
         return PendingSample(self.sample_batch_device(logits, params_list), logits)
 
 
-__all__ = ["SamplingParams", "Sampler", "PendingSample", "SamplingError"]
+MAX_TOP_LOGPROBS = 64
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` returns, in nats."""
+    logprobs: torch.Tensor      # fp32 [rows]: the given tokens'
+    entropy: torch.Tensor       # fp32 [rows]: of the whole distribution
+    top_ids: torch.Tensor       # int64 [rows, top]: the most likely tokens, likeliest first
+    top_logprobs: torch.Tensor  # fp32 [rows, top]: theirs
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """Log probabilities of ``tokens`` (int64 ``[rows]``) under ``softmax(logits)`` (``[rows,
+    vocab]`` in bf16, fp16 or fp32, before any temperature), the distributions' entropy and the
+    ``top`` most likely tokens of every row (up to 64; equal logits by the lower id).
+
+    As ``torch.log_softmax`` has it, a row with a NaN or a +inf, or of only -inf, gives NaN; so does
+    a token outside ``[0, vocab)`` (the -1 of an invalid sampling row) for its own probability. The
+    logits are read once and nothing is read back, so the call can be captured in a HIP graph.
+    Inference only: a call whose derivative would be wanted is refused."""
+    rows, vocab, stride = _rows(logits, "token_logprobs")
+    dt = _DTYPES.get(logits.dtype)
+    if dt is None:
+        raise NativeError(f"token_logprobs: unsupported logits dtype {logits.dtype}")
+    if vocab == 0:
+        raise NativeError("token_logprobs: rows must not be empty")
+    if (tokens.dtype != torch.int64 or tokens.shape != (rows,) or tokens.device != logits.device
+            or not tokens.is_contiguous()):
+        raise NativeError("token_logprobs: expected contiguous int64 tokens [rows] on the logits' "
+                          "device")
+    top = int(top)
+    if not 0 <= top <= min(vocab, MAX_TOP_LOGPROBS):
+        raise NativeError(f"token_logprobs: expected top of 0 to min(vocab, {MAX_TOP_LOGPROBS})")
+    _refuse_grad("token_logprobs", logits)
+    device = logits.device
+    cus = device_cus(device)
+    native = lib()
+    values = torch.empty(rows * (2 + top), dtype=torch.float32, device=device)
+    ids = torch.empty(rows, top, dtype=torch.int64, device=device)
+    out = TokenLogprobs(values[:rows], values[rows:2 * rows], ids,
+                        values[2 * rows:].view(rows, top))
+    need = native.mi355x_token_logprobs_workspace_bytes(rows, vocab, top, cus)
+    if need < 0:
+        raise NativeError("token_logprobs: bad shape")
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    with on_device(device):
+        check(native.mi355x_token_logprobs(
+            logits.data_ptr(), rows, vocab, stride, dt, tokens.data_ptr(), top,
+            out.logprobs.data_ptr(), out.entropy.data_ptr(), ids.data_ptr(),
+            out.top_logprobs.data_ptr(), None if ws is None else ws.data_ptr(), need, cus,
+            stream_of(logits)), "token_logprobs")
+    return out
+
+
+__all__ = ["TokenLogprobs", "token_logprobs", "SamplingParams", "Sampler", "PendingSample", "SamplingError"]

@@ -18,6 +18,9 @@ unsafe extern "C" {
         loc: *const c_void, tokens: i64, heads: i64, width: i64, capacity: i64,
         kt: i64, kh: i64, vt: i64, vh: i64, reserved: i64, index64: bool,
         error_count: *mut i32, stream: *mut c_void) -> *const c_char;
+    pub fn mi355x_copy_pages(pool: *mut c_void, planes: i64, plane_pages: i64, page_tokens: i64,
+        token_bytes: i64, src: *const i32, dst: *const i32, tokens: *const i32, pairs: i64,
+        stream: *mut c_void) -> *const c_char;
     pub fn mi355x_rms_norm(x: *const c_void, w: *const c_void, out: *mut c_void, tokens: i64,
         heads: i64, width: i64, token_stride: i64, head_stride: i64, eps: f64, dtype: c_int,
         stream: *mut c_void) -> *const c_char;
@@ -116,6 +119,12 @@ unsafe extern "C" {
         seed: u64, offset: u64, out: *mut i64, top_p_rows: bool, workspace: *mut c_void,
         workspace_bytes: i64, stream: *mut c_void) -> *const c_char;
     pub fn mi355x_sample_workspace_bytes(rows: i64, vocab: i64, top_p_rows: bool) -> i64;
+    pub fn mi355x_token_logprobs(logits: *const c_void, rows: i64, vocab: i64, row_stride: i64,
+        dtype: c_int, tokens: *const i64, top: i64, logprobs: *mut c_void, entropy: *mut c_void,
+        top_ids: *mut i64, top_logprobs: *mut c_void, workspace: *mut c_void, workspace_bytes: i64,
+        cus: i32, stream: *mut c_void) -> *const c_char;
+    pub fn mi355x_token_logprobs_workspace_bytes(rows: i64, vocab: i64, top: i64,
+        cus: i32) -> i64;
 }
 
 /// Introspection and host-side planning entries (ported tests, diagnostics); the serving
