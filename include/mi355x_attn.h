@@ -107,6 +107,26 @@ void* mi355x_decode_prepare(void* existing, const int32_t* block_table, int64_t 
                             int64_t page_size, int64_t dtype, bool graph,
                             const int32_t* host_lengths, int64_t host_rows, void* stream);
 
+/* mi355x_decode_prepare for a batch in which groups of consecutive rows share leading tokens:
+ * group g holds group_rows[g] rows (host array; they sum to the batch) whose first group_lens[g]
+ * tokens have the same K and V, in the same pages or in copies. Attention over those is computed
+ * once for the group, from the pages of its first row, and joined with every row's own; the result
+ * is that of mi355x_decode_prepare up to rounding. Shared lengths are used in whole 64-token tiles
+ * that leave each row a token, and only where that pays (mi355x_decode_plan_shared_info says).
+ * A graph plan takes groups on a re-plan if it was created with some (their sizes and lengths may
+ * change, also to 0); otherwise they are checked and not used. */
+void* mi355x_decode_prepare_shared(void* existing, const int32_t* block_table, int64_t batch,
+                                   int64_t columns, int64_t table_stride, const int32_t* seq_lens,
+                                   int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                   int64_t page_size, int64_t dtype, bool graph,
+                                   const int32_t* host_lengths, int64_t host_rows,
+                                   const int32_t* group_rows, const int32_t* group_lens,
+                                   int64_t groups, void* stream);
+
+/* out4 = {groups whose prefix is computed once, tokens of those prefixes, work items of that launch,
+ * waves of its workgroups (0: no such launch)}. Introspection. */
+const char* mi355x_decode_plan_shared_info(const void* plan, int64_t* out4);
+
 /* out[b, h, :] = softmax(q[b,h] K^T / sqrt(128)) V over the request's pages.
  * q/out: [batch, num_q_heads, 128] with the given strides (16-byte aligned
  * rows); caches: contiguous [pages, page_size, num_kv_heads, 128].
@@ -171,6 +191,20 @@ void* mi355x_prefill_prepare(void* existing, const int32_t* q_indptr, const int3
                              const int32_t* q_host, const int32_t* prefix_host,
                              int64_t num_q_heads, int64_t num_kv_heads, int64_t page_size,
                              int64_t dtype, void* stream);
+
+/* mi355x_prefill_prepare for a batch in which groups of consecutive rows share leading cached
+ * tokens, as mi355x_decode_prepare_shared: group_lens[g] is at most the cached prefix of every row
+ * of the group. */
+void* mi355x_prefill_prepare_shared(void* existing, const int32_t* q_indptr,
+                                    const int32_t* block_table, int64_t batch, int64_t columns,
+                                    int64_t table_stride, const int32_t* q_host,
+                                    const int32_t* prefix_host, int64_t num_q_heads,
+                                    int64_t num_kv_heads, int64_t page_size, int64_t dtype,
+                                    const int32_t* group_rows, const int32_t* group_lens,
+                                    int64_t groups, void* stream);
+
+/* As mi355x_decode_plan_shared_info, for a prefill plan. */
+const char* mi355x_prefill_plan_shared_info(const void* plan, int64_t* out4);
 
 /* out[t, h, :] = causal softmax attention of query row t. q: [total_q,
  * num_q_heads, 128] with strides (q_sn, q_sh, 1). Ragged plans read k/v as

@@ -50,6 +50,11 @@ SIGNATURES: dict[str, tuple] = {
     "mi355x_decode_prepare": (c_void_p, [c_void_p, c_void_p, c_i64, c_i64, c_i64, c_void_p,
                                          c_i64, c_i64, c_i64, c_i64, c_i64, c_bool, c_void_p,
                                          c_i64, c_void_p]),
+    "mi355x_decode_prepare_shared": (c_void_p, [c_void_p, c_void_p, c_i64, c_i64, c_i64, c_void_p,
+                                                c_i64, c_i64, c_i64, c_i64, c_i64, c_bool,
+                                                c_void_p, c_i64, c_void_p, c_void_p, c_i64,
+                                                c_void_p]),
+    "mi355x_decode_plan_shared_info": (c_char_p, [c_void_p, P_i64]),
     "mi355x_decode_run": (c_char_p, [c_void_p, c_void_p, c_i64, c_i64, c_void_p, c_void_p,
                                      c_void_p, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
                                      c_void_p]),
@@ -64,6 +69,10 @@ SIGNATURES: dict[str, tuple] = {
     "mi355x_prefill_prepare": (c_void_p, [c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_i64,
                                           c_void_p, c_void_p, c_i64, c_i64, c_i64, c_i64,
                                           c_void_p]),
+    "mi355x_prefill_prepare_shared": (c_void_p, [c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_i64,
+                                                 c_void_p, c_void_p, c_i64, c_i64, c_i64, c_i64,
+                                                 c_void_p, c_void_p, c_i64, c_void_p]),
+    "mi355x_prefill_plan_shared_info": (c_char_p, [c_void_p, P_i64]),
     "mi355x_prefill_run": (c_char_p, [c_void_p, c_void_p, c_i64, c_i64, c_void_p, c_i64, c_i64,
                                       c_void_p, c_i64, c_i64, c_void_p, c_i64, c_i64, c_i64,
                                       c_i64, c_i64, c_i64, c_i64, c_void_p]),

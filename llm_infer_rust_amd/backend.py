@@ -13,6 +13,9 @@ Host mirror of the reference's ``src/models/attention/backend.rs``:
 * plan reuse rules of the FlashInfer backend (``backend.rs:386-438``): a new
   batch may not be prepared while the previous one is still referenced.
 
+``AttentionMetadata.shared_prefix`` names leading tokens that rows of a batch share (several
+completions of one prompt, a common system prompt): attention over them is computed once.
+
 Only the ``mi355x`` kind is implemented by this package; the reference's own
 ``pt``/``fa``/``flashinfer`` kinds parse but are rejected by ``validate``.
 """
@@ -75,6 +78,18 @@ class DecodeHostMetadata:
     block_table_versions: list[int] | None = None
 
 
+@dataclass(frozen=True)
+class SharedPrefix:
+    """Consecutive rows of a batch that share leading tokens: group ``g`` holds ``rows[g]`` rows
+    whose first ``lens[g]`` tokens have the same K and V in the cache, in the same pages or in copies
+    (``rows`` sums to the batch; 0 or a group of one: nothing shared). Attention over them is computed
+    once for the group, read through the pages of its first row. Host values; the reference has no
+    counterpart. A statement about the cache, not a request: results are those of a batch without it
+    up to rounding, and it is not used where that would cost more than it saves."""
+    rows: Sequence[int]
+    lens: Sequence[int]
+
+
 @dataclass
 class AttentionMetadata:
     """Per-invocation metadata (``src/engine/model_runner.rs:47-59``). int32 tensors."""
@@ -91,6 +106,8 @@ class AttentionMetadata:
     # plans from them instead of reading the device tensors back (no sync per forward).
     host_cu_seqlens_q: list[int] | None = None
     host_prefix_lens: list[int] | None = None
+    # Leading tokens that rows share: of all their tokens (decode) or their cached ones (prefill).
+    shared_prefix: SharedPrefix | None = None
 
 
 @dataclass
@@ -148,6 +165,24 @@ def prefill_boundaries(metadata: AttentionMetadata, total_tokens: int) -> list[i
 # ---------------------------------------------------------------------------
 # Native plans
 # ---------------------------------------------------------------------------
+def shared_info(entry: str, handle: int) -> dict[str, int]:
+    """What a plan makes of shared prefixes: groups and tokens computed once, work items of that
+    launch and waves of its workgroups (0: no such launch)."""
+    buf = (ctypes.c_int64 * 4)()
+    check(getattr(lib(), entry)(handle, buf), "shared prefix info")
+    return dict(zip(("groups", "tokens", "items", "waves"), list(buf)))
+
+
+def shared_arrays(shared: SharedPrefix, batch: int) -> tuple[np.ndarray, np.ndarray]:
+    """Group sizes and shared lengths as int32 arrays for the planners."""
+    rows, lens = np.asarray(shared.rows), np.asarray(shared.lens)
+    if (rows.ndim != 1 or rows.shape != lens.shape or rows.size == 0
+            or rows.dtype.kind not in "iu" or lens.dtype.kind not in "iu" or int(rows.min()) <= 0
+            or int(rows.sum()) != batch or int(lens.min()) < 0 or int(lens.max()) >= 2 ** 31):
+        raise ModelError("invalid shared prefix groups")
+    return np.ascontiguousarray(rows, np.int32), np.ascontiguousarray(lens, np.int32)
+
+
 class DecodePlan:
     """Owns one native decode plan handle (``mi355x_decode_prepare``)."""
 
@@ -160,6 +195,9 @@ class DecodePlan:
         check(lib().mi355x_decode_plan_info(self.handle, buf), "decode plan info")
         keys = ("batch", "total_pages", "num_items", "chunk_tokens", "items_capacity", "cus")
         return dict(zip(keys, list(buf)))
+
+    def shared_info(self) -> dict[str, int]:
+        return shared_info("mi355x_decode_plan_shared_info", self.handle)
 
     def allocations(self) -> int:
         return int(lib().mi355x_decode_workspace_allocations(self.handle))
@@ -214,10 +252,16 @@ def prepare_decode_plan(existing: DecodePlan | None, metadata: AttentionMetadata
         if rows == 0:
             raise ModelError("invalid host decode metadata")
         host = values.ctypes.data  # ``values`` outlives the call
-    handle = lib().mi355x_decode_prepare(
-        existing.handle if existing else None, table.data_ptr(), table.size(0), table.size(1),
-        table.stride(0), lengths.data_ptr(), spec.num_heads, spec.num_kv_heads, spec.head_dim,
-        page_size, dt, graph, host, rows, stream_of(table))
+    args = (existing.handle if existing else None, table.data_ptr(), table.size(0), table.size(1),
+            table.stride(0), lengths.data_ptr(), spec.num_heads, spec.num_kv_heads, spec.head_dim,
+            page_size, dt, graph, host, rows)
+    if metadata.shared_prefix is None:
+        handle = lib().mi355x_decode_prepare(*args, stream_of(table))
+    else:
+        group_rows, group_lens = shared_arrays(metadata.shared_prefix, table.size(0))
+        handle = lib().mi355x_decode_prepare_shared(*args, group_rows.ctypes.data,
+                                                    group_lens.ctypes.data, group_rows.size,
+                                                    stream_of(table))
     if not handle:
         raise ModelError(f"mi355x decode plan failed: {last_error()}")
     if existing is not None:
@@ -347,13 +391,17 @@ class DecodeGraphState:
         self.spec = spec
         self.page_size = page_size
 
-    def prepare_replay(self, host: DecodeHostMetadata | None) -> None:
+    def prepare_replay(self, host: DecodeHostMetadata | None,
+                       shared: SharedPrefix | None = None) -> None:
+        """``shared`` covers every row of the graph, pad rows included; it is used when the graph was
+        prepared with a ``shared_prefix`` (of any groups)."""
         if host is not None and len(host.cache_seqlens) < self.table.size(0):
             seqlens = np.ones(self.table.size(0), np.int32)  # pad rows read page 0
             seqlens[:len(host.cache_seqlens)] = host.cache_seqlens
             host = DecodeHostMetadata(seqlens)
         meta = AttentionMetadata(forward_mode=BatchPhase.DECODE, decode_host=host,
-                                 block_table=self.table, cache_seqlens=self.lengths)
+                                 block_table=self.table, cache_seqlens=self.lengths,
+                                 shared_prefix=shared)
         prepare_decode_plan(self.plan, meta, self.spec, self.page_size, graph=True)
 
     def needs_req_to_token(self) -> bool:
@@ -443,5 +491,5 @@ def sm_scale(head_dim: int) -> float:
 __all__ = [
     "Attention", "AttentionBatch", "AttentionBackendKind", "AttentionMetadata", "AttentionSpec",
     "BatchPhase", "DecodeGraphState", "DecodeHostMetadata", "DecodePlan", "MetadataRequirements",
-    "ModelError", "NativeError", "PrefillMetadata", "prepare_decode_plan", "run_decode",
+    "ModelError", "NativeError", "PrefillMetadata", "SharedPrefix", "prepare_decode_plan", "run_decode",
 ]

@@ -33,6 +33,8 @@
 #include <vector>
 
 #include "common.h"
+#include "mfma.h"
+#include "shared.h"
 
 namespace mi355x {
 namespace {
@@ -46,29 +48,6 @@ constexpr int kTileBytes = kTileK * kD * 2;   // 16 KB per K or V tile
 constexpr int kStageBytes = 2 * kTileBytes;   // K + V
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxKvLen = 1 << 22;            // div_small is exact below this
-
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef float floatx16 __attribute__((ext_vector_type(16)));
-
-template <int DT>
-struct Mfma;
-
-template <>
-struct Mfma<0> {
-  __device__ __forceinline__ static floatx16 run(const uint4& a, const uint4& b, floatx16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
-                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-  }
-};
-
-template <>
-struct Mfma<1> {
-  __device__ __forceinline__ static floatx16 run(const uint4& a, const uint4& b, floatx16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
-                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
-  }
-};
 
 struct ReqInfo {  // per request, uploaded by the plan
   int32_t q_start, q_len, prefix, page_base;
@@ -112,25 +91,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // ds_read_b64_tr_b16: within 16 lanes it returns lane i the 4 elements
 // {M[4j + i/4][i%4]}_j of the 16 x 4 block M whose row p the lane p addressed.
 // ---------------------------------------------------------------------------
-
-typedef short v4i16_t __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) v4i16_t lds_v4i16;
-
-// q = x / d, r = x % d for 0 <= x < 2^22 and 1 <= d, via a float reciprocal and one
-// correction step each way.
-__device__ __forceinline__ int div_small(int x, int d, float inv, int& r) {
-  int q = static_cast<int>(static_cast<float>(x) * inv);
-  r = x - q * d;
-  if (r >= d) {
-    ++q;
-    r -= d;
-  }
-  if (r < 0) {
-    --q;
-    r += d;
-  }
-  return q;
-}
 
 // NW waves per workgroup: 8 (one workgroup per CU, a 4-stage ring) or 4 (two workgroups
 // per CU, a 2-stage ring each, so one workgroup's prologue, epilogue and barriers overlap
@@ -644,8 +604,12 @@ struct PrefillPlan {
   int64_t num_groups = 0;   // items split along the keys (merged by a second launch)
   int64_t num_records = 0;  // partial records (chunks of split items)
   // Device int32 workspace: [req info 4*B][work 4*items][ranges 4*items][kv_indptr B+1]
-  // [last_len B][groups 8*num_groups]
-  int64_t o_work = 0, o_ranges = 0, o_indptr = 0, o_last = 0, o_groups = 0;
+  // [last_len B][groups 8*num_groups][shared prefixes: header, kSharedInfoInts * B, request of
+  // every token, work items]
+  int64_t o_work = 0, o_ranges = 0, o_indptr = 0, o_last = 0, o_groups = 0, o_shared = 0;
+  // Shared prefixes (shared_nw 0: none): the whole batch then runs as sources of the shared kernel.
+  int shared_nw = 0;
+  int64_t o_shared_work = 0, shared_items = 0, shared_groups = 0, shared_tokens = 0;
   Buffer ints, indices, staging, part_o, part_lse;
   hipEvent_t upload_done = nullptr;
   uint64_t allocations = 0;
@@ -782,12 +746,13 @@ SplitPlan split_items(const std::vector<int32_t>& base, const int32_t* q_host,
 }  // namespace
 }  // namespace mi355x
 
-extern "C" void* mi355x_prefill_prepare(void* existing, const int32_t* q_indptr,
-                                        const int32_t* block_table, int64_t batch,
-                                        int64_t columns, int64_t table_stride,
-                                        const int32_t* q_host, const int32_t* prefix_host,
-                                        int64_t num_q_heads, int64_t num_kv_heads,
-                                        int64_t page_size, int64_t dtype, void* stream) {
+// group_rows / group_lens: host arrays of `groups` entries (0: no groups were given).
+static void* prepare_prefill(void* existing, const int32_t* q_indptr, const int32_t* block_table,
+                             int64_t batch, int64_t columns, int64_t table_stride,
+                             const int32_t* q_host, const int32_t* prefix_host,
+                             int64_t num_q_heads, int64_t num_kv_heads, int64_t page_size,
+                             int64_t dtype, const int32_t* group_rows, const int32_t* group_lens,
+                             int64_t groups, void* stream) {
   auto s = static_cast<hipStream_t>(stream);
   std::unique_ptr<PrefillPlan> created;
   auto* plan = static_cast<PrefillPlan*>(existing);
@@ -824,6 +789,29 @@ extern "C" void* mi355x_prefill_prepare(void* existing, const int32_t* q_indptr,
     if (paged && (!block_table || columns <= 0 || table_stride < columns)) {
       set_error("paged prefill requires a block table");
       return nullptr;
+    }
+    std::vector<int32_t> eff;  // tokens of each group's prefix that are computed once
+    bool sharing = false;
+    if (groups > 0) {
+      int64_t rows = 0;
+      for (int64_t g = 0; g < groups; ++g) {
+        if (group_rows[g] <= 0 || group_lens[g] < 0 || group_rows[g] > batch - rows) {
+          set_error("invalid shared prefix groups");
+          return nullptr;
+        }
+        for (int64_t r = rows; r < rows + group_rows[g]; ++r)
+          if (group_lens[g] > prefix_host[r]) {
+            set_error("shared prefix is longer than the cached prefix of a row of its group");
+            return nullptr;
+          }
+        rows += group_rows[g];
+      }
+      if (rows != batch) {
+        set_error("invalid shared prefix groups");
+        return nullptr;
+      }
+      sharing =
+          shared_lengths(group_rows, group_lens, groups, prefix_host, num_kv_heads, eff);
     }
     int device = 0;
     hipError_t st = hipGetDevice(&device);
@@ -866,12 +854,52 @@ extern "C" void* mi355x_prefill_prepare(void* existing, const int32_t* q_indptr,
       }
       plan->cus = cus;
     }
-    std::vector<int32_t> base(4 * n_base);
-    mi355x_prefill_schedule(q_host, prefix_host, batch, num_q_heads, num_kv_heads, base.data(),
-                            n_base);
-    const SplitPlan sp =
-        split_items(base, q_host, prefix_host, num_q_heads, num_kv_heads, plan->cus,
-                    prefill_waves(paged));
+    SplitPlan sp;
+    // With shared prefixes: every group's queries against its prefix, then every request's against
+    // its own keys.
+    std::vector<SharedSource> sources;
+    std::vector<int32_t> shared_work, source_of(batch, -1);
+    int shared_nw = 0;
+    int64_t shared_records = 0, shared_groups = 0, shared_tokens = 0;
+    if (sharing) {
+      int64_t row = 0, page = 0;
+      std::vector<SharedSource> own;
+      for (int64_t g = 0; g < groups; ++g) {
+        const int64_t end = row + group_rows[g];
+        if (eff[g] > 0) {
+          sources.push_back({q_host[row], q_host[end] - q_host[row], static_cast<int32_t>(page), 0,
+                             eff[g] / kSharedTile, kNoHorizon, eff[g], 0, 0, 0});
+          ++shared_groups;
+          shared_tokens += eff[g];
+        }
+        for (; row < end; ++row) {
+          if (eff[g] > 0) source_of[row] = static_cast<int32_t>(sources.size() - 1);
+          const int32_t q_len = q_host[row + 1] - q_host[row];
+          const int32_t kv_len = prefix_host[row] + q_len;
+          own.push_back({q_host[row], q_len, static_cast<int32_t>(page), eff[g] / kSharedTile,
+                         (kv_len + kSharedTile - 1) / kSharedTile, prefix_host[row], kv_len, 0, 0,
+                         0});
+          page += (kv_len + page_size - 1) / page_size;
+        }
+      }
+      sources.insert(sources.end(), own.begin(), own.end());
+      const int64_t heads_per_kv = num_q_heads / num_kv_heads;
+      shared_nw = shared_waves(sources, heads_per_kv);
+      shared_records = schedule_shared(
+          sources, heads_per_kv, num_kv_heads, plan->cus, shared_nw,
+          shared_capacity(sources, heads_per_kv, num_kv_heads, plan->cus, shared_nw), shared_work);
+    } else {
+      std::vector<int32_t> base(4 * n_base);
+      mi355x_prefill_schedule(q_host, prefix_host, batch, num_q_heads, num_kv_heads, base.data(),
+                              n_base);
+      sp = split_items(base, q_host, prefix_host, num_q_heads, num_kv_heads, plan->cus,
+                       prefill_waves(paged));
+    }
+    const int64_t shared_items = static_cast<int64_t>(shared_work.size()) / kSharedItemInts;
+    if (shared_items > std::numeric_limits<int32_t>::max() / 64) {
+      set_error("prefill work list is empty or too large");
+      return nullptr;
+    }
     const int64_t n_items = static_cast<int64_t>(sp.work.size() / 4);
     const int64_t n_groups = static_cast<int64_t>(sp.groups.size() / 8);
     if (n_items > std::numeric_limits<int32_t>::max() / 64) {
@@ -883,19 +911,25 @@ extern "C" void* mi355x_prefill_prepare(void* existing, const int32_t* q_indptr,
     const int64_t o_indptr = o_ranges + 4 * n_items;
     const int64_t o_last = o_indptr + batch + 1;
     const int64_t o_groups = (o_last + batch + 3) / 4 * 4;  // int4-aligned
-    const int64_t total_ints = o_groups + 8 * n_groups;
+    const int64_t o_shared = o_groups + 8 * n_groups;
+    const int64_t o_shared_work =
+        o_shared + kSharedHeaderInts + kSharedInfoInts * batch + (q_host[batch] + 3) / 4 * 4;
+    const int64_t total_ints =
+        sharing ? o_shared_work + static_cast<int64_t>(shared_work.size()) : o_shared;
     st = hipEventSynchronize(plan->upload_done);
     if (st != hipSuccess) {
       hip_error(st, "prefill upload fence");
       return nullptr;
     }
+    // fp32 rows of 128 outputs and their log2-sum-exp
     const size_t rec_bytes =
-        static_cast<size_t>(sp.records) * prefill_waves(paged) * kQPerWave * 4;
+        sharing ? static_cast<size_t>(shared_records) * 32 * 4
+                : static_cast<size_t>(sp.records) * prefill_waves(paged) * kQPerWave * 4;
     if ((st = plan->ints.reserve(total_ints * 4, plan->allocations)) != hipSuccess ||
         (st = plan->staging.reserve(total_ints * 4, plan->allocations)) != hipSuccess ||
-        (sp.records && (st = plan->part_o.reserve(rec_bytes * kD, plan->allocations)) !=
+        (rec_bytes && (st = plan->part_o.reserve(rec_bytes * kD, plan->allocations)) !=
                            hipSuccess) ||
-        (sp.records && (st = plan->part_lse.reserve(rec_bytes, plan->allocations)) !=
+        (rec_bytes && (st = plan->part_lse.reserve(rec_bytes, plan->allocations)) !=
                            hipSuccess)) {
       hip_error(st, "prefill workspace allocation");
       return nullptr;
@@ -923,8 +957,30 @@ extern "C" void* mi355x_prefill_prepare(void* existing, const int32_t* q_indptr,
         host[o_last + r] = 0;
       }
     }
-    std::memcpy(host + o_work, sp.work.data(), sp.work.size() * 4);
-    std::memcpy(host + o_ranges, sp.ranges.data(), sp.ranges.size() * 4);
+    if (n_items) {
+      std::memcpy(host + o_work, sp.work.data(), sp.work.size() * 4);
+      std::memcpy(host + o_ranges, sp.ranges.data(), sp.ranges.size() * 4);
+    }
+    if (sharing) {
+      int32_t* section = host + o_shared;
+      std::memset(section, 0, (kSharedHeaderInts + kSharedInfoInts * batch) * 4);
+      section[0] = static_cast<int32_t>(shared_items);
+      int32_t* row_of = section + kSharedHeaderInts + kSharedInfoInts * batch;
+      for (int64_t r = 0; r < batch; ++r) {
+        int32_t* info = section + kSharedHeaderInts + kSharedInfoInts * r;
+        for (int part = 0; part < 2; ++part) {
+          const int64_t i = part == 0 ? source_of[r] : shared_groups + r;
+          if (i < 0) continue;
+          const SharedSource& src = sources[i];
+          info[4 * part] = src.record;
+          info[4 * part + 1] = src.splits;
+          info[4 * part + 2] = src.row_tiles;
+          info[4 * part + 3] = src.token0;
+        }
+        std::fill(row_of + q_host[r], row_of + q_host[r + 1], static_cast<int32_t>(r));
+      }
+      std::memcpy(host + o_shared_work, shared_work.data(), shared_work.size() * 4);
+    }
     if (n_groups) std::memcpy(host + o_groups, sp.groups.data(), sp.groups.size() * 4);
     st = hipMemcpyAsync(plan->ints.ptr, host, total_ints * 4, hipMemcpyHostToDevice, s);
     if (st != hipSuccess) {
@@ -959,12 +1015,53 @@ extern "C" void* mi355x_prefill_prepare(void* existing, const int32_t* q_indptr,
     plan->o_indptr = o_indptr;
     plan->o_last = o_last;
     plan->o_groups = o_groups;
+    plan->o_shared = o_shared;
+    plan->o_shared_work = o_shared_work;
+    plan->shared_nw = shared_nw;
+    plan->shared_items = shared_items;
+    plan->shared_groups = shared_groups;
+    plan->shared_tokens = shared_tokens;
     created.release();
     return plan;
   } catch (const std::exception& e) {
     set_error(e.what());
     return nullptr;
   }
+}
+
+extern "C" void* mi355x_prefill_prepare(void* existing, const int32_t* q_indptr,
+                                        const int32_t* block_table, int64_t batch,
+                                        int64_t columns, int64_t table_stride,
+                                        const int32_t* q_host, const int32_t* prefix_host,
+                                        int64_t num_q_heads, int64_t num_kv_heads,
+                                        int64_t page_size, int64_t dtype, void* stream) {
+  return prepare_prefill(existing, q_indptr, block_table, batch, columns, table_stride, q_host,
+                         prefix_host, num_q_heads, num_kv_heads, page_size, dtype, nullptr, nullptr,
+                         0, stream);
+}
+
+extern "C" void* mi355x_prefill_prepare_shared(
+    void* existing, const int32_t* q_indptr, const int32_t* block_table, int64_t batch,
+    int64_t columns, int64_t table_stride, const int32_t* q_host, const int32_t* prefix_host,
+    int64_t num_q_heads, int64_t num_kv_heads, int64_t page_size, int64_t dtype,
+    const int32_t* group_rows, const int32_t* group_lens, int64_t groups, void* stream) {
+  if (!group_rows || !group_lens || groups <= 0) {
+    set_error("invalid shared prefix groups");
+    return nullptr;
+  }
+  return prepare_prefill(existing, q_indptr, block_table, batch, columns, table_stride, q_host,
+                         prefix_host, num_q_heads, num_kv_heads, page_size, dtype, group_rows,
+                         group_lens, groups, stream);
+}
+
+extern "C" const char* mi355x_prefill_plan_shared_info(const void* plan, int64_t* out4) {
+  if (!plan || !out4) return set_error("mi355x_prefill_plan_shared_info: null argument");
+  const auto* p = static_cast<const PrefillPlan*>(plan);
+  out4[0] = p->shared_groups;
+  out4[1] = p->shared_tokens;
+  out4[2] = p->shared_items;
+  out4[3] = p->shared_nw;
+  return nullptr;
 }
 
 extern "C" void mi355x_prefill_plan_drop(void* plan) { delete static_cast<PrefillPlan*>(plan); }
@@ -1086,6 +1183,40 @@ extern "C" const char* mi355x_prefill_run(const void* plan_ptr, const void* q, i
   const int waves = prefill_waves(p.paged);
   const int hpb = heads_per_block(num_q_heads / num_kv_heads, waves);
   auto s = static_cast<hipStream_t>(stream);
+  if (p.shared_nw) {
+    if (k_sn != num_kv_heads * kD || v_sn != k_sn || k_sh != kD || v_sh != kD)
+      return set_error("shared prefixes need contiguous caches");
+    const int32_t* section = ints + p.o_shared;
+    SharedArgs sa{};
+    sa.q = a.q;
+    sa.q_sn = q_sn;
+    sa.q_sh = q_sh;
+    sa.k = a.k;
+    sa.v = a.v;
+    sa.header = section;
+    sa.work = reinterpret_cast<const int4*>(ints + p.o_shared_work);
+    sa.indices = a.indices;
+    sa.part_o = a.part_o;
+    sa.part_lse = a.part_lse;
+    sa.group = static_cast<int32_t>(num_q_heads / num_kv_heads);
+    sa.num_kv_heads = a.num_kv_heads;
+    sa.page_size = a.page_size;
+    sa.scale_log2 = a.scale_log2;
+    if (const char* err = launch_shared(sa, dtype, p.shared_nw, p.shared_items, s)) return err;
+    SharedMergeArgs m{};
+    m.out = a.out;
+    m.o_sn = o_sn;
+    m.o_sh = o_sh;
+    m.rows = total_q * num_q_heads;
+    m.info = reinterpret_cast<const int4*>(section + kSharedHeaderInts);
+    m.row_of = section + kSharedHeaderInts + kSharedInfoInts * p.batch;
+    m.part_o = a.part_o;
+    m.part_lse = a.part_lse;
+    m.num_q_heads = a.num_q_heads;
+    m.group = sa.group;
+    m.num_kv_heads = a.num_kv_heads;
+    return launch_shared_merge(m, dtype, s);
+  }
   const int4* groups = reinterpret_cast<const int4*>(ints + p.o_groups);
   if (dtype == 0)
     launch_dt<0>(a, hpb, waves, p.paged, groups, p.num_groups, s);

@@ -32,6 +32,10 @@ class PrefillPlan:
         keys = ("batch", "total_q", "paged", "num_items", "total_pages", "split_items")
         return dict(zip(keys, list(buf)))
 
+    def shared_info(self) -> dict[str, int]:
+        from .backend import shared_info
+        return shared_info("mi355x_prefill_plan_shared_info", self.handle)
+
     def allocations(self) -> int:
         return int(lib().mi355x_prefill_workspace_allocations(self.handle))
 
@@ -82,10 +86,17 @@ def prepare_prefill_plan(existing: PrefillPlan | None, metadata, prefill, spec,
     b = len(prefill.prefixes)
     qh = (ctypes.c_int32 * (b + 1))(*prefill.boundaries)
     ph = (ctypes.c_int32 * b)(*prefill.prefixes)
-    handle = lib().mi355x_prefill_prepare(
-        existing.handle if existing else None, cu.data_ptr(), table.data_ptr(), b,
-        table.size(1), table.stride(0), qh, ph, spec.num_heads, spec.num_kv_heads, page_size, dt,
-        stream_of(cu))
+    args = (existing.handle if existing else None, cu.data_ptr(), table.data_ptr(), b,
+            table.size(1), table.stride(0), qh, ph, spec.num_heads, spec.num_kv_heads, page_size,
+            dt)
+    if metadata.shared_prefix is None:
+        handle = lib().mi355x_prefill_prepare(*args, stream_of(cu))
+    else:
+        from .backend import shared_arrays
+        group_rows, group_lens = shared_arrays(metadata.shared_prefix, b)
+        handle = lib().mi355x_prefill_prepare_shared(*args, group_rows.ctypes.data,
+                                                     group_lens.ctypes.data, group_rows.size,
+                                                     stream_of(cu))
     if not handle:
         raise ModelError(f"mi355x prefill plan failed: {last_error()}")
     plan = existing if existing is not None else PrefillPlan(handle)

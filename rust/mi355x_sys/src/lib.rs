@@ -34,6 +34,12 @@ unsafe extern "C" {
         columns: i64, table_stride: i64, seq_lens: *const i32, num_q_heads: i64,
         num_kv_heads: i64, head_dim: i64, page_size: i64, dtype: i64, graph: bool,
         host_lengths: *const i32, host_rows: i64, stream: *mut c_void) -> *mut c_void;
+    pub fn mi355x_decode_prepare_shared(existing: *mut c_void, block_table: *const i32,
+        batch: i64, columns: i64, table_stride: i64, seq_lens: *const i32, num_q_heads: i64,
+        num_kv_heads: i64, head_dim: i64, page_size: i64, dtype: i64, graph: bool,
+        host_lengths: *const i32, host_rows: i64, group_rows: *const i32,
+        group_lens: *const i32, groups: i64, stream: *mut c_void) -> *mut c_void;
+    pub fn mi355x_decode_plan_shared_info(plan: *const c_void, out4: *mut i64) -> *const c_char;
     pub fn mi355x_decode_run(plan: *const c_void, q: *const c_void, q_sn: i64, q_sh: i64,
         k_cache: *const c_void, v_cache: *const c_void, out: *mut c_void, o_sn: i64, o_sh: i64,
         batch: i64, num_q_heads: i64, num_kv_heads: i64, page_size: i64, dtype: i64,
@@ -44,6 +50,12 @@ unsafe extern "C" {
         block_table: *const i32, batch: i64, columns: i64, table_stride: i64,
         q_host: *const i32, prefix_host: *const i32, num_q_heads: i64, num_kv_heads: i64,
         page_size: i64, dtype: i64, stream: *mut c_void) -> *mut c_void;
+    pub fn mi355x_prefill_prepare_shared(existing: *mut c_void, q_indptr: *const i32,
+        block_table: *const i32, batch: i64, columns: i64, table_stride: i64,
+        q_host: *const i32, prefix_host: *const i32, num_q_heads: i64, num_kv_heads: i64,
+        page_size: i64, dtype: i64, group_rows: *const i32, group_lens: *const i32,
+        groups: i64, stream: *mut c_void) -> *mut c_void;
+    pub fn mi355x_prefill_plan_shared_info(plan: *const c_void, out4: *mut i64) -> *const c_char;
     pub fn mi355x_prefill_run(plan: *const c_void, q: *const c_void, q_sn: i64, q_sh: i64,
         k: *const c_void, k_sn: i64, k_sh: i64, v: *const c_void, v_sn: i64, v_sh: i64,
         out: *mut c_void, o_sn: i64, o_sh: i64, total_q: i64, num_q_heads: i64,

@@ -1,0 +1,249 @@
+"""Attention over prefixes that rows of a batch share, decode and several new tokens a row."""
+import gc
+
+import numpy as np
+import pytest
+import torch
+
+from llm_infer_rust_amd.backend import (AttentionMetadata, BatchPhase, DecodeHostMetadata,
+                                        ModelError, SharedPrefix)
+from shared_helpers import Batch
+
+pytestmark = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def own_lengths(rows, low, high, seed=0):
+    return np.random.default_rng(seed).integers(low, high + 1, rows).tolist()
+
+
+DECODE = [
+    # groups (rows, shared), longest own part, heads, kv heads, page, type
+    ([(4, 1100)], 150, 32, 8, 16, BF16),
+    ([(2, 64)], 1, 16, 8, 16, BF16),
+    ([(2, 65)], 1, 16, 8, 1, FP16),
+    ([(3, 63)], 70, 16, 8, 16, BF16),
+    ([(1, 500), (2, 128), (1, 9), (5, 700)], 90, 16, 8, 13, BF16),
+    ([(40, 1000)], 300, 32, 8, 16, FP16),
+    ([(70, 640)], 40, 64, 8, 64, BF16),
+    ([(33, 333), (17, 777), (3, 2000)], 100, 8, 8, 24, BF16),
+    ([(9, 4000)], 60, 8, 1, 16, BF16),
+    ([(9, 900)], 60, 6, 3, 8, FP16),
+    ([(20, 512)], 200, 16, 4, 128, BF16),
+    ([(130, 256)], 20, 4, 2, 16, BF16),
+    ([(65, 1500)], 33, 16, 16, 16, FP16),
+    ([(256, 192)], 5, 32, 8, 16, BF16),
+    ([(6, 300)] * 12, 64, 32, 4, 16, BF16),
+]
+
+
+@pytest.mark.parametrize("groups,own,heads,kv_heads,page,dtype", DECODE)
+@pytest.mark.parametrize("copies", [False, True])
+def test_decode(gpu, groups, own, heads, kv_heads, page, dtype, copies):
+    rows = sum(r for r, _ in groups)
+    b = Batch(groups, own_lengths(rows, 1, own), None, heads, kv_heads, page, dtype,
+              seed=rows + own, copies=copies)
+    got, info = b.run(b.decode_meta())
+    print(f"[shared] {info} worst {b.check(got):.2f} of the limit", flush=True)
+    plain, none = b.run(b.decode_meta(shared=False))
+    assert none["waves"] == 0
+    b.check(plain)
+
+
+EXTEND = [
+    ([(5, 700)], 0, 40, 32, 8, 16, BF16),
+    ([(48, 1024)], 0, 40, 32, 8, 16, BF16),
+    ([(7, 300), (1, 100), (4, 64), (3, 63)], 90, 7, 16, 8, 16, FP16),
+    ([(2, 128)], 5, 1, 16, 8, 1, BF16),
+    ([(3, 1000)], 300, 260, 32, 8, 13, BF16),
+    ([(20, 640)], 70, 5, 64, 8, 64, BF16),
+    ([(9, 500)], 20, 33, 8, 8, 24, BF16),
+    ([(4, 200)], 10, 70, 8, 1, 8, FP16),
+    ([(6, 333)] * 5, 64, 9, 6, 3, 128, BF16),
+]
+
+
+@pytest.mark.parametrize("groups,own,new,heads,kv_heads,page,dtype", EXTEND)
+def test_extend(gpu, groups, own, new, heads, kv_heads, page, dtype):
+    rows = sum(r for r, _ in groups)
+    fresh = own_lengths(rows, 1, new, seed=1)
+    cached = own_lengths(rows, 0, own, seed=2)
+    b = Batch(groups, [t + c for t, c in zip(fresh, cached)], fresh, heads, kv_heads, page, dtype,
+              seed=rows + new)
+    got, info = b.run(b.extend_meta())
+    print(f"[shared] {info} worst {b.check(got):.2f} of the limit", flush=True)
+    assert info["groups"] == sum(r > 1 and n >= 64 for r, n in groups)
+    plain, none = b.run(b.extend_meta(shared=False))
+    assert none["waves"] == 0
+    b.check(plain)
+
+
+def test_whole_request_is_shared(gpu):
+    """A group's lens may cover every token: the last ones are then each row's own."""
+    b = Batch([(3, 128), (2, 64), (2, 40)], [0] * 7, [1] * 7)
+    got, info = b.run(b.decode_meta())
+    b.check(got)
+    assert info["tokens"] in (0, 64)  # 127 and 63 tokens that may be shared
+
+
+def test_strided_queries_and_output(gpu):
+    b = Batch([(6, 400)], own_lengths(6, 1, 50), heads=16, kv_heads=8)
+    packed = torch.randn(6, 32 * 128, device="cuda").to(BF16)
+    packed[:, :16 * 128] = b.q.view(6, -1)
+    attention, q = b.attention(), packed[:, :16 * 128].view(6, 16, 128)
+    batch = attention.prepare(b.decode_meta(), 6)
+    assert batch.plan.plan.shared_info()["waves"]
+    out = torch.full((7, 16 * 128), 7.0, dtype=BF16, device="cuda")
+    batch.forward_into(q, None, None, b.cache(), out[:6])
+    b.check(out[:6].view(6, 16, 128))
+    assert bool((out[6] == 7).all())  # rows behind the last are left as they were
+
+
+def test_sharp_scores(gpu):
+    """Scores far apart: one key of the prefix or of the own part takes all the weight."""
+    for scale in (8.0, 60.0):
+        b = Batch([(5, 300), (2, 700)], own_lengths(7, 1, 90), heads=32, kv_heads=8, q_scale=scale)
+        want, mass = b.reference()
+        for meta in (b.decode_meta(), b.decode_meta(shared=False)):
+            got, _ = b.run(meta)
+            assert bool(torch.isfinite(got).all())
+            # sum |q k| / sqrt(128) is at most 200 * scale: its fp32 rounding moves a score by 128 *
+            # 2^-24 of that at the very most, and the output by as much of 2 |v|, |v| below 6
+            limit = 2 ** -7 * mass + 2 ** -8 * want.abs() + 200 * scale * 128 * 2 ** -24 * 12
+            assert bool(((got.double() - want).abs() <= limit).all())
+
+
+def test_nan_of_one_row_stays_there(gpu):
+    """A NaN among a row's own keys reaches that row only; one in the prefix all of its group."""
+    b = Batch([(4, 256), (3, 128)], [20] * 7, heads=16, kv_heads=8)
+    flat = b.k.view(-1, 8, 128)
+    flat[b.slots[2][270]] = float("nan")
+    got, info = b.run(b.decode_meta())
+    assert info["waves"]
+    bad = torch.isnan(got.float()).flatten(1).any(1).tolist()
+    assert bad == [False, False, True, False, False, False, False]
+    flat[b.slots[4][100]] = float("nan")
+    got, _ = b.run(b.decode_meta())
+    assert torch.isnan(got.float()).flatten(1).any(1).tolist() == [False, False, True, False, True,
+                                                                   True, True]
+
+
+def test_same_bits_every_time(gpu):
+    b = Batch([(40, 1000), (3, 500)], own_lengths(43, 1, 300), heads=32, kv_heads=8)
+    attention = b.attention()
+    first, _ = b.run(b.decode_meta(), attention)
+    for _ in range(4):
+        again, _ = b.run(b.decode_meta(), attention)
+        assert torch.equal(first, again)
+
+
+def test_offsets_past_4_gib(gpu):
+    """Pages whose slots lie past 2^31 elements of the cache."""
+    b = Batch([(4, 300)], [30] * 4, heads=32, kv_heads=8)
+    far = (2 ** 32 // (16 * 8 * 128)) + 5
+    pages = b.k.size(0)
+    for name in ("k", "v"):
+        big = torch.zeros(far + pages, 16, 8, 128, dtype=BF16, device="cuda")
+        big[far:] = getattr(b, name)
+        setattr(b, name, big)
+    b.table[b.table >= 0] += far
+    b.slots = [s + far * 16 for s in b.slots]
+    got, info = b.run(b.decode_meta())
+    assert info["waves"]
+    b.check(got)
+
+
+def test_one_plan_with_and_without_groups(gpu):
+    """An eager backend re-plans the same handle; what an earlier batch shared is forgotten."""
+    shapes = [([(40, 600)], 50), ([(2, 900)], 20), ([(1, 70), (1, 30)], 9), ([(130, 128)], 3)]
+    batches = [Batch(g, own_lengths(sum(r for r, _ in g), 1, own), heads=16, kv_heads=8, seed=i)
+               for i, (g, own) in enumerate(shapes)]
+    attention = batches[0].attention()
+    for b in batches + batches[::-1]:
+        for shared in (True, False):
+            got, _ = b.run(b.decode_meta(shared), attention)
+            b.check(got)
+            got, _ = b.run(b.extend_meta(shared), attention)
+            b.check(got)
+
+
+def test_streams(gpu):
+    b = Batch([(12, 700)], own_lengths(12, 1, 90), heads=32, kv_heads=8)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got, _ = b.run(b.decode_meta())
+    torch.cuda.current_stream().wait_stream(side)
+    b.check(got)
+
+
+@pytest.mark.parametrize("rows,heads", [(6, 32), (64, 32)])
+def test_graph(gpu, rows, heads):
+    """One captured launch serves any groups, also none; replays are checked one by one."""
+    cols = 80
+    table = torch.zeros(rows, cols, dtype=torch.int32, device="cuda")
+    lens = torch.ones(rows, dtype=torch.int32, device="cuda")
+    kinds = [[(rows, 500)], [(1, 100)] * rows, [(rows // 2, 640), (rows - rows // 2, 64)],
+             [(2, 300)] * (rows // 2), [(rows, 0)], [(rows, 1000)]]
+    batches = [Batch(g, own_lengths(rows, 1, 60, seed=i), heads=heads, kv_heads=8, seed=i)
+               for i, g in enumerate(kinds)]
+    pages = max(b.k.size(0) for b in batches)
+    k, v = (torch.zeros(pages, 16, 8, 128, dtype=BF16, device="cuda") for _ in range(2))
+    q = torch.zeros(rows, heads, 128, dtype=BF16, device="cuda")
+    attention, cache = batches[0].attention(), batches[0].cache()
+    cache.bind_kv_cache(k, v)
+    meta = AttentionMetadata(BatchPhase.DECODE, block_table=table, cache_seqlens=lens,
+                             shared_prefix=SharedPrefix([rows], [0]))
+    state = attention.prepare_decode_graph(meta)
+    batch = attention.prepare(meta, rows)
+    out = torch.zeros(rows, heads * 128, dtype=BF16, device="cuda")
+    batch.forward_into(q, None, None, cache, out)
+    torch.cuda.synchronize()
+    gc.collect()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        batch.forward_into(q, None, None, cache, out)
+    for b in batches + batches[::-1]:
+        k[:b.k.size(0)] = b.k
+        v[:b.v.size(0)] = b.v
+        q.copy_(b.q)
+        table.fill_(-1)
+        table[:, :b.table.size(1)] = b.table
+        lens.copy_(b.lens)
+        state.prepare_replay(DecodeHostMetadata(b.keys), b.shared())
+        graph.replay()
+        torch.cuda.synchronize()
+        b.check(out.view(rows, heads, 128))
+        state.prepare_replay(DecodeHostMetadata(b.keys))  # and without its groups
+        graph.replay()
+        torch.cuda.synchronize()
+        b.check(out.view(rows, heads, 128))
+
+
+def test_graph_prepared_without_groups_ignores_them(gpu):
+    b = Batch([(4, 200)], [10] * 4)
+    attention = b.attention()
+    meta = b.decode_meta(shared=False)
+    state = attention.prepare_decode_graph(meta)
+    batch = attention.prepare(meta, 4)
+    state.prepare_replay(DecodeHostMetadata(b.keys), b.shared())
+    assert state.plan.shared_info()["waves"] == 0
+    b.check(batch.forward(b.q, None, None, b.cache()).view(b.q.shape))
+
+
+def test_refusals(gpu):
+    b = Batch([(4, 200)], [10] * 4)
+    attention = b.attention()
+    for rows, lens in (([4], [211]), ([3], [200]), ([5], [200]), ([4], [-1]), ([2, 2], [200]),
+                       ([0, 4], [0, 1]), ([], []), ([4.0], [200]), ([4], [2 ** 40])):
+        for meta in (b.decode_meta(), b.extend_meta()):
+            meta.shared_prefix = SharedPrefix(rows, lens)
+            with pytest.raises(ModelError):
+                attention.prepare(meta, 4)
+                pytest.fail(f"{rows} {lens} {meta.forward_mode}")
+    meta = b.extend_meta()
+    meta.shared_prefix = SharedPrefix([4], [210])  # of the 209 cached tokens
+    with pytest.raises(ModelError):
+        attention.prepare(meta, 4)
+    got, _ = b.run(b.decode_meta(), attention)  # the backend is still usable
+    b.check(got)
