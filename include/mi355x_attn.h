@@ -123,8 +123,9 @@ void* mi355x_decode_prepare_shared(void* existing, const int32_t* block_table, i
                                    const int32_t* group_rows, const int32_t* group_lens,
                                    int64_t groups, void* stream);
 
-/* out4 = {groups whose prefix is computed once, tokens of those prefixes, work items of that launch,
- * waves of its workgroups (0: no such launch)}. Introspection. */
+/* out4 = {groups whose prefix is computed once, tokens of those prefixes, work items over them (0: the
+ * plain kernels run), those among all items that are matrix products of many query rows}.
+ * Introspection. */
 const char* mi355x_decode_plan_shared_info(const void* plan, int64_t* out4);
 
 /* out[b, h, :] = softmax(q[b,h] K^T / sqrt(128)) V over the request's pages.

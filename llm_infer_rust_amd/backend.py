@@ -166,11 +166,11 @@ def prefill_boundaries(metadata: AttentionMetadata, total_tokens: int) -> list[i
 # Native plans
 # ---------------------------------------------------------------------------
 def shared_info(entry: str, handle: int) -> dict[str, int]:
-    """What a plan makes of shared prefixes: groups and tokens computed once, work items of that
-    launch and waves of its workgroups (0: no such launch)."""
+    """What a plan makes of shared prefixes: groups and tokens computed once, work items over them
+    (0: the plain kernels run) and how many of all items are products of many query rows."""
     buf = (ctypes.c_int64 * 4)()
     check(getattr(lib(), entry)(handle, buf), "shared prefix info")
-    return dict(zip(("groups", "tokens", "items", "waves"), list(buf)))
+    return dict(zip(("groups", "tokens", "items", "products"), list(buf)))
 
 
 def shared_arrays(shared: SharedPrefix, batch: int) -> tuple[np.ndarray, np.ndarray]:

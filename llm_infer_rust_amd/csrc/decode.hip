@@ -128,7 +128,6 @@ struct DeviceBuffer {
 //   [o_work, +4*cap)     work items {request, token_begin, token_end, partial}
 //   [o_merge, +2*B)      per-request {first partial, chunk count}
 //   [o_wg, +wgs+1)       first work item of each workgroup
-//   [o_shared, ...)      shared prefixes: header, kSharedInfoInts per request, work items
 //   [o_wgrec, +32*cap)   per-workgroup start record (kWgRec ints, 128-byte aligned):
 //                        {first item, item end, request, token_begin, token_end,
 //                         partial, page base, 0} of its first item, then the KV slots
@@ -137,15 +136,14 @@ constexpr int kWgRec = 32;
 constexpr int kWgRecSlots = 8;  // offset of the slots within a record
 static_assert(kWgRecSlots + kDmaTile <= kWgRec, "a start record holds one tile's slots");
 struct IntLayout {
-  int64_t o_indptr, o_work, o_merge, o_wg, o_shared, o_wgrec, total;
-  static IntLayout make(int64_t rows, int64_t items_cap, int64_t wg_cap, int64_t shared_ints) {
+  int64_t o_indptr, o_work, o_merge, o_wg, o_wgrec, total;
+  static IntLayout make(int64_t rows, int64_t items_cap, int64_t wg_cap) {
     IntLayout l{};
     l.o_indptr = kHeaderInts;
     l.o_work = (l.o_indptr + rows + 1 + 3) / 4 * 4;
     l.o_merge = l.o_work + 4 * items_cap;
     l.o_wg = l.o_merge + 2 * rows;
-    l.o_shared = (l.o_wg + wg_cap + 1 + 3) / 4 * 4;
-    l.o_wgrec = (l.o_shared + shared_ints + kWgRec - 1) / kWgRec * kWgRec;
+    l.o_wgrec = (l.o_wg + wg_cap + 1 + kWgRec - 1) / kWgRec * kWgRec;
     l.total = l.o_wgrec + kWgRec * wg_cap;
     return l;
   }
@@ -162,15 +160,13 @@ struct DecodePlan {
   int64_t batch = 0, total_pages = 0, num_items = 0, chunk_tokens = 0, items_capacity = 0;
   int64_t num_wgs = 0, wg_capacity = 0, num_long = 0;
   int64_t cus = 0;
-  // Shared prefixes: waves of a workgroup (0: the plan computes none), workgroups, work items,
-  // groups that share and the tokens they share. A graph plan prepared with groups keeps room for
-  // any (shared_graph) and launches the same grid whether some share or not.
-  int shared_nw = 0;
-  bool shared_graph = false;
-  int64_t shared_grid = 0, shared_items = 0, shared_groups = 0, shared_tokens = 0;
   IntLayout layout{};
-  DeviceBuffer ints, indices, last_len, partial_o, partial_lse, shared_o, shared_lse;
+  DeviceBuffer ints, indices, last_len, partial_o, partial_lse;
   DeviceBuffer staging;
+  // Shared prefixes: their plan runs instead of this one's work list. A graph plan prepared with
+  // groups always runs it, whatever later batches share.
+  std::unique_ptr<SharedPlan> shared;
+  bool shared_runs = false, shared_graph = false;
   hipEvent_t upload_done = nullptr;
   uint64_t allocations = 0;
   std::vector<int32_t> host_lengths;
@@ -281,6 +277,8 @@ int64_t items_capacity_for(const LaunchShape& s, int64_t rows, int64_t row_token
   return s.wg_capacity + rows * (1 + (row_tokens + s.max_item - 1) / s.max_item);
 }
 
+}  // namespace
+
 // Balanced split-KV ("stream-K" over the flattened tile list): the workgroups of the
 // grid each take an equal share of the batch's work, walking the requests in order. Work
 // is counted in the kernel's tiles (`tile` tokens; a request's last tile may be partial)
@@ -295,13 +293,9 @@ int64_t items_capacity_for(const LaunchShape& s, int64_t rows, int64_t row_token
 // Fills work (4 ints per item), merge (2 ints per request) and, when wg is not NULL,
 // wg[i] = first item of workgroup i (wg[workgroups] = item count). Returns the item
 // count, or -1 when a capacity is too small.
-// `shared` (NULL: none): leading tokens of each request that are computed elsewhere. lengths[r] are
-// then the tokens behind them, items' ranges start there, and a request with some has partials
-// even when one item holds it.
 int64_t schedule(const int32_t* lengths, int64_t batch, int64_t workgroups, int64_t max_item,
                  int64_t tile, bool graph, int32_t* work, int64_t capacity, int32_t* merge,
-                 int64_t* share_out, int32_t* wg = nullptr, int64_t wg_capacity = 0,
-                 int64_t* wgs_out = nullptr, const int32_t* shared = nullptr) {
+                 int64_t* share_out, int32_t* wg, int64_t wg_capacity, int64_t* wgs_out) {
   constexpr int64_t kUnit = 8;  // cost units per tile
   // An item's prologue in cost units: 9/8 of a tile, as measured (per-workgroup end
   // times at configs 2 and 5 fit 2.5-2.6 us per tile + 2.4-2.9 us per item). With it,
@@ -477,22 +471,19 @@ int64_t schedule(const int32_t* lengths, int64_t batch, int64_t workgroups, int6
     const int32_t req = work[4 * i];
     int64_t n = 0;
     while (i + n < items && work[4 * (i + n)] == req) ++n;
-    const int32_t before = shared ? shared[req] : 0;
-    const bool joined = n > 1 || before > 0;
-    merge[2 * req] = static_cast<int32_t>(joined ? partials : -1);
+    merge[2 * req] = static_cast<int32_t>(n > 1 ? partials : -1);
     merge[2 * req + 1] = static_cast<int32_t>(n);
-    for (int64_t c = 0; c < n; ++c) {
-      work[4 * (i + c) + 1] += before;
-      work[4 * (i + c) + 2] += before;
-      work[4 * (i + c) + 3] = static_cast<int32_t>(joined ? partials + c : -1);
-    }
-    if (joined) partials += n;
+    for (int64_t c = 0; c < n; ++c)
+      work[4 * (i + c) + 3] = static_cast<int32_t>(n > 1 ? partials + c : -1);
+    if (n > 1) partials += n;
     i += n;
   }
   *share_out = share / kUnit * tile;
   if (wgs_out) *wgs_out = wgs;
   return items;
 }
+
+namespace {
 
 // ---------------------------------------------------------------------------
 // Page metadata pack: one workgroup per request.
@@ -1512,84 +1503,36 @@ static void* prepare_decode(void* existing, const int32_t* block_table, int64_t 
       }
     }
 
-    // Shared prefixes: what of them is computed once (whole tiles, at least one own token left), as
-    // sources of query rows against the pages of their group's first row. `own`: tokens behind.
-    std::vector<int32_t> own, before(batch, 0), eff;
-    std::vector<SharedSource> sources;
-    std::vector<int32_t> source_of(batch, -1), shared_work;
-    int64_t shared_tokens = 0;
-    if (groups > 0) {
-      int64_t rows = 0;
-      for (int64_t g = 0; g < groups; ++g) {
-        if (group_rows[g] <= 0 || group_lens[g] < 0 || group_rows[g] > batch - rows) {
-          set_error("invalid shared prefix groups");
-          return nullptr;
-        }
-        for (int64_t r = rows; r < rows + group_rows[g]; ++r)
-          if (group_lens[g] > plan->host_lengths[r]) {
-            set_error("shared prefix is longer than a row of its group");
-            return nullptr;
-          }
-        rows += group_rows[g];
-      }
-      if (rows != batch) {
-        set_error("invalid shared prefix groups");
-        return nullptr;
-      }
-      std::vector<int32_t> limit(plan->host_lengths);
-      for (int32_t& n : limit) --n;
-      if ((!graph || plan->shared_graph) &&
-          shared_lengths(group_rows, group_lens, groups, limit.data(), num_kv_heads, eff)) {
-        int64_t row = 0, page = 0;
-        for (int64_t g = 0; g < groups; ++g) {
-          if (eff[g] > 0) {
-            sources.push_back({static_cast<int32_t>(row), group_rows[g],
-                               static_cast<int32_t>(page), 0, eff[g] / kSharedTile, kNoHorizon,
-                               eff[g], 0, 0, 0});
-            shared_tokens += eff[g];
-          }
-          for (int64_t r = row; r < row + group_rows[g]; ++r) {
-            before[r] = eff[g];
-            if (eff[g] > 0) source_of[r] = static_cast<int32_t>(sources.size() - 1);
-            page += (plan->host_lengths[r] + page_size - 1) / page_size;
-          }
-          row += group_rows[g];
-        }
-      }
+    // Shared prefixes: checked always, computed once where a plan of their own does better.
+    std::vector<int32_t> first_page(batch + 1, 0), first_token(batch + 1);
+    for (int64_t r = 0; r < batch; ++r) {
+      first_token[r + 1] = static_cast<int32_t>(r + 1);
+      first_page[r + 1] = first_page[r] + static_cast<int32_t>(
+                                              (plan->host_lengths[r] + page_size - 1) / page_size);
     }
-    own = plan->host_lengths;
-    for (int64_t r = 0; r < batch; ++r) own[r] -= before[r];
-    const int64_t heads_per_kv = num_q_heads / num_kv_heads;
-    int shared_nw = 0;
-    int64_t shared_records = 0;
-    SharedCapacity shared_cap{0, 0};
-    if (plan->shared_graph) {  // one shape for whatever the rows will share
-      shared_nw = batch * heads_per_kv > 128 ? 8 : 4;
-      shared_cap = shared_decode_capacity(batch, heads_per_kv, num_kv_heads, plan->cus, shared_nw);
-    } else if (!sources.empty()) {
-      shared_nw = shared_waves(sources, heads_per_kv);
-      shared_cap = shared_capacity(sources, heads_per_kv, num_kv_heads, plan->cus, shared_nw);
-    }
-    if (!sources.empty())
-      shared_records = schedule_shared(sources, heads_per_kv, num_kv_heads, plan->cus, shared_nw,
-                                       shared_cap, shared_work);
-    const int64_t shared_items = static_cast<int64_t>(shared_work.size()) / kSharedItemInts;
-    if (shared_items > shared_cap.items || shared_records > shared_cap.records) {
-      set_error("shared prefix work list exceeds its capacity");
+    if (const char* err = groups > 0
+                              ? check_groups(group_rows, group_lens, groups, batch,
+                                             plan->host_lengths.data(),
+                                             "shared prefix is longer than a row of its group")
+                              : nullptr) {
+      set_error(err);
       return nullptr;
     }
-    const int64_t shared_ints =
-        shared_nw ? kSharedHeaderInts + kSharedInfoInts * batch +
-                        kSharedItemInts * (graph ? shared_cap.items : shared_items)
-                  : 0;
-    const int64_t shared_room = graph ? shared_cap.records : shared_records;
+    const SharedBatch sharing{batch,      first_token.data(), plan->host_lengths.data(),
+                              first_page.data(), group_rows,  group_lens,
+                              groups};
+    if ((groups > 0 || plan->shared_graph) && !plan->shared)
+      plan->shared = std::make_unique<SharedPlan>(plan->cus, num_q_heads, num_kv_heads, page_size,
+                                                  dtype);
+    const bool shared_runs =
+        plan->shared_graph || (!graph && groups > 0 && plan->shared->pays(sharing));
 
     const LaunchShape shape = launch_shape(plan->cus, num_kv_heads, page_size);
     const int64_t items_cap = items_capacity_for(shape, batch, columns * page_size);
     const int64_t wg_cap = shape.wg_capacity;
-    const IntLayout layout = IntLayout::make(batch, items_cap, wg_cap, shared_ints);
+    const IntLayout layout = IntLayout::make(batch, items_cap, wg_cap);
     const size_t int_bytes = layout.total * sizeof(int32_t);
-    // Three entries behind the last page: the shared kernel reads four at a time.
+    // Three entries behind the last page: the shared prefixes' kernel reads four at a time.
     const size_t idx_bytes = (static_cast<size_t>(batch) * columns + 3) * sizeof(int32_t);
     const size_t part_o_bytes = static_cast<size_t>(items_cap) * num_q_heads * kHeadDim * 4;
     const size_t part_lse_bytes = static_cast<size_t>(items_cap) * num_q_heads * 4;
@@ -1611,10 +1554,6 @@ static void* prepare_decode(void* existing, const int32_t* block_table, int64_t 
         (st = plan->last_len.reserve(last_bytes, plan->allocations)) != hipSuccess ||
         (st = plan->partial_o.reserve(part_o_bytes, plan->allocations)) != hipSuccess ||
         (st = plan->partial_lse.reserve(part_lse_bytes, plan->allocations)) != hipSuccess ||
-        (shared_room && (st = plan->shared_o.reserve(shared_room * kSharedRecord * 4,
-                                                     plan->allocations)) != hipSuccess) ||
-        (shared_room &&
-         (st = plan->shared_lse.reserve(shared_room * 32 * 4, plan->allocations)) != hipSuccess) ||
         (st = plan->staging.reserve(int_bytes, plan->allocations)) != hipSuccess) {
       hip_error(st, "decode workspace allocation");
       return nullptr;
@@ -1624,15 +1563,12 @@ static void* prepare_decode(void* existing, const int32_t* block_table, int64_t 
     // launched are written in full below (those past them are never read).
     std::memset(host, 0, layout.o_wgrec * sizeof(int32_t));
     int32_t* indptr = host + layout.o_indptr;
-    indptr[0] = 0;
-    for (int64_t r = 0; r < batch; ++r)
-      indptr[r + 1] = indptr[r] + static_cast<int32_t>(
-                                      (plan->host_lengths[r] + page_size - 1) / page_size);
+    std::copy(first_page.begin(), first_page.end(), indptr);
     int64_t chunk = 0, wgs = 0;
-    const int64_t items = schedule(own.data(), batch, shape.workgroups, shape.max_item, shape.tile,
-                                   graph, host + layout.o_work, items_cap, host + layout.o_merge,
-                                   &chunk, host + layout.o_wg, wg_cap, &wgs,
-                                   sources.empty() ? nullptr : before.data());
+    const int64_t items = shared_runs ? 0 : schedule(plan->host_lengths.data(), batch, shape.workgroups,
+                                   shape.max_item, shape.tile, graph, host + layout.o_work,
+                                   items_cap, host + layout.o_merge, &chunk, host + layout.o_wg,
+                                   wg_cap, &wgs);
     if (items < 0) {
       set_error("decode work list exceeds its capacity");
       return nullptr;
@@ -1640,7 +1576,7 @@ static void* prepare_decode(void* existing, const int32_t* block_table, int64_t 
     host[0] = static_cast<int32_t>(wgs);
     host[1] = static_cast<int32_t>(items);
     int64_t tokens = 0;
-    for (int64_t r = 0; r < batch; ++r) tokens += own[r];
+    for (int64_t r = 0; r < batch; ++r) tokens += plan->host_lengths[r];
     host[2] = tokens * num_kv_heads * kHeadDim * 4 >= kOnceBytes;
     // Requests that the merge gives four waves a head: those of more than kLongChunks chunks, or
     // of twice as many as often as it takes to fit the list (a batch of very long requests).
@@ -1658,21 +1594,6 @@ static void* prepare_decode(void* existing, const int32_t* block_table, int64_t 
       }
     }
     host[4] = static_cast<int32_t>(longs);
-    if (!sources.empty()) {  // the whole section is zero otherwise
-      int32_t* section = host + layout.o_shared;
-      section[0] = static_cast<int32_t>(shared_items);
-      for (int64_t r = 0; r < batch; ++r) {
-        if (source_of[r] < 0) continue;
-        const SharedSource& src = sources[source_of[r]];
-        int32_t* info = section + kSharedHeaderInts + kSharedInfoInts * r;
-        info[0] = src.record;
-        info[1] = src.splits;
-        info[2] = src.row_tiles;
-        info[3] = src.token0;
-      }
-      std::memcpy(section + kSharedHeaderInts + kSharedInfoInts * batch, shared_work.data(),
-                  shared_work.size() * sizeof(int32_t));
-    }
     // Start records: the first item of each workgroup and the page-entry index of its
     // first token (pack_page_metadata fills the slots from the block table).
     for (int64_t w = 0; w < wgs; ++w) {
@@ -1711,6 +1632,10 @@ static void* prepare_decode(void* existing, const int32_t* block_table, int64_t 
       hip_error(st, "decode upload event");
       return nullptr;
     }
+    if (shared_runs && !plan->shared->prepare(sharing, graph ? batch : 0, columns * page_size,
+                                              plan->allocations, s))
+      return nullptr;
+    plan->shared_runs = shared_runs;
     plan->batch = batch;
     plan->total_pages = total_pages;
     plan->num_items = items;
@@ -1719,11 +1644,6 @@ static void* prepare_decode(void* existing, const int32_t* block_table, int64_t 
     plan->num_wgs = wgs;
     plan->num_long = longs;
     plan->wg_capacity = wg_cap;
-    plan->shared_nw = shared_nw;
-    plan->shared_grid = graph ? (shared_nw == 8 ? plan->cus : 2 * plan->cus) : shared_items;
-    plan->shared_items = shared_items;
-    plan->shared_groups = static_cast<int64_t>(sources.size());
-    plan->shared_tokens = shared_tokens;
     plan->layout = layout;
     created.release();
     return plan;
@@ -1762,10 +1682,8 @@ extern "C" void* mi355x_decode_prepare_shared(
 extern "C" const char* mi355x_decode_plan_shared_info(const void* plan, int64_t* out4) {
   if (!plan || !out4) return set_error("mi355x_decode_plan_shared_info: null argument");
   const auto* p = static_cast<const DecodePlan*>(plan);
-  out4[0] = p->shared_groups;
-  out4[1] = p->shared_tokens;
-  out4[2] = p->shared_items;
-  out4[3] = p->shared_nw;
+  std::fill(out4, out4 + 4, 0);
+  if (p->shared_runs) p->shared->info(out4);
   return nullptr;
 }
 
@@ -1829,6 +1747,10 @@ extern "C" const char* mi355x_decode_run(const void* plan_ptr, const void* q, in
   if (q_stride_h % 8 || q_stride_n % 8 || out_stride_h % 8 || out_stride_n % 8 ||
       !aligned(q, 16) || !aligned(out, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16))
     return set_error("decode requires 16-byte aligned rows");
+  if (p.shared_runs)
+    return p.shared->run(static_cast<const int32_t*>(p.indices.ptr), q, q_stride_n, q_stride_h,
+                         k_cache, v_cache, out, out_stride_n, out_stride_h,
+                         static_cast<hipStream_t>(stream));
   DecodeArgs a{};
   a.q = static_cast<const uint16_t*>(q);
   a.q_stride_n = q_stride_n;
@@ -1859,25 +1781,6 @@ extern "C" const char* mi355x_decode_run(const void* plan_ptr, const void* q, in
   const dim3 grid(static_cast<uint32_t>(grid_x), static_cast<uint32_t>(shape.grid_y));
   const int group = static_cast<int>(num_q_heads / num_kv_heads);
   auto s = static_cast<hipStream_t>(stream);
-  const int32_t* section = a.ints + p.layout.o_shared;
-  if (p.shared_nw) {
-    SharedArgs sa{};
-    sa.q = a.q;
-    sa.q_sn = q_stride_n;
-    sa.q_sh = q_stride_h;
-    sa.k = a.k_cache;
-    sa.v = a.v_cache;
-    sa.header = section;
-    sa.work = reinterpret_cast<const int4*>(section + kSharedHeaderInts + kSharedInfoInts * p.batch);
-    sa.indices = a.indices;
-    sa.part_o = static_cast<float*>(p.shared_o.ptr);
-    sa.part_lse = static_cast<float*>(p.shared_lse.ptr);
-    sa.group = group;
-    sa.num_kv_heads = a.num_kv_heads;
-    sa.page_size = a.page_size;
-    sa.scale_log2 = a.scale_log2;
-    if (const char* err = launch_shared(sa, dtype, p.shared_nw, p.shared_grid, s)) return err;
-  }
   const bool ok =
       shape.dma
           ? (dtype == 0 ? dispatch_dma<0>(a, group, grid, waves, s)
@@ -1886,23 +1789,6 @@ extern "C" const char* mi355x_decode_run(const void* plan_ptr, const void* q, in
                         : dispatch_group<1>(a, group, grid, waves, page_size == 1, s));
   if (!ok) return set_error("unsupported query group size");
   if (const char* err = launch_status("decode_kernel")) return err;
-  if (p.shared_nw) {
-    SharedMergeArgs m{};
-    m.out = a.out;
-    m.o_sn = out_stride_n;
-    m.o_sh = out_stride_h;
-    m.rows = batch * num_q_heads;
-    m.info = reinterpret_cast<const int4*>(section + kSharedHeaderInts);
-    m.part_o = static_cast<const float*>(p.shared_o.ptr);
-    m.part_lse = static_cast<const float*>(p.shared_lse.ptr);
-    m.own_merge = a.ints + a.o_merge;
-    m.own_o = a.partial_o;
-    m.own_lse = a.partial_lse;
-    m.num_q_heads = a.num_q_heads;
-    m.group = group;
-    m.num_kv_heads = a.num_kv_heads;
-    return launch_shared_merge(m, dtype, s);
-  }
   if (p.graph || p.num_items > p.batch) {  // some request was split
     const int64_t long_slots = p.graph ? kLongSlots : p.num_long;
     if (dtype == 0)

@@ -32,6 +32,7 @@
 #include <memory>
 #include <vector>
 
+#include "buffer.h"
 #include "common.h"
 #include "mfma.h"
 #include "shared.h"
@@ -528,36 +529,6 @@ __global__ __launch_bounds__(256) void pack_prefill_pages(const int32_t* __restr
   for (int c = threadIdx.x; c < pages; c += blockDim.x) indices[begin + c] = src[c];
 }
 
-struct Buffer {
-  void* ptr = nullptr;
-  size_t capacity = 0;
-  bool pinned = false;
-  hipError_t reserve(size_t bytes, uint64_t& allocations) {
-    if (bytes <= capacity) return hipSuccess;
-    size_t grown = std::max(bytes, capacity ? capacity * 2 : size_t(65536));
-    void* fresh = nullptr;
-    hipError_t st = pinned ? hipHostMalloc(&fresh, grown, hipHostMallocDefault)
-                           : hipMalloc(&fresh, grown);
-    if (st != hipSuccess) return st;
-    release();
-    ptr = fresh;
-    capacity = grown;
-    ++allocations;
-    return hipSuccess;
-  }
-  void release() {
-    if (ptr) {
-      if (pinned)
-        (void)hipHostFree(ptr);
-      else
-        (void)hipFree(ptr);
-    }
-    ptr = nullptr;
-    capacity = 0;
-  }
-  ~Buffer() { release(); }
-};
-
 // Waves per prefill workgroup. A batch with a cached prefix (paged) streams long key
 // ranges per item, and 8-wave workgroups (one per CU, 256 query rows per item) read each
 // K/V tile for twice the rows; a batch without one (ragged, every item a causal triangle
@@ -604,12 +575,10 @@ struct PrefillPlan {
   int64_t num_groups = 0;   // items split along the keys (merged by a second launch)
   int64_t num_records = 0;  // partial records (chunks of split items)
   // Device int32 workspace: [req info 4*B][work 4*items][ranges 4*items][kv_indptr B+1]
-  // [last_len B][groups 8*num_groups][shared prefixes: header, kSharedInfoInts * B, request of
-  // every token, work items]
-  int64_t o_work = 0, o_ranges = 0, o_indptr = 0, o_last = 0, o_groups = 0, o_shared = 0;
-  // Shared prefixes (shared_nw 0: none): the whole batch then runs as sources of the shared kernel.
-  int shared_nw = 0;
-  int64_t o_shared_work = 0, shared_items = 0, shared_groups = 0, shared_tokens = 0;
+  // [last_len B][groups 8*num_groups]
+  int64_t o_work = 0, o_ranges = 0, o_indptr = 0, o_last = 0, o_groups = 0;
+  std::unique_ptr<SharedPlan> shared;  // shared prefixes: runs instead of this plan's work list
+  bool shared_runs = false;
   Buffer ints, indices, staging, part_o, part_lse;
   hipEvent_t upload_done = nullptr;
   uint64_t allocations = 0;
@@ -790,28 +759,13 @@ static void* prepare_prefill(void* existing, const int32_t* q_indptr, const int3
       set_error("paged prefill requires a block table");
       return nullptr;
     }
-    std::vector<int32_t> eff;  // tokens of each group's prefix that are computed once
-    bool sharing = false;
-    if (groups > 0) {
-      int64_t rows = 0;
-      for (int64_t g = 0; g < groups; ++g) {
-        if (group_rows[g] <= 0 || group_lens[g] < 0 || group_rows[g] > batch - rows) {
-          set_error("invalid shared prefix groups");
-          return nullptr;
-        }
-        for (int64_t r = rows; r < rows + group_rows[g]; ++r)
-          if (group_lens[g] > prefix_host[r]) {
-            set_error("shared prefix is longer than the cached prefix of a row of its group");
-            return nullptr;
-          }
-        rows += group_rows[g];
-      }
-      if (rows != batch) {
-        set_error("invalid shared prefix groups");
-        return nullptr;
-      }
-      sharing =
-          shared_lengths(group_rows, group_lens, groups, prefix_host, num_kv_heads, eff);
+    if (const char* err =
+            groups > 0 ? check_groups(group_rows, group_lens, groups, batch, prefix_host,
+                                      "shared prefix is longer than the cached prefix of a row of "
+                                      "its group")
+                       : nullptr) {
+      set_error(err);
+      return nullptr;
     }
     int device = 0;
     hipError_t st = hipGetDevice(&device);
@@ -854,51 +808,26 @@ static void* prepare_prefill(void* existing, const int32_t* q_indptr, const int3
       }
       plan->cus = cus;
     }
+    // Shared prefixes: where computing them once does better, a plan of their own runs the batch.
+    std::vector<int32_t> kv_len(batch), first_page(batch + 1, 0);
+    for (int64_t r = 0; r < batch; ++r) {
+      kv_len[r] = prefix_host[r] + q_host[r + 1] - q_host[r];
+      first_page[r + 1] =
+          first_page[r] + static_cast<int32_t>((kv_len[r] + page_size - 1) / page_size);
+    }
+    const SharedBatch sharing{batch,      q_host,     kv_len.data(), first_page.data(),
+                              group_rows, group_lens, groups};
+    if (groups > 0 && !plan->shared)
+      plan->shared = std::make_unique<SharedPlan>(plan->cus, num_q_heads, num_kv_heads, page_size,
+                                                  dtype);
+    const bool shared_runs = groups > 0 && plan->shared->pays(sharing);
     SplitPlan sp;
-    // With shared prefixes: every group's queries against its prefix, then every request's against
-    // its own keys.
-    std::vector<SharedSource> sources;
-    std::vector<int32_t> shared_work, source_of(batch, -1);
-    int shared_nw = 0;
-    int64_t shared_records = 0, shared_groups = 0, shared_tokens = 0;
-    if (sharing) {
-      int64_t row = 0, page = 0;
-      std::vector<SharedSource> own;
-      for (int64_t g = 0; g < groups; ++g) {
-        const int64_t end = row + group_rows[g];
-        if (eff[g] > 0) {
-          sources.push_back({q_host[row], q_host[end] - q_host[row], static_cast<int32_t>(page), 0,
-                             eff[g] / kSharedTile, kNoHorizon, eff[g], 0, 0, 0});
-          ++shared_groups;
-          shared_tokens += eff[g];
-        }
-        for (; row < end; ++row) {
-          if (eff[g] > 0) source_of[row] = static_cast<int32_t>(sources.size() - 1);
-          const int32_t q_len = q_host[row + 1] - q_host[row];
-          const int32_t kv_len = prefix_host[row] + q_len;
-          own.push_back({q_host[row], q_len, static_cast<int32_t>(page), eff[g] / kSharedTile,
-                         (kv_len + kSharedTile - 1) / kSharedTile, prefix_host[row], kv_len, 0, 0,
-                         0});
-          page += (kv_len + page_size - 1) / page_size;
-        }
-      }
-      sources.insert(sources.end(), own.begin(), own.end());
-      const int64_t heads_per_kv = num_q_heads / num_kv_heads;
-      shared_nw = shared_waves(sources, heads_per_kv);
-      shared_records = schedule_shared(
-          sources, heads_per_kv, num_kv_heads, plan->cus, shared_nw,
-          shared_capacity(sources, heads_per_kv, num_kv_heads, plan->cus, shared_nw), shared_work);
-    } else {
+    if (!shared_runs) {
       std::vector<int32_t> base(4 * n_base);
       mi355x_prefill_schedule(q_host, prefix_host, batch, num_q_heads, num_kv_heads, base.data(),
                               n_base);
       sp = split_items(base, q_host, prefix_host, num_q_heads, num_kv_heads, plan->cus,
                        prefill_waves(paged));
-    }
-    const int64_t shared_items = static_cast<int64_t>(shared_work.size()) / kSharedItemInts;
-    if (shared_items > std::numeric_limits<int32_t>::max() / 64) {
-      set_error("prefill work list is empty or too large");
-      return nullptr;
     }
     const int64_t n_items = static_cast<int64_t>(sp.work.size() / 4);
     const int64_t n_groups = static_cast<int64_t>(sp.groups.size() / 8);
@@ -911,25 +840,19 @@ static void* prepare_prefill(void* existing, const int32_t* q_indptr, const int3
     const int64_t o_indptr = o_ranges + 4 * n_items;
     const int64_t o_last = o_indptr + batch + 1;
     const int64_t o_groups = (o_last + batch + 3) / 4 * 4;  // int4-aligned
-    const int64_t o_shared = o_groups + 8 * n_groups;
-    const int64_t o_shared_work =
-        o_shared + kSharedHeaderInts + kSharedInfoInts * batch + (q_host[batch] + 3) / 4 * 4;
-    const int64_t total_ints =
-        sharing ? o_shared_work + static_cast<int64_t>(shared_work.size()) : o_shared;
+    const int64_t total_ints = o_groups + 8 * n_groups;
     st = hipEventSynchronize(plan->upload_done);
     if (st != hipSuccess) {
       hip_error(st, "prefill upload fence");
       return nullptr;
     }
-    // fp32 rows of 128 outputs and their log2-sum-exp
     const size_t rec_bytes =
-        sharing ? static_cast<size_t>(shared_records) * 32 * 4
-                : static_cast<size_t>(sp.records) * prefill_waves(paged) * kQPerWave * 4;
+        static_cast<size_t>(sp.records) * prefill_waves(paged) * kQPerWave * 4;
     if ((st = plan->ints.reserve(total_ints * 4, plan->allocations)) != hipSuccess ||
         (st = plan->staging.reserve(total_ints * 4, plan->allocations)) != hipSuccess ||
-        (rec_bytes && (st = plan->part_o.reserve(rec_bytes * kD, plan->allocations)) !=
+        (sp.records && (st = plan->part_o.reserve(rec_bytes * kD, plan->allocations)) !=
                            hipSuccess) ||
-        (rec_bytes && (st = plan->part_lse.reserve(rec_bytes, plan->allocations)) !=
+        (sp.records && (st = plan->part_lse.reserve(rec_bytes, plan->allocations)) !=
                            hipSuccess)) {
       hip_error(st, "prefill workspace allocation");
       return nullptr;
@@ -961,26 +884,6 @@ static void* prepare_prefill(void* existing, const int32_t* q_indptr, const int3
       std::memcpy(host + o_work, sp.work.data(), sp.work.size() * 4);
       std::memcpy(host + o_ranges, sp.ranges.data(), sp.ranges.size() * 4);
     }
-    if (sharing) {
-      int32_t* section = host + o_shared;
-      std::memset(section, 0, (kSharedHeaderInts + kSharedInfoInts * batch) * 4);
-      section[0] = static_cast<int32_t>(shared_items);
-      int32_t* row_of = section + kSharedHeaderInts + kSharedInfoInts * batch;
-      for (int64_t r = 0; r < batch; ++r) {
-        int32_t* info = section + kSharedHeaderInts + kSharedInfoInts * r;
-        for (int part = 0; part < 2; ++part) {
-          const int64_t i = part == 0 ? source_of[r] : shared_groups + r;
-          if (i < 0) continue;
-          const SharedSource& src = sources[i];
-          info[4 * part] = src.record;
-          info[4 * part + 1] = src.splits;
-          info[4 * part + 2] = src.row_tiles;
-          info[4 * part + 3] = src.token0;
-        }
-        std::fill(row_of + q_host[r], row_of + q_host[r + 1], static_cast<int32_t>(r));
-      }
-      std::memcpy(host + o_shared_work, shared_work.data(), shared_work.size() * 4);
-    }
     if (n_groups) std::memcpy(host + o_groups, sp.groups.data(), sp.groups.size() * 4);
     st = hipMemcpyAsync(plan->ints.ptr, host, total_ints * 4, hipMemcpyHostToDevice, s);
     if (st != hipSuccess) {
@@ -1003,6 +906,7 @@ static void* prepare_prefill(void* existing, const int32_t* q_indptr, const int3
       hip_error(st, "prefill upload event");
       return nullptr;
     }
+    if (shared_runs && !plan->shared->prepare(sharing, 0, 0, plan->allocations, s)) return nullptr;
     plan->batch = batch;
     plan->total_q = q_host[batch];
     plan->num_items = n_items;
@@ -1015,12 +919,7 @@ static void* prepare_prefill(void* existing, const int32_t* q_indptr, const int3
     plan->o_indptr = o_indptr;
     plan->o_last = o_last;
     plan->o_groups = o_groups;
-    plan->o_shared = o_shared;
-    plan->o_shared_work = o_shared_work;
-    plan->shared_nw = shared_nw;
-    plan->shared_items = shared_items;
-    plan->shared_groups = shared_groups;
-    plan->shared_tokens = shared_tokens;
+    plan->shared_runs = shared_runs;
     created.release();
     return plan;
   } catch (const std::exception& e) {
@@ -1057,10 +956,8 @@ extern "C" void* mi355x_prefill_prepare_shared(
 extern "C" const char* mi355x_prefill_plan_shared_info(const void* plan, int64_t* out4) {
   if (!plan || !out4) return set_error("mi355x_prefill_plan_shared_info: null argument");
   const auto* p = static_cast<const PrefillPlan*>(plan);
-  out4[0] = p->shared_groups;
-  out4[1] = p->shared_tokens;
-  out4[2] = p->shared_items;
-  out4[3] = p->shared_nw;
+  std::fill(out4, out4 + 4, 0);
+  if (p->shared_runs) p->shared->info(out4);
   return nullptr;
 }
 
@@ -1155,6 +1052,12 @@ extern "C" const char* mi355x_prefill_run(const void* plan_ptr, const void* q, i
   if (q_sn % 8 || q_sh % 8 || k_sn % 8 || k_sh % 8 || v_sn % 8 || v_sh % 8 || o_sn % 8 ||
       o_sh % 8 || !aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16))
     return set_error("prefill requires 16-byte aligned rows");
+  if (p.shared_runs) {
+    if (k_sn != num_kv_heads * kD || v_sn != k_sn || k_sh != kD || v_sh != kD)
+      return set_error("shared prefixes need contiguous caches");
+    return p.shared->run(static_cast<const int32_t*>(p.indices.ptr), q, q_sn, q_sh, k, v, out, o_sn,
+                         o_sh, static_cast<hipStream_t>(stream));
+  }
   PrefillArgs a{};
   a.q = static_cast<const uint16_t*>(q);
   a.q_sn = q_sn;
@@ -1183,40 +1086,6 @@ extern "C" const char* mi355x_prefill_run(const void* plan_ptr, const void* q, i
   const int waves = prefill_waves(p.paged);
   const int hpb = heads_per_block(num_q_heads / num_kv_heads, waves);
   auto s = static_cast<hipStream_t>(stream);
-  if (p.shared_nw) {
-    if (k_sn != num_kv_heads * kD || v_sn != k_sn || k_sh != kD || v_sh != kD)
-      return set_error("shared prefixes need contiguous caches");
-    const int32_t* section = ints + p.o_shared;
-    SharedArgs sa{};
-    sa.q = a.q;
-    sa.q_sn = q_sn;
-    sa.q_sh = q_sh;
-    sa.k = a.k;
-    sa.v = a.v;
-    sa.header = section;
-    sa.work = reinterpret_cast<const int4*>(ints + p.o_shared_work);
-    sa.indices = a.indices;
-    sa.part_o = a.part_o;
-    sa.part_lse = a.part_lse;
-    sa.group = static_cast<int32_t>(num_q_heads / num_kv_heads);
-    sa.num_kv_heads = a.num_kv_heads;
-    sa.page_size = a.page_size;
-    sa.scale_log2 = a.scale_log2;
-    if (const char* err = launch_shared(sa, dtype, p.shared_nw, p.shared_items, s)) return err;
-    SharedMergeArgs m{};
-    m.out = a.out;
-    m.o_sn = o_sn;
-    m.o_sh = o_sh;
-    m.rows = total_q * num_q_heads;
-    m.info = reinterpret_cast<const int4*>(section + kSharedHeaderInts);
-    m.row_of = section + kSharedHeaderInts + kSharedInfoInts * p.batch;
-    m.part_o = a.part_o;
-    m.part_lse = a.part_lse;
-    m.num_q_heads = a.num_q_heads;
-    m.group = sa.group;
-    m.num_kv_heads = a.num_kv_heads;
-    return launch_shared_merge(m, dtype, s);
-  }
   const int4* groups = reinterpret_cast<const int4*>(ints + p.o_groups);
   if (dtype == 0)
     launch_dt<0>(a, hpb, waves, p.paged, groups, p.num_groups, s);

@@ -1,22 +1,32 @@
-// Attention over a prefix that several requests share, computed once for all of them, and the merge
+// Attention over prefixes that requests of a batch share, computed once for all of them and joined
 // with what each has of its own. No counterpart in the reference, whose backends read every
 // request's whole cache (src/models/attention/backend.rs:316-804).
 //
-//   o = (2^a o_p + 2^b o_s) / (2^a + 2^b),  (o_p, a) and (o_s, b) the normalised outputs and log2 of
-//   the sums of 2^score over the prefix and over the request's own keys.
+//   o = sum_i 2^(a_i) o_i / sum_i 2^(a_i),  (o_i, a_i) the normalised output and the log2 of the sum
+//   of 2^score over part i of a request's keys: parts of the prefix and parts of its own.
 //
-// A group's queries (every token's G heads under a kv head, heads fastest: tokens x G rows) meet the
-// prefix's keys as one matrix product, so K and V are read once a group (and once for every 256
-// rows) where plain decode reads them once a request. One workgroup = 32 rows a wave against a
-// range of 64-key tiles, as the prefill kernel: S^T = K Q^T, P^T = 2^(S^T - m), O^T += V^T P^T on
-// 32 x 32 x 16 products, K and V tiles through an LDS ring by direct copies. Ranges are cut so that
-// the items fill the chip; each writes an fp32 partial and its log2-sum-exp, joined by one more
-// launch together with the own parts: decode's split-KV partials, or (several new tokens a request)
-// items of the same kernel, with a horizon.
+// A group's queries (every token's G heads under a kv head, heads fastest: tokens x G columns) meet
+// the prefix's keys as one matrix product, where plain decode reads the prefix once a request. Two
+// kernels, by the number of columns:
+//
+// shared_stream_kernel, up to 48 columns: the decode kernel's copy pipeline (tiles of 16 whole K and
+// V rows through an LDS ring, one wave a kv head) with up to three sets of 16 columns on the tile a
+// wave has in LDS. Streaming a tile takes a CU longer than three sets of products on it, so it is
+// bound by memory, as decode is. The own keys of requests with few new tokens are items of the same
+// launch, under the same balanced schedule.
+//
+// shared_gemm_kernel, more: 32 columns a wave against a range of 64-key tiles, as the prefill kernel
+// (S^T = K Q^T, P^T = 2^(S^T - m), O^T += V^T P^T on 32 x 32 x 16 products), K and V read once for
+// 256 columns. Own keys of requests with many new tokens go there too, under a horizon a column.
+//
+// Every part that is joined writes fp32 outputs and their log2-sum-exp; shared_merge_kernel joins
+// them. A request that shares nothing and whose keys one item holds is written directly.
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <limits>
 
+#include "buffer.h"
 #include "mfma.h"
 #include "shared.h"
 
@@ -24,14 +34,281 @@ namespace mi355x {
 namespace {
 
 constexpr int kD = 128;
-constexpr int kTileK = kSharedTile;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int32_t kNoHorizon = 1 << 30;  // queries that see every key of their range
+constexpr int64_t kMaxKeys = int64_t(1) << 22;
+
+// --- device workspace, int32
+constexpr int kHeaderInts = 4;
+constexpr int kHeaderGemmItems = 0, kHeaderStreamWgs = 1, kHeaderOnce = 2;
+constexpr int kInfoInts = 8;    // a request: {first slot, splits, tokens, token0} of the prefix's
+                                // parts, then of its own (splits 0: none)
+constexpr int kStreamInts = 8;  // {token0, tokens, first page entry, key begin | key end, slot or -1
+                                // (written directly), position of token0, 0}
+constexpr int kGemmInts = 12;   // {token0, columns, first column, kv head | first page entry, tile
+                                // begin, tile end, slot | position of token0, keys, 0, 0}
+// A slot is a token's q heads of partial outputs: row slot * Hq + qh of part_o [rows][128].
+
+struct SharedArgs {
+  const uint16_t* q;
+  int64_t q_sn, q_sh;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* out;
+  int64_t o_sn, o_sh;
+  const int32_t* header;
+  const int4* info;
+  const int32_t* row_of;  // request of a token; NULL: its own number
+  const int4* stream_work;
+  const int32_t* stream_wg;
+  const int4* gemm_work;
+  const int32_t* indices;
+  float* part_o;
+  float* part_lse;
+  int64_t rows;           // tokens * q heads
+  int32_t num_q_heads, num_kv_heads, group_log2, page_size;
+  float scale_log2;
+};
+
+// ---------------------------------------------------------------------------
+// Few columns: streamed.
+// ---------------------------------------------------------------------------
+constexpr int kStreamTile = 16;
+constexpr int kStreamStages = 2;
+constexpr int kStreamEntries = 2048;  // page entries of an item in LDS
+constexpr int kStreamColumns = 48;  // three sets: a fourth does not fit the registers
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
+
+template <int DT>
+__device__ __forceinline__ floatx4 mma_16x16x32(const uint4& a, const uint4& b, floatx4 c) {
+  if constexpr (DT == 0)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+template <int DT>
+__device__ __forceinline__ floatx4 mma_16x16x16(const uint2& a, const uint2& b, floatx4 c) {
+  if constexpr (DT == 0)
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(v4i16_t, a),
+                                                     __builtin_bit_cast(v4i16_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4_t, a),
+                                                 __builtin_bit_cast(f16x4_t, b), c, 0, 0, 0);
+}
+
+// W waves, one a kv head of the slice blockIdx.y; SETS: sets of 16 columns an item may have. Tiles
+// lie in LDS as decode_mma_kernel's: 16-byte chunk c of a head's 256 bytes at c ^ (token & 15).
+template <int DT, int W, int SETS, bool ONCE>
+__device__ __forceinline__ void stream_items(const SharedArgs& a, uint8_t* lds, int32_t* entries) {
+  constexpr int T = kStreamTile;
+  constexpr int kRow = W * 256;              // bytes of one token's slice (K or V)
+  constexpr int kHalf = T * kRow;            // K (or V) bytes of a tile
+  constexpr int kStage = 2 * kHalf;
+  constexpr int kCopies = 2 * kHalf / 1024;  // 1 KiB copies of a tile
+  constexpr int kPerWave = kCopies / W;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int col = lane & 15;   // column of a set / operand row
+  const int quad = lane >> 4;  // 16-lane group
+  const int h = blockIdx.y * W + wave;
+  const int G = 1 << a.group_log2;
+  const uint32_t lds_base = lds_address(lds);
+  const uint32_t entries_lds = lds_address(entries);
+  const uint32_t row_elems = static_cast<uint32_t>(a.num_kv_heads) * kD;
+  const uint16_t* kslice = a.k + blockIdx.y * W * kD;
+  const uint16_t* vslice = a.v + blockIdx.y * W * kD;
+  const int item_begin = a.stream_wg[blockIdx.x], item_end = a.stream_wg[blockIdx.x + 1];
+
+  for (int item = item_begin; item < item_end; ++item) {
+    const bool first_item = item == item_begin;
+    const int4 w0 = a.stream_work[2 * item], w1 = a.stream_work[2 * item + 1];
+    const int token0 = w0.x, tokens = w0.y, beg = w0.w, end = w1.x, slot = w1.y, pos0 = w1.z;
+    const int first_page = beg / a.page_size;
+    const int n_entries = (end - 1) / a.page_size - first_page + 1;
+    const int32_t* pages = a.indices + w0.z;
+    const int n_tiles = (end - beg + T - 1) / T;
+    const int sets = (tokens * G + 15) >> 4;
+    // Copy c of a tile: half c / (kCopies / 2), bytes from (c % (kCopies / 2)) * 1024 of its token
+    // rows. An item's first tile takes its pages from memory, the others from the entries in LDS.
+    auto issue = [&](int t, int stage, bool from_memory) {
+#pragma unroll
+      for (int j = 0; j < kPerWave; ++j) {
+        const int c = wave * kPerWave + j;
+        const int half = c / (kCopies / 2);
+        const int r = c % (kCopies / 2);
+        const int byte = r * 1024 + (W < 4 ? lane * 16 : 0);  // whole rows a copy: uniform token
+        const int tile_tok = byte / kRow;
+        const int tok = min(beg + t * T + tile_tok, end - 1);
+        const int page = tok / a.page_size;
+        int e;
+        if (!from_memory) {
+          e = entries[page - first_page];
+        } else if constexpr (W < 4) {
+          e = pages[page - first_page];
+        } else {
+          e = *((const __attribute__((address_space(4))) int32_t*)(pages) +
+                __builtin_amdgcn_readfirstlane(page - first_page));
+        }
+        const uint32_t at = static_cast<uint32_t>(e) * static_cast<uint32_t>(a.page_size) +
+                            static_cast<uint32_t>(tok - page * a.page_size);
+        const int chunk = W < 4 ? (byte % kRow) / 16 : ((r * 1024) % kRow) / 16 + lane;
+        const int src_chunk = (chunk & ~15) | ((chunk & 15) ^ (tile_tok & 15));
+        const uint16_t* src =
+            (half ? vslice : kslice) + static_cast<uint64_t>(at) * row_elems + src_chunk * 8;
+        if constexpr (ONCE)
+          copy_to_lds_nt(src, lds_base + stage * kStage + half * kHalf + r * 1024);
+        else
+          copy_to_lds(src, lds_base + stage * kStage + half * kHalf + r * 1024);
+      }
+    };
+    if (!first_item) __syncthreads();  // the ring and the entries are free
+    issue(0, 0, true);
+    for (int base = wave * 64; base < n_entries; base += W * 64)
+      copy_dword_to_lds(pages + min(base + lane, n_entries - 1), entries_lds + base * 4);
+    // Q^T as the B operand: the lane's column 16 c + col is head column % G of token column / G;
+    // columns past the tokens are zero.
+    uint4 qb[SETS][4];
+    int limit[SETS];  // last key the column sees
+#pragma unroll
+    for (int c = 0; c < SETS; ++c) {
+      const int column = 16 * c + col;
+      const int token = column >> a.group_log2;
+      limit[c] = min(end - 1, pos0 + token);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        qb[c][kk] = token < tokens ? ld128(a.q + static_cast<int64_t>(token0 + token) * a.q_sn +
+                                           (h * G + (column & (G - 1))) * a.q_sh + 32 * kk +
+                                           8 * quad)
+                                   : make_uint4(0, 0, 0, 0);
+    }
+    wait_vmem_loads();  // queries, entries and the first tile
+
+    floatx4 o[SETS][8];
+    float m[SETS], l[SETS];
+#pragma unroll
+    for (int c = 0; c < SETS; ++c) {
+      m[c] = -1e30f;
+      l[c] = 0.f;
+#pragma unroll
+      for (int b = 0; b < 8; ++b) o[c][b] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int t = 0; t < n_tiles; ++t) {
+      wait_vmcnt<0>();
+      __syncthreads();
+      if (t + 1 < n_tiles) issue(t + 1, (t + 1) % kStreamStages, false);
+      const uint8_t* kb = lds + (t % kStreamStages) * kStage + wave * 256;
+      const uint8_t* vb = kb + kHalf;
+      uint4 kf[4];
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        kf[kk] = *reinterpret_cast<const uint4*>(kb + col * kRow + (((4 * kk + quad) ^ col) * 16));
+      uint2 vf[8];
+      const int vt = 4 * quad + (col >> 2);
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        const int chunk = 2 * b + ((col & 3) >> 1);
+        lds_u8* vp = (lds_u8*)vb + vt * kRow + ((chunk ^ vt) * 16) + 8 * (col & 1);
+        vf[b] =
+            __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)vp));
+      }
+      const int key0 = beg + t * T + 4 * quad;
+#pragma unroll
+      for (int c = 0; c < SETS; ++c) {
+        if (c >= sets) break;  // uniform
+        floatx4 sc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) sc = mma_16x16x32<DT>(kf[kk], qb[c][kk], sc);
+        // The lane holds S[key0 + i][column].
+        float s[4];
+        float mx = m[c];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[i] = key0 + i <= limit[c] ? sc[i] * a.scale_log2 : -INFINITY;
+          mx = fmaxf(mx, s[i]);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float corr = __builtin_amdgcn_exp2f(m[c] - mx);
+        m[c] = mx;
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(s[i] - mx);
+        l[c] = l[c] * corr + ((p[0] + p[1]) + (p[2] + p[3]));
+        // rounded to the type of V for the product; the sum takes the fp32 values
+        const uint2 pb = make_uint2(Elem<DT>::pack2(p[0], p[1]), Elem<DT>::pack2(p[2], p[3]));
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[c][b][i] *= corr;
+          o[c][b] = mma_16x16x16<DT>(vf[b], pb, o[c][b]);
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < SETS; ++c) {
+      if (c >= sets) break;
+      float sum = l[c];
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      const int column = 16 * c + col;
+      const int token = column >> a.group_log2;
+      if (token >= tokens) continue;
+      const int qh = h * G + (column & (G - 1));
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // 0: no key of the part is seen
+      if (slot < 0) {
+        uint16_t* dst =
+            a.out + static_cast<int64_t>(token0 + token) * a.o_sn + qh * a.o_sh + 4 * quad;
+#pragma unroll
+        for (int b = 0; b < 8; ++b)
+          *reinterpret_cast<uint2*>(dst + 16 * b) =
+              make_uint2(Elem<DT>::pack2(o[c][b][0] * inv, o[c][b][1] * inv),
+                         Elem<DT>::pack2(o[c][b][2] * inv, o[c][b][3] * inv));
+      } else {
+        const int64_t row = static_cast<int64_t>(slot + token) * a.num_q_heads + qh;
+        float* dst = a.part_o + row * kD + 4 * quad;
+#pragma unroll
+        for (int b = 0; b < 8; ++b)
+          *reinterpret_cast<float4*>(dst + 16 * b) = make_float4(
+              o[c][b][0] * inv, o[c][b][1] * inv, o[c][b][2] * inv, o[c][b][3] * inv);
+        if (quad == 0)
+          a.part_lse[row] = sum == 0.f ? -INFINITY : m[c] + __builtin_amdgcn_logf(sum);
+      }
+    }
+  }
+}
+
+template <int DT, int W, int SETS>
+__global__ __launch_bounds__(64 * W, 2) void shared_stream_kernel(SharedArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t
+      lds[kStreamStages * 2 * kStreamTile * W * 256];
+  __shared__ int32_t entries[kStreamEntries];
+  if (static_cast<int>(blockIdx.x) >= a.header[kHeaderStreamWgs]) return;  // graph plans' grids
+  if (a.num_kv_heads < 0) {  // the copies are invisible to the compiler
+    lds[threadIdx.x] = 0;
+    entries[threadIdx.x] = 0;
+  }
+  if (a.header[kHeaderOnce])  // uniform
+    stream_items<DT, W, SETS, true>(a, lds, entries);
+  else
+    stream_items<DT, W, SETS, false>(a, lds, entries);
+}
+
+// ---------------------------------------------------------------------------
+// Many columns: matrix products of 32 columns a wave.
+// ---------------------------------------------------------------------------
+constexpr int kTileK = 64;
 constexpr int kTileBytes = kTileK * kD * 2;
 constexpr int kStageBytes = 2 * kTileBytes;  // K + V
 
 // K and V tiles lie in LDS as the prefill kernel's do: [key][d], 16-byte chunk c of key r at
 // c ^ (r & 15) (K) and c ^ 4 (r & 3) (V), which keeps the operand reads free of bank conflicts.
 template <int DT, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_kernel(SharedArgs a) {
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_gemm_kernel(SharedArgs a) {
   constexpr int kStages = NW == 8 ? 4 : 2;
   constexpr int kAhead = kStages - 1;
   constexpr int kGroupsPerWave = 16 / NW;  // 4-row groups of each tile this wave copies
@@ -65,20 +342,21 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_kernel(Shared
   const int row_in_group = lane >> 4;
   const int pos = lane & 15;
 
-  const int items = a.header[0];
+  const int items = a.header[kHeaderGemmItems];
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    const int4 w0 = a.work[3 * item], w1 = a.work[3 * item + 1], w2 = a.work[3 * item + 2];
+    const int4* work = a.gemm_work + kGemmInts / 4 * item;
+    const int4 w0 = work[0], w1 = work[1], w2 = work[2];
     const int token0 = w0.x, rows = w0.y, row0 = w0.z, kvh = w0.w;
-    const int page_base = w1.x, t_begin = w1.y, nt = w1.z - w1.y, record = w1.w;
+    const int page_base = w1.x, t_begin = w1.y, nt = w1.z - w1.y, slot = w1.w;
     const int pos0 = w2.x, kv_len = w2.y;
     const int my_row0 = row0 + wave * 32;
     const bool wave_active = my_row0 < rows;
     const int my_row = min(my_row0 + col, rows - 1);
-    const int token = my_row / a.group;
-    const int qh = kvh * a.group + (my_row - token * a.group);
+    const int token = my_row >> a.group_log2;
+    const int qh = (kvh << a.group_log2) + (my_row - (token << a.group_log2));
     const int horizon = pos0 + token;  // the last key this row sees
-    const int first_horizon = pos0 + my_row0 / a.group;
-    const int last_horizon = pos0 + min(my_row0 + 31, rows - 1) / a.group;
+    const int first_horizon = pos0 + (my_row0 >> a.group_log2);
+    const int last_horizon = pos0 + (min(my_row0 + 31, rows - 1) >> a.group_log2);
 
     uint4 qreg[8];
     {
@@ -177,18 +455,6 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_kernel(Shared
 #pragma unroll
         for (int T = 0; T < 2; ++T)
           s[T] = Mfma<DT>::run(kf[T][kk], qreg[kk], kk == 0 ? negm : s[T]);
-      uint4 vf[4][4];
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-        for (int db = 0; db < 4; ++db) {
-          lds_u8* vp = (lds_u8*)sb + v_off[db] + 16 * kk * 256;
-          const uint2 l2 =
-              __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)vp));
-          const uint2 h2 = __builtin_bit_cast(
-              uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vp + 8 * 256)));
-          vf[kk][db] = make_uint4(l2.x, l2.y, h2.x, h2.y);
-        }
       if (k0 + kTileK - 1 > first_horizon || k0 + kTileK > kv_len) {
         const int limit = min(horizon, kv_len - 1) - (k0 + 4 * half);
 #pragma unroll
@@ -248,7 +514,14 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_kernel(Shared
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-        for (int db = 0; db < 4; ++db) o[db] = Mfma<DT>::run(vf[kk][db], pb[kk], o[db]);
+        for (int db = 0; db < 4; ++db) {
+          lds_u8* vp = (lds_u8*)sb + v_off[db] + 16 * kk * 256;
+          const uint2 l2 =
+              __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)vp));
+          const uint2 h2 = __builtin_bit_cast(
+              uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vp + 8 * 256)));
+          o[db] = Mfma<DT>::run(make_uint4(l2.x, l2.y, h2.x, h2.y), pb[kk], o[db]);
+        }
     };
 
     if (fast_pages) load_ids(t_begin);
@@ -262,23 +535,37 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_kernel(Shared
       compute(t_begin + u, u % kStages, u == 0);
     }
 
-    if (wave_active && my_row0 + col < rows) {
+    // The wave's 32 x 128 outputs go out as whole rows, through its share of the ring (16-byte chunk c
+    // of row r at c ^ r): 512 bytes a row instead of 32 at a time.
+    __syncthreads();
+    if (wave_active) {
       const float row_sum = l + __shfl_xor(l, 32);
-      const float inv = row_sum > 0.f ? 1.f / row_sum : 0.f;
-      const int64_t rec = record + wave;
-      float* po = a.part_o + rec * kSharedRecord;
-      // Lanes' own order (float4 (4 db + g4) * 64 + lane): whole lines for a wave's rows.
+      const float inv = row_sum == 0.f ? 0.f : 1.f / row_sum;
+      uint8_t* tile = lds + wave * (32 * kD * 4);
 #pragma unroll
       for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4)
-          *reinterpret_cast<float4*>(po + ((4 * db + g4) * 64 + lane) * 4) =
+          *reinterpret_cast<float4*>(tile + col * 512 + ((8 * db + 2 * g4 + half) ^ col) * 16) =
               make_float4(o[db][4 * g4] * inv, o[db][4 * g4 + 1] * inv, o[db][4 * g4 + 2] * inv,
                           o[db][4 * g4 + 3] * inv);
-      if (half == 0)
-        a.part_lse[rec * 32 + col] =
-            row_sum > 0.f ? m * c + __builtin_amdgcn_logf(row_sum)
-                          : row_sum == 0.f ? -INFINITY : row_sum;  // NaN stays
+      const int heads = 1 << a.group_log2;
+      auto part_row = [&](int r) {  // partial row of the wave's row r
+        const int t = (my_row0 + r) >> a.group_log2;
+        return static_cast<int64_t>(slot + t) * a.num_q_heads + (kvh << a.group_log2) +
+               ((my_row0 + r) & (heads - 1));
+      };
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int r = 2 * j + half;
+        const float4 val =
+            *reinterpret_cast<const float4*>(tile + r * 512 + ((lane & 31) ^ r) * 16);
+        if (my_row0 + r < rows)
+          *reinterpret_cast<float4*>(a.part_o + part_row(r) * kD + (lane & 31) * 4) = val;
+      }
+      if (half == 0 && my_row0 + col < rows)
+        a.part_lse[part_row(col)] =
+            row_sum == 0.f ? -INFINITY : m * c + __builtin_amdgcn_logf(row_sum);
     }
     __syncthreads();  // the next item's copies overwrite the ring
   }
@@ -308,62 +595,36 @@ struct Join {
   }
 };
 
-// 32 threads a row (a token's q head), eight rows a workgroup: dims 4 f .. 4 f + 3 of a row sit in
-// float4 (f / 2) * 64 + row % 32 + 32 (f % 2) of a record. Bound by the rounds of loads, kUnroll
-// partials each.
+// 32 threads a row (a token's q head), eight rows a workgroup. Bound by the rounds of loads,
+// kUnroll partials each.
 template <int DT>
-__global__ __launch_bounds__(256) void shared_merge_kernel(SharedMergeArgs a) {
+__global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
   constexpr int kUnroll = 8;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (row >= a.rows) return;
   const int f = threadIdx.x & 31;
   const int token = static_cast<int>(row / a.num_q_heads);
   const int qh = static_cast<int>(row - static_cast<int64_t>(token) * a.num_q_heads);
-  const int h = qh / a.group, g = qh - h * a.group;
   const int req = a.row_of ? a.row_of[token] : token;
-  int own_first = 0, own_count = 0;
-  if (a.own_merge) {
-    own_first = a.own_merge[2 * req];
-    own_count = a.own_merge[2 * req + 1];
-  }
   Join j;
-  bool any = false;
+  const int4 parts[2] = {a.info[2 * req], a.info[2 * req + 1]};
+  if (parts[0].y + parts[1].y == 0) return;  // written directly
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
-    const int4 src = a.info[2 * req + part];  // {record, splits, row_tiles, token0}
-    if (src.y == 0) continue;
-    any = true;
-    const int i = (token - src.w) * a.group + g;
-    const int64_t first = src.x + static_cast<int64_t>(h) * src.z + i / 32;
-    const int64_t step = static_cast<int64_t>(a.num_kv_heads) * src.z;
+    const int4 src = parts[part];  // {first slot, splits, tokens, token0}
+    const int64_t first = static_cast<int64_t>(src.x + token - src.w) * a.num_q_heads + qh;
+    const int64_t step = static_cast<int64_t>(src.z) * a.num_q_heads;
     for (int s0 = 0; s0 < src.y; s0 += kUnroll) {
       float lse[kUnroll];
       float4 v[kUnroll];
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        const int64_t rec = first + min(s0 + u, src.y - 1) * step;
-        lse[u] = s0 + u < src.y ? a.part_lse[rec * 32 + i % 32] : -INFINITY;
-        v[u] = *reinterpret_cast<const float4*>(
-            a.part_o + rec * kSharedRecord + ((f >> 1) * 64 + i % 32 + 32 * (f & 1)) * 4);
+        const int64_t at = first + min(s0 + u, src.y - 1) * step;
+        lse[u] = s0 + u < src.y ? a.part_lse[at] : -INFINITY;
+        v[u] = *reinterpret_cast<const float4*>(a.part_o + at * kD + f * 4);
       }
       j.add(lse, v);
     }
-  }
-  if (own_count > 0 && (any || own_count > 1)) {
-    for (int c0 = 0; c0 < own_count; c0 += kUnroll) {
-      float lse[kUnroll];
-      float4 v[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int64_t p =
-            static_cast<int64_t>(own_first + min(c0 + u, own_count - 1)) * a.num_q_heads + qh;
-        lse[u] = c0 + u < own_count ? a.own_lse[p] : -INFINITY;
-        v[u] = *reinterpret_cast<const float4*>(a.own_o + p * kD + f * 4);
-      }
-      j.add(lse, v);
-    }
-  } else if (!any) {
-    return;  // one item held the whole request and has written it
   }
   const float inv = 1.f / j.den;
   *reinterpret_cast<uint2*>(a.out + token * a.o_sn + qh * a.o_sh + f * 4) =
@@ -371,154 +632,478 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedMergeArgs a) {
                  Elem<DT>::pack2(j.acc.z * inv, j.acc.w * inv));
 }
 
+// ---------------------------------------------------------------------------
+// Planning.
+// ---------------------------------------------------------------------------
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-int64_t slots_of(int64_t cus, int nw) { return nw == 8 ? cus : 2 * cus; }
+// The streaming launch for a kv-head count: the widest slice of whole rows that divides it.
+struct StreamShape {
+  int64_t waves, grid_y, workgroups, wg_capacity, max_item;
+};
+StreamShape stream_shape(int64_t cus, int64_t num_kv_heads, int64_t page_size) {
+  StreamShape s{};
+  for (s.waves = 8; num_kv_heads % s.waves; s.waves /= 2) {
+  }
+  s.grid_y = num_kv_heads / s.waves;
+  const int64_t lds = kStreamStages * 2 * kStreamTile * s.waves * 256 + kStreamEntries * 4;
+  // eight waves of up to 256 registers on a CU
+  const int64_t per_cu = std::max<int64_t>(1, std::min((160 * 1024) / lds, 8 / s.waves));
+  s.workgroups = std::max<int64_t>(1, cus * per_cu / s.grid_y);
+  s.wg_capacity = s.workgroups + s.workgroups / 3 + 2;  // schedule() tries more than it takes
+  s.max_item = int64_t(kStreamEntries - 1) * page_size;
+  return s;
+}
 
-// Items and records when a part of a source holds at most `length` tiles.
-SharedCapacity count_at(const std::vector<SharedSource>& sources, int64_t group,
-                        int64_t num_kv_heads, int nw, int64_t length) {
-  SharedCapacity n{0, 0};
-  for (const SharedSource& s : sources) {
-    const int64_t rows = s.tokens * group;
-    const int64_t splits =
-        std::max<int64_t>(1, ceil_div(s.tile_end - s.tile_begin, std::max<int64_t>(length, 1)));
-    n.items += ceil_div(rows, 32 * nw) * num_kv_heads * splits;
-    n.records += ceil_div(rows, 32) * num_kv_heads * splits;
+// Query tokens against a range of keys: a group's against its prefix, or a request's own.
+struct Source {
+  int32_t token0, tokens, page_base, begin, end, pos0;
+  int32_t slot = 0, splits = 0;
+};
+
+int64_t gemm_slots(int64_t cus, int nw) { return nw == 8 ? cus : 2 * cus; }
+
+struct GemmCount {
+  int64_t items = 0, slots = 0;
+};
+GemmCount count_gemm(const std::vector<Source>& sources, int64_t group, int64_t num_kv_heads,
+                     int nw, int64_t length) {
+  GemmCount n;
+  for (const Source& s : sources) {
+    const int64_t tiles = ceil_div(s.end, kTileK) - s.begin / kTileK;
+    const int64_t splits = std::max<int64_t>(1, ceil_div(tiles, length));
+    n.items += ceil_div(s.tokens * group, 32 * nw) * num_kv_heads * splits;
+    n.slots += s.tokens * splits;
   }
   return n;
 }
 
-}  // namespace
+// Tiles of a part's keys, such that the launch ends soonest: rounds of items over the chip, each as
+// long as its longest part and what an item costs besides its tiles (its queries, its first tile and
+// its partial: about two tiles), and the parts that the merge has to read.
+int64_t gemm_length(const std::vector<Source>& sources, int64_t group, int64_t num_kv_heads,
+                    int64_t cus, int nw, const GemmCount& cap) {
+  constexpr double kItemTiles = 2.0, kMergeTiles = 0.25;
+  int64_t longest = 1;
+  for (const Source& s : sources)
+    longest = std::max(longest, ceil_div(s.end, kTileK) - s.begin / kTileK);
+  int64_t length = longest;
+  double best = 0;
+  for (int64_t parts = 1; parts <= std::min<int64_t>(longest, 256); ++parts) {
+    const int64_t l = ceil_div(longest, parts);
+    const GemmCount n = count_gemm(sources, group, num_kv_heads, nw, l);
+    if (n.items > cap.items || n.slots > cap.slots) break;
+    const double est =
+        static_cast<double>(ceil_div(n.items, gemm_slots(cus, nw))) * (l + kItemTiles) +
+        kMergeTiles * parts;
+    if (parts == 1 || est < best) {
+      best = est;
+      length = l;
+    }
+  }
+  return length;
+}
 
-int shared_waves(const std::vector<SharedSource>& sources, int64_t group) {
-  // 256 rows a workgroup where they are mostly filled: K and V are read half as often. Fewer rows
-  // leave waves of it idle, which two workgroups of 128 rows a CU do not.
+// Appends the sources' work items, longest first; `slot`: the next free one.
+void schedule_gemm(std::vector<Source>& sources, int64_t group, int64_t num_kv_heads, int nw,
+                   int64_t length, int64_t& slot, std::vector<int32_t>& work) {
+  struct Item {
+    int64_t tiles;
+    int32_t source, row0, head, split, begin, end;
+  };
+  std::vector<Item> items;
+  for (size_t i = 0; i < sources.size(); ++i) {
+    Source& s = sources[i];
+    const int64_t rows = s.tokens * group;
+    const int64_t first = s.begin / kTileK, tiles = ceil_div(s.end, kTileK) - first;
+    s.splits = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(tiles, length)));
+    s.slot = static_cast<int32_t>(slot);
+    slot += static_cast<int64_t>(s.splits) * s.tokens;
+    for (int32_t p = 0; p < s.splits; ++p)
+      for (int64_t row0 = 0; row0 < rows; row0 += 32 * nw) {
+        const int64_t begin = first + tiles * p / s.splits;
+        int64_t end = first + tiles * (p + 1) / s.splits;
+        if (s.pos0 < kNoHorizon) {  // no tile past what the item's last row sees
+          const int64_t last = s.pos0 + (std::min<int64_t>(row0 + 32 * nw, rows) - 1) / group;
+          end = std::max<int64_t>(begin, std::min<int64_t>(end, last / kTileK + 1));
+        }
+        for (int32_t h = 0; h < num_kv_heads; ++h)
+          items.push_back({end - begin, static_cast<int32_t>(i), static_cast<int32_t>(row0), h, p,
+                           static_cast<int32_t>(begin), static_cast<int32_t>(end)});
+      }
+  }
+  // Heads stay fastest, so that with 8 of them a head's items, which read the same keys, meet in the
+  // L2 of one XCD.
+  std::stable_sort(items.begin(), items.end(),
+                   [](const Item& x, const Item& y) { return x.tiles > y.tiles; });
+  work.reserve(items.size() * kGemmInts);
+  for (const Item& it : items) {
+    const Source& s = sources[it.source];
+    work.insert(work.end(), {s.token0, static_cast<int32_t>(s.tokens * group), it.row0, it.head,
+                             s.page_base, it.begin, it.end, s.slot + it.split * s.tokens, s.pos0,
+                             s.end, 0, 0});
+  }
+}
+
+// 256 columns a workgroup where they are mostly filled: K and V are read half as often. Fewer leave
+// waves of it idle, which two workgroups of 128 a CU do not.
+int gemm_waves(const std::vector<Source>& sources, int64_t group) {
   int64_t cost8 = 0, cost4 = 0;
-  for (const SharedSource& s : sources) {
-    const int64_t rows = s.tokens * group, tiles = s.tile_end - s.tile_begin;
+  for (const Source& s : sources) {
+    const int64_t rows = s.tokens * group, tiles = ceil_div(s.end, kTileK) - s.begin / kTileK;
     cost8 += 2 * ceil_div(rows, 256) * tiles;
     cost4 += ceil_div(rows, 128) * tiles;
   }
   return cost8 <= cost4 ? 8 : 4;
 }
 
-SharedCapacity shared_capacity(const std::vector<SharedSource>& sources, int64_t group,
-                               int64_t num_kv_heads, int64_t cus, int nw) {
-  const SharedCapacity whole =
-      count_at(sources, group, num_kv_heads, nw, std::numeric_limits<int32_t>::max());
-  return {whole.items + slots_of(cus, nw), whole.records + slots_of(cus, nw) * nw};
-}
+}  // namespace
 
-SharedCapacity shared_decode_capacity(int64_t rows, int64_t group, int64_t num_kv_heads,
-                                      int64_t cus, int nw) {
-  // At most rows / 2 groups share, each with a last tile that is not full.
-  const int64_t groups = rows / 2;
-  return {(rows * group / (32 * nw) + groups) * num_kv_heads + slots_of(cus, nw),
-          (rows * group / 32 + groups) * num_kv_heads + slots_of(cus, nw) * nw};
-}
-
-int64_t schedule_shared(std::vector<SharedSource>& sources, int64_t group, int64_t num_kv_heads,
-                        int64_t cus, int nw, const SharedCapacity& cap,
-                        std::vector<int32_t>& work) {
-  int64_t longest = 1;
-  for (const SharedSource& s : sources)
-    longest = std::max<int64_t>(longest, s.tile_end - s.tile_begin);
-  // The length of a part that ends the launch soonest: rounds of items over the chip, each as long
-  // as its longest part and what an item costs besides its tiles (its queries, its first tile and
-  // its partial: about two tiles), and the parts that the merge has to read.
-  constexpr double kItemTiles = 2.0, kMergeTiles = 0.25;
-  const int64_t slots = slots_of(cus, nw);
-  int64_t length = longest;
-  double best = 0;
-  for (int64_t parts = 1; parts <= std::min<int64_t>(longest, 256); ++parts) {
-    const int64_t l = ceil_div(longest, parts);
-    const SharedCapacity n = count_at(sources, group, num_kv_heads, nw, l);
-    if (n.items > cap.items || n.records > cap.records) break;
-    const double est = static_cast<double>(ceil_div(n.items, slots)) * (l + kItemTiles) +
-                       kMergeTiles * parts;
-    if (parts == 1 || est < best) {
-      best = est;
-      length = l;
-    }
-  }
-  struct Item {
-    int64_t tiles;
-    int32_t source, row0, head, split, begin, end;
-  };
-  std::vector<Item> items;
-  int64_t records = 0;
-  for (size_t i = 0; i < sources.size(); ++i) {
-    SharedSource& s = sources[i];
-    const int64_t rows = s.tokens * group, tiles = s.tile_end - s.tile_begin;
-    s.splits = static_cast<int32_t>(std::max<int64_t>(1, ceil_div(tiles, length)));
-    s.row_tiles = static_cast<int32_t>(ceil_div(rows, 32));
-    s.record = static_cast<int32_t>(records);
-    records += static_cast<int64_t>(s.splits) * num_kv_heads * s.row_tiles;
-    for (int32_t p = 0; p < s.splits; ++p)
-      for (int64_t row0 = 0; row0 < rows; row0 += 32 * nw) {
-        const int32_t begin = static_cast<int32_t>(s.tile_begin + tiles * p / s.splits);
-        int64_t end = s.tile_begin + tiles * (p + 1) / s.splits;
-        if (s.pos0 < kNoHorizon) {  // no tile past what the item's last row sees
-          const int64_t last = s.pos0 + (std::min<int64_t>(row0 + 32 * nw, rows) - 1) / group;
-          end = std::max<int64_t>(begin, std::min<int64_t>(end, last / kSharedTile + 1));
-        }
-        for (int32_t h = 0; h < num_kv_heads; ++h)
-          items.push_back({end - begin, static_cast<int32_t>(i), static_cast<int32_t>(row0), h, p,
-                           begin, static_cast<int32_t>(end)});
-      }
-  }
-  // Longest first; heads stay fastest, so that with 8 of them a head's items, which read the same
-  // keys, meet in the L2 of one XCD.
-  std::stable_sort(items.begin(), items.end(),
-                   [](const Item& x, const Item& y) { return x.tiles > y.tiles; });
-  work.reserve(work.size() + items.size() * kSharedItemInts);
-  for (const Item& it : items) {
-    const SharedSource& s = sources[it.source];
-    const int64_t rec = s.record +
-                        (static_cast<int64_t>(it.split) * num_kv_heads + it.head) * s.row_tiles +
-                        it.row0 / 32;
-    work.insert(work.end(),
-                {s.token0, static_cast<int32_t>(s.tokens * group), it.row0, it.head, s.page_base,
-                 it.begin, it.end, static_cast<int32_t>(rec), s.pos0, s.kv_len, 0, 0});
-  }
-  return records;
-}
-
-bool shared_lengths(const int32_t* group_rows, const int32_t* group_lens, int64_t groups,
-                    const int32_t* limit, int64_t num_kv_heads, std::vector<int32_t>& eff) {
-  eff.assign(groups, 0);
-  bool any = false;
+const char* check_groups(const int32_t* group_rows, const int32_t* group_lens, int64_t groups,
+                         int64_t batch, const int32_t* cached, const char* too_long) {
   int64_t row = 0;
   for (int64_t g = 0; g < groups; ++g) {
-    int64_t len = std::min<int64_t>(group_lens[g], kSharedMaxKeys - kSharedTile);
-    for (int64_t r = row; r < row + group_rows[g]; ++r) len = std::min<int64_t>(len, limit[r]);
-    row += group_rows[g];
-    if (group_rows[g] < 2) continue;
-    eff[g] = static_cast<int32_t>(len / kSharedTile * kSharedTile);
-    any |= eff[g] > 0;
+    if (group_rows[g] <= 0 || group_lens[g] < 0 || group_rows[g] > batch - row)
+      return "invalid shared prefix groups";
+    for (const int64_t end = row + group_rows[g]; row < end; ++row)
+      if (group_lens[g] > cached[row]) return too_long;
   }
-  return any;
+  return row == batch ? nullptr : "invalid shared prefix groups";
 }
 
-const char* launch_shared(const SharedArgs& a, int64_t dtype, int nw, int64_t grid,
-                          hipStream_t s) {
-  const dim3 blocks(static_cast<uint32_t>(grid));
-  if (dtype == 0) {
-    if (nw == 8) shared_kernel<0, 8><<<blocks, dim3(512), 0, s>>>(a);
-    else shared_kernel<0, 4><<<blocks, dim3(256), 0, s>>>(a);
-  } else {
-    if (nw == 8) shared_kernel<1, 8><<<blocks, dim3(512), 0, s>>>(a);
-    else shared_kernel<1, 4><<<blocks, dim3(256), 0, s>>>(a);
+struct SharedPlan::State {
+  int64_t cus, num_q_heads, num_kv_heads, page_size, dtype, group;
+  int group_log2 = 0;
+  StreamShape shape{};
+  // Current plan.
+  int64_t batch = 0, tokens = 0;
+  bool by_token = false;  // requests of one token each
+  int64_t stream_grid = 0, gemm_grid = 0, gemm_items = 0;
+  int nw = 8, sets = 1;
+  int64_t groups_shared = 0, tokens_shared = 0, prefix_items = 0;
+  int64_t o_info = 0, o_row_of = 0, o_stream = 0, o_wg = 0, o_gemm = 0;
+  Buffer ints, staging, part_o, part_lse;
+  hipEvent_t upload_done = nullptr;
+
+  ~State() {
+    if (upload_done) {
+      (void)hipEventSynchronize(upload_done);
+      (void)hipEventDestroy(upload_done);
+    }
   }
-  return launch_status("shared_kernel");
+
+  // Whole tiles of each group's prefix that leave every request its own tokens; 0 for groups of one.
+  std::vector<int32_t> lengths(const SharedBatch& b) const {
+    std::vector<int32_t> eff(b.groups, 0);
+    int64_t row = 0;
+    for (int64_t g = 0; g < b.groups; ++g) {
+      int64_t len = std::min<int64_t>(b.group_lens[g], kMaxKeys - kTileK);
+      for (int64_t r = row; r < row + b.group_rows[g]; ++r)
+        len = std::min<int64_t>(len, b.kv_len[r] - (b.q_start[r + 1] - b.q_start[r]));
+      if (b.group_rows[g] > 1) eff[g] = static_cast<int32_t>(len / kTileK * kTileK);
+      row += b.group_rows[g];
+    }
+    return eff;
+  }
+};
+
+SharedPlan::SharedPlan(int64_t cus, int64_t num_q_heads, int64_t num_kv_heads, int64_t page_size,
+                       int64_t dtype)
+    : st_(new State{cus, num_q_heads, num_kv_heads, page_size, dtype,
+                    num_q_heads / num_kv_heads}) {
+  while ((1 << st_->group_log2) < st_->group) ++st_->group_log2;
+  st_->shape = stream_shape(cus, num_kv_heads, page_size);
+  st_->staging.pinned = true;
+}
+SharedPlan::~SharedPlan() = default;
+
+bool SharedPlan::pays(const SharedBatch& b) const {
+  for (const int32_t n : st_->lengths(b))
+    if (n > 0) return true;
+  return false;
 }
 
-const char* launch_shared_merge(const SharedMergeArgs& a, int64_t dtype, hipStream_t s) {
-  const dim3 blocks(static_cast<uint32_t>((a.rows + 7) / 8));
-  if (dtype == 0) shared_merge_kernel<0><<<blocks, dim3(256), 0, s>>>(a);
-  else shared_merge_kernel<1><<<blocks, dim3(256), 0, s>>>(a);
+bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph_tokens,
+                         uint64_t& allocations, hipStream_t s) {
+  State& st = *st_;
+  const int64_t group = st.group, heads = st.num_kv_heads;
+  const int64_t tokens = b.q_start[b.batch];
+  std::vector<int32_t> eff = st.lengths(b);
+  std::vector<Source> stream, gemm;             // own and prefix sources of either kernel
+  struct Of { int32_t kind, index; };           // 0 none, 1 stream, 2 gemm
+  std::vector<Of> prefix_of, own_of;
+  std::vector<int32_t> lens, work, merge, wg, gemm_work;
+  GemmCount cap;
+  int64_t items = 0, wgs = 0, slot = 0, items_cap = 0;
+  bool once = true;
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    stream.clear();
+    gemm.clear();
+    prefix_of.assign(b.batch, {0, 0});
+    own_of.assign(b.batch, {0, 0});
+    once = true;
+    st.groups_shared = st.tokens_shared = 0;
+    for (int64_t r = 0, g = 0, left = 0, before = 0; r < b.batch; ++r) {
+      if (left == 0 && g < b.groups) {  // a group begins
+        left = b.group_rows[g];
+        before = eff[g];
+        ++g;
+        if (before > 0) {
+          ++st.groups_shared;
+          st.tokens_shared += before;
+          const int64_t all = b.q_start[r + left] - b.q_start[r];
+          const Source src{b.q_start[r], static_cast<int32_t>(all), b.page_base[r], 0,
+                           static_cast<int32_t>(before), kNoHorizon};
+          if (all * group <= kStreamColumns) {
+            for (int64_t i = r; i < r + left; ++i)
+              prefix_of[i] = {1, static_cast<int32_t>(stream.size())};
+            stream.push_back(src);
+          } else {
+            for (int64_t i = r; i < r + left; ++i)
+              prefix_of[i] = {2, static_cast<int32_t>(gemm.size())};
+            gemm.push_back(src);
+          }
+        }
+      }
+      const int32_t t = b.q_start[r + 1] - b.q_start[r];
+      const Source own{b.q_start[r], t, b.page_base[r], static_cast<int32_t>(left ? before : 0),
+                       b.kv_len[r], b.kv_len[r] - t};
+      if (left) --left;
+      if (t * group <= kStreamColumns) {
+        own_of[r] = {1, static_cast<int32_t>(stream.size())};
+        stream.push_back(own);
+      } else {
+        own_of[r] = {2, static_cast<int32_t>(gemm.size())};
+        gemm.push_back(own);
+      }
+    }
+    // The streaming launch.
+    lens.clear();
+    items_cap = st.shape.wg_capacity;
+    int64_t bytes = 0;
+    int columns = 1;
+    for (const Source& src : stream) {
+      lens.push_back(src.end - src.begin);
+      items_cap += 1 + ceil_div(lens.back(), st.shape.max_item);
+      bytes += int64_t(lens.back()) * heads * kD * 4;
+      columns = std::max<int>(columns, src.tokens * static_cast<int>(group));
+    }
+    once = bytes >= int64_t(8) << 20;  // as the decode kernel's copies
+    st.sets = columns <= 16 ? 1 : columns <= 32 ? 2 : 3;
+    work.resize(4 * items_cap);
+    merge.resize(2 * stream.size());
+    wg.resize(st.shape.wg_capacity + 1);
+    int64_t share = 0;
+    items = wgs = slot = 0;
+    if (!stream.empty()) {
+      items = schedule(lens.data(), static_cast<int64_t>(stream.size()), st.shape.workgroups,
+                       st.shape.max_item, kStreamTile, /*graph=*/true, work.data(), items_cap,
+                       merge.data(), &share, wg.data(), st.shape.wg_capacity, &wgs);
+      if (items < 0) {
+        set_error("shared prefix work list exceeds its capacity");
+        return false;
+      }
+    }
+    // Items of a source are consecutive: its slots follow each other.
+    std::vector<bool> joined(stream.size(), true);
+    for (int64_t r = 0; r < b.batch; ++r)
+      if (own_of[r].kind == 1 && prefix_of[r].kind == 0)
+        joined[own_of[r].index] = merge[2 * own_of[r].index + 1] > 1;
+    for (size_t i = 0; i < stream.size(); ++i) {
+      Source& src = stream[i];
+      src.splits = joined[i] ? merge[2 * i + 1] : 0;
+      src.slot = static_cast<int32_t>(slot);
+      slot += static_cast<int64_t>(src.splits) * src.tokens;
+    }
+    // The matrix products.
+    gemm_work.clear();
+    cap = {};
+    if (graph_rows) {
+      st.nw = graph_rows * group > 128 ? 8 : 4;
+      const int64_t per = 32 * st.nw / group;  // tokens of an item
+      // at most rows / 2 groups share, each with a last tile that is not full
+      cap.items = (graph_rows / per + graph_rows / 2) * heads + gemm_slots(st.cus, st.nw);
+      cap.slots = graph_rows + gemm_slots(st.cus, st.nw) * per / heads;
+    } else if (!gemm.empty()) {
+      st.nw = gemm_waves(gemm, group);
+      cap = count_gemm(gemm, group, heads, st.nw, std::numeric_limits<int32_t>::max());
+      cap.items += gemm_slots(st.cus, st.nw);
+      cap.slots += gemm_slots(st.cus, st.nw) * 32 * st.nw / group;
+    }
+    const int64_t stream_slots = slot;
+    if (!gemm.empty())
+      schedule_gemm(gemm, group, heads, st.nw,
+                    gemm_length(gemm, group, heads, st.cus, st.nw, cap), slot, gemm_work);
+    if (!graph_rows) break;
+    // A graph plan has room for 64 MiB of partial outputs of the streaming launch, beside a slot an
+    // item: a batch that needs more (dozens of small groups) shares nothing.
+    const int64_t room = (int64_t(64) << 20) / (st.num_q_heads * kD * 4);
+    if (stream_slots <= room + items) break;
+    std::fill(eff.begin(), eff.end(), 0);
+  }
+  st.gemm_items = static_cast<int64_t>(gemm_work.size()) / kGemmInts;
+
+  // Layout; a graph plan's does not depend on what is shared.
+  const bool by_token = tokens == b.batch;
+  int64_t stream_cap = items, wg_cap = wgs, gemm_cap = st.gemm_items, slot_cap = slot;
+  if (graph_rows) {
+    // a workgroup's share, and each request's and prefix's own items and cuts
+    const int64_t most = st.shape.wg_capacity + (graph_rows + graph_rows / 2) *
+                                                    (1 + ceil_div(graph_tokens, st.shape.max_item));
+    stream_cap = most;
+    wg_cap = st.shape.wg_capacity;
+    gemm_cap = cap.items;
+    slot_cap = (int64_t(64) << 20) / (st.num_q_heads * kD * 4) + most + cap.slots;
+  }
+  const int64_t o_info = kHeaderInts;
+  const int64_t o_row_of = o_info + kInfoInts * b.batch;
+  const int64_t o_stream = o_row_of + (by_token ? 0 : ceil_div(tokens, 4) * 4);
+  const int64_t o_gemm = o_stream + kStreamInts * stream_cap;
+  const int64_t o_wg = o_gemm + kGemmInts * gemm_cap;
+  const int64_t total = o_wg + wg_cap + 1;
+  const size_t rows = static_cast<size_t>(slot_cap) * st.num_q_heads;
+  hipError_t err = hipSuccess;
+  if (!st.upload_done) err = hipEventCreateWithFlags(&st.upload_done, hipEventDisableTiming);
+  if (err == hipSuccess) err = hipEventSynchronize(st.upload_done);  // staging is free
+  const bool grows = total * 4 > static_cast<int64_t>(st.ints.capacity) ||
+                     rows * kD * 4 > st.part_o.capacity || rows * 4 > st.part_lse.capacity;
+  if (graph_rows && st.batch && grows) {
+    set_error("graph decode metadata capacity exceeded");
+    return false;
+  }
+  if (err == hipSuccess) err = st.ints.reserve(total * 4, allocations);
+  if (err == hipSuccess) err = st.staging.reserve(total * 4, allocations);
+  if (err == hipSuccess) err = st.part_o.reserve(rows * kD * 4, allocations);
+  if (err == hipSuccess) err = st.part_lse.reserve(rows * 4, allocations);
+  if (err != hipSuccess) {
+    hip_error(err, "shared prefix workspace");
+    return false;
+  }
+  int32_t* host = static_cast<int32_t*>(st.staging.ptr);
+  host[kHeaderGemmItems] = static_cast<int32_t>(st.gemm_items);
+  host[kHeaderStreamWgs] = static_cast<int32_t>(wgs);
+  host[kHeaderOnce] = once;
+  host[3] = 0;
+  for (int64_t r = 0; r < b.batch; ++r) {
+    int32_t* info = host + o_info + kInfoInts * r;
+    for (const Of& of : {prefix_of[r], own_of[r]}) {
+      const Source* src = of.kind == 0 ? nullptr : of.kind == 1 ? &stream[of.index]
+                                                                : &gemm[of.index];
+      info[0] = src ? src->slot : 0;
+      info[1] = src ? src->splits : 0;
+      info[2] = src ? src->tokens : 0;
+      info[3] = src ? src->token0 : 0;
+      info += 4;
+    }
+    if (!by_token)
+      std::fill(host + o_row_of + b.q_start[r], host + o_row_of + b.q_start[r + 1],
+                static_cast<int32_t>(r));
+  }
+  st.prefix_items = st.gemm_items;
+  for (int64_t i = 0, part = 0; i < items; ++i) {
+    const int32_t of = work[4 * i];
+    part = i && work[4 * (i - 1)] == of ? part + 1 : 0;
+    const Source& src = stream[of];
+    const int32_t begin = src.begin + work[4 * i + 1], end = src.begin + work[4 * i + 2];
+    const int32_t out[kStreamInts] = {
+        src.token0, src.tokens,
+        src.page_base + begin / static_cast<int32_t>(st.page_size), begin, end,
+        src.splits ? src.slot + static_cast<int32_t>(part) * src.tokens : -1, src.pos0, 0};
+    std::memcpy(host + o_stream + kStreamInts * i, out, sizeof out);
+    st.prefix_items += src.pos0 == kNoHorizon;
+  }
+  std::copy(wg.begin(), wg.begin() + (stream.empty() ? 0 : wgs + 1), host + o_wg);
+  std::copy(gemm_work.begin(), gemm_work.end(), host + o_gemm);
+  // wg comes last and only its used part is written: a graph plan's unused workgroups leave early.
+  err = hipMemcpyAsync(st.ints.ptr, host, (o_wg + wgs + 1) * 4, hipMemcpyHostToDevice, s);
+  if (err == hipSuccess) err = hipEventRecord(st.upload_done, s);
+  if (err != hipSuccess) {
+    hip_error(err, "shared prefix upload");
+    return false;
+  }
+  st.batch = b.batch;
+  st.tokens = tokens;
+  st.by_token = by_token;
+  if (graph_rows) st.sets = 3;
+  st.stream_grid = graph_rows ? wg_cap : wgs;
+  st.gemm_grid = graph_rows ? gemm_slots(st.cus, st.nw) : st.gemm_items;
+  st.o_info = o_info;
+  st.o_row_of = o_row_of;
+  st.o_stream = o_stream;
+  st.o_gemm = o_gemm;
+  st.o_wg = o_wg;
+  return true;
+}
+
+void SharedPlan::info(int64_t* out4) const {
+  out4[0] = st_->groups_shared;
+  out4[1] = st_->tokens_shared;
+  out4[2] = st_->prefix_items;
+  out4[3] = st_->gemm_items;
+}
+
+namespace {
+template <int DT, int W>
+void launch_stream(const SharedArgs& a, int sets, dim3 grid, hipStream_t s) {
+  if (sets == 1) shared_stream_kernel<DT, W, 1><<<grid, dim3(64 * W), 0, s>>>(a);
+  else if (sets == 2) shared_stream_kernel<DT, W, 2><<<grid, dim3(64 * W), 0, s>>>(a);
+  else shared_stream_kernel<DT, W, 3><<<grid, dim3(64 * W), 0, s>>>(a);
+}
+template <int DT>
+const char* launch_all(const SharedArgs& a, int64_t waves, int sets, dim3 stream_grid,
+                       int64_t gemm_grid, int nw, hipStream_t s) {
+  if (gemm_grid) {
+    const dim3 blocks(static_cast<uint32_t>(gemm_grid));
+    if (nw == 8) shared_gemm_kernel<DT, 8><<<blocks, dim3(512), 0, s>>>(a);
+    else shared_gemm_kernel<DT, 4><<<blocks, dim3(256), 0, s>>>(a);
+    if (const char* err = launch_status("shared_gemm_kernel")) return err;
+  }
+  if (stream_grid.x) {
+    if (waves == 8) launch_stream<DT, 8>(a, sets, stream_grid, s);
+    else if (waves == 4) launch_stream<DT, 4>(a, sets, stream_grid, s);
+    else if (waves == 2) launch_stream<DT, 2>(a, sets, stream_grid, s);
+    else launch_stream<DT, 1>(a, sets, stream_grid, s);
+    if (const char* err = launch_status("shared_stream_kernel")) return err;
+  }
+  shared_merge_kernel<DT><<<dim3(static_cast<uint32_t>((a.rows + 7) / 8)), dim3(256), 0, s>>>(a);
   return launch_status("shared_merge_kernel");
+}
+}  // namespace
+
+const char* SharedPlan::run(const int32_t* indices, const void* q, int64_t q_sn, int64_t q_sh,
+                            const void* k, const void* v, void* out, int64_t o_sn, int64_t o_sh,
+                            hipStream_t s) const {
+  const State& st = *st_;
+  const int32_t* ints = static_cast<const int32_t*>(st.ints.ptr);
+  SharedArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_sn = q_sn;
+  a.q_sh = q_sh;
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.out = static_cast<uint16_t*>(out);
+  a.o_sn = o_sn;
+  a.o_sh = o_sh;
+  a.header = ints;
+  a.info = reinterpret_cast<const int4*>(ints + st.o_info);
+  a.row_of = st.by_token ? nullptr : ints + st.o_row_of;
+  a.stream_work = reinterpret_cast<const int4*>(ints + st.o_stream);
+  a.stream_wg = ints + st.o_wg;
+  a.gemm_work = reinterpret_cast<const int4*>(ints + st.o_gemm);
+  a.indices = indices;
+  a.part_o = static_cast<float*>(st.part_o.ptr);
+  a.part_lse = static_cast<float*>(st.part_lse.ptr);
+  a.rows = st.tokens * st.num_q_heads;
+  a.num_q_heads = static_cast<int32_t>(st.num_q_heads);
+  a.num_kv_heads = static_cast<int32_t>(st.num_kv_heads);
+  a.group_log2 = st.group_log2;
+  a.page_size = static_cast<int32_t>(st.page_size);
+  a.scale_log2 = (1.0f / std::sqrt(static_cast<float>(kD))) * kLog2e;
+  const dim3 stream_grid(static_cast<uint32_t>(st.stream_grid),
+                         static_cast<uint32_t>(st.shape.grid_y));
+  return st.dtype == 0
+             ? launch_all<0>(a, st.shape.waves, st.sets, stream_grid, st.gemm_grid, st.nw, s)
+             : launch_all<1>(a, st.shape.waves, st.sets, stream_grid, st.gemm_grid, st.nw, s);
 }
 
 }  // namespace mi355x

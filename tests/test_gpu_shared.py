@@ -46,7 +46,7 @@ def test_decode(gpu, groups, own, heads, kv_heads, page, dtype, copies):
     got, info = b.run(b.decode_meta())
     print(f"[shared] {info} worst {b.check(got):.2f} of the limit", flush=True)
     plain, none = b.run(b.decode_meta(shared=False))
-    assert none["waves"] == 0
+    assert none["items"] == 0
     b.check(plain)
 
 
@@ -74,7 +74,7 @@ def test_extend(gpu, groups, own, new, heads, kv_heads, page, dtype):
     print(f"[shared] {info} worst {b.check(got):.2f} of the limit", flush=True)
     assert info["groups"] == sum(r > 1 and n >= 64 for r, n in groups)
     plain, none = b.run(b.extend_meta(shared=False))
-    assert none["waves"] == 0
+    assert none["items"] == 0
     b.check(plain)
 
 
@@ -92,7 +92,7 @@ def test_strided_queries_and_output(gpu):
     packed[:, :16 * 128] = b.q.view(6, -1)
     attention, q = b.attention(), packed[:, :16 * 128].view(6, 16, 128)
     batch = attention.prepare(b.decode_meta(), 6)
-    assert batch.plan.plan.shared_info()["waves"]
+    assert batch.plan.plan.shared_info()["items"]
     out = torch.full((7, 16 * 128), 7.0, dtype=BF16, device="cuda")
     batch.forward_into(q, None, None, b.cache(), out[:6])
     b.check(out[:6].view(6, 16, 128))
@@ -119,7 +119,7 @@ def test_nan_of_one_row_stays_there(gpu):
     flat = b.k.view(-1, 8, 128)
     flat[b.slots[2][270]] = float("nan")
     got, info = b.run(b.decode_meta())
-    assert info["waves"]
+    assert info["items"]
     bad = torch.isnan(got.float()).flatten(1).any(1).tolist()
     assert bad == [False, False, True, False, False, False, False]
     flat[b.slots[4][100]] = float("nan")
@@ -149,7 +149,7 @@ def test_offsets_past_4_gib(gpu):
     b.table[b.table >= 0] += far
     b.slots = [s + far * 16 for s in b.slots]
     got, info = b.run(b.decode_meta())
-    assert info["waves"]
+    assert info["items"]
     b.check(got)
 
 
@@ -227,7 +227,7 @@ def test_graph_prepared_without_groups_ignores_them(gpu):
     state = attention.prepare_decode_graph(meta)
     batch = attention.prepare(meta, 4)
     state.prepare_replay(DecodeHostMetadata(b.keys), b.shared())
-    assert state.plan.shared_info()["waves"] == 0
+    assert state.plan.shared_info()["items"] == 0
     b.check(batch.forward(b.q, None, None, b.cache()).view(b.q.shape))
 
 
