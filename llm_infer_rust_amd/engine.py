@@ -24,6 +24,11 @@ Mirrors the parts of the reference engine that feed the attention hot path:
 * the CPU/GPU overlap of consecutive decode steps (``scheduler.rs:935-1000`` step_overlap):
   the next graph step is launched with its input tokens copied on the device from this step's
   sampling output, before the host reads them (``Engine._launch_ahead``).
+
+Beyond the reference, ``SamplingParams.n`` draws several completions of one prompt: it is prefilled
+once, then forked (``Engine._fork``: whole pages are held by all, the page it ends in is copied), and
+with ``EngineConfig.share_prefixes`` decode attention over it is computed once for all of them.
+``SamplingParams.logprobs`` keeps every token's log probability and the likeliest alternatives.
 """
 from __future__ import annotations
 
@@ -35,11 +40,12 @@ import numpy as np
 import torch
 
 from . import _native
-from .backend import AttentionMetadata, BatchPhase, DecodeHostMetadata
+from .backend import AttentionMetadata, BatchPhase, DecodeHostMetadata, SharedPrefix
 from .batch import BatchContext, BatchRequest, DecodeBatch, DecodeRequest, DecodeTables
 from .kv_cache import KVCacheLayout, KVCachePool, ModelError
 from .model import Qwen3Model
-from .sampling import Sampler, SamplingParams
+from .sampling import (MAX_TOP_LOGPROBS, PendingLogprobs, Sampler, SamplingParams, TokenDetail,
+                       token_logprobs)
 
 
 @dataclass
@@ -57,6 +63,10 @@ class EngineConfig:
     # length). False: the serial step of ``scheduler.rs:225-271`` every time.
     overlap_decode: bool = True
     seed: int = 0
+    # Compute decode attention over the prompt that completions of a request share (SamplingParams.n)
+    # once for all of them. Decode graphs are then captured in a form that can; a step that shares
+    # nothing takes slightly longer in it than in the form that cannot.
+    share_prefixes: bool = False
 
 
 @dataclass(eq=False)
@@ -72,6 +82,16 @@ class Request:
     arrival: float = 0.0
     first_token_time: float | None = None
     finish_time: float | None = None
+    # All completions of the prompt, this request's own among them; the first one is prefilled and
+    # the others are forked from it. One alone: a list of itself.
+    completions: list["Request"] = field(default_factory=list, repr=False)
+    details: list[TokenDetail] = field(default_factory=list)  # with params.logprobs, one a token
+
+    @property
+    def slots(self) -> int:
+        """Running slots it takes: those of completions still to be forked from it included."""
+        unforked = len(self.completions) if self.completions[:1] == [self] and not self.output else 1
+        return max(unforked, 1)
 
     @property
     def cached_len(self) -> int:
@@ -88,10 +108,12 @@ class Request:
 
 
 class PageAllocator:
-    """Physical pages 1..num_pages; page 0 is the reserved zero page."""
+    """Physical pages 1..num_pages; page 0 is the reserved zero page. A page may have several
+    holders; it is free again when the last one has released it."""
 
     def __init__(self, num_pages: int):
         self.free = list(range(num_pages, 0, -1))
+        self.more_holders: dict[int, int] = {}  # of pages with more than one: how many more
 
     def alloc(self, n: int) -> list[int]:
         if n > len(self.free):
@@ -100,8 +122,23 @@ class PageAllocator:
         del self.free[len(self.free) - n:]
         return out
 
+    def share(self, pages: list[int]) -> None:
+        """One more holder of each page."""
+        for p in pages:
+            self.more_holders[p] = self.more_holders.get(p, 0) + 1
+
     def release(self, pages: list[int]) -> None:
-        self.free.extend(reversed(pages))
+        if not self.more_holders:
+            self.free.extend(reversed(pages))
+            return
+        for p in reversed(pages):
+            more = self.more_holders.get(p, 0)
+            if more == 0:
+                self.free.append(p)
+            elif more == 1:
+                del self.more_holders[p]
+            else:
+                self.more_holders[p] = more - 1
 
 
 def _words(a: np.ndarray) -> np.ndarray:
@@ -166,6 +203,7 @@ class _Ahead:
     graph: _DecodeGraph
     host: np.ndarray
     lens: np.ndarray
+    shared: SharedPrefix | None
 
     def same_rows(self, rows: list) -> bool:
         """Staged for exactly these rows, in this order (none of them ends by length)."""
@@ -208,7 +246,7 @@ class Engine:
         self._pending_rows: list[Request] | None = None
         self.graphs: dict[int, _DecodeGraph] = {}
         self.stats = {"prefill_batches": 0, "decode_steps": 0, "graph_steps": 0,
-                      "ahead_steps": 0, "overlap_steps": 0}
+                      "ahead_steps": 0, "overlap_steps": 0, "forks": 0}
         if cfg.use_graphs:
             self.capture_graphs()
 
@@ -221,10 +259,55 @@ class Engine:
             raise ModelError("prompt must be a non-empty 1-D id list")
         if prompt.size + params.max_tokens > self.cfg.max_seq_len:
             raise ModelError("prompt + max_tokens exceeds max_seq_len")
-        req = Request(self._next_uid, prompt, params, eos_token_id, arrival=time.perf_counter())
-        self._next_uid += 1
-        self.waiting.append(req)
-        return req
+        if params.n > self.cfg.max_running_req:
+            raise ModelError("more completions than running requests")
+        if params.logprobs is not None and not 0 <= params.logprobs <= MAX_TOP_LOGPROBS:
+            raise ModelError(f"logprobs must be 0 to {MAX_TOP_LOGPROBS}")
+        now = time.perf_counter()
+        completions = [Request(self._next_uid + i, prompt, params, eos_token_id, arrival=now)
+                       for i in range(params.n)]
+        for r in completions:
+            r.completions = completions
+        self._next_uid += params.n
+        self.waiting.append(completions[0])
+        return completions[0]
+
+    def _fork(self, leader: Request) -> list[Request]:
+        """The other completions of a prefilled prompt join the running requests right behind it.
+        Its whole pages get more holders; the page it ends in is copied for each."""
+        others = leader.completions[1:]
+        whole, rest = divmod(leader.prompt.size, self.page_size)
+        own = self.pages.alloc(len(others)) if rest else []
+        at = self.running.index(leader)
+        self.running[at + 1:at + 1] = others
+        for i, req in enumerate(others):
+            self.pages.share(leader.pages[:whole])
+            req.pages = leader.pages[:whole] + own[i:i + 1]
+            req.cursor = leader.cursor
+            req.admitted = True
+        if rest:
+            self.pool.copy_pages([leader.pages[whole]] * len(others), own, [rest] * len(others))
+        self.stats["forks"] += len(others)
+        return others
+
+    def _shared(self, rows: list[Request], batch: int | None = None) -> SharedPrefix | None:
+        """Neighbouring rows that are completions of one prompt, for the attention plan; ``batch``
+        counts pad rows too."""
+        if not self.cfg.share_prefixes:
+            return None
+        sizes, lens, last = [], [], None
+        for r in rows:
+            if last is not None and r.completions is last:
+                sizes[-1] += 1
+                continue
+            last = r.completions
+            sizes.append(1)
+            lens.append(r.prompt.size)
+        lens = [n if size > 1 else 0 for n, size in zip(lens, sizes)]
+        if batch is not None and batch > len(rows):
+            sizes.append(batch - len(rows))
+            lens.append(0)
+        return SharedPrefix(sizes, lens)
 
     def _ensure_pages(self, req: Request, tokens: int) -> None:
         need = -(-tokens // self.page_size) - len(req.pages)
@@ -274,16 +357,16 @@ class Engine:
     def _select_prefill(self) -> list[tuple[Request, int]]:
         budget = self.cfg.max_prefill_tokens_per_batch
         picked: list[tuple[Request, int]] = []
-        admitted = len(self.running)
+        admitted = sum(r.slots for r in self.running)
         # A chunked request continues first (scheduler/prefill.rs select_continuation).
         queue = [r for r in self.running if r.cursor < r.prompt.size] + self.waiting
         for req in queue:
             if budget <= 0:
                 break
             if not req.admitted:
-                if admitted >= self.cfg.max_running_req:
+                if admitted + req.slots > self.cfg.max_running_req:
                     break
-                admitted += 1
+                admitted += req.slots
             remaining = req.prompt.size - req.cursor
             take = min(remaining, budget)
             if take < remaining:  # chunks end on a page boundary
@@ -321,6 +404,11 @@ class Engine:
             req.cursor += take
         done = [req for req, _ in picked if req.cursor == req.prompt.size]
         self.stats["prefill_batches"] += 1
+        if any(len(req.completions) > 1 for req in done):  # a row of logits for every completion
+            rows = [i for i, req in enumerate(done) for _ in req.completions]
+            logits = logits.index_select(0, self._upload(np.asarray(rows, np.int64))[0])
+            done = [r for req in done for r in ([req] + self._fork(req) if len(req.completions) > 1
+                                                else [req])]
         if done:
             self._sample_and_commit(logits, done)
 
@@ -350,7 +438,7 @@ class Engine:
                 self.stats["ahead_steps"] += 1
             else:
                 host, lens = self._stage_replay(graph, self._decode_batch(rows))
-            self._launch_replay(graph, host, lens)
+            self._launch_replay(graph, host, lens, self._shared(rows, graph.bs))
             logits = graph.logits[:n]
             self.stats["graph_steps"] += 1
         else:
@@ -359,7 +447,7 @@ class Engine:
                 b.input_ids, b.positions, b.write_loc, b.cache_seqlens, b.block_table)
             meta = AttentionMetadata(BatchPhase.DECODE, decode_host=DecodeHostMetadata(
                 b.cache_seqlens.tolist()), write_loc=loc_d, block_table=table_d,
-                cache_seqlens=lens_d)
+                cache_seqlens=lens_d, shared_prefix=self._shared(rows))
             batch = self.model.attention.prepare(meta, n)
             logits = self.model.forward(ids_d, pos_d, batch, loc_d)
             del batch
@@ -389,7 +477,8 @@ class Engine:
                 self._ensure_pages(req, length)
             reqs.append(DecodeRequest(req.uid, length, 0, req.pages))
         host, lens = self._stage_replay(graph, self.tables.prepare(reqs))
-        self._ahead = _Ahead([r.uid for r in nxt], lengths, graph, host, lens)
+        self._ahead = _Ahead([r.uid for r in nxt], lengths, graph, host, lens,
+                             self._shared(nxt, graph.bs))
 
     def _launch_ahead(self, pending, rows: list[Request]) -> _InFlight | None:
         """Launch the staged step now when it decodes exactly this step's rows: its words go
@@ -404,12 +493,18 @@ class Engine:
         g, n = ahead.graph, len(rows)
         self._send(ahead.host.size, g.block)
         torch.clamp(pending.ids, min=0, out=g.input_ids[:n])
-        g.state.prepare_replay(DecodeHostMetadata(ahead.lens))
+        g.state.prepare_replay(DecodeHostMetadata(ahead.lens), ahead.shared)
         g.graph.replay()
         return _InFlight(rows, g)
 
     def _sample_and_commit(self, logits: torch.Tensor, rows: list[Request]) -> None:
         pending = self.sampler.defer_batch(logits, [r.params for r in rows])
+        # Before the next step is launched, which writes its logits over these.
+        wanted = [r.params.logprobs for r in rows if r.params.logprobs is not None]
+        details = None
+        if wanted:
+            details = PendingLogprobs(token_logprobs(
+                logits, pending.ids, top=min(max(wanted), logits.size(1))))
         ahead_rows, self._pending_rows = self._pending_rows, None
         inflight = None
         if ahead_rows is not None:
@@ -418,6 +513,10 @@ class Engine:
         ids = pending.finish()
         now = time.perf_counter()
         done = []
+        if details is not None:
+            for req, d in zip(rows, details.finish()):
+                if req.params.logprobs is not None:
+                    req.details.append(d._replace(top=d.top[:req.params.logprobs]))
         for req, tok in zip(rows, ids):
             req.output.append(tok)
             if req.first_token_time is None:
@@ -477,7 +576,8 @@ class Engine:
         for bs in sorted(self._bucket_sizes(), reverse=True):
             g = _DecodeGraph(bs, self.cols, model.cfg.vocab_size, self.device, model.dtype)
             meta = AttentionMetadata(BatchPhase.DECODE, write_loc=g.write_loc,
-                                     block_table=g.block_table, cache_seqlens=g.cache_seqlens)
+                                     block_table=g.block_table, cache_seqlens=g.cache_seqlens,
+                                     shared_prefix=self._shared([], bs))
             g.state = model.attention.prepare_decode_graph(meta)
             g.state.prepare_replay(DecodeHostMetadata([1] * bs))
             g.batch = model.attention.prepare(meta, bs)
@@ -515,10 +615,11 @@ class Engine:
         table[n:] = 0
         return host, lens
 
-    def _launch_replay(self, g: _DecodeGraph, host: np.ndarray, lens: np.ndarray) -> None:
+    def _launch_replay(self, g: _DecodeGraph, host: np.ndarray, lens: np.ndarray,
+                       shared: SharedPrefix | None) -> None:
         """One copy into the graph's inputs, the host-length re-plan, the replay."""
         self._send(host.size, g.block)
-        g.state.prepare_replay(DecodeHostMetadata(lens))
+        g.state.prepare_replay(DecodeHostMetadata(lens), shared)
         g.graph.replay()
 
     # ------------------------------------------------------------------ loop

@@ -45,10 +45,14 @@ class SamplingParams:
     top_p: float = 1.0
     ignore_eos: bool = False
     max_tokens: int = 1024
+    # Completions of the prompt, and how many alternatives every token's log probability comes with
+    # (None: no log probabilities). The reference draws one completion and returns its ids.
+    n: int = 1
+    logprobs: int | None = None
 
     def normalized(self) -> "SamplingParams":
         top_p = self.top_p if (math.isfinite(self.top_p) and 0.0 <= self.top_p <= 1.0) else 1.0
-        return replace(self, max_tokens=max(self.max_tokens, 1), top_p=top_p)
+        return replace(self, max_tokens=max(self.max_tokens, 1), top_p=top_p, n=max(self.n, 1))
 
 
 # The split sampler cuts rows with a top_k up to this among their listed largest logits. A
@@ -136,6 +140,31 @@ class PendingSample:
         if any(i < 0 for i in ids):
             raise SamplingError("invalid probability distribution")
         return ids
+
+
+class TokenDetail(NamedTuple):
+    """A sampled token's log probability, the entropy of its distribution and the most likely tokens
+    there with theirs, in nats, before any temperature."""
+    logprob: float
+    entropy: float
+    top: list[tuple[int, float]]
+
+
+class PendingLogprobs:
+    """Log probabilities on their way to pinned host memory behind an event."""
+
+    def __init__(self, values: "TokenLogprobs"):
+        self._values = values  # keeps them alive until the copies have run
+        self._host = [torch.empty(t.shape, dtype=t.dtype, pin_memory=True) for t in values]
+        for host, t in zip(self._host, values):
+            host.copy_(t, non_blocking=True)
+        self._event = torch.cuda.Event()
+        self._event.record(torch.cuda.current_stream(values.logprobs.device))
+
+    def finish(self) -> list[TokenDetail]:
+        self._event.synchronize()
+        lp, entropy, ids, top = (t.tolist() for t in self._host)
+        return [TokenDetail(a, e, list(zip(i, t))) for a, e, i, t in zip(lp, entropy, ids, top)]
 
 
 class Sampler:
@@ -292,4 +321,4 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     return out
 
 
-__all__ = ["TokenLogprobs", "token_logprobs", "SamplingParams", "Sampler", "PendingSample", "SamplingError"]
+__all__ = ["TokenLogprobs", "TokenDetail", "PendingLogprobs", "token_logprobs", "SamplingParams", "Sampler", "PendingSample", "SamplingError"]
