@@ -9,9 +9,9 @@
 // the prefix's keys as one matrix product, where plain decode reads the prefix once a request. Two
 // kernels, by the number of columns:
 //
-// shared_stream_kernel, up to 48 columns: the decode kernel's copy pipeline (tiles of 16 whole K and
-// V rows through an LDS ring, one wave a kv head) with up to three sets of 16 columns on the tile a
-// wave has in LDS. Streaming a tile takes a CU longer than three sets of products on it, so it is
+// shared_stream_kernel, up to 32 columns: the decode kernel's copy pipeline (tiles of 16 whole K and
+// V rows through an LDS ring, one wave a kv head) with up to two sets of 16 columns on the tile a
+// wave has in LDS. Streaming a tile takes a CU longer than two sets of products on it, so it is
 // bound by memory, as decode is. The own keys of requests with few new tokens are items of the same
 // launch, under the same balanced schedule.
 //
@@ -66,7 +66,7 @@ struct SharedArgs {
   float* part_o;
   float* part_lse;
   int64_t rows;           // tokens * q heads
-  int32_t num_q_heads, num_kv_heads, group_log2, page_size;
+  int32_t num_q_heads, num_kv_heads, group_log2, page_size, gemm_grid;
   float scale_log2;
 };
 
@@ -76,7 +76,7 @@ struct SharedArgs {
 constexpr int kStreamTile = 16;
 constexpr int kStreamStages = 2;
 constexpr int kStreamEntries = 2048;  // page entries of an item in LDS
-constexpr int kStreamColumns = 48;  // three sets: a fourth does not fit the registers
+constexpr int kStreamColumns = 32;  // two sets: a third does not fit the registers
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
@@ -101,10 +101,11 @@ __device__ __forceinline__ floatx4 mma_16x16x16(const uint2& a, const uint2& b, 
                                                  __builtin_bit_cast(f16x4_t, b), c, 0, 0, 0);
 }
 
-// W waves, one a kv head of the slice blockIdx.y; SETS: sets of 16 columns an item may have. Tiles
+// W waves, one a kv head of the slice; SETS: sets of 16 columns an item may have. Tiles
 // lie in LDS as decode_mma_kernel's: 16-byte chunk c of a head's 256 bytes at c ^ (token & 15).
 template <int DT, int W, int SETS, bool ONCE>
-__device__ __forceinline__ void stream_items(const SharedArgs& a, uint8_t* lds, int32_t* entries) {
+__device__ __forceinline__ void stream_items(const SharedArgs& a, uint8_t* lds, int32_t* entries,
+                                             int wg, int slice) {
   constexpr int T = kStreamTile;
   constexpr int kRow = W * 256;              // bytes of one token's slice (K or V)
   constexpr int kHalf = T * kRow;            // K (or V) bytes of a tile
@@ -115,14 +116,14 @@ __device__ __forceinline__ void stream_items(const SharedArgs& a, uint8_t* lds, 
   const int lane = threadIdx.x & 63;
   const int col = lane & 15;   // column of a set / operand row
   const int quad = lane >> 4;  // 16-lane group
-  const int h = blockIdx.y * W + wave;
+  const int h = slice * W + wave;
   const int G = 1 << a.group_log2;
   const uint32_t lds_base = lds_address(lds);
   const uint32_t entries_lds = lds_address(entries);
   const uint32_t row_elems = static_cast<uint32_t>(a.num_kv_heads) * kD;
-  const uint16_t* kslice = a.k + blockIdx.y * W * kD;
-  const uint16_t* vslice = a.v + blockIdx.y * W * kD;
-  const int item_begin = a.stream_wg[blockIdx.x], item_end = a.stream_wg[blockIdx.x + 1];
+  const uint16_t* kslice = a.k + slice * W * kD;
+  const uint16_t* vslice = a.v + slice * W * kD;
+  const int item_begin = a.stream_wg[wg], item_end = a.stream_wg[wg + 1];
 
   for (int item = item_begin; item < item_end; ++item) {
     const bool first_item = item == item_begin;
@@ -217,37 +218,49 @@ __device__ __forceinline__ void stream_items(const SharedArgs& a, uint8_t* lds, 
             __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)vp));
       }
       const int key0 = beg + t * T + 4 * quad;
+      // The steps of the sets side by side.
+      floatx4 sc[SETS];
+#pragma unroll
+      for (int c = 0; c < SETS; ++c) sc[c] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int c = 0; c < SETS; ++c) sc[c] = mma_16x16x32<DT>(kf[kk], qb[c][kk], sc[c]);
+      // The lane holds S[key0 + i][column].
+      float s[SETS][4], mx[SETS], corr[SETS];
 #pragma unroll
       for (int c = 0; c < SETS; ++c) {
-        if (c >= sets) break;  // uniform
-        floatx4 sc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) sc = mma_16x16x32<DT>(kf[kk], qb[c][kk], sc);
-        // The lane holds S[key0 + i][column].
-        float s[4];
-        float mx = m[c];
+        mx[c] = m[c];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[i] = key0 + i <= limit[c] ? sc[i] * a.scale_log2 : -INFINITY;
-          mx = fmaxf(mx, s[i]);
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float corr = __builtin_amdgcn_exp2f(m[c] - mx);
-        m[c] = mx;
-        float p[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(s[i] - mx);
-        l[c] = l[c] * corr + ((p[0] + p[1]) + (p[2] + p[3]));
-        // rounded to the type of V for the product; the sum takes the fp32 values
-        const uint2 pb = make_uint2(Elem<DT>::pack2(p[0], p[1]), Elem<DT>::pack2(p[2], p[3]));
-#pragma unroll
-        for (int b = 0; b < 8; ++b) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[c][b][i] *= corr;
-          o[c][b] = mma_16x16x16<DT>(vf[b], pb, o[c][b]);
+          s[c][i] = key0 + i <= limit[c] ? sc[c][i] * a.scale_log2 : -INFINITY;
+          mx[c] = fmaxf(mx[c], s[c][i]);
         }
       }
+#pragma unroll
+      for (int c = 0; c < SETS; ++c) mx[c] = fmaxf(mx[c], __shfl_xor(mx[c], 16));
+#pragma unroll
+      for (int c = 0; c < SETS; ++c) mx[c] = fmaxf(mx[c], __shfl_xor(mx[c], 32));
+      uint2 pb[SETS];
+#pragma unroll
+      for (int c = 0; c < SETS; ++c) {
+        corr[c] = __builtin_amdgcn_exp2f(m[c] - mx[c]);
+        m[c] = mx[c];
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(s[c][i] - mx[c]);
+        l[c] = l[c] * corr[c] + ((p[0] + p[1]) + (p[2] + p[3]));
+        // rounded to the type of V for the product; the sum takes the fp32 values
+        pb[c] = make_uint2(Elem<DT>::pack2(p[0], p[1]), Elem<DT>::pack2(p[2], p[3]));
+      }
+#pragma unroll
+      for (int b = 0; b < 8; ++b)
+#pragma unroll
+        for (int c = 0; c < SETS; ++c) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[c][b][i] *= corr[c];
+          o[c][b] = mma_16x16x16<DT>(vf[b], pb[c], o[c][b]);
+        }
     }
 #pragma unroll
     for (int c = 0; c < SETS; ++c) {
@@ -282,22 +295,6 @@ __device__ __forceinline__ void stream_items(const SharedArgs& a, uint8_t* lds, 
   }
 }
 
-template <int DT, int W, int SETS>
-__global__ __launch_bounds__(64 * W, 2) void shared_stream_kernel(SharedArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint8_t
-      lds[kStreamStages * 2 * kStreamTile * W * 256];
-  __shared__ int32_t entries[kStreamEntries];
-  if (static_cast<int>(blockIdx.x) >= a.header[kHeaderStreamWgs]) return;  // graph plans' grids
-  if (a.num_kv_heads < 0) {  // the copies are invisible to the compiler
-    lds[threadIdx.x] = 0;
-    entries[threadIdx.x] = 0;
-  }
-  if (a.header[kHeaderOnce])  // uniform
-    stream_items<DT, W, SETS, true>(a, lds, entries);
-  else
-    stream_items<DT, W, SETS, false>(a, lds, entries);
-}
-
 // ---------------------------------------------------------------------------
 // Many columns: matrix products of 32 columns a wave.
 // ---------------------------------------------------------------------------
@@ -307,19 +304,19 @@ constexpr int kStageBytes = 2 * kTileBytes;  // K + V
 
 // K and V tiles lie in LDS as the prefill kernel's do: [key][d], 16-byte chunk c of key r at
 // c ^ (r & 15) (K) and c ^ 4 (r & 3) (V), which keeps the operand reads free of bank conflicts.
+// NW waves: 8 read K and V once for 256 columns through a ring of four tiles; 4 leave half of the CU
+// to another workgroup.
 template <int DT, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_gemm_kernel(SharedArgs a) {
-  constexpr int kStages = NW == 8 ? 4 : 2;
+__device__ __forceinline__ void gemm_items(const SharedArgs& a, uint8_t* lds, int first_item,
+                                           int step) {
+  constexpr int kStages = NW / 2;
   constexpr int kAhead = kStages - 1;
   constexpr int kGroupsPerWave = 16 / NW;  // 4-row groups of each tile this wave copies
   constexpr int kCopiesPerTile = 2 * kGroupsPerWave;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * kStageBytes];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int col = lane & 31;
   const int half = lane >> 5;
-  // The copies are invisible to the compiler: one store it sees, never taken.
-  if (a.num_kv_heads < 0) lds[threadIdx.x] = 0;
   const uint32_t lds_base = lds_address(lds);
   const int64_t slot_stride = static_cast<int64_t>(a.num_kv_heads) * kD;
   const float inv_page = 1.0f / static_cast<float>(a.page_size);
@@ -327,7 +324,6 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_gemm_kernel(S
       a.page_size >= 4 && a.page_size <= kTileK && kTileK % a.page_size == 0;
   const int pages_per_tile = fast_pages ? kTileK / a.page_size : 0;
   const float c = a.scale_log2;
-  const float lazy_limit = 8.f / c;  // 2^8 in p
 
   // Operand read offsets, as in the prefill kernel.
   const int gq = lane >> 4;
@@ -341,9 +337,10 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_gemm_kernel(S
                 8 * (p16 & 1);
   const int row_in_group = lane >> 4;
   const int pos = lane & 15;
+  const int heads = 1 << a.group_log2;
 
   const int items = a.header[kHeaderGemmItems];
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+  for (int item = first_item; item < items; item += step) {
     const int4* work = a.gemm_work + kGemmInts / 4 * item;
     const int4 w0 = work[0], w1 = work[1], w2 = work[2];
     const int token0 = w0.x, rows = w0.y, row0 = w0.z, kvh = w0.w;
@@ -351,15 +348,15 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_gemm_kernel(S
     const int pos0 = w2.x, kv_len = w2.y;
     const int my_row0 = row0 + wave * 32;
     const bool wave_active = my_row0 < rows;
-    const int my_row = min(my_row0 + col, rows - 1);
-    const int token = my_row >> a.group_log2;
-    const int qh = (kvh << a.group_log2) + (my_row - (token << a.group_log2));
-    const int horizon = pos0 + token;  // the last key this row sees
     const int first_horizon = pos0 + (my_row0 >> a.group_log2);
     const int last_horizon = pos0 + (min(my_row0 + 31, rows - 1) >> a.group_log2);
+    const int row = min(my_row0 + col, rows - 1);
+    const int token = row >> a.group_log2;
+    const int horizon = min(pos0 + token, kv_len - 1);  // the last key the column sees
 
     uint4 qreg[8];
     {
+      const int qh = (kvh << a.group_log2) + (row & (heads - 1));
       const uint16_t* qp = a.q + static_cast<int64_t>(token0 + token) * a.q_sn + qh * a.q_sh;
 #pragma unroll
       for (int s = 0; s < 8; ++s) qreg[s] = ld128(qp + 16 * s + 8 * half);
@@ -390,9 +387,9 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_gemm_kernel(S
         int off;
         const int sel = div_small(key, a.page_size, inv_page, off) - p0;
         const int page = sel == 0 ? i0 : sel == 1 ? i1 : sel == 2 ? i2 : i3;
-        const int64_t slot = static_cast<int64_t>(page) * a.page_size + off;
-        copy_to_lds(k_head + slot * slot_stride + (pos ^ (row & 15)) * 8, sbase + g * 1024);
-        copy_to_lds(v_head + slot * slot_stride + (pos ^ (4 * (row & 3))) * 8,
+        const int64_t at = static_cast<int64_t>(page) * a.page_size + off;
+        copy_to_lds(k_head + at * slot_stride + (pos ^ (row & 15)) * 8, sbase + g * 1024);
+        copy_to_lds(v_head + at * slot_stride + (pos ^ (4 * (row & 3))) * 8,
                     sbase + kTileBytes + g * 1024);
       }
     };
@@ -428,15 +425,13 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_gemm_kernel(S
     };
 
     floatx16 o[4];
+    // ref: the lane's reference, in log2 units; p = 2^(c s - ref), one fma a score. Its rounding
+    // scales p and the sums alike.
+    float ref = 0.f, l = 0.f;
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
-    // m: this lane's reference of the raw scores; the accumulators start at -m, p = 2^(c (s - m)).
-    float m = 0.f, l = 0.f;
-    floatx16 negm;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) negm[r] = 0.f;
 
     auto compute = [&](int t, int stage, bool first) {
       const int k0 = t * kTileK;
@@ -451,12 +446,15 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_gemm_kernel(S
               sb + (32 * T + col) * 256 + (((2 * kk + half) ^ (col & 15)) * 16));
       floatx16 s[2];
 #pragma unroll
+      for (int T = 0; T < 2; ++T)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[T][r] = 0.f;
+#pragma unroll
       for (int kk = 0; kk < 8; ++kk)
 #pragma unroll
-        for (int T = 0; T < 2; ++T)
-          s[T] = Mfma<DT>::run(kf[T][kk], qreg[kk], kk == 0 ? negm : s[T]);
+        for (int T = 0; T < 2; ++T) s[T] = Mfma<DT>::run(kf[T][kk], qreg[kk], s[T]);
       if (k0 + kTileK - 1 > first_horizon || k0 + kTileK > kv_len) {
-        const int limit = min(horizon, kv_len - 1) - (k0 + 4 * half);
+        const int limit = horizon - (k0 + 4 * half);
 #pragma unroll
         for (int T = 0; T < 2; ++T)
 #pragma unroll
@@ -473,25 +471,20 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_gemm_kernel(S
       {
         const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx),
                                                           false, false);
-        mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * c;
       }
-      // m moves on the first tile and then only when a row's maximum passes it by 8 / c. A first
-      // tile wholly past a row's horizon (mx = -inf) leaves m at 0.
-      if (first || __any(mx > lazy_limit)) {
-        const float shift = first ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
-        const float alpha = first ? 1.f : __builtin_amdgcn_exp2f(-shift * c);
-        m += shift;
+      // The reference moves on the first tile and then only when a row's maximum passes it by 8, so
+      // that p stays below 2^8. A first tile wholly past a row's horizon leaves it at 0.
+      if (first || __any(mx > ref + 8.f)) {
+        const float to = first ? (mx == -INFINITY ? 0.f : mx) : fmaxf(ref, mx);
+        // nothing is accumulated before the first tile
+        const float alpha = first ? 1.f : __builtin_amdgcn_exp2f(ref - to);
+        ref = to;
         l *= alpha;
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[0][r] -= shift;
-          s[1][r] -= shift;
-          negm[r] = -m;
-        }
       }
       uint4 pb[4];
       float ls[4] = {0.f, 0.f, 0.f, 0.f};
@@ -502,7 +495,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_gemm_kernel(S
           float p[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(s[T][8 * hh + i] * c);
+            p[i] = __builtin_amdgcn_exp2f(fmaf(s[T][8 * hh + i], c, -ref));
             ls[i & 3] += p[i];
           }
           // rounded to the type of V for the product; the row sums take the fp32 values
@@ -549,7 +542,6 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_gemm_kernel(S
           *reinterpret_cast<float4*>(tile + col * 512 + ((8 * db + 2 * g4 + half) ^ col) * 16) =
               make_float4(o[db][4 * g4] * inv, o[db][4 * g4 + 1] * inv, o[db][4 * g4 + 2] * inv,
                           o[db][4 * g4 + 3] * inv);
-      const int heads = 1 << a.group_log2;
       auto part_row = [&](int r) {  // partial row of the wave's row r
         const int t = (my_row0 + r) >> a.group_log2;
         return static_cast<int64_t>(slot + t) * a.num_q_heads + (kvh << a.group_log2) +
@@ -565,10 +557,63 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void shared_gemm_kernel(S
       }
       if (half == 0 && my_row0 + col < rows)
         a.part_lse[part_row(col)] =
-            row_sum == 0.f ? -INFINITY : m * c + __builtin_amdgcn_logf(row_sum);
+            row_sum == 0.f ? -INFINITY : ref + __builtin_amdgcn_logf(row_sum);
     }
     __syncthreads();  // the next item's copies overwrite the ring
   }
+}
+
+// Both in one launch, where a slice of four kv heads lets a workgroup of either kind have half of a
+// CU: the products of one hide behind the copies of the other. The first gemm_grid workgroups take
+// the products, one a CU; the others stream, and have the CUs to themselves afterwards.
+template <int DT, int SETS>
+__global__ __launch_bounds__(256, 2) void shared_kernel(SharedArgs a) {
+  constexpr int kRing = kStreamStages * 2 * kStreamTile * 4 * 256;
+  static_assert(kRing == 2 * kStageBytes, "either ring");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kRing];
+  __shared__ int32_t entries[kStreamEntries];
+  if (a.num_kv_heads < 0) {  // the copies are invisible to the compiler: stores it sees, never taken
+    lds[threadIdx.x] = 0;
+    entries[threadIdx.x] = 0;
+  }
+  const int block = blockIdx.x;
+  if (block < a.gemm_grid) {
+    gemm_items<DT, 4>(a, lds, block, a.gemm_grid);
+    return;
+  }
+  const int slices = a.num_kv_heads / 4;
+  const int wg = (block - a.gemm_grid) / slices, slice = (block - a.gemm_grid) - wg * slices;
+  if (wg >= a.header[kHeaderStreamWgs]) return;  // graph plans' grids
+  if (a.header[kHeaderOnce])                     // uniform
+    stream_items<DT, 4, SETS, true>(a, lds, entries, wg, slice);
+  else
+    stream_items<DT, 4, SETS, false>(a, lds, entries, wg, slice);
+}
+
+// One and two kv heads a slice: the launches follow each other.
+template <int DT, int W, int SETS>
+__global__ __launch_bounds__(64 * W, 2) void shared_stream_kernel(SharedArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t
+      lds[kStreamStages * 2 * kStreamTile * W * 256];
+  __shared__ int32_t entries[kStreamEntries];
+  if (a.num_kv_heads < 0) {
+    lds[threadIdx.x] = 0;
+    entries[threadIdx.x] = 0;
+  }
+  const int slices = a.num_kv_heads / W;
+  const int wg = blockIdx.x / slices, slice = blockIdx.x - wg * slices;
+  if (wg >= a.header[kHeaderStreamWgs]) return;
+  if (a.header[kHeaderOnce])
+    stream_items<DT, W, SETS, true>(a, lds, entries, wg, slice);
+  else
+    stream_items<DT, W, SETS, false>(a, lds, entries, wg, slice);
+}
+
+template <int DT, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void shared_gemm_kernel(SharedArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[NW / 2 * kStageBytes];
+  if (a.num_kv_heads < 0) lds[threadIdx.x] = 0;
+  gemm_items<DT, NW>(a, lds, blockIdx.x, gridDim.x);
 }
 
 // Running softmax join of partial outputs, four dims a thread.
@@ -595,26 +640,32 @@ struct Join {
   }
 };
 
-// 32 threads a row (a token's q head), eight rows a workgroup. Bound by the rounds of loads,
-// kUnroll partials each.
-template <int DT>
+// 32 threads a row (a token's q head) and run of partials; RUNS threads groups share a row's partials
+// and join through LDS. Bound by the rounds of loads, kUnroll partials each.
+template <int DT, int RUNS>
 __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
   constexpr int kUnroll = 8;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (row >= a.rows) return;
+  constexpr int kRows = 8 / RUNS;  // rows of a workgroup
   const int f = threadIdx.x & 31;
-  const int token = static_cast<int>(row / a.num_q_heads);
-  const int qh = static_cast<int>(row - static_cast<int64_t>(token) * a.num_q_heads);
+  const int sub = threadIdx.x >> 5;
+  const int run = sub % RUNS;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + sub / RUNS;
+  const bool in_range = row < a.rows;
+  if (RUNS == 1 && !in_range) return;
+  const int64_t at_row = in_range ? row : a.rows - 1;
+  const int token = static_cast<int>(at_row / a.num_q_heads);
+  const int qh = static_cast<int>(at_row - static_cast<int64_t>(token) * a.num_q_heads);
   const int req = a.row_of ? a.row_of[token] : token;
   Join j;
   const int4 parts[2] = {a.info[2 * req], a.info[2 * req + 1]};
-  if (parts[0].y + parts[1].y == 0) return;  // written directly
+  const bool joined = parts[0].y + parts[1].y > 0;  // else written directly
+  if (RUNS == 1 && !joined) return;
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
     const int4 src = parts[part];  // {first slot, splits, tokens, token0}
     const int64_t first = static_cast<int64_t>(src.x + token - src.w) * a.num_q_heads + qh;
     const int64_t step = static_cast<int64_t>(src.z) * a.num_q_heads;
-    for (int s0 = 0; s0 < src.y; s0 += kUnroll) {
+    for (int s0 = run * kUnroll; s0 < src.y; s0 += RUNS * kUnroll) {
       float lse[kUnroll];
       float4 v[kUnroll];
 #pragma unroll
@@ -626,10 +677,45 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
       j.add(lse, v);
     }
   }
+  if constexpr (RUNS > 1) {
+    __shared__ float4 acc[8][32];
+    __shared__ float2 stat[8];
+    acc[sub][f] = j.acc;
+    if (f == 0) stat[sub] = make_float2(j.mx, j.den);
+    __syncthreads();
+    if (run > 0 || !in_range || !joined) return;
+    float mx = j.mx;
+#pragma unroll
+    for (int r = 1; r < RUNS; ++r) mx = fmaxf(mx, stat[sub + r].x);
+    j.den = 0.f;
+    j.acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < RUNS; ++r) {
+      const float2 st = stat[sub + r];
+      const float w = st.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.x - mx);
+      const float4 v = acc[sub + r][f];
+      j.den = fmaf(w, st.y, j.den);
+      j.acc = make_float4(fmaf(w, v.x, j.acc.x), fmaf(w, v.y, j.acc.y), fmaf(w, v.z, j.acc.z),
+                          fmaf(w, v.w, j.acc.w));
+    }
+  }
   const float inv = 1.f / j.den;
   *reinterpret_cast<uint2*>(a.out + token * a.o_sn + qh * a.o_sh + f * 4) =
       make_uint2(Elem<DT>::pack2(j.acc.x * inv, j.acc.y * inv),
                  Elem<DT>::pack2(j.acc.z * inv, j.acc.w * inv));
+}
+
+// Up to this many rows a workgroup's threads all work on one: few rows have many parts, and leave
+// most of the chip idle.
+constexpr int64_t kMergeTogether = 512;
+
+template <int DT>
+void launch_merge(const SharedArgs& a, hipStream_t s) {
+  if (a.rows <= kMergeTogether)
+    shared_merge_kernel<DT, 8><<<dim3(static_cast<uint32_t>(a.rows)), dim3(256), 0, s>>>(a);
+  else
+    shared_merge_kernel<DT, 1><<<dim3(static_cast<uint32_t>((a.rows + 7) / 8)), dim3(256), 0, s>>>(
+        a);
 }
 
 // ---------------------------------------------------------------------------
@@ -643,7 +729,7 @@ struct StreamShape {
 };
 StreamShape stream_shape(int64_t cus, int64_t num_kv_heads, int64_t page_size) {
   StreamShape s{};
-  for (s.waves = 8; num_kv_heads % s.waves; s.waves /= 2) {
+  for (s.waves = 4; num_kv_heads % s.waves; s.waves /= 2) {
   }
   s.grid_y = num_kv_heads / s.waves;
   const int64_t lds = kStreamStages * 2 * kStreamTile * s.waves * 256 + kStreamEntries * 4;
@@ -661,18 +747,17 @@ struct Source {
   int32_t slot = 0, splits = 0;
 };
 
-int64_t gemm_slots(int64_t cus, int nw) { return nw == 8 ? cus : 2 * cus; }
 
 struct GemmCount {
   int64_t items = 0, slots = 0;
 };
 GemmCount count_gemm(const std::vector<Source>& sources, int64_t group, int64_t num_kv_heads,
-                     int nw, int64_t length) {
+                     int64_t columns, int64_t length) {
   GemmCount n;
   for (const Source& s : sources) {
     const int64_t tiles = ceil_div(s.end, kTileK) - s.begin / kTileK;
     const int64_t splits = std::max<int64_t>(1, ceil_div(tiles, length));
-    n.items += ceil_div(s.tokens * group, 32 * nw) * num_kv_heads * splits;
+    n.items += ceil_div(s.tokens * group, columns) * num_kv_heads * splits;
     n.slots += s.tokens * splits;
   }
   return n;
@@ -682,7 +767,7 @@ GemmCount count_gemm(const std::vector<Source>& sources, int64_t group, int64_t 
 // long as its longest part and what an item costs besides its tiles (its queries, its first tile and
 // its partial: about two tiles), and the parts that the merge has to read.
 int64_t gemm_length(const std::vector<Source>& sources, int64_t group, int64_t num_kv_heads,
-                    int64_t cus, int nw, const GemmCount& cap) {
+                    int64_t columns, int64_t slots, const GemmCount& cap) {
   constexpr double kItemTiles = 2.0, kMergeTiles = 0.25;
   int64_t longest = 1;
   for (const Source& s : sources)
@@ -691,10 +776,10 @@ int64_t gemm_length(const std::vector<Source>& sources, int64_t group, int64_t n
   double best = 0;
   for (int64_t parts = 1; parts <= std::min<int64_t>(longest, 256); ++parts) {
     const int64_t l = ceil_div(longest, parts);
-    const GemmCount n = count_gemm(sources, group, num_kv_heads, nw, l);
+    const GemmCount n = count_gemm(sources, group, num_kv_heads, columns, l);
     if (n.items > cap.items || n.slots > cap.slots) break;
     const double est =
-        static_cast<double>(ceil_div(n.items, gemm_slots(cus, nw))) * (l + kItemTiles) +
+        static_cast<double>(ceil_div(n.items, slots)) * (l + kItemTiles) +
         kMergeTiles * parts;
     if (parts == 1 || est < best) {
       best = est;
@@ -705,8 +790,8 @@ int64_t gemm_length(const std::vector<Source>& sources, int64_t group, int64_t n
 }
 
 // Appends the sources' work items, longest first; `slot`: the next free one.
-void schedule_gemm(std::vector<Source>& sources, int64_t group, int64_t num_kv_heads, int nw,
-                   int64_t length, int64_t& slot, std::vector<int32_t>& work) {
+void schedule_gemm(std::vector<Source>& sources, int64_t group, int64_t num_kv_heads,
+                   int64_t columns, int64_t length, int64_t& slot, std::vector<int32_t>& work) {
   struct Item {
     int64_t tiles;
     int32_t source, row0, head, split, begin, end;
@@ -720,11 +805,11 @@ void schedule_gemm(std::vector<Source>& sources, int64_t group, int64_t num_kv_h
     s.slot = static_cast<int32_t>(slot);
     slot += static_cast<int64_t>(s.splits) * s.tokens;
     for (int32_t p = 0; p < s.splits; ++p)
-      for (int64_t row0 = 0; row0 < rows; row0 += 32 * nw) {
+      for (int64_t row0 = 0; row0 < rows; row0 += columns) {
         const int64_t begin = first + tiles * p / s.splits;
         int64_t end = first + tiles * (p + 1) / s.splits;
         if (s.pos0 < kNoHorizon) {  // no tile past what the item's last row sees
-          const int64_t last = s.pos0 + (std::min<int64_t>(row0 + 32 * nw, rows) - 1) / group;
+          const int64_t last = s.pos0 + (std::min<int64_t>(row0 + columns, rows) - 1) / group;
           end = std::max<int64_t>(begin, std::min<int64_t>(end, last / kTileK + 1));
         }
         for (int32_t h = 0; h < num_kv_heads; ++h)
@@ -743,18 +828,6 @@ void schedule_gemm(std::vector<Source>& sources, int64_t group, int64_t num_kv_h
                              s.page_base, it.begin, it.end, s.slot + it.split * s.tokens, s.pos0,
                              s.end, 0, 0});
   }
-}
-
-// 256 columns a workgroup where they are mostly filled: K and V are read half as often. Fewer leave
-// waves of it idle, which two workgroups of 128 a CU do not.
-int gemm_waves(const std::vector<Source>& sources, int64_t group) {
-  int64_t cost8 = 0, cost4 = 0;
-  for (const Source& s : sources) {
-    const int64_t rows = s.tokens * group, tiles = ceil_div(s.end, kTileK) - s.begin / kTileK;
-    cost8 += 2 * ceil_div(rows, 256) * tiles;
-    cost4 += ceil_div(rows, 128) * tiles;
-  }
-  return cost8 <= cost4 ? 8 : 4;
 }
 
 }  // namespace
@@ -779,7 +852,8 @@ struct SharedPlan::State {
   int64_t batch = 0, tokens = 0;
   bool by_token = false;  // requests of one token each
   int64_t stream_grid = 0, gemm_grid = 0, gemm_items = 0;
-  int nw = 8, sets = 1;
+  int sets = 1, nw = 4;
+  bool fused = false;  // products and copies in one launch
   int64_t groups_shared = 0, tokens_shared = 0, prefix_items = 0;
   int64_t o_info = 0, o_row_of = 0, o_stream = 0, o_wg = 0, o_gemm = 0;
   Buffer ints, staging, part_o, part_lse;
@@ -834,7 +908,7 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
   std::vector<Of> prefix_of, own_of;
   std::vector<int32_t> lens, work, merge, wg, gemm_work;
   GemmCount cap;
-  int64_t items = 0, wgs = 0, slot = 0, items_cap = 0;
+  int64_t items = 0, wgs = 0, slot = 0, items_cap = 0, gemm_slots = 0;
   bool once = true;
   for (int attempt = 0; attempt < 2; ++attempt) {
     stream.clear();
@@ -881,15 +955,15 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
     lens.clear();
     items_cap = st.shape.wg_capacity;
     int64_t bytes = 0;
-    int columns = 1;
+    int widest = 1;
     for (const Source& src : stream) {
       lens.push_back(src.end - src.begin);
       items_cap += 1 + ceil_div(lens.back(), st.shape.max_item);
       bytes += int64_t(lens.back()) * heads * kD * 4;
-      columns = std::max<int>(columns, src.tokens * static_cast<int>(group));
+      widest = std::max<int>(widest, src.tokens * static_cast<int>(group));
     }
     once = bytes >= int64_t(8) << 20;  // as the decode kernel's copies
-    st.sets = columns <= 16 ? 1 : columns <= 32 ? 2 : 3;
+    st.sets = widest <= 16 ? 1 : 2;
     work.resize(4 * items_cap);
     merge.resize(2 * stream.size());
     wg.resize(st.shape.wg_capacity + 1);
@@ -917,23 +991,36 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
     }
     // The matrix products.
     gemm_work.clear();
-    cap = {};
+    // The products run beside the copies (see shared_kernel), one workgroup of 128 columns a CU, where
+    // the copies take long enough to hide a good part of them; before them otherwise, with 256
+    // columns a CU where a workgroup of eight waves is mostly filled.
+    int64_t cost4 = 0, cost8 = 0;  // tiles of a CU's half and of a CU
+    for (const Source& src : gemm) {
+      const int64_t tiles = ceil_div(src.end, kTileK) - src.begin / kTileK;
+      cost4 += ceil_div(src.tokens * group, 128) * tiles * heads;
+      cost8 += ceil_div(src.tokens * group, 256) * tiles * heads;
+    }
+    constexpr double kTileUs = 2.2, kBytesPerUs = 5.5e6;
+    const double gemm_us = kTileUs * static_cast<double>(cost4) / static_cast<double>(2 * st.cus);
+    const double stream_us = static_cast<double>(bytes) / kBytesPerUs;
+    st.fused = st.shape.waves == 4 && (graph_rows || stream_us > 0.3 * gemm_us);
+    st.nw = !st.fused && !graph_rows && 2 * cost8 <= cost4 ? 8 : 4;
+    const int64_t columns = 32 * st.nw;
+    gemm_slots = st.fused || st.nw == 8 ? st.cus : 2 * st.cus;
     if (graph_rows) {
-      st.nw = graph_rows * group > 128 ? 8 : 4;
-      const int64_t per = 32 * st.nw / group;  // tokens of an item
+      const int64_t per = columns / group;  // tokens of an item
       // at most rows / 2 groups share, each with a last tile that is not full
-      cap.items = (graph_rows / per + graph_rows / 2) * heads + gemm_slots(st.cus, st.nw);
-      cap.slots = graph_rows + gemm_slots(st.cus, st.nw) * per / heads;
-    } else if (!gemm.empty()) {
-      st.nw = gemm_waves(gemm, group);
-      cap = count_gemm(gemm, group, heads, st.nw, std::numeric_limits<int32_t>::max());
-      cap.items += gemm_slots(st.cus, st.nw);
-      cap.slots += gemm_slots(st.cus, st.nw) * 32 * st.nw / group;
+      cap.items = (graph_rows / per + graph_rows / 2) * heads + gemm_slots;
+      cap.slots = graph_rows + gemm_slots * per / heads;
+    } else {
+      cap = count_gemm(gemm, group, heads, columns, std::numeric_limits<int32_t>::max());
+      cap.items += gemm_slots;
+      cap.slots += gemm_slots * columns / group;
     }
     const int64_t stream_slots = slot;
     if (!gemm.empty())
-      schedule_gemm(gemm, group, heads, st.nw,
-                    gemm_length(gemm, group, heads, st.cus, st.nw, cap), slot, gemm_work);
+      schedule_gemm(gemm, group, heads, columns,
+                    gemm_length(gemm, group, heads, columns, gemm_slots, cap), slot, gemm_work);
     if (!graph_rows) break;
     // A graph plan has room for 64 MiB of partial outputs of the streaming launch, beside a slot an
     // item: a batch that needs more (dozens of small groups) shares nothing.
@@ -1024,9 +1111,9 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
   st.batch = b.batch;
   st.tokens = tokens;
   st.by_token = by_token;
-  if (graph_rows) st.sets = 3;
+  if (graph_rows) st.sets = 2;
   st.stream_grid = graph_rows ? wg_cap : wgs;
-  st.gemm_grid = graph_rows ? gemm_slots(st.cus, st.nw) : st.gemm_items;
+  st.gemm_grid = graph_rows ? gemm_slots : std::min(gemm_slots, st.gemm_items);
   st.o_info = o_info;
   st.o_row_of = o_row_of;
   st.o_stream = o_stream;
@@ -1044,28 +1131,35 @@ void SharedPlan::info(int64_t* out4) const {
 
 namespace {
 template <int DT, int W>
-void launch_stream(const SharedArgs& a, int sets, dim3 grid, hipStream_t s) {
-  if (sets == 1) shared_stream_kernel<DT, W, 1><<<grid, dim3(64 * W), 0, s>>>(a);
-  else if (sets == 2) shared_stream_kernel<DT, W, 2><<<grid, dim3(64 * W), 0, s>>>(a);
-  else shared_stream_kernel<DT, W, 3><<<grid, dim3(64 * W), 0, s>>>(a);
+void launch_stream(const SharedArgs& a, int sets, uint32_t grid, hipStream_t s) {
+  if (sets == 1) shared_stream_kernel<DT, W, 1><<<dim3(grid), dim3(64 * W), 0, s>>>(a);
+  else shared_stream_kernel<DT, W, 2><<<dim3(grid), dim3(64 * W), 0, s>>>(a);
 }
 template <int DT>
-const char* launch_all(const SharedArgs& a, int64_t waves, int sets, dim3 stream_grid,
-                       int64_t gemm_grid, int nw, hipStream_t s) {
-  if (gemm_grid) {
-    const dim3 blocks(static_cast<uint32_t>(gemm_grid));
-    if (nw == 8) shared_gemm_kernel<DT, 8><<<blocks, dim3(512), 0, s>>>(a);
-    else shared_gemm_kernel<DT, 4><<<blocks, dim3(256), 0, s>>>(a);
-    if (const char* err = launch_status("shared_gemm_kernel")) return err;
+const char* launch_all(SharedArgs a, int64_t waves, int sets, int nw, bool fused,
+                       int64_t stream_grid, hipStream_t s) {
+  const uint32_t streams = static_cast<uint32_t>(stream_grid);
+  if (!fused) {
+    const dim3 grid(static_cast<uint32_t>(a.gemm_grid));
+    if (a.gemm_grid) {
+      if (nw == 8) shared_gemm_kernel<DT, 8><<<grid, dim3(512), 0, s>>>(a);
+      else shared_gemm_kernel<DT, 4><<<grid, dim3(256), 0, s>>>(a);
+      if (const char* err = launch_status("shared_gemm_kernel")) return err;
+    }
+    a.gemm_grid = 0;
   }
-  if (stream_grid.x) {
-    if (waves == 8) launch_stream<DT, 8>(a, sets, stream_grid, s);
-    else if (waves == 4) launch_stream<DT, 4>(a, sets, stream_grid, s);
-    else if (waves == 2) launch_stream<DT, 2>(a, sets, stream_grid, s);
-    else launch_stream<DT, 1>(a, sets, stream_grid, s);
+  const uint32_t products = static_cast<uint32_t>(a.gemm_grid);
+  if (waves == 4 && products + streams) {
+    const dim3 grid(products + streams), block(256);
+    if (sets == 1) shared_kernel<DT, 1><<<grid, block, 0, s>>>(a);
+    else shared_kernel<DT, 2><<<grid, block, 0, s>>>(a);
+    if (const char* err = launch_status("shared_kernel")) return err;
+  } else if (streams) {
+    if (waves == 2) launch_stream<DT, 2>(a, sets, streams, s);
+    else launch_stream<DT, 1>(a, sets, streams, s);
     if (const char* err = launch_status("shared_stream_kernel")) return err;
   }
-  shared_merge_kernel<DT><<<dim3(static_cast<uint32_t>((a.rows + 7) / 8)), dim3(256), 0, s>>>(a);
+  launch_merge<DT>(a, s);
   return launch_status("shared_merge_kernel");
 }
 }  // namespace
@@ -1099,11 +1193,11 @@ const char* SharedPlan::run(const int32_t* indices, const void* q, int64_t q_sn,
   a.group_log2 = st.group_log2;
   a.page_size = static_cast<int32_t>(st.page_size);
   a.scale_log2 = (1.0f / std::sqrt(static_cast<float>(kD))) * kLog2e;
-  const dim3 stream_grid(static_cast<uint32_t>(st.stream_grid),
-                         static_cast<uint32_t>(st.shape.grid_y));
+  a.gemm_grid = static_cast<int32_t>(st.gemm_grid);
+  const int64_t stream_grid = st.stream_grid * st.shape.grid_y;
   return st.dtype == 0
-             ? launch_all<0>(a, st.shape.waves, st.sets, stream_grid, st.gemm_grid, st.nw, s)
-             : launch_all<1>(a, st.shape.waves, st.sets, stream_grid, st.gemm_grid, st.nw, s);
+             ? launch_all<0>(a, st.shape.waves, st.sets, st.nw, st.fused, stream_grid, s)
+             : launch_all<1>(a, st.shape.waves, st.sets, st.nw, st.fused, stream_grid, s);
 }
 
 }  // namespace mi355x
