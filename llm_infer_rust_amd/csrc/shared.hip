@@ -40,7 +40,7 @@ constexpr int64_t kMaxKeys = int64_t(1) << 22;
 
 // --- device workspace, int32
 constexpr int kHeaderInts = 4;
-constexpr int kHeaderGemmItems = 0, kHeaderStreamWgs = 1, kHeaderOnce = 2;
+constexpr int kHeaderGemmItems = 0, kHeaderStreamWgs = 1, kHeaderOnce = 2, kHeaderGemmWgs = 3;
 constexpr int kInfoInts = 8;    // a request: {first slot, splits, tokens, token0} of the prefix's
                                 // parts, then of its own (splits 0: none)
 constexpr int kStreamInts = 8;  // {token0, tokens, first page entry, key begin | key end, slot or -1
@@ -590,6 +590,33 @@ __global__ __launch_bounds__(256, 2) void shared_kernel(SharedArgs a) {
     stream_items<DT, 4, SETS, false>(a, lds, entries, wg, slice);
 }
 
+// The same with whole CUs for either kind: products of 256 columns on some, copies of eight kv heads
+// on the others and, when the products are done, on all.
+template <int DT, int SETS>
+__global__ __launch_bounds__(512, 2) void shared_wide_kernel(SharedArgs a) {
+  constexpr int kRing = kStreamStages * 2 * kStreamTile * 8 * 256;
+  static_assert(kRing == 4 * kStageBytes, "either ring");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kRing];
+  __shared__ int32_t entries[kStreamEntries];
+  if (a.num_kv_heads < 0) {
+    lds[threadIdx.x] = 0;
+    entries[threadIdx.x] = 0;
+  }
+  const int block = blockIdx.x;
+  if (block < a.gemm_grid) {
+    const int wgs = a.header[kHeaderGemmWgs];
+    if (block < wgs) gemm_items<DT, 8>(a, lds, block, wgs);
+    return;
+  }
+  const int slices = a.num_kv_heads / 8;
+  const int wg = (block - a.gemm_grid) / slices, slice = (block - a.gemm_grid) - wg * slices;
+  if (wg >= a.header[kHeaderStreamWgs]) return;
+  if (a.header[kHeaderOnce])
+    stream_items<DT, 8, SETS, true>(a, lds, entries, wg, slice);
+  else
+    stream_items<DT, 8, SETS, false>(a, lds, entries, wg, slice);
+}
+
 // One and two kv heads a slice: the launches follow each other.
 template <int DT, int W, int SETS>
 __global__ __launch_bounds__(64 * W, 2) void shared_stream_kernel(SharedArgs a) {
@@ -727,9 +754,15 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct StreamShape {
   int64_t waves, grid_y, workgroups, wg_capacity, max_item;
 };
-StreamShape stream_shape(int64_t cus, int64_t num_kv_heads, int64_t page_size) {
+enum class Form {
+  kInTurn,  // products, then copies
+  kHalves,  // shared_kernel: half a CU for a workgroup of either kind (four kv heads a slice)
+  kWhole,   // shared_wide_kernel: a CU for a workgroup of either kind (eight)
+};
+
+StreamShape stream_shape(int64_t cus, int64_t num_kv_heads, int64_t page_size, int64_t widest) {
   StreamShape s{};
-  for (s.waves = 4; num_kv_heads % s.waves; s.waves /= 2) {
+  for (s.waves = widest; num_kv_heads % s.waves; s.waves /= 2) {
   }
   s.grid_y = num_kv_heads / s.waves;
   const int64_t lds = kStreamStages * 2 * kStreamTile * s.waves * 256 + kStreamEntries * 4;
@@ -766,27 +799,30 @@ GemmCount count_gemm(const std::vector<Source>& sources, int64_t group, int64_t 
 // Tiles of a part's keys, such that the launch ends soonest: rounds of items over the chip, each as
 // long as its longest part and what an item costs besides its tiles (its queries, its first tile and
 // its partial: about two tiles), and the parts that the merge has to read.
-int64_t gemm_length(const std::vector<Source>& sources, int64_t group, int64_t num_kv_heads,
-                    int64_t columns, int64_t slots, const GemmCount& cap) {
+struct GemmLength {
+  int64_t tiles;
+  double tile_times;  // until the last item has ended, in tiles
+};
+GemmLength gemm_length(const std::vector<Source>& sources, int64_t group, int64_t num_kv_heads,
+                       int64_t columns, int64_t slots, const GemmCount& cap) {
   constexpr double kItemTiles = 2.0, kMergeTiles = 0.25;
   int64_t longest = 1;
   for (const Source& s : sources)
     longest = std::max(longest, ceil_div(s.end, kTileK) - s.begin / kTileK);
-  int64_t length = longest;
-  double best = 0;
+  GemmLength best{longest, 0};
+  double least = 0;
   for (int64_t parts = 1; parts <= std::min<int64_t>(longest, 256); ++parts) {
     const int64_t l = ceil_div(longest, parts);
     const GemmCount n = count_gemm(sources, group, num_kv_heads, columns, l);
     if (n.items > cap.items || n.slots > cap.slots) break;
-    const double est =
-        static_cast<double>(ceil_div(n.items, slots)) * (l + kItemTiles) +
-        kMergeTiles * parts;
-    if (parts == 1 || est < best) {
-      best = est;
-      length = l;
+    const double run = static_cast<double>(ceil_div(n.items, slots)) * (l + kItemTiles);
+    const double est = run + kMergeTiles * parts;
+    if (parts == 1 || est < least) {
+      least = est;
+      best = {l, run};
     }
   }
-  return length;
+  return best;
 }
 
 // Appends the sources' work items, longest first; `slot`: the next free one.
@@ -851,9 +887,10 @@ struct SharedPlan::State {
   // Current plan.
   int64_t batch = 0, tokens = 0;
   bool by_token = false;  // requests of one token each
-  int64_t stream_grid = 0, gemm_grid = 0, gemm_items = 0;
+  int64_t stream_grid = 0, gemm_grid = 0, gemm_items = 0, gemm_wgs = 0;
   int sets = 1, nw = 4;
-  bool fused = false;  // products and copies in one launch
+  Form form = Form::kInTurn;
+  int64_t slices = 1;  // kv-head slices of the streaming launch
   int64_t groups_shared = 0, tokens_shared = 0, prefix_items = 0;
   int64_t o_info = 0, o_row_of = 0, o_stream = 0, o_wg = 0, o_gemm = 0;
   Buffer ints, staging, part_o, part_lse;
@@ -886,7 +923,7 @@ SharedPlan::SharedPlan(int64_t cus, int64_t num_q_heads, int64_t num_kv_heads, i
     : st_(new State{cus, num_q_heads, num_kv_heads, page_size, dtype,
                     num_q_heads / num_kv_heads}) {
   while ((1 << st_->group_log2) < st_->group) ++st_->group_log2;
-  st_->shape = stream_shape(cus, num_kv_heads, page_size);
+  st_->shape = stream_shape(cus, num_kv_heads, page_size, 4);
   st_->staging.pinned = true;
 }
 SharedPlan::~SharedPlan() = default;
@@ -908,8 +945,9 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
   std::vector<Of> prefix_of, own_of;
   std::vector<int32_t> lens, work, merge, wg, gemm_work;
   GemmCount cap;
-  int64_t items = 0, wgs = 0, slot = 0, items_cap = 0, gemm_slots = 0;
+  int64_t items = 0, wgs = 0, slot = 0, items_cap = 0;
   bool once = true;
+  StreamShape graph_shape{};
   for (int attempt = 0; attempt < 2; ++attempt) {
     stream.clear();
     gemm.clear();
@@ -951,28 +989,95 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
         gemm.push_back(own);
       }
     }
+    // How the products and the copies share the chip, by what either takes alone.
+    int64_t cost4 = 0, cost8 = 0;  // tiles of half a CU and of a CU
+    for (const Source& src : gemm) {
+      const int64_t tiles = ceil_div(src.end, kTileK) - src.begin / kTileK;
+      cost4 += ceil_div(src.tokens * group, 128) * tiles * heads;
+      cost8 += ceil_div(src.tokens * group, 256) * tiles * heads;
+    }
+    int64_t bytes = 0;
+    for (const Source& src : stream) bytes += int64_t(src.end - src.begin) * heads * kD * 4;
+    // A CU's tile of 256 columns, where all CUs multiply and where others stream; the copies' rate.
+    constexpr double kTileUs = 2.4, kMixedTileUs = 1.68, kBytesPerUs = 5.86e6;
+    const double gemm_us = kTileUs * static_cast<double>(cost8) / static_cast<double>(st.cus);
+    const double stream_us = static_cast<double>(bytes) / kBytesPerUs;
+    StreamShape shape = st.shape;
+    int64_t gemm_wgs = 0;
+    // Bounds on the products' items and partial outputs, beside one part a source: a graph plan's
+    // hold for whatever its rows will share.
+    auto capacity = [&](int64_t columns) {
+      const int64_t extra = 2 * st.cus, per = columns / group;  // tokens of an item
+      if (graph_rows) {
+        // at most rows / 2 groups share, each with a last tile that is not full
+        cap.items = (graph_rows / per + graph_rows / 2) * heads + extra;
+        cap.slots = graph_rows + extra * per / heads;
+      } else {
+        cap = count_gemm(gemm, group, heads, columns, std::numeric_limits<int32_t>::max());
+        cap.items += extra;
+        cap.slots += extra * per;
+      }
+    };
+    // Whole CUs: as many for the products as end the launch soonest. A CU streams no faster for
+    // others' idling, so that the copies take longer by the share that the products have.
+    double whole_us = std::numeric_limits<double>::infinity();
+    if (heads % 8 == 0 && (!gemm.empty() || graph_rows)) {
+      capacity(256);
+      for (int64_t wgs8 = st.cus / 16; wgs8 <= st.cus - st.cus / 8 && !gemm.empty(); wgs8 += 4) {
+        const double run =
+            kMixedTileUs * gemm_length(gemm, group, heads, 256, wgs8, cap).tile_times;
+        const double est =
+            std::max(run, stream_us * static_cast<double>(st.cus) / (st.cus - wgs8)) + 5;
+        if (est < whole_us) {
+          whole_us = est;
+          gemm_wgs = wgs8;
+        }
+      }
+    }
+    // Half CUs: a fit to measured mixes (products alone, copies alone -> kernel, us: 38 and 92 -> 145,
+    // 38 and 34 -> 72, 19 and 17 -> 39, 10 and 46 -> 68, 10 and 7 -> 23; on whole CUs 119, 79, 46, 60
+    // and 29).
+    const double halves_us = 0.6 * gemm_us + 1.26 * stream_us + 6;
+    st.form = Form::kInTurn;
+    if (heads % 8 == 0 && (graph_rows ? graph_rows * group > 128 : whole_us < halves_us))
+      st.form = Form::kWhole;
+    else if (st.shape.waves == 4 && (graph_rows || stream_us > 0.3 * gemm_us))
+      st.form = Form::kHalves;
+    st.nw = st.form == Form::kWhole || (st.form == Form::kInTurn && 2 * cost8 <= cost4) ? 8 : 4;
+    const int64_t columns = 32 * st.nw;
+    if (st.form != Form::kWhole)
+      gemm_wgs = st.form == Form::kHalves || st.nw == 8 ? st.cus : 2 * st.cus;
+    capacity(columns);
+    if (st.form == Form::kWhole) {
+      // A share for every CU that streams: more of them end later where the last ones find no CU free
+      // (64 rows sharing 8,192 tokens, 192 such CUs: 192 shares 41.8 us, 256 49.7, 384 43, 512 49).
+      shape = stream_shape(st.cus, heads, st.page_size, 8);
+      shape.workgroups = (st.cus - gemm_wgs) / shape.grid_y;
+      if (!graph_rows)
+        shape.wg_capacity = shape.workgroups + shape.workgroups / 3 + 2;
+      else
+        shape.wg_capacity = st.cus / shape.grid_y + st.cus / 3 + 2;
+    }
     // The streaming launch.
     lens.clear();
-    items_cap = st.shape.wg_capacity;
-    int64_t bytes = 0;
+    items_cap = shape.wg_capacity;
     int widest = 1;
     for (const Source& src : stream) {
       lens.push_back(src.end - src.begin);
-      items_cap += 1 + ceil_div(lens.back(), st.shape.max_item);
-      bytes += int64_t(lens.back()) * heads * kD * 4;
+      items_cap += 1 + ceil_div(lens.back(), shape.max_item);
       widest = std::max<int>(widest, src.tokens * static_cast<int>(group));
     }
     once = bytes >= int64_t(8) << 20;  // as the decode kernel's copies
     st.sets = widest <= 16 ? 1 : 2;
     work.resize(4 * items_cap);
     merge.resize(2 * stream.size());
-    wg.resize(st.shape.wg_capacity + 1);
+    wg.resize(shape.wg_capacity + 1);
     int64_t share = 0;
     items = wgs = slot = 0;
     if (!stream.empty()) {
-      items = schedule(lens.data(), static_cast<int64_t>(stream.size()), st.shape.workgroups,
-                       st.shape.max_item, kStreamTile, /*graph=*/true, work.data(), items_cap,
-                       merge.data(), &share, wg.data(), st.shape.wg_capacity, &wgs);
+      items = schedule(lens.data(), static_cast<int64_t>(stream.size()), shape.workgroups,
+                       shape.max_item, kStreamTile, /*graph=*/true, work.data(), items_cap,
+                       merge.data(), &share, wg.data(), shape.wg_capacity, &wgs);
       if (items < 0) {
         set_error("shared prefix work list exceeds its capacity");
         return false;
@@ -991,36 +1096,14 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
     }
     // The matrix products.
     gemm_work.clear();
-    // The products run beside the copies (see shared_kernel), one workgroup of 128 columns a CU, where
-    // the copies take long enough to hide a good part of them; before them otherwise, with 256
-    // columns a CU where a workgroup of eight waves is mostly filled.
-    int64_t cost4 = 0, cost8 = 0;  // tiles of a CU's half and of a CU
-    for (const Source& src : gemm) {
-      const int64_t tiles = ceil_div(src.end, kTileK) - src.begin / kTileK;
-      cost4 += ceil_div(src.tokens * group, 128) * tiles * heads;
-      cost8 += ceil_div(src.tokens * group, 256) * tiles * heads;
-    }
-    constexpr double kTileUs = 2.2, kBytesPerUs = 5.5e6;
-    const double gemm_us = kTileUs * static_cast<double>(cost4) / static_cast<double>(2 * st.cus);
-    const double stream_us = static_cast<double>(bytes) / kBytesPerUs;
-    st.fused = st.shape.waves == 4 && (graph_rows || stream_us > 0.3 * gemm_us);
-    st.nw = !st.fused && !graph_rows && 2 * cost8 <= cost4 ? 8 : 4;
-    const int64_t columns = 32 * st.nw;
-    gemm_slots = st.fused || st.nw == 8 ? st.cus : 2 * st.cus;
-    if (graph_rows) {
-      const int64_t per = columns / group;  // tokens of an item
-      // at most rows / 2 groups share, each with a last tile that is not full
-      cap.items = (graph_rows / per + graph_rows / 2) * heads + gemm_slots;
-      cap.slots = graph_rows + gemm_slots * per / heads;
-    } else {
-      cap = count_gemm(gemm, group, heads, columns, std::numeric_limits<int32_t>::max());
-      cap.items += gemm_slots;
-      cap.slots += gemm_slots * columns / group;
-    }
     const int64_t stream_slots = slot;
     if (!gemm.empty())
       schedule_gemm(gemm, group, heads, columns,
-                    gemm_length(gemm, group, heads, columns, gemm_slots, cap), slot, gemm_work);
+                    gemm_length(gemm, group, heads, columns, gemm_wgs, cap).tiles, slot,
+                    gemm_work);
+    st.slices = shape.grid_y;
+    graph_shape = shape;
+    st.gemm_wgs = std::min(gemm_wgs, static_cast<int64_t>(gemm_work.size()) / kGemmInts);
     if (!graph_rows) break;
     // A graph plan has room for 64 MiB of partial outputs of the streaming launch, beside a slot an
     // item: a batch that needs more (dozens of small groups) shares nothing.
@@ -1035,10 +1118,11 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
   int64_t stream_cap = items, wg_cap = wgs, gemm_cap = st.gemm_items, slot_cap = slot;
   if (graph_rows) {
     // a workgroup's share, and each request's and prefix's own items and cuts
-    const int64_t most = st.shape.wg_capacity + (graph_rows + graph_rows / 2) *
-                                                    (1 + ceil_div(graph_tokens, st.shape.max_item));
+    const int64_t most = graph_shape.wg_capacity +
+                         (graph_rows + graph_rows / 2) *
+                             (1 + ceil_div(graph_tokens, graph_shape.max_item));
     stream_cap = most;
-    wg_cap = st.shape.wg_capacity;
+    wg_cap = graph_shape.wg_capacity;
     gemm_cap = cap.items;
     slot_cap = (int64_t(64) << 20) / (st.num_q_heads * kD * 4) + most + cap.slots;
   }
@@ -1070,7 +1154,7 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
   host[kHeaderGemmItems] = static_cast<int32_t>(st.gemm_items);
   host[kHeaderStreamWgs] = static_cast<int32_t>(wgs);
   host[kHeaderOnce] = once;
-  host[3] = 0;
+  host[kHeaderGemmWgs] = static_cast<int32_t>(st.gemm_wgs);
   for (int64_t r = 0; r < b.batch; ++r) {
     int32_t* info = host + o_info + kInfoInts * r;
     for (const Of& of : {prefix_of[r], own_of[r]}) {
@@ -1113,7 +1197,7 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
   st.by_token = by_token;
   if (graph_rows) st.sets = 2;
   st.stream_grid = graph_rows ? wg_cap : wgs;
-  st.gemm_grid = graph_rows ? gemm_slots : std::min(gemm_slots, st.gemm_items);
+  st.gemm_grid = graph_rows ? st.cus : st.gemm_wgs;
   st.o_info = o_info;
   st.o_row_of = o_row_of;
   st.o_stream = o_stream;
@@ -1136,28 +1220,34 @@ void launch_stream(const SharedArgs& a, int sets, uint32_t grid, hipStream_t s) 
   else shared_stream_kernel<DT, W, 2><<<dim3(grid), dim3(64 * W), 0, s>>>(a);
 }
 template <int DT>
-const char* launch_all(SharedArgs a, int64_t waves, int sets, int nw, bool fused,
+const char* launch_all(SharedArgs a, Form form, int64_t waves, int sets, int nw,
                        int64_t stream_grid, hipStream_t s) {
   const uint32_t streams = static_cast<uint32_t>(stream_grid);
-  if (!fused) {
-    const dim3 grid(static_cast<uint32_t>(a.gemm_grid));
-    if (a.gemm_grid) {
-      if (nw == 8) shared_gemm_kernel<DT, 8><<<grid, dim3(512), 0, s>>>(a);
-      else shared_gemm_kernel<DT, 4><<<grid, dim3(256), 0, s>>>(a);
+  const uint32_t products = static_cast<uint32_t>(a.gemm_grid);
+  if (form == Form::kInTurn) {
+    if (products) {
+      if (nw == 8) shared_gemm_kernel<DT, 8><<<dim3(products), dim3(512), 0, s>>>(a);
+      else shared_gemm_kernel<DT, 4><<<dim3(products), dim3(256), 0, s>>>(a);
       if (const char* err = launch_status("shared_gemm_kernel")) return err;
     }
     a.gemm_grid = 0;
-  }
-  const uint32_t products = static_cast<uint32_t>(a.gemm_grid);
-  if (waves == 4 && products + streams) {
-    const dim3 grid(products + streams), block(256);
-    if (sets == 1) shared_kernel<DT, 1><<<grid, block, 0, s>>>(a);
-    else shared_kernel<DT, 2><<<grid, block, 0, s>>>(a);
+    if (streams) {
+      if (waves == 2) launch_stream<DT, 2>(a, sets, streams, s);
+      else if (waves == 1) launch_stream<DT, 1>(a, sets, streams, s);
+      else if (sets == 1) shared_kernel<DT, 1><<<dim3(streams), dim3(256), 0, s>>>(a);
+      else shared_kernel<DT, 2><<<dim3(streams), dim3(256), 0, s>>>(a);
+      if (const char* err = launch_status("shared_stream_kernel")) return err;
+    }
+  } else {
+    const dim3 grid(products + streams);
+    if (form == Form::kWhole) {
+      if (sets == 1) shared_wide_kernel<DT, 1><<<grid, dim3(512), 0, s>>>(a);
+      else shared_wide_kernel<DT, 2><<<grid, dim3(512), 0, s>>>(a);
+    } else {
+      if (sets == 1) shared_kernel<DT, 1><<<grid, dim3(256), 0, s>>>(a);
+      else shared_kernel<DT, 2><<<grid, dim3(256), 0, s>>>(a);
+    }
     if (const char* err = launch_status("shared_kernel")) return err;
-  } else if (streams) {
-    if (waves == 2) launch_stream<DT, 2>(a, sets, streams, s);
-    else launch_stream<DT, 1>(a, sets, streams, s);
-    if (const char* err = launch_status("shared_stream_kernel")) return err;
   }
   launch_merge<DT>(a, s);
   return launch_status("shared_merge_kernel");
@@ -1194,10 +1284,10 @@ const char* SharedPlan::run(const int32_t* indices, const void* q, int64_t q_sn,
   a.page_size = static_cast<int32_t>(st.page_size);
   a.scale_log2 = (1.0f / std::sqrt(static_cast<float>(kD))) * kLog2e;
   a.gemm_grid = static_cast<int32_t>(st.gemm_grid);
-  const int64_t stream_grid = st.stream_grid * st.shape.grid_y;
+  const int64_t stream_grid = st.stream_grid * st.slices;
   return st.dtype == 0
-             ? launch_all<0>(a, st.shape.waves, st.sets, st.nw, st.fused, stream_grid, s)
-             : launch_all<1>(a, st.shape.waves, st.sets, st.nw, st.fused, stream_grid, s);
+             ? launch_all<0>(a, st.form, st.shape.waves, st.sets, st.nw, stream_grid, s)
+             : launch_all<1>(a, st.form, st.shape.waves, st.sets, st.nw, stream_grid, s);
 }
 
 }  // namespace mi355x
