@@ -6,9 +6,10 @@
 // another page of every plane. The destinations are distinct and none of them is a source, so the
 // copies are independent of each other. Bound by memory: every byte is read and written once.
 //
-// The pairs travel as kernel arguments, kBatch a launch: no upload, no staging buffer that a later
-// call would have to wait for, and a captured launch carries its own.
+// The pairs travel as kernel arguments, some hundreds a launch: no upload, no staging buffer that a
+// later call would have to wait for, and a captured launch carries its own.
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 #include "common.h"
@@ -17,33 +18,81 @@ namespace mi355x {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;  // 16-byte words of a thread, loaded together
-constexpr int kBatch = 240; // pairs of a launch: 12 bytes each, under the 4 KiB of arguments
 
-struct CopyBatch {
-  int32_t src[kBatch], dst[kBatch], tokens[kBatch];
+// Whole pages, and pages of which some tokens are copied: under the 4 KiB of arguments.
+struct WholeBatch {
+  static constexpr int kPairs = 480;
+  int32_t src[kPairs], dst[kPairs];
+  __device__ int64_t tokens(int, int64_t page_tokens) const { return page_tokens; }
+};
+struct PartialBatch {
+  static constexpr int kPairs = 320;
+  int32_t src[kPairs], dst[kPairs], valid[kPairs];
+  __device__ int64_t tokens(int pair, int64_t) const { return valid[pair]; }
 };
 
-// Grid: {parts of a page, pairs, planes}; a workgroup copies kThreads * kUnroll words.
-template <typename Word>
+// Grid: {parts of a page, pairs, planes}; a thread copies a word. us, one word a thread against four
+// loaded together: 255 copies of 14 tokens in 56 planes 62 and 94 (5.3 TB/s written and read, most of
+// the sources from the caches), 400 pages of 64 tokens in 8 planes 139 and 158 (6.0 TB/s).
+template <typename Word, typename Batch>
 __global__ __launch_bounds__(kThreads) void copy_pages_kernel(uint8_t* pool, int64_t plane_bytes,
-                                                              int64_t page_bytes,
-                                                              int64_t token_bytes,
-                                                              CopyBatch batch) {
+                                                              int64_t page_tokens,
+                                                              int64_t token_bytes, Batch batch) {
   const int pair = blockIdx.y;
-  const int64_t bytes = batch.tokens[pair] * token_bytes;
-  const int64_t words = bytes / static_cast<int64_t>(sizeof(Word));
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kThreads * kUnroll) + threadIdx.x;
+  const int64_t page_bytes = page_tokens * token_bytes;
+  const int64_t words =
+      batch.tokens(pair, page_tokens) * token_bytes / static_cast<int64_t>(sizeof(Word));
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (at >= words) return;
   uint8_t* plane = pool + blockIdx.z * plane_bytes;
   const Word* src = reinterpret_cast<const Word*>(plane + batch.src[pair] * page_bytes);
   Word* dst = reinterpret_cast<Word*>(plane + batch.dst[pair] * page_bytes);
-  Word w[kUnroll];
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u)
-    if (first + u * kThreads < words) w[u] = src[first + u * kThreads];
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u)
-    if (first + u * kThreads < words) dst[first + u * kThreads] = w[u];
+  dst[at] = src[at];
+}
+
+struct Pool {
+  uint8_t* base;
+  int64_t planes, plane_pages, page_tokens, token_bytes;
+};
+
+// `most`: the longest copy's tokens.
+template <typename Word, typename Batch>
+const char* launch(const Pool& p, const Batch& batch, int pairs, int64_t most, hipStream_t s) {
+  const int64_t words = most * p.token_bytes / static_cast<int64_t>(sizeof(Word));
+  const int64_t parts = (words + kThreads - 1) / kThreads;
+  if (parts > (int64_t(1) << 31) / kThreads)
+    return set_error("mi355x_copy_pages: page too large");
+  const dim3 grid(static_cast<uint32_t>(parts), static_cast<uint32_t>(pairs),
+                  static_cast<uint32_t>(p.planes));
+  copy_pages_kernel<Word><<<grid, dim3(kThreads), 0, s>>>(
+      p.base, p.plane_pages * p.page_tokens * p.token_bytes, p.page_tokens, p.token_bytes, batch);
+  return launch_status("mi355x_copy_pages");
+}
+
+// Launches of about equal size for all pairs.
+template <typename Batch>
+const char* copy_all(const Pool& p, const int32_t* src, const int32_t* dst, const int32_t* tokens,
+                     int64_t pairs, bool wide, hipStream_t s) {
+  const int64_t launches = (pairs + Batch::kPairs - 1) / Batch::kPairs;
+  Batch batch;
+  for (int64_t l = 0; l < launches; ++l) {
+    int n = 0;
+    int64_t most = 0;
+    for (int64_t i = pairs * l / launches; i < pairs * (l + 1) / launches; ++i) {
+      const int32_t t = tokens ? tokens[i] : static_cast<int32_t>(p.page_tokens);
+      if (t == 0) continue;
+      batch.src[n] = src[i];
+      batch.dst[n] = dst[i];
+      if constexpr (std::is_same_v<Batch, PartialBatch>) batch.valid[n] = t;
+      ++n;
+      most = std::max<int64_t>(most, t);
+    }
+    if (n == 0) continue;
+    if (const char* err = wide ? launch<uint4>(p, batch, n, most, s)
+                               : launch<uint16_t>(p, batch, n, most, s))
+      return err;
+  }
+  return nullptr;
 }
 
 // One mark a page of the pool, kept between calls of a thread and cleared after each.
@@ -90,39 +139,11 @@ extern "C" const char* mi355x_copy_pages(void* pool, int64_t planes, int64_t pla
     if (!aligned(pool, 2)) return set_error("mi355x_copy_pages: misaligned pool");
     if (const char* err = check_pairs(plane_pages, page_tokens, src, dst, tokens, pairs))
       return err;
-    const int64_t page_bytes = page_tokens * token_bytes;
     const bool wide = token_bytes % 16 == 0 && aligned(pool, 16);
-    const int64_t word = wide ? 16 : 2;
+    const Pool p{static_cast<uint8_t*>(pool), planes, plane_pages, page_tokens, token_bytes};
     auto s = static_cast<hipStream_t>(stream);
-    CopyBatch batch;
-    for (int64_t done = 0; done < pairs;) {
-      int n = 0;
-      int64_t most = 0;
-      for (; done < pairs && n < kBatch; ++done) {
-        const int32_t t = tokens ? tokens[done] : static_cast<int32_t>(page_tokens);
-        if (t == 0) continue;
-        batch.src[n] = src[done];
-        batch.dst[n] = dst[done];
-        batch.tokens[n++] = t;
-        most = std::max<int64_t>(most, t);
-      }
-      if (n == 0) break;
-      const int64_t parts = (most * token_bytes / word + kThreads * kUnroll - 1) /
-                            (kThreads * kUnroll);
-      if (parts > (int64_t(1) << 31) / kThreads)
-        return set_error("mi355x_copy_pages: page too large");
-      const dim3 grid(static_cast<uint32_t>(parts), static_cast<uint32_t>(n),
-                      static_cast<uint32_t>(planes));
-      auto* base = static_cast<uint8_t*>(pool);
-      if (wide)
-        copy_pages_kernel<uint4><<<grid, dim3(kThreads), 0, s>>>(
-            base, plane_pages * page_bytes, page_bytes, token_bytes, batch);
-      else
-        copy_pages_kernel<uint16_t><<<grid, dim3(kThreads), 0, s>>>(
-            base, plane_pages * page_bytes, page_bytes, token_bytes, batch);
-      if (const char* err = launch_status("mi355x_copy_pages")) return err;
-    }
-    return nullptr;
+    return tokens ? copy_all<PartialBatch>(p, src, dst, tokens, pairs, wide, s)
+                  : copy_all<WholeBatch>(p, src, dst, nullptr, pairs, wide, s);
   } catch (const std::exception& e) {
     return set_error(e.what());
   }

@@ -23,6 +23,7 @@
 // them. A request that shares nothing and whose keys one item holds is written directly.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 #include <limits>
 
@@ -453,6 +454,23 @@ __device__ __forceinline__ void gemm_items(const SharedArgs& a, uint8_t* lds, in
       for (int kk = 0; kk < 8; ++kk)
 #pragma unroll
         for (int T = 0; T < 2; ++T) s[T] = Mfma<DT>::run(kf[T][kk], qreg[kk], s[T]);
+      auto load_v = [&](int kk, int db) {
+        lds_u8* vp = (lds_u8*)sb + v_off[db] + 16 * kk * 256;
+        const uint2 l2 =
+            __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)vp));
+        const uint2 h2 = __builtin_bit_cast(
+            uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vp + 8 * 256)));
+        return make_uint4(l2.x, l2.y, h2.x, h2.y);
+      };
+      // Half of V's operands are loaded behind the scores' products, the others where they are used:
+      // all of them early do not fit the registers (256 rows over 8,192 tokens, four layers: none
+      // early 516 us, half 511, all, with spills, 551).
+      constexpr int kEarly = NW == 8 ? 2 : 0;
+      uint4 vf[2][4];
+#pragma unroll
+      for (int kk = 0; kk < kEarly; ++kk)
+#pragma unroll
+        for (int db = 0; db < 4; ++db) vf[kk][db] = load_v(kk, db);
       if (k0 + kTileK - 1 > first_horizon || k0 + kTileK > kv_len) {
         const int limit = horizon - (k0 + 4 * half);
 #pragma unroll
@@ -507,14 +525,8 @@ __device__ __forceinline__ void gemm_items(const SharedArgs& a, uint8_t* lds, in
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-        for (int db = 0; db < 4; ++db) {
-          lds_u8* vp = (lds_u8*)sb + v_off[db] + 16 * kk * 256;
-          const uint2 l2 =
-              __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)vp));
-          const uint2 h2 = __builtin_bit_cast(
-              uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vp + 8 * 256)));
-          o[db] = Mfma<DT>::run(make_uint4(l2.x, l2.y, h2.x, h2.y), pb[kk], o[db]);
-        }
+        for (int db = 0; db < 4; ++db)
+          o[db] = Mfma<DT>::run(kk < kEarly ? vf[kk & 1][db] : load_v(kk, db), pb[kk], o[db]);
     };
 
     if (fast_pages) load_ids(t_begin);
@@ -783,40 +795,53 @@ struct Source {
 
 struct GemmCount {
   int64_t items = 0, slots = 0;
+  int64_t longs = 0;    // items of at least half the longest part's tiles ...
+  int64_t rest = 0;     // ... and what the others take, in tiles
 };
+constexpr int64_t kItemTiles = 2;  // an item besides its tiles: its queries, first tile, partial
 GemmCount count_gemm(const std::vector<Source>& sources, int64_t group, int64_t num_kv_heads,
                      int64_t columns, int64_t length) {
   GemmCount n;
   for (const Source& s : sources) {
     const int64_t tiles = ceil_div(s.end, kTileK) - s.begin / kTileK;
     const int64_t splits = std::max<int64_t>(1, ceil_div(tiles, length));
-    n.items += ceil_div(s.tokens * group, columns) * num_kv_heads * splits;
+    const int64_t items = ceil_div(s.tokens * group, columns) * num_kv_heads * splits;
+    n.items += items;
     n.slots += s.tokens * splits;
+    if (2 * tiles >= splits * length)
+      n.longs += items;
+    else
+      n.rest += items * (ceil_div(tiles, splits) + kItemTiles);
   }
   return n;
 }
 
-// Tiles of a part's keys, such that the launch ends soonest: rounds of items over the chip, each as
-// long as its longest part and what an item costs besides its tiles (its queries, its first tile and
-// its partial: about two tiles), and the parts that the merge has to read.
+// Tiles of a part's keys, such that the launch and its merge end soonest: rounds of long items over
+// the chip, the short ones in what the last round leaves, and the partial outputs that are written and
+// read again (`merge_tiles` a slot, in tiles of time).
 struct GemmLength {
   int64_t tiles;
   double tile_times;  // until the last item has ended, in tiles
 };
 GemmLength gemm_length(const std::vector<Source>& sources, int64_t group, int64_t num_kv_heads,
-                       int64_t columns, int64_t slots, const GemmCount& cap) {
-  constexpr double kItemTiles = 2.0, kMergeTiles = 0.25;
+                       int64_t columns, int64_t wgs, double merge_tiles, const GemmCount& cap) {
   int64_t longest = 1;
   for (const Source& s : sources)
     longest = std::max(longest, ceil_div(s.end, kTileK) - s.begin / kTileK);
   GemmLength best{longest, 0};
   double least = 0;
-  for (int64_t parts = 1; parts <= std::min<int64_t>(longest, 256); ++parts) {
+  for (int64_t parts = 1, last = 0; parts <= std::min<int64_t>(longest, 256);
+       parts += 1 + parts / 8) {
     const int64_t l = ceil_div(longest, parts);
+    if (l == last) continue;
+    last = l;
     const GemmCount n = count_gemm(sources, group, num_kv_heads, columns, l);
     if (n.items > cap.items || n.slots > cap.slots) break;
-    const double run = static_cast<double>(ceil_div(n.items, slots)) * (l + kItemTiles);
-    const double est = run + kMergeTiles * parts;
+    const int64_t rounds = ceil_div(n.longs, wgs);
+    const int64_t idle = (rounds * wgs - n.longs) * (l + kItemTiles);
+    const double run = static_cast<double>(rounds * (l + kItemTiles)) +
+                       static_cast<double>(std::max<int64_t>(0, n.rest - idle)) / wgs;
+    const double est = run + merge_tiles * n.slots;
     if (parts == 1 || est < least) {
       least = est;
       best = {l, run};
@@ -880,6 +905,21 @@ const char* check_groups(const int32_t* group_rows, const int32_t* group_lens, i
   return row == batch ? nullptr : "invalid shared prefix groups";
 }
 
+namespace {
+// Bytes of K and V that sharing has to save a layer: less is lost again on the products' launch and
+// the merge. us a layer, plain against shared (32 heads, 8 kv heads): 2 rows of 1,024 tokens (4 MB)
+// 11.7, 13.2; 8 of 256 (7 MB) 13.5, 13.1; 4 of 1,024 (12 MB) 13.4, 13.3; 16 of 1,024 (60 MB) 16.2,
+// 14.3; 256 of 1,024 117, 33. With fewer kv heads than a slice has the plain kernel is the slower one
+// throughout (one kv head: 22, 13). MI355X_SHARED_FROM (bytes) overrides it and kShortest (tuning
+// knob, read for every plan).
+int64_t least_saved(int64_t num_kv_heads) {
+  if (const char* env = std::getenv("MI355X_SHARED_FROM")) return std::strtoll(env, nullptr, 10);
+  return num_kv_heads % 4 ? 0 : int64_t(8) << 20;
+}
+// Prefixes of 64 tokens are not worth it in any batch (256 rows: 24.4 us plain, 30.5 shared).
+int32_t shortest_prefix() { return std::getenv("MI355X_SHARED_FROM") ? kTileK : 2 * kTileK; }
+}  // namespace
+
 struct SharedPlan::State {
   int64_t cus, num_q_heads, num_kv_heads, page_size, dtype, group;
   int group_log2 = 0;
@@ -911,7 +951,8 @@ struct SharedPlan::State {
       int64_t len = std::min<int64_t>(b.group_lens[g], kMaxKeys - kTileK);
       for (int64_t r = row; r < row + b.group_rows[g]; ++r)
         len = std::min<int64_t>(len, b.kv_len[r] - (b.q_start[r + 1] - b.q_start[r]));
-      if (b.group_rows[g] > 1) eff[g] = static_cast<int32_t>(len / kTileK * kTileK);
+      if (b.group_rows[g] > 1 && len >= shortest_prefix())
+        eff[g] = static_cast<int32_t>(len / kTileK * kTileK);
       row += b.group_rows[g];
     }
     return eff;
@@ -929,9 +970,14 @@ SharedPlan::SharedPlan(int64_t cus, int64_t num_q_heads, int64_t num_kv_heads, i
 SharedPlan::~SharedPlan() = default;
 
 bool SharedPlan::pays(const SharedBatch& b) const {
-  for (const int32_t n : st_->lengths(b))
-    if (n > 0) return true;
-  return false;
+  const std::vector<int32_t> eff = st_->lengths(b);
+  int64_t saved = 0;
+  bool any = false;
+  for (int64_t g = 0; g < b.groups; ++g) {
+    saved += int64_t(b.group_rows[g] - 1) * eff[g] * st_->num_kv_heads * kD * 4;
+    any |= eff[g] > 0;
+  }
+  return any && saved >= least_saved(st_->num_kv_heads);
 }
 
 bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph_tokens,
@@ -989,8 +1035,12 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
         gemm.push_back(own);
       }
     }
-    // How the products and the copies share the chip, by what either takes alone.
-    int64_t cost4 = 0, cost8 = 0;  // tiles of half a CU and of a CU
+    // How the products and the copies share the chip. Whole CUs for either wherever there are both and
+    // eight kv heads (us a layer, in turn, in halves, on whole CUs: 256 rows sharing 8,192 tokens 141,
+    // 136, 117; 64 sharing 2,048 44, 38, 29; 75 rows of up to 16 new tokens in 8 groups 65, 63, 54);
+    // halves with four; in turn where the copies are next to nothing (48 rows of up to 40 new tokens
+    // 103, 141, 110).
+    int64_t cost4 = 0, cost8 = 0;  // tiles of 128 and of 256 columns
     for (const Source& src : gemm) {
       const int64_t tiles = ceil_div(src.end, kTileK) - src.begin / kTileK;
       cost4 += ceil_div(src.tokens * group, 128) * tiles * heads;
@@ -998,65 +1048,55 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
     }
     int64_t bytes = 0;
     for (const Source& src : stream) bytes += int64_t(src.end - src.begin) * heads * kD * 4;
-    // A CU's tile of 256 columns, where all CUs multiply and where others stream; the copies' rate.
-    constexpr double kTileUs = 2.4, kMixedTileUs = 1.68, kBytesPerUs = 5.86e6;
-    const double gemm_us = kTileUs * static_cast<double>(cost8) / static_cast<double>(st.cus);
+    // A CU's tile of 256 columns while others stream, and the copies' rate on the whole chip.
+    constexpr double kTileUs = 1.68, kBytesPerUs = 5.86e6;
     const double stream_us = static_cast<double>(bytes) / kBytesPerUs;
-    StreamShape shape = st.shape;
-    int64_t gemm_wgs = 0;
+    st.form = st.shape.waves == 4 && !stream.empty() ? Form::kHalves : Form::kInTurn;
+    if (heads % 8 == 0 && (graph_rows ? graph_rows * group > 128
+                                      : !gemm.empty() && stream_us > 1))
+      st.form = Form::kWhole;
+    else if (!graph_rows && !gemm.empty() && stream_us <= 1)
+      st.form = Form::kInTurn;
+    st.nw = st.form == Form::kWhole || (st.form == Form::kInTurn && 4 * cost8 <= 3 * cost4) ? 8 : 4;
+    const int64_t columns = 32 * st.nw;
     // Bounds on the products' items and partial outputs, beside one part a source: a graph plan's
     // hold for whatever its rows will share.
-    auto capacity = [&](int64_t columns) {
-      const int64_t extra = 2 * st.cus, per = columns / group;  // tokens of an item
-      if (graph_rows) {
-        // at most rows / 2 groups share, each with a last tile that is not full
-        cap.items = (graph_rows / per + graph_rows / 2) * heads + extra;
-        cap.slots = graph_rows + extra * per / heads;
-      } else {
-        cap = count_gemm(gemm, group, heads, columns, std::numeric_limits<int32_t>::max());
-        cap.items += extra;
-        cap.slots += extra * per;
-      }
-    };
-    // Whole CUs: as many for the products as end the launch soonest. A CU streams no faster for
-    // others' idling, so that the copies take longer by the share that the products have.
-    double whole_us = std::numeric_limits<double>::infinity();
-    if (heads % 8 == 0 && (!gemm.empty() || graph_rows)) {
-      capacity(256);
-      for (int64_t wgs8 = st.cus / 16; wgs8 <= st.cus - st.cus / 8 && !gemm.empty(); wgs8 += 4) {
+    const int64_t extra = 2 * st.cus, per = columns / group;  // tokens of an item
+    if (graph_rows) {
+      // at most rows / 2 groups share, each with a last tile that is not full
+      cap.items = (graph_rows / per + graph_rows / 2) * heads + extra;
+      cap.slots = graph_rows + extra * per / heads;
+    } else {
+      cap = count_gemm(gemm, group, heads, columns, std::numeric_limits<int32_t>::max());
+      cap.items += extra;
+      cap.slots += extra * per;
+    }
+    // A slot's partial outputs, written and read at about 5 TB/s.
+    const double merge_tiles = static_cast<double>(st.num_q_heads * 1056) / 5e6 / kTileUs;
+    StreamShape shape = st.shape;
+    int64_t gemm_wgs = st.form == Form::kHalves || st.nw == 8 ? st.cus : 2 * st.cus;
+    if (st.form == Form::kWhole) {
+      // As many CUs for the products as end the launch soonest. A CU streams no faster for others'
+      // not streaming: the copies take longer by the products' share.
+      double least = std::numeric_limits<double>::infinity();
+      gemm_wgs = 0;
+      for (int64_t wgs8 = std::max<int64_t>(1, st.cus / 16);
+           wgs8 <= st.cus - st.cus / 8 && !gemm.empty();
+           wgs8 += std::max<int64_t>({1, st.cus / 32, wgs8 / 8})) {
         const double run =
-            kMixedTileUs * gemm_length(gemm, group, heads, 256, wgs8, cap).tile_times;
+            kTileUs * gemm_length(gemm, group, heads, columns, wgs8, merge_tiles, cap).tile_times;
         const double est =
-            std::max(run, stream_us * static_cast<double>(st.cus) / (st.cus - wgs8)) + 5;
-        if (est < whole_us) {
-          whole_us = est;
+            std::max(run, stream_us * static_cast<double>(st.cus) / (st.cus - wgs8));
+        if (est < least) {
+          least = est;
           gemm_wgs = wgs8;
         }
       }
-    }
-    // Half CUs: a fit to measured mixes (products alone, copies alone -> kernel, us: 38 and 92 -> 145,
-    // 38 and 34 -> 72, 19 and 17 -> 39, 10 and 46 -> 68, 10 and 7 -> 23; on whole CUs 119, 79, 46, 60
-    // and 29).
-    const double halves_us = 0.6 * gemm_us + 1.26 * stream_us + 6;
-    st.form = Form::kInTurn;
-    if (heads % 8 == 0 && (graph_rows ? graph_rows * group > 128 : whole_us < halves_us))
-      st.form = Form::kWhole;
-    else if (st.shape.waves == 4 && (graph_rows || stream_us > 0.3 * gemm_us))
-      st.form = Form::kHalves;
-    st.nw = st.form == Form::kWhole || (st.form == Form::kInTurn && 2 * cost8 <= cost4) ? 8 : 4;
-    const int64_t columns = 32 * st.nw;
-    if (st.form != Form::kWhole)
-      gemm_wgs = st.form == Form::kHalves || st.nw == 8 ? st.cus : 2 * st.cus;
-    capacity(columns);
-    if (st.form == Form::kWhole) {
       // A share for every CU that streams: more of them end later where the last ones find no CU free
       // (64 rows sharing 8,192 tokens, 192 such CUs: 192 shares 41.8 us, 256 49.7, 384 43, 512 49).
       shape = stream_shape(st.cus, heads, st.page_size, 8);
-      shape.workgroups = (st.cus - gemm_wgs) / shape.grid_y;
-      if (!graph_rows)
-        shape.wg_capacity = shape.workgroups + shape.workgroups / 3 + 2;
-      else
-        shape.wg_capacity = st.cus / shape.grid_y + st.cus / 3 + 2;
+      shape.workgroups = std::max<int64_t>(1, (st.cus - gemm_wgs) / shape.grid_y);
+      shape.wg_capacity = st.cus / shape.grid_y + st.cus / 3 + 2;
     }
     // The streaming launch.
     lens.clear();
@@ -1099,7 +1139,7 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
     const int64_t stream_slots = slot;
     if (!gemm.empty())
       schedule_gemm(gemm, group, heads, columns,
-                    gemm_length(gemm, group, heads, columns, gemm_wgs, cap).tiles, slot,
+                    gemm_length(gemm, group, heads, columns, gemm_wgs, merge_tiles, cap).tiles, slot,
                     gemm_work);
     st.slices = shape.grid_y;
     graph_shape = shape;

@@ -50,7 +50,8 @@ def check_rows(eng, oracle, reqs, vocab):
 
 @pytest.mark.parametrize("use_graphs", [True, False])
 @pytest.mark.parametrize("share", [True, False])
-def test_completions_match_oracle(gpu, use_graphs, share):
+def test_completions_match_oracle(gpu, use_graphs, share, monkeypatch):
+    monkeypatch.setenv("MI355X_SHARED_FROM", "0")
     model, oracle = build(TINY, 1, gpu)
     eng = engine(model, use_graphs=use_graphs, share_prefixes=share)
     rng = np.random.default_rng(7)
@@ -72,8 +73,9 @@ def test_completions_match_oracle(gpu, use_graphs, share):
         assert len(group) == count and (count == 1 or len(set(group)) > 1)
 
 
-def test_completions_of_different_lengths(gpu):
+def test_completions_of_different_lengths(gpu, monkeypatch):
     """Completions that end early leave the others of their group, and their pages, alone."""
+    monkeypatch.setenv("MI355X_SHARED_FROM", "0")
     model, oracle = build(TINY, 2, gpu)
     for share in (True, False):
         eng = engine(model, share_prefixes=share)
@@ -89,8 +91,9 @@ def test_completions_of_different_lengths(gpu):
         check_rows(eng, oracle, reqs, TINY.vocab_size)
 
 
-def test_shared_prompt_is_used(gpu):
+def test_shared_prompt_is_used(gpu, monkeypatch):
     """Eager steps plan the common prompt as a shared prefix, graph steps too."""
+    monkeypatch.setenv("MI355X_SHARED_FROM", "0")
     model, _ = build(TINY, 3, gpu)
     for graphs in (True, False):
         eng = engine(model, use_graphs=graphs, share_prefixes=True)

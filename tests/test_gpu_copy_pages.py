@@ -48,7 +48,7 @@ def test_more_pairs_than_a_launch_holds(gpu):
     pool = make(2, 1500, 4, 2, 16)
     rng = np.random.default_rng(0)
     ids = rng.permutation(1500) + 1
-    for n in (240, 241, 480, 700):
+    for n in (240, 320, 321, 480, 481, 700):
         src, dst = ids[:n], ids[n:2 * n]
         tokens = rng.integers(0, 5, n)
         want = expect(pool, src.tolist(), dst.tolist(), tokens.tolist())

@@ -10,6 +10,13 @@ from llm_infer_rust_amd.backend import (AttentionMetadata, BatchPhase, DecodeHos
 from shared_helpers import Batch
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def shared_however_little_it_saves(monkeypatch):
+    monkeypatch.setenv("MI355X_SHARED_FROM", "0")
+
+
 BF16, FP16 = torch.bfloat16, torch.float16
 
 
@@ -76,6 +83,20 @@ def test_extend(gpu, groups, own, new, heads, kv_heads, page, dtype):
     plain, none = b.run(b.extend_meta(shared=False))
     assert none["items"] == 0
     b.check(plain)
+
+
+def test_what_saves_little_is_left_to_the_plain_kernels(gpu, monkeypatch):
+    """By default 8 MiB of K and V a layer are saved, by prefixes of at least 128 tokens, or nothing
+    is shared; with fewer kv heads than a slice holds it always is."""
+    monkeypatch.delenv("MI355X_SHARED_FROM")
+    for groups, kv_heads, used in (([(2, 1024)], 8, False), ([(4, 1024)], 8, True),
+                                   ([(256, 127)], 8, False), ([(40, 128), (3, 64)], 8, True),
+                                   ([(2, 128)], 1, True), ([(1, 5000)], 1, False)):
+        b = Batch(groups, [3] * sum(r for r, _ in groups), heads=4 * kv_heads, kv_heads=kv_heads)
+        got, info = b.run(b.decode_meta())
+        assert (info["items"] > 0) == used, (groups, info)
+        b.check(got)
+        assert info["tokens"] == (sum(n for r, n in groups if r > 1 and n >= 128) if used else 0)
 
 
 def test_whole_request_is_shared(gpu):
