@@ -21,6 +21,7 @@
 // selected by repeated maxima instead, at the cost of a pass over the row an alternative.
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "common.h"
 
@@ -32,9 +33,14 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMaxTop = 64;            // one lane an alternative
 constexpr int kGroup = 32;             // logits under one maximum in LDS
 constexpr int kCandidates = 1024;      // (key, index) entries in LDS
-constexpr int kWide = 512, kNarrow = 64;  // threads of a workgroup: long rows, short rows
-// Rows up to this go to single waves: eight groups of 512 threads wait for each other at barriers
-// about as long as such a row takes.
+// Threads of a workgroup, for long rows and short ones. us, 256 threads a long row against 512 and 128:
+// 4,096 rows of 151,936 bf16 logits with 5 alternatives 230 (5.4 TB/s), 239, 268, without 216 (5.8
+// TB/s), 219, 229; 256 rows with 20 alternatives 27.0, 30.2, 42.8, without 16.7, 23, 27. Bound by memory
+// and, nearly as much, by the dozen vector operations a logit. Registers are not capped for another
+// workgroup a CU: at 80 they spill (414 us).
+constexpr int kWide = 256, kNarrow = 64;
+// Rows up to this go to single waves, which have no barriers to wait at (4,096 rows of 8,000 logits:
+// 22 us, with four waves a row 40).
 constexpr int64_t kNarrowVocab = 8192;
 // Logits under one workgroup: bounds the maxima in LDS to 32 KiB.
 constexpr int64_t kMaxSegment = 262144;
@@ -84,37 +90,82 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 __device__ __forceinline__ uint64_t rank_key(float x, uint32_t index) {
   return (static_cast<uint64_t>(order_key(x)) << 32) | ~index;
 }
+__device__ __forceinline__ float rank_value(uint64_t key) {
+  const uint32_t k = static_cast<uint32_t>(key >> 32);
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
 __device__ __forceinline__ uint32_t rank_index(uint64_t key) {
   return ~static_cast<uint32_t>(key);
 }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int mask) {
-  const uint32_t lo = __shfl_xor(static_cast<uint32_t>(v), mask);
-  const uint32_t hi = __shfl_xor(static_cast<uint32_t>(v >> 32), mask);
+// The value of lane ^ MASK, by register moves (LDS shuffles take several times as long, and sorting
+// is a chain of them).
+template <int MASK>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  constexpr int kQuadReverse = 0x1B, kRowRotate8 = 0x128;
+  auto move = [](uint32_t x, auto ctrl) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+        0, static_cast<int>(x), decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  if constexpr (MASK == 1) {
+    return move(v, std::integral_constant<int, kDppQuadSwap1>{});
+  } else if constexpr (MASK == 2) {
+    return move(v, std::integral_constant<int, kDppQuadSwap2>{});
+  } else if constexpr (MASK == 4) {  // 7 - i, then 3 - i within four
+    return move(move(v, std::integral_constant<int, kDppRowHalfMirror>{}),
+                std::integral_constant<int, kQuadReverse>{});
+  } else if constexpr (MASK == 8) {
+    return move(v, std::integral_constant<int, kRowRotate8>{});
+  } else if constexpr (MASK == 16) {
+    const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? s[0] : s[1];
+  } else if constexpr (MASK == 32) {
+    const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? s[0] : s[1];
+  } else {
+    static_assert(MASK == 63, "one bit, or all");
+    return lane_xor<32>(
+        lane_xor<16>(move(v, std::integral_constant<int, kDppRowMirror>{})));
+  }
+}
+template <int MASK>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
+  const uint32_t lo = lane_xor<MASK>(static_cast<uint32_t>(v));
+  const uint32_t hi = lane_xor<MASK>(static_cast<uint32_t>(v >> 32));
   return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+template <int MASK>
+__device__ __forceinline__ float lane_xor(float v) {
+  return __uint_as_float(lane_xor<MASK>(__float_as_uint(v)));
+}
+// f(std::integral_constant<int, 2^i>) for the strides FROM, FROM / 2, .. 1.
+template <int FROM, typename F>
+__device__ __forceinline__ void strides_down(F&& f) {
+  f(std::integral_constant<int, FROM>{});
+  if constexpr (FROM > 1) strides_down<FROM / 2>(f);
 }
 __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
-// The wave's 64 keys in descending order, lane 0 the largest.
+// The wave's 64 keys in descending order, lane 0 the largest: SIZE keys at a time.
+template <int SIZE = 64>
 __device__ __forceinline__ uint64_t sort_desc(uint64_t v, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 64; size *= 2)
-#pragma unroll
-    for (int stride = size / 2; stride >= 1; stride /= 2) {
-      const uint64_t o = shfl_xor64(v, stride);
-      const bool larger = ((lane & size) == 0 || size == 64) == ((lane & stride) == 0);
-      v = (v > o) == larger ? v : o;
-    }
+  if constexpr (SIZE > 2) v = sort_desc<SIZE / 2>(v, lane);
+  strides_down<SIZE / 2>([&](auto stride) {
+    constexpr int kStride = decltype(stride)::value;
+    const uint64_t o = lane_xor<kStride>(v);
+    const bool larger = ((lane & SIZE) == 0 || SIZE == 64) == ((lane & kStride) == 0);
+    v = (v > o) == larger ? v : o;
+  });
   return v;
 }
 // The 64 largest of two descending runs, descending.
 __device__ __forceinline__ uint64_t merge_desc(uint64_t a, uint64_t b, int lane) {
-  uint64_t v = max64(a, shfl_xor64(b, 63));
-#pragma unroll
-  for (int stride = 32; stride >= 1; stride /= 2) {
-    const uint64_t o = shfl_xor64(v, stride);
-    v = (v > o) == ((lane & stride) == 0) ? v : o;
-  }
+  uint64_t v = max64(a, lane_xor<63>(b));
+  strides_down<32>([&](auto stride) {
+    constexpr int kStride = decltype(stride)::value;
+    const uint64_t o = lane_xor<kStride>(v);
+    v = (v > o) == ((lane & kStride) == 0) ? v : o;
+  });
   return v;
 }
 
@@ -149,9 +200,10 @@ __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
   return r;
 }
 __device__ __forceinline__ Stats wave_join(Stats v) {
-#pragma unroll
-  for (int off = 1; off < kWave; off *= 2)
-    v = join(v, {__shfl_xor(v.m, off), __shfl_xor(v.s, off), __shfl_xor(v.w, off)});
+  strides_down<32>([&](auto stride) {
+    constexpr int kStride = decltype(stride)::value;
+    v = join(v, {lane_xor<kStride>(v.m), lane_xor<kStride>(v.s), lane_xor<kStride>(v.w)});
+  });
   return v;
 }
 
@@ -169,12 +221,20 @@ struct LogprobArgs {
   uint64_t* part_keys;   // [rows][segments][top]
 };
 
-// What one wave writes of a row whose sums and alternatives (descending over the lanes) it has.
+// The given token's logit: NaN outside the vocabulary. Loaded at a kernel's start, as it takes two
+// loads in turn.
 template <int DT>
-__device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, const Stats& st,
-                                          uint64_t key, int lane) {
+__device__ __forceinline__ float given_logit(const LogprobArgs& a, int64_t row) {
   using R = Row<DT>;
-  const auto* x = static_cast<const typename R::Word*>(a.logits) + row * a.stride;
+  const int64_t tok = a.tokens[row];
+  return tok >= 0 && tok < a.vocab
+             ? R::value(static_cast<const typename R::Word*>(a.logits)[row * a.stride + tok])
+             : __builtin_nanf("");
+}
+
+// What one wave writes of a row whose sums and alternatives (descending over the lanes) it has.
+__device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, const Stats& st,
+                                          uint64_t key, float given, int lane) {
   // v_log_f32 (log2); s >= 1 or 0, NaN for rows with a NaN or +inf. A row of only -inf: s = 0.
   const float bits = __builtin_amdgcn_logf(st.s);
   auto lp = [&](float v) {
@@ -183,14 +243,12 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, con
     return (fmaf(v, kLog2e, -(st.m * kLog2e)) - bits) * kLn2;
   };
   if (lane == 0) {
-    const int64_t tok = a.tokens[row];
-    a.lp[row] = tok >= 0 && tok < a.vocab ? lp(R::value(x[tok])) : __builtin_nanf("");
+    a.lp[row] = lp(given);
     a.entropy[row] = (bits - st.w / st.s) * kLn2;
   }
   if (lane < a.top) {
-    const uint32_t id = rank_index(key);
-    a.ids[row * a.top + lane] = id;
-    a.top_lp[row * a.top + lane] = lp(R::value(x[id]));
+    a.ids[row * a.top + lane] = rank_index(key);
+    a.top_lp[row * a.top + lane] = lp(rank_value(key));
   }
 }
 
@@ -208,8 +266,7 @@ struct Scratch {
 // Largest of the threads' keys, in every thread.
 template <int THREADS>
 __device__ __forceinline__ uint64_t block_max(Scratch<THREADS>& sh, uint64_t v) {
-#pragma unroll
-  for (int off = 1; off < kWave; off *= 2) v = max64(v, shfl_xor64(v, off));
+  strides_down<32>([&](auto stride) { v = max64(v, lane_xor<decltype(stride)::value>(v)); });
   if constexpr (THREADS > kWave) {
     if (threadIdx.x % kWave == 0) sh.best[threadIdx.x / kWave] = v;
     __syncthreads();
@@ -348,6 +405,9 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a) {
   const int steps = (all_vecs + VPT * THREADS - 1) / (VPT * THREADS);
   const int whole_steps = vecs / (VPT * THREADS);
 
+  float given = 0.f;
+  if (wave == 0 && a.segments == 1) given = given_logit<DT>(a, row);
+
   float m = -kFarRef, ref = 0.f, s = 0.f, w = 0.f;
   float best = -INFINITY;
   uint32_t best_vec = 0xffffffffu;
@@ -405,9 +465,9 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a) {
       for (int j = 0; j < VPT; ++j) now[j] = next[j];
     }
   }
+  uint4 raw[VPT];
   if (steps > whole_steps) {  // the last step: vectors that are there, the row's end by logits
     constexpr uint32_t kNone = DT == 0 ? 0xff80ff80u : DT == 1 ? 0xfc00fc00u : 0xff800000u;
-    uint4 raw[VPT];
     int have = 0;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
@@ -457,6 +517,27 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a) {
       if (wave == 0) find_bound<DT, THREADS>(sh, a.top, lane);
       __syncthreads();
       const uint32_t bound = sh.bound_key, bound_vec = sh.bound_vec;
+      auto consider = [&](float value, int v, int at) {
+        const uint32_t k = order_key(value) >> R::kKeyShift;
+        if (k > bound || (k == bound && static_cast<uint32_t>(v) <= bound_vec)) {
+          const uint32_t slot = atomicAdd(&sh.count, 1u);
+          if (slot < kCandidates) sh.cand[slot] = rank_key(value, static_cast<uint32_t>(begin) + at);
+        }
+      };
+      if (whole_steps == 0) {
+        // All of it is still in registers: the threads whose largest is in reach compare their own.
+        if (sh.key[tid] >= bound && sh.key[tid] != 0) {
+#pragma unroll
+          for (int j = 0; j < VPT; ++j) {
+            const int v = j * THREADS + tid;
+            float f[V];
+            R::widen(raw[j], f);
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+              if (v * V + i < n) consider(f[i], v, v * V + i);
+          }
+        }
+      } else {
       // Groups in reach: one wave reads a group's kGroup logits twice at a time, two groups.
       for (int step = 0; step < steps; ++step) {
         const float gm = group_max[step * THREADS + tid];
@@ -471,16 +552,9 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a) {
           const int e = lane % kGroup;
           const int v = (step * VPT + e / V) * THREADS + wave * kWave + who;
           const int at = v * V + e % V;
-          if (who >= 0 && at < n) {
-            const float value = R::value(x[at]);
-            const uint32_t k = order_key(value) >> R::kKeyShift;
-            if (k > bound || (k == bound && static_cast<uint32_t>(v) <= bound_vec)) {
-              const uint32_t slot = atomicAdd(&sh.count, 1u);
-              if (slot < kCandidates)
-                sh.cand[slot] = rank_key(value, static_cast<uint32_t>(begin) + at);
-            }
-          }
+          if (who >= 0 && at < n) consider(R::value(x[at]), v, at);
         }
+      }
       }
       __syncthreads();
       const int count = static_cast<int>(sh.count);
@@ -498,7 +572,7 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a) {
   }
   if (wave != 0) return;
   if (a.segments == 1) {
-    write_row<DT>(a, row, st, key, lane);
+    write_row(a, row, st, key, given, lane);
     return;
   }
   const int64_t part = row * a.segments + seg;
@@ -511,15 +585,32 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a) {
 template <int DT>
 __global__ __launch_bounds__(1024) void logprob_join_kernel(LogprobArgs a) {
   constexpr int kWaves = 16;
+  constexpr int kRuns = 4;  // a wave's runs at a time, loaded together
   __shared__ uint64_t runs[kWaves][kWave];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int64_t row = blockIdx.x;
+  const int64_t part0 = row * a.segments;
+  float given = 0.f;
+  Stats st{-FLT_MAX, 0.f, 0.f};
+  if (wave == 0) {
+    given = given_logit<DT>(a, row);
+    for (int seg = lane; seg < a.segments; seg += kWave) {
+      const float4 p = a.part_stats[part0 + seg];
+      st = join(st, {p.x, p.y, p.z});
+    }
+  }
   uint64_t key = 0;
   if (a.top) {
-    for (int seg = wave; seg < a.segments; seg += kWaves) {
-      const int64_t part = row * a.segments + seg;
-      const uint64_t run = lane < a.top ? a.part_keys[part * a.top + lane] : 0;
-      key = seg == wave ? run : merge_desc(key, run, lane);
+    for (int first = wave; first < a.segments; first += kRuns * kWaves) {
+      uint64_t run[kRuns];
+#pragma unroll
+      for (int r = 0; r < kRuns; ++r) {
+        const int seg = first + r * kWaves;
+        run[r] = seg < a.segments && lane < a.top ? a.part_keys[(part0 + seg) * a.top + lane] : 0;
+      }
+#pragma unroll
+      for (int r = 0; r < kRuns; ++r)
+        if (first + r * kWaves < a.segments) key = merge_desc(key, run[r], lane);
     }
     const int waves = min(kWaves, a.segments);
     for (int stride = 1; stride < waves; stride *= 4) {  // uniform
@@ -533,21 +624,17 @@ __global__ __launch_bounds__(1024) void logprob_join_kernel(LogprobArgs a) {
     }
   }
   if (wave != 0) return;
-  Stats st{-FLT_MAX, 0.f, 0.f};
-  for (int seg = lane; seg < a.segments; seg += kWave) {
-    const float4 p = a.part_stats[row * a.segments + seg];
-    st = join(st, {p.x, p.y, p.z});
-  }
-  write_row<DT>(a, row, wave_join(st), key, lane);
+  write_row(a, row, wave_join(st), key, given, lane);
 }
 
-// Segments of a row, so that few rows fill the chip.
+// Segments of a row, so that few rows fill the chip: a workgroup a CU (two a CU: 256 rows of 151,936
+// logits 29.5 us against 27.0, of 32,000 18.4 against 14.2).
 struct Split {
   int64_t segments, length;
 };
 Split split_of(int64_t rows, int64_t vocab, int64_t cus) {
   const int64_t least = (vocab + kMaxSegment - 1) / kMaxSegment;
-  int64_t want = rows > 0 ? (2 * cus + rows - 1) / rows : 1;
+  int64_t want = rows > 0 ? (cus + rows - 1) / rows : 1;
   want = std::min(want, vocab / 2048);  // shorter ones cost more to join than they save
   const int64_t segments = std::max<int64_t>(least, std::min<int64_t>(want, 64));
   const int64_t length = ((vocab + segments - 1) / segments + 7) / 8 * 8;

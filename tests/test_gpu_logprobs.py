@@ -30,8 +30,8 @@ def reference(x, tokens, top):
 
 
 def tolerance(x):
-    """A thread's chain of fp32 additions holds at most 1,024 terms (a row of 262,144 logits over
-    512 threads, two chains) with the trees above it, each off by 2^-24 of the sum; a term's own
+    """A thread's chain of fp32 additions holds at most 1,024 terms (a segment of 262,144 logits
+    over 256 threads) with the trees above it, each off by 2^-24 of the sum; a term's own
     exponent is off by 2^-24 of its distance R to the row's maximum, in log2 units, and so is the
     result's. Eight for the exp2, log2 and the products around them."""
     d = x.detach().cpu().double()
