@@ -511,7 +511,8 @@ const char* mi355x_sample_split(const void* logits, int64_t rows, int64_t vocab,
 int64_t mi355x_sample_workspace_bytes(int64_t rows, int64_t vocab, bool top_p_rows);
 
 /* Log probabilities of given tokens, entropy and the most likely alternatives of logits rows
- * (dtype 0 bf16, 1 fp16, 2 fp32; row stride in elements, any alignment of the type):
+ * of up to 16,777,216 (dtype 0 bf16, 1 fp16, 2 fp32; row stride in elements, any alignment of the
+ * type):
  * logprobs[r] = log softmax(x[r])[tokens[r]] (NaN for a token outside [0, vocab)), entropy[r] =
  * -sum p log p in nats, top_ids[r, :] the `top` (0 to 64, at most vocab) largest logits, largest
  * first, equal ones by the lower index, top_logprobs[r, :] theirs. logprobs, entropy and

@@ -42,6 +42,7 @@ constexpr int kWide = 256, kNarrow = 64;
 // Rows up to this go to single waves, which have no barriers to wait at (4,096 rows of 8,000 logits:
 // 22 us, with four waves a row 40).
 constexpr int64_t kNarrowVocab = 8192;
+constexpr int kMaxSegments = 64;       // of a row: what the joining workgroup holds
 // Logits under one workgroup: bounds the maxima in LDS to 32 KiB.
 constexpr int64_t kMaxSegment = 262144;
 // A reference from here on is left to careful_stats: the streaming loop's exponents are off by the
@@ -580,13 +581,12 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a) {
   if (lane < a.top) a.part_keys[part * a.top + lane] = key;
 }
 
-// Joins a row's segments: a workgroup of 16 waves, each merging every 16th segment's descending
-// run, then four waves four runs each, then one wave the last four.
+// Joins a row's segments, whose descending runs lie in LDS: 16 waves merge four each, then four waves
+// four of theirs, then one the last four. The merge stands in one place, in a loop: a launch of a few
+// workgroups pays for fetching its instructions, and unrolled copies cost more than they save.
 template <int DT>
 __global__ __launch_bounds__(1024) void logprob_join_kernel(LogprobArgs a) {
-  constexpr int kWaves = 16;
-  constexpr int kRuns = 4;  // a wave's runs at a time, loaded together
-  __shared__ uint64_t runs[kWaves][kWave];
+  __shared__ uint64_t runs[kMaxSegments][kWave];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int64_t row = blockIdx.x;
   const int64_t part0 = row * a.segments;
@@ -594,33 +594,32 @@ __global__ __launch_bounds__(1024) void logprob_join_kernel(LogprobArgs a) {
   Stats st{-FLT_MAX, 0.f, 0.f};
   if (wave == 0) {
     given = given_logit<DT>(a, row);
-    for (int seg = lane; seg < a.segments; seg += kWave) {
-      const float4 p = a.part_stats[part0 + seg];
-      st = join(st, {p.x, p.y, p.z});
+    if (lane < a.segments) {
+      const float4 p = a.part_stats[part0 + lane];
+      st = {p.x, p.y, p.z};
     }
   }
   uint64_t key = 0;
   if (a.top) {
-    for (int first = wave; first < a.segments; first += kRuns * kWaves) {
-      uint64_t run[kRuns];
+    uint64_t mine[4];
 #pragma unroll
-      for (int r = 0; r < kRuns; ++r) {
-        const int seg = first + r * kWaves;
-        run[r] = seg < a.segments && lane < a.top ? a.part_keys[(part0 + seg) * a.top + lane] : 0;
-      }
-#pragma unroll
-      for (int r = 0; r < kRuns; ++r)
-        if (first + r * kWaves < a.segments) key = merge_desc(key, run[r], lane);
+    for (int r = 0; r < 4; ++r) {
+      const int seg = 4 * wave + r;
+      mine[r] = seg < a.segments && lane < a.top ? a.part_keys[(part0 + seg) * a.top + lane] : 0;
     }
-    const int waves = min(kWaves, a.segments);
-    for (int stride = 1; stride < waves; stride *= 4) {  // uniform
-      const int step = stride * 4;
-      runs[wave][lane] = key;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) runs[4 * wave + r][lane] = mine[r];
+#pragma unroll 1
+    for (int step = 1; step < a.segments; step *= 4) {  // uniform; run 4 step w + i step, i < 4
       __syncthreads();
-      if (wave % step == 0)
-        for (int i = 1; i < 4; ++i)
-          if (wave + i * stride < waves) key = merge_desc(key, runs[wave + i * stride][lane], lane);
-      __syncthreads();
+      const int first = wave * 4 * step;
+      if (first < a.segments) {
+        key = runs[first][lane];
+#pragma unroll 1
+        for (int i = 1; i < 4 && first + i * step < a.segments; ++i)
+          key = merge_desc(key, runs[first + i * step][lane], lane);
+        runs[first][lane] = key;
+      }
     }
   }
   if (wave != 0) return;
@@ -636,7 +635,7 @@ Split split_of(int64_t rows, int64_t vocab, int64_t cus) {
   const int64_t least = (vocab + kMaxSegment - 1) / kMaxSegment;
   int64_t want = rows > 0 ? (cus + rows - 1) / rows : 1;
   want = std::min(want, vocab / 2048);  // shorter ones cost more to join than they save
-  const int64_t segments = std::max<int64_t>(least, std::min<int64_t>(want, 64));
+  const int64_t segments = std::max<int64_t>(least, std::min<int64_t>(want, kMaxSegments));
   const int64_t length = ((vocab + segments - 1) / segments + 7) / 8 * 8;
   return {(vocab + length - 1) / length, length};
 }
@@ -660,7 +659,7 @@ void launch(LogprobArgs a, int64_t rows, hipStream_t s) {
 }
 
 bool valid_shape(int64_t rows, int64_t vocab, int64_t top, int32_t cus) {
-  return rows >= 0 && vocab > 0 && vocab < (int64_t(1) << 31) - 8 && top >= 0 && top <= kMaxTop &&
+  return rows >= 0 && vocab > 0 && vocab <= kMaxSegments * kMaxSegment && top >= 0 && top <= kMaxTop &&
          top <= vocab && cus > 0 && rows < (int64_t(1) << 31);
 }
 

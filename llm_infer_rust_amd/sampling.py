@@ -291,8 +291,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     dt = _DTYPES.get(logits.dtype)
     if dt is None:
         raise NativeError(f"token_logprobs: unsupported logits dtype {logits.dtype}")
-    if vocab == 0:
-        raise NativeError("token_logprobs: rows must not be empty")
+    if not 0 < vocab <= 1 << 24:
+        raise NativeError("token_logprobs: expected rows of 1 to 16,777,216 logits")
     if (tokens.dtype != torch.int64 or tokens.shape != (rows,) or tokens.device != logits.device
             or not tokens.is_contiguous()):
         raise NativeError("token_logprobs: expected contiguous int64 tokens [rows] on the logits' "
