@@ -32,7 +32,7 @@ import numpy as np
 import torch
 
 from . import _native
-from ._native import NativeError, check, dtype_code, last_error, lib, stream_of
+from ._native import NativeError, check, dtype_code, last_error, lib, on_device, stream_of
 from .kv_cache import BaseAttention, ModelError
 
 
@@ -255,13 +255,14 @@ def prepare_decode_plan(existing: DecodePlan | None, metadata: AttentionMetadata
     args = (existing.handle if existing else None, table.data_ptr(), table.size(0), table.size(1),
             table.stride(0), lengths.data_ptr(), spec.num_heads, spec.num_kv_heads, spec.head_dim,
             page_size, dt, graph, host, rows)
-    if metadata.shared_prefix is None:
-        handle = lib().mi355x_decode_prepare(*args, stream_of(table))
-    else:
-        group_rows, group_lens = shared_arrays(metadata.shared_prefix, table.size(0))
-        handle = lib().mi355x_decode_prepare_shared(*args, group_rows.ctypes.data,
-                                                    group_lens.ctypes.data, group_rows.size,
-                                                    stream_of(table))
+    with on_device(table.device):
+        if metadata.shared_prefix is None:
+            handle = lib().mi355x_decode_prepare(*args, stream_of(table))
+        else:
+            group_rows, group_lens = shared_arrays(metadata.shared_prefix, table.size(0))
+            handle = lib().mi355x_decode_prepare_shared(*args, group_rows.ctypes.data,
+                                                        group_lens.ctypes.data, group_rows.size,
+                                                        stream_of(table))
     if not handle:
         raise ModelError(f"mi355x decode plan failed: {last_error()}")
     if existing is not None:
@@ -283,10 +284,12 @@ def run_decode(plan: DecodePlan, q: torch.Tensor, k_cache: torch.Tensor, v_cache
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
         raise ModelError("invalid decode output")
-    check(lib().mi355x_decode_run(
-        plan.handle, q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
-        v_cache.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), q.size(0), q.size(1),
-        k_cache.size(2), k_cache.size(1), dtype_code(q), stream_of(q)), "mi355x decode")
+    with on_device(q.device):
+        check(lib().mi355x_decode_run(
+            plan.handle, q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
+            v_cache.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), q.size(0),
+            q.size(1), k_cache.size(2), k_cache.size(1), dtype_code(q), stream_of(q)),
+            "mi355x decode")
     return out
 
 

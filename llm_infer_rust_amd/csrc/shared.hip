@@ -926,6 +926,7 @@ struct SharedPlan::State {
   StreamShape shape{};
   // Current plan.
   int64_t batch = 0, tokens = 0;
+  bool ready = false;
   bool by_token = false;  // requests of one token each
   int64_t stream_grid = 0, gemm_grid = 0, gemm_items = 0, gemm_wgs = 0;
   int sets = 1, nw = 4;
@@ -983,188 +984,174 @@ bool SharedPlan::pays(const SharedBatch& b) const {
 bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph_tokens,
                          uint64_t& allocations, hipStream_t s) {
   State& st = *st_;
+  st.ready = false;
   const int64_t group = st.group, heads = st.num_kv_heads;
   const int64_t tokens = b.q_start[b.batch];
-  std::vector<int32_t> eff = st.lengths(b);
+  const std::vector<int32_t> eff = st.lengths(b);
   std::vector<Source> stream, gemm;             // own and prefix sources of either kernel
   struct Of { int32_t kind, index; };           // 0 none, 1 stream, 2 gemm
-  std::vector<Of> prefix_of, own_of;
+  std::vector<Of> prefix_of(b.batch, Of{0, 0}), own_of(b.batch, Of{0, 0});
   std::vector<int32_t> lens, work, merge, wg, gemm_work;
   GemmCount cap;
   int64_t items = 0, wgs = 0, slot = 0, items_cap = 0;
   bool once = true;
-  StreamShape graph_shape{};
-  for (int attempt = 0; attempt < 2; ++attempt) {
-    stream.clear();
-    gemm.clear();
-    prefix_of.assign(b.batch, {0, 0});
-    own_of.assign(b.batch, {0, 0});
-    once = true;
-    st.groups_shared = st.tokens_shared = 0;
-    for (int64_t r = 0, g = 0, left = 0, before = 0; r < b.batch; ++r) {
-      if (left == 0 && g < b.groups) {  // a group begins
-        left = b.group_rows[g];
-        before = eff[g];
-        ++g;
-        if (before > 0) {
-          ++st.groups_shared;
-          st.tokens_shared += before;
-          const int64_t all = b.q_start[r + left] - b.q_start[r];
-          const Source src{b.q_start[r], static_cast<int32_t>(all), b.page_base[r], 0,
-                           static_cast<int32_t>(before), kNoHorizon};
-          if (all * group <= kStreamColumns) {
-            for (int64_t i = r; i < r + left; ++i)
-              prefix_of[i] = {1, static_cast<int32_t>(stream.size())};
-            stream.push_back(src);
-          } else {
-            for (int64_t i = r; i < r + left; ++i)
-              prefix_of[i] = {2, static_cast<int32_t>(gemm.size())};
-            gemm.push_back(src);
-          }
+  st.groups_shared = st.tokens_shared = 0;
+  for (int64_t r = 0, g = 0, left = 0, before = 0; r < b.batch; ++r) {
+    if (left == 0 && g < b.groups) {  // a group begins
+      left = b.group_rows[g];
+      before = eff[g];
+      ++g;
+      if (before > 0) {
+        ++st.groups_shared;
+        st.tokens_shared += before;
+        const int64_t all = b.q_start[r + left] - b.q_start[r];
+        const Source src{b.q_start[r], static_cast<int32_t>(all), b.page_base[r], 0,
+                         static_cast<int32_t>(before), kNoHorizon};
+        if (all * group <= kStreamColumns) {
+          for (int64_t i = r; i < r + left; ++i)
+            prefix_of[i] = {1, static_cast<int32_t>(stream.size())};
+          stream.push_back(src);
+        } else {
+          for (int64_t i = r; i < r + left; ++i)
+            prefix_of[i] = {2, static_cast<int32_t>(gemm.size())};
+          gemm.push_back(src);
         }
       }
-      const int32_t t = b.q_start[r + 1] - b.q_start[r];
-      const Source own{b.q_start[r], t, b.page_base[r], static_cast<int32_t>(left ? before : 0),
-                       b.kv_len[r], b.kv_len[r] - t};
-      if (left) --left;
-      if (t * group <= kStreamColumns) {
-        own_of[r] = {1, static_cast<int32_t>(stream.size())};
-        stream.push_back(own);
-      } else {
-        own_of[r] = {2, static_cast<int32_t>(gemm.size())};
-        gemm.push_back(own);
-      }
     }
-    // How the products and the copies share the chip. Whole CUs for either wherever there are both and
-    // eight kv heads (us a layer, in turn, in halves, on whole CUs: 256 rows sharing 8,192 tokens 141,
-    // 136, 117; 64 sharing 2,048 44, 38, 29; 75 rows of up to 16 new tokens in 8 groups 65, 63, 54);
-    // halves with four; in turn where the copies are next to nothing (48 rows of up to 40 new tokens
-    // 103, 141, 110).
-    int64_t cost4 = 0, cost8 = 0;  // tiles of 128 and of 256 columns
-    for (const Source& src : gemm) {
-      const int64_t tiles = ceil_div(src.end, kTileK) - src.begin / kTileK;
-      cost4 += ceil_div(src.tokens * group, 128) * tiles * heads;
-      cost8 += ceil_div(src.tokens * group, 256) * tiles * heads;
-    }
-    int64_t bytes = 0;
-    for (const Source& src : stream) bytes += int64_t(src.end - src.begin) * heads * kD * 4;
-    // A CU's tile of 256 columns while others stream, and the copies' rate on the whole chip.
-    constexpr double kTileUs = 1.68, kBytesPerUs = 5.86e6;
-    const double stream_us = static_cast<double>(bytes) / kBytesPerUs;
-    st.form = st.shape.waves == 4 && !stream.empty() ? Form::kHalves : Form::kInTurn;
-    if (heads % 8 == 0 && (graph_rows ? graph_rows * group > 128
-                                      : !gemm.empty() && stream_us > 1))
-      st.form = Form::kWhole;
-    else if (!graph_rows && !gemm.empty() && stream_us <= 1)
-      st.form = Form::kInTurn;
-    st.nw = st.form == Form::kWhole || (st.form == Form::kInTurn && 4 * cost8 <= 3 * cost4) ? 8 : 4;
-    const int64_t columns = 32 * st.nw;
-    // Bounds on the products' items and partial outputs, beside one part a source: a graph plan's
-    // hold for whatever its rows will share.
-    const int64_t extra = 2 * st.cus, per = columns / group;  // tokens of an item
-    if (graph_rows) {
-      // at most rows / 2 groups share, each with a last tile that is not full
-      cap.items = (graph_rows / per + graph_rows / 2) * heads + extra;
-      cap.slots = graph_rows + extra * per / heads;
+    const int32_t t = b.q_start[r + 1] - b.q_start[r];
+    const Source own{b.q_start[r], t, b.page_base[r], static_cast<int32_t>(left ? before : 0),
+                     b.kv_len[r], b.kv_len[r] - t};
+    if (left) --left;
+    if (t * group <= kStreamColumns) {
+      own_of[r] = {1, static_cast<int32_t>(stream.size())};
+      stream.push_back(own);
     } else {
-      cap = count_gemm(gemm, group, heads, columns, std::numeric_limits<int32_t>::max());
-      cap.items += extra;
-      cap.slots += extra * per;
+      own_of[r] = {2, static_cast<int32_t>(gemm.size())};
+      gemm.push_back(own);
     }
-    // A slot's partial outputs, written and read at about 5 TB/s.
-    const double merge_tiles = static_cast<double>(st.num_q_heads * 1056) / 5e6 / kTileUs;
-    StreamShape shape = st.shape;
-    int64_t gemm_wgs = st.form == Form::kHalves || st.nw == 8 ? st.cus : 2 * st.cus;
-    if (st.form == Form::kWhole) {
-      // As many CUs for the products as end the launch soonest. A CU streams no faster for others'
-      // not streaming: the copies take longer by the products' share.
-      double least = std::numeric_limits<double>::infinity();
-      gemm_wgs = 0;
-      for (int64_t wgs8 = std::max<int64_t>(1, st.cus / 16);
-           wgs8 <= st.cus - st.cus / 8 && !gemm.empty();
-           wgs8 += std::max<int64_t>({1, st.cus / 32, wgs8 / 8})) {
-        const double run =
-            kTileUs * gemm_length(gemm, group, heads, columns, wgs8, merge_tiles, cap).tile_times;
-        const double est =
-            std::max(run, stream_us * static_cast<double>(st.cus) / (st.cus - wgs8));
-        if (est < least) {
-          least = est;
-          gemm_wgs = wgs8;
-        }
-      }
-      // A share for every CU that streams: more of them end later where the last ones find no CU free
-      // (64 rows sharing 8,192 tokens, 192 such CUs: 192 shares 41.8 us, 256 49.7, 384 43, 512 49).
-      shape = stream_shape(st.cus, heads, st.page_size, 8);
-      shape.workgroups = std::max<int64_t>(1, (st.cus - gemm_wgs) / shape.grid_y);
-      shape.wg_capacity = st.cus / shape.grid_y + st.cus / 3 + 2;
-    }
-    // The streaming launch.
-    lens.clear();
-    items_cap = shape.wg_capacity;
-    int widest = 1;
-    for (const Source& src : stream) {
-      lens.push_back(src.end - src.begin);
-      items_cap += 1 + ceil_div(lens.back(), shape.max_item);
-      widest = std::max<int>(widest, src.tokens * static_cast<int>(group));
-    }
-    once = bytes >= int64_t(8) << 20;  // as the decode kernel's copies
-    st.sets = widest <= 16 ? 1 : 2;
-    work.resize(4 * items_cap);
-    merge.resize(2 * stream.size());
-    wg.resize(shape.wg_capacity + 1);
-    int64_t share = 0;
-    items = wgs = slot = 0;
-    if (!stream.empty()) {
-      items = schedule(lens.data(), static_cast<int64_t>(stream.size()), shape.workgroups,
-                       shape.max_item, kStreamTile, /*graph=*/true, work.data(), items_cap,
-                       merge.data(), &share, wg.data(), shape.wg_capacity, &wgs);
-      if (items < 0) {
-        set_error("shared prefix work list exceeds its capacity");
-        return false;
-      }
-    }
-    // Items of a source are consecutive: its slots follow each other.
-    std::vector<bool> joined(stream.size(), true);
-    for (int64_t r = 0; r < b.batch; ++r)
-      if (own_of[r].kind == 1 && prefix_of[r].kind == 0)
-        joined[own_of[r].index] = merge[2 * own_of[r].index + 1] > 1;
-    for (size_t i = 0; i < stream.size(); ++i) {
-      Source& src = stream[i];
-      src.splits = joined[i] ? merge[2 * i + 1] : 0;
-      src.slot = static_cast<int32_t>(slot);
-      slot += static_cast<int64_t>(src.splits) * src.tokens;
-    }
-    // The matrix products.
-    gemm_work.clear();
-    const int64_t stream_slots = slot;
-    if (!gemm.empty())
-      schedule_gemm(gemm, group, heads, columns,
-                    gemm_length(gemm, group, heads, columns, gemm_wgs, merge_tiles, cap).tiles, slot,
-                    gemm_work);
-    st.slices = shape.grid_y;
-    graph_shape = shape;
-    st.gemm_wgs = std::min(gemm_wgs, static_cast<int64_t>(gemm_work.size()) / kGemmInts);
-    if (!graph_rows) break;
-    // A graph plan has room for 64 MiB of partial outputs of the streaming launch, beside a slot an
-    // item: a batch that needs more (dozens of small groups) shares nothing.
-    const int64_t room = (int64_t(64) << 20) / (st.num_q_heads * kD * 4);
-    if (stream_slots <= room + items) break;
-    std::fill(eff.begin(), eff.end(), 0);
   }
+  // How the products and the copies share the chip. Whole CUs for either wherever there are both and
+  // eight kv heads (us a layer, in turn, in halves, on whole CUs: 256 rows sharing 8,192 tokens 141,
+  // 136, 117; 64 sharing 2,048 44, 38, 29; 75 rows of up to 16 new tokens in 8 groups 65, 63, 54);
+  // halves with four; in turn where the copies are next to nothing (48 rows of up to 40 new tokens
+  // 103, 141, 110).
+  int64_t cost4 = 0, cost8 = 0;  // tiles of 128 and of 256 columns
+  for (const Source& src : gemm) {
+    const int64_t tiles = ceil_div(src.end, kTileK) - src.begin / kTileK;
+    cost4 += ceil_div(src.tokens * group, 128) * tiles * heads;
+    cost8 += ceil_div(src.tokens * group, 256) * tiles * heads;
+  }
+  int64_t bytes = 0;
+  for (const Source& src : stream) bytes += int64_t(src.end - src.begin) * heads * kD * 4;
+  // A CU's tile of 256 columns while others stream, and the copies' rate on the whole chip.
+  constexpr double kTileUs = 1.68, kBytesPerUs = 5.86e6;
+  const double stream_us = static_cast<double>(bytes) / kBytesPerUs;
+  st.form = st.shape.waves == 4 && !stream.empty() ? Form::kHalves : Form::kInTurn;
+  if (heads % 8 == 0 && (graph_rows ? graph_rows * group > 128
+                                    : !gemm.empty() && stream_us > 1))
+    st.form = Form::kWhole;
+  else if (!graph_rows && !gemm.empty() && stream_us <= 1)
+    st.form = Form::kInTurn;
+  // Fixed for a graph plan, whose captured launch holds one of the two.
+  const bool filled = !graph_rows && st.form == Form::kInTurn && 4 * cost8 <= 3 * cost4;
+  st.nw = st.form == Form::kWhole || filled ? 8 : 4;
+  const int64_t columns = 32 * st.nw;
+  // Bounds on the products' items and partial outputs, beside one part a source: a graph plan's
+  // hold for whatever its rows will share.
+  const int64_t extra = graph_rows ? st.cus : 2 * st.cus, per = columns / group;  // tokens of an item
+  if (graph_rows) {
+    // at most rows / 2 groups share, each with a last tile that is not full
+    cap.items = (graph_rows / per + graph_rows / 2) * heads + extra;
+    cap.slots = graph_rows + extra * per / heads;
+  } else {
+    cap = count_gemm(gemm, group, heads, columns, std::numeric_limits<int32_t>::max());
+    cap.items += extra;
+    cap.slots += extra * per;
+  }
+  // A slot's partial outputs, written and read at about 5 TB/s.
+  const double merge_tiles = static_cast<double>(st.num_q_heads * 1056) / 5e6 / kTileUs;
+  StreamShape shape = st.shape;
+  int64_t gemm_wgs = st.form == Form::kHalves || st.nw == 8 ? st.cus : 2 * st.cus;
+  if (st.form == Form::kWhole) {
+    // As many CUs for the products as end the launch soonest. A CU streams no faster for others'
+    // not streaming: the copies take longer by the products' share.
+    double least = std::numeric_limits<double>::infinity();
+    gemm_wgs = 0;
+    for (int64_t wgs8 = std::max<int64_t>(1, st.cus / 16);
+         wgs8 <= st.cus - st.cus / 8 && !gemm.empty();
+         wgs8 += std::max<int64_t>({1, st.cus / 32, wgs8 / 8})) {
+      const double run =
+          kTileUs * gemm_length(gemm, group, heads, columns, wgs8, merge_tiles, cap).tile_times;
+      const double est =
+          std::max(run, stream_us * static_cast<double>(st.cus) / (st.cus - wgs8));
+      if (est < least) {
+        least = est;
+        gemm_wgs = wgs8;
+      }
+    }
+    // A share for every CU that streams: more of them end later where the last ones find no CU free
+    // (64 rows sharing 8,192 tokens, 192 such CUs: 192 shares 41.8 us, 256 49.7, 384 43, 512 49).
+    shape = stream_shape(st.cus, heads, st.page_size, 8);
+    shape.workgroups = std::max<int64_t>(1, (st.cus - gemm_wgs) / shape.grid_y);
+    shape.wg_capacity = st.cus / shape.grid_y + st.cus / 3 + 2;
+  }
+  // The streaming launch.
+  items_cap = shape.wg_capacity;
+  int widest = 1;
+  for (const Source& src : stream) {
+    lens.push_back(src.end - src.begin);
+    items_cap += 1 + ceil_div(lens.back(), shape.max_item);
+    widest = std::max<int>(widest, src.tokens * static_cast<int>(group));
+  }
+  once = bytes >= int64_t(8) << 20;  // as the decode kernel's copies
+  st.sets = widest <= 16 ? 1 : 2;
+  work.resize(4 * items_cap);
+  merge.resize(2 * stream.size());
+  wg.resize(shape.wg_capacity + 1);
+  int64_t share = 0;
+  items = wgs = slot = 0;
+  if (!stream.empty()) {
+    items = schedule(lens.data(), static_cast<int64_t>(stream.size()), shape.workgroups,
+                     shape.max_item, kStreamTile, /*graph=*/true, work.data(), items_cap,
+                     merge.data(), &share, wg.data(), shape.wg_capacity, &wgs);
+    if (items < 0) {
+      set_error("shared prefix work list exceeds its capacity");
+      return false;
+    }
+  }
+  // Items of a source are consecutive: its slots follow each other.
+  std::vector<bool> joined(stream.size(), true);
+  for (int64_t r = 0; r < b.batch; ++r)
+    if (own_of[r].kind == 1 && prefix_of[r].kind == 0)
+      joined[own_of[r].index] = merge[2 * own_of[r].index + 1] > 1;
+  for (size_t i = 0; i < stream.size(); ++i) {
+    Source& src = stream[i];
+    src.splits = joined[i] ? merge[2 * i + 1] : 0;
+    src.slot = static_cast<int32_t>(slot);
+    slot += static_cast<int64_t>(src.splits) * src.tokens;
+  }
+  // The matrix products.
+  if (!gemm.empty())
+    schedule_gemm(gemm, group, heads, columns,
+                  gemm_length(gemm, group, heads, columns, gemm_wgs, merge_tiles, cap).tiles, slot,
+                  gemm_work);
+  st.slices = shape.grid_y;
+  st.gemm_wgs = std::min(gemm_wgs, static_cast<int64_t>(gemm_work.size()) / kGemmInts);
   st.gemm_items = static_cast<int64_t>(gemm_work.size()) / kGemmInts;
 
   // Layout; a graph plan's does not depend on what is shared.
   const bool by_token = tokens == b.batch;
   int64_t stream_cap = items, wg_cap = wgs, gemm_cap = st.gemm_items, slot_cap = slot;
   if (graph_rows) {
-    // a workgroup's share, and each request's and prefix's own items and cuts
-    const int64_t most = graph_shape.wg_capacity +
-                         (graph_rows + graph_rows / 2) *
-                             (1 + ceil_div(graph_tokens, graph_shape.max_item));
-    stream_cap = most;
-    wg_cap = graph_shape.wg_capacity;
+    // A workgroup's share, and each request's and prefix's own items and cuts; a slot an item of a
+    // request, and as many as a streamed prefix has tokens an item of one.
+    const int64_t cuts = 1 + ceil_div(graph_tokens, shape.max_item);
+    stream_cap = shape.wg_capacity + (graph_rows + graph_rows / 2) * cuts;
+    wg_cap = shape.wg_capacity;
     gemm_cap = cap.items;
-    slot_cap = (int64_t(64) << 20) / (st.num_q_heads * kD * 4) + most + cap.slots;
+    slot_cap = stream_cap + cap.slots +
+               (shape.wg_capacity + graph_rows / 2 * cuts) *
+                   std::min<int64_t>(kStreamColumns / group, graph_rows);
   }
   const int64_t o_info = kHeaderInts;
   const int64_t o_row_of = o_info + kInfoInts * b.batch;
@@ -1210,7 +1197,9 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
       std::fill(host + o_row_of + b.q_start[r], host + o_row_of + b.q_start[r + 1],
                 static_cast<int32_t>(r));
   }
-  st.prefix_items = st.gemm_items;
+  st.prefix_items = 0;
+  for (size_t i = 0; i < gemm_work.size(); i += kGemmInts)
+    st.prefix_items += gemm_work[i + 8] == kNoHorizon;
   for (int64_t i = 0, part = 0; i < items; ++i) {
     const int32_t of = work[4 * i];
     part = i && work[4 * (i - 1)] == of ? part + 1 : 0;
@@ -1232,6 +1221,7 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
     hip_error(err, "shared prefix upload");
     return false;
   }
+  st.ready = true;
   st.batch = b.batch;
   st.tokens = tokens;
   st.by_token = by_token;
@@ -1298,6 +1288,7 @@ const char* SharedPlan::run(const int32_t* indices, const void* q, int64_t q_sn,
                             const void* k, const void* v, void* out, int64_t o_sn, int64_t o_sh,
                             hipStream_t s) const {
   const State& st = *st_;
+  if (!st.ready) return set_error("shared prefixes were not prepared");
   const int32_t* ints = static_cast<const int32_t*>(st.ints.ptr);
   SharedArgs a{};
   a.q = static_cast<const uint16_t*>(q);

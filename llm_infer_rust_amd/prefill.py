@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _native
-from ._native import check, dtype_code, last_error, lib, stream_of
+from ._native import check, dtype_code, last_error, lib, on_device, stream_of
 from .kv_cache import ModelError
 
 
@@ -89,14 +89,15 @@ def prepare_prefill_plan(existing: PrefillPlan | None, metadata, prefill, spec,
     args = (existing.handle if existing else None, cu.data_ptr(), table.data_ptr(), b,
             table.size(1), table.stride(0), qh, ph, spec.num_heads, spec.num_kv_heads, page_size,
             dt)
-    if metadata.shared_prefix is None:
-        handle = lib().mi355x_prefill_prepare(*args, stream_of(cu))
-    else:
-        from .backend import shared_arrays
-        group_rows, group_lens = shared_arrays(metadata.shared_prefix, b)
-        handle = lib().mi355x_prefill_prepare_shared(*args, group_rows.ctypes.data,
-                                                     group_lens.ctypes.data, group_rows.size,
-                                                     stream_of(cu))
+    with on_device(cu.device):
+        if metadata.shared_prefix is None:
+            handle = lib().mi355x_prefill_prepare(*args, stream_of(cu))
+        else:
+            from .backend import shared_arrays
+            group_rows, group_lens = shared_arrays(metadata.shared_prefix, b)
+            handle = lib().mi355x_prefill_prepare_shared(*args, group_rows.ctypes.data,
+                                                         group_lens.ctypes.data, group_rows.size,
+                                                         stream_of(cu))
     if not handle:
         raise ModelError(f"mi355x prefill plan failed: {last_error()}")
     plan = existing if existing is not None else PrefillPlan(handle)
@@ -133,9 +134,10 @@ def run_prefill(plan: PrefillPlan, q: torch.Tensor, k: torch.Tensor, v: torch.Te
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ModelError("invalid static prefill output")
-    check(lib().mi355x_prefill_run(
-        plan.handle, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k_sn, 128,
-        v.data_ptr(), v_sn, 128, out.data_ptr(), out.stride(0), out.stride(1), q.size(0),
-        q.size(1), hkv, plan.page_size, dtype_code(q), stream_of(q)), "mi355x prefill")
+    with on_device(q.device):
+        check(lib().mi355x_prefill_run(
+            plan.handle, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k_sn, 128,
+            v.data_ptr(), v_sn, 128, out.data_ptr(), out.stride(0), out.stride(1), q.size(0),
+            q.size(1), hkv, plan.page_size, dtype_code(q), stream_of(q)), "mi355x prefill")
     return out
 

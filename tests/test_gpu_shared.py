@@ -39,6 +39,8 @@ DECODE = [
     ([(20, 512)], 200, 16, 4, 128, BF16),
     ([(130, 256)], 20, 4, 2, 16, BF16),
     ([(65, 1500)], 33, 16, 16, 16, FP16),
+    ([(50, 300), (4, 200)], 33, 24, 12, 16, BF16),
+    ([(30, 300), (4, 200)], 33, 20, 5, 16, BF16),
     ([(256, 192)], 5, 32, 8, 16, BF16),
     ([(6, 300)] * 12, 64, 32, 4, 16, BF16),
 ]
@@ -198,18 +200,19 @@ def test_streams(gpu):
     b.check(got)
 
 
-@pytest.mark.parametrize("rows,heads", [(6, 32), (64, 32)])
-def test_graph(gpu, rows, heads):
+@pytest.mark.parametrize("rows,heads,kv_heads", [(6, 32, 8), (64, 32, 8), (64, 32, 4), (64, 8, 1),
+                                                 (40, 16, 2), (200, 8, 8), (64, 24, 12)])
+def test_graph(gpu, rows, heads, kv_heads):
     """One captured launch serves any groups, also none; replays are checked one by one."""
     cols = 80
     table = torch.zeros(rows, cols, dtype=torch.int32, device="cuda")
     lens = torch.ones(rows, dtype=torch.int32, device="cuda")
     kinds = [[(rows, 500)], [(1, 100)] * rows, [(rows // 2, 640), (rows - rows // 2, 64)],
-             [(2, 300)] * (rows // 2), [(rows, 0)], [(rows, 1000)]]
-    batches = [Batch(g, own_lengths(rows, 1, 60, seed=i), heads=heads, kv_heads=8, seed=i)
+             [(2, 300)] * (rows // 2), [(rows, 0)], [(rows - 2, 1000), (2, 100)]]
+    batches = [Batch(g, own_lengths(rows, 1, 60, seed=i), heads=heads, kv_heads=kv_heads, seed=i)
                for i, g in enumerate(kinds)]
     pages = max(b.k.size(0) for b in batches)
-    k, v = (torch.zeros(pages, 16, 8, 128, dtype=BF16, device="cuda") for _ in range(2))
+    k, v = (torch.zeros(pages, 16, kv_heads, 128, dtype=BF16, device="cuda") for _ in range(2))
     q = torch.zeros(rows, heads, 128, dtype=BF16, device="cuda")
     attention, cache = batches[0].attention(), batches[0].cache()
     cache.bind_kv_cache(k, v)
