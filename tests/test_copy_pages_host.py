@@ -1,11 +1,13 @@
 """What page copies refuse, without a GPU: the checks of the C entry (addresses are never
 dereferenced) and of the pool's method."""
 import ctypes
+from array import array
 
+import numpy as np
 import pytest
 import torch
 
-from llm_infer_rust_amd import _native
+from llm_infer_rust_amd import _native, kv_cache
 from llm_infer_rust_amd.kv_cache import KVCacheLayout, KVCachePool
 
 A = 0x10000
@@ -59,3 +61,16 @@ def test_method_refuses():
     pool = KVCachePool(KVCacheLayout(2, 4, 16, 2, 8), torch.bfloat16, "cpu")
     with pytest.raises(_native.NativeError):
         pool.copy_pages([1], [2])
+
+
+def test_host_ids():
+    want = [3, 0, 2 ** 31 - 1, -2 ** 31]
+    for values in (want, tuple(want), np.array(want), np.array(want, np.int32), torch.tensor(want),
+                   [np.int64(w) for w in want], array("q", want)):
+        assert list(kv_cache._host_ids(values)) == want
+    assert list(kv_cache._host_ids(range(5, 8))) == [5, 6, 7]
+    assert list(kv_cache._host_ids(np.arange(8)[::2])) == [0, 2, 4, 6]
+    for values in ([1.5], [[1]], [2 ** 31], [-2 ** 31 - 1], np.array([2 ** 31]), np.array([1.0]),
+                   np.array([[1]]), b"abcd", "1234", ["1"], [None]):
+        with pytest.raises(kv_cache.ModelError):
+            kv_cache._host_ids(values)
