@@ -280,16 +280,17 @@ def run_decode(plan: DecodePlan, q: torch.Tensor, k_cache: torch.Tensor, v_cache
     if q.dim() != 3 or q.stride(2) != 1 or not k_cache.is_contiguous() \
             or not v_cache.is_contiguous() or k_cache.dim() != 4:
         raise ModelError("mi355x decode requires [B,Hq,D] queries and contiguous caches")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out is None:  # 1.3 us; from shape, type and device 3.4
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
         raise ModelError("invalid decode output")
+    rows, heads, _ = q.shape
+    _, page_size, kv_heads, _ = k_cache.shape
     with on_device(q.device):
         check(lib().mi355x_decode_run(
-            plan.handle, q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
-            v_cache.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), q.size(0),
-            q.size(1), k_cache.size(2), k_cache.size(1), dtype_code(q), stream_of(q)),
-            "mi355x decode")
+            plan.handle, q.data_ptr(), *q.stride()[:2], k_cache.data_ptr(), v_cache.data_ptr(),
+            out.data_ptr(), *out.stride()[:2], rows, heads, kv_heads, page_size, dtype_code(q),
+            stream_of(q)), "mi355x decode")
     return out
 
 
@@ -494,5 +495,6 @@ def sm_scale(head_dim: int) -> float:
 __all__ = [
     "Attention", "AttentionBatch", "AttentionBackendKind", "AttentionMetadata", "AttentionSpec",
     "BatchPhase", "DecodeGraphState", "DecodeHostMetadata", "DecodePlan", "MetadataRequirements",
-    "ModelError", "NativeError", "PrefillMetadata", "SharedPrefix", "prepare_decode_plan", "run_decode",
+    "ModelError", "NativeError", "PrefillMetadata", "SharedPrefix", "prepare_decode_plan",
+    "run_decode",
 ]

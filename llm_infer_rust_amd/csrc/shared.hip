@@ -7,17 +7,21 @@
 //
 // A group's queries (every token's G heads under a kv head, heads fastest: tokens x G columns) meet
 // the prefix's keys as one matrix product, where plain decode reads the prefix once a request. Two
-// kernels, by the number of columns:
+// loops, by the number of columns:
 //
-// shared_stream_kernel, up to 32 columns: the decode kernel's copy pipeline (tiles of 16 whole K and
-// V rows through an LDS ring, one wave a kv head) with up to two sets of 16 columns on the tile a
-// wave has in LDS. Streaming a tile takes a CU longer than two sets of products on it, so it is
-// bound by memory, as decode is. The own keys of requests with few new tokens are items of the same
-// launch, under the same balanced schedule.
+// stream_items, up to 32 columns: the decode kernel's copy pipeline (tiles of 16 whole K and V rows
+// through an LDS ring, one wave a kv head) with up to two sets of 16 columns on the tile a wave has
+// in LDS. Streaming a tile takes a CU longer than two sets of products on it, so it is bound by
+// memory, as decode is. The own keys of requests with few new tokens are items too, under the same
+// balanced schedule.
 //
-// shared_gemm_kernel, more: 32 columns a wave against a range of 64-key tiles, as the prefill kernel
+// gemm_items, more: 32 columns a wave against a range of 64-key tiles, as the prefill kernel
 // (S^T = K Q^T, P^T = 2^(S^T - m), O^T += V^T P^T on 32 x 32 x 16 products), K and V read once for
 // 256 columns. Own keys of requests with many new tokens go there too, under a horizon a column.
+//
+// One is bound by memory and the other by the matrix cores, so one launch holds both where the number
+// of kv heads lets it: shared_wide_kernel on whole CUs for either, shared_kernel on halves of a CU.
+// shared_gemm_kernel and shared_stream_kernel follow each other elsewhere.
 //
 // Every part that is joined writes fp32 outputs and their log2-sum-exp; shared_merge_kernel joins
 // them. A request that shares nothing and whose keys one item holds is written directly.

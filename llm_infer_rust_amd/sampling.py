@@ -321,4 +321,5 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     return out
 
 
-__all__ = ["TokenLogprobs", "TokenDetail", "PendingLogprobs", "token_logprobs", "SamplingParams", "Sampler", "PendingSample", "SamplingError"]
+__all__ = ["MAX_TOP_LOGPROBS", "PendingLogprobs", "PendingSample", "Sampler", "SamplingError",
+           "SamplingParams", "TokenDetail", "TokenLogprobs", "token_logprobs"]
