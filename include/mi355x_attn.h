@@ -520,7 +520,8 @@ int64_t mi355x_sample_workspace_bytes(int64_t rows, int64_t vocab, bool top_p_ro
  * +inf) or a +inf, and one of only -inf, gets NaN for every probability and its entropy. Sums are
  * fp32. Few rows are spread over several workgroups each: their parts go to `workspace` (16-byte
  * aligned, mi355x_token_logprobs_workspace_bytes for the same sizes and compute units; calls that
- * overlap need workspaces of their own). No reference counterpart. */
+ * overlap need workspaces of their own). At most 2^24 - 1 rows of more than 8,192 logits or 2^26 - 1
+ * shorter ones a call. No reference counterpart. */
 const char* mi355x_token_logprobs(const void* logits, int64_t rows, int64_t vocab,
                                   int64_t row_stride, int dtype, const int64_t* tokens,
                                   int64_t top, void* logprobs, void* entropy, int64_t* top_ids,

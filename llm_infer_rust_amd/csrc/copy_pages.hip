@@ -55,13 +55,15 @@ struct Pool {
   int64_t planes, plane_pages, page_tokens, token_bytes;
 };
 
+// Workgroups that copy some tokens of a page.
+int64_t parts_of(const Pool& p, int64_t tokens, int64_t word) {
+  return (tokens * p.token_bytes / word + kThreads - 1) / kThreads;
+}
+
 // `most`: the longest copy's tokens.
 template <typename Word, typename Batch>
 const char* launch(const Pool& p, const Batch& batch, int pairs, int64_t most, hipStream_t s) {
-  const int64_t words = most * p.token_bytes / static_cast<int64_t>(sizeof(Word));
-  const int64_t parts = (words + kThreads - 1) / kThreads;
-  if (parts > (int64_t(1) << 31) / kThreads)
-    return set_error("mi355x_copy_pages: page too large");
+  const int64_t parts = parts_of(p, most, sizeof(Word));
   const dim3 grid(static_cast<uint32_t>(parts), static_cast<uint32_t>(pairs),
                   static_cast<uint32_t>(p.planes));
   copy_pages_kernel<Word><<<grid, dim3(kThreads), 0, s>>>(
@@ -69,11 +71,16 @@ const char* launch(const Pool& p, const Batch& batch, int pairs, int64_t most, h
   return launch_status("mi355x_copy_pages");
 }
 
-// Launches of about equal size for all pairs.
+// Launches of about equal size for all pairs, each of fewer than 2^32 threads (a grid of more would be
+// cut short without an error).
 template <typename Batch>
 const char* copy_all(const Pool& p, const int32_t* src, const int32_t* dst, const int32_t* tokens,
                      int64_t pairs, bool wide, hipStream_t s) {
-  const int64_t launches = (pairs + Batch::kPairs - 1) / Batch::kPairs;
+  const int64_t pair_threads =
+      parts_of(p, p.page_tokens, wide ? sizeof(uint4) : sizeof(uint16_t)) * kThreads * p.planes;
+  const int64_t room = std::min<int64_t>(Batch::kPairs, ((int64_t(1) << 32) - 1) / pair_threads);
+  if (room == 0) return set_error("mi355x_copy_pages: page too large");
+  const int64_t launches = (pairs + room - 1) / room;
   Batch batch;
   for (int64_t l = 0; l < launches; ++l) {
     int n = 0;

@@ -640,14 +640,16 @@ Split split_of(int64_t rows, int64_t vocab, int64_t cus) {
   return {(vocab + length - 1) / length, length};
 }
 
+int threads_of(const Split& sp) {
+  return sp.length <= kNarrowVocab && sp.segments == 1 ? kNarrow : kWide;
+}
+
 template <int DT>
-void launch(LogprobArgs a, int64_t rows, hipStream_t s) {
-  const bool narrow = a.segment <= kNarrowVocab && a.segments == 1;
-  const int threads = narrow ? kNarrow : kWide;
+void launch(LogprobArgs a, int64_t rows, int threads, hipStream_t s) {
   const int64_t steps = (a.segment + kGroup * threads - 1) / (kGroup * threads);
   const uint32_t lds = a.top ? static_cast<uint32_t>(steps * threads * sizeof(float)) : 0;
   const dim3 grid(static_cast<uint32_t>(rows * a.segments)), block(threads);
-  if (narrow) {
+  if (threads == kNarrow) {
     if (a.top) logprob_kernel<DT, kNarrow, true><<<grid, block, lds, s>>>(a);
     else logprob_kernel<DT, kNarrow, false><<<grid, block, lds, s>>>(a);
   } else {
@@ -689,8 +691,9 @@ extern "C" const char* mi355x_token_logprobs(const void* logits, int64_t rows, i
   if (!aligned(logits, dtype == 2 ? 4 : 2) || (rows > 1 && row_stride < vocab))
     return set_error("mi355x_token_logprobs: rows must not overlap");
   const Split sp = split_of(rows, vocab, cus);
-  if (rows * sp.segments >= int64_t(1) << 31)
-    return set_error("mi355x_token_logprobs: launch too large");
+  // A grid of 2^32 threads or more would be cut short without an error.
+  if (rows * sp.segments * threads_of(sp) >= int64_t(1) << 32)
+    return set_error("mi355x_token_logprobs: too many rows for a launch");
   LogprobArgs a{};
   if (sp.segments > 1) {
     if (!workspace || !aligned(workspace, 16) ||
@@ -711,8 +714,9 @@ extern "C" const char* mi355x_token_logprobs(const void* logits, int64_t rows, i
   a.segments = static_cast<int32_t>(sp.segments);
   a.segment = sp.length;
   auto s = static_cast<hipStream_t>(stream);
-  if (dtype == 0) launch<0>(a, rows, s);
-  else if (dtype == 1) launch<1>(a, rows, s);
-  else launch<2>(a, rows, s);
+  const int threads = threads_of(sp);
+  if (dtype == 0) launch<0>(a, rows, threads, s);
+  else if (dtype == 1) launch<1>(a, rows, threads, s);
+  else launch<2>(a, rows, threads, s);
   return launch_status("mi355x_token_logprobs");
 }

@@ -978,6 +978,8 @@ bool SharedPlan::pays(const SharedBatch& b) const {
   const std::vector<int32_t> eff = st_->lengths(b);
   int64_t saved = 0;
   bool any = false;
+  // The merge takes 32 threads a row of a q head, and a grid of 2^32 would be cut short.
+  if (int64_t(b.q_start[b.batch]) * st_->num_q_heads >= int64_t(1) << 26) return false;
   for (int64_t g = 0; g < b.groups; ++g) {
     saved += int64_t(b.group_rows[g] - 1) * eff[g] * st_->num_kv_heads * kD * 4;
     any |= eff[g] > 0;

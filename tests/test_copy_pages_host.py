@@ -39,6 +39,7 @@ def copy(src, dst, tokens=None, planes=2, pages=8, page_tokens=16, token_bytes=2
     (dict(src=[1], dst=[2], page_tokens=0), b"geometry"),
     (dict(src=[1], dst=[2], token_bytes=3), b"geometry"),
     (dict(src=[1], dst=[2], pairs=-1), b"geometry"),
+    (dict(src=[1], dst=[2], planes=65535, page_tokens=1 << 20, token_bytes=2), b"page too large"),
     (dict(src=[1], dst=[2], pool=None), b"null"),
     (dict(src=[1], dst=[2], pool=0x10001), b"misaligned"),
 ])
