@@ -32,7 +32,7 @@ struct PartialBatch {
 };
 
 // Grid: {parts of a page, pairs, planes}; a thread copies a word. us, one word a thread against four
-// loaded together: 255 copies of 14 tokens of few sources in 56 planes 62 and 94 (the sources come
+// loaded together: 255 copies of 9 tokens of few sources in 56 planes 62 and 94 (the sources come
 // from the caches), 400 pages of 64 tokens in 8 planes 139 and 158 (6.0 TB/s read and written).
 template <typename Word, typename Batch>
 __global__ __launch_bounds__(kThreads) void copy_pages_kernel(uint8_t* pool, int64_t plane_bytes,
