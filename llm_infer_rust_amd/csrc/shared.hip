@@ -1036,6 +1036,24 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
       gemm.push_back(own);
     }
   }
+  int64_t bytes = 0;
+  for (const Source& src : stream) bytes += int64_t(src.end - src.begin) * heads * kD * 4;
+  // A CU's tile of 256 columns while others stream, and the copies' rate on the whole chip.
+  constexpr double kTileUs = 1.68, kBytesPerUs = 5.86e6;
+  double stream_us = static_cast<double>(bytes) / kBytesPerUs;
+  // A few requests with little of their own take products too: not half a CU's worth of items and no
+  // launch that would wait for the others' (48 rows of up to 40 new tokens behind 4,096, two layers 226
+  // us, 213; 20 of up to 100 211, 198; 30 of up to 14, where the items are at this bound, 84.4, 85.2).
+  if (!graph_rows && !gemm.empty() && stream_us <= 1 &&
+      2 * static_cast<int64_t>(stream.size()) * heads <= st.cus) {
+    for (std::vector<Of>* ofs : {&prefix_of, &own_of})
+      for (Of& of : *ofs)
+        if (of.kind == 1) of = {2, of.index + static_cast<int32_t>(gemm.size())};
+    gemm.insert(gemm.end(), stream.begin(), stream.end());
+    stream.clear();
+    bytes = 0;
+    stream_us = 0;
+  }
   // How the products and the copies share the chip. Whole CUs for either wherever there are both and
   // eight kv heads (us a layer, in turn, in halves, on whole CUs: 256 rows sharing 8,192 tokens 141,
   // 136, 117; 64 sharing 2,048 44, 38, 29; 75 rows of up to 16 new tokens in 8 groups 65, 63, 54);
@@ -1047,11 +1065,6 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
     cost4 += ceil_div(src.tokens * group, 128) * tiles * heads;
     cost8 += ceil_div(src.tokens * group, 256) * tiles * heads;
   }
-  int64_t bytes = 0;
-  for (const Source& src : stream) bytes += int64_t(src.end - src.begin) * heads * kD * 4;
-  // A CU's tile of 256 columns while others stream, and the copies' rate on the whole chip.
-  constexpr double kTileUs = 1.68, kBytesPerUs = 5.86e6;
-  const double stream_us = static_cast<double>(bytes) / kBytesPerUs;
   st.form = st.shape.waves == 4 && !stream.empty() ? Form::kHalves : Form::kInTurn;
   if (heads % 8 == 0 && (graph_rows ? graph_rows * group > 128
                                     : !gemm.empty() && stream_us > 1))
