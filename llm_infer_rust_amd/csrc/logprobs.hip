@@ -34,10 +34,12 @@ constexpr int kMaxTop = 64;            // one lane an alternative
 constexpr int kGroup = 32;             // logits under one maximum in LDS
 constexpr int kCandidates = 1024;      // (key, index) entries in LDS
 constexpr int kListed = 128;           // groups that a wave lists before it reads them ...
+constexpr int kLook = 4;               // maxima that a thread looks at together
 constexpr int kReads = 4;              // ... two at a time in each of so many loads
 // Threads of a workgroup, for long rows and short ones. us, 256 threads a long row against 512 and 128:
-// 4,096 rows of 151,936 bf16 logits with 5 alternatives 230 (5.4 TB/s), 239, 268, without 216 (5.8
-// TB/s), 219, 229; 256 rows with 20 alternatives 27.0, 30.2, 42.8, without 16.7, 23, 27. Bound by memory
+// 4,096 rows of 151,936 bf16 logits with 5 alternatives 230, 239, 268 (now 228 at 256, 5.45 TB/s),
+// without 216 (5.8 TB/s), 219, 229; 256 rows with 20 alternatives 27.0, 30.2, 42.8 (now 23.5), without
+// 16.7, 23, 27. Bound by memory
 // and, nearly as much, by the dozen vector operations a logit. Registers are not capped for another
 // workgroup a CU: at 80 they spill (414 us).
 constexpr int kWide = 256, kNarrow = 64;
@@ -544,7 +546,7 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a) {
       } else {
         // Groups in reach are listed, then read some at a time: read where they are found, each read
         // waits for the one before it (256 rows of 151,936 logits with 20 alternatives 25.9 us, listed
-        // 24.0; 4,096 rows with 5 231 and 228.7).
+        // 24.0, with some maxima looked at together 23.5; 4,096 rows with 5 231, 229 and 228.3).
         uint16_t* list = sh.groups[wave];
         int listed = 0;
         auto read_listed = [&] {
@@ -566,15 +568,22 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a) {
           }
           listed = 0;
         };
-        for (int step = 0; step < steps; ++step) {
-          const float gm = group_max[step * THREADS + tid];
-          const bool in_row = step * VPT * THREADS + tid < all_vecs;
-          const uint64_t hits = __ballot(in_row && order_key(gm) >> R::kKeyShift >= bound);
-          if (hits >> lane & 1)
-            list[listed + __popcll(hits & ((uint64_t(1) << lane) - 1))] =
-                static_cast<uint16_t>(step * THREADS + tid);
-          listed += __popcll(hits);
-          if (listed > kListed - kWave) read_listed();
+        for (int step = 0; step < steps; step += kLook) {
+          float gm[kLook];
+#pragma unroll
+          for (int j = 0; j < kLook; ++j)
+            gm[j] = group_max[min(step + j, steps - 1) * THREADS + tid];
+#pragma unroll
+          for (int j = 0; j < kLook; ++j) {
+            const int at = (step + j) * THREADS + tid;
+            const bool in_row = step + j < steps && (step + j) * VPT * THREADS + tid < all_vecs;
+            const uint64_t hits = __ballot(in_row && order_key(gm[j]) >> R::kKeyShift >= bound);
+            if (hits == 0) continue;
+            if (hits >> lane & 1)
+              list[listed + __popcll(hits & ((uint64_t(1) << lane) - 1))] = static_cast<uint16_t>(at);
+            listed += __popcll(hits);
+            if (listed > kListed - kWave) read_listed();
+          }
         }
         read_listed();
       }
