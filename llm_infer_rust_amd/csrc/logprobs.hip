@@ -39,9 +39,8 @@ constexpr int kReads = 4;              // ... two at a time in each of so many l
 // Threads of a workgroup, for long rows and short ones. us, 256 threads a long row against 512 and 128:
 // 4,096 rows of 151,936 bf16 logits with 5 alternatives 230, 239, 268 (now 228 at 256, 5.45 TB/s),
 // without 216 (5.8 TB/s), 219, 229; 256 rows with 20 alternatives 27.0, 30.2, 42.8 (now 23.5), without
-// 16.7, 23, 27. Bound by memory
-// and, nearly as much, by the dozen vector operations a logit. Registers are not capped for another
-// workgroup a CU: at 80 they spill (414 us).
+// 16.7, 23, 27. Bound by memory and, nearly as much, by the dozen vector operations a logit. Registers
+// are not capped for another workgroup a CU: at 80 they spill (414 us).
 constexpr int kWide = 256, kNarrow = 64;
 // Rows up to this go to single waves, which have no barriers to wait at (4,096 rows of 8,000 logits:
 // 22 us, with four waves a row 40).
