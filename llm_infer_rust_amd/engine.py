@@ -203,7 +203,7 @@ class _Ahead:
     graph: _DecodeGraph
     host: np.ndarray
     lens: np.ndarray
-    shared: SharedPrefix | None
+    shared: SharedPrefix | None = None
 
     def same_rows(self, rows: list) -> bool:
         """Staged for exactly these rows, in this order (none of them ends by length)."""
@@ -616,7 +616,7 @@ class Engine:
         return host, lens
 
     def _launch_replay(self, g: _DecodeGraph, host: np.ndarray, lens: np.ndarray,
-                       shared: SharedPrefix | None) -> None:
+                       shared: SharedPrefix | None = None) -> None:
         """One copy into the graph's inputs, the host-length re-plan, the replay."""
         self._send(host.size, g.block)
         g.state.prepare_replay(DecodeHostMetadata(lens), shared)
