@@ -1565,10 +1565,11 @@ static void* prepare_decode(void* existing, const int32_t* block_table, int64_t 
     int32_t* indptr = host + layout.o_indptr;
     std::copy(first_page.begin(), first_page.end(), indptr);
     int64_t chunk = 0, wgs = 0;
-    const int64_t items = shared_runs ? 0 : schedule(plan->host_lengths.data(), batch, shape.workgroups,
-                                   shape.max_item, shape.tile, graph, host + layout.o_work,
-                                   items_cap, host + layout.o_merge, &chunk, host + layout.o_wg,
-                                   wg_cap, &wgs);
+    const int64_t items =
+        shared_runs ? 0
+                    : schedule(plan->host_lengths.data(), batch, shape.workgroups, shape.max_item,
+                               shape.tile, graph, host + layout.o_work, items_cap,
+                               host + layout.o_merge, &chunk, host + layout.o_wg, wg_cap, &wgs);
     if (items < 0) {
       set_error("decode work list exceeds its capacity");
       return nullptr;
