@@ -41,7 +41,7 @@ namespace {
 constexpr int kD = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int32_t kNoHorizon = 1 << 30;  // queries that see every key of their range
-constexpr int64_t kMaxKeys = int64_t(1) << 22;
+constexpr int64_t kMaxKeys = int64_t(1) << 22;  // of the products: div_small is exact below this
 
 // --- device workspace, int32
 constexpr int kHeaderInts = 4;
@@ -1045,7 +1045,9 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
   // launch that would wait for the others' (48 rows of up to 40 new tokens behind 4,096, two layers 226
   // us, 213; 20 of up to 100 211, 198; 30 of up to 14, where the items are at this bound, 84.4, 85.2).
   if (!graph_rows && !gemm.empty() && stream_us <= 1 &&
-      2 * static_cast<int64_t>(stream.size()) * heads <= st.cus) {
+      2 * static_cast<int64_t>(stream.size()) * heads <= st.cus &&
+      std::none_of(stream.begin(), stream.end(),
+                   [](const Source& src) { return src.end > kMaxKeys; })) {
     for (std::vector<Of>* ofs : {&prefix_of, &own_of})
       for (Of& of : *ofs)
         if (of.kind == 1) of = {2, of.index + static_cast<int32_t>(gemm.size())};

@@ -1,5 +1,7 @@
 """Several completions of one prompt through the engine: prefilled once, forked, their prompt's
 attention computed once where asked for, log probabilities with every token."""
+from dataclasses import replace
+
 import numpy as np
 import pytest
 import torch
@@ -127,3 +129,19 @@ def test_greedy_completions_agree(gpu):
     reqs = eng.add_request(np.arange(90), SamplingParams(n=4, max_tokens=20)).completions
     eng.run_until_complete()
     assert len({tuple(r.output) for r in reqs}) == 1
+
+
+def test_many_completions_in_one_graph(gpu, monkeypatch):
+    """Enough rows and heads for a decode graph whose products and copies each have whole CUs."""
+    monkeypatch.setenv("MI355X_SHARED_FROM", "0")
+    cfg = replace(TINY, num_attention_heads=32, num_kv_heads=8)
+    model, oracle = build(cfg, 7, gpu)
+    eng = engine(model, max_running_req=64, graph_batch_sizes=(64,), share_prefixes=True)
+    rng = np.random.default_rng(3)
+    reqs = [r for n, count in ((150, 36), (70, 20))
+            for r in eng.add_request(rng.integers(0, cfg.vocab_size, n), SamplingParams(
+                temperature=1.0, n=count, max_tokens=4, logprobs=2)).completions]
+    eng.run_until_complete()
+    assert eng.stats["forks"] == 54 and eng.stats["graph_steps"] > 0
+    assert len(eng.pages.free) == eng.pool.layout.num_pages
+    check_rows(eng, oracle, reqs, cfg.vocab_size)
