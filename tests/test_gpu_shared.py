@@ -136,6 +136,41 @@ def test_sharp_scores(gpu):
             assert bool(((got.double() - want).abs() <= limit).all())
 
 
+def ascending(rows=40, keys=4096, heads=32, kv_heads=8, dtype=BF16):
+    """Queries along the first axis and one key in 64 that they like, each a little more than the one
+    before; only the last of them has a value. Its weight is the largest there is, and the output is
+    that weight times the value, whatever the others' weights are rounded to."""
+    b = Batch([(rows, keys)], [1] * rows, None, heads, kv_heads, 16, dtype)
+    g = torch.Generator().manual_seed(1)
+    b.q.zero_()
+    b.q[:, :, 0] = (8 + 40 * torch.rand(rows, heads, generator=g)).to(dtype).cuda()
+    k, v = b.k.view(-1, kv_heads, 128), b.v.view(-1, kv_heads, 128)
+    k.zero_()
+    k[:, :, 0] = -64
+    last = v[b.slots[0][keys - 7]].clone()
+    v.zero_()
+    for i in range(keys // 64):
+        k[b.slots[0][64 * i + 57], :, 0] = i / 8
+    v[b.slots[0][keys - 7]] = last
+    return b
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_the_largest_weight_is_exact(gpu, dtype):
+    """Decode rows keep the largest probability at 1, with shared prefixes too: the output is rounded
+    once (half a step). Beside that, the sum's fp32 weights: scores of up to 2^7 in log2 units and
+    their references are off by 2^-24 of that each, and the weights by ln 2 times both: 2e-5."""
+    b = ascending(dtype=dtype)
+    want, _ = b.reference()
+    limit = (torch.finfo(dtype).eps / 2 + 2e-5) * want.abs() + 1e-7
+    for meta in (b.decode_meta(shared=False), b.decode_meta()):
+        got, info = b.run(meta)
+        print(f"[shared] {info}", flush=True)
+        worst = float(((got.double() - want).abs() / limit).max())
+        assert worst <= 1.0, worst
+    assert info["products"] and info["items"] <= 8 * 64 // 2  # parts of two tiles and more
+
+
 def test_nan_of_one_row_stays_there(gpu):
     """A NaN among a row's own keys reaches that row only; one in the prefix all of its group."""
     b = Batch([(4, 256), (3, 128)], [20] * 7, heads=16, kv_heads=8)
