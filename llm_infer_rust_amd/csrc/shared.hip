@@ -506,9 +506,10 @@ __device__ __forceinline__ void gemm_items(const SharedArgs& a, uint8_t* lds, in
         mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * c;
       }
       // The reference moves on the first tile and then when a row's maximum passes it by more than
-      // the slack. A first tile wholly past a row's horizon leaves it at 0.
+      // the slack. A first tile without a finite score (past a row's horizon, or all -inf) leaves it
+      // below every other, so that later scores count however far below 0 they are.
       if (first || __any(mx > ref + a.slack)) {
-        const float to = first ? (mx == -INFINITY ? 0.f : mx) : fmaxf(ref, mx);
+        const float to = fmaxf(first ? -1e30f : ref, mx);
         // nothing is accumulated before the first tile
         const float alpha = first ? 1.f : __builtin_amdgcn_exp2f(ref - to);
         ref = to;

@@ -171,6 +171,21 @@ def test_the_largest_weight_is_exact(gpu, dtype):
     assert info["products"] and info["items"] <= 8 * 64 // 2  # parts of two tiles and more
 
 
+def test_a_first_tile_without_weight(gpu):
+    """Scores of -inf in the first tiles, and all others far below 0: what has weight there counts."""
+    b = ascending(keys=2048)
+    k = b.k.view(-1, 8, 128)
+    for slots in b.slots:
+        k[slots, :, 0] = -64  # from -65 to -391 in log2 units
+        k[slots[-1], :, 0] = -66
+    for tile in range(0, 32, 2):  # the first tile of every part of an even number of them
+        k[b.slots[0][64 * tile:64 * tile + 64], :, 0] = -float("inf")
+    b.v.copy_(torch.randn(b.v.shape, generator=torch.Generator().manual_seed(2)).to(BF16).cuda())
+    got, info = b.run(b.decode_meta())
+    assert info["products"]
+    b.check(got)
+
+
 def test_nan_of_one_row_stays_there(gpu):
     """A NaN among a row's own keys reaches that row only; one in the prefix all of its group."""
     b = Batch([(4, 256), (3, 128)], [20] * 7, heads=16, kv_heads=8)
