@@ -242,6 +242,7 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, con
   // v_log_f32 (log2); s >= 1 or 0, NaN for rows with a NaN or +inf. A row of only -inf: s = 0.
   const float bits = __builtin_amdgcn_logf(st.s);
   auto lp = [&](float v) {
+    if (bits != bits) return bits;  // of joined parts only s shows a NaN: the largest m is a number
     if (!near(st.m)) return (v - st.m) - bits * kLn2;
     if (fabsf(v) >= kOverflow) return v - st.m;  // log2 s is far below its rounding
     return (fmaf(v, kLog2e, -(st.m * kLog2e)) - bits) * kLn2;

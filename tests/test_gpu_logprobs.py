@@ -131,6 +131,21 @@ def test_strides_and_alignment(gpu, dtype):
     check(base[:, :2000][::2], torch.arange(20, device=gpu), 3)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(2, 40000), (1, 151936), (600, 9000)])
+def test_a_nan_beside_masked_logits(gpu, dtype, rows, vocab):
+    """One NaN makes every probability of its row NaN, those of masked tokens too, in any split of
+    the row."""
+    lowest = torch.finfo(dtype).min
+    for masked in (-INF, lowest):
+        x, _ = make(rows, vocab, dtype, seed=8)
+        x[:, ::3] = masked
+        x[:, vocab // 2 + 1 - (vocab // 2) % 3] = float("nan")
+        for token in (0, 1, vocab // 3 * 3 - 3):
+            got = check(x, torch.full((rows,), token, device=gpu), 4)
+            assert bool(got.logprobs.isnan().all()) and bool(got.top_logprobs.isnan().all())
+
+
 def test_rows_do_not_depend_on_their_number(gpu):
     """The alternatives of a row are the same in any batch; its sums as far as rounding goes."""
     x, tokens = make(700, 30000, torch.bfloat16, seed=9)
