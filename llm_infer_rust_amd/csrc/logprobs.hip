@@ -178,13 +178,20 @@ struct Stats {
   float m, s, w;
 };
 
-// log2(e) times the reference as the sums were formed with it: rounded, or exact for a far one.
+// log2(e) times a reference as the sums are formed with it: rounded. Contracted into a difference it
+// would not be, and parts whose references differ would be joined with weights that are off by its
+// rounding (2^-4 at logits of a million).
+__device__ __forceinline__ float in_log2(float m) {
+#pragma clang fp contract(off)
+  return m * kLog2e;
+}
 __device__ __forceinline__ bool near(float m) { return fabsf(m) < kFarRef; }
-__device__ __forceinline__ float ref_step(float a, float b) {  // a's less b's
+// What a's sums are relative to, less what b's are. A far reference is an exact one.
+__device__ __forceinline__ float ref_step(float a, float b) {
   if (a == b) return 0.f;
-  if (near(a) && near(b)) return a * kLog2e - b * kLog2e;
-  if (near(b)) return fmaf(a, kLog2e, -(b * kLog2e));
-  if (near(a)) return -fmaf(b, kLog2e, -(a * kLog2e));
+  if (near(a) && near(b)) return in_log2(a) - in_log2(b);
+  if (near(b)) return fmaf(a, kLog2e, -in_log2(b));
+  if (near(a)) return -fmaf(b, kLog2e, -in_log2(a));
   return (a - b) * kLog2e;
 }
 __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
@@ -245,7 +252,7 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, con
     if (bits != bits) return bits;  // of joined parts only s shows a NaN: the largest m is a number
     if (!near(st.m)) return (v - st.m) - bits * kLn2;
     if (fabsf(v) >= kOverflow) return v - st.m;  // log2 s is far below its rounding
-    return (fmaf(v, kLog2e, -(st.m * kLog2e)) - bits) * kLn2;
+    return (fmaf(v, kLog2e, -in_log2(st.m)) - bits) * kLn2;
   };
   if (lane == 0) {
     a.lp[row] = lp(given);
@@ -438,7 +445,7 @@ __global__ __launch_bounds__(THREADS) void logprob_kernel(LogprobArgs a) {
     }
     if constexpr (TOP) group_max[step * THREADS + tid] = top;
     if (top > m) {
-      const float to = top * kLog2e;
+      const float to = in_log2(top);
       const float d = fmaxf(ref - to, kFarStep);
       const float c = s == 0.f ? 0.f : __builtin_amdgcn_exp2f(d);
       w = fmaf(d, s, w) * c;

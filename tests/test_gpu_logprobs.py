@@ -146,6 +146,16 @@ def test_a_nan_beside_masked_logits(gpu, dtype, rows, vocab):
             assert bool(got.logprobs.isnan().all()) and bool(got.top_logprobs.isnan().all())
 
 
+@pytest.mark.parametrize("rows,vocab", [(2, 40000), (1, 151936), (600, 9000), (700, 5000)])
+@pytest.mark.parametrize("offset", [3e3, 6e4, 9e5, 1e6, -9e5])
+def test_rows_far_from_zero(gpu, rows, vocab, offset):
+    """fp32 logits some units apart around a far offset: only their differences count."""
+    x, tokens = make(rows, vocab, torch.float32, seed=rows, scale=4.0)
+    check(x + offset, tokens, 5)
+    ramp = torch.linspace(-20, 20, vocab, device=gpu)  # every thread's reference moves all along
+    check((ramp + offset).expand(rows, vocab).contiguous(), tokens, 5)
+
+
 def test_rows_do_not_depend_on_their_number(gpu):
     """The alternatives of a row are the same in any batch; its sums as far as rounding goes."""
     x, tokens = make(700, 30000, torch.bfloat16, seed=9)
