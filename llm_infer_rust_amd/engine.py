@@ -86,6 +86,7 @@ class Request:
     # the others are forked from it. One alone: a list of itself.
     completions: list["Request"] = field(default_factory=list, repr=False)
     details: list[TokenDetail] = field(default_factory=list)  # with params.logprobs, one a token
+    fork_pages: list[int] = field(default_factory=list)  # the others' copies of the last page
 
     @property
     def slots(self) -> int:
@@ -274,10 +275,11 @@ class Engine:
 
     def _fork(self, leader: Request) -> list[Request]:
         """The other completions of a prefilled prompt join the running requests right behind it.
-        Its whole pages get more holders; the page it ends in is copied for each."""
+        Its whole pages get more holders; the page it ends in is copied for each, to the pages that
+        ``_reserve_fork`` took."""
         others = leader.completions[1:]
         whole, rest = divmod(leader.prompt.size, self.page_size)
-        own = self.pages.alloc(len(others)) if rest else []
+        own, leader.fork_pages = leader.fork_pages, []
         at = self.running.index(leader)
         self.running[at + 1:at + 1] = others
         for i, req in enumerate(others):
@@ -289,6 +291,14 @@ class Engine:
             self.pool.copy_pages([leader.pages[whole]] * len(others), own, [rest] * len(others))
         self.stats["forks"] += len(others)
         return others
+
+    def _reserve_fork(self, leader: Request) -> None:
+        """Pages for the copies of the page that the prompt ends in. Taken before the batch that ends
+        the prompt runs: a fork cannot fail after cursors have moved, and a batch without enough pages
+        is tried again as it was, with what it already took."""
+        copies = len(leader.completions) - 1 if leader.prompt.size % self.page_size else 0
+        if copies > len(leader.fork_pages):
+            leader.fork_pages.extend(self.pages.alloc(copies - len(leader.fork_pages)))
 
     def _shared(self, rows: list[Request], batch: int | None = None) -> SharedPrefix | None:
         """Neighbouring rows that are completions of one prompt, for the attention plan; ``batch``
@@ -385,6 +395,8 @@ class Engine:
                 self.waiting.remove(req)
                 self.running.append(req)
             self._ensure_pages(req, req.cursor + take)
+            if req.cursor + take == req.prompt.size:
+                self._reserve_fork(req)
             rows.append(BatchRequest(req.prompt, req.cursor, req.cursor + take, req.pages))
         b = self.batches.prepare_prefill(rows)
         # Logits only for requests whose prompt ends in this batch (possibly none).
