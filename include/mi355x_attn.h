@@ -112,7 +112,8 @@ void* mi355x_decode_prepare(void* existing, const int32_t* block_table, int64_t 
  * tokens have the same K and V, in the same pages or in copies. Attention over those is computed
  * once for the group, from the pages of its first row, and joined with every row's own; the result
  * is that of mi355x_decode_prepare up to rounding. Shared lengths are used in whole 64-token tiles
- * that leave each row a token, and only where that pays (mi355x_decode_plan_shared_info says).
+ * that leave each row a token, and only where that pays and its partial outputs have room
+ * (mi355x_decode_plan_shared_info says; otherwise the plan is that of mi355x_decode_prepare).
  * A graph plan takes groups on a re-plan if it was created with some (their sizes and lengths may
  * change, also to 0); otherwise they are checked and not used. */
 void* mi355x_decode_prepare_shared(void* existing, const int32_t* block_table, int64_t batch,

@@ -17,14 +17,20 @@ struct Buffer {
     if (bytes <= capacity) return hipSuccess;
     size_t grown = std::max(bytes, capacity ? capacity * 2 : size_t(65536));
     void* fresh = nullptr;
-    hipError_t st = pinned ? hipHostMalloc(&fresh, grown, hipHostMallocDefault)
-                           : hipMalloc(&fresh, grown);
+    hipError_t st = allocate(&fresh, grown);
+    if (st != hipSuccess && grown > bytes) st = allocate(&fresh, grown = bytes);
     if (st != hipSuccess) return st;
     release();
     ptr = fresh;
     capacity = grown;
     ++allocations;
     return hipSuccess;
+  }
+  hipError_t allocate(void** out, size_t bytes) const {
+    const hipError_t st =
+        pinned ? hipHostMalloc(out, bytes, hipHostMallocDefault) : hipMalloc(out, bytes);
+    if (st != hipSuccess) (void)hipGetLastError();  // answered here, not by the next launch's check
+    return st;
   }
   void release() {
     if (ptr) {

@@ -1524,8 +1524,15 @@ static void* prepare_decode(void* existing, const int32_t* block_table, int64_t 
     if ((groups > 0 || plan->shared_graph) && !plan->shared)
       plan->shared = std::make_unique<SharedPlan>(plan->cus, num_q_heads, num_kv_heads, page_size,
                                                   dtype);
-    const bool shared_runs =
+    bool shared_runs =
         plan->shared_graph || (!graph && groups > 0 && plan->shared->pays(sharing));
+    plan->batch = 0;  // nothing runs until all of the new plan stands
+    if (shared_runs) {
+      const SharedFit fit = plan->shared->prepare(sharing, graph ? batch : 0, columns * page_size,
+                                                  plan->allocations, s);
+      if (fit == SharedFit::kError) return nullptr;
+      shared_runs = fit == SharedFit::kRuns;
+    }
 
     const LaunchShape shape = launch_shape(plan->cus, num_kv_heads, page_size);
     const int64_t items_cap = items_capacity_for(shape, batch, columns * page_size);
@@ -1633,9 +1640,6 @@ static void* prepare_decode(void* existing, const int32_t* block_table, int64_t 
       hip_error(st, "decode upload event");
       return nullptr;
     }
-    if (shared_runs && !plan->shared->prepare(sharing, graph ? batch : 0, columns * page_size,
-                                              plan->allocations, s))
-      return nullptr;
     plan->shared_runs = shared_runs;
     plan->batch = batch;
     plan->total_pages = total_pages;
@@ -1741,6 +1745,7 @@ extern "C" const char* mi355x_decode_run(const void* plan_ptr, const void* q, in
                                          void* stream) {
   if (!plan_ptr) return set_error("decode was not prepared");
   const auto& p = *static_cast<const DecodePlan*>(plan_ptr);
+  if (!p.batch) return set_error("decode was not prepared");
   if (!q || !k_cache || !v_cache || !out) return set_error("mi355x_decode_run: null pointer");
   if (num_q_heads != p.num_q_heads || num_kv_heads != p.num_kv_heads ||
       page_size != p.page_size || dtype != p.dtype || batch != p.batch)

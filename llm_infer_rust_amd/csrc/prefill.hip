@@ -820,7 +820,13 @@ static void* prepare_prefill(void* existing, const int32_t* q_indptr, const int3
     if (groups > 0 && !plan->shared)
       plan->shared = std::make_unique<SharedPlan>(plan->cus, num_q_heads, num_kv_heads, page_size,
                                                   dtype);
-    const bool shared_runs = groups > 0 && plan->shared->pays(sharing);
+    bool shared_runs = groups > 0 && plan->shared->pays(sharing);
+    plan->batch = 0;  // nothing runs until all of the new plan stands
+    if (shared_runs) {
+      const SharedFit fit = plan->shared->prepare(sharing, 0, 0, plan->allocations, s);
+      if (fit == SharedFit::kError) return nullptr;
+      shared_runs = fit == SharedFit::kRuns;
+    }
     SplitPlan sp;
     if (!shared_runs) {
       std::vector<int32_t> base(4 * n_base);
@@ -906,7 +912,6 @@ static void* prepare_prefill(void* existing, const int32_t* q_indptr, const int3
       hip_error(st, "prefill upload event");
       return nullptr;
     }
-    if (shared_runs && !plan->shared->prepare(sharing, 0, 0, plan->allocations, s)) return nullptr;
     plan->batch = batch;
     plan->total_q = q_host[batch];
     plan->num_items = n_items;
@@ -1045,6 +1050,7 @@ extern "C" const char* mi355x_prefill_run(const void* plan_ptr, const void* q, i
                                           void* stream) {
   if (!plan_ptr) return set_error("prefill was not prepared");
   const auto& p = *static_cast<const PrefillPlan*>(plan_ptr);
+  if (!p.batch) return set_error("prefill was not prepared");
   if (!q || !k || !v || !out) return set_error("mi355x_prefill_run: null pointer");
   if (total_q != p.total_q || num_q_heads != p.num_q_heads || num_kv_heads != p.num_kv_heads ||
       page_size != p.page_size || dtype != p.dtype)

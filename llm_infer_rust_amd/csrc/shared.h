@@ -35,6 +35,8 @@ struct SharedBatch {
 const char* check_groups(const int32_t* group_rows, const int32_t* group_lens, int64_t groups,
                          int64_t batch, const int32_t* cached, const char* too_long);
 
+enum class SharedFit { kRuns, kPlain, kError };  // kPlain: the plain kernels are to run the batch
+
 class SharedPlan {
  public:
   SharedPlan(int64_t cus, int64_t num_q_heads, int64_t num_kv_heads, int64_t page_size,
@@ -42,11 +44,12 @@ class SharedPlan {
   ~SharedPlan();
   // Whether computing the shared prefixes of such a batch once beats the plain kernels.
   bool pays(const SharedBatch& b) const;
-  // Plans and uploads. Graph plans (graph_rows > 0: as many requests of one token and up to
-  // graph_tokens keys) hold room for any groups and launch the same grids whatever is shared. False:
+  // Plans and uploads. kPlain: partial outputs of more than most_partials(), or no memory for them.
+  // Graph plans (graph_rows > 0: as many requests of one token and up to graph_tokens keys) hold room
+  // for any groups and launch the same grids whatever is shared; they are never kPlain. kError:
   // mi355x_attn_error says why.
-  bool prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph_tokens,
-               uint64_t& allocations, hipStream_t s);
+  SharedFit prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph_tokens,
+                    uint64_t& allocations, hipStream_t s);
   const char* run(const int32_t* indices, const void* q, int64_t q_sn, int64_t q_sh, const void* k,
                   const void* v, void* out, int64_t o_sn, int64_t o_sh, hipStream_t s) const;
   void info(int64_t* out4) const;

@@ -933,6 +933,14 @@ int64_t least_saved(int64_t num_kv_heads) {
 }
 // Prefixes of 64 tokens are not worth it in any batch (256 rows: 24.4 us plain, 30.5 shared).
 int32_t shortest_prefix() { return std::getenv("MI355X_SHARED_FROM") ? kTileK : 2 * kTileK; }
+// Most bytes of partial outputs of a batch: the workspace stands beside the caller's memory and is kept.
+// A token takes 516 bytes a q head and part, at least two parts: 4 GiB are some 40,000 new tokens of 64
+// heads, without a limit a batch could ask for more than 64 GiB. MI355X_SHARED_MOST overrides it (tuning
+// knob, read for every plan).
+int64_t most_partials() {
+  if (const char* env = std::getenv("MI355X_SHARED_MOST")) return std::strtoll(env, nullptr, 10);
+  return int64_t(4) << 30;
+}
 }  // namespace
 
 struct SharedPlan::State {
@@ -998,8 +1006,8 @@ bool SharedPlan::pays(const SharedBatch& b) const {
   return any && saved >= least_saved(st_->num_kv_heads);
 }
 
-bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph_tokens,
-                         uint64_t& allocations, hipStream_t s) {
+SharedFit SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph_tokens,
+                              uint64_t& allocations, hipStream_t s) {
   State& st = *st_;
   st.ready = false;
   const int64_t group = st.group, heads = st.num_kv_heads;
@@ -1148,7 +1156,7 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
                      merge.data(), &share, wg.data(), shape.wg_capacity, &wgs);
     if (items < 0) {
       set_error("shared prefix work list exceeds its capacity");
-      return false;
+      return SharedFit::kError;
     }
   }
   // Items of a source are consecutive: its slots follow each other.
@@ -1192,6 +1200,8 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
   const int64_t o_wg = o_gemm + kGemmInts * gemm_cap;
   const int64_t total = o_wg + wg_cap + 1;
   const size_t rows = static_cast<size_t>(slot_cap) * st.num_q_heads;
+  if (!graph_rows && static_cast<int64_t>(rows * (kD + 1) * 4) > most_partials())
+    return SharedFit::kPlain;
   hipError_t err = hipSuccess;
   if (!st.upload_done) err = hipEventCreateWithFlags(&st.upload_done, hipEventDisableTiming);
   if (err == hipSuccess) err = hipEventSynchronize(st.upload_done);  // staging is free
@@ -1199,15 +1209,16 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
                      rows * kD * 4 > st.part_o.capacity || rows * 4 > st.part_lse.capacity;
   if (graph_rows && st.batch && grows) {
     set_error("graph decode metadata capacity exceeded");
-    return false;
+    return SharedFit::kError;
   }
   if (err == hipSuccess) err = st.ints.reserve(total * 4, allocations);
   if (err == hipSuccess) err = st.staging.reserve(total * 4, allocations);
   if (err == hipSuccess) err = st.part_o.reserve(rows * kD * 4, allocations);
   if (err == hipSuccess) err = st.part_lse.reserve(rows * 4, allocations);
+  if (err == hipErrorOutOfMemory && !graph_rows) return SharedFit::kPlain;
   if (err != hipSuccess) {
     hip_error(err, "shared prefix workspace");
-    return false;
+    return SharedFit::kError;
   }
   int32_t* host = static_cast<int32_t*>(st.staging.ptr);
   host[kHeaderGemmItems] = static_cast<int32_t>(st.gemm_items);
@@ -1251,7 +1262,7 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
   if (err == hipSuccess) err = hipEventRecord(st.upload_done, s);
   if (err != hipSuccess) {
     hip_error(err, "shared prefix upload");
-    return false;
+    return SharedFit::kError;
   }
   st.ready = true;
   st.batch = b.batch;
@@ -1265,7 +1276,7 @@ bool SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph
   st.o_stream = o_stream;
   st.o_gemm = o_gemm;
   st.o_wg = o_wg;
-  return true;
+  return SharedFit::kRuns;
 }
 
 void SharedPlan::info(int64_t* out4) const {

@@ -101,6 +101,40 @@ def test_what_saves_little_is_left_to_the_plain_kernels(gpu, monkeypatch):
         assert info["tokens"] == (sum(n for r, n in groups if r > 1 and n >= 128) if used else 0)
 
 
+def test_partials_of_no_use_are_left_to_the_plain_kernels(gpu, monkeypatch):
+    """A batch whose partial outputs pass the limit runs plain, on the same plan as ones that share."""
+    d = Batch([(40, 600)], own_lengths(40, 1, 50), heads=16, kv_heads=8)
+    e = Batch([(9, 500)], [30] * 9, [30] * 9, heads=16, kv_heads=8)
+    attention = d.attention()
+    for most in (None, 100_000, None, 0, 1 << 40):
+        if most is None:
+            monkeypatch.delenv("MI355X_SHARED_MOST", raising=False)
+        else:
+            monkeypatch.setenv("MI355X_SHARED_MOST", str(most))
+        for b, meta in ((d, d.decode_meta()), (e, e.extend_meta())):
+            got, info = b.run(meta, attention)
+            assert (info["items"] > 0) == (most is None or most > 100_000)
+            b.check(got)
+
+
+def test_partials_have_a_limit(gpu):
+    """4 GiB by default: 516 bytes a token, q head and part, at least two parts. Planned, not run."""
+    rows, prefix = 1100, 4096
+    table = torch.arange(1, prefix // 16 + 6, dtype=torch.int32, device=gpu).repeat(rows, 1)
+    attention = Batch([(2, 64)], [1, 1], heads=64).attention()
+    for new in (8, 64):  # 0.54 GiB and 4.3 GiB at the least
+        starts = [i * new for i in range(rows + 1)]
+        meta = AttentionMetadata(
+            BatchPhase.PREFILL, block_table=table,
+            cu_seqlens_q=torch.tensor(starts, dtype=torch.int32, device=gpu),
+            prefix_lens=torch.full((rows,), prefix, dtype=torch.int32, device=gpu),
+            host_cu_seqlens_q=starts, host_prefix_lens=[prefix] * rows,
+            shared_prefix=SharedPrefix([rows], [prefix]))
+        batch = attention.prepare(meta, starts[-1])
+        assert (batch.plan.plan.shared_info()["items"] > 0) == (new == 8)
+        del batch
+
+
 def test_whole_request_is_shared(gpu):
     """A group's lens may cover every token: the last ones are then each row's own."""
     b = Batch([(3, 128), (2, 64), (2, 40)], [0] * 7, [1] * 7)
