@@ -712,6 +712,61 @@ SplitPlan split_items(const std::vector<int32_t>& base, const int32_t* q_host,
   }
   return out;
 }
+// us that a paged batch takes, to compare with what sharing its prefixes would: items or chunks of the
+// work list over the CUs, the long ones in rounds. A tile takes a CU as long as its waves with queries
+// need; 4 tiles' time beside them an item, 2 us a launch. Rows that fill their columns share nothing a
+// product could save, and sharing writes partial outputs: 48 rows of 128 new tokens behind 512 take 84 us
+// here and 202 shared, behind 8,192 740 and 862; of 16 behind 8,192 343 and 142. Over 350 batches
+// (2 to 128 rows, 1 to 2,048 new tokens, nine head layouts) the choice costs 0.3% on average, 18% at most.
+double estimated_us(const int32_t* q_host, const int32_t* prefix_host, int64_t batch,
+                    int64_t num_q_heads, int64_t num_kv_heads, int64_t cus) {
+  const int waves = prefill_waves(true);
+  const int hpb = heads_per_block(num_q_heads / num_kv_heads, waves);
+  const int64_t bq = kQPerWave * (waves / hpb);
+  const int64_t alike = num_q_heads / hpb;  // items of a query tile
+  struct Tile {
+    int64_t tiles;
+    double tile_us;
+  };
+  std::vector<Tile> items;
+  int64_t total = 0, longest = 0;
+  for (int64_t r = 0; r < batch; ++r) {
+    const int64_t q_len = q_host[r + 1] - q_host[r];
+    for (int64_t q0 = 0; q0 < q_len; q0 += bq) {
+      const int64_t queries = std::min(bq, q_len - q0);
+      const int64_t tiles = (prefix_host[r] + q0 + queries + kTileK - 1) / kTileK;
+      const double busy =
+          static_cast<double>((queries + kQPerWave - 1) / kQPerWave * hpb) / waves;
+      items.push_back({tiles, 1.1 + 0.65 * busy * busy});
+      total += tiles * alike;
+      longest = std::max(longest, tiles);
+    }
+  }
+  const int64_t share = (total + cus - 1) / cus;  // cut as split_items does
+  const bool split = longest > 2 * share && longest > 2 * kMinChunkTiles;
+  const int64_t chunk = std::max(kMinChunkTiles, share);
+  double most = 0, all_us = 0, long_us = 0;
+  int64_t longs = 0, partials = 0;
+  auto parts_of = [&](const Tile& t) {
+    return split && t.tiles > chunk ? (t.tiles + chunk - 1) / chunk : 1;
+  };
+  auto us_of = [&](const Tile& t) {
+    return (static_cast<double>(t.tiles) / parts_of(t) + 4) * t.tile_us;
+  };
+  for (const Tile& t : items) most = std::max(most, us_of(t));
+  for (const Tile& t : items) {
+    const int64_t n = alike * parts_of(t);
+    all_us += us_of(t) * n;
+    if (parts_of(t) > 1) partials += n;
+    if (2 * us_of(t) <= most) continue;
+    longs += n;
+    long_us += us_of(t) * n;
+  }
+  const double rounds = static_cast<double>((longs + cus - 1) / cus) * (long_us / longs);
+  return 2 + std::max({most, rounds, all_us / cus}) +
+         static_cast<double>(partials * waves * kQPerWave * 1056) / 5e6;
+}
+
 }  // namespace
 }  // namespace mi355x
 
@@ -815,7 +870,7 @@ static void* prepare_prefill(void* existing, const int32_t* q_indptr, const int3
       first_page[r + 1] =
           first_page[r] + static_cast<int32_t>((kv_len[r] + page_size - 1) / page_size);
     }
-    const SharedBatch sharing{batch,      q_host,     kv_len.data(), first_page.data(),
+    SharedBatch sharing{batch,      q_host,     kv_len.data(), first_page.data(),
                               group_rows, group_lens, groups};
     if (groups > 0 && !plan->shared)
       plan->shared = std::make_unique<SharedPlan>(plan->cus, num_q_heads, num_kv_heads, page_size,
@@ -823,6 +878,8 @@ static void* prepare_prefill(void* existing, const int32_t* q_indptr, const int3
     bool shared_runs = groups > 0 && plan->shared->pays(sharing);
     plan->batch = 0;  // nothing runs until all of the new plan stands
     if (shared_runs) {
+      sharing.plain_us =
+          estimated_us(q_host, prefix_host, batch, num_q_heads, num_kv_heads, plan->cus);
       const SharedFit fit = plan->shared->prepare(sharing, 0, 0, plan->allocations, s);
       if (fit == SharedFit::kError) return nullptr;
       shared_runs = fit == SharedFit::kRuns;

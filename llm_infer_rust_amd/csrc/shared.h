@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cstdint>
+#include <limits>
 #include <memory>
 #include <vector>
 
@@ -29,6 +30,8 @@ struct SharedBatch {
   const int32_t* group_rows; // [groups]
   const int32_t* group_lens; // [groups] leading keys that a group's requests share
   int64_t groups;
+  // us that the plain kernels are estimated to take; a plan that is estimated no quicker does not run.
+  double plain_us = std::numeric_limits<double>::infinity();
 };
 
 // nullptr, or why the groups are refused. cached[r]: keys of request r that may be shared.
@@ -44,7 +47,8 @@ class SharedPlan {
   ~SharedPlan();
   // Whether computing the shared prefixes of such a batch once beats the plain kernels.
   bool pays(const SharedBatch& b) const;
-  // Plans and uploads. kPlain: partial outputs of more than most_partials(), or no memory for them.
+  // Plans and uploads. kPlain: no quicker than plain_us, partial outputs of more than most_partials(), or
+  // no memory for them.
   // Graph plans (graph_rows > 0: as many requests of one token and up to graph_tokens keys) hold room
   // for any groups and launch the same grids whatever is shared; they are never kPlain. kError:
   // mi355x_attn_error says why.

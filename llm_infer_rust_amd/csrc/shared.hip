@@ -925,14 +925,15 @@ namespace {
 // the merge. us a layer, plain against shared (32 heads, 8 kv heads): 2 rows of 1,024 tokens (4 MB)
 // 11.7, 13.2; 8 of 256 (7 MB) 13.5, 13.1; 4 of 1,024 (12 MB) 13.4, 13.3; 16 of 1,024 (60 MB) 16.2,
 // 14.3; 256 of 1,024 117, 33. With fewer kv heads than a slice has the plain kernel is the slower one
-// throughout (one kv head: 22, 13). MI355X_SHARED_FROM (bytes) overrides it and kShortest (tuning
-// knob, read for every plan).
+// throughout (one kv head: 22, 13). MI355X_SHARED_FROM (bytes) overrides it, the shortest prefix and the
+// comparison with the plain kernels' time (tuning knob, read for every plan).
+bool forced() { return std::getenv("MI355X_SHARED_FROM") != nullptr; }
 int64_t least_saved(int64_t num_kv_heads) {
-  if (const char* env = std::getenv("MI355X_SHARED_FROM")) return std::strtoll(env, nullptr, 10);
+  if (forced()) return std::strtoll(std::getenv("MI355X_SHARED_FROM"), nullptr, 10);
   return num_kv_heads % 4 ? 0 : int64_t(8) << 20;
 }
 // Prefixes of 64 tokens are not worth it in any batch (256 rows: 24.4 us plain, 30.5 shared).
-int32_t shortest_prefix() { return std::getenv("MI355X_SHARED_FROM") ? kTileK : 2 * kTileK; }
+int32_t shortest_prefix() { return forced() ? kTileK : 2 * kTileK; }
 // Most bytes of partial outputs of a batch: the workspace stands beside the caller's memory and is kept.
 // A token takes 516 bytes a q head and part, at least two parts: 4 GiB are some 40,000 new tokens of 64
 // heads, without a limit a batch could ask for more than 64 GiB. MI355X_SHARED_MOST overrides it (tuning
@@ -1059,6 +1060,9 @@ SharedFit SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t 
   for (const Source& src : stream) bytes += int64_t(src.end - src.begin) * heads * kD * 4;
   // A CU's tile of 256 columns while others stream, and the copies' rate on the whole chip.
   constexpr double kTileUs = 1.68, kBytesPerUs = 5.86e6;
+  // A tile of 128 columns while the CU does another, and what a plan costs beside its loops, more where
+  // it has both.
+  constexpr double kNarrowTileUs = 1.28, kLaunchesUs = 8, kBothUs = 5;
   double stream_us = static_cast<double>(bytes) / kBytesPerUs;
   // A few requests with little of their own take products too: not half a CU's worth of items and no
   // launch that would wait for the others' (48 rows of up to 40 new tokens behind 4,096, two layers 226
@@ -1171,10 +1175,23 @@ SharedFit SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t 
     slot += static_cast<int64_t>(src.splits) * src.tokens;
   }
   // The matrix products.
+  GemmLength length{};
   if (!gemm.empty())
-    schedule_gemm(gemm, group, heads, columns,
-                  gemm_length(gemm, group, heads, columns, gemm_wgs, merge_tiles, cap).tiles, slot,
-                  gemm_work);
+    length = gemm_length(gemm, group, heads, columns, gemm_wgs, merge_tiles, cap);
+  if (!graph_rows && !forced()) {
+    // Against the plain kernels' time: the launches, products and copies as above (they take an eighth
+    // longer than their loops alone), partial outputs written and read.
+    const double products_us = (st.nw == 8 ? kTileUs : kNarrowTileUs) * length.tile_times;
+    if (st.form == Form::kWhole) stream_us *= static_cast<double>(st.cus) / (st.cus - gemm_wgs);
+    const double both = st.form == Form::kInTurn ? products_us + stream_us
+                                                 : std::max(products_us, stream_us);
+    const int64_t slots =
+        slot + count_gemm(gemm, group, heads, columns, std::max<int64_t>(1, length.tiles)).slots;
+    const double partials_us = static_cast<double>(slots * st.num_q_heads * 1056) / 5e6;
+    const double beside_us = kLaunchesUs + (stream.empty() || gemm.empty() ? 0 : kBothUs);
+    if (beside_us + 1.12 * both + partials_us >= b.plain_us) return SharedFit::kPlain;
+  }
+  schedule_gemm(gemm, group, heads, columns, length.tiles, slot, gemm_work);
   st.slices = shape.grid_y;
   st.gemm_wgs = std::min(gemm_wgs, static_cast<int64_t>(gemm_work.size()) / kGemmInts);
   st.gemm_items = static_cast<int64_t>(gemm_work.size()) / kGemmInts;

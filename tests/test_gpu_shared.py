@@ -101,6 +101,33 @@ def test_what_saves_little_is_left_to_the_plain_kernels(gpu, monkeypatch):
         assert info["tokens"] == (sum(n for r, n in groups if r > 1 and n >= 128) if used else 0)
 
 
+@pytest.mark.parametrize("rows,new,prefix,heads,kv_heads,used", [
+    # us, plain and shared: where the plain kernel's columns are full, sharing is the slower one
+    (48, 128, 512, 32, 8, False),    # 84, 202
+    (16, 512, 2048, 32, 8, False),   # 333, 464
+    (48, 64, 512, 64, 8, False),     # 83, 191
+    (4, 1024, 2048, 32, 8, False),   # 186, 274
+    (48, 16, 2048, 32, 8, True),     # 100, 62
+    (16, 2, 8192, 16, 8, True),      # 154, 21
+    (48, 64, 8192, 16, 8, True),     # 326, 257
+    (2, 16, 512, 8, 1, True),        # 21.3, 16.7
+])
+def test_extends_share_where_that_is_quicker(gpu, monkeypatch, rows, new, prefix, heads, kv_heads,
+                                             used):
+    monkeypatch.delenv("MI355X_SHARED_FROM")
+    table = torch.arange(1, (prefix + new) // 16 + 2, dtype=torch.int32, device=gpu).repeat(rows, 1)
+    starts = [i * new for i in range(rows + 1)]
+    meta = AttentionMetadata(
+        BatchPhase.PREFILL, block_table=table,
+        cu_seqlens_q=torch.tensor(starts, dtype=torch.int32, device=gpu),
+        prefix_lens=torch.full((rows,), prefix, dtype=torch.int32, device=gpu),
+        host_cu_seqlens_q=starts, host_prefix_lens=[prefix] * rows,
+        shared_prefix=SharedPrefix([rows], [prefix]))
+    attention = Batch([(2, 64)], [1, 1], heads=heads, kv_heads=kv_heads).attention()
+    batch = attention.prepare(meta, starts[-1])
+    assert (batch.plan.plan.shared_info()["items"] > 0) == used
+
+
 def test_partials_of_no_use_are_left_to_the_plain_kernels(gpu, monkeypatch):
     """A batch whose partial outputs pass the limit runs plain, on the same plan as ones that share."""
     d = Batch([(40, 600)], own_lengths(40, 1, 50), heads=16, kv_heads=8)
