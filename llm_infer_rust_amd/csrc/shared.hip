@@ -928,9 +928,14 @@ namespace {
 // throughout (one kv head: 22, 13). MI355X_SHARED_FROM (bytes) overrides it, the shortest prefix and the
 // comparison with the plain kernels' time (tuning knob, read for every plan).
 bool forced() { return std::getenv("MI355X_SHARED_FROM") != nullptr; }
+// Four kv heads are one slice on halves of CUs, which streams rows' own keys at 5.2 TB/s where the plain
+// kernel reaches 5.9: there the prefix has to save a third of what the rows read of their own, and twice the
+// bytes (us, 48 rows, 32 heads: 256 shared tokens and 3,000 own 56.4, 63.7; 512 63.1, 67.4; 1,024 69.9, 67.7;
+// 12 rows, 1,024 and 3,000 23.7, 27.3, 512 and 64 10.2, 11.2; 1,500 and 1,500 20.2, 18.5).
+constexpr int64_t kOneSliceOwn = 3;
 int64_t least_saved(int64_t num_kv_heads) {
   if (forced()) return std::strtoll(std::getenv("MI355X_SHARED_FROM"), nullptr, 10);
-  return num_kv_heads % 4 ? 0 : int64_t(8) << 20;
+  return num_kv_heads % 4 ? 0 : int64_t(num_kv_heads == 4 ? 16 : 8) << 20;
 }
 // Prefixes of 64 tokens are not worth it in any batch (256 rows: 24.4 us plain, 30.5 shared).
 int32_t shortest_prefix() { return forced() ? kTileK : 2 * kTileK; }
@@ -996,15 +1001,18 @@ SharedPlan::~SharedPlan() = default;
 
 bool SharedPlan::pays(const SharedBatch& b) const {
   const std::vector<int32_t> eff = st_->lengths(b);
-  int64_t saved = 0;
+  int64_t saved = 0, own = 0;
   bool any = false;
   // The merge takes 32 threads a row of a q head, and a grid of 2^32 would be cut short.
   if (int64_t(b.q_start[b.batch]) * st_->num_q_heads >= int64_t(1) << 26) return false;
-  for (int64_t g = 0; g < b.groups; ++g) {
-    saved += int64_t(b.group_rows[g] - 1) * eff[g] * st_->num_kv_heads * kD * 4;
+  for (int64_t g = 0, row = 0; g < b.groups; ++g) {
+    saved += int64_t(b.group_rows[g] - 1) * eff[g];
     any |= eff[g] > 0;
+    for (const int64_t end = row + b.group_rows[g]; row < end; ++row) own += b.kv_len[row] - eff[g];
   }
-  return any && saved >= least_saved(st_->num_kv_heads);
+  const int64_t heads = st_->num_kv_heads;
+  if (!any || saved * heads * kD * 4 < least_saved(heads)) return false;
+  return forced() || heads != 4 || kOneSliceOwn * saved >= own;
 }
 
 SharedFit SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph_tokens,

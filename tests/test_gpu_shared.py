@@ -101,6 +101,19 @@ def test_what_saves_little_is_left_to_the_plain_kernels(gpu, monkeypatch):
         assert info["tokens"] == (sum(n for r, n in groups if r > 1 and n >= 128) if used else 0)
 
 
+def test_four_kv_heads_share_where_the_prefix_is_long(gpu, monkeypatch):
+    """One slice of four heads streams rows' own keys slower than the plain kernel: the prefix saves 16
+    MiB and a third of what the rows read of their own, or it is not shared."""
+    monkeypatch.delenv("MI355X_SHARED_FROM")
+    for groups, own, used in (([(48, 256)], 3000, False), ([(48, 2000)], 1000, True),
+                              ([(12, 512)], 64, False), ([(48, 256)], 64, True),
+                              ([(12, 1024)], 3000, False), ([(20, 900), (28, 128)], 2500, False)):
+        b = Batch(groups, [own] * sum(r for r, _ in groups), heads=16, kv_heads=4)
+        got, info = b.run(b.decode_meta())
+        assert (info["items"] > 0) == used, (groups, own, info)
+        b.check(got)
+
+
 @pytest.mark.parametrize("rows,new,prefix,heads,kv_heads,used", [
     # us, plain and shared: where the plain kernel's columns are full, sharing is the slower one
     (48, 128, 512, 32, 8, False),    # 84, 202
