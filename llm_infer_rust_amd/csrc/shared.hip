@@ -921,22 +921,23 @@ const char* check_groups(const int32_t* group_rows, const int32_t* group_lens, i
 }
 
 namespace {
+// MI355X_SHARED_FROM (bytes) overrides from when on prefixes are shared: least_saved(), the shortest
+// prefix, kOneSliceOwn and the comparison with the plain kernels' time (tuning knob, read for every plan).
+bool forced() { return std::getenv("MI355X_SHARED_FROM") != nullptr; }
 // Bytes of K and V that sharing has to save a layer: less is lost again on the products' launch and
 // the merge. us a layer, plain against shared (32 heads, 8 kv heads): 2 rows of 1,024 tokens (4 MB)
 // 11.7, 13.2; 8 of 256 (7 MB) 13.5, 13.1; 4 of 1,024 (12 MB) 13.4, 13.3; 16 of 1,024 (60 MB) 16.2,
 // 14.3; 256 of 1,024 117, 33. With fewer kv heads than a slice has the plain kernel is the slower one
-// throughout (one kv head: 22, 13). MI355X_SHARED_FROM (bytes) overrides it, the shortest prefix and the
-// comparison with the plain kernels' time (tuning knob, read for every plan).
-bool forced() { return std::getenv("MI355X_SHARED_FROM") != nullptr; }
+// throughout (one kv head: 22, 13).
+int64_t least_saved(int64_t num_kv_heads) {
+  if (forced()) return std::strtoll(std::getenv("MI355X_SHARED_FROM"), nullptr, 10);
+  return num_kv_heads % 4 ? 0 : int64_t(num_kv_heads == 4 ? 16 : 8) << 20;
+}
 // Four kv heads are one slice on halves of CUs, which streams rows' own keys at 5.2 TB/s where the plain
 // kernel reaches 5.9: there the prefix has to save a third of what the rows read of their own, and twice the
 // bytes (us, 48 rows, 32 heads: 256 shared tokens and 3,000 own 56.4, 63.7; 512 63.1, 67.4; 1,024 69.9, 67.7;
 // 12 rows, 1,024 and 3,000 23.7, 27.3, 512 and 64 10.2, 11.2; 1,500 and 1,500 20.2, 18.5).
 constexpr int64_t kOneSliceOwn = 3;
-int64_t least_saved(int64_t num_kv_heads) {
-  if (forced()) return std::strtoll(std::getenv("MI355X_SHARED_FROM"), nullptr, 10);
-  return num_kv_heads % 4 ? 0 : int64_t(num_kv_heads == 4 ? 16 : 8) << 20;
-}
 // Prefixes of 64 tokens are not worth it in any batch (256 rows: 24.4 us plain, 30.5 shared).
 int32_t shortest_prefix() { return forced() ? kTileK : 2 * kTileK; }
 // Most bytes of partial outputs of a batch: the workspace stands beside the caller's memory and is kept.

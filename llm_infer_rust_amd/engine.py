@@ -64,8 +64,11 @@ class EngineConfig:
     overlap_decode: bool = True
     seed: int = 0
     # Compute decode attention over the prompt that completions of a request share (SamplingParams.n)
-    # once for all of them. Decode graphs are then captured in a form that can; a step that shares
-    # nothing takes slightly longer in it than in the form that cannot.
+    # once for all of them. Decode graphs are then captured in a form that can, and a step that shares
+    # little takes up to 2 us a layer longer in it (32 heads, 8 kv heads: 8 rows alone 13.3 us in the
+    # form that cannot, 15.5; 4 rows behind 1,100 tokens 10.2, 12.2; 64 alone 99, 101; 64 behind 2,048
+    # 87, 31). Every captured batch size has partial outputs of its own for whatever its rows may share:
+    # 3.3 GiB in all for the default sizes with these heads, 27 MiB for 1 row to 129 for 256.
     share_prefixes: bool = False
 
 

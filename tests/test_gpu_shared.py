@@ -59,6 +59,15 @@ def test_decode(gpu, groups, own, heads, kv_heads, page, dtype, copies):
     b.check(plain)
 
 
+@pytest.mark.parametrize("groups,own,heads,kv_heads,page,dtype", DECODE)
+def test_decode_shares_every_group(gpu, groups, own, heads, kv_heads, page, dtype):
+    rows = sum(r for r, _ in groups)
+    b = Batch(groups, own_lengths(rows, 1, own), None, heads, kv_heads, page, dtype)
+    _, info = b.run(b.decode_meta())
+    shared = [n for r, n in groups if r > 1 and n >= 64]
+    assert info["groups"] == len(shared) and info["tokens"] == sum(n // 64 * 64 for n in shared)
+
+
 EXTEND = [
     ([(5, 700)], 0, 40, 32, 8, 16, BF16),
     ([(48, 1024)], 0, 40, 32, 8, 16, BF16),
