@@ -714,12 +714,14 @@ SplitPlan split_items(const std::vector<int32_t>& base, const int32_t* q_host,
 }
 // us that a paged batch takes, to compare with what sharing its prefixes would: items or chunks of the
 // work list over the CUs, the long ones in rounds. A tile takes a CU as long as its waves with queries
-// need; 4 tiles' time beside them an item, 2 us a launch. Rows that fill their columns share nothing a
-// product could save, and sharing writes partial outputs: 48 rows of 128 new tokens behind 512 take 84 us
-// here and 202 shared, behind 8,192 740 and 862; of 16 behind 8,192 343 and 142. Over 350 batches
-// (2 to 128 rows, 1 to 2,048 new tokens, nine head layouts) the choice costs 0.3% on average, 18% at most.
+// need; 4 tiles' time beside them an item, 2 us a launch. No less than `tokens` keys and values from memory
+// (shared ones once: the other rows find them in the caches), which short rows read at 4.2 TB/s. Rows that
+// fill their columns share nothing a product could save, and sharing writes partial outputs: 48 rows of 128
+// new tokens behind 512 take 84 us here and 202 shared, behind 8,192 740 and 862; of 16 behind 8,192 343 and
+// 142. Over 720 batches (2 to 256 rows, 1 to 2,048 new tokens, ten head layouts, pages of 1 to 64) the choice
+// costs 0.8% on average; where the two are close, a batch of 20 to 40 us can take up to half as long again.
 double estimated_us(const int32_t* q_host, const int32_t* prefix_host, int64_t batch,
-                    int64_t num_q_heads, int64_t num_kv_heads, int64_t cus) {
+                    int64_t num_q_heads, int64_t num_kv_heads, int64_t cus, int64_t tokens) {
   const int waves = prefill_waves(true);
   const int hpb = heads_per_block(num_q_heads / num_kv_heads, waves);
   const int64_t bq = kQPerWave * (waves / hpb);
@@ -763,7 +765,8 @@ double estimated_us(const int32_t* q_host, const int32_t* prefix_host, int64_t b
     long_us += us_of(t) * n;
   }
   const double rounds = static_cast<double>((longs + cus - 1) / cus) * (long_us / longs);
-  return 2 + std::max({most, rounds, all_us / cus}) +
+  const double memory_us = 3 + static_cast<double>(tokens * num_kv_heads * kD * 4) / 4.2e6;
+  return 2 + std::max({most, rounds, all_us / cus, memory_us}) +
          static_cast<double>(partials * waves * kQPerWave * 1056) / 5e6;
 }
 
@@ -878,8 +881,11 @@ static void* prepare_prefill(void* existing, const int32_t* q_indptr, const int3
     bool shared_runs = groups > 0 && plan->shared->pays(sharing);
     plan->batch = 0;  // nothing runs until all of the new plan stands
     if (shared_runs) {
-      sharing.plain_us =
-          estimated_us(q_host, prefix_host, batch, num_q_heads, num_kv_heads, plan->cus);
+      int64_t tokens = 0;
+      for (const int32_t n : kv_len) tokens += n;
+      for (int64_t g = 0; g < groups; ++g) tokens -= int64_t(group_rows[g] - 1) * group_lens[g];
+      sharing.plain_us = estimated_us(q_host, prefix_host, batch, num_q_heads, num_kv_heads,
+                                      plan->cus, tokens);
       const SharedFit fit = plan->shared->prepare(sharing, 0, 0, plan->allocations, s);
       if (fit == SharedFit::kError) return nullptr;
       shared_runs = fit == SharedFit::kRuns;
