@@ -1529,7 +1529,7 @@ static void* prepare_decode(void* existing, const int32_t* block_table, int64_t 
     plan->batch = 0;  // nothing runs until all of the new plan stands
     if (shared_runs) {
       const SharedFit fit = plan->shared->prepare(sharing, graph ? batch : 0, columns * page_size,
-                                                  plan->allocations, s);
+                                                  plan->allocations);
       if (fit == SharedFit::kError) return nullptr;
       shared_runs = fit == SharedFit::kRuns;
     }
@@ -1640,6 +1640,7 @@ static void* prepare_decode(void* existing, const int32_t* block_table, int64_t 
       hip_error(st, "decode upload event");
       return nullptr;
     }
+    if (shared_runs && !plan->shared->upload(sharing, s)) return nullptr;
     plan->shared_runs = shared_runs;
     plan->batch = batch;
     plan->total_pages = total_pages;

@@ -886,7 +886,7 @@ static void* prepare_prefill(void* existing, const int32_t* q_indptr, const int3
       for (int64_t g = 0; g < groups; ++g) tokens -= int64_t(group_rows[g] - 1) * group_lens[g];
       sharing.plain_us = estimated_us(q_host, prefix_host, batch, num_q_heads, num_kv_heads,
                                       plan->cus, tokens);
-      const SharedFit fit = plan->shared->prepare(sharing, 0, 0, plan->allocations, s);
+      const SharedFit fit = plan->shared->prepare(sharing, 0, 0, plan->allocations);
       if (fit == SharedFit::kError) return nullptr;
       shared_runs = fit == SharedFit::kRuns;
     }
@@ -975,6 +975,7 @@ static void* prepare_prefill(void* existing, const int32_t* q_indptr, const int3
       hip_error(st, "prefill upload event");
       return nullptr;
     }
+    if (shared_runs && !plan->shared->upload(sharing, s)) return nullptr;
     plan->batch = batch;
     plan->total_q = q_host[batch];
     plan->num_items = n_items;

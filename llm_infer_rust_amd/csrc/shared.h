@@ -47,13 +47,15 @@ class SharedPlan {
   ~SharedPlan();
   // Whether computing the shared prefixes of such a batch once beats the plain kernels.
   bool pays(const SharedBatch& b) const;
-  // Plans and uploads. kPlain: no quicker than plain_us, partial outputs of more than most_partials(), or
-  // no memory for them.
-  // Graph plans (graph_rows > 0: as many requests of one token and up to graph_tokens keys) hold room
-  // for any groups and launch the same grids whatever is shared; they are never kPlain. kError:
-  // mi355x_attn_error says why.
+  // Plans, on the host. kPlain: no quicker than plain_us, partial outputs of more than most_partials(), or
+  // no memory for them. Graph plans (graph_rows > 0: as many requests of one token and up to graph_tokens
+  // keys) hold room for any groups and launch the same grids whatever is shared; they are never kPlain.
+  // kError, and false of upload(): mi355x_attn_error says why.
   SharedFit prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph_tokens,
-                    uint64_t& allocations, hipStream_t s);
+                    uint64_t& allocations);
+  // Lays out what prepare() planned for the same batch, beside what the stream runs meanwhile, and sends
+  // it. The plan runs from then on.
+  bool upload(const SharedBatch& b, hipStream_t s);
   const char* run(const int32_t* indices, const void* q, int64_t q_sn, int64_t q_sh, const void* k,
                   const void* v, void* out, int64_t o_sn, int64_t o_sh, hipStream_t s) const;
   void info(int64_t* out4) const;

@@ -964,6 +964,17 @@ struct SharedPlan::State {
   int64_t slices = 1;  // kv-head slices of the streaming launch
   int64_t groups_shared = 0, tokens_shared = 0, prefix_items = 0;
   int64_t o_info = 0, o_row_of = 0, o_stream = 0, o_wg = 0, o_gemm = 0;
+  // What prepare() has decided, for upload() to lay out.
+  struct Of {
+    int32_t kind, index;  // 0 none, 1 of stream, 2 of gemm
+  };
+  struct Draft {
+    std::vector<Source> stream, gemm;  // own and prefix sources of either kernel
+    std::vector<Of> prefix_of, own_of;
+    std::vector<int32_t> work, wg;     // the streaming schedule's
+    int64_t items = 0, wgs = 0, slot = 0, columns = 0, tiles = 0;
+    bool once = true;
+  } draft;
   Buffer ints, staging, part_o, part_lse;
   hipEvent_t upload_done = nullptr;
 
@@ -1017,19 +1028,23 @@ bool SharedPlan::pays(const SharedBatch& b) const {
 }
 
 SharedFit SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t graph_tokens,
-                              uint64_t& allocations, hipStream_t s) {
+                              uint64_t& allocations) {
   State& st = *st_;
   st.ready = false;
   const int64_t group = st.group, heads = st.num_kv_heads;
   const int64_t tokens = b.q_start[b.batch];
   const std::vector<int32_t> eff = st.lengths(b);
-  std::vector<Source> stream, gemm;             // own and prefix sources of either kernel
-  struct Of { int32_t kind, index; };           // 0 none, 1 stream, 2 gemm
-  std::vector<Of> prefix_of(b.batch, Of{0, 0}), own_of(b.batch, Of{0, 0});
-  std::vector<int32_t> lens, work, merge, wg, gemm_work;
+  using Of = State::Of;
+  st.draft = {};
+  std::vector<Source>&stream = st.draft.stream, &gemm = st.draft.gemm;
+  std::vector<Of>&prefix_of = st.draft.prefix_of, &own_of = st.draft.own_of;
+  std::vector<int32_t>&work = st.draft.work, &wg = st.draft.wg;
+  int64_t &items = st.draft.items, &wgs = st.draft.wgs, &slot = st.draft.slot;
+  std::vector<int32_t> lens, merge;
   GemmCount cap;
-  int64_t items = 0, wgs = 0, slot = 0, items_cap = 0;
-  bool once = true;
+  int64_t items_cap = 0;
+  prefix_of.assign(b.batch, Of{0, 0});
+  own_of.assign(b.batch, Of{0, 0});
   st.groups_shared = st.tokens_shared = 0;
   for (int64_t r = 0, g = 0, left = 0, before = 0; r < b.batch; ++r) {
     if (left == 0 && g < b.groups) {  // a group begins
@@ -1156,13 +1171,12 @@ SharedFit SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t 
     items_cap += 1 + ceil_div(lens.back(), shape.max_item);
     widest = std::max<int>(widest, src.tokens * static_cast<int>(group));
   }
-  once = bytes >= int64_t(8) << 20;  // as the decode kernel's copies
+  st.draft.once = bytes >= int64_t(8) << 20;  // as the decode kernel's copies
   st.sets = widest <= 16 ? 1 : 2;
   work.resize(4 * items_cap);
   merge.resize(2 * stream.size());
   wg.resize(shape.wg_capacity + 1);
   int64_t share = 0;
-  items = wgs = slot = 0;
   if (!stream.empty()) {
     items = schedule(lens.data(), static_cast<int64_t>(stream.size()), shape.workgroups,
                      shape.max_item, kStreamTile, /*graph=*/true, work.data(), items_cap,
@@ -1185,8 +1199,12 @@ SharedFit SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t 
   }
   // The matrix products.
   GemmLength length{};
-  if (!gemm.empty())
+  GemmCount products;
+  if (!gemm.empty()) {
     length = gemm_length(gemm, group, heads, columns, gemm_wgs, merge_tiles, cap);
+    products = count_gemm(gemm, group, heads, columns, length.tiles);
+  }
+  const int64_t slots = slot + products.slots;
   if (!graph_rows && !forced()) {
     // Against the plain kernels' time: the launches, products and copies as above (they take an eighth
     // longer than their loops alone), partial outputs written and read.
@@ -1194,20 +1212,19 @@ SharedFit SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t 
     if (st.form == Form::kWhole) stream_us *= static_cast<double>(st.cus) / (st.cus - gemm_wgs);
     const double both = st.form == Form::kInTurn ? products_us + stream_us
                                                  : std::max(products_us, stream_us);
-    const int64_t slots =
-        slot + count_gemm(gemm, group, heads, columns, std::max<int64_t>(1, length.tiles)).slots;
     const double partials_us = static_cast<double>(slots * st.num_q_heads * 1056) / 5e6;
     const double beside_us = kLaunchesUs + (stream.empty() || gemm.empty() ? 0 : kBothUs);
     if (beside_us + 1.12 * both + partials_us >= b.plain_us) return SharedFit::kPlain;
   }
-  schedule_gemm(gemm, group, heads, columns, length.tiles, slot, gemm_work);
+  st.draft.columns = columns;
+  st.draft.tiles = length.tiles;
   st.slices = shape.grid_y;
-  st.gemm_wgs = std::min(gemm_wgs, static_cast<int64_t>(gemm_work.size()) / kGemmInts);
-  st.gemm_items = static_cast<int64_t>(gemm_work.size()) / kGemmInts;
+  st.gemm_wgs = std::min(gemm_wgs, products.items);
+  st.gemm_items = products.items;
 
   // Layout; a graph plan's does not depend on what is shared.
-  const bool by_token = tokens == b.batch;
-  int64_t stream_cap = items, wg_cap = wgs, gemm_cap = st.gemm_items, slot_cap = slot;
+  st.by_token = tokens == b.batch;
+  int64_t stream_cap = items, wg_cap = wgs, gemm_cap = st.gemm_items, slot_cap = slots;
   if (graph_rows) {
     // A workgroup's share, and each request's and prefix's own items and cuts; a slot an item of a
     // request, and as many as a streamed prefix has tokens an item of one.
@@ -1219,12 +1236,12 @@ SharedFit SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t 
                (shape.wg_capacity + graph_rows / 2 * cuts) *
                    std::min<int64_t>(kStreamColumns / group, graph_rows);
   }
-  const int64_t o_info = kHeaderInts;
-  const int64_t o_row_of = o_info + kInfoInts * b.batch;
-  const int64_t o_stream = o_row_of + (by_token ? 0 : ceil_div(tokens, 4) * 4);
-  const int64_t o_gemm = o_stream + kStreamInts * stream_cap;
-  const int64_t o_wg = o_gemm + kGemmInts * gemm_cap;
-  const int64_t total = o_wg + wg_cap + 1;
+  st.o_info = kHeaderInts;
+  st.o_row_of = st.o_info + kInfoInts * b.batch;
+  st.o_stream = st.o_row_of + (st.by_token ? 0 : ceil_div(tokens, 4) * 4);
+  st.o_gemm = st.o_stream + kStreamInts * stream_cap;
+  st.o_wg = st.o_gemm + kGemmInts * gemm_cap;
+  const int64_t total = st.o_wg + wg_cap + 1;
   const size_t rows = static_cast<size_t>(slot_cap) * st.num_q_heads;
   if (!graph_rows && static_cast<int64_t>(rows * (kD + 1) * 4) > most_partials())
     return SharedFit::kPlain;
@@ -1246,63 +1263,66 @@ SharedFit SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t 
     hip_error(err, "shared prefix workspace");
     return SharedFit::kError;
   }
+  st.tokens = tokens;
+  if (graph_rows) st.sets = 2;
+  st.stream_grid = graph_rows ? wg_cap : wgs;
+  st.gemm_grid = graph_rows ? st.cus : st.gemm_wgs;
+  return SharedFit::kRuns;
+}
+
+bool SharedPlan::upload(const SharedBatch& b, hipStream_t s) {
+  State& st = *st_;
+  State::Draft& d = st.draft;
+  std::vector<int32_t> gemm_work;
+  schedule_gemm(d.gemm, st.group, st.num_kv_heads, d.columns, d.tiles, d.slot, gemm_work);
   int32_t* host = static_cast<int32_t*>(st.staging.ptr);
   host[kHeaderGemmItems] = static_cast<int32_t>(st.gemm_items);
-  host[kHeaderStreamWgs] = static_cast<int32_t>(wgs);
-  host[kHeaderOnce] = once;
+  host[kHeaderStreamWgs] = static_cast<int32_t>(d.wgs);
+  host[kHeaderOnce] = d.once;
   host[kHeaderGemmWgs] = static_cast<int32_t>(st.gemm_wgs);
   for (int64_t r = 0; r < b.batch; ++r) {
-    int32_t* info = host + o_info + kInfoInts * r;
-    for (const Of& of : {prefix_of[r], own_of[r]}) {
-      const Source* src = of.kind == 0 ? nullptr : of.kind == 1 ? &stream[of.index]
-                                                                : &gemm[of.index];
+    int32_t* info = host + st.o_info + kInfoInts * r;
+    for (const State::Of& of : {d.prefix_of[r], d.own_of[r]}) {
+      const Source* src = of.kind == 0 ? nullptr : of.kind == 1 ? &d.stream[of.index]
+                                                                : &d.gemm[of.index];
       info[0] = src ? src->slot : 0;
       info[1] = src ? src->splits : 0;
       info[2] = src ? src->tokens : 0;
       info[3] = src ? src->token0 : 0;
       info += 4;
     }
-    if (!by_token)
-      std::fill(host + o_row_of + b.q_start[r], host + o_row_of + b.q_start[r + 1],
+    if (!st.by_token)
+      std::fill(host + st.o_row_of + b.q_start[r], host + st.o_row_of + b.q_start[r + 1],
                 static_cast<int32_t>(r));
   }
   st.prefix_items = 0;
   for (size_t i = 0; i < gemm_work.size(); i += kGemmInts)
     st.prefix_items += gemm_work[i + 8] == kNoHorizon;
-  for (int64_t i = 0, part = 0; i < items; ++i) {
-    const int32_t of = work[4 * i];
-    part = i && work[4 * (i - 1)] == of ? part + 1 : 0;
-    const Source& src = stream[of];
-    const int32_t begin = src.begin + work[4 * i + 1], end = src.begin + work[4 * i + 2];
+  for (int64_t i = 0, part = 0; i < d.items; ++i) {
+    const int32_t of = d.work[4 * i];
+    part = i && d.work[4 * (i - 1)] == of ? part + 1 : 0;
+    const Source& src = d.stream[of];
+    const int32_t begin = src.begin + d.work[4 * i + 1], end = src.begin + d.work[4 * i + 2];
     const int32_t out[kStreamInts] = {
         src.token0, src.tokens,
         src.page_base + begin / static_cast<int32_t>(st.page_size), begin, end,
         src.splits ? src.slot + static_cast<int32_t>(part) * src.tokens : -1, src.pos0, 0};
-    std::memcpy(host + o_stream + kStreamInts * i, out, sizeof out);
+    std::memcpy(host + st.o_stream + kStreamInts * i, out, sizeof out);
     st.prefix_items += src.pos0 == kNoHorizon;
   }
-  std::copy(wg.begin(), wg.begin() + (stream.empty() ? 0 : wgs + 1), host + o_wg);
-  std::copy(gemm_work.begin(), gemm_work.end(), host + o_gemm);
+  std::copy(d.wg.begin(), d.wg.begin() + (d.stream.empty() ? 0 : d.wgs + 1), host + st.o_wg);
+  std::copy(gemm_work.begin(), gemm_work.end(), host + st.o_gemm);
   // wg comes last and only its used part is written: a graph plan's unused workgroups leave early.
-  err = hipMemcpyAsync(st.ints.ptr, host, (o_wg + wgs + 1) * 4, hipMemcpyHostToDevice, s);
+  hipError_t err =
+      hipMemcpyAsync(st.ints.ptr, host, (st.o_wg + d.wgs + 1) * 4, hipMemcpyHostToDevice, s);
   if (err == hipSuccess) err = hipEventRecord(st.upload_done, s);
   if (err != hipSuccess) {
     hip_error(err, "shared prefix upload");
-    return SharedFit::kError;
+    return false;
   }
   st.ready = true;
   st.batch = b.batch;
-  st.tokens = tokens;
-  st.by_token = by_token;
-  if (graph_rows) st.sets = 2;
-  st.stream_grid = graph_rows ? wg_cap : wgs;
-  st.gemm_grid = graph_rows ? st.cus : st.gemm_wgs;
-  st.o_info = o_info;
-  st.o_row_of = o_row_of;
-  st.o_stream = o_stream;
-  st.o_gemm = o_gemm;
-  st.o_wg = o_wg;
-  return SharedFit::kRuns;
+  return true;
 }
 
 void SharedPlan::info(int64_t* out4) const {
