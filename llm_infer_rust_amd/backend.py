@@ -85,7 +85,9 @@ class SharedPrefix:
     (``rows`` sums to the batch; 0 or a group of one: nothing shared). Attention over them is computed
     once for the group, read through the pages of its first row. Host values; the reference has no
     counterpart. A statement about the cache, not a request: results are those of a batch without it
-    up to rounding, and it is not used where that would cost more than it saves."""
+    up to rounding, and an eager plan uses it only where that is estimated to save time and its
+    workspace has room (``DecodePlan.shared_info`` says). A captured decode plan that was prepared with
+    groups always takes the form that can share."""
     rows: Sequence[int]
     lens: Sequence[int]
 

@@ -477,8 +477,8 @@ __device__ __forceinline__ void gemm_items(const SharedArgs& a, uint8_t* lds, in
         return make_uint4(l2.x, l2.y, h2.x, h2.y);
       };
       // Half of V's operands are loaded behind the scores' products, the others where they are used:
-      // all of them early do not fit the registers (256 rows over 8,192 tokens, four layers: none
-      // early 516 us, half 511, all, with spills, 551).
+      // all of them early do not fit the registers (us a layer, 256 rows sharing 8,192 tokens: none
+      // early 125.5, half 124.8, all, with spills, 135).
       constexpr int kEarly = NW == 8 ? 2 : 0;
       uint4 vf[2][4];
 #pragma unroll
@@ -1104,8 +1104,8 @@ SharedFit SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t 
     stream_us = 0;
   }
   // How the products and the copies share the chip. Whole CUs for either wherever there are both and
-  // eight kv heads (us a layer, in turn, in halves, on whole CUs: 256 rows sharing 8,192 tokens 141,
-  // 136, 117; 64 sharing 2,048 44, 38, 29; 75 rows of up to 16 new tokens in 8 groups 65, 63, 54);
+  // eight kv heads (us a layer, in turn, in halves, on whole CUs: 256 rows sharing 8,192 tokens 142,
+  // 137, 125; 64 sharing 2,048 43, 36, 30; 75 rows of up to 16 new tokens in 8 groups 65, 63, 54);
   // halves with four; in turn where the copies are next to nothing (48 rows of up to 40 new tokens
   // 103, 141, 110).
   int64_t cost4 = 0, cost8 = 0;  // tiles of 128 and of 256 columns
@@ -1158,7 +1158,7 @@ SharedFit SharedPlan::prepare(const SharedBatch& b, int64_t graph_rows, int64_t 
       }
     }
     // A share for every CU that streams: more of them end later where the last ones find no CU free
-    // (64 rows sharing 8,192 tokens, 192 such CUs: 192 shares 41.8 us, 256 49.7, 384 43, 512 49).
+    // (64 rows sharing 8,192 tokens, 154 such CUs: 154 shares 35 us, 192 46, 224 41, 256 39).
     shape = stream_shape(st.cus, heads, st.page_size, 8);
     shape.workgroups = std::max<int64_t>(1, (st.cus - gemm_wgs) / shape.grid_y);
     shape.wg_capacity = st.cus / shape.grid_y + st.cus / 3 + 2;
